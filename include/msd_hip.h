@@ -188,6 +188,55 @@ int msd_groupnorm_tokens_workspace(const void *x, void *y, const float *gamma, c
                                    size_t workspace_bytes, void *stream);
 
 /*
+ * GroupNorm over channels-last tensors: x and y are [batch, positions, channels], the order of a
+ * channels-last convolution and of tokens; y may alias x exactly.  Optionally, chunk
+ * [batch, channels] (or NULL) is added in front, rounded to the storage type as msd_chunkwise_add
+ * does, and SiLU follows.  Formula as msd_groupnorm.  No counterpart in the reference, whose
+ * tensors are NCHW; the three steps are those of M/nn/ResBlock.cpp:188-199,222-232.
+ *
+ * For msd_groupnorm_channels_last_backward the call can also keep, each NULL or:
+ *   stats        [batch, groups, 2] mean and 1 / sqrt(variance + eps), 8-byte aligned
+ *   codes,       [batch, positions, channels] int8 and [batch, positions, ceil(channels /
+ *   code_scales  MSD_CODE_BLOCK)] float: the normalised tensor (x, or x + chunk) in 8 bits.  The
+ *                channels of a position are cut into blocks of MSD_CODE_BLOCK; with a = the
+ *                largest finite |value| of a block, code = round(value * (127 / a)) (to even,
+ *                clamped to +-127) and scale = a / 127, in float32; a < 1e-30: all zero.
+ * workspace: 8-byte aligned device memory of at least the bytes that
+ * msd_groupnorm_channels_last_workspace reports (backward = 0), apart from all else; its contents need
+ * not be set, are left undefined, and belong to this call until it (or every replay of it) is
+ * done.  The call allocates nothing, shares nothing with other calls, and gives the same bits
+ * every time, inside a stream capture and outside.
+ */
+#define MSD_CODE_BLOCK 32
+int msd_groupnorm_channels_last(const void *x, const void *chunk, void *y, const float *gamma, const float *beta,
+                                size_t batch, size_t positions, size_t channels, size_t groups, float eps,
+                                int fuse_silu, int dtype, float *stats, int8_t *codes, float *code_scales,
+                                void *workspace, size_t workspace_bytes, void *stream);
+
+/* Bytes of workspace for a forward (backward = 0) or a backward call of that shape.  Host only. */
+int msd_groupnorm_channels_last_workspace(size_t batch, size_t positions, size_t channels, size_t groups,
+                                          int dtype, int backward, size_t *bytes);
+
+/*
+ * Gradient of msd_groupnorm_channels_last: from dy [batch, positions, channels], the stats that the
+ * forward call kept, and either x (and chunk, where the forward call had one) or codes and
+ * code_scales (then x = chunk = NULL; the values that the codes stand for take the place of the
+ * normalised tensor):
+ *   dx [batch, positions, channels], which may alias dy exactly; the gradient of x and, summed over
+ *   the positions, of chunk (dchunk [batch, channels] in the storage type, or NULL: not wanted);
+ *   dgamma, dbeta [channels] float32, both or both NULL.
+ * Sums are float32, added in a fixed order without atomics: the same bits every time.
+ * workspace as for the forward call (backward = 1).  No positions or no samples: dgamma, dbeta and
+ * dchunk are set to zero.  No counterpart in the reference, which has no gradients.
+ */
+int msd_groupnorm_channels_last_backward(const void *dy, const void *x, const void *chunk, const int8_t *codes,
+                                         const float *code_scales, const float *stats, const float *gamma,
+                                         const float *beta, void *dx, float *dgamma, float *dbeta, void *dchunk,
+                                         size_t batch, size_t positions, size_t channels, size_t groups,
+                                         int fuse_silu, int dtype, void *workspace, size_t workspace_bytes,
+                                         void *stream);
+
+/*
  * dst[i, k, j] = src[i, j, k]: the permute3D_0_2_1 kernel (K/util.cl:47-64) that
  * SpatialTransformer::forward enqueues between NCHW and token layout
  * (M/nn/SpatialTransformer.cpp:132-139,157-164).  dst must not overlap src.

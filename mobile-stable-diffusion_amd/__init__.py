@@ -7,7 +7,9 @@ current torch stream through the C ABI; torch is used for device memory and
 streams, nothing else.  There is no fallback: if the library was not built
 the loader raises.
 """
+import collections
 import ctypes
+import functools
 import importlib.util
 import os
 import sys
@@ -25,6 +27,7 @@ TUNE_GN_SPLIT, TUNE_GN_THREADS, TUNE_LN_CHUNK, TUNE_LN_THREADS, TUNE_GEGLU_VECTO
     TUNE_SOFTMAX_ROWS, TUNE_GN_SPIN_LIMIT, TUNE_GN_WRITERS, TUNE_DEVICE_CUS, TUNE_DEVICE_XCDS, \
     TUNE_GN_PLAN_RULE_ONLY = range(12)
 ERR_SCRATCH_LIMIT = -2
+CODE_BLOCK = 32  # channels that share a scale in an 8-bit checkpoint: MSD_CODE_BLOCK of include/msd_hip.h
 TOKENS_WORKSPACE_BYTES = 128  # per (sample, group): MSD_TOKENS_WORKSPACE_BYTES of include/msd_hip.h
 
 # every symbol include/msd_hip.h declares
@@ -34,6 +37,7 @@ C_ABI_SYMBOLS = (
     "msd_silu", "msd_gelu", "msd_quick_gelu", "msd_timestep_embedding", "msd_ddim_timesteps",
     "msd_elemwise_add", "msd_chunkwise_add", "msd_chunk_add_groupnorm", "msd_add_layernorm", "msd_copy",
     "msd_groupnorm_tokens", "msd_groupnorm_tokens_workspace", "msd_permute_0_2_1",
+    "msd_groupnorm_channels_last", "msd_groupnorm_channels_last_workspace", "msd_groupnorm_channels_last_backward",
     "msd_linear_rows", "msd_linear_rows_grouped", "msd_softmax", "msd_alphas_cumprod", "msd_ddim_schedule", "msd_ddim_update",
 )
 ACT_NONE, ACT_SILU = 0, 1
@@ -75,6 +79,9 @@ def load_library(path=None):
     lib.msd_permute_0_2_1.argtypes = [vp, vp, sz, sz, sz, it, vp]
     lib.msd_groupnorm_tokens.argtypes = [vp, vp, vp, vp, sz, sz, sz, sz, fl, it, vp]
     lib.msd_groupnorm_tokens_workspace.argtypes = [vp, vp, vp, vp, sz, sz, sz, sz, fl, it, vp, sz, vp]
+    lib.msd_groupnorm_channels_last.argtypes = [vp, vp, vp, vp, vp, sz, sz, sz, sz, fl, it, it, vp, vp, vp, vp, sz, vp]
+    lib.msd_groupnorm_channels_last_workspace.argtypes = [sz, sz, sz, sz, it, it, ctypes.POINTER(sz)]
+    lib.msd_groupnorm_channels_last_backward.argtypes = [vp] * 12 + [sz, sz, sz, sz, it, it, vp, sz, vp]
     lib.msd_elemwise_add.argtypes = [vp, vp, vp, sz, it, vp]
     lib.msd_chunkwise_add.argtypes = [vp, vp, vp, sz, sz, it, vp]
     lib.msd_chunk_add_groupnorm.argtypes = [vp, vp, vp, vp, vp, sz, sz, sz, sz, fl, it, it, vp]
@@ -311,6 +318,126 @@ def groupnorm_tokens(x, gamma, beta, groups, eps=1e-6):
     check(lib.msd_groupnorm_tokens_workspace(xp, out.data_ptr(), gp, bp, batch, channels, hw, groups, eps, _dtype_code(x),
                                              workspace.data_ptr(), size, _stream()))
     return out
+
+
+def _channels_last(x, what="x"):
+    """(batch, positions, channels) of a [batch, C, H, W] tensor in torch.channels_last order or a contiguous
+    [batch, positions, C] one, on the current device."""
+    torch = _torch or _bind_torch()
+    if not x.is_cuda or x.get_device() != torch.cuda.current_device():
+        raise MsdError("%s must be on the current device (got %s)" % (what, x.device))
+    if x.dim() == 4 and x.is_contiguous(memory_format=torch.channels_last):
+        batch, channels, h, w = x.shape
+        return batch, h * w, channels
+    if x.dim() == 3 and x.is_contiguous():
+        return tuple(x.shape)
+    raise MsdError("%s must be [batch, C, H, W] in torch.channels_last order or a contiguous [batch, positions, C]" % what)
+
+
+def _same_layout(t, like, what):
+    """An operand laid out as `like`, which _channels_last has checked."""
+    if t.shape != like.shape or t.dtype != like.dtype:
+        raise MsdError("%s must be %s of shape %s (got %s, %s)" % (what, like.dtype, tuple(like.shape), t.dtype, tuple(t.shape)))
+    _channels_last(t, what)
+    return t.data_ptr()
+
+
+@functools.lru_cache(maxsize=1024)
+def _channels_last_workspace(batch, positions, channels, groups, dtype_code, backward):
+    size = ctypes.c_size_t(0)
+    check(load_library().msd_groupnorm_channels_last_workspace(batch, positions, channels, groups, dtype_code, backward,
+                                                               ctypes.byref(size)))
+    return size.value
+
+
+KeptNorm = collections.namedtuple("KeptNorm", "x chunk codes scales stats gamma beta groups fuse_silu with_chunk")
+KeptNorm.__doc__ = """What groupnorm_channels_last_kept keeps for the gradient: the mean and 1 / sqrt(variance + eps) of every group
+(stats, float32 [batch, groups, 2]) and either x and chunk themselves or, in 8 bits, codes (int8, in the order of x) and scales
+(float32 [batch, positions, ceil(C / 32)]; a code times its block's scale is the value it stands for)."""
+
+
+def _pointer(t):
+    return None if t is None else t.data_ptr()
+
+
+def _channels_last_forward(x, gamma, beta, groups, eps, fuse_silu, chunk, out, stats, codes, scales):
+    lib = _lib or load_library()
+    batch, positions, channels = _channels_last(x)
+    code = _dtype_code(x)
+    if out is None:
+        out = _torch.empty_like(x)
+    yp = _same_layout(out, x, "out")
+    cp = _same(chunk, x, batch * channels, "chunk") if chunk is not None else None
+    gp, bp = _affine(gamma, channels, x, "gamma"), _affine(beta, channels, x, "beta")
+    if groups <= 0 or channels % groups:
+        raise MsdError("groups must divide the channels (got %d, %d)" % (groups, channels))
+    size = _channels_last_workspace(batch, positions, channels, groups, code, 0)
+    workspace = x.new_empty(size, dtype=_torch.uint8)
+    check(lib.msd_groupnorm_channels_last(x.data_ptr(), cp, yp, gp, bp, batch, positions, channels, groups, eps, int(fuse_silu), code,
+                                          _pointer(stats), _pointer(codes), _pointer(scales),
+                                          workspace.data_ptr(), size, _stream()))
+    return out
+
+
+def groupnorm_channels_last(x, gamma, beta, groups, eps=1e-5, fuse_silu=False, chunk=None, out=None):
+    """GroupNorm(x + chunk[:, :, None]) (+ SiLU) over channels-last tensors: x is [batch, C, H, W] in torch.channels_last order or a
+    contiguous [batch, positions, C]; gamma / beta float32 [C]; chunk [batch, C] in x's dtype or None.  out may be x (in place)."""
+    return _channels_last_forward(x, gamma, beta, groups, eps, fuse_silu, chunk, out, None, None, None)
+
+
+def groupnorm_channels_last_kept(x, gamma, beta, groups, eps=1e-5, fuse_silu=False, chunk=None, keep8=False, out=None):
+    """groupnorm_channels_last, and a KeptNorm for groupnorm_channels_last_backward.  It holds x and chunk, which must not
+    change until then (out must not be x), or with keep8 their sum in 8 bits, a quarter of float32 and a half of float16
+    (out may be x)."""
+    batch, positions, channels = _channels_last(x)
+    if out is not None and not keep8 and out.data_ptr() == x.data_ptr() and x.numel():
+        raise MsdError("out must not be x unless keep8: the gradient needs x")
+    torch = _torch
+    if groups <= 0:
+        raise MsdError("groups must be positive")
+    stats = x.new_empty((batch, groups, 2), dtype=torch.float32)
+    codes = scales = None
+    if keep8:
+        codes = torch.empty_like(x, dtype=torch.int8)
+        scales = x.new_empty((batch, positions, -(-channels // CODE_BLOCK)), dtype=torch.float32)
+    y = _channels_last_forward(x, gamma, beta, groups, eps, fuse_silu, chunk, out, stats, codes, scales)
+    return y, KeptNorm(None if keep8 else x, None if keep8 else chunk, codes, scales, stats, gamma, beta, groups, bool(fuse_silu),
+                       chunk is not None)
+
+
+def groupnorm_channels_last_backward(dy, kept, affine=True, out=None):
+    """-> (dx, dgamma, dbeta, dchunk) from dy, laid out as the forward call's x, and what that call kept.  dgamma and dbeta are
+    float32 [C] (None unless affine); dchunk is [batch, C] in dy's dtype (None where the forward call had no chunk).
+    out: receives dx; may be dy."""
+    lib = _lib or load_library()
+    batch, positions, channels = _channels_last(dy, "dy")
+    code = _dtype_code(dy)
+    if kept.codes is not None:
+        if kept.codes.shape != dy.shape:
+            raise MsdError("dy must have the shape of the forward call's x")
+        _channels_last(kept.codes, "codes")
+        xp = cp = None
+        qp, sp = kept.codes.data_ptr(), _dev(kept.scales)
+    else:
+        xp = _same_layout(kept.x, dy, "the forward call's x")
+        cp = _same(kept.chunk, dy, batch * channels, "chunk") if kept.chunk is not None else None
+        qp = sp = None
+    if out is None:
+        out = _torch.empty_like(dy)
+    dxp = _same_layout(out, dy, "out")
+    gp, bp = _affine(kept.gamma, channels, dy, "gamma"), _affine(kept.beta, channels, dy, "beta")
+    tp = _affine(kept.stats, 2 * batch * kept.groups, dy, "stats")
+    dgamma = dbeta = dchunk = None
+    if affine:
+        dgamma, dbeta = _torch.empty_like(kept.gamma), _torch.empty_like(kept.beta)
+    if kept.with_chunk:
+        dchunk = dy.new_empty((batch, channels))
+    size = _channels_last_workspace(batch, positions, channels, kept.groups, code, 1)
+    workspace = dy.new_empty(size, dtype=_torch.uint8)
+    check(lib.msd_groupnorm_channels_last_backward(
+        dy.data_ptr(), xp, cp, qp, sp, tp, gp, bp, dxp, _pointer(dgamma), _pointer(dbeta), _pointer(dchunk), batch, positions, channels, kept.groups, int(kept.fuse_silu), code,
+        workspace.data_ptr(), size, _stream()))
+    return out, dgamma, dbeta, dchunk
 
 
 def permute_0_2_1(x):

@@ -1,6 +1,7 @@
 // C ABI of libmsd_hip.so (declared in include/msd_hip.h): argument checks, dtype
 // dispatch and the per-(device, stream) GroupNorm scratch.
 #include <cmath>
+#include <initializer_list>
 #include <unordered_map>
 
 #include <hip/hip_fp16.h>
@@ -398,6 +399,97 @@ int msd_groupnorm_tokens_workspace(const void *x, void *y, const float *gamma, c
         return MSD_ERR_INVALID_VALUE;
     return groupnorm_tokens_entry(x, y, gamma, beta, batch, channels, hw, groups, eps, dtype,
                                   static_cast<float2 *>(workspace), stream);
+}
+
+// Checks of a channels-last call; *count: elements of the tensor, *need: bytes of workspace.
+static int channels_last_checks(size_t batch, size_t positions, size_t channels, size_t groups, int dtype, bool backward,
+                                size_t *count, size_t *need) {
+    if (groups == 0 || channels == 0 || channels % groups != 0) return MSD_ERR_INVALID_VALUE;
+    if (dtype != MSD_DTYPE_F32 && dtype != MSD_DTYPE_F16) return MSD_ERR_INVALID_VALUE;
+    if (__builtin_mul_overflow(batch, channels, count) || *count > (SIZE_MAX >> 3) ||
+        __builtin_mul_overflow(*count, positions, count) || *count > (SIZE_MAX >> 3))
+        return MSD_ERR_INVALID_VALUE;
+    *need = batch * positions != 0 ? cl_workspace_bytes(elt_bytes(dtype), batch, positions, channels, groups, backward) : 0;
+    return *need == SIZE_MAX ? MSD_ERR_INVALID_VALUE : MSD_OK;
+}
+static size_t code_scale_bytes(size_t batch, size_t positions, size_t channels) {
+    return batch * positions * ((channels + MSD_CODE_BLOCK - 1) / MSD_CODE_BLOCK) * sizeof(float);
+}
+// Whether [p, p + bytes) shares a byte with any of the other ranges (null ones have none).
+struct Range {
+    const void *at;
+    size_t bytes;
+};
+static bool overlaps_any(const void *p, size_t bytes, std::initializer_list<Range> others) {
+    for (const Range &r : others)
+        if (p != nullptr && r.at != nullptr && ranges_overlap(p, bytes, r.at, r.bytes)) return true;
+    return false;
+}
+
+int msd_groupnorm_channels_last_workspace(size_t batch, size_t positions, size_t channels, size_t groups, int dtype,
+                                          int backward, size_t *bytes) {
+    size_t count;
+    if (!bytes) return MSD_ERR_INVALID_VALUE;
+    return channels_last_checks(batch, positions, channels, groups, dtype, backward != 0, &count, bytes);
+}
+
+int msd_groupnorm_channels_last(const void *x, const void *chunk, void *y, const float *gamma, const float *beta, size_t batch,
+                                size_t positions, size_t channels, size_t groups, float eps, int fuse_silu, int dtype,
+                                float *stats, int8_t *codes, float *code_scales, void *workspace, size_t workspace_bytes,
+                                void *stream) {
+    size_t count, need;
+    const int rc = channels_last_checks(batch, positions, channels, groups, dtype, false, &count, &need);
+    if (rc != MSD_OK) return rc;
+    if (count == 0) return MSD_OK;
+    if (!x || !y || !gamma || !beta || (codes == nullptr) != (code_scales == nullptr)) return MSD_ERR_INVALID_VALUE;
+    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 7u) != 0 || workspace_bytes < need ||
+        (reinterpret_cast<uintptr_t>(stats) & 7u) != 0)
+        return MSD_ERR_INVALID_VALUE;
+    const size_t bytes = count * elt_bytes(dtype), added = batch * channels * elt_bytes(dtype), affine = channels * sizeof(float);
+    const size_t stat_bytes = 2 * batch * groups * sizeof(float), scale_bytes = code_scale_bytes(batch, positions, channels);
+    const Range in = {x, bytes}, add = {chunk, added}, g = {gamma, affine}, b = {beta, affine}, st = {stats, stat_bytes};
+    const Range c = {codes, count}, cs = {code_scales, scale_bytes}, w = {workspace, need};
+    if (shifted_overlap(x, y, bytes) || overlaps_any(y, bytes, {add, g, b, st, c, cs, w}) ||
+        overlaps_any(stats, stat_bytes, {in, add, g, b, c, cs, w}) || overlaps_any(codes, count, {in, add, g, b, cs, w}) ||
+        overlaps_any(code_scales, scale_bytes, {in, add, g, b, w}) || overlaps_any(workspace, need, {in, add, g, b}))
+        return MSD_ERR_INVALID_VALUE;
+    const ClForward a = {x, chunk, y, gamma, beta, stats, codes, code_scales, workspace};
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (dtype == MSD_DTYPE_F32) return cl_forward_dispatch<float>(a, batch, positions, channels, groups, eps, fuse_silu != 0, s);
+    return cl_forward_dispatch<__half>(a, batch, positions, channels, groups, eps, fuse_silu != 0, s);
+}
+
+int msd_groupnorm_channels_last_backward(const void *dy, const void *x, const void *chunk, const int8_t *codes,
+                                         const float *code_scales, const float *stats, const float *gamma, const float *beta,
+                                         void *dx, float *dgamma, float *dbeta, void *dchunk, size_t batch, size_t positions,
+                                         size_t channels, size_t groups, int fuse_silu, int dtype, void *workspace,
+                                         size_t workspace_bytes, void *stream) {
+    size_t count, need;
+    const int rc = channels_last_checks(batch, positions, channels, groups, dtype, true, &count, &need);
+    if (rc != MSD_OK) return rc;
+    if ((dgamma == nullptr) != (dbeta == nullptr)) return MSD_ERR_INVALID_VALUE;
+    if (count != 0) {
+        if (!dy || !stats || !gamma || !beta || !dx || (codes == nullptr) != (code_scales == nullptr)) return MSD_ERR_INVALID_VALUE;
+        if ((x == nullptr) == (codes == nullptr) || (codes != nullptr && chunk != nullptr)) return MSD_ERR_INVALID_VALUE;
+        if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 7u) != 0 || workspace_bytes < need ||
+            (reinterpret_cast<uintptr_t>(stats) & 7u) != 0)
+            return MSD_ERR_INVALID_VALUE;
+    }
+    const size_t bytes = count * elt_bytes(dtype), added = batch * channels * elt_bytes(dtype), affine = channels * sizeof(float);
+    const size_t stat_bytes = 2 * batch * groups * sizeof(float), scale_bytes = code_scale_bytes(batch, positions, channels);
+    const Range d = {dy, bytes}, in = {x, bytes}, add = {chunk, added}, c = {codes, count}, cs = {code_scales, scale_bytes};
+    const Range st = {stats, stat_bytes}, g = {gamma, affine}, b = {beta, affine}, w = {workspace, need};
+    const Range to = {dx, bytes}, dg = {dgamma, affine}, db = {dbeta, affine};
+    if ((dx != dy && overlaps_any(dx, bytes, {d})) || overlaps_any(dx, bytes, {in, add, c, cs, st, g, b, w, dg, db}) ||
+        overlaps_any(dgamma, affine, {d, in, add, c, cs, st, g, b, w, db}) ||
+        overlaps_any(dbeta, affine, {d, in, add, c, cs, st, g, b, w}) ||
+        overlaps_any(dchunk, added, {d, in, add, c, cs, st, g, b, w, to, dg, db}) ||
+        overlaps_any(workspace, need, {d, in, add, c, cs, st, g, b}))
+        return MSD_ERR_INVALID_VALUE;
+    const ClBackward a = {dy, x, chunk, codes, code_scales, stats, gamma, beta, dx, dgamma, dbeta, dchunk, workspace};
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (dtype == MSD_DTYPE_F32) return cl_backward_dispatch<float>(a, batch, positions, channels, groups, fuse_silu != 0, s);
+    return cl_backward_dispatch<__half>(a, batch, positions, channels, groups, fuse_silu != 0, s);
 }
 
 static int layernorm_entry(const void *x, const void *res, void *sum, void *y, const float *gamma,

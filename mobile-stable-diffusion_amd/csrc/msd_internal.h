@@ -139,6 +139,34 @@ int gn_dispatch(const void *x, const void *chunk, void *y, const float *gamma, c
 template <typename T>
 int gn_tokens_dispatch(const void *x, void *y, const float *gamma, const float *beta, size_t batch,
                        size_t channels, size_t hw, size_t groups, float eps, float2 *partials, hipStream_t stream);
+// Channels last (gn_channels_last.hip): x, y, dy, dx are [batch, positions, channels]; chunk [batch, channels] or null;
+// stats [batch, groups][2], mean and 1 / sqrt(variance + eps); codes and scales: the input in 8 bits, or null
+struct ClForward {
+    const void *x, *chunk;
+    void *y;
+    const float *gamma, *beta;
+    float *stats;  // or null
+    int8_t *codes;
+    float *scales;
+    void *workspace;
+};
+struct ClBackward {
+    const void *dy, *x, *chunk;
+    const int8_t *codes;  // in place of x and chunk
+    const float *scales, *stats, *gamma, *beta;
+    void *dx;
+    float *dgamma, *dbeta;  // both or neither
+    void *dchunk;           // or null
+    void *workspace;
+};
+// SIZE_MAX for a shape beyond what the kernels count in 32 bits
+size_t cl_workspace_bytes(size_t elt, size_t batch, size_t positions, size_t channels, size_t groups, bool backward);
+template <typename T>
+int cl_forward_dispatch(const ClForward &a, size_t batch, size_t positions, size_t channels, size_t groups, float eps, bool silu,
+                        hipStream_t stream);
+template <typename T>
+int cl_backward_dispatch(const ClBackward &a, size_t batch, size_t positions, size_t channels, size_t groups, bool silu,
+                         hipStream_t stream);
 // res / sum may be null (plain LayerNorm); otherwise sum = x + res is written and normalised
 template <typename T>
 int ln_dispatch(const void *x, const void *res, void *sum, void *y, const float *gamma,
