@@ -365,6 +365,30 @@ int msd_linear_rows_grouped(const void *x, const void *const *weights, const flo
                             int act_in, int act_out, int dtype, void *stream);
 
 /*
+ * The same layers with the weight in 4 bits: w[n, k] = (code[n, k] - 8) * scale[n, k / group].
+ *   packed  [n, k / 2] bytes, the code (0 ... 15) of an even k in the low half of its byte and that
+ *           of the next k in the high half
+ *   scales  [n, k / group] in the storage type `dtype`; group is 32, 64 or 128 and divides k
+ * Everything else as for msd_linear_rows and msd_linear_rows_grouped, m <= 8 included; products and
+ * sums are float32, and a row has the same bits whatever rows and whatever layers come with it, as
+ * long as the operands' alignment is the same (16 bytes for x and packed is the fast one).
+ *   msd_q4_pack  makes codes and scales of a weight w [n, k] in the storage type: with a = the
+ *           largest finite |w| of a group, scale = a / 7 rounded to the storage type and code =
+ *           round(w * (1 / scale)) (to even, clamped to +-7) + 8; a < 1e-30 or a scale of 0: the
+ *           scale is 0 and the codes are 8.  packed and scales lie apart from w and each other.
+ * n and k are at most 2^28.  No counterpart in the reference, whose weights are float32.
+ */
+int msd_q4_pack(const void *w, uint8_t *packed, void *scales, size_t n, size_t k, size_t group, int dtype,
+                void *stream);
+int msd_linear_rows_q4(const void *x, const uint8_t *packed, const void *scales, const float *bias, void *y,
+                       size_t m, size_t n, size_t k, size_t group, int act_in, int act_out, int dtype,
+                       void *stream);
+int msd_linear_rows_q4_grouped(const void *x, const uint8_t *const *packed, const void *const *scales,
+                               const float *const *biases, void *const *ys, const size_t *ns, size_t count,
+                               size_t m, size_t k, size_t group, int act_in, int act_out, int dtype,
+                               void *stream);
+
+/*
  * Row softmax over the last dimension of [rows, cols]; y may alias x (every reference
  * call site is in place).  Replaces the softmax kernel K/util.cl:150-187 enqueued by
  * CrossAttention::forward (M/nn/CrossAttention.cpp:362-377) and AttnBlock::forward

@@ -38,7 +38,7 @@ C_ABI_SYMBOLS = (
     "msd_elemwise_add", "msd_chunkwise_add", "msd_chunk_add_groupnorm", "msd_add_layernorm", "msd_copy",
     "msd_groupnorm_tokens", "msd_groupnorm_tokens_workspace", "msd_permute_0_2_1",
     "msd_groupnorm_channels_last", "msd_groupnorm_channels_last_workspace", "msd_groupnorm_channels_last_backward",
-    "msd_linear_rows", "msd_linear_rows_grouped", "msd_softmax", "msd_alphas_cumprod", "msd_ddim_schedule", "msd_ddim_update",
+    "msd_linear_rows", "msd_linear_rows_grouped", "msd_q4_pack", "msd_linear_rows_q4", "msd_linear_rows_q4_grouped", "msd_softmax", "msd_alphas_cumprod", "msd_ddim_schedule", "msd_ddim_update",
 )
 ACT_NONE, ACT_SILU = 0, 1
 
@@ -94,6 +94,9 @@ def load_library(path=None):
     lib.msd_softmax.argtypes = [vp, vp, sz, sz, it, it, vp]
     lib.msd_linear_rows_grouped.argtypes = [vp, ctypes.POINTER(vp), ctypes.POINTER(vp), ctypes.POINTER(vp),
                                             ctypes.POINTER(sz), sz, sz, sz, it, it, it, vp]
+    lib.msd_q4_pack.argtypes = [vp, vp, vp, sz, sz, sz, it, vp]
+    lib.msd_linear_rows_q4.argtypes = [vp, vp, vp, vp, vp, sz, sz, sz, sz, it, it, it, vp]
+    lib.msd_linear_rows_q4_grouped.argtypes = [vp] + [ctypes.POINTER(vp)] * 4 + [ctypes.POINTER(sz), sz, sz, sz, sz, it, it, it, vp]
     flp, inp = ctypes.POINTER(ctypes.c_float), ctypes.POINTER(ctypes.c_int)
     lib.msd_alphas_cumprod.argtypes = [flp]
     lib.msd_ddim_schedule.argtypes = [it, inp, flp, flp, flp, it]
@@ -635,6 +638,86 @@ def linear_rows_grouped(x, weights, biases=None, act_in=ACT_NONE, act_out=ACT_NO
     pointers = ctypes.c_void_p * count
     check(lib.msd_linear_rows_grouped(xp, pointers(*wp), pointers(*bp), pointers(*yp), (ctypes.c_size_t * count)(*ns), count,
                                       m, k, act_in, act_out, _dtype_code(x), _stream()))
+    return outs
+
+
+def q4_pack(weight, group=64):
+    """(packed, scales) of a weight [n, k] for linear_rows_q4: uint8 [n, k / 2], two 4-bit codes to a byte, and [n, k / group] in
+    the weight's dtype; group is 32, 64 or 128 and divides k."""
+    lib = _lib or load_library()
+    wp = _on_current_device(weight, "weight")
+    if weight.dim() != 2 or group not in (32, 64, 128) or weight.shape[1] % group:
+        raise MsdError("weight must be [n, k] with k a multiple of group, which is 32, 64 or 128")
+    n, k = weight.shape
+    packed, scales = weight.new_empty((n, k // 2), dtype=_torch.uint8), weight.new_empty((n, k // group))
+    check(lib.msd_q4_pack(wp, packed.data_ptr(), scales.data_ptr(), n, k, group, _dtype_code(weight), _stream()))
+    return packed, scales
+
+
+def _on_current_device(t, what):
+    """A contiguous tensor on the device whose stream the call goes to."""
+    torch = _torch or _bind_torch()
+    if not t.is_cuda or t.get_device() != torch.cuda.current_device() or not t.is_contiguous():
+        raise MsdError("%s must be a contiguous tensor on the current device (got %s)" % (what, t.device))
+    return t.data_ptr()
+
+
+def _q4_weight(packed, scales, x, k, group, what):
+    """Columns of a packed weight that fits x [m, k] and the group."""
+    if packed.dim() != 2 or packed.dtype != _torch.uint8 or 2 * packed.shape[1] != k or packed.get_device() != x.get_device() \
+            or not packed.is_contiguous():
+        raise MsdError("%spacked must be contiguous uint8 [n, %d] on %s" % (what, k // 2, x.device))
+    if scales.shape != (packed.shape[0], k // group) or scales.dtype != x.dtype or scales.get_device() != x.get_device() \
+            or not scales.is_contiguous():
+        raise MsdError("%sscales must be contiguous %s [%d, %d] on %s" % (what, x.dtype, packed.shape[0], k // group, x.device))
+    return packed.shape[0]
+
+
+def _q4_group(x, scales):
+    """Weights per scale, from x [m, k] and scales [n, k / group]."""
+    if x.dim() != 2 or scales.dim() != 2:
+        raise MsdError("x must be [m, k] and scales [n, k / group]")
+    k, count = x.shape[1], scales.shape[1]
+    group = k // count if count else 0
+    if group not in (32, 64, 128) or group * count != k:
+        raise MsdError("scales must hold one value per 32, 64 or 128 of k = %d (got %d)" % (k, count))
+    return group
+
+
+def linear_rows_q4(x, packed, scales, bias=None, act_in=ACT_NONE, act_out=ACT_NONE, out=None):
+    """linear_rows with the weight in 4 bits: x [m <= 8, k], packed uint8 [n, k / 2] and scales [n, k / group] (x's dtype) as
+    q4_pack makes them, bias float32 [n] or None -> [m, n]."""
+    lib = _lib or load_library()
+    xp = _on_current_device(x, "x")
+    group = _q4_group(x, scales)
+    m, k = x.shape
+    n = _q4_weight(packed, scales, x, k, group, "")
+    bp = _affine(bias, n, x, "bias") if bias is not None else None
+    out = x.new_empty((m, n)) if out is None else out
+    check(lib.msd_linear_rows_q4(xp, packed.data_ptr(), scales.data_ptr(), bp, _same(out, x, m * n, "out"), m, n, k, group, act_in,
+                                 act_out, _dtype_code(x), _stream()))
+    return out
+
+
+def linear_rows_q4_grouped(x, packed, scales, biases=None, act_in=ACT_NONE, act_out=ACT_NONE):
+    """One launch for several such layers on the same x [m <= 8, k], all with the same group: lists of packed weights, scales and
+    biases (or None) -> list of [m, n_i] tensors."""
+    lib = _lib or load_library()
+    xp = _on_current_device(x, "x")
+    if len(packed) != len(scales) or (biases is not None and len(biases) != len(packed)):
+        raise MsdError("packed, scales and biases must be lists of one length")
+    if not packed:
+        return []
+    group = _q4_group(x, scales[0])
+    m, k = x.shape
+    ns = [_q4_weight(p, s, x, k, group, "layer %d: " % i) for i, (p, s) in enumerate(zip(packed, scales))]
+    bp = [_affine(b, n, x, "biases[%d]" % i) if b is not None else None for i, (b, n) in enumerate(zip(biases or [None] * len(ns), ns))]
+    outs = [x.new_empty((m, n)) for n in ns]
+    count = len(ns)
+    pointers = ctypes.c_void_p * count
+    check(lib.msd_linear_rows_q4_grouped(xp, pointers(*[p.data_ptr() for p in packed]), pointers(*[s.data_ptr() for s in scales]),
+                                         pointers(*bp), pointers(*[o.data_ptr() for o in outs]), (ctypes.c_size_t * count)(*ns), count,
+                                         m, k, group, act_in, act_out, _dtype_code(x), _stream()))
     return outs
 
 

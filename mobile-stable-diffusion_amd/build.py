@@ -52,7 +52,8 @@ def _run(cmd):
     return out
 
 
-HIP_SOURCES = ["api.hip", "gn_plan.hip", "groupnorm.hip", "gn_channels_last.hip", "layernorm.hip", "stream_ops.hip", "embed_ops.hip"]
+HIP_SOURCES = ["api.hip", "gn_plan.hip", "groupnorm.hip", "gn_channels_last.hip", "layernorm.hip", "stream_ops.hip", "embed_ops.hip",
+               "linear_q4.hip"]
 
 
 def build_hip():

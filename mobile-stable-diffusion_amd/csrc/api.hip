@@ -673,6 +673,57 @@ int msd_linear_rows_grouped(const void *x, const void *const *weights, const flo
     return linear_rows_grouped_dispatch<__half>(x, weights, biases, ys, ns, count, m, k, act_in, act_out, s);
 }
 
+static bool q4_group(size_t k, size_t group) { return (group == 32 || group == 64 || group == 128) && k % group == 0; }
+constexpr size_t kQ4MaxExtent = (size_t)1 << 28;  // as for msd_linear_rows_grouped
+
+int msd_q4_pack(const void *w, uint8_t *packed, void *scales, size_t n, size_t k, size_t group, int dtype, void *stream) {
+    if (dtype != MSD_DTYPE_F32 && dtype != MSD_DTYPE_F16) return MSD_ERR_INVALID_VALUE;
+    if (!q4_group(k, group) || n > kQ4MaxExtent || k > kQ4MaxExtent) return MSD_ERR_INVALID_VALUE;
+    if (n * k == 0) return MSD_OK;
+    if (!w || !packed || !scales) return MSD_ERR_INVALID_VALUE;
+    const size_t elt = elt_bytes(dtype), in = n * k * elt, codes = n * (k / 2), s = n * (k / group) * elt;
+    if (overlaps_any(packed, codes, {{w, in}, {scales, s}}) || overlaps_any(scales, s, {{w, in}})) return MSD_ERR_INVALID_VALUE;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    if (dtype == MSD_DTYPE_F32) return q4_pack_dispatch<float>(w, packed, scales, n, k, group, st);
+    return q4_pack_dispatch<__half>(w, packed, scales, n, k, group, st);
+}
+
+int msd_linear_rows_q4_grouped(const void *x, const uint8_t *const *packed, const void *const *scales, const float *const *biases,
+                               void *const *ys, const size_t *ns, size_t count, size_t m, size_t k, size_t group, int act_in,
+                               int act_out, int dtype, void *stream) {
+    if (dtype != MSD_DTYPE_F32 && dtype != MSD_DTYPE_F16) return MSD_ERR_INVALID_VALUE;
+    if ((act_in != MSD_ACT_NONE && act_in != MSD_ACT_SILU) || (act_out != MSD_ACT_NONE && act_out != MSD_ACT_SILU))
+        return MSD_ERR_INVALID_VALUE;
+    if (m > 8 || !q4_group(k, group) || k > kQ4MaxExtent) return MSD_ERR_INVALID_VALUE;
+    if (count != 0 && (!packed || !scales || !ys || !ns)) return MSD_ERR_INVALID_VALUE;
+    const size_t elt = elt_bytes(dtype);
+    for (size_t i = 0; i < count && m != 0; i++) {
+        if (ns[i] == 0) continue;
+        if (!ys[i] || (k != 0 && (!x || !packed[i] || !scales[i])) || ns[i] > kQ4MaxExtent) return MSD_ERR_INVALID_VALUE;
+    }
+    for (size_t i = 0; i < count && m != 0; i++) {  // as for msd_linear_rows_grouped
+        if (ns[i] == 0) continue;
+        const size_t bytes = m * ns[i] * elt;
+        if (overlaps_any(ys[i], bytes, {{x, m * k * elt}})) return MSD_ERR_INVALID_VALUE;
+        for (size_t j = 0; j < count; j++) {
+            if (ns[j] == 0) continue;
+            if (overlaps_any(ys[i], bytes, {{packed[j], ns[j] * (k / 2)}, {scales[j], ns[j] * (k / group) * elt},
+                                            {biases ? biases[j] : nullptr, ns[j] * sizeof(float)},
+                                            {j != i ? ys[j] : nullptr, m * ns[j] * elt}}))
+                return MSD_ERR_INVALID_VALUE;
+        }
+    }
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (dtype == MSD_DTYPE_F32)
+        return linear_q4_dispatch<float>(x, packed, scales, biases, ys, ns, count, m, k, group, act_in, act_out, s);
+    return linear_q4_dispatch<__half>(x, packed, scales, biases, ys, ns, count, m, k, group, act_in, act_out, s);
+}
+
+int msd_linear_rows_q4(const void *x, const uint8_t *packed, const void *scales, const float *bias, void *y, size_t m, size_t n,
+                       size_t k, size_t group, int act_in, int act_out, int dtype, void *stream) {
+    return msd_linear_rows_q4_grouped(x, &packed, &scales, &bias, &y, &n, 1, m, k, group, act_in, act_out, dtype, stream);
+}
+
 int msd_softmax(const void *x, void *y, size_t rows, size_t cols, int stable, int dtype,
                 void *stream) {
     if (dtype != MSD_DTYPE_F32 && dtype != MSD_DTYPE_F16) return MSD_ERR_INVALID_VALUE;

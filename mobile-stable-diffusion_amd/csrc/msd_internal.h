@@ -197,6 +197,14 @@ template <typename T>
 int linear_rows_grouped_dispatch(const void *x, const void *const *ws, const float *const *biases,
                                  void *const *ys, const size_t *ns, size_t count, size_t m, size_t k,
                                  int act_in, int act_out, hipStream_t stream);
+// A weight [n, k] in 4 bits: codes, two to a byte, and one scale per `group` (32, 64 or 128, a divisor of k) of them
+template <typename T>
+int q4_pack_dispatch(const void *w, uint8_t *packed, void *scales, size_t n, size_t k, size_t group, hipStream_t stream);
+// linear_rows_grouped_dispatch with such weights
+template <typename T>
+int linear_q4_dispatch(const void *x, const uint8_t *const *packed, const void *const *scales, const float *const *biases,
+                       void *const *ys, const size_t *ns, size_t count, size_t m, size_t k, size_t group, int act_in, int act_out,
+                       hipStream_t stream);
 template <typename T>
 int softmax_dispatch(const void *x, void *y, size_t rows, size_t cols, int stable, hipStream_t stream);
 template <typename T>
