@@ -199,8 +199,9 @@ int msd_groupnorm_tokens_workspace(const void *x, void *y, const float *gamma, c
  *   codes,       [batch, positions, channels] int8 and [batch, positions, ceil(channels /
  *   code_scales  MSD_CODE_BLOCK)] float: the normalised tensor (x, or x + chunk) in 8 bits.  The
  *                channels of a position are cut into blocks of MSD_CODE_BLOCK; with a = the
- *                largest finite |value| of a block, code = round(value * (127 / a)) (to even,
- *                clamped to +-127) and scale = a / 127, in float32; a < 1e-30: all zero.
+ *                largest finite |value| of a block, code = round(value * (127 * (1 / a))) (to
+ *                even, clamped to +-127) and scale = a * (1 / 127), every step rounded to
+ *                float32; a < 1e-30: all zero.
  * workspace: 8-byte aligned device memory of at least the bytes that
  * msd_groupnorm_channels_last_workspace reports (backward = 0), apart from all else; its contents need
  * not be set, are left undefined, and belong to this call until it (or every replay of it) is

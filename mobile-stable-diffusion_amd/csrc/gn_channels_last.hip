@@ -31,7 +31,7 @@ constexpr uint32_t kClRows = 4;         // rows a lane requests before it uses t
 constexpr uint32_t kClMaxParts = 128;   // partial sums per group up to which every workgroup adds them up itself
 constexpr uint32_t kClTeam = 16;        // lanes that add up a group
 constexpr uint32_t kCodeBlock = 32;     // channels of one position that share a scale
-constexpr float kCodeTiny = 1e-30f;     // blocks below this are kept as zeros (127 / a would not be finite)
+constexpr float kCodeTiny = 1e-30f;     // blocks below this are kept as zeros (1 / a would not be finite)
 
 struct ClPlan {
     uint32_t positions, channels, columns, groups;
@@ -112,8 +112,8 @@ __device__ __forceinline__ float finite_abs(float v) {
     const float a = fabsf(v);
     return a <= 3.402823466e38f ? a : 0.0f;  // (false for NaN)
 }
-__device__ __forceinline__ float code_inverse(float most) { return most < kCodeTiny ? 0.0f : 127.0f / most; }
-__device__ __forceinline__ float code_scale(float most) { return most < kCodeTiny ? 0.0f : most / 127.0f; }
+__device__ __forceinline__ float code_inverse(float most) { return most < kCodeTiny ? 0.0f : 127.0f * (1.0f / most); }
+__device__ __forceinline__ float code_scale(float most) { return most < kCodeTiny ? 0.0f : most * (1.0f / 127.0f); }
 __device__ __forceinline__ int code_of(float h, float inv) {
     return (int)fminf(fmaxf(__builtin_rintf(h * inv), -127.0f), 127.0f);
 }

@@ -42,9 +42,9 @@ def checkpoint(h):
     finite = torch.where(blocks.abs() <= torch.finfo(torch.float32).max, blocks.abs(), torch.zeros(()))
     most = finite.amax(dim=-1)
     empty = most < TINY
-    inv = torch.where(empty, torch.zeros(()), torch.tensor(127.0) / most)
+    inv = torch.where(empty, torch.zeros(()), torch.tensor(127.0) * (torch.tensor(1.0) / most))
     codes = torch.round(blocks * inv[..., None]).nan_to_num(-127.0).clamp(-127, 127).to(torch.int8)
-    return codes.reshape(b, p, -1)[:, :, :c].contiguous(), torch.where(empty, torch.zeros(()), most / torch.tensor(127.0))
+    return codes.reshape(b, p, -1)[:, :, :c].contiguous(), torch.where(empty, torch.zeros(()), most * (torch.tensor(1.0) / torch.tensor(127.0)))
 
 
 def restored(codes, scales):
