@@ -20,6 +20,7 @@ CSRC_DIR = os.path.join(_PKG_DIR, "csrc")
 LIB_HIP_PATH = os.path.join(CSRC_DIR, "libmsd_hip.so")
 LIB_NN_PATH = os.path.join(CSRC_DIR, "libmsd_nn.so")
 TORCH_CALLS_PATH = os.path.join(CSRC_DIR, "msd_torch_calls.so")
+TORCH_CALLS_CL_Q4_PATH = os.path.join(CSRC_DIR, "msd_torch_calls_cl_q4.so")  # channels-last norms, 4-bit weights
 
 DTYPE_F32 = 0
 DTYPE_F16 = 1
@@ -105,8 +106,9 @@ def load_library(path=None):
         if name != "msd_error_string":
             getattr(lib, name).restype = it
     _lib = lib
-    if not isinstance(_native, _Unbound):
-        _bind_addresses(_native)
+    for native in (_native, _native_cl_q4):
+        if not isinstance(native, _Unbound):
+            _bind_addresses(native)
     return lib
 
 
@@ -129,6 +131,11 @@ class _Unbound:
         return getattr(_bind_native(), name)
 
 
+class _UnboundClQ4(_Unbound):
+    def __getattr__(self, name):
+        return getattr(_bind_native_cl_q4(), name)
+
+
 class _NoNative:
     """Stands for the native calls where there are none: every call takes its general path."""
 
@@ -142,7 +149,7 @@ class _NoNative:
         pass
 
 
-_native = _Unbound()
+_native, _native_cl_q4 = _Unbound(), _UnboundClQ4()  # (two extensions: csrc/torch_calls.cpp, csrc/torch_calls_cl_q4.cpp)
 
 
 def _bind_addresses(native):
@@ -154,10 +161,11 @@ def _running(torch):
     return "Python %d.%d, torch %s (%s)" % (sys.version_info[:2] + (torch.version.__version__, torch.version.git_version))
 
 
-def _load_native(torch):
+def _load_native(torch, path=None):
     """The extension, or what stands for it where it is not built or was built for another torch: the C ABI takes tensors of
     any torch, but the extension reads them as its own torch lays them out."""
-    spec = importlib.util.spec_from_file_location("msd_torch_calls", TORCH_CALLS_PATH)
+    path = path or TORCH_CALLS_PATH
+    spec = importlib.util.spec_from_file_location(os.path.splitext(os.path.basename(path))[0], path)
     try:
         native = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(native)
@@ -167,7 +175,7 @@ def _load_native(torch):
         why = "was built for %s, this is %s" % (built_for, _running(torch))
     except ImportError as e:  # (no such file, or symbols that this torch does not have)
         why = "does not load: %s" % e
-    warnings.warn("%s %s; a call takes about 2.5 us longer without it (run __graft_entry__.build())" % (TORCH_CALLS_PATH, why),
+    warnings.warn("%s %s; a call takes about 2.5 us longer without it (run __graft_entry__.build())" % (path, why),
                   RuntimeWarning, stacklevel=4)
     return _NoNative()
 
@@ -181,6 +189,17 @@ def _bind_native():
         _bind_addresses(native)
         _native = native
     return _native
+
+
+def _bind_native_cl_q4():
+    global _native_cl_q4
+    load_library()
+    torch = _bind_torch()
+    if isinstance(_native_cl_q4, _Unbound):
+        native = _load_native(torch, TORCH_CALLS_CL_Q4_PATH)
+        _bind_addresses(native)
+        _native_cl_q4 = native
+    return _native_cl_q4
 
 
 _torch = None
@@ -385,6 +404,9 @@ def _channels_last_forward(x, gamma, beta, groups, eps, fuse_silu, chunk, out, s
 def groupnorm_channels_last(x, gamma, beta, groups, eps=1e-5, fuse_silu=False, chunk=None, out=None):
     """GroupNorm(x + chunk[:, :, None]) (+ SiLU) over channels-last tensors: x is [batch, C, H, W] in torch.channels_last order or a
     contiguous [batch, positions, C]; gamma / beta float32 [C]; chunk [batch, C] in x's dtype or None.  out may be x (in place)."""
+    done = _native_cl_q4.groupnorm_channels_last(x, gamma, beta, groups, eps, fuse_silu, chunk, out)
+    if done is not None:
+        return done
     return _channels_last_forward(x, gamma, beta, groups, eps, fuse_silu, chunk, out, None, None, None)
 
 
@@ -392,6 +414,11 @@ def groupnorm_channels_last_kept(x, gamma, beta, groups, eps=1e-5, fuse_silu=Fal
     """groupnorm_channels_last, and a KeptNorm for groupnorm_channels_last_backward.  It holds x and chunk, which must not
     change until then (out must not be x), or with keep8 their sum in 8 bits, a quarter of float32 and a half of float16
     (out may be x)."""
+    done = _native_cl_q4.groupnorm_channels_last_kept(x, gamma, beta, groups, eps, fuse_silu, chunk, out, keep8)
+    if done is not None:
+        y, codes, scales, stats = done
+        return y, KeptNorm(None if keep8 else x, None if keep8 else chunk, codes, scales, stats, gamma, beta, groups, fuse_silu,
+                           chunk is not None)
     batch, positions, channels = _channels_last(x)
     if out is not None and not keep8 and out.data_ptr() == x.data_ptr() and x.numel():
         raise MsdError("out must not be x unless keep8: the gradient needs x")
@@ -412,6 +439,9 @@ def groupnorm_channels_last_backward(dy, kept, affine=True, out=None):
     """-> (dx, dgamma, dbeta, dchunk) from dy, laid out as the forward call's x, and what that call kept.  dgamma and dbeta are
     float32 [C] (None unless affine); dchunk is [batch, C] in dy's dtype (None where the forward call had no chunk).
     out: receives dx; may be dy."""
+    done = _native_cl_q4.groupnorm_channels_last_backward(dy, affine, out, *kept)
+    if done is not None:
+        return done
     lib = _lib or load_library()
     batch, positions, channels = _channels_last(dy, "dy")
     code = _dtype_code(dy)
@@ -687,6 +717,9 @@ def _q4_group(x, scales):
 def linear_rows_q4(x, packed, scales, bias=None, act_in=ACT_NONE, act_out=ACT_NONE, out=None):
     """linear_rows with the weight in 4 bits: x [m <= 8, k], packed uint8 [n, k / 2] and scales [n, k / group] (x's dtype) as
     q4_pack makes them, bias float32 [n] or None -> [m, n]."""
+    done = _native_cl_q4.linear_rows_q4(x, packed, scales, bias, act_in, act_out, out)
+    if done is not None:
+        return done
     lib = _lib or load_library()
     xp = _on_current_device(x, "x")
     group = _q4_group(x, scales)
@@ -702,6 +735,9 @@ def linear_rows_q4(x, packed, scales, bias=None, act_in=ACT_NONE, act_out=ACT_NO
 def linear_rows_q4_grouped(x, packed, scales, biases=None, act_in=ACT_NONE, act_out=ACT_NONE):
     """One launch for several such layers on the same x [m <= 8, k], all with the same group: lists of packed weights, scales and
     biases (or None) -> list of [m, n_i] tensors."""
+    done = _native_cl_q4.linear_rows_q4_grouped(x, packed, scales, biases, act_in, act_out)
+    if done is not None:
+        return done
     lib = _lib or load_library()
     xp = _on_current_device(x, "x")
     if len(packed) != len(scales) or (biases is not None and len(biases) != len(packed)):

@@ -2,7 +2,7 @@
 
     libmsd_hip.so   HIP kernels + the C ABI declared in include/msd_hip.h
     libmsd_nn.so    C++ host layer objects (GroupNorm / LayerNorm / GEGLU / ...) on top of it
-    msd_torch_calls.so  the package's calls for plain torch tensors (a CPython extension, host only)
+    msd_torch_calls.so, msd_torch_calls_cl_q4.so  the package's calls for plain torch tensors (CPython extensions, host only)
     cli/msd_compare golden-file comparison tool (host only)
     cli/msd_layer_check  runs the layer objects against golden .npy files (needs a GPU)
 
@@ -38,7 +38,7 @@ DEVICE_FLAGS = [
 
 LIB_HIP = os.path.join(CSRC, "libmsd_hip.so")
 LIB_NN = os.path.join(CSRC, "libmsd_nn.so")
-TORCH_CALLS = os.path.join(CSRC, "msd_torch_calls.so")
+TORCH_CALLS = [os.path.join(CSRC, name) for name in ("msd_torch_calls.so", "msd_torch_calls_cl_q4.so")]
 CLI_COMPARE = os.path.join(CSRC, "cli", "msd_compare")
 CLI_LAYER_CHECK = os.path.join(CSRC, "cli", "msd_layer_check")
 
@@ -103,20 +103,22 @@ def _runs_with(torch_dir):
 
 
 def build_torch_calls():
-    """msd_torch_calls.so: host C++ against the headers and libraries of the torch that will import it; None where there is no
+    """The extensions: host C++ against the headers and libraries of the torch that will import them; none where there is no
     such torch, which nothing else here needs.  NDEBUG, as torch itself is built: without it pybind11's headers give the library
     a thread-local counter that nothing here reads, and glibc takes the slow path of every thread-local access of a process
     (torch's and the runtime's among them) until the thread has touched those of the library loaded last (torch.empty 1.26 us
     against 1.00)."""
     torch_dir = torch_with_hip_headers()
     if torch_dir is None:
-        return None
-    _run([os.environ.get("CXX", "g++"), "-O2", "-DNDEBUG", "-std=c++17", "-fPIC", "-shared", "-DUSE_ROCM", "-D__HIP_PLATFORM_AMD__",
-          '-DMSD_BUILT_FOR="%s"' % _runs_with(torch_dir),
-          "-Wall", "-Wno-deprecated-declarations", "-isystem", os.path.join(torch_dir, "include"),
-          "-isystem", "/opt/rocm/include", "-isystem", sysconfig.get_paths()["include"],
-          os.path.join(CSRC, "torch_calls.cpp"), "-o", TORCH_CALLS, "-L", os.path.join(torch_dir, "lib"), "-ltorch_python",
-          "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip", "-L/opt/rocm/lib", "-lamdhip64"])
+        return []
+    for path in TORCH_CALLS:
+        source = os.path.basename(path)[len("msd_"):].replace(".so", ".cpp")
+        _run([os.environ.get("CXX", "g++"), "-O2", "-DNDEBUG", "-std=c++17", "-fPIC", "-shared", "-DUSE_ROCM", "-D__HIP_PLATFORM_AMD__",
+              '-DMSD_BUILT_FOR="%s"' % _runs_with(torch_dir),
+              "-Wall", "-Wno-deprecated-declarations", "-isystem", os.path.join(torch_dir, "include"),
+              "-isystem", "/opt/rocm/include", "-isystem", sysconfig.get_paths()["include"],
+              os.path.join(CSRC, source), "-o", path, "-L", os.path.join(torch_dir, "lib"), "-ltorch_python",
+              "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip", "-L/opt/rocm/lib", "-lamdhip64"])
     return TORCH_CALLS
 
 
@@ -147,13 +149,12 @@ def build_all(verbose=True):
     if nn:
         built.append(build_layer_check())
     torch_calls = build_torch_calls()
-    if torch_calls:
-        built.append(torch_calls)
+    built += torch_calls
     if verbose:
         for b in built:
             print("built", b)
         if not torch_calls:
-            print("skipped", TORCH_CALLS, "(no torch with HIP headers here)")
+            print("skipped", *TORCH_CALLS, "(no torch with HIP headers here)")
     return built
 
 
