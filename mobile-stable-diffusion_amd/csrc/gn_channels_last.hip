@@ -9,10 +9,12 @@
 //   dx = rstd (gamma dz - m1 - u m2);  dgamma = sum_b S2;  dbeta = sum_b S1
 //   dchunk[b, c] = sum_p dx = rstd (gamma S1 - P m1 - m2 sum_p u)
 //
-// A group's statistics need all positions of a sample, so each direction is a pass of sums and a pass
-// that applies them.  A workgroup owns `tx` columns (a column: VEC neighbouring channels, what a lane
-// moves at once) of a slice of positions; its lanes lie along the columns first, so a wavefront reads
-// whole rows one after the other, and a lane keeps its channels, whose constants stay in registers.
+// A column is VEC neighbouring channels, what a lane moves at once.  A workgroup owns `tx` columns (a
+// chunk) of some positions; its lanes lie along the columns first, so a wavefront reads whole rows one
+// after the other, and a lane keeps its channels, whose constants stay in registers.
+// A group's statistics need all positions of a sample.  Small samples: a workgroup has all positions of
+// its chunk in registers, one launch (cl_unit_kernel, cl_unit_grads_kernel).  Others: a launch of sums
+// over slices of the positions and a launch that joins them and applies them.
 #include "msd_device.h"
 #include "msd_internal.h"
 
@@ -25,11 +27,15 @@
 namespace msd {
 namespace {
 
-constexpr uint32_t kClThreads = 512;    // most lanes of a workgroup
+constexpr uint32_t kClThreads = 512;    // most lanes of a workgroup that has a slice of the positions
+constexpr uint32_t kClBlocks = 512;     // workgroups of a launch of slices: two per CU
 constexpr uint32_t kClMaxTx = 320;      // most columns of a workgroup
-constexpr uint32_t kClRows = 4;         // rows a lane requests before it uses the first
-constexpr uint32_t kClMaxParts = 128;   // partial sums per group up to which every workgroup adds them up itself
-constexpr uint32_t kClTeam = 16;        // lanes that add up a group
+constexpr uint32_t kClRows = 2;         // rows a lane uses while as many are on their way
+constexpr uint32_t kClMaxParts = 128;   // slices up to which every workgroup joins their sums itself
+constexpr uint32_t kClJoinThreads = 256;
+constexpr uint32_t kClTeam = 16;        // lanes that add up a group's channels
+constexpr uint32_t kClUnitThreads = 1024;
+constexpr uint32_t kClUnitMaxK = 4;     // most rows a lane holds of a workgroup that has all positions
 constexpr uint32_t kCodeBlock = 32;     // channels of one position that share a scale
 constexpr float kCodeTiny = 1e-30f;     // blocks below this are kept as zeros (1 / a would not be finite)
 
@@ -38,7 +44,7 @@ struct ClPlan {
     uint32_t tx, ty, chunks;            // columns and rows of a workgroup; workgroups along the columns
     uint32_t slices, rows;              // workgroups along the positions, positions of each (but the last)
     uint32_t spans;                     // most chunks that share one group
-    FastDiv per_group, by_tx;
+    FastDiv per_group, by_tx, by_slices, by_chunks;
 };
 
 // What a workgroup is: sample, slice, chunk and its bounds.
@@ -46,10 +52,10 @@ struct ClTile {
     uint32_t b, slice, chunk, col0, cols, row0, rows, tx, ty;
     bool live;
     __device__ ClTile(const ClPlan &p, uint32_t block) {
-        slice = block % p.slices;
-        const uint32_t rest = block / p.slices;
-        chunk = rest % p.chunks;
-        b = rest / p.chunks;
+        const uint32_t rest = fast_div(block, p.by_slices);
+        slice = block - rest * p.slices;
+        b = fast_div(rest, p.by_chunks);
+        chunk = rest - b * p.chunks;
         col0 = chunk * p.tx;
         cols = min(p.tx, p.columns - col0);
         row0 = slice * p.rows;
@@ -60,7 +66,7 @@ struct ClTile {
     }
 };
 
-// Groups that have channels in [c0, c1), and which of a group's chunks this is.
+// Groups that have channels in [c0, c1).
 struct ClGroups {
     uint32_t first, count;
     __device__ ClGroups(const ClPlan &p, uint32_t c0, uint32_t c1) {
@@ -77,6 +83,19 @@ struct Row<T, 16 / sizeof(T)> {
     __device__ __forceinline__ void load(const T *p) { v = *reinterpret_cast<const u32x4 *>(p); }
     __device__ __forceinline__ void floats(float *f) const { Store<T>::unpack(v, f); }
     static __device__ __forceinline__ void store(T *p, const float *f) { *reinterpret_cast<u32x4 *>(p) = Store<T>::pack(f); }
+    // the sum, rounded to the storage type (of halves: once, as by way of float32, whose 24 bits are 2 * 11 + 2)
+    __device__ __forceinline__ void add(const Row &o) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if constexpr (sizeof(T) == 4) {
+                v[i] = __float_as_uint(__uint_as_float(v[i]) + __uint_as_float(o.v[i]));
+            } else {
+                const uint32_t a = v[i], b = o.v[i];
+                const __half2 h = __hadd2(*reinterpret_cast<const __half2 *>(&a), *reinterpret_cast<const __half2 *>(&b));
+                v[i] = *reinterpret_cast<const uint32_t *>(&h);
+            }
+        }
+    }
 };
 template <typename T>
 struct Row<T, 1> {
@@ -84,6 +103,7 @@ struct Row<T, 1> {
     __device__ __forceinline__ void load(const T *p) { v = *p; }
     __device__ __forceinline__ void floats(float *f) const { f[0] = Store<T>::load1(&v); }
     static __device__ __forceinline__ void store(T *p, const float *f) { Store<T>::store1(p, f[0]); }
+    __device__ __forceinline__ void add(const Row &o) { Store<T>::store1(&v, Store<T>::load1(&v) + Store<T>::load1(&o.v)); }
 };
 
 // The codes of VEC neighbouring channels and their scale.
@@ -93,8 +113,7 @@ struct Codes {
     float scale;
     __device__ __forceinline__ void load(const int8_t *p, const float *s) {
         if constexpr (VEC == 8) {
-            const uint2 w = *reinterpret_cast<const uint2 *>(p);
-            *reinterpret_cast<uint2 *>(v) = w;
+            *reinterpret_cast<uint2 *>(v) = *reinterpret_cast<const uint2 *>(p);
         } else if constexpr (VEC == 4) {
             *reinterpret_cast<uint32_t *>(v) = *reinterpret_cast<const uint32_t *>(p);
         } else {
@@ -118,16 +137,31 @@ __device__ __forceinline__ int code_of(float h, float inv) {
     return (int)fminf(fmaxf(__builtin_rintf(h * inv), -127.0f), 127.0f);
 }
 
-// h of a row: the input, plus the addend in the storage type.
-template <typename T, int VEC, bool ADD>
-__device__ __forceinline__ void add_chunk(float *f, const float *add) {
-    if (ADD) {
+// Stores the codes of a lane's VEC channels, and their scale from the first lane of the block.  The lanes of a block are
+// neighbours of one row: chunks begin at whole blocks, and their columns are a multiple of a block's.
+template <int VEC>
+__device__ __forceinline__ void keep_codes(const float *f, int8_t *codes, float *scale, bool first) {
+    float most = 0.0f;
 #pragma unroll
-        for (int e = 0; e < VEC; e++) f[e] = round_to_storage<T>(f[e] + add[e]);
+    for (int e = 0; e < VEC; e++) most = fmaxf(most, finite_abs(f[e]));
+    most = team_max<kCodeBlock / VEC>(most);
+    const float inv = code_inverse(most);
+    uint32_t w[VEC / 4];
+#pragma unroll
+    for (int e = 0; e < VEC; e += 4) {
+        w[e / 4] = 0;
+#pragma unroll
+        for (int k = 0; k < 4; k++) w[e / 4] |= (uint32_t)(code_of(f[e + k], inv) & 255) << (8 * k);
     }
+    if constexpr (VEC == 8) *reinterpret_cast<uint2 *>(codes) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint32_t *>(codes) = w[0];
+    if (first) *scale = code_scale(most);
 }
 
-// Adds `count` floats per channel over the rows of the workgroup: red holds [ty][cols * VEC].
+// ---------------------------------------------------------------------------
+// Sums over the rows of a workgroup, through LDS: red holds [ty][cc], a lane has put its channels there.
+// On return row 0 has the totals.
+// ---------------------------------------------------------------------------
 template <int VEC>
 __device__ __forceinline__ void put_channels(float *red, const ClTile &t, const float *v) {
     if (t.live) {
@@ -136,239 +170,466 @@ __device__ __forceinline__ void put_channels(float *red, const ClTile &t, const 
     }
 }
 
+// Sums of rows first, first + step, ... of a column; four reads under way at a time.
+template <int N>
+__device__ __forceinline__ void add_column(const float *red, uint32_t stride, uint32_t cc, uint32_t c, uint32_t first, uint32_t step,
+                                           uint32_t ty, float *total) {
+#pragma unroll
+    for (int i = 0; i < N; i++) total[i] = 0.0f;
+    for (uint32_t r = first; r < ty; r += 4 * step) {
+        float v[N][4];
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+#pragma unroll
+            for (int i = 0; i < N; i++) v[i][k] = red[i * stride + min(r + k * step, ty - 1) * cc + c];
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+#pragma unroll
+            for (int i = 0; i < N; i++) total[i] += r + k * step < ty ? v[i][k] : 0.0f;
+    }
+}
+
+template <int N>
+__device__ __forceinline__ void add_rows(float *red, uint32_t stride, uint32_t ty, uint32_t cc) {
+    const uint32_t lanes = min(blockDim.x / cc, ty / 4);  // lanes that share a channel
+    float total[N];
+    __syncthreads();
+    if (lanes > 1) {
+        const uint32_t j = threadIdx.x / cc, c = threadIdx.x - j * cc;
+        if (j < lanes) {
+            add_column<N>(red, stride, cc, c, j, lanes, ty, total);
+#pragma unroll
+            for (int i = 0; i < N; i++) red[i * stride + threadIdx.x] = total[i];  // (row j: no other lane reads this one's rows)
+        }
+        __syncthreads();
+        ty = lanes;
+    }
+    for (uint32_t c = threadIdx.x; c < cc; c += blockDim.x) {
+        add_column<N>(red, stride, cc, c, 0, 1, ty, total);
+#pragma unroll
+        for (int i = 0; i < N; i++) red[i * stride + c] = total[i];
+    }
+    __syncthreads();
+}
+
+// Mean and squared deviations of every group's part in a workgroup's channels and rows, from the channels' sums of deviations
+// from shift[c] (red: [2][ty][cc], of values and of squares): done(i, mean, m2, channels) by the first lane of a team, for group
+// i of `groups`.  Deviations are taken channel by channel from a value of the channel, so that a mean far from zero costs no
+// digits; the channels, of equal size n, are joined by M2 = sum M2_c + n sum (mean_c - mean)^2.
+template <typename F>
+__device__ __forceinline__ void group_moments(float *red, const float *shift, uint32_t ty, uint32_t cc, uint32_t c0, float n,
+                                              const ClPlan &p, const ClGroups &groups, F done) {
+    const uint32_t stride = ty * cc;
+    add_rows<2>(red, stride, ty, cc);
+    for (uint32_t c = threadIdx.x; c < cc; c += blockDim.x) {
+        const float a = red[c], m2 = fmaf(-a / n, a, red[stride + c]);
+        red[c] = shift[c] + a / n;
+        red[stride + c] = m2 < 0.0f ? 0.0f : m2;  // (NaN stays)
+    }
+    __syncthreads();
+    const uint32_t team = threadIdx.x / kClTeam, lane = threadIdx.x % kClTeam, teams = blockDim.x / kClTeam;
+    for (uint32_t i = team; i < groups.count; i += teams) {
+        const uint32_t g = groups.first + i;
+        const uint32_t lo = max(g * p.per_group.d, c0) - c0, hi = min((g + 1) * p.per_group.d, c0 + cc) - c0;
+        constexpr uint32_t kHeld = 5;  // channels a lane keeps in registers between the two sums
+        float sum = 0.0f, m2 = 0.0f, means[kHeld], m2s[kHeld];
+#pragma unroll
+        for (uint32_t k = 0; k < kHeld; k++) {
+            const uint32_t c = min(lo + lane + k * kClTeam, hi - 1);
+            means[k] = red[c];
+            m2s[k] = red[stride + c];
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < kHeld; k++) sum += lo + lane + k * kClTeam < hi ? means[k] : 0.0f;
+        for (uint32_t c = lo + lane + kHeld * kClTeam; c < hi; c += kClTeam) sum += red[c];
+        const float mean = team_sum<kClTeam>(sum) / (float)(hi - lo);
+#pragma unroll
+        for (uint32_t k = 0; k < kHeld; k++) {
+            const float d = means[k] - mean;
+            m2 += lo + lane + k * kClTeam < hi ? fmaf(n * d, d, m2s[k]) : 0.0f;
+        }
+        for (uint32_t c = lo + lane + kHeld * kClTeam; c < hi; c += kClTeam) {
+            const float d = red[c] - mean;
+            m2 += fmaf(n * d, d, red[stride + c]);
+        }
+        m2 = team_sum<kClTeam>(m2);
+        if (lane == 0) done(i, mean, m2, (float)(hi - lo));
+    }
+}
+
+// Sums over every group's part of two values per channel.
+template <typename F>
+__device__ __forceinline__ void group_sums(const float *va, const float *vb, uint32_t cc, uint32_t c0, const ClPlan &p,
+                                           const ClGroups &groups, F done) {
+    const uint32_t team = threadIdx.x / kClTeam, lane = threadIdx.x % kClTeam, teams = blockDim.x / kClTeam;
+    for (uint32_t i = team; i < groups.count; i += teams) {
+        const uint32_t g = groups.first + i;
+        const uint32_t lo = max(g * p.per_group.d, c0) - c0, hi = min((g + 1) * p.per_group.d, c0 + cc) - c0;
+        float a = 0.0f, q = 0.0f;
+#pragma unroll 4
+        for (uint32_t c = lo + lane; c < hi; c += kClTeam) {
+            a += va[c];
+            q += vb[c];
+        }
+        a = team_sum<kClTeam>(a);
+        q = team_sum<kClTeam>(q);
+        if (lane == 0) done(i, a, q);
+    }
+}
+
+// Adds a row's deviations from `shift` to the sums.
+template <int VEC>
+__device__ __forceinline__ void add_moments(const float *f, const float *shift, float *s1, float *s2) {
+#pragma unroll
+    for (int e = 0; e < VEC; e++) {
+        const float d = f[e] - shift[e];
+        s1[e] += d;
+        s2[e] = fmaf(d, d, s2[e]);
+    }
+}
+
 // ---------------------------------------------------------------------------
-// Statistics: mean and sum of squared deviations of a slice's part of every group.  Deviations are taken from the
-// slice's first row, channel by channel, so that a mean far from zero costs no digits; channels are then joined by the
-// formula for parts of equal size, M2 = sum M2_c + n sum (mean_c - mean)^2.
+// Statistics of a slice of positions: partials [batch][slices][spans][groups], (mean, M2).
 // ---------------------------------------------------------------------------
 template <typename T, int VEC, bool ADD>
 __global__ __launch_bounds__(kClThreads) void cl_stats_kernel(const T *x, const T *chunk, float2 *partials, ClPlan p) {
     extern __shared__ float lds[];
     const ClTile t(p, blockIdx.x);
     const uint32_t cc = t.cols * VEC, c0 = t.col0 * VEC;
-    float s1[VEC], s2[VEC], shift[VEC], add[VEC];
+    float s1[VEC], s2[VEC], shift[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; e++) s1[e] = s2[e] = 0.0f;
     if (t.live) {
         const uint32_t c = c0 + t.tx * VEC;
         const T *at = x + ((size_t)t.b * p.positions + t.row0) * p.channels + c;
-        Row<T, VEC> r[kClRows], first;
+        Row<T, VEC> r[kClRows], next[kClRows], first, add;
+        auto request = [&](Row<T, VEC> *to, uint32_t row) {
+#pragma unroll
+            for (uint32_t i = 0; i < kClRows; i++) to[i].load(at + min(row + i * p.ty, t.rows - 1) * p.channels);
+        };
         first.load(at);
+        request(r, t.ty);
         if (ADD) {
-            Row<T, VEC> a;
-            a.load(chunk + (size_t)t.b * p.channels + c);
-            a.floats(add);
+            add.load(chunk + (size_t)t.b * p.channels + c);
+            first.add(add);
         }
         first.floats(shift);
-        add_chunk<T, VEC, ADD>(shift, add);
-        for (uint32_t row = t.ty; row < t.rows; row += p.ty * kClRows) {
-#pragma unroll
-            for (uint32_t i = 0; i < kClRows; i++) r[i].load(at + (size_t)min(row + i * p.ty, t.rows - 1) * p.channels);
+        for (uint32_t row = t.ty; row < t.rows;) {
+            const uint32_t ahead = row + p.ty * kClRows;
+            if (ahead < t.rows) request(next, ahead);
 #pragma unroll
             for (uint32_t i = 0; i < kClRows; i++) {
                 if (row + i * p.ty < t.rows) {
+                    if (ADD) r[i].add(add);
                     float f[VEC];
                     r[i].floats(f);
-                    add_chunk<T, VEC, ADD>(f, add);
-#pragma unroll
-                    for (int e = 0; e < VEC; e++) {
-                        const float d = f[e] - shift[e];
-                        s1[e] += d;
-                        s2[e] = fmaf(d, d, s2[e]);
-                    }
+                    add_moments<VEC>(f, shift, s1, s2);
                 }
+                r[i] = next[i];
             }
+            row = ahead;
         }
     }
-    float *red1 = lds, *red2 = lds + p.ty * cc, *first_row = red2 + p.ty * cc;
-    put_channels<VEC>(red1, t, s1);
-    put_channels<VEC>(red2, t, s2);
+    float *first_row = lds + 2 * p.ty * cc;
+    put_channels<VEC>(lds, t, s1);
+    put_channels<VEC>(lds + p.ty * cc, t, s2);
     if (t.ty == 0) put_channels<VEC>(first_row, t, shift);
-    __syncthreads();
-    const float n = (float)t.rows;
-    for (uint32_t c = threadIdx.x; c < cc; c += blockDim.x) {
-        float a = 0.0f, q = 0.0f;
-        for (uint32_t j = 0; j < p.ty; j++) {
-            a += red1[j * cc + c];
-            q += red2[j * cc + c];
-        }
-        red1[c] = first_row[c] + a / n;                 // mean of the channel
-        const float m2 = fmaf(-a / n, a, q);            // its squared deviations
-        red2[c] = m2 < 0.0f ? 0.0f : m2;                // (NaN stays)
-    }
-    __syncthreads();
     const ClGroups groups(p, c0, c0 + cc);
-    const uint32_t team = threadIdx.x / kClTeam, lane = threadIdx.x % kClTeam, teams = blockDim.x / kClTeam;
-    for (uint32_t i = team; i < groups.count; i += teams) {
-        const uint32_t g = groups.first + i;
-        const uint32_t lo = max(g * p.per_group.d, c0) - c0, hi = min((g + 1) * p.per_group.d, c0 + cc) - c0;
-        float sum = 0.0f;
-        for (uint32_t c = lo + lane; c < hi; c += kClTeam) sum += red1[c];
-        const float mean = team_sum<kClTeam>(sum) / (float)(hi - lo);
-        float m2 = 0.0f;
-        for (uint32_t c = lo + lane; c < hi; c += kClTeam) {
-            const float d = red1[c] - mean;
-            m2 += fmaf(n * d, d, red2[c]);
+    group_moments(lds, first_row, p.ty, cc, c0, (float)t.rows, p, groups, [&](uint32_t i, float mean, float m2, float) {
+        const uint32_t g = groups.first + i, span = p.spans == 1 ? 0 : t.chunk - g * p.per_group.d / VEC / p.tx;
+        partials[(((size_t)t.b * p.slices + t.slice) * p.spans + span) * p.groups + g] = make_float2(mean, m2);
+    });
+}
+
+// ---------------------------------------------------------------------------
+// Joining the slices.
+// ---------------------------------------------------------------------------
+struct ClParts {  // what a launch of sums left
+    const float2 *at;
+    uint32_t slices, rows;
+};
+
+// A group's value from the parts of its slices.  Statistics: means by their distance from the first slice's, which costs no
+// digits; M2 = sum of the parts' M2 and of their n times the squared distance of their mean from the whole's.
+template <bool STATS>
+struct PartSum {
+    const ClPlan &p;
+    const ClParts &parts;
+    float shift, a = 0.0f, q = 0.0f, r = 0.0f;
+    __device__ PartSum(const ClPlan &p, const ClParts &parts, const float2 *first) : p(p), parts(parts), shift(STATS ? first->x : 0.0f) {}
+    __device__ __forceinline__ void add(uint32_t s, float2 v) {
+        if (STATS) {
+            const float w = (float)min(parts.rows, p.positions - s * parts.rows), d = v.x - shift;
+            a = fmaf(w, d, a);
+            r = fmaf(w * d, d, r);
+        } else {
+            a += v.x;
         }
-        m2 = team_sum<kClTeam>(m2);
-        const uint32_t span = t.chunk - g * p.per_group.d / VEC / p.tx;
-        if (lane == 0)
-            partials[(((size_t)t.b * p.slices + t.slice) * p.spans + span) * p.groups + g] = make_float2(mean, m2);
+        q += v.y;
+    }
+    __device__ __forceinline__ float2 value(float eps) const {
+        const float count = (float)p.positions, per = (float)p.per_group.d;
+        if (!STATS) return make_float2(a / (count * per), q / (count * per));
+        const float off = a / count, m2 = fmaf(per, fmaf(-off, a, r), q);  // (off: the mean's distance from the shift)
+        return make_float2(shift + off, 1.0f / sqrtf((m2 < 0.0f ? 0.0f : m2) / (count * per) + eps));
+    }
+};
+
+// By the 32 lanes of every half wavefront, one a group; they share the slices.  red: [blockDim / 64][3][32].
+template <bool STATS>
+__device__ __forceinline__ void join_whole_groups(const ClPlan &p, const ClParts &parts, uint32_t b, const ClGroups &groups, float eps,
+                                                  float2 *of_group, float (*red)[3][32]) {
+    const uint32_t lane = threadIdx.x % 32, half = threadIdx.x / 32, halves = blockDim.x / 32;
+    for (uint32_t g0 = 0; g0 < groups.count; g0 += 32) {
+        const float2 *at = parts.at + (size_t)b * parts.slices * p.groups + groups.first + min(g0 + lane, groups.count - 1);
+        PartSum<STATS> sum(p, parts, at);
+#pragma unroll 4
+        for (uint32_t s = half; s < parts.slices; s += halves) sum.add(s, at[(size_t)s * p.groups]);
+        sum.a = half_pair_sum(sum.a);
+        sum.q = half_pair_sum(sum.q);
+        if (STATS) sum.r = half_pair_sum(sum.r);
+        if (threadIdx.x % kWave < 32) {
+            red[threadIdx.x / kWave][0][lane] = sum.a;
+            red[threadIdx.x / kWave][1][lane] = sum.q;
+            red[threadIdx.x / kWave][2][lane] = sum.r;
+        }
+        __syncthreads();
+        if (threadIdx.x < 32 && g0 + lane < groups.count) {
+            for (uint32_t w = 1; w < blockDim.x / kWave; w++) {
+                sum.a += red[w][0][lane];
+                sum.q += red[w][1][lane];
+                sum.r += red[w][2][lane];
+            }
+            of_group[g0 + lane] = sum.value(eps);
+        }
+        __syncthreads();
     }
 }
 
-// How many values partial (slice, span) of group g is of.
-__device__ __forceinline__ float part_count(const ClPlan &p, uint32_t vec, uint32_t g, uint32_t slice, uint32_t span) {
-    const uint32_t lo = g * p.per_group.d, hi = lo + p.per_group.d, chunk_channels = p.tx * vec;
-    const uint32_t c0 = (lo / chunk_channels + span) * chunk_channels;
-    const uint32_t a = max(lo, c0), b = min(hi, c0 + chunk_channels);
-    return (float)min(p.rows, p.positions - slice * p.rows) * (float)(b - a);
-}
-__device__ __forceinline__ uint32_t group_spans(const ClPlan &p, uint32_t vec, uint32_t g) {
-    const uint32_t lo = g * p.per_group.d, hi = lo + p.per_group.d, chunk_channels = p.tx * vec;
-    return (hi - 1) / chunk_channels - lo / chunk_channels + 1;
-}
-
+// The same where a group can be spread over several chunks, by a team of TEAM lanes per group.
 template <int TEAM>
 __device__ __forceinline__ float sum_over(float v) {
     if constexpr (TEAM > 1) v = team_sum<TEAM>(v);
     return v;
 }
-
-// Mean and 1 / sqrt(variance + eps) of group g of sample b, by a team of TEAM lanes; every lane gets them.
-template <int TEAM>
-__device__ __forceinline__ float2 join_stats(const ClPlan &p, uint32_t vec, const float2 *partials, uint32_t b, uint32_t g,
-                                             float eps, uint32_t lane) {
-    const uint32_t spans = group_spans(p, vec, g), parts = p.slices * spans;
-    const float2 *at = partials + (size_t)b * p.slices * p.spans * p.groups + g;
+template <bool STATS, int TEAM>
+__device__ __forceinline__ float2 join_spread_group(const ClPlan &p, const ClParts &parts, uint32_t vec, uint32_t b, uint32_t g,
+                                                    float eps, uint32_t lane) {
+    const uint32_t lo = g * p.per_group.d, hi = lo + p.per_group.d, chunk_channels = p.tx * vec, first = lo / chunk_channels;
+    const uint32_t spans = (hi - 1) / chunk_channels - first + 1, count = parts.slices * spans;
+    const float2 *at = parts.at + (size_t)b * parts.slices * p.spans * p.groups + g;
     const float total = (float)p.positions * (float)p.per_group.d;
-    float sum = 0.0f;
-    for (uint32_t i = lane; i < parts; i += TEAM) {
-        const uint32_t slice = i / spans, span = i % spans;
-        sum = fmaf(at[((size_t)slice * p.spans + span) * p.groups].x, part_count(p, vec, g, slice, span) / total, sum);
-    }
-    const float mean = sum_over<TEAM>(sum);
-    float m2 = 0.0f;
-    for (uint32_t i = lane; i < parts; i += TEAM) {
-        const uint32_t slice = i / spans, span = i % spans;
-        const float2 v = at[((size_t)slice * p.spans + span) * p.groups];
-        const float d = v.x - mean;
-        m2 += fmaf(part_count(p, vec, g, slice, span) * d, d, v.y);
-    }
-    m2 = sum_over<TEAM>(m2);
-    return make_float2(mean, 1.0f / sqrtf(m2 / total + eps));
-}
-
-// Means over group g of the two summands of the gradient.
-template <int TEAM>
-__device__ __forceinline__ float2 join_sums(const ClPlan &p, uint32_t vec, const float2 *partials, uint32_t b, uint32_t g,
-                                            uint32_t lane) {
-    const uint32_t spans = group_spans(p, vec, g), parts = p.slices * spans;
-    const float2 *at = partials + (size_t)b * p.slices * p.spans * p.groups + g;
+    auto part = [&](uint32_t i) { return at[((size_t)(i / spans) * p.spans + i % spans) * p.groups]; };
+    auto size = [&](uint32_t i) {
+        const uint32_t c0 = (first + i % spans) * chunk_channels, s = i / spans;
+        return (float)min(parts.rows, p.positions - s * parts.rows) * (float)(min(hi, c0 + chunk_channels) - max(lo, c0));
+    };
     float a = 0.0f, q = 0.0f;
-    for (uint32_t i = lane; i < parts; i += TEAM) {
-        const float2 v = at[((size_t)(i / spans) * p.spans + i % spans) * p.groups];
-        a += v.x;
+    for (uint32_t i = lane; i < count; i += TEAM) {
+        const float2 v = part(i);
+        a = STATS ? fmaf(v.x, size(i) / total, a) : a + v.x;
         q += v.y;
     }
     a = sum_over<TEAM>(a);
+    if (STATS) {
+        q = 0.0f;
+        for (uint32_t i = lane; i < count; i += TEAM) {
+            const float2 v = part(i);
+            const float d = v.x - a;
+            q += fmaf(size(i) * d, d, v.y);
+        }
+    }
     q = sum_over<TEAM>(q);
-    const float total = (float)p.positions * (float)p.per_group.d;
-    return make_float2(a / total, q / total);
+    return STATS ? make_float2(a, 1.0f / sqrtf(q / total + eps)) : make_float2(a / total, q / total);
 }
 
-// One wavefront per (sample, group), for more parts than every workgroup should add up by itself.
 template <bool STATS>
-__global__ __launch_bounds__(kWave) void cl_join_kernel(const float2 *partials, float2 *joined, float eps, uint32_t vec, ClPlan p) {
-    const uint32_t b = blockIdx.x / p.groups, g = blockIdx.x % p.groups;
-    const float2 v = STATS ? join_stats<kWave>(p, vec, partials, b, g, eps, threadIdx.x)
-                           : join_sums<kWave>(p, vec, partials, b, g, threadIdx.x);
-    if (threadIdx.x == 0) joined[blockIdx.x] = v;
+__device__ __forceinline__ void join_groups(const ClPlan &p, const ClParts &parts, const float2 *joined, uint32_t vec, uint32_t b,
+                                            const ClGroups &groups, float eps, float2 *of_group, float (*red)[3][32]) {
+    if (joined != nullptr) {
+        for (uint32_t i = threadIdx.x; i < groups.count; i += blockDim.x) of_group[i] = joined[(size_t)b * p.groups + groups.first + i];
+    } else if (p.spans == 1) {
+        join_whole_groups<STATS>(p, parts, b, groups, eps, of_group, red);
+    } else {
+        for (uint32_t i = threadIdx.x / kClTeam; i < groups.count; i += blockDim.x / kClTeam) {
+            const float2 v = join_spread_group<STATS, kClTeam>(p, parts, vec, b, groups.first + i, eps, threadIdx.x % kClTeam);
+            if (threadIdx.x % kClTeam == 0) of_group[i] = v;
+        }
+    }
+    __syncthreads();
+}
+
+// For more slices than every workgroup should join by itself: a workgroup per group of a sample.
+template <bool STATS>
+__global__ __launch_bounds__(kClJoinThreads) void cl_join_kernel(ClParts parts, float2 *joined, float eps, uint32_t vec, ClPlan p) {
+    __shared__ float red[3][kClJoinThreads / kWave];
+    const uint32_t b = blockIdx.x / p.groups, g = blockIdx.x - b * p.groups;
+    if (p.spans != 1) {
+        if (threadIdx.x >= kWave) return;
+        const float2 v = join_spread_group<STATS, kWave>(p, parts, vec, b, g, eps, threadIdx.x);
+        if (threadIdx.x == 0) joined[blockIdx.x] = v;
+        return;
+    }
+    const float2 *at = parts.at + (size_t)b * parts.slices * p.groups + g;
+    PartSum<STATS> sum(p, parts, at);
+#pragma unroll 4
+    for (uint32_t s = threadIdx.x; s < parts.slices; s += kClJoinThreads) sum.add(s, at[(size_t)s * p.groups]);
+    sum.a = block_sum<kClJoinThreads / kWave>(sum.a, red[0]);
+    sum.q = block_sum<kClJoinThreads / kWave>(sum.q, red[1]);
+    sum.r = block_sum<kClJoinThreads / kWave>(sum.r, red[2]);
+    if (threadIdx.x == 0) joined[blockIdx.x] = sum.value(eps);
 }
 
 // ---------------------------------------------------------------------------
 // y = act(gamma (h - mean) rstd + beta), and with KEEP the 8-bit codes of h.
 // `joined`: the statistics, where cl_join_kernel has been there.  `stats`: receives them, or null.
 // ---------------------------------------------------------------------------
-template <typename T, int VEC, bool ADD, bool SILU, bool KEEP>
-__global__ __launch_bounds__(kClThreads) void cl_apply_kernel(const T *x, const T *chunk, T *y, const float *gamma,
-                                                              const float *beta, const float2 *partials,
-                                                              const float2 *joined, float2 *stats, int8_t *codes,
-                                                              float *scales, float eps, ClPlan p) {
-    extern __shared__ float2 of_group[];
-    const ClTile t(p, blockIdx.x);
-    const uint32_t c0 = t.col0 * VEC, cc = t.cols * VEC;
-    const ClGroups groups(p, c0, c0 + cc);
-    const uint32_t team = threadIdx.x / kClTeam, team_lane = threadIdx.x % kClTeam, teams = blockDim.x / kClTeam;
-    for (uint32_t i = team; i < groups.count; i += teams) {
-        const uint32_t g = groups.first + i;
-        const float2 v = joined != nullptr ? joined[(size_t)t.b * p.groups + g]
-                                           : join_stats<kClTeam>(p, VEC, partials, t.b, g, eps, team_lane);
-        if (team_lane == 0) {
-            of_group[i] = v;
-            if (stats != nullptr && t.slice == 0) stats[(size_t)t.b * p.groups + g] = v;  // (a group's chunks agree)
+// A lane's constants, channel by channel: z = (h - mean) mul + off.
+template <int VEC>
+struct Affine {
+    float mean[VEC], mul[VEC], off[VEC];
+    __device__ __forceinline__ void request(const float *gamma, const float *beta, uint32_t c) {
+#pragma unroll
+        for (int e = 0; e < VEC; e++) {
+            mul[e] = gamma[c + e];
+            off[e] = beta[c + e];
         }
     }
-    __syncthreads();
-    if (!t.live) return;
-    const uint32_t c = c0 + t.tx * VEC;
-    float mean[VEC], mul[VEC], off[VEC], add[VEC];
-    if (ADD) {
-        Row<T, VEC> a;
-        a.load(chunk + (size_t)t.b * p.channels + c);
-        a.floats(add);
-    }
+    __device__ __forceinline__ void take(const ClPlan &p, const float2 *of_group, uint32_t first_group, uint32_t c) {
 #pragma unroll
-    for (int e = 0; e < VEC; e++) {
-        const float2 s = of_group[fast_div(c + e, p.per_group) - groups.first];
-        mean[e] = s.x;
-        mul[e] = s.y * gamma[c + e];
-        off[e] = beta[c + e];
+        for (int e = 0; e < VEC; e++) {
+            const float2 s = of_group[fast_div(c + e, p.per_group) - first_group];
+            mean[e] = s.x;
+            mul[e] *= s.y;
+        }
     }
+    template <bool SILU>
+    __device__ __forceinline__ void apply(float *f) const {
+#pragma unroll
+        for (int e = 0; e < VEC; e++) {
+            const float z = fmaf(f[e] - mean[e], mul[e], off[e]);
+            f[e] = SILU ? silu_f(z) : z;
+        }
+    }
+};
+
+template <typename T, int VEC, bool ADD, bool SILU, bool KEEP>
+__global__ __launch_bounds__(kClThreads) void cl_apply_kernel(const T *x, const T *chunk, T *y, const float *gamma,
+                                                              const float *beta, ClParts parts, const float2 *joined,
+                                                              float2 *stats, int8_t *codes, float *scales, float eps, ClPlan p) {
+    extern __shared__ float2 of_group[];
+    __shared__ float red[kClThreads / kWave][3][32];
+    const ClTile t(p, blockIdx.x);
+    const uint32_t c0 = t.col0 * VEC, cc = t.cols * VEC, c = c0 + t.tx * VEC;
     const size_t base = ((size_t)t.b * p.positions + t.row0) * p.channels + c;
-    const uint32_t blocks = (p.channels + kCodeBlock - 1) / kCodeBlock;
-    for (uint32_t row = t.ty; row < t.rows; row += p.ty * kClRows) {
-        Row<T, VEC> r[kClRows];
+    Row<T, VEC> r[kClRows], next[kClRows], add;
+    Affine<VEC> affine;
+    auto request = [&](Row<T, VEC> *to, uint32_t row) {
 #pragma unroll
-        for (uint32_t i = 0; i < kClRows; i++) r[i].load(x + base + (size_t)min(row + i * p.ty, t.rows - 1) * p.channels);
+        for (uint32_t i = 0; i < kClRows; i++) to[i].load(x + base + min(row + i * p.ty, t.rows - 1) * p.channels);
+    };
+    if (t.live) {  // on their way while the slices are joined
+        request(r, t.ty);
+        affine.request(gamma, beta, c);
+        if (ADD) add.load(chunk + (size_t)t.b * p.channels + c);
+    }
+    const ClGroups groups(p, c0, c0 + cc);
+    join_groups<true>(p, parts, joined, VEC, t.b, groups, eps, of_group, red);
+    if (stats != nullptr && t.slice == 0)  // (the chunks of a spread group have the same values)
+        for (uint32_t i = threadIdx.x; i < groups.count; i += blockDim.x) stats[(size_t)t.b * p.groups + groups.first + i] = of_group[i];
+    if (!t.live) return;
+    affine.take(p, of_group, groups.first, c);
+    const uint32_t blocks = (p.channels + kCodeBlock - 1) / kCodeBlock;
+    for (uint32_t row = t.ty; row < t.rows;) {
+        const uint32_t ahead = row + p.ty * kClRows;
+        if (ahead < t.rows) request(next, ahead);
 #pragma unroll
         for (uint32_t i = 0; i < kClRows; i++) {
             const uint32_t at = row + i * p.ty;
-            if (at >= t.rows) break;
-            float f[VEC];
-            r[i].floats(f);
-            add_chunk<T, VEC, ADD>(f, add);
-            if (KEEP) {
-                float most = 0.0f;
-#pragma unroll
-                for (int e = 0; e < VEC; e++) most = fmaxf(most, finite_abs(f[e]));
-                most = team_max<kCodeBlock / VEC>(most);  // (the lanes of a block share a row: tx is a multiple of their number)
-                const float inv = code_inverse(most);
-                uint32_t packed[VEC / 4 + (VEC < 4)];
-#pragma unroll
-                for (int e = 0; e < VEC; e += 4) {
-                    uint32_t w = 0;
-#pragma unroll
-                    for (int k = 0; k < 4 && e + k < VEC; k++) w |= (uint32_t)(code_of(f[e + k], inv) & 255) << (8 * k);
-                    packed[e / 4] = w;
-                }
-                uint32_t *to = reinterpret_cast<uint32_t *>(codes + base + (size_t)at * p.channels);
-                if constexpr (VEC == 8) *reinterpret_cast<uint2 *>(to) = make_uint2(packed[0], packed[1]);
-                else *to = packed[0];
-                if (t.tx % (kCodeBlock / VEC) == 0)
-                    scales[((size_t)t.b * p.positions + t.row0 + at) * blocks + c / kCodeBlock] = code_scale(most);
+            if (at < t.rows) {
+                if (ADD) r[i].add(add);
+                float f[VEC];
+                r[i].floats(f);
+                if constexpr (KEEP)
+                    keep_codes<VEC>(f, codes + base + at * p.channels,
+                                    scales + ((size_t)t.b * p.positions + t.row0 + at) * blocks + c / kCodeBlock,
+                                    t.tx % (kCodeBlock / VEC) == 0);
+                affine.template apply<SILU>(f);
+                Row<T, VEC>::store(y + base + at * p.channels, f);
             }
-#pragma unroll
-            for (int e = 0; e < VEC; e++) {
-                const float z = fmaf(f[e] - mean[e], mul[e], off[e]);
-                f[e] = SILU ? silu_f(z) : z;
-            }
-            Row<T, VEC>::store(y + base + (size_t)at * p.channels, f);
+            r[i] = next[i];
         }
+        row = ahead;
     }
 }
 
-// The 8-bit codes where the lanes of cl_apply_kernel are not whole blocks: 32 lanes per block.
+// The whole of it where a workgroup has all positions of its chunk (whole groups): K rows a lane.
+template <typename T, int VEC, int K, bool KEEP>
+__global__ __launch_bounds__(kClUnitThreads) void cl_unit_kernel(const T *x, const T *chunk, T *y, const float *gamma,
+                                                                 const float *beta, float2 *stats, int8_t *codes, float *scales,
+                                                                 float eps, int silu, ClPlan p) {
+    extern __shared__ float lds[];
+    const ClTile t(p, blockIdx.x);
+    const uint32_t c0 = t.col0 * VEC, cc = t.cols * VEC, c = c0 + t.tx * VEC;
+    const size_t base = (size_t)t.b * p.positions * p.channels + c;
+    Row<T, VEC> r[K], first;
+    Affine<VEC> affine;
+    float s1[VEC], s2[VEC], shift[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; e++) s1[e] = s2[e] = 0.0f;
+    if (t.live) {
+#pragma unroll
+        for (int i = 0; i < K; i++) r[i].load(x + base + min(t.ty + i * p.ty, p.positions - 1) * p.channels);
+        first.load(x + base);
+        affine.request(gamma, beta, c);
+        if (chunk != nullptr) {
+            Row<T, VEC> add;
+            add.load(chunk + (size_t)t.b * p.channels + c);
+            first.add(add);
+#pragma unroll
+            for (int i = 0; i < K; i++) r[i].add(add);
+        }
+        first.floats(shift);
+#pragma unroll
+        for (int i = 0; i < K; i++) {
+            if (t.ty + i * p.ty < p.positions) {
+                float f[VEC];
+                r[i].floats(f);
+                add_moments<VEC>(f, shift, s1, s2);
+            }
+        }
+    }
+    float *first_row = lds + 2 * p.ty * cc;
+    float2 *of_group = reinterpret_cast<float2 *>(first_row + (cc + 1) / 2 * 2);
+    put_channels<VEC>(lds, t, s1);
+    put_channels<VEC>(lds + p.ty * cc, t, s2);
+    if (t.ty == 0) put_channels<VEC>(first_row, t, shift);
+    const ClGroups groups(p, c0, c0 + cc);
+    const float n = (float)p.positions;
+    group_moments(lds, first_row, p.ty, cc, c0, n, p, groups, [&](uint32_t i, float mean, float m2, float channels) {
+        const float2 v = make_float2(mean, 1.0f / sqrtf(m2 / (n * channels) + eps));
+        of_group[i] = v;
+        if (stats != nullptr) stats[(size_t)t.b * p.groups + groups.first + i] = v;
+    });
+    __syncthreads();
+    if (!t.live) return;
+    affine.take(p, of_group, groups.first, c);
+#pragma unroll
+    for (int i = 0; i < K; i++) {
+        const uint32_t at = t.ty + i * p.ty;
+        if (at >= p.positions) break;
+        float f[VEC];
+        r[i].floats(f);
+        if constexpr (KEEP)
+            keep_codes<VEC>(f, codes + base + at * p.channels, scales + ((size_t)t.b * p.positions + at) * (p.channels / kCodeBlock) + c / kCodeBlock,
+                            t.tx % (kCodeBlock / VEC) == 0);
+        if (silu) affine.template apply<true>(f);
+        else affine.template apply<false>(f);
+        Row<T, VEC>::store(y + base + at * p.channels, f);
+    }
+}
+
+// The 8-bit codes where the lanes of the kernels above are not whole blocks: 32 lanes per block.
 template <typename T>
 __global__ __launch_bounds__(256) void cl_codes_kernel(const T *x, const T *chunk, int8_t *codes, float *scales,
                                                        size_t rows, uint32_t positions, uint32_t channels) {
@@ -389,7 +650,7 @@ __global__ __launch_bounds__(256) void cl_codes_kernel(const T *x, const T *chun
 }
 
 // ---------------------------------------------------------------------------
-// Gradient.  What both of its passes read: h from the input, from input and addend, or from the codes.
+// Gradient.  What its passes read: h from the input, from input and addend, or from the codes.
 // ---------------------------------------------------------------------------
 enum { kFromX = 0, kFromXAdd = 1, kFromCodes = 2 };
 
@@ -397,9 +658,10 @@ template <typename T, int VEC, int FROM>
 struct HRow {
     Row<T, VEC> x;
     __device__ __forceinline__ void load(const T *xp, const int8_t *, const float *, size_t at, size_t) { x.load(xp + at); }
-    __device__ __forceinline__ void floats(float *f, const float *add) const {
-        x.floats(f);
-        add_chunk<T, VEC, FROM == kFromXAdd>(f, add);
+    __device__ __forceinline__ void floats(float *f, const Row<T, VEC> &add) const {
+        Row<T, VEC> h = x;
+        if (FROM == kFromXAdd) h.add(add);
+        h.floats(f);
     }
 };
 template <typename T, int VEC>
@@ -408,13 +670,79 @@ struct HRow<T, VEC, kFromCodes> {
     __device__ __forceinline__ void load(const T *, const int8_t *codes, const float *scales, size_t at, size_t scale_at) {
         q.load(codes + at, scales + scale_at);
     }
-    __device__ __forceinline__ void floats(float *f, const float *) const { q.floats(f); }
+    __device__ __forceinline__ void floats(float *f, const Row<T, VEC> &) const { q.floats(f); }
+};
+
+template <typename T, int VEC, int FROM>
+struct GradRow {
+    HRow<T, VEC, FROM> h;
+    Row<T, VEC> dy;
+    __device__ __forceinline__ void load(const T *dyp, const T *x, const int8_t *codes, const float *scales, size_t at, size_t scale_at) {
+        h.load(x, codes, scales, at, scale_at);
+        dy.load(dyp + at);
+    }
+    __device__ __forceinline__ void floats(float *f, float *d, const Row<T, VEC> &add) const {
+        h.floats(f, add);
+        dy.floats(d);
+    }
 };
 
 // d silu(z) / dz = s (1 + z (1 - s))
 __device__ __forceinline__ float silu_slope(float z) {
     const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * z));
     return s * fmaf(z, 1.0f - s, 1.0f);
+}
+
+// A lane's constants: z = (h - mean) mul + off, mul = rstd gamma.  The sums are of dz, dz (h - mean) and h - mean: rstd
+// multiplies the last two when they are whole.
+template <int VEC>
+struct Normal {
+    float mean[VEC], mul[VEC], off[VEC];
+    __device__ __forceinline__ void load(const ClPlan &p, const float2 *stats, const float *gammas, const float *betas, uint32_t b, uint32_t c) {
+#pragma unroll
+        for (int e = 0; e < VEC; e++) {
+            const float2 s = stats[(size_t)b * p.groups + fast_div(c + e, p.per_group)];
+            mean[e] = s.x;
+            mul[e] = s.y * gammas[c + e];
+            off[e] = betas[c + e];
+        }
+    }
+    template <bool SILU>
+    __device__ __forceinline__ void add_sums(const float *h, const float *d, float (*sums)[VEC]) const {
+#pragma unroll
+        for (int e = 0; e < VEC; e++) {
+            const float hc = h[e] - mean[e];
+            const float dz = SILU ? d[e] * silu_slope(fmaf(hc, mul[e], off[e])) : d[e];
+            sums[0][e] += dz;
+            sums[1][e] = fmaf(dz, hc, sums[1][e]);
+            sums[2][e] += hc;
+        }
+    }
+};
+
+// A lane's constants for dx = mul dz - low - (h - mean) slope: mul = rstd gamma, low = rstd m1, slope = rstd^2 m2.
+template <int VEC>
+struct Slope {
+    Normal<VEC> normal;
+    float low[VEC], slope[VEC];
+    __device__ __forceinline__ void set(int e, float rstd, float2 m) {
+        low[e] = rstd * m.x;
+        slope[e] = rstd * rstd * m.y;
+    }
+    template <bool SILU>
+    __device__ __forceinline__ void apply(float *h, const float *d) const {  // h becomes dx
+#pragma unroll
+        for (int e = 0; e < VEC; e++) {
+            const float hc = h[e] - normal.mean[e];
+            const float dz = SILU ? d[e] * silu_slope(fmaf(hc, normal.mul[e], normal.off[e])) : d[e];
+            h[e] = fmaf(normal.mul[e], dz, -low[e]) - hc * slope[e];
+        }
+    }
+};
+
+// dchunk of a channel from its sums: sum_p dx.
+__device__ __forceinline__ float chunk_gradient(float2 stat, float gamma, float positions, float2 m, float s1, float su) {
+    return stat.y * (gamma * s1 - positions * m.x - m.y * su);
 }
 
 // Sums over a slice of positions: per channel S1, S2 and sum_p u (channel_sums [batch][slices][3][channels]), per group
@@ -432,264 +760,427 @@ __global__ __launch_bounds__(kClThreads) void cl_sums_kernel(const T *dy, const 
     for (int e = 0; e < VEC; e++) sums[0][e] = sums[1][e] = sums[2][e] = 0.0f;
     if (t.live) {
         const uint32_t c = c0 + t.tx * VEC;
-        float mean[VEC], rstd[VEC], g[VEC], off[VEC], add[VEC];
-        if (FROM == kFromXAdd) {
-            Row<T, VEC> a;
-            a.load(chunk + (size_t)t.b * p.channels + c);
-            a.floats(add);
-        }
-#pragma unroll
-        for (int e = 0; e < VEC; e++) {
-            const float2 s = stats[(size_t)t.b * p.groups + fast_div(c + e, p.per_group)];
-            mean[e] = s.x;
-            rstd[e] = s.y;
-            g[e] = gamma[c + e];
-            off[e] = beta[c + e];
-        }
+        Row<T, VEC> add;
         const size_t first = (size_t)t.b * p.positions + t.row0, base = first * p.channels + c;
         const uint32_t blocks = (p.channels + kCodeBlock - 1) / kCodeBlock;
-        for (uint32_t row = t.ty; row < t.rows; row += p.ty * kClRows) {
-            HRow<T, VEC, FROM> hr[kClRows];
-            Row<T, VEC> dr[kClRows];
+        GradRow<T, VEC, FROM> r[kClRows], next[kClRows];
+        auto request = [&](GradRow<T, VEC, FROM> *to, uint32_t row) {
 #pragma unroll
             for (uint32_t i = 0; i < kClRows; i++) {
                 const uint32_t at = min(row + i * p.ty, t.rows - 1);
-                hr[i].load(x, codes, scales, base + (size_t)at * p.channels, (first + at) * blocks + c / kCodeBlock);
-                dr[i].load(dy + base + (size_t)at * p.channels);
+                to[i].load(dy, x, codes, scales, base + at * p.channels, (first + at) * blocks + c / kCodeBlock);
             }
+        };
+        request(r, t.ty);
+        if (FROM == kFromXAdd) add.load(chunk + (size_t)t.b * p.channels + c);
+        Normal<VEC> normal;
+        normal.load(p, stats, gamma, beta, t.b, c);
+        for (uint32_t row = t.ty; row < t.rows;) {
+            const uint32_t ahead = row + p.ty * kClRows;
+            if (ahead < t.rows) request(next, ahead);
 #pragma unroll
             for (uint32_t i = 0; i < kClRows; i++) {
                 if (row + i * p.ty < t.rows) {
                     float f[VEC], d[VEC];
-                    hr[i].floats(f, add);
-                    dr[i].floats(d);
-#pragma unroll
-                    for (int e = 0; e < VEC; e++) {
-                        const float u = (f[e] - mean[e]) * rstd[e];
-                        const float dz = SILU ? d[e] * silu_slope(fmaf(u, g[e], off[e])) : d[e];
-                        sums[0][e] += dz;
-                        sums[1][e] = fmaf(dz, u, sums[1][e]);
-                        sums[2][e] += u;
-                    }
+                    r[i].floats(f, d, add);
+                    normal.template add_sums<SILU>(f, d, sums);
                 }
+                r[i] = next[i];
             }
+            row = ahead;
         }
     }
-    float *red = lds, *totals = lds + p.ty * cc;  // totals: gamma S1, gamma S2
-    for (int q = 0; q < 3; q++) {
-        if (q != 0) __syncthreads();
-        put_channels<VEC>(red, t, sums[q]);
-        __syncthreads();
-        for (uint32_t c = threadIdx.x; c < cc; c += blockDim.x) {
-            float a = 0.0f;
-            for (uint32_t j = 0; j < p.ty; j++) a += red[j * cc + c];
-            channel_sums[(((size_t)t.b * p.slices + t.slice) * 3 + q) * p.channels + c0 + c] = a;
-            if (q < 2) totals[q * cc + c] = gamma[c0 + c] * a;
-        }
+    const uint32_t stride = p.ty * cc;
+#pragma unroll
+    for (int q = 0; q < 3; q++) put_channels<VEC>(lds + q * stride, t, sums[q]);
+    add_rows<3>(lds, stride, p.ty, cc);
+    float *to = channel_sums + ((size_t)t.b * p.slices + t.slice) * 3 * p.channels + c0;
+    for (uint32_t c = threadIdx.x; c < cc; c += blockDim.x) {
+        const float g = gamma[c0 + c], rstd = stats[(size_t)t.b * p.groups + fast_div(c0 + c, p.per_group)].y;
+        const float s1 = lds[c], s2 = rstd * lds[stride + c];
+        to[c] = s1;
+        to[p.channels + c] = s2;
+        to[2 * p.channels + c] = rstd * lds[2 * stride + c];
+        lds[c] = g * s1;
+        lds[stride + c] = g * s2;
     }
     __syncthreads();
     const ClGroups groups(p, c0, c0 + cc);
-    const uint32_t team = threadIdx.x / kClTeam, lane = threadIdx.x % kClTeam, teams = blockDim.x / kClTeam;
-    for (uint32_t i = team; i < groups.count; i += teams) {
-        const uint32_t g = groups.first + i;
-        const uint32_t lo = max(g * p.per_group.d, c0) - c0, hi = min((g + 1) * p.per_group.d, c0 + cc) - c0;
-        float a = 0.0f, q = 0.0f;
-        for (uint32_t c = lo + lane; c < hi; c += kClTeam) {
-            a += totals[c];
-            q += totals[cc + c];
+    group_sums(lds, lds + stride, cc, c0, p, groups, [&](uint32_t i, float a, float q) {
+        const uint32_t g = groups.first + i, span = p.spans == 1 ? 0 : t.chunk - g * p.per_group.d / VEC / p.tx;
+        partials[(((size_t)t.b * p.slices + t.slice) * p.spans + span) * p.groups + g] = make_float2(a, q);
+    });
+}
+
+// Gradients of gamma and beta (the first `affine_tiles` blocks of `channel_blocks`) and of the addend (the others: a tile of a
+// sample each) from the channels' sums: 64 channels a block, its wavefronts share the samples and slices.
+struct ClChannelGrads {
+    const float *sums;
+    float *dgamma, *dbeta;
+    void *dchunk;
+    uint32_t affine_tiles, blocks, batch;
+};
+
+template <typename T>
+__device__ __forceinline__ void channel_grads(const ClChannelGrads &a, uint32_t block, const float2 *stats, const float *gamma,
+                                              const ClParts &parts, const float2 *joined, uint32_t vec, const ClPlan &p,
+                                              float (*red)[kClThreads / kWave][kWave]) {
+    constexpr uint32_t kAhead = 8;
+    const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, waves = blockDim.x / kWave;
+    const uint32_t tiles = (p.channels + kWave - 1) / kWave;
+    const bool affine = block < a.affine_tiles;
+    const uint32_t job = affine ? block : block - a.affine_tiles;
+    const uint32_t b = job / tiles, c = (job - b * tiles) * kWave + lane, at_c = min(c, p.channels - 1);
+    const uint32_t count = affine ? a.batch * parts.slices : parts.slices;
+    const float *at = a.sums + (size_t)b * parts.slices * 3 * p.channels + at_c;
+    float s[3] = {0.0f, 0.0f, 0.0f}, m[2] = {0.0f, 0.0f};
+    const uint32_t g = fast_div(at_c, p.per_group);
+    const int other = affine ? 1 : 2;  // S2 for the affine gradients, sum_p u for the addend's
+    for (uint32_t i0 = wave; i0 < count; i0 += waves * kAhead) {
+        float v[2][kAhead];
+#pragma unroll
+        for (uint32_t k = 0; k < kAhead; k++) {
+            const float *from = at + (size_t)min(i0 + k * waves, count - 1) * 3 * p.channels;
+            v[0][k] = from[0];
+            v[1][k] = from[other * p.channels];
         }
-        a = team_sum<kClTeam>(a);
-        q = team_sum<kClTeam>(q);
-        const uint32_t span = t.chunk - g * p.per_group.d / VEC / p.tx;
-        if (lane == 0) partials[(((size_t)t.b * p.slices + t.slice) * p.spans + span) * p.groups + g] = make_float2(a, q);
+#pragma unroll
+        for (uint32_t k = 0; k < kAhead; k++) {
+            if (i0 + k * waves < count) {
+                s[0] += v[0][k];
+                s[1] += v[1][k];
+            }
+        }
     }
+    red[0][wave][lane] = s[0];
+    red[1][wave][lane] = s[1];
+    if (!affine && joined == nullptr && p.spans == 1) {  // the group's means, by the same wavefronts
+        const float2 *from = parts.at + (size_t)b * parts.slices * p.groups + g;
+#pragma unroll 4
+        for (uint32_t i = wave; i < parts.slices; i += waves) {
+            const float2 v = from[(size_t)i * p.groups];
+            m[0] += v.x;
+            m[1] += v.y;
+        }
+        red[2][wave][lane] = m[0];
+        red[3][wave][lane] = m[1];
+    }
+    __syncthreads();
+    if (wave != 0 || c >= p.channels) return;
+    float total[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int q = 0; q < 4; q++)
+        for (uint32_t w = 0; w < waves; w++) total[q] += red[q][w][lane];
+    if (affine) {
+        a.dbeta[c] = total[0];
+        a.dgamma[c] = total[1];
+        return;
+    }
+    const float n = (float)p.positions * (float)p.per_group.d;
+    const float2 means = joined != nullptr ? joined[(size_t)b * p.groups + g]
+                         : p.spans == 1    ? make_float2(total[2] / n, total[3] / n)
+                                           : join_spread_group<false, 1>(p, parts, vec, b, g, 0.0f, 0);
+    Store<T>::store1(static_cast<T *>(a.dchunk) + (size_t)b * p.channels + c,
+                     chunk_gradient(stats[(size_t)b * p.groups + g], gamma[c], (float)p.positions, means, total[0], total[1]));
 }
 
 template <typename T, int VEC, int FROM, bool SILU>
 __global__ __launch_bounds__(kClThreads) void cl_dx_kernel(const T *dy, const T *x, const T *chunk, const int8_t *codes,
                                                            const float *scales, const float2 *stats, const float *gamma,
-                                                           const float *beta, T *dx, const float2 *partials,
-                                                           const float2 *joined, ClPlan p) {
+                                                           const float *beta, T *dx, ClParts parts, const float2 *joined,
+                                                           ClChannelGrads grads, ClPlan p) {
     extern __shared__ float2 of_group[];
-    const ClTile t(p, blockIdx.x);
-    const uint32_t c0 = t.col0 * VEC, cc = t.cols * VEC;
-    const ClGroups groups(p, c0, c0 + cc);
-    const uint32_t team = threadIdx.x / kClTeam, team_lane = threadIdx.x % kClTeam, teams = blockDim.x / kClTeam;
-    for (uint32_t i = team; i < groups.count; i += teams) {
-        const uint32_t g = groups.first + i;
-        const float2 v = joined != nullptr ? joined[(size_t)t.b * p.groups + g]
-                                           : join_sums<kClTeam>(p, VEC, partials, t.b, g, team_lane);
-        if (team_lane == 0) of_group[i] = v;
+    __shared__ float red[4][kClThreads / kWave][kWave];
+    if (blockIdx.x < grads.blocks) {  // (first, so that they run beside the others)
+        channel_grads<T>(grads, blockIdx.x, stats, gamma, parts, joined, VEC, p, red);
+        return;
     }
-    __syncthreads();
-    if (!t.live) return;
-    const uint32_t c = c0 + t.tx * VEC;
-    // dx = mul dz - low - (h - mean) slope, with mul = rstd gamma, low = rstd m1, slope = rstd^2 m2
-    float mean[VEC], mul[VEC], off[VEC], low[VEC], slope[VEC], add[VEC];
-    if (FROM == kFromXAdd) {
-        Row<T, VEC> a;
-        a.load(chunk + (size_t)t.b * p.channels + c);
-        a.floats(add);
-    }
-#pragma unroll
-    for (int e = 0; e < VEC; e++) {
-        const uint32_t g = fast_div(c + e, p.per_group);
-        const float2 s = stats[(size_t)t.b * p.groups + g], m = of_group[g - groups.first];
-        mean[e] = s.x;
-        mul[e] = s.y * gamma[c + e];
-        off[e] = beta[c + e];
-        low[e] = s.y * m.x;
-        slope[e] = s.y * s.y * m.y;
-    }
+    const ClTile t(p, blockIdx.x - grads.blocks);
+    const uint32_t c0 = t.col0 * VEC, cc = t.cols * VEC, c = c0 + t.tx * VEC;
     const size_t first = (size_t)t.b * p.positions + t.row0, base = first * p.channels + c;
     const uint32_t blocks = (p.channels + kCodeBlock - 1) / kCodeBlock;
-    for (uint32_t row = t.ty; row < t.rows; row += p.ty * kClRows) {
-        HRow<T, VEC, FROM> hr[kClRows];
-        Row<T, VEC> dr[kClRows];
+    GradRow<T, VEC, FROM> r[kClRows], next[kClRows];
+    Row<T, VEC> add;
+    auto request = [&](GradRow<T, VEC, FROM> *to, uint32_t row) {
 #pragma unroll
         for (uint32_t i = 0; i < kClRows; i++) {
             const uint32_t at = min(row + i * p.ty, t.rows - 1);
-            hr[i].load(x, codes, scales, base + (size_t)at * p.channels, (first + at) * blocks + c / kCodeBlock);
-            dr[i].load(dy + base + (size_t)at * p.channels);
+            to[i].load(dy, x, codes, scales, base + at * p.channels, (first + at) * blocks + c / kCodeBlock);
         }
+    };
+    Slope<VEC> s;
+    if (t.live) {
+        request(r, t.ty);
+        if (FROM == kFromXAdd) add.load(chunk + (size_t)t.b * p.channels + c);
+        s.normal.load(p, stats, gamma, beta, t.b, c);
+    }
+    const ClGroups groups(p, c0, c0 + cc);
+    join_groups<false>(p, parts, joined, VEC, t.b, groups, 0.0f, of_group, reinterpret_cast<float(*)[3][32]>(&red[0][0][0]));
+    if (!t.live) return;
+#pragma unroll
+    for (int e = 0; e < VEC; e++) {
+        const uint32_t g = fast_div(c + e, p.per_group);
+        s.set(e, stats[(size_t)t.b * p.groups + g].y, of_group[g - groups.first]);
+    }
+    for (uint32_t row = t.ty; row < t.rows;) {
+        const uint32_t ahead = row + p.ty * kClRows;
+        if (ahead < t.rows) request(next, ahead);
 #pragma unroll
         for (uint32_t i = 0; i < kClRows; i++) {
             const uint32_t at = row + i * p.ty;
-            if (at >= t.rows) break;
-            float f[VEC], d[VEC];
-            hr[i].floats(f, add);
-            dr[i].floats(d);
-#pragma unroll
-            for (int e = 0; e < VEC; e++) {
-                const float hc = f[e] - mean[e];
-                const float dz = SILU ? d[e] * silu_slope(fmaf(hc, mul[e], off[e])) : d[e];
-                f[e] = fmaf(mul[e], dz, -low[e]) - hc * slope[e];
+            if (at < t.rows) {
+                float f[VEC], d[VEC];
+                r[i].floats(f, d, add);
+                s.template apply<SILU>(f, d);
+                Row<T, VEC>::store(dx + base + at * p.channels, f);
             }
-            Row<T, VEC>::store(dx + base + (size_t)at * p.channels, f);
+            r[i] = next[i];
         }
+        row = ahead;
     }
 }
 
-// Gradients of gamma and beta (the blocks of tile i < tiles) and of the addend (the others, one tile of one sample each)
-// from the channels' sums: 64 channels a block, its wavefronts share the samples and slices.
-template <typename T>
-__global__ __launch_bounds__(kClThreads) void cl_channel_grads_kernel(const float *channel_sums, const float2 *stats,
-                                                                      const float *gamma, const float2 *partials,
-                                                                      const float2 *joined, float *dgamma, float *dbeta,
-                                                                      T *dchunk, uint32_t affine_tiles, uint32_t vec,
-                                                                      uint32_t batch, ClPlan p) {
-    constexpr uint32_t kWaves = kClThreads / kWave;
-    __shared__ float red[3][kWaves][kWave];
-    const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    const uint32_t tiles = (p.channels + kWave - 1) / kWave;
-    const bool affine = blockIdx.x < affine_tiles;
-    const uint32_t job = affine ? blockIdx.x : blockIdx.x - affine_tiles;
-    const uint32_t c = job % tiles * kWave + lane, b = job / tiles;
-    const uint32_t parts = affine ? batch * p.slices : p.slices;
-    float a[3] = {0.0f, 0.0f, 0.0f};
-    if (c < p.channels) {
-        const float *at = channel_sums + (size_t)b * p.slices * 3 * p.channels + c;
-        for (uint32_t i = wave; i < parts; i += kWaves) {
+// The whole of it where a workgroup has all positions of its chunk (whole groups): K rows a lane.  channel_sums
+// [batch][2][channels]: S1 and S2, for cl_affine_grads_kernel, or, of one sample, dbeta and dgamma themselves (or null).
+template <typename T, int VEC, int K, int FROM>
+__global__ __launch_bounds__(kClUnitThreads) void cl_unit_grads_kernel(const T *dy, const T *x, const T *chunk, const int8_t *codes,
+                                                                       const float *scales, const float2 *stats, const float *gamma,
+                                                                       const float *beta, T *dx, float *s1_to, float *s2_to, T *dchunk,
+                                                                       uint32_t sample_stride, int silu, ClPlan p) {
+    extern __shared__ float lds[];
+    const ClTile t(p, blockIdx.x);
+    const uint32_t c0 = t.col0 * VEC, cc = t.cols * VEC, c = c0 + t.tx * VEC;
+    const size_t first = (size_t)t.b * p.positions, base = first * p.channels + c;
+    const uint32_t blocks = (p.channels + kCodeBlock - 1) / kCodeBlock;
+    GradRow<T, VEC, FROM> r[K];
+    Row<T, VEC> add;
+    Slope<VEC> s;
+    float sums[3][VEC];
 #pragma unroll
-            for (int q = 0; q < 3; q++) a[q] += at[((size_t)i * 3 + q) * p.channels];
+    for (int e = 0; e < VEC; e++) sums[0][e] = sums[1][e] = sums[2][e] = 0.0f;
+    if (t.live) {
+#pragma unroll
+        for (int i = 0; i < K; i++) {
+            const uint32_t at = min(t.ty + i * p.ty, p.positions - 1);
+            r[i].load(dy, x, codes, scales, base + at * p.channels, (first + at) * blocks + c / kCodeBlock);
+        }
+        if (FROM == kFromXAdd) add.load(chunk + (size_t)t.b * p.channels + c);
+        s.normal.load(p, stats, gamma, beta, t.b, c);
+#pragma unroll
+        for (int i = 0; i < K; i++) {
+            if (t.ty + i * p.ty < p.positions) {
+                float f[VEC], d[VEC];
+                r[i].floats(f, d, add);
+                if (silu) s.normal.template add_sums<true>(f, d, sums);
+                else s.normal.template add_sums<false>(f, d, sums);
+            }
         }
     }
+    const uint32_t stride = p.ty * cc;
+    float *weighted = lds + 3 * stride;  // [2][cc]: gamma S1, gamma S2
+    float2 *of_group = reinterpret_cast<float2 *>(weighted + 2 * cc + (stride + cc) % 2);
 #pragma unroll
-    for (int q = 0; q < 3; q++) red[q][wave][lane] = a[q];
+    for (int q = 0; q < 3; q++) put_channels<VEC>(lds + q * stride, t, sums[q]);
+    add_rows<3>(lds, stride, p.ty, cc);
+    for (uint32_t k = threadIdx.x; k < cc; k += blockDim.x) {
+        const float g = gamma[c0 + k], rstd = stats[(size_t)t.b * p.groups + fast_div(c0 + k, p.per_group)].y;
+        const float s1 = lds[k], s2 = rstd * lds[stride + k];
+        lds[2 * stride + k] *= rstd;
+        weighted[k] = g * s1;
+        weighted[cc + k] = g * s2;
+        if (s1_to != nullptr) {
+            s1_to[(size_t)t.b * sample_stride + c0 + k] = s1;
+            s2_to[(size_t)t.b * sample_stride + c0 + k] = s2;
+        }
+    }
     __syncthreads();
-    if (wave != 0 || c >= p.channels) return;
+    const ClGroups groups(p, c0, c0 + cc);
+    const float n = (float)p.positions * (float)p.per_group.d;
+    group_sums(weighted, weighted + cc, cc, c0, p, groups, [&](uint32_t i, float a, float q) { of_group[i] = make_float2(a / n, q / n); });
+    __syncthreads();
+    if (dchunk != nullptr) {
+        for (uint32_t k = threadIdx.x; k < cc; k += blockDim.x) {
+            const uint32_t g = fast_div(c0 + k, p.per_group);
+            Store<T>::store1(dchunk + (size_t)t.b * p.channels + c0 + k,
+                             chunk_gradient(stats[(size_t)t.b * p.groups + g], gamma[c0 + k], (float)p.positions, of_group[g - groups.first],
+                                            lds[k], lds[2 * stride + k]));
+        }
+    }
+    if (!t.live) return;
 #pragma unroll
-    for (int q = 0; q < 3; q++) {
-        a[q] = 0.0f;
-        for (uint32_t w = 0; w < kWaves; w++) a[q] += red[q][w][lane];
+    for (int e = 0; e < VEC; e++) {
+        const uint32_t g = fast_div(c + e, p.per_group);
+        s.set(e, stats[(size_t)t.b * p.groups + g].y, of_group[g - groups.first]);
     }
-    if (affine) {
-        dbeta[c] = a[0];
-        dgamma[c] = a[1];
-        return;
+#pragma unroll
+    for (int i = 0; i < K; i++) {
+        const uint32_t at = t.ty + i * p.ty;
+        if (at >= p.positions) break;
+        float f[VEC], d[VEC];
+        r[i].floats(f, d, add);
+        if (silu) s.template apply<true>(f, d);
+        else s.template apply<false>(f, d);
+        Row<T, VEC>::store(dx + base + at * p.channels, f);
     }
-    const uint32_t g = fast_div(c, p.per_group);
-    const float2 s = stats[(size_t)b * p.groups + g];
-    const float2 m = joined != nullptr ? joined[(size_t)b * p.groups + g] : join_sums<1>(p, vec, partials, b, g, 0);
-    Store<T>::store1(dchunk + (size_t)b * p.channels + c,
-                     s.y * (gamma[c] * a[0] - (float)p.positions * m.x - m.y * a[2]));
+}
+
+// dbeta and dgamma: sums over the samples of S1 and S2 ([batch][2][channels]).
+__global__ __launch_bounds__(kWave) void cl_affine_grads_kernel(const float *sums, float *dgamma, float *dbeta, uint32_t batch,
+                                                                uint32_t channels) {
+    const uint32_t c = blockIdx.x * kWave + threadIdx.x;
+    if (c >= channels) return;
+    float a = 0.0f, q = 0.0f;
+#pragma unroll 8
+    for (uint32_t b = 0; b < batch; b++) {
+        a += sums[(size_t)b * 2 * channels + c];
+        q += sums[((size_t)b * 2 + 1) * channels + c];
+    }
+    dbeta[c] = a;
+    dgamma[c] = q;
 }
 
 // ---- host ----
 constexpr uint64_t kClMaxBlocks = 0x7FFFFFFFull;
+constexpr uint32_t kClSliceElements = 1u << 28;  // of a slice: offsets in it are counted in 32 bits
 
-// Plan of a shape; false where it is beyond what the kernels count in 32 bits.
-bool cl_plan(size_t elt, size_t batch, size_t positions, size_t channels, size_t groups, bool vectors, ClPlan *p, uint32_t *vec) {
-    if (positions > 0x7FFFFFFFull || channels > 0x3FFFFFFFull || batch > 0x7FFFFFFFull || batch * groups > 0x7FFFFFFFull)
+// The shape's own numbers; false where they are beyond what the kernels count in 32 bits.
+bool cl_shape(size_t elt, size_t batch, size_t positions, size_t channels, size_t groups, bool vectors, ClPlan *p, uint32_t *vec) {
+    if (positions > 0x7FFFFFFFull || channels > 0x0FFFFFFFull || batch > 0x7FFFFFFFull || batch * groups > 0x7FFFFFFFull)
         return false;
     const uint32_t epv = (uint32_t)(16 / elt);
     *vec = vectors && channels % epv == 0 ? epv : 1;
-    const uint32_t per_group = (uint32_t)(channels / groups), columns = (uint32_t)(channels / *vec);
+    *p = ClPlan{};
     p->positions = (uint32_t)positions;
     p->channels = (uint32_t)channels;
-    p->columns = columns;
+    p->columns = (uint32_t)(channels / *vec);
     p->groups = (uint32_t)groups;
-    p->per_group = make_fast_div(per_group);
+    p->per_group = make_fast_div((uint32_t)(channels / groups));
+    return true;
+}
+
+void finish_plan(ClPlan *p, uint32_t tx, uint32_t ty, uint32_t slices, uint32_t vec) {
+    p->tx = tx;
+    p->ty = ty;
+    p->chunks = (p->columns + tx - 1) / tx;
+    p->rows = (p->positions + slices - 1) / slices;
+    p->slices = (p->positions + p->rows - 1) / p->rows;
+    const uint64_t chunk_channels = (uint64_t)tx * vec;
+    p->spans = chunk_channels % p->per_group.d == 0 || p->chunks == 1
+                   ? 1 : (uint32_t)std::min<uint64_t>(p->chunks, (p->per_group.d + chunk_channels - 2) / chunk_channels + 1);
+    p->by_tx = make_fast_div(tx);
+    p->by_slices = make_fast_div(p->slices);
+    p->by_chunks = make_fast_div(p->chunks);
+}
+
+// Columns of the smallest chunk of whole groups (and, for codes, of whole blocks).
+uint64_t whole_columns(const ClPlan &p, uint32_t vec, bool blocks) {
+    const uint64_t columns = std::lcm<uint64_t, uint64_t>(p.per_group.d, vec) / vec;
+    return blocks ? std::lcm<uint64_t, uint64_t>(columns, std::max<uint32_t>(1, kCodeBlock / vec)) : columns;
+}
+
+// A workgroup with all positions of some whole groups: K rows a lane; 0 where that is too much for one.
+uint32_t unit_plan(ClPlan *p, uint32_t vec, size_t batch, uint32_t max_k) {
+    const uint64_t whole = whole_columns(*p, vec, false);
+    if (whole > kClUnitThreads || whole * p->positions > kClUnitThreads * max_k) return 0;
+    if ((uint64_t)p->positions * p->channels > kClSliceElements) return 0;
+    uint64_t tx = whole;  // more of them where they are short
+    while (tx * 2 <= p->columns && tx * 2 * p->positions <= 128) tx *= 2;
+    if (batch * ((p->columns + tx - 1) / tx) > kClMaxBlocks) return 0;
+    uint32_t k = 1;
+    while (k * (kClUnitThreads / tx) < p->positions) k *= 2;
+    if (k > max_k) return 0;
+    finish_plan(p, (uint32_t)tx, (p->positions + k - 1) / k, 1, vec);
+    return k;
+}
+
+// (a gradient holds two rows for one: of 8 channels each, no more than two fit the registers)
+uint32_t unit_grads_max_k(uint32_t vec) { return vec == 8 ? 2 : kClUnitMaxK; }
+
+bool slice_plan(ClPlan *p, uint32_t vec, size_t batch) {
     // whole groups and whole code blocks in a chunk where that leaves it short enough, else whole code blocks
-    const uint32_t block_columns = kCodeBlock / *vec;
-    const uint64_t unit = std::lcm<uint64_t, uint64_t>(std::lcm<uint64_t, uint64_t>(per_group, *vec) / *vec, block_columns);
-    const uint32_t n = (columns + kClMaxTx - 1) / kClMaxTx, even = (columns + n - 1) / n;
+    const uint32_t block_columns = kCodeBlock / vec;
+    const uint64_t unit = whole_columns(*p, vec, true);
+    const uint32_t n = (p->columns + kClMaxTx - 1) / kClMaxTx, even = (p->columns + n - 1) / n;
     const uint64_t whole = (even + unit - 1) / unit * unit;
-    p->tx = n == 1 ? columns : whole <= kClThreads ? (uint32_t)whole : (even + block_columns - 1) / block_columns * block_columns;
-    p->chunks = (columns + p->tx - 1) / p->tx;
-    p->by_tx = make_fast_div(p->tx);
-    p->ty = std::max<uint32_t>(1, std::min<uint32_t>(kClThreads / p->tx, p->positions));
-    const uint64_t across = (uint64_t)batch * p->chunks;
-    const uint64_t most = std::max<uint64_t>(1, 1024 / across);
-    const uint64_t wanted = ((uint64_t)positions + (uint64_t)p->ty * kClRows - 1) / ((uint64_t)p->ty * kClRows);
-    const uint64_t slices = std::max<uint64_t>(1, std::min(wanted, most));
-    p->rows = (uint32_t)((positions + slices - 1) / slices);
-    p->slices = (uint32_t)((positions + p->rows - 1) / p->rows);
-    const uint32_t chunk_channels = p->tx * *vec;
-    p->spans = p->chunks == 1 ? 1 : (uint32_t)std::min<uint64_t>(p->chunks, ((uint64_t)per_group + chunk_channels - 2) / chunk_channels + 1);
+    const uint32_t tx = n == 1 ? p->columns : whole <= kClThreads ? (uint32_t)whole : (even + block_columns - 1) / block_columns * block_columns;
+    const uint32_t ty = std::max<uint32_t>(1, std::min<uint32_t>(kClThreads / tx, p->positions));
+    const uint64_t across = (uint64_t)batch * ((p->columns + tx - 1) / tx);
+    const uint64_t most = std::max<uint64_t>(1, kClBlocks / across);
+    const uint64_t wanted = ((uint64_t)p->positions + (uint64_t)ty * kClRows - 1) / ((uint64_t)ty * kClRows);
+    const uint64_t least = ((uint64_t)p->positions * p->channels + kClSliceElements - 1) / kClSliceElements;
+    finish_plan(p, tx, ty, (uint32_t)std::min<uint64_t>(p->positions, std::max({(uint64_t)1, std::min(wanted, most), least * 2})), vec);
     return across * p->slices <= kClMaxBlocks;
 }
 
 size_t partial_floats(const ClPlan &p, size_t batch) { return 2 * batch * p.slices * p.spans * p.groups; }
 size_t joined_floats(const ClPlan &p, size_t batch) { return 2 * batch * p.groups; }
-size_t channel_floats(const ClPlan &p, size_t batch) { return 3 * batch * p.slices * (size_t)p.channels; }
+size_t channel_floats(const ClPlan &p, size_t batch) { return (3 * batch * p.slices * (size_t)p.channels + 1) / 2 * 2; }
 bool joins(const ClPlan &p) { return p.slices * p.spans > kClMaxParts; }
 uint32_t cl_lanes(const ClPlan &p) { return (p.tx * p.ty + kWave - 1) / kWave * kWave; }
+size_t chunk_channels(const ClPlan &p, uint32_t vec) { return (size_t)std::min(p.tx, p.columns) * vec; }
 
-// f(std::bool_constant) of a runtime flag
+// f(std::bool_constant) of a runtime flag, f(std::integral_constant) of a number of rows
 template <typename F>
 void with_flag(bool flag, F f) {
     if (flag) f(std::true_type{});
     else f(std::false_type{});
 }
+template <typename F>
+void with_rows(uint32_t k, F f) {
+    if (k == 1) f(std::integral_constant<int, 1>{});
+    else if (k == 2) f(std::integral_constant<int, 2>{});
+    else f(std::integral_constant<int, 4>{});
+}
+
+template <bool STATS>
+float2 *join_launch(const ClPlan &p, const ClParts &parts, float2 *joined, size_t batch, float eps, uint32_t vec, hipStream_t stream) {
+    launch(cl_join_kernel<STATS>, dim3((uint32_t)(batch * p.groups)), dim3(kClJoinThreads), 0, stream, parts, joined, eps, vec, p);
+    return joined;
+}
 
 template <typename T, int VEC>
-int cl_forward(const ClPlan &p, const ClForward &a, size_t batch, float eps, bool silu, hipStream_t stream) {
+int cl_forward(ClPlan p, const ClForward &a, size_t batch, float eps, bool silu, hipStream_t stream) {
     const T *x = static_cast<const T *>(a.x), *chunk = static_cast<const T *>(a.chunk);
-    float2 *partials = static_cast<float2 *>(a.workspace), *joined = nullptr, *stats = reinterpret_cast<float2 *>(a.stats);
-    const dim3 grid((uint32_t)(batch * p.chunks * p.slices)), block(cl_lanes(p));
-    const size_t cc = (size_t)std::min(p.tx, p.columns) * VEC;
-    with_flag(chunk != nullptr, [&](auto add) {
-        launch(cl_stats_kernel<T, VEC, add.value>, grid, block, (2 * p.ty + 1) * cc * sizeof(float), stream, x, chunk, partials, p);
-    });
-    if (joins(p)) {
-        joined = stats != nullptr ? stats : partials + partial_floats(p, batch) / 2;
-        launch(cl_join_kernel<true>, dim3((uint32_t)(batch * p.groups)), dim3(kWave), 0, stream, partials, joined, eps, VEC, p);
-        stats = nullptr;
-    }
-    const bool keep_here = a.codes != nullptr && VEC > 1 && p.channels % kCodeBlock == 0;
+    T *y = static_cast<T *>(a.y);
+    float2 *stats = reinterpret_cast<float2 *>(a.stats);
+    const uint32_t k = unit_plan(&p, VEC, batch, kClUnitMaxK);
+    if (k == 0 && !slice_plan(&p, VEC, batch)) return MSD_ERR_INVALID_VALUE;
+    const bool keep_here = a.codes != nullptr && VEC > 1 && p.channels % kCodeBlock == 0 && p.tx * VEC % kCodeBlock == 0;
     if (a.codes != nullptr && !keep_here) {
         const size_t rows = batch * p.positions, blocks = rows * ((p.channels + kCodeBlock - 1) / kCodeBlock);
         launch(cl_codes_kernel<T>, dim3((uint32_t)std::min<size_t>(8192, (blocks + 7) / 8)), dim3(256), 0, stream, x, chunk,
                a.codes, a.scales, rows, p.positions, p.channels);
+    }
+    if (k != 0) {
+        const size_t cc = chunk_channels(p, VEC);
+        const size_t lds = (2 * p.ty * cc + (cc + 1) / 2 * 2) * sizeof(float) + std::min<size_t>(p.groups, cc) * sizeof(float2);
+        with_rows(k, [&](auto rows) {
+            with_flag(keep_here, [&](auto keep) {
+                if constexpr (VEC > 1 || !keep.value)
+                    launch(cl_unit_kernel<T, VEC, rows.value, keep.value>, dim3((uint32_t)(batch * p.chunks)), dim3(cl_lanes(p)), lds, stream,
+                           x, chunk, y, a.gamma, a.beta, stats, a.codes, a.scales, eps, silu, p);
+            });
+        });
+        return launch_status();
+    }
+    float2 *partials = static_cast<float2 *>(a.workspace), *joined = nullptr;
+    const ClParts parts = {partials, p.slices, p.rows};
+    const dim3 grid((uint32_t)(batch * p.chunks * p.slices)), block(cl_lanes(p));
+    const size_t cc = chunk_channels(p, VEC);
+    with_flag(chunk != nullptr, [&](auto add) {
+        launch(cl_stats_kernel<T, VEC, add.value>, grid, block, (2 * p.ty + 1) * cc * sizeof(float), stream, x, chunk, partials, p);
+    });
+    if (joins(p)) {
+        joined = join_launch<true>(p, parts, stats != nullptr ? stats : partials + partial_floats(p, batch) / 2, batch, eps, VEC, stream);
+        stats = nullptr;
     }
     with_flag(chunk != nullptr, [&](auto add) {
         with_flag(silu, [&](auto act) {
             with_flag(keep_here, [&](auto keep) {
                 if constexpr (VEC > 1 || !keep.value)
                     launch(cl_apply_kernel<T, VEC, add.value, act.value, keep.value>, grid, block,
-                           std::min<size_t>(p.groups, cc) * sizeof(float2), stream, x, chunk, static_cast<T *>(a.y), a.gamma, a.beta,
-                           partials, joined, stats, a.codes, a.scales, eps, p);
+                           std::min<size_t>(p.groups, cc) * sizeof(float2), stream, x, chunk, y, a.gamma, a.beta, parts, joined, stats,
+                           a.codes, a.scales, eps, p);
             });
         });
     });
@@ -697,38 +1188,51 @@ int cl_forward(const ClPlan &p, const ClForward &a, size_t batch, float eps, boo
 }
 
 template <typename T, int VEC, int FROM>
-void cl_backward_from(const ClPlan &p, const ClBackward &a, size_t batch, bool silu, hipStream_t stream) {
+int cl_backward_from(ClPlan p, const ClBackward &a, size_t batch, bool silu, hipStream_t stream) {
     const T *dy = static_cast<const T *>(a.dy), *x = static_cast<const T *>(a.x), *chunk = static_cast<const T *>(a.chunk);
+    T *dx = static_cast<T *>(a.dx), *dchunk = static_cast<T *>(a.dchunk);
     const float2 *stats = reinterpret_cast<const float2 *>(a.stats);
     float *channel_sums = static_cast<float *>(a.workspace);
-    float2 *partials = reinterpret_cast<float2 *>(channel_sums + (channel_floats(p, batch) + 1) / 2 * 2), *joined = nullptr;
+    const uint32_t tiles = (p.channels + kWave - 1) / kWave;
+    if (const uint32_t k = unit_plan(&p, VEC, batch, unit_grads_max_k(VEC))) {
+        const size_t cc = chunk_channels(p, VEC);
+        const size_t lds = (3 * p.ty * cc + 2 * cc + 1) * sizeof(float) + std::min<size_t>(p.groups, cc) * sizeof(float2);
+        const bool affine = a.dgamma != nullptr, one = batch == 1;
+        float *s1 = !affine ? nullptr : one ? a.dbeta : channel_sums, *s2 = !affine ? nullptr : one ? a.dgamma : channel_sums + p.channels;
+        with_rows(k, [&](auto rows) {
+            if constexpr (VEC < 8 || rows.value <= 2)
+                launch(cl_unit_grads_kernel<T, VEC, rows.value, FROM>, dim3((uint32_t)(batch * p.chunks)), dim3(cl_lanes(p)), lds, stream, dy,
+                       x, chunk, a.codes, a.scales, stats, a.gamma, a.beta, dx, s1, s2, dchunk, 2 * p.channels, silu, p);
+        });
+        if (affine && !one)
+            launch(cl_affine_grads_kernel, dim3(tiles), dim3(kWave), 0, stream, channel_sums, a.dgamma, a.dbeta, (uint32_t)batch, p.channels);
+        return launch_status();
+    }
+    if (!slice_plan(&p, VEC, batch)) return MSD_ERR_INVALID_VALUE;
+    float2 *partials = reinterpret_cast<float2 *>(channel_sums + channel_floats(p, batch)), *joined = nullptr;
+    const ClParts parts = {partials, p.slices, p.rows};
     const dim3 grid((uint32_t)(batch * p.chunks * p.slices)), block(cl_lanes(p));
-    const size_t cc = (size_t)std::min(p.tx, p.columns) * VEC;
+    const size_t cc = chunk_channels(p, VEC);
     with_flag(silu, [&](auto act) {
-        launch(cl_sums_kernel<T, VEC, FROM, act.value>, grid, block, (p.ty + 2) * cc * sizeof(float), stream, dy, x, chunk, a.codes,
+        launch(cl_sums_kernel<T, VEC, FROM, act.value>, grid, block, 3 * p.ty * cc * sizeof(float), stream, dy, x, chunk, a.codes,
                a.scales, stats, a.gamma, a.beta, partials, channel_sums, p);
     });
-    if (joins(p)) {
-        joined = partials + partial_floats(p, batch) / 2;
-        launch(cl_join_kernel<false>, dim3((uint32_t)(batch * p.groups)), dim3(kWave), 0, stream, partials, joined, 0.0f, VEC, p);
-    }
+    if (joins(p)) joined = join_launch<false>(p, parts, partials + partial_floats(p, batch) / 2, batch, 0.0f, VEC, stream);
+    const size_t affine = a.dgamma != nullptr ? tiles : 0, added = dchunk != nullptr ? batch * tiles : 0;
+    if (affine + added + grid.x > kClMaxBlocks) return MSD_ERR_INVALID_VALUE;
+    const ClChannelGrads grads = {channel_sums, a.dgamma, a.dbeta, dchunk, (uint32_t)affine, (uint32_t)(affine + added), (uint32_t)batch};
     with_flag(silu, [&](auto act) {
-        launch(cl_dx_kernel<T, VEC, FROM, act.value>, grid, block, std::min<size_t>(p.groups, cc) * sizeof(float2), stream, dy, x,
-               chunk, a.codes, a.scales, stats, a.gamma, a.beta, static_cast<T *>(a.dx), partials, joined, p);
+        launch(cl_dx_kernel<T, VEC, FROM, act.value>, dim3(grid.x + grads.blocks), block, std::min<size_t>(p.groups, cc) * sizeof(float2),
+               stream, dy, x, chunk, a.codes, a.scales, stats, a.gamma, a.beta, dx, parts, joined, grads, p);
     });
-    const uint32_t tiles = (p.channels + kWave - 1) / kWave;
-    const size_t affine = a.dgamma != nullptr ? tiles : 0, added = a.dchunk != nullptr ? batch * tiles : 0;
-    if (affine + added != 0)
-        launch(cl_channel_grads_kernel<T>, dim3((uint32_t)(affine + added)), dim3(kClThreads), 0, stream, channel_sums, stats,
-               a.gamma, partials, joined, a.dgamma, a.dbeta, static_cast<T *>(a.dchunk), (uint32_t)affine, VEC, (uint32_t)batch, p);
+    return launch_status();
 }
 
 template <typename T, int VEC>
 int cl_backward(const ClPlan &p, const ClBackward &a, size_t batch, bool silu, hipStream_t stream) {
-    if (a.codes != nullptr) cl_backward_from<T, VEC, kFromCodes>(p, a, batch, silu, stream);
-    else if (a.chunk != nullptr) cl_backward_from<T, VEC, kFromXAdd>(p, a, batch, silu, stream);
-    else cl_backward_from<T, VEC, kFromX>(p, a, batch, silu, stream);
-    return launch_status();
+    if (a.codes != nullptr) return cl_backward_from<T, VEC, kFromCodes>(p, a, batch, silu, stream);
+    if (a.chunk != nullptr) return cl_backward_from<T, VEC, kFromXAdd>(p, a, batch, silu, stream);
+    return cl_backward_from<T, VEC, kFromX>(p, a, batch, silu, stream);
 }
 
 template <typename T>
@@ -745,14 +1249,17 @@ bool all_aligned16(std::initializer_list<const void *> pointers) {
 }  // namespace
 
 size_t cl_workspace_bytes(size_t elt, size_t batch, size_t positions, size_t channels, size_t groups, bool backward) {
-    size_t most = 0;
+    size_t most = 16;  // (never nothing)
     for (const bool vectors : {false, true}) {  // (what the operands' alignment allows is not known here)
         ClPlan p;
         uint32_t vec;
-        if (!cl_plan(elt, batch, positions, channels, groups, vectors, &p, &vec)) return SIZE_MAX;
-        size_t floats = partial_floats(p, batch) + (joins(p) ? joined_floats(p, batch) : 0);
-        if (backward) floats += (channel_floats(p, batch) + 1) / 2 * 2;
-        most = std::max(most, floats * sizeof(float));
+        if (!cl_shape(elt, batch, positions, channels, groups, vectors, &p, &vec)) return SIZE_MAX;
+        if (unit_plan(&p, vec, batch, backward ? unit_grads_max_k(vec) : kClUnitMaxK) != 0) {
+            if (backward) most = std::max(most, 2 * batch * channels * sizeof(float));
+            continue;
+        }
+        if (!slice_plan(&p, vec, batch)) return SIZE_MAX;
+        most = std::max(most, (partial_floats(p, batch) + (joins(p) ? joined_floats(p, batch) : 0) + (backward ? channel_floats(p, batch) : 0)) * sizeof(float));
     }
     return most;
 }
@@ -764,7 +1271,7 @@ int cl_forward_dispatch(const ClForward &a, size_t batch, size_t positions, size
     ClPlan p;
     uint32_t vec;
     const bool vectors = all_aligned16({a.x, a.chunk, a.y, a.codes});
-    if (!cl_plan(sizeof(T), batch, positions, channels, groups, vectors, &p, &vec)) return MSD_ERR_INVALID_VALUE;
+    if (!cl_shape(sizeof(T), batch, positions, channels, groups, vectors, &p, &vec)) return MSD_ERR_INVALID_VALUE;
     return vec == 1 ? cl_forward<T, 1>(p, a, batch, eps, silu, stream)
                     : cl_forward<T, 16 / sizeof(T)>(p, a, batch, eps, silu, stream);
 }
@@ -776,6 +1283,7 @@ int cl_backward_dispatch(const ClBackward &a, size_t batch, size_t positions, si
                          hipStream_t stream) {
     if (batch == 0 || positions == 0) {  // sums over nothing
         const size_t added = a.dchunk != nullptr ? batch * channels : 0, most = std::max(a.dgamma != nullptr ? channels : 0, added);
+        if ((most + 255) / 256 > kClMaxBlocks) return MSD_ERR_INVALID_VALUE;
         if (most != 0)
             launch(cl_zero_kernel<T>, dim3((uint32_t)((most + 255) / 256)), dim3(256), 0, stream, a.dgamma, a.dbeta,
                    static_cast<T *>(a.dchunk), channels, added);
@@ -784,7 +1292,7 @@ int cl_backward_dispatch(const ClBackward &a, size_t batch, size_t positions, si
     ClPlan p;
     uint32_t vec;
     const bool vectors = all_aligned16({a.dy, a.x, a.chunk, a.codes, a.dx});
-    if (!cl_plan(sizeof(T), batch, positions, channels, groups, vectors, &p, &vec)) return MSD_ERR_INVALID_VALUE;
+    if (!cl_shape(sizeof(T), batch, positions, channels, groups, vectors, &p, &vec)) return MSD_ERR_INVALID_VALUE;
     return vec == 1 ? cl_backward<T, 1>(p, a, batch, silu, stream) : cl_backward<T, 16 / sizeof(T)>(p, a, batch, silu, stream);
 }
 template int cl_backward_dispatch<float>(const ClBackward &, size_t, size_t, size_t, size_t, bool, hipStream_t);
