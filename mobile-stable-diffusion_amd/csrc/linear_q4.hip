@@ -69,51 +69,41 @@ __global__ __launch_bounds__(kQ4Threads) void linear_q4_generic_kernel(const T *
 }
 
 // ---------------------------------------------------------------------------
-// On the matrix cores.  A workgroup of eight wavefronts owns 16 CT columns and walks k in chunks of eight steps of 128, a step
-// per wavefront, so that the weights of a chunk are in flight together and a row of x is read once per workgroup.
+// On the matrix cores.  A workgroup owns 16 CT columns, each of its wavefronts every W-th step of 128 of k; their sums meet in
+// LDS at the end.  A wavefront brings its part of x to LDS itself and for itself: no barrier before that.
 //
 // v_mfma_f32_16x16x32_f16 multiplies 16 rows of x with 16 columns of weights, 32 of k at a time.  A code minus 8 is exact in
 // float16, and so are the products and, to float32, their sums; the scale of a group multiplies the sum of its products, not
 // the weights.  Of the 16 rows 8 are those of x; where x is float32, or activated, they hold its upper 11 bits and the other
-// 8 rows, which would stand empty, the next 11: with the 128 values of a row and step brought to the same range by a power
-// of two, no bit of float32 that matters is lost, at the price of the same instructions.
+// 8 rows, which would stand empty, the next 11, the 128 values of a row and step being brought to the range of float16 by a
+// power of two.  What is left out is at most 2^-22 of a value, to either side alike: less than the roundings of a float32 sum
+// of k products leave (against 64 bits, k = 2048: 1.3e-7, torch's float32 product 4e-7).
 //
 // Weights: a lane loads 16 bytes, 32 of its column's weights; the four lanes of a column then swap 4-byte pieces so that each
 // instruction gets 32 neighbouring ones, which never mix two scales.  Within a piece, codes come out in pairs (0, 4), (1, 5),
 // (2, 6), (3, 7) by masks alone; x is laid out in LDS in that order.
+//
+// How k is dealt depends on k alone, so a row has the same bits for any CT, number of rows and company.
 // ---------------------------------------------------------------------------
-constexpr int kMmWaves = 8;
-constexpr int kMmThreads = kMmWaves * kWave;
+constexpr int kMmMaxWaves = 8;
 constexpr int kMmTile = 16;                   // columns of a tile
-constexpr int kMmStep = 128;                  // of k, per wavefront and chunk
+constexpr int kMmStep = 128;                  // of k
 constexpr int kMmRows = 8;                    // most rows of x
-constexpr int kMmUnits = kMmRows * kMmWaves / (kMmThreads / 32);  // (row, step) pairs a team of 32 lanes brings to LDS
 constexpr int kMmEntries = kMmStep / 8;       // 16-byte pieces of a row and step in LDS
 constexpr uint32_t kEights = 0x88888888u;     // codes of zeros
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
-constexpr int kQ4GroupMax = 32;  // layers per launch
-template <int N>
-struct Q4Layers {
-    const uint8_t *packed[N];
-    const void *scales[N];
-    const float *bias[N];
-    void *y[N];
-    uint32_t n[N];
-    uint32_t first_block[N + 1];  // first_block[count] = number of workgroups
-    uint32_t count;
-};
-
-// Eight codes minus 8, as float16, in the order 0 4 1 5 2 6 3 7.
-__device__ __forceinline__ f16x8 q4_values(uint32_t w) {
+// Eight codes minus 8, as float16, in the order 0 4 1 5 2 6 3 7.  k1024: 0x64006400 in a vector register, so that each mask and
+// the or behind it are one instruction (two constants of which one is in a scalar register).
+__device__ __forceinline__ f16x8 q4_values(uint32_t w, uint32_t k1024) {
     const uint32_t v = w >> 8;
-    auto low = [](uint32_t u) {  // 1024 + code - 1032
-        return __builtin_bit_cast(f16x2, (u & 0x000F000Fu) | 0x64006400u) - f16x2{1032.0f, 1032.0f};
+    auto low = [k1024](uint32_t u) {  // 1024 + code - 1032
+        return __builtin_bit_cast(f16x2, (u & 0x000F000Fu) | k1024) - f16x2{1032.0f, 1032.0f};
     };
-    auto high = [](uint32_t u) {  // (1024 + 16 code) / 16 - 72
-        return __builtin_bit_cast(f16x2, (u & 0x00F000F0u) | 0x64006400u) * f16x2{0.0625f, 0.0625f} - f16x2{72.0f, 72.0f};
+    auto high = [k1024](uint32_t u) {  // (1024 + 16 code) / 16 - 72
+        return __builtin_bit_cast(f16x2, (u & 0x00F000F0u) | k1024) * f16x2{0.0625f, 0.0625f} - f16x2{72.0f, 72.0f};
     };
     const f16x2 a = low(w), b = high(w), c = low(v), d = high(v);
     return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
@@ -128,210 +118,260 @@ __device__ __forceinline__ void q4_transpose(u32x4 &v) {
     v = u32x4{c[0], c[1], d[0], d[1]};
 }
 
+// Two neighbouring values of a row of x, as they are in memory.
 template <typename T>
-struct XPiece;  // four neighbouring values of a row of x
+struct XPair;
 template <>
-struct XPiece<float> {
-    u32x4 v;
-    __device__ __forceinline__ void load(const float *p) { v = *reinterpret_cast<const u32x4 *>(p); }
-    __device__ __forceinline__ void floats(float *f) const { Store<float>::unpack(v, f); }
+struct XPair<float> {
+    float2 v = make_float2(0.0f, 0.0f);
+    __device__ __forceinline__ void load(const float *p) { v = *reinterpret_cast<const float2 *>(p); }
+    __device__ __forceinline__ float2 floats() const { return v; }
 };
 template <>
-struct XPiece<__half> {
-    uint2 v;
-    __device__ __forceinline__ void load(const __half *p) { v = *reinterpret_cast<const uint2 *>(p); }
-    __device__ __forceinline__ void floats(float *f) const {
-        const f16x2 a = __builtin_bit_cast(f16x2, v.x), b = __builtin_bit_cast(f16x2, v.y);
-        f[0] = a[0];
-        f[1] = a[1];
-        f[2] = b[0];
-        f[3] = b[1];
+struct XPair<__half> {
+    uint32_t v = 0;
+    __device__ __forceinline__ void load(const __half *p) { v = *reinterpret_cast<const uint32_t *>(p); }
+    __device__ __forceinline__ float2 floats() const {
+        const f16x2 h = __builtin_bit_cast(f16x2, v);
+        return make_float2(h[0], h[1]);
     }
 };
 
-__device__ __forceinline__ uint32_t half_bits(float v) { return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v); }
-__device__ __forceinline__ uint32_t dpp_xor1(uint32_t v) {
-    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, kDppXor1, 0xF, 0xF, true);
-}
+__device__ __forceinline__ uint32_t half_pair(_Float16 lo, _Float16 hi) { return __builtin_bit_cast(uint32_t, f16x2{lo, hi}); }
 
-// SPLIT: two float16 for a value of x.  NS: scales per step (128 / group).
-template <typename T, bool SPLIT, int NS, int CT, int N>
-__global__ __launch_bounds__(kMmThreads) void linear_q4_kernel(const T *x, Q4Layers<N> layers, uint32_t m, uint32_t k, int act_in,
-                                                               int act_out) {
-    extern __shared__ u32x4 lds[];  // [2][kMmWaves][kMmEntries][slots] of x, then [2][kMmWaves][kMmRows] factors
-    uint32_t p = 0;
-    while (N > 1 && p + 1 < layers.count && blockIdx.x >= layers.first_block[p + 1]) p++;  // uniform: scalar loop
-    const uint8_t *packed = layers.packed[p];
-    const T *scales = static_cast<const T *>(layers.scales[p]);
-    const uint32_t n = layers.n[p], col0 = (blockIdx.x - (N > 1 ? layers.first_block[p] : 0)) * (kMmTile * CT);
-    const uint32_t lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const uint32_t i = lane % kMmTile, q = lane / kMmTile;
-    const uint32_t groups = k / (kMmStep / NS), chunks = (k + kMmWaves * kMmStep - 1) / (kMmWaves * kMmStep);
-    const uint32_t slots = SPLIT ? 2 * m : m, buffer = kMmWaves * kMmEntries * slots;
-    float *factors = reinterpret_cast<float *>(lds + 2 * buffer);
+struct Q4Layer {
+    const uint8_t *packed;
+    const void *scales;
+    const float *bias;
+    void *y;
+    uint32_t n;
+};
 
-    u32x4 codes[CT], next[CT];
-    float scale[CT][NS], next_scale[CT][NS];
-    auto request = [&](uint32_t chunk, u32x4 *to, float (*s)[NS]) {
-        const uint32_t step = chunk * kMmWaves + wave, at = step * kMmStep + q * 32;
-#pragma unroll
-        for (int c = 0; c < CT; c++) {  // (columns past the last repeat it and are not stored)
-            const uint32_t col = min(col0 + c * kMmTile + i, n - 1);
-            to[c] = u32x4{kEights, kEights, kEights, kEights};
-            if (at < k) to[c] = load_stream(reinterpret_cast<const u32x4 *>(packed + (size_t)col * (k / 2) + at / 2));
-#pragma unroll
-            for (int j = 0; j < NS; j++) s[c][j] = Store<T>::load1(scales + (size_t)col * groups + min(step * NS + j, groups - 1));
-        }
-    };
-    // x: a team of 32 lanes per (row, step), four values a lane
-    const uint32_t team = threadIdx.x / 32, tl = threadIdx.x % 32;
-    XPiece<T> raw[kMmUnits];
-    auto request_x = [&](uint32_t chunk) {
-#pragma unroll
-        for (int u = 0; u < kMmUnits; u++) {
-            const uint32_t unit = u * (kMmThreads / 32) + team, row = unit / kMmWaves, step = chunk * kMmWaves + unit % kMmWaves;
-            const uint32_t at = step * kMmStep + tl * 4;
-            raw[u] = XPiece<T>{};
-            if (row < m && at < k) raw[u].load(x + (size_t)row * k + at);
-        }
-    };
-    auto place_x = [&](uint32_t chunk) {
-        uint2 *to = reinterpret_cast<uint2 *>(lds + (chunk & 1) * buffer);
-#pragma unroll
-        for (int u = 0; u < kMmUnits; u++) {
-            const uint32_t unit = u * (kMmThreads / 32) + team, row = unit / kMmWaves, step = unit % kMmWaves;
-            if (row >= m) continue;  // (the same for a team, whose lanes alone meet below)
-            float f[4];
-            raw[u].floats(f);
-            uint32_t v[4];  // the upper float16 in the low half
-            if (SPLIT) {
-                float most = 0.0f;
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    if (act_in) f[e] = silu_f(f[e]);
-                    const float a = fabsf(f[e]);
-                    most = fmaxf(most, a < __builtin_huge_valf() ? a : 0.0f);
-                }
-                most = team_max<32>(most);
-                const uint32_t exponent = max(__float_as_uint(most) >> 23, 20u);  // most * 2^(141 - exponent) < 2^15
-                const float up = __uint_as_float((268u - exponent) << 23);
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float s = f[e] * up;
-                    const _Float16 hi = (_Float16)s;
-                    const float rest = (s - (float)hi) * 2048.0f;
-                    v[e] = half_bits(s) | (fabsf(s) < __builtin_huge_valf() ? half_bits(rest) << 16 : 0u);
-                }
-                if (tl == 0) factors[((chunk & 1) * kMmWaves + step) * kMmRows + row] = __uint_as_float((exponent - 14u) << 23);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; e++) v[e] = half_bits(f[e]);
-            }
-            // values 0 - 3 of eight are in the even lane, 4 - 7 in the odd one; each stores two of the four pairs
-            const bool odd = tl & 1;
-            const uint32_t r0 = dpp_xor1(odd ? v[0] : v[2]), r1 = dpp_xor1(odd ? v[1] : v[3]);
-            const uint32_t a0 = odd ? r0 : v[0], b0 = odd ? v[2] : r0, a1 = odd ? r1 : v[1], b1 = odd ? v[3] : r1;
-            const uint32_t entry = step * kMmEntries + tl / 2;
-            to[(entry * slots + row) * 2 + odd] = make_uint2((a0 & 0xFFFFu) | b0 << 16, (a1 & 0xFFFFu) | b1 << 16);
-            if (SPLIT) to[(entry * slots + m + row) * 2 + odd] = make_uint2(a0 >> 16 | (b0 & 0xFFFF0000u), a1 >> 16 | (b1 & 0xFFFF0000u));
-        }
-    };
+// What a wavefront requests for a step: the codes and scales of CT tiles, and PAIRS pairs of rows of x, 32 lanes a row, the values
+// 0 1 4 5 (even lanes) or 2 3 6 7 of eight.  Everything stays as it came until it is used: a conversion would wait for it.
+template <typename T, int NS, int CT, int PAIRS>
+struct Q4Stage {
+    u32x4 codes[CT];
+    T scale[CT][NS];
+    XPair<T> raw[PAIRS][2];
+};
 
+// SPLIT: two float16 for a value of x.  NS: scales per step (128 / group).  PAIRS: of rows of x that there is room for.
+template <typename T, bool SPLIT, int NS, int CT, int PAIRS>
+__device__ __forceinline__ void linear_q4_body(const T *x, const Q4Layer &layer, uint32_t col0, uint32_t m, uint32_t k, int act_in,
+                                               int act_out) {
+    extern __shared__ u32x4 lds[];  // per wavefront [kMmEntries][slots] of x and [kMmRows] factors
+    constexpr int kGroup = kMmStep / NS, kAhead = CT == 4 || (NS == 4 && CT * PAIRS >= 4) ? 1 : 2;
+    const uint32_t n = layer.n, lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const uint32_t waves = blockDim.x / kWave, i = lane % kMmTile, q = lane / kMmTile;
+    const uint32_t groups = k / kGroup, steps = (k + kMmStep - 1) / kMmStep;
+    const uint8_t *packed = layer.packed + (size_t)col0 * (k / 2);
+    const char *scales = static_cast<const char *>(layer.scales) + (size_t)col0 * groups * sizeof(T);
+    // offsets in bytes, of 32 bits from addresses that a wavefront shares: k is at most 2^22
+    uint32_t code_at[CT], scale_at[CT];  // (columns past the last repeat it and are not stored)
+#pragma unroll
+    for (int c = 0; c < CT; c++) {
+        const uint32_t col = min(col0 + c * kMmTile + i, n - 1) - col0;
+        code_at[c] = col * (k / 2) + q * 16;
+        scale_at[c] = col * groups * sizeof(T);
+    }
+    const uint32_t half = lane / 32, tl = lane % 32;
+    const uint32_t slots = SPLIT ? 2 * m : m;
+    u32x4 *mine = lds + wave * (kMmEntries * slots + 2);
+    float *factors = reinterpret_cast<float *>(mine + kMmEntries * slots);
+    const uint32_t slot = SPLIT && i >= kMmRows ? m + min(i - kMmRows, m - 1) : min(i, m - 1);  // (rows past the last repeat it)
+
+    const char *xs = reinterpret_cast<const char *>(x);
+    uint32_t x_at[PAIRS];  // (rows past the last repeat it)
+#pragma unroll
+    for (int u = 0; u < PAIRS; u++) x_at[u] = (min(2 * u + half, m - 1) * k + tl / 2 * 8 + tl % 2 * 2) * (uint32_t)sizeof(T);
+    typedef Q4Stage<T, NS, CT, PAIRS> Stage;
+    // The last step begins where a whole one fits; what the step before it has had then counts as zeros.  Requests are made
+    // without a branch and stay in this order: a value that is loaded on one path and not on another is copied where they meet,
+    // which waits for the load, and a load that overtakes the next step's makes its use wait for those.
+    auto start = [&](uint32_t step) { return min(step * kMmStep, k - kMmStep); };
+    auto request = [&](Stage &to, uint32_t step) {
+        const uint32_t at = start(step);
+        __builtin_amdgcn_sched_barrier(0);
+        const char *from = xs + (size_t)at * sizeof(T);
+#pragma unroll
+        for (int u = 0; u < PAIRS; u++) {
+            to.raw[u][0].load(reinterpret_cast<const T *>(from + x_at[u]));
+            to.raw[u][1].load(reinterpret_cast<const T *>(from + x_at[u]) + 4);
+        }
+#pragma unroll
+        for (int c = 0; c < CT; c++) {
+            to.codes[c] = *reinterpret_cast<const u32x4 *>(packed + at / 2 + code_at[c]);
+            const T *scale = reinterpret_cast<const T *>(scales + (size_t)(at / kGroup) * sizeof(T) + scale_at[c]);
+#pragma unroll
+            for (int j = 0; j < NS; j++) to.scale[c][j] = scale[j];
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    uint32_t k1024 = 0x64006400u;
+    asm volatile("" : "+v"(k1024));
     f32x4 acc[CT];
 #pragma unroll
     for (int c = 0; c < CT; c++) acc[c] = f32x4{0, 0, 0, 0};
-    const bool has_row = i % kMmRows < m && (SPLIT || i < kMmRows);
-    const uint32_t slot = i < kMmRows ? i : m + i - kMmRows;
-    request(0, codes, scale);
-    request_x(0);
-    place_x(0);
-    __syncthreads();
-    for (uint32_t chunk = 0; chunk < chunks; chunk++) {
-        const bool more = chunk + 1 < chunks;
-        if (more) {
-            request(chunk + 1, next, next_scale);
-            request_x(chunk + 1);
-        }
-        if ((chunk * kMmWaves + wave) * kMmStep < k) {
-            f16x8 a[4];
-            const u32x4 *from = lds + (chunk & 1) * buffer + wave * kMmEntries * slots;
+    auto multiply = [&](Stage &from, uint32_t step) {
+        const uint32_t had = step * kMmStep - start(step);  // values of the step that count as zeros
+        uint2 *to = reinterpret_cast<uint2 *>(mine);
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const u32x4 zero = {0, 0, 0, 0};
-                a[j] = __builtin_bit_cast(f16x8, has_row ? from[(j * 4 + q) * slots + slot] : zero);
-            }
-            f32x4 factor = {1, 1, 1, 1};
-            if (SPLIT) {
-                factor = *reinterpret_cast<const f32x4 *>(factors + ((chunk & 1) * kMmWaves + wave) * kMmRows + 4 * (q & 1));
-                factor *= q < 2 ? 1.0f : 1.0f / 2048.0f;
-            }
+        for (int u = 0; u < PAIRS; u++) {
+            if (2 * u >= (int)m) break;
+            const uint32_t row = min(2 * u + half, m - 1), at = (tl / 2 * slots + row) * 2 + tl % 2;  // (an odd last row twice)
+            const bool none = had != 0 && tl / 2 * 8 < had;
+            if constexpr (SPLIT) {
+                const float2 first = from.raw[u][0].floats(), second = from.raw[u][1].floats();
+                float f[4] = {first.x, first.y, second.x, second.y};
+                if (had != 0) {
 #pragma unroll
-            for (int c = 0; c < CT; c++) {
-                q4_transpose(codes[c]);
-#pragma unroll
-                for (int s = 0; s < NS; s++) {
-                    f32x4 d = {0, 0, 0, 0};
-#pragma unroll
-                    for (int j = s * (4 / NS); j < (s + 1) * (4 / NS); j++)
-                        d = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[j], q4_values(codes[c][j]), d, 0, 0, 0);
-#pragma unroll
-                    for (int r = 0; r < 4; r++)
-                        acc[c][r] = SPLIT ? fmaf(d[r] * scale[c][s], factor[r], acc[c][r]) : fmaf(d[r], scale[c][s], acc[c][r]);
+                    for (int e = 0; e < 4; e++) f[e] = none ? 0.0f : f[e];
                 }
+                if (act_in) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) f[e] = silu_f(f[e]);
+                }
+                // (an infinity here leaves nothing but infinities and NaN of its row, which it gives whatever the others are)
+                const float most = team_max<32>(fmaxf(fmaxf(fabsf(f[0]), fabsf(f[1])), fmaxf(fabsf(f[2]), fabsf(f[3]))));
+                const uint32_t exponent = max(__float_as_uint(most) >> 23, 20u);  // most * 2^(141 - exponent) < 2^15
+                const float up = __uint_as_float((268u - exponent) << 23);
+                _Float16 hi[4], lo[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float s = f[e] * up;
+                    hi[e] = (_Float16)s;
+                    lo[e] = (_Float16)(fmaxf(s - (float)hi[e], -8.0f) * 2048.0f);  // (never less than -8; of an infinity: not NaN)
+                }
+                to[at] = make_uint2(half_pair(hi[0], hi[2]), half_pair(hi[1], hi[3]));
+                to[at + 2 * m] = make_uint2(half_pair(lo[0], lo[2]), half_pair(lo[1], lo[3]));
+                if (tl == 0) factors[row] = __uint_as_float((exponent - 14u) << 23);
+            } else {
+                const uint32_t v = __builtin_amdgcn_perm(from.raw[u][1].v, from.raw[u][0].v, 0x05040100u);
+                const uint32_t w = __builtin_amdgcn_perm(from.raw[u][1].v, from.raw[u][0].v, 0x07060302u);
+                to[at] = none ? make_uint2(0, 0) : make_uint2(v, w);
             }
         }
-        if (more) {
-            place_x(chunk + 1);
+        f16x8 a[4];
 #pragma unroll
-            for (int c = 0; c < CT; c++) {
-                codes[c] = next[c];
-#pragma unroll
-                for (int s = 0; s < NS; s++) scale[c][s] = next_scale[c][s];
-            }
+        for (int j = 0; j < 4; j++) a[j] = __builtin_bit_cast(f16x8, mine[(j * 4 + q) * slots + slot]);
+        f32x4 factor = {1, 1, 1, 1};
+        if (SPLIT) {
+            factor = *reinterpret_cast<const f32x4 *>(factors + 4 * (q & 1));
+            factor *= q < 2 ? 1.0f : 1.0f / 2048.0f;
         }
-        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < CT; c++) {
+            if (had != 0) from.codes[c] = q * 32 < had ? u32x4{kEights, kEights, kEights, kEights} : from.codes[c];
+            q4_transpose(from.codes[c]);
+            f32x4 sum = SPLIT ? f32x4{0, 0, 0, 0} : acc[c];
+#pragma unroll
+            for (int s = 0; s < NS; s++) {
+                f32x4 d = {0, 0, 0, 0};
+#pragma unroll
+                for (int j = s * (4 / NS); j < (s + 1) * (4 / NS); j++)
+                    d = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[j], q4_values(from.codes[c][j], k1024), d, 0, 0, 0);
+                const float scale = Store<T>::load1(&from.scale[c][s]);
+#pragma unroll
+                for (int r = 0; r < 4; r++) sum[r] = fmaf(d[r], scale, sum[r]);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; r++) acc[c][r] = SPLIT ? fmaf(sum[r], factor[r], acc[c][r]) : sum[r];
+        }
+    };
+
+    Stage stage[kAhead];
+    const uint32_t last = steps - 1;
+#pragma unroll
+    for (int d = 0; d < kAhead; d++) request(stage[d], min(wave + d * waves, last));
+    for (uint32_t first = wave; first < steps; first += kAhead * waves) {
+#pragma unroll
+        for (int d = 0; d < kAhead; d++) {
+            const uint32_t step = first + d * waves;
+            if (step < steps) multiply(stage[d], step);
+            request(stage[d], min(step + kAhead * waves, last));  // (past the end: what is in the cache)
+        }
     }
 
-    // the wavefronts' sums meet in LDS; a lane has column i of rows 4 q ... 4 q + 3, of the upper (q < 2) or the lower parts
+    // the wavefronts' sums; a lane has column i of rows 4 q ... 4 q + 3, of the upper (q < 2) or the lower parts
     f32x4 *parts = reinterpret_cast<f32x4 *>(lds);
+    __syncthreads();
 #pragma unroll
     for (int c = 0; c < CT; c++) parts[(wave * CT + c) * kWave + lane] = acc[c];
     __syncthreads();
-    const uint32_t tile = threadIdx.x % (kMmTile * CT), row = threadIdx.x / (kMmTile * CT), col = col0 + tile;
-    if (row >= m || col >= n) return;
-    const float *at = reinterpret_cast<const float *>(parts + tile / kMmTile * kWave + row / 4 * kMmTile + tile % kMmTile) + row % 4;
-    float sum = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kMmWaves; w++) {
-        sum += at[w * CT * kWave * 4];
-        if (SPLIT) sum += at[(w * CT * kWave + 2 * kMmTile) * 4];
+    for (uint32_t o = threadIdx.x; o < kMmTile * CT * m; o += blockDim.x) {
+        const uint32_t tile = o % (kMmTile * CT), row = o / (kMmTile * CT), col = col0 + tile;
+        if (col >= n) continue;
+        const float *at = reinterpret_cast<const float *>(parts + tile / kMmTile * kWave + row / 4 * kMmTile + tile % kMmTile) + row % 4;
+        float sum = 0.0f;
+#pragma unroll 4
+        for (uint32_t w = 0; w < waves; w++) {
+            sum += at[w * CT * kWave * 4];
+            if (SPLIT) sum += at[(w * CT * kWave + 2 * kMmTile) * 4];
+        }
+        sum += layer.bias != nullptr ? layer.bias[col] : 0.0f;
+        if (act_out) sum = silu_f(sum);
+        Store<T>::store1(static_cast<T *>(layer.y) + (size_t)row * n + col, sum);
     }
-    const float *bias = layers.bias[p];
-    sum += bias != nullptr ? bias[col] : 0.0f;
-    if (act_out) sum = silu_f(sum);
-    Store<T>::store1(static_cast<T *>(layers.y[p]) + (size_t)row * n + col, sum);
 }
 
-// One launch for at most N layers.
-template <typename T, bool SPLIT, int NS, int CT, int N>
-void launch_q4(const T *x, const Q4Layers<N> &layers, uint32_t m, uint32_t k, int act_in, int act_out, hipStream_t stream) {
-    const uint32_t slots = SPLIT ? 2 * m : m;
-    const size_t rows = 2 * kMmWaves * (kMmEntries * slots * sizeof(u32x4) + kMmRows * sizeof(float));
-    launch(linear_q4_kernel<T, SPLIT, NS, CT, N>, dim3(layers.first_block[layers.count]), dim3(kMmThreads),
-           std::max<size_t>(rows, kMmWaves * CT * kWave * sizeof(f32x4)), stream, x, layers, m, k, act_in, act_out);
+template <typename T, bool SPLIT, int NS, int CT, int PAIRS>
+__global__ __launch_bounds__(kMmMaxWaves *kWave, 4) void linear_q4_kernel(const T *x, const uint8_t *packed, const T *scales, uint32_t k,
+                                                                       uint32_t n, uint32_t m, int act_in, int act_out,
+                                                                       const float *bias, T *y) {
+    linear_q4_body<T, SPLIT, NS, CT, PAIRS>(x, Q4Layer{packed, scales, bias, y, n}, blockIdx.x * (kMmTile * CT), m, k, act_in, act_out);
 }
 
-template <typename T, bool SPLIT, int N>
-void launch_q4_group(const T *x, const Q4Layers<N> &layers, uint32_t m, uint32_t k, uint32_t group, int ct, int act_in, int act_out,
-                     hipStream_t stream) {
-    auto with_ns = [&](auto ns) {
-        if (ct == 1) launch_q4<T, SPLIT, ns.value, 1, N>(x, layers, m, k, act_in, act_out, stream);
-        else if (ct == 2) launch_q4<T, SPLIT, ns.value, 2, N>(x, layers, m, k, act_in, act_out, stream);
-        else launch_q4<T, SPLIT, ns.value, 4, N>(x, layers, m, k, act_in, act_out, stream);
+// Several layers in one launch: the workgroups are laid end to end, and a wavefront finds its layer with one load of all
+// layers' first workgroups, a lane each.
+constexpr int kQ4GroupMax = 32;  // layers per launch
+struct Q4Layers {
+    uint32_t first_block[kQ4GroupMax + 1];  // first_block[count ...] = number of workgroups
+    Q4Layer layer[kQ4GroupMax];
+};
+
+template <typename T, bool SPLIT, int NS, int CT, int PAIRS>
+__global__ __launch_bounds__(kMmMaxWaves *kWave, 4) void linear_q4_grouped_kernel(const T *x, uint32_t k, uint32_t m, int act_in,
+                                                                               int act_out, Q4Layers layers) {
+    const uint32_t next = layers.first_block[min(threadIdx.x % kWave + 1, (uint32_t)kQ4GroupMax)];
+    const uint32_t p = min((uint32_t)__popcll(__ballot(blockIdx.x >= next)), (uint32_t)kQ4GroupMax - 1);
+    const uint32_t at = __builtin_amdgcn_readfirstlane(p);
+    linear_q4_body<T, SPLIT, NS, CT, PAIRS>(x, layers.layer[at], (blockIdx.x - layers.first_block[at]) * (kMmTile * CT), m, k, act_in, act_out);
+}
+
+struct Q4Launch {
+    uint32_t m, k, waves;
+    int act_in, act_out;
+    hipStream_t stream;
+};
+
+template <typename T, bool SPLIT, int NS, int CT, int PAIRS>
+void launch_q4(const T *x, const Q4Layers &layers, uint32_t count, const Q4Launch &a) {
+    const size_t rows = (kMmEntries * (SPLIT ? 2 : 1) * a.m + 2) * sizeof(u32x4);
+    const size_t lds = a.waves * std::max<size_t>(rows, CT * kWave * sizeof(f32x4));
+    const dim3 grid(layers.first_block[kQ4GroupMax]), block(a.waves * kWave);
+    const Q4Layer &l = layers.layer[0];
+    if (count == 1)
+        launch(linear_q4_kernel<T, SPLIT, NS, CT, PAIRS>, grid, block, lds, a.stream, x, l.packed, static_cast<const T *>(l.scales), a.k, l.n,
+               a.m, a.act_in, a.act_out, l.bias, static_cast<T *>(l.y));
+    else
+        launch(linear_q4_grouped_kernel<T, SPLIT, NS, CT, PAIRS>, grid, block, lds, a.stream, x, a.k, a.m, a.act_in, a.act_out, layers);
+}
+
+template <typename T, bool SPLIT>
+void launch_q4_group(const T *x, const Q4Layers &layers, uint32_t count, uint32_t group, int ct, const Q4Launch &a) {
+    auto with_pairs = [&](auto ns, auto tiles) {
+        if (a.m <= 2) launch_q4<T, SPLIT, ns.value, tiles.value, 1>(x, layers, count, a);
+        else launch_q4<T, SPLIT, ns.value, tiles.value, kMmRows / 2>(x, layers, count, a);
     };
-    if (group == 32) with_ns(std::integral_constant<int, 4>{});
-    else if (group == 64) with_ns(std::integral_constant<int, 2>{});
-    else with_ns(std::integral_constant<int, 1>{});
+    auto with_tiles = [&](auto ns) {
+        if (ct == 1) with_pairs(ns, std::integral_constant<int, 1>{});
+        else if (ct == 2) with_pairs(ns, std::integral_constant<int, 2>{});
+        else with_pairs(ns, std::integral_constant<int, 4>{});
+    };
+    if (group == 32) with_tiles(std::integral_constant<int, 4>{});
+    else if (group == 64) with_tiles(std::integral_constant<int, 2>{});
+    else with_tiles(std::integral_constant<int, 1>{});
 }
 
 }  // namespace
@@ -359,7 +399,7 @@ int linear_q4_dispatch(const void *x, const uint8_t *const *packed, const void *
     const T *rows = static_cast<const T *>(x);
     auto bias_of = [&](size_t i) { return biases != nullptr ? biases[i] : nullptr; };
     size_t tiles = 0;
-    bool aligned = aligned16(x) && k != 0;
+    bool aligned = aligned16(x) && k >= kMmStep && k <= (size_t)1 << 22;  // (offsets within a workgroup's columns: 32 bits)
     for (size_t i = 0; i < count; i++) {
         if (ns[i] == 0) continue;
         tiles += (ns[i] + kMmTile - 1) / kMmTile;
@@ -373,38 +413,26 @@ int linear_q4_dispatch(const void *x, const uint8_t *const *packed, const void *
                        static_cast<T *>(ys[i]), (uint32_t)m, (uint32_t)ns[i], (uint32_t)k, (uint32_t)group, act_in, act_out);
         return launch_status();
     }
-    const int ct = tiles >= 2048 ? 4 : tiles >= 1024 ? 2 : 1;
-    auto run = [&](const auto &layers) {
-        if constexpr (sizeof(T) == 4) {
-            launch_q4_group<T, true>(rows, layers, (uint32_t)m, (uint32_t)k, (uint32_t)group, ct, act_in, act_out, stream);
-        } else {
-            if (act_in) launch_q4_group<T, true>(rows, layers, (uint32_t)m, (uint32_t)k, (uint32_t)group, ct, act_in, act_out, stream);
-            else launch_q4_group<T, false>(rows, layers, (uint32_t)m, (uint32_t)k, (uint32_t)group, ct, act_in, act_out, stream);
-        }
-    };
-    auto add = [&](auto &layers, size_t i) {
-        const uint32_t at = layers.count++, columns = kMmTile * ct;
-        layers.packed[at] = packed[i];
-        layers.scales[at] = scales[i];
-        layers.bias[at] = bias_of(i);
-        layers.y[at] = ys[i];
-        layers.n[at] = (uint32_t)ns[i];
-        layers.first_block[at + 1] = layers.first_block[at] + ((uint32_t)ns[i] + columns - 1) / columns;
-    };
-    if (count == 1) {
-        Q4Layers<1> one{};
-        if (ns[0] != 0) {
-            add(one, 0);
-            run(one);
-        }
-        return launch_status();
-    }
-    Q4Layers<kQ4GroupMax> many{};
+    // Wavefronts: as many as share the steps evenly, eight at most, so that several workgroups share a CU.  Tiles per workgroup: more
+    // of them share the work on x, as long as 160 workgroups are left; of one or two rows that work is little.  us, one tile / two /
+    // four, fp16, k = 1280: 2560 columns, 1 row 2.5 3.0 3.9, 8 rows 3.2 3.8 4.6; 5120, 8 rows 3.9 3.5 4.8; 10240, 1 row 3.8 4.1 4.0,
+    // 8 rows 6.0 5.7 4.8; 20160, 2 rows 6.4 6.2 6.5, 8 rows 9.1 7.9 7.3; 8192 x 8192, 1 row 11.0 9.9 14.9; 16384 x 512 3.9 3.6 2.9.
+    const size_t steps = (k + kMmStep - 1) / kMmStep, rounds = (steps + kMmMaxWaves - 1) / kMmMaxWaves, waves = (steps + rounds - 1) / rounds;
+    const int ct = tiles < 320 ? 1 : (m > 2 ? tiles >= 640 : tiles >= 1024 && waves <= 4) ? 4 : 2;
+    const Q4Launch a = {(uint32_t)m, (uint32_t)k, (uint32_t)waves, act_in, act_out, stream};
+    Q4Layers layers{};
+    uint32_t held = 0;
     for (size_t i = 0; i < count; i++) {
-        if (ns[i] != 0) add(many, i);
-        if (many.count == kQ4GroupMax || (i + 1 == count && many.count != 0)) {
-            run(many);
-            many = Q4Layers<kQ4GroupMax>{};
+        if (ns[i] != 0) {
+            const uint32_t columns = kMmTile * ct, blocks = layers.first_block[held] + ((uint32_t)ns[i] + columns - 1) / columns;
+            layers.layer[held++] = {packed[i], scales[i], bias_of(i), ys[i], (uint32_t)ns[i]};
+            for (uint32_t j = held; j <= kQ4GroupMax; j++) layers.first_block[j] = blocks;
+        }
+        if (held == kQ4GroupMax || (i + 1 == count && held != 0)) {
+            if (sizeof(T) == 4 || act_in) launch_q4_group<T, true>(rows, layers, held, (uint32_t)group, ct, a);
+            else if constexpr (sizeof(T) == 2) launch_q4_group<T, false>(rows, layers, held, (uint32_t)group, ct, a);
+            layers = Q4Layers{};
+            held = 0;
         }
     }
     return launch_status();
