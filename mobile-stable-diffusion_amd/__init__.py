@@ -734,7 +734,7 @@ def linear_rows_q4(x, packed, scales, bias=None, act_in=ACT_NONE, act_out=ACT_NO
 
 def linear_rows_q4_grouped(x, packed, scales, biases=None, act_in=ACT_NONE, act_out=ACT_NONE):
     """One launch for several such layers on the same x [m <= 8, k], all with the same group: lists of packed weights, scales and
-    biases (or None) -> list of [m, n_i] tensors."""
+    biases (or None) -> list of [m, n_i] tensors, which share one allocation."""
     done = _native_cl_q4.linear_rows_q4_grouped(x, packed, scales, biases, act_in, act_out)
     if done is not None:
         return done
@@ -748,7 +748,12 @@ def linear_rows_q4_grouped(x, packed, scales, biases=None, act_in=ACT_NONE, act_
     m, k = x.shape
     ns = [_q4_weight(p, s, x, k, group, "layer %d: " % i) for i, (p, s) in enumerate(zip(packed, scales))]
     bp = [_affine(b, n, x, "biases[%d]" % i) if b is not None else None for i, (b, n) in enumerate(zip(biases or [None] * len(ns), ns))]
-    outs = [x.new_empty((m, n)) for n in ns]
+    unit = 256 // x.element_size()
+    whole = x.new_empty(sum(-(-m * n // unit) * unit for n in ns))
+    outs, at = [], 0
+    for n in ns:
+        outs.append(whole[at:at + m * n].view(m, n))
+        at += -(-m * n // unit) * unit
     count = len(ns)
     pointers = ctypes.c_void_p * count
     check(lib.msd_linear_rows_q4_grouped(xp, pointers(*[p.data_ptr() for p in packed]), pointers(*[s.data_ptr() for s in scales]),

@@ -1,7 +1,10 @@
 // C ABI of libmsd_hip.so (declared in include/msd_hip.h): argument checks, dtype
 // dispatch and the per-(device, stream) GroupNorm scratch.
+#include <algorithm>
 #include <cmath>
 #include <initializer_list>
+#include <memory>
+#include <new>
 #include <unordered_map>
 
 #include <hip/hip_fp16.h>
@@ -140,6 +143,38 @@ Tuning g_tuning{};
 }  // namespace msd
 
 using namespace msd;
+
+// Whether the outputs of `count` problems (ns[i] columns of `row_bytes` bytes each) lie apart from each other and from every input:
+// inputs(i, check) calls check(pointer, bytes) for those of problem i.  With the outputs in order, an input can only meet the last
+// one that begins before its end (22 problems: 1 us, every pair 4).
+namespace {
+template <typename F>
+bool outputs_apart(size_t count, void *const *ys, const size_t *ns, size_t row_bytes, F inputs) {
+    typedef std::pair<uintptr_t, uintptr_t> Span;
+    constexpr size_t kHere = 64;
+    Span here[kHere];
+    std::unique_ptr<Span[]> more(count > kHere ? new (std::nothrow) Span[count] : nullptr);
+    Span *spans = count > kHere ? more.get() : here;
+    if (spans == nullptr) return false;
+    size_t n = 0;
+    for (size_t i = 0; i < count; i++)
+        if (ns[i] != 0) spans[n++] = {reinterpret_cast<uintptr_t>(ys[i]), reinterpret_cast<uintptr_t>(ys[i]) + ns[i] * row_bytes};
+    std::sort(spans, spans + n);
+    for (size_t i = 1; i < n; i++)
+        if (spans[i].first < spans[i - 1].second) return false;
+    bool apart = true;
+    for (size_t i = 0; i < count; i++) {
+        if (ns[i] == 0) continue;
+        inputs(i, [&](const void *p, size_t bytes) {
+            const uintptr_t from = reinterpret_cast<uintptr_t>(p);
+            if (p == nullptr || bytes == 0) return;
+            const Span *end = std::lower_bound(spans, spans + n, Span{from + bytes, 0});
+            if (end != spans && end[-1].second > from) apart = false;
+        });
+    }
+    return apart;
+}
+}  // namespace
 
 extern "C" {
 
@@ -701,18 +736,13 @@ int msd_linear_rows_q4_grouped(const void *x, const uint8_t *const *packed, cons
         if (ns[i] == 0) continue;
         if (!ys[i] || (k != 0 && (!x || !packed[i] || !scales[i])) || ns[i] > kQ4MaxExtent) return MSD_ERR_INVALID_VALUE;
     }
-    for (size_t i = 0; i < count && m != 0; i++) {  // as for msd_linear_rows_grouped
-        if (ns[i] == 0) continue;
-        const size_t bytes = m * ns[i] * elt;
-        if (overlaps_any(ys[i], bytes, {{x, m * k * elt}})) return MSD_ERR_INVALID_VALUE;
-        for (size_t j = 0; j < count; j++) {
-            if (ns[j] == 0) continue;
-            if (overlaps_any(ys[i], bytes, {{packed[j], ns[j] * (k / 2)}, {scales[j], ns[j] * (k / group) * elt},
-                                            {biases ? biases[j] : nullptr, ns[j] * sizeof(float)},
-                                            {j != i ? ys[j] : nullptr, m * ns[j] * elt}}))
-                return MSD_ERR_INVALID_VALUE;
-        }
-    }
+    if (m != 0 && !outputs_apart(count, ys, ns, m * elt, [&](size_t i, auto check) {
+            check(x, m * k * elt);
+            check(packed[i], ns[i] * (k / 2));
+            check(scales[i], ns[i] * (k / group) * elt);
+            check(biases ? biases[i] : nullptr, ns[i] * sizeof(float));
+        }))
+        return MSD_ERR_INVALID_VALUE;
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (dtype == MSD_DTYPE_F32)
         return linear_q4_dispatch<float>(x, packed, scales, biases, ys, ns, count, m, k, group, act_in, act_out, s);

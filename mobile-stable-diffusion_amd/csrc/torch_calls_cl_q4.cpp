@@ -239,6 +239,25 @@ PyObject *linear_rows_q4(PyObject *, Args a, Py_ssize_t n) {  // x, packed, scal
     });
 }
 
+// Tensors [m, n] for every n, side by side in one allocation at multiples of 256 bytes (22 allocations of their own: 5 us more).
+std::vector<at::Tensor> parts_of_one(const std::vector<size_t> &ns, int64_t m, const at::Tensor &like) {
+    const int64_t unit = 256 / (int64_t)like.element_size();
+    int64_t total = 0;
+    for (const size_t n : ns) total += (m * (int64_t)n + unit - 1) / unit * unit;
+    const at::Tensor whole = new_tensor({total}, like.scalar_type(), like);
+    std::vector<at::Tensor> parts;
+    parts.reserve(ns.size());
+    int64_t at = 0;
+    for (const size_t n : ns) {
+        auto impl = c10::make_intrusive<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(), whole.dtype());
+        impl->set_sizes_contiguous({m, (int64_t)n});
+        impl->set_storage_offset(at);
+        parts.emplace_back(std::move(impl));
+        at += (m * (int64_t)n + unit - 1) / unit * unit;
+    }
+    return parts;
+}
+
 PyObject *linear_rows_q4_grouped(PyObject *, Args a, Py_ssize_t n) {  // x, packed, scales, biases, act_in, act_out
     return plainly([&]() -> PyObject * {
         Call c(n, 6);
@@ -259,12 +278,9 @@ PyObject *linear_rows_q4_grouped(PyObject *, Args a, Py_ssize_t n) {  // x, pack
             ns[i] = (size_t)cols;
         }
         if (!c.ok) return nullptr;
-        std::vector<Out> outs(count);
+        std::vector<at::Tensor> outs = parts_of_one(ns, r.m, *r.x);
         std::vector<void *> ys(count);
-        for (Py_ssize_t i = 0; i < count; i++) {
-            outs[i].make(new_tensor({r.m, (int64_t)ns[i]}, r.x->scalar_type(), *r.x));
-            ys[i] = outs[i].data;
-        }
+        for (Py_ssize_t i = 0; i < count; i++) ys[i] = outs[i].data_ptr();
         const void *xp = r.x->data_ptr();
         const int rc = on_stream([&](void *s) {
             return abi.msd_linear_rows_q4_grouped(xp, qs.data(), ss.data(), bs.data(), ys.data(), ns.data(), count, r.m, r.k, r.group,
@@ -273,7 +289,7 @@ PyObject *linear_rows_q4_grouped(PyObject *, Args a, Py_ssize_t n) {  // x, pack
         if (failed(rc)) return nullptr;
         PyObject *list = PyList_New(count);
         if (list == nullptr) return nullptr;
-        for (Py_ssize_t i = 0; i < count; i++) PyList_SET_ITEM(list, i, outs[i].result());
+        for (Py_ssize_t i = 0; i < count; i++) PyList_SET_ITEM(list, i, THPVariable_Wrap(std::move(outs[i])));
         return list;
     });
 }
