@@ -28,10 +28,10 @@ namespace msd {
 namespace {
 
 constexpr uint32_t kClThreads = 512;    // most lanes of a workgroup that has a slice of the positions
-constexpr uint32_t kClBlocks = 512;     // workgroups of a launch of slices: two per CU
+constexpr uint32_t kClBlocks = 256;     // workgroups of a launch of slices: one per CU
 constexpr uint32_t kClMaxTx = 320;      // most columns of a workgroup
 constexpr uint32_t kClRows = 2;         // rows a lane uses while as many are on their way
-constexpr uint32_t kClMaxParts = 128;   // slices up to which every workgroup joins their sums itself
+constexpr uint32_t kClMaxParts = 256;   // slices up to which every workgroup joins their sums itself
 constexpr uint32_t kClJoinThreads = 256;
 constexpr uint32_t kClTeam = 16;        // lanes that add up a group's channels
 constexpr uint32_t kClUnitThreads = 1024;
@@ -42,28 +42,53 @@ constexpr float kCodeTiny = 1e-30f;     // blocks below this are kept as zeros (
 struct ClPlan {
     uint32_t positions, channels, columns, groups;
     uint32_t tx, ty, chunks;            // columns and rows of a workgroup; workgroups along the columns
-    uint32_t slices, rows;              // workgroups along the positions, positions of each (but the last)
+    uint32_t slices;                    // workgroups along the positions: each takes every slices-th block of ty of them
     uint32_t spans;                     // most chunks that share one group
     FastDiv per_group, by_tx, by_slices, by_chunks;
 };
 
-// What a workgroup is: sample, slice, chunk and its bounds.
+// What a wavefront needs to ask for its data comes as plain values in front of all else, which arrive in scalar registers with the
+// launch (16 words of them); a plan as a structure is loaded from memory first.
+#define CL_GEOMETRY                                                                                                       \
+    uint32_t positions, uint32_t channels, uint32_t counts, uint32_t mul_tx, uint32_t mul_slices, uint32_t mul_chunks,   \
+        uint32_t shifts, uint32_t ty
+#define CL_TILE(VEC, block) ClTile(block, (VEC), positions, channels, counts, mul_tx, mul_slices, mul_chunks, shifts, ty)
+#define CL_GEOMETRY_OF(p)                                                                                                 \
+    (p).positions, (p).channels, (p).slices | (p).chunks << 16, (p).by_tx.mul, (p).by_slices.mul,               \
+        (p).by_chunks.mul, (p).tx | (p).by_tx.shift << 16 | (p).by_slices.shift << 21 | (p).by_chunks.shift << 26, (p).ty
+constexpr uint32_t kClMaxCount = 0xFFFF;  // slices, chunks
+
+// What a workgroup is: sample, slice, chunk and its bounds; a lane's rows are first, first + step, ... below the positions.
+// Blocks of neighbouring rows go to neighbouring workgroups: with a run of rows each, workgroups a power of two apart would all
+// be at the same memory channels (128 channels at 512 x 512: 3.7 TB/s).
 struct ClTile {
-    uint32_t b, slice, chunk, col0, cols, row0, rows, tx, ty;
+    uint32_t b, slice, chunk, col0, cols, tx, ty, first, step;
     bool live;
-    __device__ ClTile(const ClPlan &p, uint32_t block) {
-        const uint32_t rest = fast_div(block, p.by_slices);
-        slice = block - rest * p.slices;
-        b = fast_div(rest, p.by_chunks);
-        chunk = rest - b * p.chunks;
-        col0 = chunk * p.tx;
-        cols = min(p.tx, p.columns - col0);
-        row0 = slice * p.rows;
-        rows = min(p.rows, p.positions - row0);
-        ty = fast_div(threadIdx.x, p.by_tx);
-        tx = threadIdx.x - ty * p.tx;
-        live = ty < p.ty && tx < cols;
+    __device__ __forceinline__ ClTile(uint32_t block, uint32_t vec, uint32_t positions, uint32_t channels, uint32_t counts, uint32_t mul_tx,
+                                      uint32_t mul_slices, uint32_t mul_chunks, uint32_t shifts, uint32_t rows) {
+        const uint32_t slices = counts & 0xFFFFu, chunks = counts >> 16, width = shifts & 0xFFFFu;
+        const uint32_t rest = fast_div(block, FastDiv{mul_slices, (shifts >> 21) & 31u, 0});
+        slice = block - rest * slices;
+        b = fast_div(rest, FastDiv{mul_chunks, shifts >> 26, 0});
+        chunk = rest - b * chunks;
+        col0 = chunk * width;
+        cols = min(width, channels / vec - col0);
+        ty = fast_div(threadIdx.x, FastDiv{mul_tx, (shifts >> 16) & 31u, 0});
+        tx = threadIdx.x - ty * width;
+        first = slice * rows + ty;
+        step = slices * rows;
+        live = ty < rows && tx < cols;
     }
+};
+// Rows of the slices, which take turns with blocks of ty.
+struct SliceRows {
+    uint32_t whole, rest, ty;
+    __device__ __forceinline__ SliceRows(uint32_t positions, uint32_t slices, uint32_t ty) : ty(ty) {
+        const uint32_t round = slices * ty, rounds = positions / round;
+        whole = rounds * ty;
+        rest = positions - rounds * round;
+    }
+    __device__ __forceinline__ uint32_t of(uint32_t slice) const { return whole + min(rest - min(rest, slice * ty), ty); }
 };
 
 // Groups that have channels in [c0, c1).
@@ -82,7 +107,7 @@ struct Row<T, 16 / sizeof(T)> {
     u32x4 v;
     __device__ __forceinline__ void load(const T *p) { v = *reinterpret_cast<const u32x4 *>(p); }
     __device__ __forceinline__ void floats(float *f) const { Store<T>::unpack(v, f); }
-    static __device__ __forceinline__ void store(T *p, const float *f) { *reinterpret_cast<u32x4 *>(p) = Store<T>::pack(f); }
+    static __device__ __forceinline__ void store(T *p, const float *f) { store_stream(reinterpret_cast<u32x4 *>(p), Store<T>::pack(f)); }
     // the sum, rounded to the storage type (of halves: once, as by way of float32, whose 24 bits are 2 * 11 + 2)
     __device__ __forceinline__ void add(const Row &o) {
 #pragma unroll
@@ -109,21 +134,26 @@ struct Row<T, 1> {
 // The codes of VEC neighbouring channels and their scale.
 template <int VEC>
 struct Codes {
-    int8_t v[VEC];
+    uint32_t w[(VEC + 3) / 4];
     float scale;
     __device__ __forceinline__ void load(const int8_t *p, const float *s) {
         if constexpr (VEC == 8) {
-            *reinterpret_cast<uint2 *>(v) = *reinterpret_cast<const uint2 *>(p);
+            const uint2 v = *reinterpret_cast<const uint2 *>(p);
+            w[0] = v.x;
+            w[1] = v.y;
         } else if constexpr (VEC == 4) {
-            *reinterpret_cast<uint32_t *>(v) = *reinterpret_cast<const uint32_t *>(p);
+            w[0] = *reinterpret_cast<const uint32_t *>(p);
         } else {
-            v[0] = *p;
+            w[0] = *reinterpret_cast<const uint8_t *>(p);
         }
         scale = *s;
     }
     __device__ __forceinline__ void floats(float *f) const {
 #pragma unroll
-        for (int e = 0; e < VEC; e++) f[e] = (float)v[e] * scale;
+        for (int e = 0; e < VEC; e++) {  // (bytes become floats in one instruction: as code + 128)
+            const uint32_t v = w[e / 4] ^ 0x80808080u;
+            f[e] = ((float)((v >> (8 * (e % 4))) & 255u) - 128.0f) * scale;
+        }
     }
 };
 
@@ -143,15 +173,29 @@ template <int VEC>
 __device__ __forceinline__ void keep_codes(const float *f, int8_t *codes, float *scale, bool first) {
     float most = 0.0f;
 #pragma unroll
-    for (int e = 0; e < VEC; e++) most = fmaxf(most, finite_abs(f[e]));
+    for (int e = 0; e < VEC; e++) most = fmaxf(most, fabsf(f[e]));
     most = team_max<kCodeBlock / VEC>(most);
+    const bool infinite = most > 3.402823466e38f;  // (the same for all lanes of the block; NaN are not seen here)
+    if (infinite) {
+        most = 0.0f;
+#pragma unroll
+        for (int e = 0; e < VEC; e++) most = fmaxf(most, finite_abs(f[e]));
+        most = team_max<kCodeBlock / VEC>(most);
+    }
     const float inv = code_inverse(most);
     uint32_t w[VEC / 4];
 #pragma unroll
     for (int e = 0; e < VEC; e += 4) {
-        w[e / 4] = 0;
+        uint32_t c[4];
 #pragma unroll
-        for (int k = 0; k < 4; k++) w[e / 4] |= (uint32_t)(code_of(f[e + k], inv) & 255) << (8 * k);
+        for (int k = 0; k < 4; k++) {
+            // 1.5 * 2^23 leaves the whole part, rounded to even, in the low bits; products of finite values are within +-127
+            float v = f[e + k] * inv;
+            asm volatile("" : "+v"(v));  // (the product is rounded by itself)
+            c[k] = __float_as_uint(v + 12582912.0f);
+            if (infinite || f[e + k] != f[e + k]) c[k] = (uint32_t)code_of(f[e + k], inv);
+        }
+        w[e / 4] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(c[3], c[2], 0x0C0C0400u), __builtin_amdgcn_perm(c[1], c[0], 0x0C0C0400u), 0x05040100u);
     }
     if constexpr (VEC == 8) *reinterpret_cast<uint2 *>(codes) = make_uint2(w[0], w[1]);
     else *reinterpret_cast<uint32_t *>(codes) = w[0];
@@ -291,51 +335,68 @@ __device__ __forceinline__ void add_moments(const float *f, const float *shift, 
 // ---------------------------------------------------------------------------
 // Statistics of a slice of positions: partials [batch][slices][spans][groups], (mean, M2).
 // ---------------------------------------------------------------------------
+// A lane's walk over its rows first, first + step, ... below `rows`, kClRows at a time and as many on their way.  Requests are made
+// without a branch (behind the last row: the last row again, which is in the cache) and stay in order, so that a use waits for
+// its own request and not for the ones behind it.
+template <typename Stage, typename Request, typename Use>
+__device__ __forceinline__ void walk_rows(uint32_t first, uint32_t step, uint32_t rows, Stage (&stage)[2][kClRows], Request request, Use use) {
+    auto requests = [&](Stage *to, uint32_t row) {
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (uint32_t i = 0; i < kClRows; i++) request(to[i], min(row + i * step, rows - 1));
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto uses = [&](Stage *from, uint32_t row) {
+#pragma unroll
+        for (uint32_t i = 0; i < kClRows; i++)
+            if (row + i * step < rows) use(from[i], row + i * step);
+    };
+    const uint32_t ahead = kClRows * step;
+    for (uint32_t row = first; row < rows; row += 2 * ahead) {
+        uses(stage[0], row);
+        requests(stage[0], row + 2 * ahead);
+        uses(stage[1], row + ahead);
+        requests(stage[1], row + 3 * ahead);
+    }
+}
+template <typename Stage, typename Request>
+__device__ __forceinline__ void first_rows(uint32_t first, uint32_t step, uint32_t rows, Stage (&stage)[2][kClRows], Request request) {
+#pragma unroll
+    for (uint32_t i = 0; i < 2 * kClRows; i++) request(stage[i / kClRows][i % kClRows], min(first + i * step, rows - 1));
+    __builtin_amdgcn_sched_barrier(0);
+}
+
 template <typename T, int VEC, bool ADD>
-__global__ __launch_bounds__(kClThreads) void cl_stats_kernel(const T *x, const T *chunk, float2 *partials, ClPlan p) {
+__global__ __launch_bounds__(kClThreads) void cl_stats_kernel(const T *x, const T *chunk, CL_GEOMETRY, float2 *partials, ClPlan p) {
     extern __shared__ float lds[];
-    const ClTile t(p, blockIdx.x);
+    const ClTile t = CL_TILE(VEC, blockIdx.x);
     const uint32_t cc = t.cols * VEC, c0 = t.col0 * VEC;
     float s1[VEC], s2[VEC], shift[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; e++) s1[e] = s2[e] = 0.0f;
     if (t.live) {
         const uint32_t c = c0 + t.tx * VEC;
-        const T *at = x + ((size_t)t.b * p.positions + t.row0) * p.channels + c;
-        Row<T, VEC> r[kClRows], next[kClRows], first, add;
-        auto request = [&](Row<T, VEC> *to, uint32_t row) {
-#pragma unroll
-            for (uint32_t i = 0; i < kClRows; i++) to[i].load(at + min(row + i * p.ty, t.rows - 1) * p.channels);
-        };
-        first.load(at);
-        request(r, t.ty);
-        if (ADD) {
-            add.load(chunk + (size_t)t.b * p.channels + c);
-            first.add(add);
-        }
+        const T *at = x + (size_t)t.b * positions * channels + c;
+        Row<T, VEC> r[2][kClRows], first, add;
+        auto request = [&](Row<T, VEC> &to, uint32_t row) { to.load(at + (size_t)row * channels); };
+        first.load(at + (size_t)(t.slice * ty) * channels);
+        if (ADD) add.load(chunk + (size_t)t.b * channels + c);
+        first_rows(t.first, t.step, positions, r, request);
+        if (ADD) first.add(add);
         first.floats(shift);
-        for (uint32_t row = t.ty; row < t.rows;) {
-            const uint32_t ahead = row + p.ty * kClRows;
-            if (ahead < t.rows) request(next, ahead);
-#pragma unroll
-            for (uint32_t i = 0; i < kClRows; i++) {
-                if (row + i * p.ty < t.rows) {
-                    if (ADD) r[i].add(add);
-                    float f[VEC];
-                    r[i].floats(f);
-                    add_moments<VEC>(f, shift, s1, s2);
-                }
-                r[i] = next[i];
-            }
-            row = ahead;
-        }
+        walk_rows(t.first, t.step, positions, r, request, [&](Row<T, VEC> &row, uint32_t) {
+            if (ADD) row.add(add);
+            float f[VEC];
+            row.floats(f);
+            add_moments<VEC>(f, shift, s1, s2);
+        });
     }
-    float *first_row = lds + 2 * p.ty * cc;
+    float *first_row = lds + 2 * ty * cc;
     put_channels<VEC>(lds, t, s1);
-    put_channels<VEC>(lds + p.ty * cc, t, s2);
+    put_channels<VEC>(lds + ty * cc, t, s2);
     if (t.ty == 0) put_channels<VEC>(first_row, t, shift);
     const ClGroups groups(p, c0, c0 + cc);
-    group_moments(lds, first_row, p.ty, cc, c0, (float)t.rows, p, groups, [&](uint32_t i, float mean, float m2, float) {
+    group_moments(lds, first_row, ty, cc, c0, (float)SliceRows(positions, p.slices, ty).of(t.slice), p, groups, [&](uint32_t i, float mean, float m2, float) {
         const uint32_t g = groups.first + i, span = p.spans == 1 ? 0 : t.chunk - g * p.per_group.d / VEC / p.tx;
         partials[(((size_t)t.b * p.slices + t.slice) * p.spans + span) * p.groups + g] = make_float2(mean, m2);
     });
@@ -346,7 +407,7 @@ __global__ __launch_bounds__(kClThreads) void cl_stats_kernel(const T *x, const 
 // ---------------------------------------------------------------------------
 struct ClParts {  // what a launch of sums left
     const float2 *at;
-    uint32_t slices, rows;
+    uint32_t slices, ty;
 };
 
 // A group's value from the parts of its slices.  Statistics: means by their distance from the first slice's, which costs no
@@ -355,11 +416,25 @@ template <bool STATS>
 struct PartSum {
     const ClPlan &p;
     const ClParts &parts;
+    const SliceRows rows;
     float shift, a = 0.0f, q = 0.0f, r = 0.0f;
-    __device__ PartSum(const ClPlan &p, const ClParts &parts, const float2 *first) : p(p), parts(parts), shift(STATS ? first->x : 0.0f) {}
+    __device__ __forceinline__ PartSum(const ClPlan &p, const ClParts &parts, const float2 *first)
+        : p(p), parts(parts), rows(p.positions, parts.slices, parts.ty), shift(STATS ? first->x : 0.0f) {}
+    // slices s, s + step, ...: twelve requests under way at a time
+    __device__ __forceinline__ void add_all(const float2 *at, uint32_t first, uint32_t step) {
+        constexpr uint32_t kBatch = 12;
+        for (uint32_t s = first; s < parts.slices; s += kBatch * step) {
+            float2 v[kBatch];
+#pragma unroll
+            for (uint32_t k = 0; k < kBatch; k++) v[k] = at[(size_t)min(s + k * step, parts.slices - 1) * p.groups];
+#pragma unroll
+            for (uint32_t k = 0; k < kBatch; k++)
+                if (s + k * step < parts.slices) add(s + k * step, v[k]);
+        }
+    }
     __device__ __forceinline__ void add(uint32_t s, float2 v) {
         if (STATS) {
-            const float w = (float)min(parts.rows, p.positions - s * parts.rows), d = v.x - shift;
+            const float w = (float)rows.of(s), d = v.x - shift;
             a = fmaf(w, d, a);
             r = fmaf(w * d, d, r);
         } else {
@@ -383,8 +458,7 @@ __device__ __forceinline__ void join_whole_groups(const ClPlan &p, const ClParts
     for (uint32_t g0 = 0; g0 < groups.count; g0 += 32) {
         const float2 *at = parts.at + (size_t)b * parts.slices * p.groups + groups.first + min(g0 + lane, groups.count - 1);
         PartSum<STATS> sum(p, parts, at);
-#pragma unroll 4
-        for (uint32_t s = half; s < parts.slices; s += halves) sum.add(s, at[(size_t)s * p.groups]);
+        sum.add_all(at, half, halves);
         sum.a = half_pair_sum(sum.a);
         sum.q = half_pair_sum(sum.q);
         if (STATS) sum.r = half_pair_sum(sum.r);
@@ -420,9 +494,10 @@ __device__ __forceinline__ float2 join_spread_group(const ClPlan &p, const ClPar
     const float2 *at = parts.at + (size_t)b * parts.slices * p.spans * p.groups + g;
     const float total = (float)p.positions * (float)p.per_group.d;
     auto part = [&](uint32_t i) { return at[((size_t)(i / spans) * p.spans + i % spans) * p.groups]; };
+    const SliceRows rows(p.positions, parts.slices, parts.ty);
     auto size = [&](uint32_t i) {
         const uint32_t c0 = (first + i % spans) * chunk_channels, s = i / spans;
-        return (float)min(parts.rows, p.positions - s * parts.rows) * (float)(min(hi, c0 + chunk_channels) - max(lo, c0));
+        return (float)rows.of(s) * (float)(min(hi, c0 + chunk_channels) - max(lo, c0));
     };
     float a = 0.0f, q = 0.0f;
     for (uint32_t i = lane; i < count; i += TEAM) {
@@ -472,8 +547,7 @@ __global__ __launch_bounds__(kClJoinThreads) void cl_join_kernel(ClParts parts, 
     }
     const float2 *at = parts.at + (size_t)b * parts.slices * p.groups + g;
     PartSum<STATS> sum(p, parts, at);
-#pragma unroll 4
-    for (uint32_t s = threadIdx.x; s < parts.slices; s += kClJoinThreads) sum.add(s, at[(size_t)s * p.groups]);
+    sum.add_all(at, threadIdx.x, kClJoinThreads);
     sum.a = block_sum<kClJoinThreads / kWave>(sum.a, red[0]);
     sum.q = block_sum<kClJoinThreads / kWave>(sum.q, red[1]);
     sum.r = block_sum<kClJoinThreads / kWave>(sum.r, red[2]);
@@ -509,29 +583,28 @@ struct Affine {
         for (int e = 0; e < VEC; e++) {
             const float z = fmaf(f[e] - mean[e], mul[e], off[e]);
             f[e] = SILU ? silu_f(z) : z;
+            // float32 first, then the storage type: some instances would round once, and no two give other bits
+            asm volatile("" : "+v"(f[e]));
         }
     }
 };
 
 template <typename T, int VEC, bool ADD, bool SILU, bool KEEP>
-__global__ __launch_bounds__(kClThreads) void cl_apply_kernel(const T *x, const T *chunk, T *y, const float *gamma,
-                                                              const float *beta, ClParts parts, const float2 *joined,
+__global__ __launch_bounds__(kClThreads) void cl_apply_kernel(const T *x, const T *chunk, CL_GEOMETRY, const float *gamma,
+                                                              const float *beta, T *y, ClParts parts, const float2 *joined,
                                                               float2 *stats, int8_t *codes, float *scales, float eps, ClPlan p) {
     extern __shared__ float2 of_group[];
     __shared__ float red[kClThreads / kWave][3][32];
-    const ClTile t(p, blockIdx.x);
+    const ClTile t = CL_TILE(VEC, blockIdx.x);
     const uint32_t c0 = t.col0 * VEC, cc = t.cols * VEC, c = c0 + t.tx * VEC;
-    const size_t base = ((size_t)t.b * p.positions + t.row0) * p.channels + c;
-    Row<T, VEC> r[kClRows], next[kClRows], add;
+    const size_t first = (size_t)t.b * positions, base = first * channels + c;
+    Row<T, VEC> r[2][kClRows], add;
     Affine<VEC> affine;
-    auto request = [&](Row<T, VEC> *to, uint32_t row) {
-#pragma unroll
-        for (uint32_t i = 0; i < kClRows; i++) to[i].load(x + base + min(row + i * p.ty, t.rows - 1) * p.channels);
-    };
+    auto request = [&](Row<T, VEC> &to, uint32_t row) { to.load(x + base + (size_t)row * channels); };
     if (t.live) {  // on their way while the slices are joined
-        request(r, t.ty);
+        if (ADD) add.load(chunk + (size_t)t.b * channels + c);
+        first_rows(t.first, t.step, positions, r, request);
         affine.request(gamma, beta, c);
-        if (ADD) add.load(chunk + (size_t)t.b * p.channels + c);
     }
     const ClGroups groups(p, c0, c0 + cc);
     join_groups<true>(p, parts, joined, VEC, t.b, groups, eps, of_group, red);
@@ -539,39 +612,27 @@ __global__ __launch_bounds__(kClThreads) void cl_apply_kernel(const T *x, const 
         for (uint32_t i = threadIdx.x; i < groups.count; i += blockDim.x) stats[(size_t)t.b * p.groups + groups.first + i] = of_group[i];
     if (!t.live) return;
     affine.take(p, of_group, groups.first, c);
-    const uint32_t blocks = (p.channels + kCodeBlock - 1) / kCodeBlock;
-    for (uint32_t row = t.ty; row < t.rows;) {
-        const uint32_t ahead = row + p.ty * kClRows;
-        if (ahead < t.rows) request(next, ahead);
-#pragma unroll
-        for (uint32_t i = 0; i < kClRows; i++) {
-            const uint32_t at = row + i * p.ty;
-            if (at < t.rows) {
-                if (ADD) r[i].add(add);
-                float f[VEC];
-                r[i].floats(f);
-                if constexpr (KEEP)
-                    keep_codes<VEC>(f, codes + base + at * p.channels,
-                                    scales + ((size_t)t.b * p.positions + t.row0 + at) * blocks + c / kCodeBlock,
-                                    t.tx % (kCodeBlock / VEC) == 0);
-                affine.template apply<SILU>(f);
-                Row<T, VEC>::store(y + base + at * p.channels, f);
-            }
-            r[i] = next[i];
-        }
-        row = ahead;
-    }
+    const uint32_t blocks = (channels + kCodeBlock - 1) / kCodeBlock;
+    walk_rows(t.first, t.step, positions, r, request, [&](Row<T, VEC> &row, uint32_t at) {
+        if (ADD) row.add(add);
+        float f[VEC];
+        row.floats(f);
+        if constexpr (KEEP)
+            keep_codes<VEC>(f, codes + base + (size_t)at * channels, scales + (first + at) * blocks + c / kCodeBlock, t.tx % (kCodeBlock / VEC) == 0);
+        affine.template apply<SILU>(f);
+        Row<T, VEC>::store(y + base + (size_t)at * channels, f);
+    });
 }
 
 // The whole of it where a workgroup has all positions of its chunk (whole groups): K rows a lane.
 template <typename T, int VEC, int K, bool KEEP>
-__global__ __launch_bounds__(kClUnitThreads) void cl_unit_kernel(const T *x, const T *chunk, T *y, const float *gamma,
-                                                                 const float *beta, float2 *stats, int8_t *codes, float *scales,
+__global__ __launch_bounds__(kClUnitThreads) void cl_unit_kernel(const T *x, const T *chunk, CL_GEOMETRY, const float *gamma,
+                                                                 const float *beta, T *y, float2 *stats, int8_t *codes, float *scales,
                                                                  float eps, int silu, ClPlan p) {
     extern __shared__ float lds[];
-    const ClTile t(p, blockIdx.x);
+    const ClTile t = CL_TILE(VEC, blockIdx.x);
     const uint32_t c0 = t.col0 * VEC, cc = t.cols * VEC, c = c0 + t.tx * VEC;
-    const size_t base = (size_t)t.b * p.positions * p.channels + c;
+    const size_t base = (size_t)t.b * positions * channels + c;
     Row<T, VEC> r[K], first;
     Affine<VEC> affine;
     float s1[VEC], s2[VEC], shift[VEC];
@@ -579,35 +640,37 @@ __global__ __launch_bounds__(kClUnitThreads) void cl_unit_kernel(const T *x, con
     for (int e = 0; e < VEC; e++) s1[e] = s2[e] = 0.0f;
     if (t.live) {
 #pragma unroll
-        for (int i = 0; i < K; i++) r[i].load(x + base + min(t.ty + i * p.ty, p.positions - 1) * p.channels);
+        for (int i = 0; i < K; i++) r[i].load(x + base + min(t.ty + i * ty, positions - 1) * channels);
         first.load(x + base);
-        affine.request(gamma, beta, c);
         if (chunk != nullptr) {
             Row<T, VEC> add;
-            add.load(chunk + (size_t)t.b * p.channels + c);
+            add.load(chunk + (size_t)t.b * channels + c);
+            affine.request(gamma, beta, c);
             first.add(add);
 #pragma unroll
             for (int i = 0; i < K; i++) r[i].add(add);
+        } else {
+            affine.request(gamma, beta, c);
         }
         first.floats(shift);
 #pragma unroll
         for (int i = 0; i < K; i++) {
-            if (t.ty + i * p.ty < p.positions) {
+            if (t.ty + i * ty < positions) {
                 float f[VEC];
                 r[i].floats(f);
                 add_moments<VEC>(f, shift, s1, s2);
             }
         }
     }
-    float *first_row = lds + 2 * p.ty * cc;
+    float *first_row = lds + 2 * ty * cc;
     float2 *of_group = reinterpret_cast<float2 *>(first_row + (cc + 1) / 2 * 2);
     put_channels<VEC>(lds, t, s1);
-    put_channels<VEC>(lds + p.ty * cc, t, s2);
+    put_channels<VEC>(lds + ty * cc, t, s2);
     if (t.ty == 0) put_channels<VEC>(first_row, t, shift);
     const ClGroups groups(p, c0, c0 + cc);
-    const float n = (float)p.positions;
-    group_moments(lds, first_row, p.ty, cc, c0, n, p, groups, [&](uint32_t i, float mean, float m2, float channels) {
-        const float2 v = make_float2(mean, 1.0f / sqrtf(m2 / (n * channels) + eps));
+    const float n = (float)positions;
+    group_moments(lds, first_row, ty, cc, c0, n, p, groups, [&](uint32_t i, float mean, float m2, float members) {
+        const float2 v = make_float2(mean, 1.0f / sqrtf(m2 / (n * members) + eps));
         of_group[i] = v;
         if (stats != nullptr) stats[(size_t)t.b * p.groups + groups.first + i] = v;
     });
@@ -616,16 +679,16 @@ __global__ __launch_bounds__(kClUnitThreads) void cl_unit_kernel(const T *x, con
     affine.take(p, of_group, groups.first, c);
 #pragma unroll
     for (int i = 0; i < K; i++) {
-        const uint32_t at = t.ty + i * p.ty;
-        if (at >= p.positions) break;
+        const uint32_t at = t.ty + i * ty;
+        if (at >= positions) break;
         float f[VEC];
         r[i].floats(f);
         if constexpr (KEEP)
-            keep_codes<VEC>(f, codes + base + at * p.channels, scales + ((size_t)t.b * p.positions + at) * (p.channels / kCodeBlock) + c / kCodeBlock,
+            keep_codes<VEC>(f, codes + base + at * channels, scales + ((size_t)t.b * positions + at) * (channels / kCodeBlock) + c / kCodeBlock,
                             t.tx % (kCodeBlock / VEC) == 0);
         if (silu) affine.template apply<true>(f);
         else affine.template apply<false>(f);
-        Row<T, VEC>::store(y + base + at * p.channels, f);
+        Row<T, VEC>::store(y + base + at * channels, f);
     }
 }
 
@@ -654,43 +717,39 @@ __global__ __launch_bounds__(256) void cl_codes_kernel(const T *x, const T *chun
 // ---------------------------------------------------------------------------
 enum { kFromX = 0, kFromXAdd = 1, kFromCodes = 2 };
 
-template <typename T, int VEC, int FROM>
-struct HRow {
-    Row<T, VEC> x;
-    __device__ __forceinline__ void load(const T *xp, const int8_t *, const float *, size_t at, size_t) { x.load(xp + at); }
-    __device__ __forceinline__ void floats(float *f, const Row<T, VEC> &add) const {
-        Row<T, VEC> h = x;
-        if (FROM == kFromXAdd) h.add(add);
-        h.floats(f);
-    }
-};
-template <typename T, int VEC>
-struct HRow<T, VEC, kFromCodes> {
-    Codes<VEC> q;
-    __device__ __forceinline__ void load(const T *, const int8_t *codes, const float *scales, size_t at, size_t scale_at) {
-        q.load(codes + at, scales + scale_at);
-    }
-    __device__ __forceinline__ void floats(float *f, const Row<T, VEC> &) const { q.floats(f); }
-};
-
+// `h` is x or the codes, `more` the addend or the codes' scales.
 template <typename T, int VEC, int FROM>
 struct GradRow {
-    HRow<T, VEC, FROM> h;
-    Row<T, VEC> dy;
-    __device__ __forceinline__ void load(const T *dyp, const T *x, const int8_t *codes, const float *scales, size_t at, size_t scale_at) {
-        h.load(x, codes, scales, at, scale_at);
+    Row<T, VEC> x, dy;
+    __device__ __forceinline__ void load(const T *dyp, const void *h, const void *, size_t at, size_t) {
+        x.load(static_cast<const T *>(h) + at);
         dy.load(dyp + at);
     }
     __device__ __forceinline__ void floats(float *f, float *d, const Row<T, VEC> &add) const {
-        h.floats(f, add);
+        Row<T, VEC> sum = x;
+        if (FROM == kFromXAdd) sum.add(add);
+        sum.floats(f);
+        dy.floats(d);
+    }
+};
+template <typename T, int VEC>
+struct GradRow<T, VEC, kFromCodes> {
+    Codes<VEC> q;
+    Row<T, VEC> dy;
+    __device__ __forceinline__ void load(const T *dyp, const void *h, const void *more, size_t at, size_t scale_at) {
+        q.load(static_cast<const int8_t *>(h) + at, static_cast<const float *>(more) + scale_at);
+        dy.load(dyp + at);
+    }
+    __device__ __forceinline__ void floats(float *f, float *d, const Row<T, VEC> &) const {
+        q.floats(f);
         dy.floats(d);
     }
 };
 
-// d silu(z) / dz = s (1 + z (1 - s))
+// d silu(z) / dz = s + z (s - s^2)
 __device__ __forceinline__ float silu_slope(float z) {
     const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * z));
-    return s * fmaf(z, 1.0f - s, 1.0f);
+    return fmaf(z, fmaf(-s, s, s), s);
 }
 
 // A lane's constants: z = (h - mean) mul + off, mul = rstd gamma.  The sums are of dz, dz (h - mean) and h - mean: rstd
@@ -748,59 +807,44 @@ __device__ __forceinline__ float chunk_gradient(float2 stat, float gamma, float 
 // Sums over a slice of positions: per channel S1, S2 and sum_p u (channel_sums [batch][slices][3][channels]), per group
 // sum gamma dz and sum gamma dz u (partials, as in cl_stats_kernel).
 template <typename T, int VEC, int FROM, bool SILU>
-__global__ __launch_bounds__(kClThreads) void cl_sums_kernel(const T *dy, const T *x, const T *chunk, const int8_t *codes,
-                                                             const float *scales, const float2 *stats, const float *gamma,
-                                                             const float *beta, float2 *partials, float *channel_sums,
-                                                             ClPlan p) {
+__global__ __launch_bounds__(kClThreads) void cl_sums_kernel(const T *dy, const void *h, const void *more, CL_GEOMETRY, const float2 *stats,
+                                                             const float *gamma, const float *beta, float2 *partials,
+                                                             float *channel_sums, ClPlan p) {
     extern __shared__ float lds[];
-    const ClTile t(p, blockIdx.x);
+    const ClTile t = CL_TILE(VEC, blockIdx.x);
     const uint32_t cc = t.cols * VEC, c0 = t.col0 * VEC;
     float sums[3][VEC];
 #pragma unroll
     for (int e = 0; e < VEC; e++) sums[0][e] = sums[1][e] = sums[2][e] = 0.0f;
     if (t.live) {
-        const uint32_t c = c0 + t.tx * VEC;
+        const uint32_t c = c0 + t.tx * VEC, blocks = (channels + kCodeBlock - 1) / kCodeBlock;
+        const size_t first = (size_t)t.b * positions, base = first * channels + c;
         Row<T, VEC> add;
-        const size_t first = (size_t)t.b * p.positions + t.row0, base = first * p.channels + c;
-        const uint32_t blocks = (p.channels + kCodeBlock - 1) / kCodeBlock;
-        GradRow<T, VEC, FROM> r[kClRows], next[kClRows];
-        auto request = [&](GradRow<T, VEC, FROM> *to, uint32_t row) {
-#pragma unroll
-            for (uint32_t i = 0; i < kClRows; i++) {
-                const uint32_t at = min(row + i * p.ty, t.rows - 1);
-                to[i].load(dy, x, codes, scales, base + at * p.channels, (first + at) * blocks + c / kCodeBlock);
-            }
+        GradRow<T, VEC, FROM> r[2][kClRows];
+        auto request = [&](GradRow<T, VEC, FROM> &to, uint32_t row) {
+            to.load(dy, h, more, base + (size_t)row * channels, (first + row) * blocks + c / kCodeBlock);
         };
-        request(r, t.ty);
-        if (FROM == kFromXAdd) add.load(chunk + (size_t)t.b * p.channels + c);
+        if (FROM == kFromXAdd) add.load(static_cast<const T *>(more) + (size_t)t.b * channels + c);
+        first_rows(t.first, t.step, positions, r, request);
         Normal<VEC> normal;
         normal.load(p, stats, gamma, beta, t.b, c);
-        for (uint32_t row = t.ty; row < t.rows;) {
-            const uint32_t ahead = row + p.ty * kClRows;
-            if (ahead < t.rows) request(next, ahead);
-#pragma unroll
-            for (uint32_t i = 0; i < kClRows; i++) {
-                if (row + i * p.ty < t.rows) {
-                    float f[VEC], d[VEC];
-                    r[i].floats(f, d, add);
-                    normal.template add_sums<SILU>(f, d, sums);
-                }
-                r[i] = next[i];
-            }
-            row = ahead;
-        }
+        walk_rows(t.first, t.step, positions, r, request, [&](GradRow<T, VEC, FROM> &row, uint32_t) {
+            float f[VEC], d[VEC];
+            row.floats(f, d, add);
+            normal.template add_sums<SILU>(f, d, sums);
+        });
     }
-    const uint32_t stride = p.ty * cc;
+    const uint32_t stride = ty * cc;
 #pragma unroll
     for (int q = 0; q < 3; q++) put_channels<VEC>(lds + q * stride, t, sums[q]);
-    add_rows<3>(lds, stride, p.ty, cc);
-    float *to = channel_sums + ((size_t)t.b * p.slices + t.slice) * 3 * p.channels + c0;
+    add_rows<3>(lds, stride, ty, cc);
+    float *to = channel_sums + ((size_t)t.b * p.slices + t.slice) * 3 * channels + c0;
     for (uint32_t c = threadIdx.x; c < cc; c += blockDim.x) {
         const float g = gamma[c0 + c], rstd = stats[(size_t)t.b * p.groups + fast_div(c0 + c, p.per_group)].y;
         const float s1 = lds[c], s2 = rstd * lds[stride + c];
         to[c] = s1;
-        to[p.channels + c] = s2;
-        to[2 * p.channels + c] = rstd * lds[2 * stride + c];
+        to[channels + c] = s2;
+        to[2 * channels + c] = rstd * lds[2 * stride + c];
         lds[c] = g * s1;
         lds[stride + c] = g * s2;
     }
@@ -818,7 +862,7 @@ struct ClChannelGrads {
     const float *sums;
     float *dgamma, *dbeta;
     void *dchunk;
-    uint32_t affine_tiles, blocks, batch;
+    uint32_t affine_tiles, batch;
 };
 
 template <typename T>
@@ -885,33 +929,27 @@ __device__ __forceinline__ void channel_grads(const ClChannelGrads &a, uint32_t 
 }
 
 template <typename T, int VEC, int FROM, bool SILU>
-__global__ __launch_bounds__(kClThreads) void cl_dx_kernel(const T *dy, const T *x, const T *chunk, const int8_t *codes,
-                                                           const float *scales, const float2 *stats, const float *gamma,
-                                                           const float *beta, T *dx, ClParts parts, const float2 *joined,
-                                                           ClChannelGrads grads, ClPlan p) {
+__global__ __launch_bounds__(kClThreads) void cl_dx_kernel(const T *dy, const void *h, const void *more, CL_GEOMETRY, uint32_t channel_blocks,
+                                                           const float2 *stats, const float *gamma, const float *beta, T *dx,
+                                                           ClParts parts, const float2 *joined, ClChannelGrads grads, ClPlan p) {
     extern __shared__ float2 of_group[];
     __shared__ float red[4][kClThreads / kWave][kWave];
-    if (blockIdx.x < grads.blocks) {  // (first, so that they run beside the others)
+    if (blockIdx.x < channel_blocks) {  // (first, so that they run beside the others)
         channel_grads<T>(grads, blockIdx.x, stats, gamma, parts, joined, VEC, p, red);
         return;
     }
-    const ClTile t(p, blockIdx.x - grads.blocks);
-    const uint32_t c0 = t.col0 * VEC, cc = t.cols * VEC, c = c0 + t.tx * VEC;
-    const size_t first = (size_t)t.b * p.positions + t.row0, base = first * p.channels + c;
-    const uint32_t blocks = (p.channels + kCodeBlock - 1) / kCodeBlock;
-    GradRow<T, VEC, FROM> r[kClRows], next[kClRows];
+    const ClTile t = CL_TILE(VEC, blockIdx.x - channel_blocks);
+    const uint32_t c0 = t.col0 * VEC, cc = t.cols * VEC, c = c0 + t.tx * VEC, blocks = (channels + kCodeBlock - 1) / kCodeBlock;
+    const size_t first = (size_t)t.b * positions, base = first * channels + c;
+    GradRow<T, VEC, FROM> r[2][kClRows];
     Row<T, VEC> add;
-    auto request = [&](GradRow<T, VEC, FROM> *to, uint32_t row) {
-#pragma unroll
-        for (uint32_t i = 0; i < kClRows; i++) {
-            const uint32_t at = min(row + i * p.ty, t.rows - 1);
-            to[i].load(dy, x, codes, scales, base + at * p.channels, (first + at) * blocks + c / kCodeBlock);
-        }
+    auto request = [&](GradRow<T, VEC, FROM> &to, uint32_t row) {
+        to.load(dy, h, more, base + (size_t)row * channels, (first + row) * blocks + c / kCodeBlock);
     };
     Slope<VEC> s;
     if (t.live) {
-        request(r, t.ty);
-        if (FROM == kFromXAdd) add.load(chunk + (size_t)t.b * p.channels + c);
+        if (FROM == kFromXAdd) add.load(static_cast<const T *>(more) + (size_t)t.b * channels + c);
+        first_rows(t.first, t.step, positions, r, request);
         s.normal.load(p, stats, gamma, beta, t.b, c);
     }
     const ClGroups groups(p, c0, c0 + cc);
@@ -922,36 +960,25 @@ __global__ __launch_bounds__(kClThreads) void cl_dx_kernel(const T *dy, const T 
         const uint32_t g = fast_div(c + e, p.per_group);
         s.set(e, stats[(size_t)t.b * p.groups + g].y, of_group[g - groups.first]);
     }
-    for (uint32_t row = t.ty; row < t.rows;) {
-        const uint32_t ahead = row + p.ty * kClRows;
-        if (ahead < t.rows) request(next, ahead);
-#pragma unroll
-        for (uint32_t i = 0; i < kClRows; i++) {
-            const uint32_t at = row + i * p.ty;
-            if (at < t.rows) {
-                float f[VEC], d[VEC];
-                r[i].floats(f, d, add);
-                s.template apply<SILU>(f, d);
-                Row<T, VEC>::store(dx + base + at * p.channels, f);
-            }
-            r[i] = next[i];
-        }
-        row = ahead;
-    }
+    walk_rows(t.first, t.step, positions, r, request, [&](GradRow<T, VEC, FROM> &row, uint32_t at) {
+        float f[VEC], d[VEC];
+        row.floats(f, d, add);
+        s.template apply<SILU>(f, d);
+        Row<T, VEC>::store(dx + base + (size_t)at * channels, f);
+    });
 }
 
 // The whole of it where a workgroup has all positions of its chunk (whole groups): K rows a lane.  channel_sums
 // [batch][2][channels]: S1 and S2, for cl_affine_grads_kernel, or, of one sample, dbeta and dgamma themselves (or null).
 template <typename T, int VEC, int K, int FROM>
-__global__ __launch_bounds__(kClUnitThreads) void cl_unit_grads_kernel(const T *dy, const T *x, const T *chunk, const int8_t *codes,
-                                                                       const float *scales, const float2 *stats, const float *gamma,
-                                                                       const float *beta, T *dx, float *s1_to, float *s2_to, T *dchunk,
+__global__ __launch_bounds__(kClUnitThreads) void cl_unit_grads_kernel(const T *dy, const void *h, const void *more, CL_GEOMETRY,
+                                                                       const float2 *stats, const float *gamma, const float *beta,
+                                                                       T *dx, float *s1_to, float *s2_to, T *dchunk,
                                                                        uint32_t sample_stride, int silu, ClPlan p) {
     extern __shared__ float lds[];
-    const ClTile t(p, blockIdx.x);
-    const uint32_t c0 = t.col0 * VEC, cc = t.cols * VEC, c = c0 + t.tx * VEC;
-    const size_t first = (size_t)t.b * p.positions, base = first * p.channels + c;
-    const uint32_t blocks = (p.channels + kCodeBlock - 1) / kCodeBlock;
+    const ClTile t = CL_TILE(VEC, blockIdx.x);
+    const uint32_t c0 = t.col0 * VEC, cc = t.cols * VEC, c = c0 + t.tx * VEC, blocks = (channels + kCodeBlock - 1) / kCodeBlock;
+    const size_t first = (size_t)t.b * positions, base = first * channels + c;
     GradRow<T, VEC, FROM> r[K];
     Row<T, VEC> add;
     Slope<VEC> s;
@@ -961,14 +988,14 @@ __global__ __launch_bounds__(kClUnitThreads) void cl_unit_grads_kernel(const T *
     if (t.live) {
 #pragma unroll
         for (int i = 0; i < K; i++) {
-            const uint32_t at = min(t.ty + i * p.ty, p.positions - 1);
-            r[i].load(dy, x, codes, scales, base + at * p.channels, (first + at) * blocks + c / kCodeBlock);
+            const uint32_t at = min(t.ty + i * ty, positions - 1);
+            r[i].load(dy, h, more, base + at * channels, (first + at) * blocks + c / kCodeBlock);
         }
-        if (FROM == kFromXAdd) add.load(chunk + (size_t)t.b * p.channels + c);
+        if (FROM == kFromXAdd) add.load(static_cast<const T *>(more) + (size_t)t.b * channels + c);
         s.normal.load(p, stats, gamma, beta, t.b, c);
 #pragma unroll
         for (int i = 0; i < K; i++) {
-            if (t.ty + i * p.ty < p.positions) {
+            if (t.ty + i * ty < positions) {
                 float f[VEC], d[VEC];
                 r[i].floats(f, d, add);
                 if (silu) s.normal.template add_sums<true>(f, d, sums);
@@ -976,12 +1003,12 @@ __global__ __launch_bounds__(kClUnitThreads) void cl_unit_grads_kernel(const T *
             }
         }
     }
-    const uint32_t stride = p.ty * cc;
+    const uint32_t stride = ty * cc;
     float *weighted = lds + 3 * stride;  // [2][cc]: gamma S1, gamma S2
     float2 *of_group = reinterpret_cast<float2 *>(weighted + 2 * cc + (stride + cc) % 2);
 #pragma unroll
     for (int q = 0; q < 3; q++) put_channels<VEC>(lds + q * stride, t, sums[q]);
-    add_rows<3>(lds, stride, p.ty, cc);
+    add_rows<3>(lds, stride, ty, cc);
     for (uint32_t k = threadIdx.x; k < cc; k += blockDim.x) {
         const float g = gamma[c0 + k], rstd = stats[(size_t)t.b * p.groups + fast_div(c0 + k, p.per_group)].y;
         const float s1 = lds[k], s2 = rstd * lds[stride + k];
@@ -995,14 +1022,14 @@ __global__ __launch_bounds__(kClUnitThreads) void cl_unit_grads_kernel(const T *
     }
     __syncthreads();
     const ClGroups groups(p, c0, c0 + cc);
-    const float n = (float)p.positions * (float)p.per_group.d;
+    const float n = (float)positions * (float)p.per_group.d;
     group_sums(weighted, weighted + cc, cc, c0, p, groups, [&](uint32_t i, float a, float q) { of_group[i] = make_float2(a / n, q / n); });
     __syncthreads();
     if (dchunk != nullptr) {
         for (uint32_t k = threadIdx.x; k < cc; k += blockDim.x) {
             const uint32_t g = fast_div(c0 + k, p.per_group);
-            Store<T>::store1(dchunk + (size_t)t.b * p.channels + c0 + k,
-                             chunk_gradient(stats[(size_t)t.b * p.groups + g], gamma[c0 + k], (float)p.positions, of_group[g - groups.first],
+            Store<T>::store1(dchunk + (size_t)t.b * channels + c0 + k,
+                             chunk_gradient(stats[(size_t)t.b * p.groups + g], gamma[c0 + k], (float)positions, of_group[g - groups.first],
                                             lds[k], lds[2 * stride + k]));
         }
     }
@@ -1014,13 +1041,13 @@ __global__ __launch_bounds__(kClUnitThreads) void cl_unit_grads_kernel(const T *
     }
 #pragma unroll
     for (int i = 0; i < K; i++) {
-        const uint32_t at = t.ty + i * p.ty;
-        if (at >= p.positions) break;
+        const uint32_t at = t.ty + i * ty;
+        if (at >= positions) break;
         float f[VEC], d[VEC];
         r[i].floats(f, d, add);
         if (silu) s.template apply<true>(f, d);
         else s.template apply<false>(f, d);
-        Row<T, VEC>::store(dx + base + at * p.channels, f);
+        Row<T, VEC>::store(dx + base + at * channels, f);
     }
 }
 
@@ -1041,11 +1068,12 @@ __global__ __launch_bounds__(kWave) void cl_affine_grads_kernel(const float *sum
 
 // ---- host ----
 constexpr uint64_t kClMaxBlocks = 0x7FFFFFFFull;
-constexpr uint32_t kClSliceElements = 1u << 28;  // of a slice: offsets in it are counted in 32 bits
+constexpr size_t kClMaxChannels = (size_t)1 << 22;
+constexpr uint64_t kClUnitElements = 1u << 28;  // of a sample that workgroups have whole: offsets in it are counted in 32 bits
 
 // The shape's own numbers; false where they are beyond what the kernels count in 32 bits.
 bool cl_shape(size_t elt, size_t batch, size_t positions, size_t channels, size_t groups, bool vectors, ClPlan *p, uint32_t *vec) {
-    if (positions > 0x7FFFFFFFull || channels > 0x0FFFFFFFull || batch > 0x7FFFFFFFull || batch * groups > 0x7FFFFFFFull)
+    if (positions > 0x7FFFFFFFull || channels > kClMaxChannels || batch > 0x7FFFFFFFull || batch * groups > 0x7FFFFFFFull)
         return false;
     const uint32_t epv = (uint32_t)(16 / elt);
     *vec = vectors && channels % epv == 0 ? epv : 1;
@@ -1062,8 +1090,7 @@ void finish_plan(ClPlan *p, uint32_t tx, uint32_t ty, uint32_t slices, uint32_t 
     p->tx = tx;
     p->ty = ty;
     p->chunks = (p->columns + tx - 1) / tx;
-    p->rows = (p->positions + slices - 1) / slices;
-    p->slices = (p->positions + p->rows - 1) / p->rows;
+    p->slices = std::min(slices, (p->positions + ty - 1) / ty);  // (each has a row)
     const uint64_t chunk_channels = (uint64_t)tx * vec;
     p->spans = chunk_channels % p->per_group.d == 0 || p->chunks == 1
                    ? 1 : (uint32_t)std::min<uint64_t>(p->chunks, (p->per_group.d + chunk_channels - 2) / chunk_channels + 1);
@@ -1082,10 +1109,11 @@ uint64_t whole_columns(const ClPlan &p, uint32_t vec, bool blocks) {
 uint32_t unit_plan(ClPlan *p, uint32_t vec, size_t batch, uint32_t max_k) {
     const uint64_t whole = whole_columns(*p, vec, false);
     if (whole > kClUnitThreads || whole * p->positions > kClUnitThreads * max_k) return 0;
-    if ((uint64_t)p->positions * p->channels > kClSliceElements) return 0;
+    if ((uint64_t)p->positions * p->channels > kClUnitElements) return 0;
     uint64_t tx = whole;  // more of them where they are short
     while (tx * 2 <= p->columns && tx * 2 * p->positions <= 128) tx *= 2;
-    if (batch * ((p->columns + tx - 1) / tx) > kClMaxBlocks) return 0;
+    const uint64_t chunks = (p->columns + tx - 1) / tx;
+    if (chunks > kClMaxCount || batch * chunks > kClMaxBlocks) return 0;
     uint32_t k = 1;
     while (k * (kClUnitThreads / tx) < p->positions) k *= 2;
     if (k > max_k) return 0;
@@ -1107,9 +1135,8 @@ bool slice_plan(ClPlan *p, uint32_t vec, size_t batch) {
     const uint64_t across = (uint64_t)batch * ((p->columns + tx - 1) / tx);
     const uint64_t most = std::max<uint64_t>(1, kClBlocks / across);
     const uint64_t wanted = ((uint64_t)p->positions + (uint64_t)ty * kClRows - 1) / ((uint64_t)ty * kClRows);
-    const uint64_t least = ((uint64_t)p->positions * p->channels + kClSliceElements - 1) / kClSliceElements;
-    finish_plan(p, tx, ty, (uint32_t)std::min<uint64_t>(p->positions, std::max({(uint64_t)1, std::min(wanted, most), least * 2})), vec);
-    return across * p->slices <= kClMaxBlocks;
+    finish_plan(p, tx, ty, (uint32_t)std::min(wanted, most), vec);
+    return p->slices <= kClMaxCount && p->chunks <= kClMaxCount && across * p->slices <= kClMaxBlocks;
 }
 
 size_t partial_floats(const ClPlan &p, size_t batch) { return 2 * batch * p.slices * p.spans * p.groups; }
@@ -1158,17 +1185,18 @@ int cl_forward(ClPlan p, const ClForward &a, size_t batch, float eps, bool silu,
             with_flag(keep_here, [&](auto keep) {
                 if constexpr (VEC > 1 || !keep.value)
                     launch(cl_unit_kernel<T, VEC, rows.value, keep.value>, dim3((uint32_t)(batch * p.chunks)), dim3(cl_lanes(p)), lds, stream,
-                           x, chunk, y, a.gamma, a.beta, stats, a.codes, a.scales, eps, silu, p);
+                           x, chunk, CL_GEOMETRY_OF(p), a.gamma, a.beta, y, stats, a.codes, a.scales, eps, silu, p);
             });
         });
         return launch_status();
     }
     float2 *partials = static_cast<float2 *>(a.workspace), *joined = nullptr;
-    const ClParts parts = {partials, p.slices, p.rows};
+    const ClParts parts = {partials, p.slices, p.ty};
     const dim3 grid((uint32_t)(batch * p.chunks * p.slices)), block(cl_lanes(p));
     const size_t cc = chunk_channels(p, VEC);
     with_flag(chunk != nullptr, [&](auto add) {
-        launch(cl_stats_kernel<T, VEC, add.value>, grid, block, (2 * p.ty + 1) * cc * sizeof(float), stream, x, chunk, partials, p);
+        launch(cl_stats_kernel<T, VEC, add.value>, grid, block, (2 * p.ty + 1) * cc * sizeof(float), stream, x, chunk, CL_GEOMETRY_OF(p),
+               partials, p);
     });
     if (joins(p)) {
         joined = join_launch<true>(p, parts, stats != nullptr ? stats : partials + partial_floats(p, batch) / 2, batch, eps, VEC, stream);
@@ -1179,8 +1207,8 @@ int cl_forward(ClPlan p, const ClForward &a, size_t batch, float eps, bool silu,
             with_flag(keep_here, [&](auto keep) {
                 if constexpr (VEC > 1 || !keep.value)
                     launch(cl_apply_kernel<T, VEC, add.value, act.value, keep.value>, grid, block,
-                           std::min<size_t>(p.groups, cc) * sizeof(float2), stream, x, chunk, y, a.gamma, a.beta, parts, joined, stats,
-                           a.codes, a.scales, eps, p);
+                           std::min<size_t>(p.groups, cc) * sizeof(float2), stream, x, chunk, CL_GEOMETRY_OF(p), a.gamma, a.beta, y, parts,
+                           joined, stats, a.codes, a.scales, eps, p);
             });
         });
     });
@@ -1189,7 +1217,8 @@ int cl_forward(ClPlan p, const ClForward &a, size_t batch, float eps, bool silu,
 
 template <typename T, int VEC, int FROM>
 int cl_backward_from(ClPlan p, const ClBackward &a, size_t batch, bool silu, hipStream_t stream) {
-    const T *dy = static_cast<const T *>(a.dy), *x = static_cast<const T *>(a.x), *chunk = static_cast<const T *>(a.chunk);
+    const T *dy = static_cast<const T *>(a.dy);
+    const void *h = FROM == kFromCodes ? a.codes : a.x, *more = FROM == kFromCodes ? a.scales : a.chunk;
     T *dx = static_cast<T *>(a.dx), *dchunk = static_cast<T *>(a.dchunk);
     const float2 *stats = reinterpret_cast<const float2 *>(a.stats);
     float *channel_sums = static_cast<float *>(a.workspace);
@@ -1202,7 +1231,7 @@ int cl_backward_from(ClPlan p, const ClBackward &a, size_t batch, bool silu, hip
         with_rows(k, [&](auto rows) {
             if constexpr (VEC < 8 || rows.value <= 2)
                 launch(cl_unit_grads_kernel<T, VEC, rows.value, FROM>, dim3((uint32_t)(batch * p.chunks)), dim3(cl_lanes(p)), lds, stream, dy,
-                       x, chunk, a.codes, a.scales, stats, a.gamma, a.beta, dx, s1, s2, dchunk, 2 * p.channels, silu, p);
+                       h, more, CL_GEOMETRY_OF(p), stats, a.gamma, a.beta, dx, s1, s2, dchunk, 2 * p.channels, silu, p);
         });
         if (affine && !one)
             launch(cl_affine_grads_kernel, dim3(tiles), dim3(kWave), 0, stream, channel_sums, a.dgamma, a.dbeta, (uint32_t)batch, p.channels);
@@ -1210,20 +1239,21 @@ int cl_backward_from(ClPlan p, const ClBackward &a, size_t batch, bool silu, hip
     }
     if (!slice_plan(&p, VEC, batch)) return MSD_ERR_INVALID_VALUE;
     float2 *partials = reinterpret_cast<float2 *>(channel_sums + channel_floats(p, batch)), *joined = nullptr;
-    const ClParts parts = {partials, p.slices, p.rows};
+    const ClParts parts = {partials, p.slices, p.ty};
     const dim3 grid((uint32_t)(batch * p.chunks * p.slices)), block(cl_lanes(p));
     const size_t cc = chunk_channels(p, VEC);
     with_flag(silu, [&](auto act) {
-        launch(cl_sums_kernel<T, VEC, FROM, act.value>, grid, block, 3 * p.ty * cc * sizeof(float), stream, dy, x, chunk, a.codes,
-               a.scales, stats, a.gamma, a.beta, partials, channel_sums, p);
+        launch(cl_sums_kernel<T, VEC, FROM, act.value>, grid, block, 3 * p.ty * cc * sizeof(float), stream, dy, h, more,
+               CL_GEOMETRY_OF(p), stats, a.gamma, a.beta, partials, channel_sums, p);
     });
     if (joins(p)) joined = join_launch<false>(p, parts, partials + partial_floats(p, batch) / 2, batch, 0.0f, VEC, stream);
     const size_t affine = a.dgamma != nullptr ? tiles : 0, added = dchunk != nullptr ? batch * tiles : 0;
     if (affine + added + grid.x > kClMaxBlocks) return MSD_ERR_INVALID_VALUE;
-    const ClChannelGrads grads = {channel_sums, a.dgamma, a.dbeta, dchunk, (uint32_t)affine, (uint32_t)(affine + added), (uint32_t)batch};
+    const ClChannelGrads grads = {channel_sums, a.dgamma, a.dbeta, dchunk, (uint32_t)affine, (uint32_t)batch};
+    const uint32_t channel_blocks = (uint32_t)(affine + added);
     with_flag(silu, [&](auto act) {
-        launch(cl_dx_kernel<T, VEC, FROM, act.value>, dim3(grid.x + grads.blocks), block, std::min<size_t>(p.groups, cc) * sizeof(float2),
-               stream, dy, x, chunk, a.codes, a.scales, stats, a.gamma, a.beta, dx, parts, joined, grads, p);
+        launch(cl_dx_kernel<T, VEC, FROM, act.value>, dim3(grid.x + channel_blocks), block, std::min<size_t>(p.groups, cc) * sizeof(float2),
+               stream, dy, h, more, CL_GEOMETRY_OF(p), channel_blocks, stats, a.gamma, a.beta, dx, parts, joined, grads, p);
     });
     return launch_status();
 }
