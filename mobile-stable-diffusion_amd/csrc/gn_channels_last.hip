@@ -183,20 +183,26 @@ __device__ __forceinline__ void keep_codes(const float *f, int8_t *codes, float 
         most = team_max<kCodeBlock / VEC>(most);
     }
     const float inv = code_inverse(most);
+    uint32_t c[VEC], seen = 0;
+#pragma unroll
+    for (int e = 0; e < VEC; e++) {
+        // 1.5 * 2^23 leaves the whole part, rounded to even, in the low bits; products of finite values are within +-127
+        float v = f[e] * inv;
+        asm volatile("" : "+v"(v));  // (the product is rounded by itself)
+        c[e] = __float_as_uint(v + 12582912.0f);
+        seen |= c[e];
+    }
+    // the sums of finite values have the exponent 0x96, so that only a NaN sets bit 29; one test for all of them, where a choice for
+    // each element made the kernel compute both sides (8 instructions an element in place of 2)
+    if (infinite || (seen & 0x20000000u) != 0) {
+        asm volatile("");  // (a branch: not to be computed beside the above)
+#pragma unroll
+        for (int e = 0; e < VEC; e++) c[e] = (uint32_t)code_of(f[e], inv);
+    }
     uint32_t w[VEC / 4];
 #pragma unroll
-    for (int e = 0; e < VEC; e += 4) {
-        uint32_t c[4];
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            // 1.5 * 2^23 leaves the whole part, rounded to even, in the low bits; products of finite values are within +-127
-            float v = f[e + k] * inv;
-            asm volatile("" : "+v"(v));  // (the product is rounded by itself)
-            c[k] = __float_as_uint(v + 12582912.0f);
-            if (infinite || f[e + k] != f[e + k]) c[k] = (uint32_t)code_of(f[e + k], inv);
-        }
-        w[e / 4] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(c[3], c[2], 0x0C0C0400u), __builtin_amdgcn_perm(c[1], c[0], 0x0C0C0400u), 0x05040100u);
-    }
+    for (int e = 0; e < VEC; e += 4)
+        w[e / 4] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(c[e + 3], c[e + 2], 0x0C0C0400u), __builtin_amdgcn_perm(c[e + 1], c[e], 0x0C0C0400u), 0x05040100u);
     if constexpr (VEC == 8) *reinterpret_cast<uint2 *>(codes) = make_uint2(w[0], w[1]);
     else *reinterpret_cast<uint32_t *>(codes) = w[0];
     if (first) *scale = code_scale(most);
