@@ -206,7 +206,8 @@ int msd_groupnorm_tokens_workspace(const void *x, void *y, const float *gamma, c
  * msd_groupnorm_channels_last_workspace reports (backward = 0), apart from all else; its contents need
  * not be set, are left undefined, and belong to this call until it (or every replay of it) is
  * done.  The call allocates nothing, shares nothing with other calls, and gives the same bits
- * every time, inside a stream capture and outside.  At most 2^22 channels.
+ * every time, inside a stream capture and outside.  At most 2^22 channels, and samples as a launch of
+ * 2^32 lanes has room for (2^20 at least of up to 2560 channels); beyond that it is refused.
  */
 #define MSD_CODE_BLOCK 32
 int msd_groupnorm_channels_last(const void *x, const void *chunk, void *y, const float *gamma, const float *beta,

@@ -1073,7 +1073,8 @@ __global__ __launch_bounds__(kWave) void cl_affine_grads_kernel(const float *sum
 }
 
 // ---- host ----
-constexpr uint64_t kClMaxBlocks = 0x7FFFFFFFull;
+// A grid holds less than 2^32 lanes.
+bool fits_grid(uint64_t blocks, uint32_t lanes) { return blocks <= 0xFFFFFFFFull / lanes; }
 constexpr size_t kClMaxChannels = (size_t)1 << 22;
 constexpr uint64_t kClUnitElements = 1u << 28;  // of a sample that workgroups have whole: offsets in it are counted in 32 bits
 
@@ -1091,6 +1092,9 @@ bool cl_shape(size_t elt, size_t batch, size_t positions, size_t channels, size_
     p->per_group = make_fast_div((uint32_t)(channels / groups));
     return true;
 }
+
+uint32_t cl_lanes(const ClPlan &p) { return (p.tx * p.ty + kWave - 1) / kWave * kWave; }
+bool joins(const ClPlan &p) { return p.slices * p.spans > kClMaxParts; }
 
 void finish_plan(ClPlan *p, uint32_t tx, uint32_t ty, uint32_t slices, uint32_t vec) {
     p->tx = tx;
@@ -1119,12 +1123,12 @@ uint32_t unit_plan(ClPlan *p, uint32_t vec, size_t batch, uint32_t max_k) {
     uint64_t tx = whole;  // more of them where they are short
     while (tx * 2 <= p->columns && tx * 2 * p->positions <= 128) tx *= 2;
     const uint64_t chunks = (p->columns + tx - 1) / tx;
-    if (chunks > kClMaxCount || batch * chunks > kClMaxBlocks) return 0;
+    if (chunks > kClMaxCount) return 0;
     uint32_t k = 1;
     while (k * (kClUnitThreads / tx) < p->positions) k *= 2;
     if (k > max_k) return 0;
     finish_plan(p, (uint32_t)tx, (p->positions + k - 1) / k, 1, vec);
-    return k;
+    return fits_grid(batch * chunks, cl_lanes(*p)) ? k : 0;
 }
 
 // (a gradient holds two rows for one: of 8 channels each, no more than two fit the registers)
@@ -1142,14 +1146,13 @@ bool slice_plan(ClPlan *p, uint32_t vec, size_t batch) {
     const uint64_t most = std::max<uint64_t>(1, kClBlocks / across);
     const uint64_t wanted = ((uint64_t)p->positions + (uint64_t)ty * kClRows - 1) / ((uint64_t)ty * kClRows);
     finish_plan(p, tx, ty, (uint32_t)std::min(wanted, most), vec);
-    return p->slices <= kClMaxCount && p->chunks <= kClMaxCount && across * p->slices <= kClMaxBlocks;
+    return p->slices <= kClMaxCount && p->chunks <= kClMaxCount && fits_grid(across * p->slices, cl_lanes(*p)) &&
+           (!joins(*p) || fits_grid(batch * p->groups, kClJoinThreads));
 }
 
 size_t partial_floats(const ClPlan &p, size_t batch) { return 2 * batch * p.slices * p.spans * p.groups; }
 size_t joined_floats(const ClPlan &p, size_t batch) { return 2 * batch * p.groups; }
 size_t channel_floats(const ClPlan &p, size_t batch) { return (3 * batch * p.slices * (size_t)p.channels + 1) / 2 * 2; }
-bool joins(const ClPlan &p) { return p.slices * p.spans > kClMaxParts; }
-uint32_t cl_lanes(const ClPlan &p) { return (p.tx * p.ty + kWave - 1) / kWave * kWave; }
 size_t chunk_channels(const ClPlan &p, uint32_t vec) { return (size_t)std::min(p.tx, p.columns) * vec; }
 
 // f(std::bool_constant) of a runtime flag, f(std::integral_constant) of a number of rows
@@ -1244,6 +1247,8 @@ int cl_backward_from(ClPlan p, const ClBackward &a, size_t batch, bool silu, hip
         return launch_status();
     }
     if (!slice_plan(&p, VEC, batch)) return MSD_ERR_INVALID_VALUE;
+    const size_t affine = a.dgamma != nullptr ? tiles : 0, added = dchunk != nullptr ? batch * tiles : 0;
+    if (!fits_grid(affine + added + (uint64_t)batch * p.chunks * p.slices, cl_lanes(p))) return MSD_ERR_INVALID_VALUE;
     float2 *partials = reinterpret_cast<float2 *>(channel_sums + channel_floats(p, batch)), *joined = nullptr;
     const ClParts parts = {partials, p.slices, p.ty};
     const dim3 grid((uint32_t)(batch * p.chunks * p.slices)), block(cl_lanes(p));
@@ -1253,8 +1258,6 @@ int cl_backward_from(ClPlan p, const ClBackward &a, size_t batch, bool silu, hip
                CL_GEOMETRY_OF(p), stats, a.gamma, a.beta, partials, channel_sums, p);
     });
     if (joins(p)) joined = join_launch<false>(p, parts, partials + partial_floats(p, batch) / 2, batch, 0.0f, VEC, stream);
-    const size_t affine = a.dgamma != nullptr ? tiles : 0, added = dchunk != nullptr ? batch * tiles : 0;
-    if (affine + added + grid.x > kClMaxBlocks) return MSD_ERR_INVALID_VALUE;
     const ClChannelGrads grads = {channel_sums, a.dgamma, a.dbeta, dchunk, (uint32_t)affine, (uint32_t)batch};
     const uint32_t channel_blocks = (uint32_t)(affine + added);
     with_flag(silu, [&](auto act) {
@@ -1319,7 +1322,7 @@ int cl_backward_dispatch(const ClBackward &a, size_t batch, size_t positions, si
                          hipStream_t stream) {
     if (batch == 0 || positions == 0) {  // sums over nothing
         const size_t added = a.dchunk != nullptr ? batch * channels : 0, most = std::max(a.dgamma != nullptr ? channels : 0, added);
-        if ((most + 255) / 256 > kClMaxBlocks) return MSD_ERR_INVALID_VALUE;
+        if (!fits_grid((most + 255) / 256, 256)) return MSD_ERR_INVALID_VALUE;
         if (most != 0)
             launch(cl_zero_kernel<T>, dim3((uint32_t)((most + 255) / 256)), dim3(256), 0, stream, a.dgamma, a.dbeta,
                    static_cast<T *>(a.dchunk), channels, added);

@@ -37,33 +37,35 @@ __global__ __launch_bounds__(kPackThreads) void q4_pack_kernel(const T *w, uint8
 // Any alignment: a wavefront per column, a lane per byte of its codes.
 // ---------------------------------------------------------------------------
 constexpr uint32_t kQ4Threads = 256;
+constexpr size_t kQ4MaxBlocks = 0xFFFFFFFFu / 512;  // (a grid holds less than 2^32 lanes)
 
 template <typename T>
 __global__ __launch_bounds__(kQ4Threads) void linear_q4_generic_kernel(const T *x, const uint8_t *packed, const T *scales,
                                                                        const float *bias, T *y, uint32_t m, uint32_t n,
                                                                        uint32_t k, uint32_t group, int act_in, int act_out) {
-    const uint32_t lane = threadIdx.x % kWave, col = blockIdx.x * (kQ4Threads / kWave) + threadIdx.x / kWave;
-    if (col >= n) return;
-    const uint8_t *row = packed + (size_t)col * (k / 2);
-    for (uint32_t i = 0; i < m; i++) {
-        const T *xr = x + (size_t)i * k;
-        float acc = 0.0f;
-        for (uint32_t j = lane; j < k / 2; j += kWave) {
-            float a = Store<T>::load1(xr + 2 * j), b = Store<T>::load1(xr + 2 * j + 1);
-            if (act_in) {
-                a = silu_f(a);
-                b = silu_f(b);
+    const uint32_t lane = threadIdx.x % kWave, step = gridDim.x * (kQ4Threads / kWave);
+    for (uint32_t col = blockIdx.x * (kQ4Threads / kWave) + threadIdx.x / kWave; col < n; col += step) {
+        const uint8_t *row = packed + (size_t)col * (k / 2);
+        for (uint32_t i = 0; i < m; i++) {
+            const T *xr = x + (size_t)i * k;
+            float acc = 0.0f;
+            for (uint32_t j = lane; j < k / 2; j += kWave) {
+                float a = Store<T>::load1(xr + 2 * j), b = Store<T>::load1(xr + 2 * j + 1);
+                if (act_in) {
+                    a = silu_f(a);
+                    b = silu_f(b);
+                }
+                const uint32_t codes = row[j];
+                const float s = Store<T>::load1(scales + (size_t)col * (k / group) + 2 * j / group);
+                acc = fmaf(a, (float)((int)(codes & 15) - 8) * s, acc);  // (a code times x could be infinite)
+                acc = fmaf(b, (float)((int)(codes >> 4) - 8) * s, acc);
             }
-            const uint32_t codes = row[j];
-            const float s = Store<T>::load1(scales + (size_t)col * (k / group) + 2 * j / group);
-            acc = fmaf(a, (float)((int)(codes & 15) - 8) * s, acc);  // (a code times x could be infinite)
-            acc = fmaf(b, (float)((int)(codes >> 4) - 8) * s, acc);
-        }
-        acc = wave_sum(acc);
-        if (lane == 0) {
-            float r = acc + (bias != nullptr ? bias[col] : 0.0f);
-            if (act_out) r = silu_f(r);
-            Store<T>::store1(y + (size_t)i * n + col, r);
+            acc = wave_sum(acc);
+            if (lane == 0) {
+                float r = acc + (bias != nullptr ? bias[col] : 0.0f);
+                if (act_out) r = silu_f(r);
+                Store<T>::store1(y + (size_t)i * n + col, r);
+            }
         }
     }
 }
@@ -408,7 +410,7 @@ int linear_q4_dispatch(const void *x, const uint8_t *const *packed, const void *
     if (!aligned) {
         for (size_t i = 0; i < count; i++)
             if (ns[i] != 0)
-                launch(linear_q4_generic_kernel<T>, dim3((uint32_t)((ns[i] + kQ4Threads / kWave - 1) / (kQ4Threads / kWave))),
+                launch(linear_q4_generic_kernel<T>, dim3((uint32_t)std::min<size_t>(kQ4MaxBlocks, (ns[i] + kQ4Threads / kWave - 1) / (kQ4Threads / kWave))),
                        dim3(kQ4Threads), 0, stream, rows, packed[i], static_cast<const T *>(scales[i]), bias_of(i),
                        static_cast<T *>(ys[i]), (uint32_t)m, (uint32_t)ns[i], (uint32_t)k, (uint32_t)group, act_in, act_out);
         return launch_status();
@@ -420,21 +422,27 @@ int linear_q4_dispatch(const void *x, const uint8_t *const *packed, const void *
     const size_t steps = (k + kMmStep - 1) / kMmStep, rounds = (steps + kMmMaxWaves - 1) / kMmMaxWaves, waves = (steps + rounds - 1) / rounds;
     const int ct = tiles < 320 ? 1 : (m > 2 ? tiles >= 640 : tiles >= 1024 && waves <= 4) ? 4 : 2;
     const Q4Launch a = {(uint32_t)m, (uint32_t)k, (uint32_t)waves, act_in, act_out, stream};
+    const size_t columns = (size_t)kMmTile * ct;
+    auto blocks_of = [&](size_t i) { return (ns[i] + columns - 1) / columns; };
+    for (size_t i = 0; i < count; i++)
+        if (blocks_of(i) > kQ4MaxBlocks) return MSD_ERR_INVALID_VALUE;
     Q4Layers layers{};
     uint32_t held = 0;
+    auto send = [&] {
+        if (held == 0) return;
+        if (sizeof(T) == 4 || act_in) launch_q4_group<T, true>(rows, layers, held, (uint32_t)group, ct, a);
+        else if constexpr (sizeof(T) == 2) launch_q4_group<T, false>(rows, layers, held, (uint32_t)group, ct, a);
+        layers = Q4Layers{};
+        held = 0;
+    };
     for (size_t i = 0; i < count; i++) {
-        if (ns[i] != 0) {
-            const uint32_t columns = kMmTile * ct, blocks = layers.first_block[held] + ((uint32_t)ns[i] + columns - 1) / columns;
-            layers.layer[held++] = {packed[i], scales[i], bias_of(i), ys[i], (uint32_t)ns[i]};
-            for (uint32_t j = held; j <= kQ4GroupMax; j++) layers.first_block[j] = blocks;
-        }
-        if (held == kQ4GroupMax || (i + 1 == count && held != 0)) {
-            if (sizeof(T) == 4 || act_in) launch_q4_group<T, true>(rows, layers, held, (uint32_t)group, ct, a);
-            else if constexpr (sizeof(T) == 2) launch_q4_group<T, false>(rows, layers, held, (uint32_t)group, ct, a);
-            layers = Q4Layers{};
-            held = 0;
-        }
+        if (ns[i] == 0) continue;
+        if (held == kQ4GroupMax || layers.first_block[held] + blocks_of(i) > kQ4MaxBlocks) send();
+        const uint32_t blocks = layers.first_block[held] + (uint32_t)blocks_of(i);
+        layers.layer[held++] = {packed[i], scales[i], bias_of(i), ys[i], (uint32_t)ns[i]};
+        for (uint32_t j = held; j <= kQ4GroupMax; j++) layers.first_block[j] = blocks;
     }
+    send();
     return launch_status();
 }
 template int linear_q4_dispatch<float>(const void *, const uint8_t *const *, const void *const *, const float *const *, void *const *,

@@ -150,3 +150,14 @@ def test_operands_that_do_not_fit(msd, cuda):
         with pytest.raises(msd.MsdError):
             call()
             pytest.fail("call %d was not refused" % i)
+
+
+def test_launches_of_more_lanes_than_a_grid_holds(msd):
+    lib, size = msd.load_library(), ctypes.c_size_t(0)
+    for batch, positions, channels, fits in ((1 << 22, 8, 320, True), (1 << 24, 8, 320, False), (1 << 23, 4096, 320, False),
+                                             (1 << 20, 1, 2560, True), (1 << 23, 4096, 32, False)):
+        for backward in (0, 1):
+            rc = lib.msd_groupnorm_channels_last_workspace(batch, positions, channels, 32, 1, backward, ctypes.byref(size))
+            assert (rc == 0) == fits, (batch, positions, channels, backward)
+    at = [p((i + 1) << 42) for i in range(4)]  # 2^28 columns of 1024: apart from each other
+    assert lib.msd_linear_rows_q4(at[0], at[1], at[2], None, at[3], 1, 1 << 28, 1024, 128, 0, 0, 1, None) == 1
