@@ -34,7 +34,8 @@ __global__ __launch_bounds__(kPackThreads) void q4_pack_kernel(const T *w, uint8
 }
 
 // ---------------------------------------------------------------------------
-// Any alignment: a wavefront per column, a lane per byte of its codes.
+// Any alignment: a wavefront per column, a lane per byte of its codes.  25 times the time of the kernel below (16384 x 8192, 8 rows
+// float16: 539 us), for views that begin in the middle of 16 bytes and for k below 128 or above 2^22.
 // ---------------------------------------------------------------------------
 constexpr uint32_t kQ4Threads = 256;
 constexpr size_t kQ4MaxBlocks = 0xFFFFFFFFu / 512;  // (a grid holds less than 2^32 lanes)
@@ -86,6 +87,11 @@ __global__ __launch_bounds__(kQ4Threads) void linear_q4_generic_kernel(const T *
 // (2, 6), (3, 7) by masks alone; x is laid out in LDS in that order.
 //
 // How k is dealt depends on k alone, so a row has the same bits for any CT, number of rows and company.
+//
+// What bounds it: codes and scales are read once, 69 MB at 16384 x 8192 in 21.7 us, 3.2 TB/s (half of what memory gives): a
+// wavefront issues an instruction every 16 cycles or so and has some 9 for eight codes of a lane, two wavefronts share a SIMD, and
+// requests are one step ahead; four wavefronts (CT = 2) do the work on x twice.  Small calls are latency: 1280 x 1280, 1 row
+// float16 3.6 us of 0.9 MB, 22 projections of 20160 x 1280, 2 rows float16 8.0, 8 rows float32 12.4.
 // ---------------------------------------------------------------------------
 constexpr int kMmMaxWaves = 8;
 constexpr int kMmTile = 16;                   // columns of a tile
