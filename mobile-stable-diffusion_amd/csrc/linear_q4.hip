@@ -88,10 +88,12 @@ __global__ __launch_bounds__(kQ4Threads) void linear_q4_generic_kernel(const T *
 //
 // How k is dealt depends on k alone, so a row has the same bits for any CT, number of rows and company.
 //
-// What bounds it: codes and scales are read once, 69 MB at 16384 x 8192 in 21.7 us, 3.2 TB/s (half of what memory gives): a
-// wavefront issues an instruction every 16 cycles or so and has some 9 for eight codes of a lane, two wavefronts share a SIMD, and
-// requests are one step ahead; four wavefronts (CT = 2) do the work on x twice.  Small calls are latency: 1280 x 1280, 1 row
-// float16 3.6 us of 0.9 MB, 22 projections of 20160 x 1280, 2 rows float16 8.0, 8 rows float32 12.4.
+// What bounds it: codes and scales are read once, 69 MB at 16384 x 8192 in 21.7 us, 3.2 TB/s (half of what memory gives).  A
+// wavefront there (two to a SIMD) issues an instruction in 23 % of its cycles, 40 % it waits for its requests, which are one step
+// ahead, 37 % for the instruction before (each eight codes are nine instructions and an MFMA that wait for one another).  Neither
+// side alone gives: sixteen wavefronts a workgroup 25.4 us against 23.1 (passes in a graph), workgroups that begin at different
+// steps, so that not all are at the same channels of memory, 23.9.  Small calls are latency: 1280 x 1280, 1 row float16 3.6 us of
+// 0.9 MB, 22 projections of 20160 x 1280, 2 rows float16 8.3, 8 rows float32 12.4.
 // ---------------------------------------------------------------------------
 constexpr int kMmMaxWaves = 8;
 constexpr int kMmTile = 16;                   // columns of a tile
