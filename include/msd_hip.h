@@ -378,7 +378,8 @@ int msd_linear_rows_grouped(const void *x, const void *const *weights, const flo
  *           largest finite |w| of a group, scale = a / 7 rounded to the storage type and code =
  *           round(w * (1 / scale)) (to even, clamped to +-7) + 8; a < 1e-30 or a scale of 0: the
  *           scale is 0 and the codes are 8.  packed and scales lie apart from w and each other.
- * n and k are at most 2^28.  No counterpart in the reference, whose weights are float32.
+ * n and k are at most 2^28 (a launch of 2^32 lanes is refused).  No counterpart in the reference, whose
+ * weights are float32.
  */
 int msd_q4_pack(const void *w, uint8_t *packed, void *scales, size_t n, size_t k, size_t group, int dtype,
                 void *stream);
