@@ -446,11 +446,11 @@ def groupnorm_channels_last_backward(dy, kept, affine=True, out=None):
     batch, positions, channels = _channels_last(dy, "dy")
     code = _dtype_code(dy)
     if kept.codes is not None:
-        if kept.codes.shape != dy.shape:
-            raise MsdError("dy must have the shape of the forward call's x")
+        if kept.codes.dtype != _torch.int8 or kept.codes.shape != dy.shape:
+            raise MsdError("codes must be int8 of dy's shape %s (got %s, %s)" % (tuple(dy.shape), kept.codes.dtype, tuple(kept.codes.shape)))
         _channels_last(kept.codes, "codes")
         xp = cp = None
-        qp, sp = kept.codes.data_ptr(), _dev(kept.scales)
+        qp, sp = kept.codes.data_ptr(), _affine(kept.scales, batch * positions * -(-channels // CODE_BLOCK), dy, "scales")
     else:
         xp = _same_layout(kept.x, dy, "the forward call's x")
         cp = _same(kept.chunk, dy, batch * channels, "chunk") if kept.chunk is not None else None

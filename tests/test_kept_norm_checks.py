@@ -1,0 +1,92 @@
+"""groupnorm_channels_last_backward checks everything that a KeptNorm hands to the kernels, before anything is launched: on the
+CPU, with tensors that only say that they are on a device and a library that records what would be launched."""
+import pytest
+
+torch = pytest.importorskip("torch")
+
+
+class OnDevice(torch.Tensor):
+    """A CPU tensor that says it is on device 0."""
+    is_cuda = True
+
+    def get_device(self):
+        return 0
+
+
+def _on(t):
+    return t.as_subclass(OnDevice)
+
+
+class Library:
+    """Stands for the loaded library: workspaces as it says, gradients recorded and not made."""
+
+    def __init__(self, lib):
+        self.lib, self.made = lib, []
+
+    def msd_groupnorm_channels_last_backward(self, *args):
+        self.made.append(args)
+        return 0
+
+    def __getattr__(self, name):
+        return getattr(self.lib, name)
+
+
+@pytest.fixture
+def library(msd, monkeypatch):
+    lib = Library(msd.load_library())
+    monkeypatch.setattr(msd, "_lib", lib)
+    monkeypatch.setattr(msd, "_native_cl_q4", msd._NoNative())
+    monkeypatch.setattr(msd, "_stream", lambda: None)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    return lib
+
+
+def _kept(msd, b, p, c, groups, keep8):
+    g = _on(torch.ones(c))
+    x = codes = scales = None
+    if keep8:
+        codes, scales = _on(torch.zeros((b, p, c), dtype=torch.int8)), _on(torch.zeros((b, p, -(-c // 32))))
+    else:
+        x = _on(torch.zeros((b, p, c)))
+    return msd.KeptNorm(x, None, codes, scales, _on(torch.ones((b, groups, 2))), g, _on(torch.zeros(c)), groups, True, False)
+
+
+def test_a_kept_norm_that_fits_is_taken(msd, library):
+    for keep8 in (False, True):
+        msd.groupnorm_channels_last_backward(_on(torch.zeros(2, 5, 48)), _kept(msd, 2, 5, 48, 8, keep8))
+    assert len(library.made) == 2
+
+
+@pytest.mark.parametrize("change", [
+    dict(scales=torch.zeros((2, 5, 2), dtype=torch.float16)), dict(scales=torch.zeros((2, 5, 2), dtype=torch.float64)),
+    dict(scales=torch.zeros(2, 5, 1)), dict(scales=torch.zeros(2, 4, 2)), dict(scales=torch.zeros(2, 5, 3)), dict(scales=torch.zeros(0)),
+    dict(scales=torch.zeros(2, 2, 5).transpose(1, 2)),
+    dict(codes=torch.zeros((2, 5, 48), dtype=torch.uint8)), dict(codes=torch.zeros((2, 5, 48), dtype=torch.float16)),
+    dict(codes=torch.zeros((2, 5, 47), dtype=torch.int8)), dict(codes=torch.zeros((1, 5, 48), dtype=torch.int8)),
+    dict(codes=torch.zeros((2, 48, 5), dtype=torch.int8).transpose(1, 2)),
+    dict(stats=torch.ones(2, 7, 2)), dict(stats=torch.ones((2, 8, 2), dtype=torch.float16)), dict(gamma=torch.ones(47)),
+    dict(beta=torch.ones(48, dtype=torch.float16)), dict(groups=7), dict(groups=0),
+], ids=lambda change: "-".join("%s %s %s" % (k, getattr(v, "dtype", v), tuple(getattr(v, "shape", ()))) for k, v in change.items()))
+def test_kept_codes_and_scales_that_do_not_fit_are_refused(msd, library, change):
+    kept = _kept(msd, 2, 5, 48, 8, True)._replace(**{k: _on(v) if torch.is_tensor(v) else v for k, v in change.items()})
+    with pytest.raises(msd.MsdError):
+        msd.groupnorm_channels_last_backward(_on(torch.zeros(2, 5, 48)), kept)
+    assert not library.made
+
+
+@pytest.mark.parametrize("name", ["codes", "scales"])
+def test_codes_and_scales_elsewhere_are_refused(msd, library, name):
+    kept = _kept(msd, 2, 5, 48, 8, True)
+    with pytest.raises(msd.MsdError):
+        msd.groupnorm_channels_last_backward(_on(torch.zeros(2, 5, 48)), kept._replace(**{name: getattr(kept, name).as_subclass(torch.Tensor)}))
+    assert not library.made
+
+
+@pytest.mark.gpu
+def test_refused_on_the_device_too(msd, cuda):
+    x, g = torch.randn(2, 5, 48, device=cuda), torch.ones(48, device=cuda)
+    _, kept = msd.groupnorm_channels_last_kept(x, g, g, 8, keep8=True)
+    for change in (dict(scales=kept.scales.half()), dict(scales=kept.scales[:1]), dict(scales=kept.scales.cpu()), dict(codes=kept.codes.view(torch.uint8)),
+                   dict(codes=kept.codes.cpu())):
+        with pytest.raises(msd.MsdError):
+            msd.groupnorm_channels_last_backward(x, kept._replace(**change))
