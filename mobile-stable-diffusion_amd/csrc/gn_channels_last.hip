@@ -994,6 +994,17 @@ __global__ __launch_bounds__(kClThreads) void cl_dx_kernel(const T *dy, const vo
     });
 }
 
+// LDS of cl_unit_grads_kernel, in floats: three sums [ty][cc] and gamma S1, gamma S2 [2][cc]; then, where a float2 may begin, the
+// groups' means.
+struct UnitGradsLds {
+    uint32_t sums, weighted, of_group;
+    __host__ __device__ constexpr UnitGradsLds(uint32_t ty, uint32_t cc)
+        : sums(ty * cc), weighted(3 * sums), of_group((weighted + 2 * cc + 1) / 2 * 2) {}
+    constexpr size_t bytes(size_t groups) const { return of_group * sizeof(float) + groups * sizeof(float2); }
+};
+static_assert(UnitGradsLds(1, 5).of_group == 26 && UnitGradsLds(2, 5).of_group == 40 && UnitGradsLds(3, 7).of_group == 78 &&
+              UnitGradsLds(2, 8).of_group == 64, "rounded up to whole float2");
+
 // The whole of it where a workgroup has all positions of its chunk (whole groups): K rows a lane.  channel_sums
 // [batch][2][channels]: S1 and S2, for cl_affine_grads_kernel, or, of one sample, dbeta and dgamma themselves (or null).
 // 2560 channels at 9 x 7, 2 samples float32: 6.2 us, and 2.1 for dgamma and dbeta.
@@ -1030,9 +1041,10 @@ __global__ __launch_bounds__(kClUnitThreads) void cl_unit_grads_kernel(const T *
             }
         }
     }
-    const uint32_t stride = ty * cc;
-    float *weighted = lds + 3 * stride;  // [2][cc]: gamma S1, gamma S2
-    float2 *of_group = reinterpret_cast<float2 *>(weighted + 2 * cc + (stride + cc) % 2);
+    const UnitGradsLds at_lds(ty, cc);
+    const uint32_t stride = at_lds.sums;
+    float *weighted = lds + at_lds.weighted;
+    float2 *of_group = reinterpret_cast<float2 *>(lds + at_lds.of_group);
 #pragma unroll
     for (int q = 0; q < 3; q++) put_channels<VEC>(lds + q * stride, t, sums[q]);
     add_rows<3>(lds, stride, ty, cc);
@@ -1255,7 +1267,7 @@ int cl_backward_from(ClPlan p, const ClBackward &a, size_t batch, bool silu, hip
     const uint32_t tiles = (p.channels + kWave - 1) / kWave;
     if (const uint32_t k = unit_plan(&p, VEC, batch, unit_grads_max_k(VEC))) {
         const size_t cc = chunk_channels(p, VEC);
-        const size_t lds = (3 * p.ty * cc + 2 * cc + 1) * sizeof(float) + std::min<size_t>(p.groups, cc) * sizeof(float2);
+        const size_t lds = UnitGradsLds(p.ty, (uint32_t)cc).bytes(std::min<size_t>(p.groups, cc));
         const bool affine = a.dgamma != nullptr, one = batch == 1;
         float *s1 = !affine ? nullptr : one ? a.dbeta : channel_sums, *s2 = !affine ? nullptr : one ? a.dgamma : channel_sums + p.channels;
         with_rows(k, [&](auto rows) {
