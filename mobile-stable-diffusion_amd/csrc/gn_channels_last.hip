@@ -45,6 +45,7 @@ constexpr uint32_t kClJoinThreads = 256;
 constexpr uint32_t kClTeam = 16;        // lanes that add up a group's channels
 constexpr uint32_t kClUnitThreads = 1024;
 constexpr uint32_t kClUnitMaxK = 4;     // most rows a lane holds of a workgroup that has all positions
+constexpr size_t kClMaxLds = 160 * 1024;  // of a workgroup
 constexpr uint32_t kCodeBlock = 32;     // channels of one position that share a scale
 constexpr float kCodeTiny = 1e-30f;     // blocks below this are kept as zeros (1 / a would not be finite)
 
@@ -644,6 +645,13 @@ __global__ __launch_bounds__(kClThreads) void cl_apply_kernel(const T *x, const 
     });
 }
 
+// LDS of cl_unit_kernel, in floats: two sums [ty][cc] and the first row [cc]; then, where a float2 may begin, the groups' statistics.
+struct UnitLds {
+    uint32_t first_row, of_group;
+    __host__ __device__ constexpr UnitLds(uint32_t ty, uint32_t cc) : first_row(2 * ty * cc), of_group((first_row + cc + 1) / 2 * 2) {}
+    constexpr size_t bytes(size_t groups) const { return of_group * sizeof(float) + groups * sizeof(float2); }
+};
+
 // The whole of it where a workgroup has all positions of its chunk (whole groups): K rows a lane.  Latency bounds it: a load, the
 // sums through LDS, a store.  Passes in a graph, us, so and in slices: 1280 channels at 8 x 8 float16 5.6 and 9.9, at 16 x 16, 2
 // samples (K = 4) 7.5 and 10.9; with the gradient 19.1 and 24.0, of 2560 at 9 x 7 float32 (K = 2) 12.9 and 19.7.
@@ -684,8 +692,9 @@ __global__ __launch_bounds__(kClUnitThreads) void cl_unit_kernel(const T *x, con
             }
         }
     }
-    float *first_row = lds + 2 * ty * cc;
-    float2 *of_group = reinterpret_cast<float2 *>(first_row + (cc + 1) / 2 * 2);
+    const UnitLds at_lds(ty, cc);
+    float *first_row = lds + at_lds.first_row;
+    float2 *of_group = reinterpret_cast<float2 *>(lds + at_lds.of_group);
     put_channels<VEC>(lds, t, s1);
     put_channels<VEC>(lds + ty * cc, t, s2);
     if (t.ty == 0) put_channels<VEC>(first_row, t, shift);
@@ -1148,8 +1157,20 @@ uint64_t whole_columns(const ClPlan &p, uint32_t vec, bool blocks) {
     return blocks ? std::lcm<uint64_t, uint64_t>(columns, std::max<uint32_t>(1, kCodeBlock / vec)) : columns;
 }
 
+size_t chunk_channels(const ClPlan &p, uint32_t vec) { return (size_t)std::min(p.tx, p.columns) * vec; }
+// What a workgroup of unit_plan asks for of LDS (its chunk is whole groups).
+size_t unit_lds(const ClPlan &p, uint32_t vec, bool backward) {
+    const uint32_t cc = (uint32_t)chunk_channels(p, vec);
+    const size_t groups = cc / p.per_group.d;
+    return backward ? UnitGradsLds(p.ty, cc).bytes(groups) : UnitLds(p.ty, cc).bytes(groups);
+}
+
+// (a gradient holds two rows for one: of 8 channels each, no more than two fit the registers)
+uint32_t unit_max_k(uint32_t vec, bool backward) { return backward && vec == 8 ? 2 : kClUnitMaxK; }
+
 // A workgroup with all positions of some whole groups: K rows a lane; 0 where that is too much for one.
-uint32_t unit_plan(ClPlan *p, uint32_t vec, size_t batch, uint32_t max_k) {
+uint32_t unit_plan(ClPlan *p, uint32_t vec, size_t batch, bool backward) {
+    const uint32_t max_k = unit_max_k(vec, backward);
     const uint64_t whole = whole_columns(*p, vec, false);
     if (whole > kClUnitThreads || whole * p->positions > kClUnitThreads * max_k) return 0;
     if ((uint64_t)p->positions * p->channels > kClUnitElements) return 0;
@@ -1161,11 +1182,8 @@ uint32_t unit_plan(ClPlan *p, uint32_t vec, size_t batch, uint32_t max_k) {
     while (k * (kClUnitThreads / tx) < p->positions) k *= 2;
     if (k > max_k) return 0;
     finish_plan(p, (uint32_t)tx, (p->positions + k - 1) / k, 1, vec);
-    return fits_grid(batch * chunks, cl_lanes(*p)) ? k : 0;
+    return fits_grid(batch * chunks, cl_lanes(*p)) && unit_lds(*p, vec, backward) <= kClMaxLds ? k : 0;
 }
-
-// (a gradient holds two rows for one: of 8 channels each, no more than two fit the registers)
-uint32_t unit_grads_max_k(uint32_t vec) { return vec == 8 ? 2 : kClUnitMaxK; }
 
 bool slice_plan(ClPlan *p, uint32_t vec, size_t batch) {
     // whole groups and whole code blocks in a chunk where that leaves it short enough, else whole code blocks
@@ -1186,7 +1204,6 @@ bool slice_plan(ClPlan *p, uint32_t vec, size_t batch) {
 size_t partial_floats(const ClPlan &p, size_t batch) { return 2 * batch * p.slices * p.spans * p.groups; }
 size_t joined_floats(const ClPlan &p, size_t batch) { return 2 * batch * p.groups; }
 size_t channel_floats(const ClPlan &p, size_t batch) { return (3 * batch * p.slices * (size_t)p.channels + 1) / 2 * 2; }
-size_t chunk_channels(const ClPlan &p, uint32_t vec) { return (size_t)std::min(p.tx, p.columns) * vec; }
 
 // f(std::bool_constant) of a runtime flag, f(std::integral_constant) of a number of rows
 template <typename F>
@@ -1212,7 +1229,7 @@ int cl_forward(ClPlan p, const ClForward &a, size_t batch, float eps, bool silu,
     const T *x = static_cast<const T *>(a.x), *chunk = static_cast<const T *>(a.chunk);
     T *y = static_cast<T *>(a.y);
     float2 *stats = reinterpret_cast<float2 *>(a.stats);
-    const uint32_t k = unit_plan(&p, VEC, batch, kClUnitMaxK);
+    const uint32_t k = unit_plan(&p, VEC, batch, false);
     if (k == 0 && !slice_plan(&p, VEC, batch)) return MSD_ERR_INVALID_VALUE;
     const bool keep_here = a.codes != nullptr && VEC > 1 && p.channels % kCodeBlock == 0 && p.tx * VEC % kCodeBlock == 0;
     if (a.codes != nullptr && !keep_here) {
@@ -1221,8 +1238,7 @@ int cl_forward(ClPlan p, const ClForward &a, size_t batch, float eps, bool silu,
                a.codes, a.scales, rows, p.positions, p.channels);
     }
     if (k != 0) {
-        const size_t cc = chunk_channels(p, VEC);
-        const size_t lds = (2 * p.ty * cc + (cc + 1) / 2 * 2) * sizeof(float) + std::min<size_t>(p.groups, cc) * sizeof(float2);
+        const size_t lds = unit_lds(p, VEC, false);
         with_rows(k, [&](auto rows) {
             with_flag(keep_here, [&](auto keep) {
                 if constexpr (VEC > 1 || !keep.value)
@@ -1265,9 +1281,8 @@ int cl_backward_from(ClPlan p, const ClBackward &a, size_t batch, bool silu, hip
     const float2 *stats = reinterpret_cast<const float2 *>(a.stats);
     float *channel_sums = static_cast<float *>(a.workspace);
     const uint32_t tiles = (p.channels + kWave - 1) / kWave;
-    if (const uint32_t k = unit_plan(&p, VEC, batch, unit_grads_max_k(VEC))) {
-        const size_t cc = chunk_channels(p, VEC);
-        const size_t lds = UnitGradsLds(p.ty, (uint32_t)cc).bytes(std::min<size_t>(p.groups, cc));
+    if (const uint32_t k = unit_plan(&p, VEC, batch, true)) {
+        const size_t lds = unit_lds(p, VEC, true);
         const bool affine = a.dgamma != nullptr, one = batch == 1;
         float *s1 = !affine ? nullptr : one ? a.dbeta : channel_sums, *s2 = !affine ? nullptr : one ? a.dgamma : channel_sums + p.channels;
         with_rows(k, [&](auto rows) {
@@ -1326,7 +1341,7 @@ size_t cl_workspace_bytes(size_t elt, size_t batch, size_t positions, size_t cha
         ClPlan p;
         uint32_t vec;
         if (!cl_shape(elt, batch, positions, channels, groups, vectors, &p, &vec)) return SIZE_MAX;
-        if (unit_plan(&p, vec, batch, backward ? unit_grads_max_k(vec) : kClUnitMaxK) != 0) {
+        if (unit_plan(&p, vec, batch, backward) != 0) {
             if (backward) most = std::max(most, 2 * batch * channels * sizeof(float));
             continue;
         }
