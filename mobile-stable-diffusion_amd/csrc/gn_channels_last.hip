@@ -40,8 +40,7 @@ constexpr uint32_t kClThreads = 512;    // most lanes of a workgroup that has a 
 constexpr uint32_t kClBlocks = 256;     // workgroups of a launch of slices: one per CU
 constexpr uint32_t kClMaxTx = 320;      // columns of a workgroup (rounded up to whole groups, kClThreads at most)
 constexpr uint32_t kClRows = 2;         // rows a lane uses while as many are on their way
-constexpr uint32_t kClMaxParts = 256;   // parts of a group up to which every workgroup joins them itself (only wide groups have more)
-constexpr uint32_t kClJoinThreads = 256;
+constexpr uint32_t kClMaxParts = 256;   // parts of a group up to which every workgroup joins them itself (groups over more chunks have more)
 constexpr uint32_t kClTeam = 16;        // lanes that add up a group's channels
 constexpr uint32_t kClUnitThreads = 1024;
 constexpr uint32_t kClUnitMaxK = 4;     // most rows a lane holds of a workgroup that has all positions
@@ -551,24 +550,12 @@ __device__ __forceinline__ void join_groups(const ClPlan &p, const ClParts &part
     __syncthreads();
 }
 
-// For more slices than every workgroup should join by itself: a workgroup per group of a sample.
+// For groups over more chunks than every workgroup should join by itself: a wavefront per group of a sample.
 template <bool STATS>
-__global__ __launch_bounds__(kClJoinThreads) void cl_join_kernel(ClParts parts, float2 *joined, float eps, uint32_t vec, ClPlan p) {
-    __shared__ float red[3][kClJoinThreads / kWave];
+__global__ __launch_bounds__(kWave) void cl_join_kernel(ClParts parts, float2 *joined, float eps, uint32_t vec, ClPlan p) {
     const uint32_t b = blockIdx.x / p.groups, g = blockIdx.x - b * p.groups;
-    if (p.spans != 1) {
-        if (threadIdx.x >= kWave) return;
-        const float2 v = join_spread_group<STATS, kWave>(p, parts, vec, b, g, eps, threadIdx.x);
-        if (threadIdx.x == 0) joined[blockIdx.x] = v;
-        return;
-    }
-    const float2 *at = parts.at + (size_t)b * parts.slices * p.groups + g;
-    PartSum<STATS> sum(p, parts, at);
-    sum.add_all(at, threadIdx.x, kClJoinThreads);
-    sum.a = block_sum<kClJoinThreads / kWave>(sum.a, red[0]);
-    sum.q = block_sum<kClJoinThreads / kWave>(sum.q, red[1]);
-    sum.r = block_sum<kClJoinThreads / kWave>(sum.r, red[2]);
-    if (threadIdx.x == 0) joined[blockIdx.x] = sum.value(eps);
+    const float2 v = join_spread_group<STATS, kWave>(p, parts, vec, b, g, eps, threadIdx.x);
+    if (threadIdx.x == 0) joined[blockIdx.x] = v;
 }
 
 // ---------------------------------------------------------------------------
@@ -1198,7 +1185,7 @@ bool slice_plan(ClPlan *p, uint32_t vec, size_t batch) {
     const uint64_t wanted = ((uint64_t)p->positions + (uint64_t)ty * kClRows - 1) / ((uint64_t)ty * kClRows);
     finish_plan(p, tx, ty, (uint32_t)std::min(wanted, most), vec);
     return p->slices <= kClMaxCount && p->chunks <= kClMaxCount && fits_grid(across * p->slices, cl_lanes(*p)) &&
-           (!joins(*p) || fits_grid(batch * p->groups, kClJoinThreads));
+           (!joins(*p) || fits_grid(batch * p->groups, kWave));
 }
 
 size_t partial_floats(const ClPlan &p, size_t batch) { return 2 * batch * p.slices * p.spans * p.groups; }
@@ -1220,7 +1207,7 @@ void with_rows(uint32_t k, F f) {
 
 template <bool STATS>
 float2 *join_launch(const ClPlan &p, const ClParts &parts, float2 *joined, size_t batch, float eps, uint32_t vec, hipStream_t stream) {
-    launch(cl_join_kernel<STATS>, dim3((uint32_t)(batch * p.groups)), dim3(kClJoinThreads), 0, stream, parts, joined, eps, vec, p);
+    launch(cl_join_kernel<STATS>, dim3((uint32_t)(batch * p.groups)), dim3(kWave), 0, stream, parts, joined, eps, vec, p);
     return joined;
 }
 

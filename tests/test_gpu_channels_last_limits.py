@@ -34,3 +34,10 @@ def _check(msd, cuda, b, p, c, groups, half, act, chunk, keep8, seed=0):
 def test_groups_that_fill_a_workgroups_lds(msd, cuda, b, p, c, groups, half):
     for act, chunk, keep8 in ((True, False, False), (False, True, False), (True, True, True)):
         _check(msd, cuda, b, p, c, groups, half, act, chunk, keep8)
+
+
+# more than 256 chunks of 320 columns share a group, whose parts are then joined by a launch of their own
+@pytest.mark.parametrize("b,p,c,groups,half", [(1, 3, 82001, 1, False), (2, 2, 2 * 82001, 2, True), (1, 2, 4 * 82080, 1, False), (2, 1, 8 * 82080, 1, True)])
+def test_groups_over_more_chunks_than_a_workgroup_joins(msd, cuda, b, p, c, groups, half):
+    for act, chunk, keep8 in ((True, True, False), (False, False, True)):
+        _check(msd, cuda, b, p, c, groups, half, act, chunk, keep8)
