@@ -91,13 +91,23 @@ struct ClTile {
 };
 // Rows of the slices, which take turns with blocks of ty.
 struct SliceRows {
-    uint32_t whole, rest, ty;
+    uint32_t each, rest, ty;
     __device__ __forceinline__ SliceRows(uint32_t positions, uint32_t slices, uint32_t ty) : ty(ty) {
-        const uint32_t round = slices * ty, rounds = positions / round;
-        whole = rounds * ty;
-        rest = positions - rounds * round;
+        const uint32_t round = slices * ty;
+        each = positions / round;
+        rest = positions - each * round;
     }
-    __device__ __forceinline__ uint32_t of(uint32_t slice) const { return whole + min(rest - min(rest, slice * ty), ty); }
+    __device__ __forceinline__ uint32_t extra(uint32_t slice) const { return min(rest - min(rest, slice * ty), ty); }
+    __device__ __forceinline__ uint32_t of(uint32_t slice) const { return each * ty + extra(slice); }
+};
+// Rows of the lanes of a column, the same for all columns of a workgroup: `each`, and one more in the first `extra` lanes.
+struct LaneRows {
+    uint32_t extra;
+    float each, more, all;
+    __device__ __forceinline__ LaneRows(uint32_t n, uint32_t extra, uint32_t ty)
+        : extra(extra), each(uniform((float)n)), more(uniform((float)(n + 1))), all(uniform((float)(n * ty + extra))) {}
+    __device__ __forceinline__ float of(uint32_t lane) const { return lane < extra ? more : each; }
+    static __device__ __forceinline__ float uniform(float v) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v))); }
 };
 
 // Groups that have channels in [c0, c1).
@@ -271,26 +281,139 @@ __device__ __forceinline__ void add_rows(float *red, uint32_t stride, uint32_t t
     __syncthreads();
 }
 
-// Mean and squared deviations of every group's part in a workgroup's channels and rows, from the channels' sums of deviations
-// from shift[c] (red: [2][ty][cc], of values and of squares): done(i, mean, m2, channels) by the first lane of a team, for group
-// i of `groups`.  Deviations are taken channel by channel from a value of the channel, so that a mean far from zero costs no
-// digits; the channels, of equal size n, are joined by M2 = sum M2_c + n sum (mean_c - mean)^2.
-template <typename F>
-__device__ __forceinline__ void group_moments(float *red, const float *shift, uint32_t ty, uint32_t cc, uint32_t c0, float n,
-                                              const ClPlan &p, const ClGroups &groups, F done) {
-    const uint32_t stride = ty * cc;
-    add_rows<2>(red, stride, ty, cc);
-    for (uint32_t c = threadIdx.x; c < cc; c += blockDim.x) {
-        const float a = red[c], m2 = fmaf(-a / n, a, red[stride + c]);
-        red[c] = shift[c] + a / n;
-        red[stride + c] = m2 < 0.0f ? 0.0f : m2;  // (NaN stays)
+// Mean and squared deviations of every channel from those of its lanes.  red: [2][ty][cc], the lanes' means and sums of squared
+// deviations from them (SQUARES; otherwise every lane has one row, and there are none); on return row 0 has the channel's.  Two sums
+// one after the other, of the means and of M2_lane + n_lane (mean_lane - mean)^2: nothing is subtracted from a sum, whatever the rows
+// are.  parts: [2][blockDim].
+//
+// `lanes` (a power of two) share a channel: lane j sums rows j, j + lanes, ..., of which HELD stay in registers between the two
+// sums.  As few instructions as that takes: with weights and bounds worked out for each row the sums of 320 channels' slices took 0.5 us
+// more (16 samples of 64 x 64, float16).
+constexpr uint32_t kMostLanes = 16;
+template <bool SQUARES, uint32_t HELD>
+struct ChannelLanes {
+    const float *red;  // of the channel
+    uint32_t stride, ty, cc, j, log_lanes, whole;
+    const LaneRows &rows;
+    float means[HELD], m2s[HELD];
+
+    __device__ __forceinline__ ChannelLanes(const float *red, uint32_t stride, uint32_t ty, uint32_t cc, uint32_t j, uint32_t log_lanes, const LaneRows &rows)
+        : red(red + j * cc), stride(stride), ty(ty), cc(cc), j(j), log_lanes(log_lanes), whole(ty >> log_lanes), rows(rows) {}
+    // f(row, mean, M2) for this lane's rows; `held`: the first are in registers
+    template <typename F>
+    __device__ __forceinline__ void each_row(bool held, F f) {
+        const uint32_t step = cc << log_lanes;
+        const float *at = red;
+#pragma unroll
+        for (uint32_t k = 0; k < HELD; k++) {
+            if (!held && k < whole) {
+                means[k] = at[0];
+                if (SQUARES) m2s[k] = at[stride];
+                at += step;
+            }
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < HELD; k++)
+            if (k < whole) f(j + (k << log_lanes), means[k], SQUARES ? m2s[k] : 0.0f);
+        at = red + HELD * step;
+        for (uint32_t k = HELD; k < whole; k += 4) {
+            float mean[4], m2[4];
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++) {
+                const float *from = at + min(i, whole - 1 - k) * step;
+                mean[i] = from[0];
+                m2[i] = SQUARES ? from[stride] : 0.0f;
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++)
+                if (k + i < whole) f(j + ((k + i) << log_lanes), mean[i], m2[i]);
+            at += 4 * step;
+        }
+        const uint32_t last = j + (whole << log_lanes);
+        if (last < ty) {
+            const float *from = red + whole * step;
+            f(last, from[0], SQUARES ? from[stride] : 0.0f);
+        }
+    }
+    __device__ __forceinline__ float offsets(float pivot) {
+        float sum = 0.0f;
+        each_row(false, [&](uint32_t row, float mean, float) { sum = fmaf(rows.of(row), mean - pivot, sum); });
+        return sum;
+    }
+    __device__ __forceinline__ float squares(float whole_mean) {
+        float sum = 0.0f;
+        each_row(true, [&](uint32_t row, float mean, float m2) {
+            const float d = mean - whole_mean;
+            sum = fmaf(rows.of(row) * d, d, sum);
+            if (SQUARES) sum += m2;
+        });
+        return sum;
+    }
+};
+
+template <bool SQUARES, uint32_t HELD>
+__device__ __forceinline__ void join_lanes(float *red, float *parts, uint32_t ty, uint32_t cc, const LaneRows &rows) {
+    const uint32_t stride = ty * cc, log_lanes = 31 - __builtin_clz(max(min(min(blockDim.x / cc, ty / 4), kMostLanes), 1u)), lanes = 1u << log_lanes;
+    const float one_nth = LaneRows::uniform(1.0f / rows.all);
+    __syncthreads();
+    if (lanes == 1) {
+        for (uint32_t c = threadIdx.x; c < cc; c += blockDim.x) {
+            ChannelLanes<SQUARES, HELD> channel(red + c, stride, ty, cc, 0, 0, rows);
+            const float pivot = red[c], mean = fmaf(channel.offsets(pivot), one_nth, pivot), m2 = channel.squares(mean);
+            red[c] = mean;
+            red[stride + c] = m2;
+        }
+    } else {
+        auto sum_parts = [&](const float *from) {  // [lanes][cc]
+            float v[kMostLanes], sum = 0.0f;
+#pragma unroll
+            for (uint32_t k = 0; k < kMostLanes; k++) {
+                if (k >= lanes) break;
+                v[k] = from[k * cc];
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < kMostLanes; k++) {
+                if (k >= lanes) break;
+                sum += v[k];
+            }
+            return sum;
+        };
+        const uint32_t j = threadIdx.x / cc, c = threadIdx.x - j * cc;
+        ChannelLanes<SQUARES, HELD> channel(red + c, stride, ty, cc, j, log_lanes, rows);
+        float pivot = 0.0f, mean = 0.0f;
+        if (j < lanes) {
+            pivot = red[c];
+            parts[threadIdx.x] = channel.offsets(pivot);
+        }
+        __syncthreads();
+        if (j < lanes) {
+            mean = fmaf(sum_parts(parts + c), one_nth, pivot);
+            parts[blockDim.x + threadIdx.x] = channel.squares(mean);
+        }
+        __syncthreads();
+        if (j == 0) {
+            red[c] = mean;
+            red[stride + c] = sum_parts(parts + blockDim.x + c);
+        }
     }
     __syncthreads();
+}
+
+// Mean and squared deviations of every group's part in a workgroup's channels and rows, from the lanes' (red and parts as for
+// join_lanes): done(i, mean, m2, channels) by the first lane of a team, for group i of `groups`.  The channels, of equal size n,
+// are joined by M2 = sum M2_c + n sum (mean_c - mean)^2.
+template <bool SQUARES, uint32_t HELD, typename F>
+__device__ __forceinline__ void group_moments(float *red, float *parts, uint32_t ty, uint32_t cc, uint32_t c0, const LaneRows &rows,
+                                              const ClPlan &p, const ClGroups &groups, F done) {
+    const uint32_t stride = ty * cc;
+    const float n = rows.all;
+    join_lanes<SQUARES, HELD>(red, parts, ty, cc, rows);
     const uint32_t team = threadIdx.x / kClTeam, lane = threadIdx.x % kClTeam, teams = blockDim.x / kClTeam;
     for (uint32_t i = team; i < groups.count; i += teams) {
         const uint32_t g = groups.first + i;
         const uint32_t lo = max(g * p.per_group.d, c0) - c0, hi = min((g + 1) * p.per_group.d, c0 + cc) - c0;
         constexpr uint32_t kHeld = 5;  // channels a lane keeps in registers between the two sums
+        const float pivot = red[lo];
         float sum = 0.0f, m2 = 0.0f, means[kHeld], m2s[kHeld];
 #pragma unroll
         for (uint32_t k = 0; k < kHeld; k++) {
@@ -299,9 +422,9 @@ __device__ __forceinline__ void group_moments(float *red, const float *shift, ui
             m2s[k] = red[stride + c];
         }
 #pragma unroll
-        for (uint32_t k = 0; k < kHeld; k++) sum += lo + lane + k * kClTeam < hi ? means[k] : 0.0f;
-        for (uint32_t c = lo + lane + kHeld * kClTeam; c < hi; c += kClTeam) sum += red[c];
-        const float mean = team_sum<kClTeam>(sum) / (float)(hi - lo);
+        for (uint32_t k = 0; k < kHeld; k++) sum += lo + lane + k * kClTeam < hi ? means[k] - pivot : 0.0f;
+        for (uint32_t c = lo + lane + kHeld * kClTeam; c < hi; c += kClTeam) sum += red[c] - pivot;
+        const float mean = pivot + team_sum<kClTeam>(sum) / (float)(hi - lo);
 #pragma unroll
         for (uint32_t k = 0; k < kHeld; k++) {
             const float d = means[k] - mean;
@@ -336,16 +459,46 @@ __device__ __forceinline__ void group_sums(const float *va, const float *vb, uin
     }
 }
 
-// Adds a row's deviations from `shift` to the sums.
+// Sums of a lane's rows, channel by channel: deviations from a pivot and their squares.  The pivot is the first row until it moves
+// to the mean of the rows so far.  A lane moves it when it has had 8, 64, 512, ... rows: with n rows in all, of which the pivot is the
+// mean of n / 8 or more, the square that `finish` subtracts is at most 8 times what is left, whatever the rows are (with the
+// slice's first row as the pivot of all, as many times as the slice has rows: a first row of 0 and 65535 of 100 +- 0.01 in each of
+// 16 samples had 1 / sqrt(variance) off by 4.7e-4, now by 6e-7).
 template <int VEC>
-__device__ __forceinline__ void add_moments(const float *f, const float *shift, float *s1, float *s2) {
+struct Moments {
+    float pivot[VEC], s1[VEC], s2[VEC];
+    __device__ __forceinline__ Moments() {
 #pragma unroll
-    for (int e = 0; e < VEC; e++) {
-        const float d = f[e] - shift[e];
-        s1[e] += d;
-        s2[e] = fmaf(d, d, s2[e]);
+        for (int e = 0; e < VEC; e++) pivot[e] = s1[e] = s2[e] = 0.0f;
     }
-}
+    __device__ __forceinline__ void add(const float *f) {
+#pragma unroll
+        for (int e = 0; e < VEC; e++) {
+            const float d = f[e] - pivot[e];
+            s1[e] += d;
+            s2[e] = fmaf(d, d, s2[e]);
+        }
+    }
+    __device__ __forceinline__ void move(float n, float one_nth) {  // to the mean of the n rows that were added
+#pragma unroll
+        for (int e = 0; e < VEC; e++) {
+            const float to = fmaf(s1[e], one_nth, pivot[e]), d = to - pivot[e], rest = fmaf(-n, d, s1[e]);
+            s2[e] = fmaf(-d, s1[e] + rest, s2[e]);
+            s1[e] = rest;
+            pivot[e] = to;
+        }
+    }
+    // s1 and s2 become the mean and the squared deviations from it of n rows (n = 0: nothing)
+    __device__ __forceinline__ void finish(float n) {
+        const float one_nth = 1.0f / fmaxf(n, 1.0f);
+#pragma unroll
+        for (int e = 0; e < VEC; e++) {
+            const float off = s1[e] * one_nth, m2 = fmaf(-off, s1[e], s2[e]);
+            s1[e] = n == 0.0f ? 0.0f : pivot[e] + off;
+            s2[e] = m2 < 0.0f ? 0.0f : m2;  // (NaN stays)
+        }
+    }
+};
 
 // ---------------------------------------------------------------------------
 // Statistics of a slice of positions: partials [batch][slices][spans][groups], (mean, M2).
@@ -354,8 +507,10 @@ __device__ __forceinline__ void add_moments(const float *f, const float *shift, 
 // A lane's walk over its rows first, first + step, ... below `rows`, kClRows at a time and as many on their way.  Requests are made
 // without a branch (behind the last row: the last row again, which is in the cache) and stay in order, so that a use waits for
 // its own request and not for the ones behind it.
-template <typename Stage, typename Request, typename Use>
-__device__ __forceinline__ void walk_rows(uint32_t first, uint32_t step, uint32_t rows, Stage (&stage)[2][kClRows], Request request, Use use) {
+// between(): after every 2 kClRows rows that are not the last.
+template <typename Stage, typename Request, typename Use, typename Between>
+__device__ __forceinline__ void walk_rows(uint32_t first, uint32_t step, uint32_t rows, Stage (&stage)[2][kClRows], Request request, Use use,
+                                          Between between) {
     auto requests = [&](Stage *to, uint32_t row) {
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -373,7 +528,12 @@ __device__ __forceinline__ void walk_rows(uint32_t first, uint32_t step, uint32_
         requests(stage[0], row + 2 * ahead);
         uses(stage[1], row + ahead);
         requests(stage[1], row + 3 * ahead);
+        if (row + 2 * ahead < rows) between();
     }
+}
+template <typename Stage, typename Request, typename Use>
+__device__ __forceinline__ void walk_rows(uint32_t first, uint32_t step, uint32_t rows, Stage (&stage)[2][kClRows], Request request, Use use) {
+    walk_rows(first, step, rows, stage, request, use, [] {});
 }
 template <typename Stage, typename Request>
 __device__ __forceinline__ void first_rows(uint32_t first, uint32_t step, uint32_t rows, Stage (&stage)[2][kClRows], Request request) {
@@ -387,32 +547,37 @@ __global__ __launch_bounds__(kClThreads) void cl_stats_kernel(const T *x, const 
     extern __shared__ float lds[];
     const ClTile t = CL_TILE(VEC, blockIdx.x);
     const uint32_t cc = t.cols * VEC, c0 = t.col0 * VEC;
-    float s1[VEC], s2[VEC], shift[VEC];
-#pragma unroll
-    for (int e = 0; e < VEC; e++) s1[e] = s2[e] = 0.0f;
+    Moments<VEC> m;
     if (t.live) {
         const uint32_t c = c0 + t.tx * VEC;
         const T *at = x + (size_t)t.b * positions * channels + c;
-        Row<T, VEC> r[2][kClRows], first, add;
+        Row<T, VEC> r[2][kClRows], add;
         auto request = [&](Row<T, VEC> &to, uint32_t row) { to.load(at + (size_t)row * channels); };
-        first.load(at + (size_t)(t.slice * ty) * channels);
         if (ADD) add.load(chunk + (size_t)t.b * channels + c);
         first_rows(t.first, t.step, positions, r, request);
+        Row<T, VEC> first = r[0][0];
         if (ADD) first.add(add);
-        first.floats(shift);
+        first.floats(m.pivot);
+        uint32_t rounds = 0, next = 8 / (2 * kClRows);
         walk_rows(t.first, t.step, positions, r, request, [&](Row<T, VEC> &row, uint32_t) {
             if (ADD) row.add(add);
             float f[VEC];
             row.floats(f);
-            add_moments<VEC>(f, shift, s1, s2);
+            m.add(f);
+        }, [&] {
+            if (++rounds != next) return;
+            const float n = (float)(2 * kClRows * rounds);
+            m.move(n, 1.0f / n);
+            next *= 8;
         });
     }
-    float *first_row = lds + 2 * ty * cc;
-    put_channels<VEC>(lds, t, s1);
-    put_channels<VEC>(lds + ty * cc, t, s2);
-    if (t.ty == 0) put_channels<VEC>(first_row, t, shift);
+    const SliceRows of_slices(positions, counts & 0xFFFFu, ty);
+    const LaneRows rows(of_slices.each, of_slices.extra(t.slice), ty);
+    m.finish(rows.of(t.ty));
+    put_channels<VEC>(lds, t, m.s1);
+    put_channels<VEC>(lds + ty * cc, t, m.s2);
     const ClGroups groups(p, c0, c0 + cc);
-    group_moments(lds, first_row, ty, cc, c0, (float)SliceRows(positions, p.slices, ty).of(t.slice), p, groups, [&](uint32_t i, float mean, float m2, float) {
+    group_moments<true, VEC == 8 ? 12 : 8>(lds, lds + 2 * ty * cc, ty, cc, c0, rows, p, groups, [&](uint32_t i, float mean, float m2, float) {
         const uint32_t g = groups.first + i, span = p.spans == 1 ? 0 : t.chunk - g * p.per_group.d / VEC / p.tx;
         partials[(((size_t)t.b * p.slices + t.slice) * p.spans + span) * p.groups + g] = make_float2(mean, m2);
     });
@@ -426,71 +591,121 @@ struct ClParts {  // what a launch of sums left
     uint32_t slices, ty;
 };
 
-// A group's value from the parts of its slices.  Statistics: means by their distance from the first slice's, which costs no
-// digits; M2 = sum of the parts' M2 and of their n times the squared distance of their mean from the whole's.
-template <bool STATS>
-struct PartSum {
-    const ClPlan &p;
-    const ClParts &parts;
-    const SliceRows rows;
-    float shift, a = 0.0f, q = 0.0f, r = 0.0f;
-    __device__ __forceinline__ PartSum(const ClPlan &p, const ClParts &parts, const float2 *first)
-        : p(p), parts(parts), rows(p.positions, parts.slices, parts.ty), shift(STATS ? first->x : 0.0f) {}
-    // slices s, s + step, ...: twelve requests under way at a time
-    __device__ __forceinline__ void add_all(const float2 *at, uint32_t first, uint32_t step) {
-        constexpr uint32_t kBatch = 12;
-        for (uint32_t s = first; s < parts.slices; s += kBatch * step) {
-            float2 v[kBatch];
-#pragma unroll
-            for (uint32_t k = 0; k < kBatch; k++) v[k] = at[(size_t)min(s + k * step, parts.slices - 1) * p.groups];
-#pragma unroll
-            for (uint32_t k = 0; k < kBatch; k++)
-                if (s + k * step < parts.slices) add(s + k * step, v[k]);
-        }
-    }
-    __device__ __forceinline__ void add(uint32_t s, float2 v) {
-        if (STATS) {
-            const float w = (float)rows.of(s), d = v.x - shift;
-            a = fmaf(w, d, a);
-            r = fmaf(w * d, d, r);
-        } else {
-            a += v.x;
-        }
-        q += v.y;
-    }
-    __device__ __forceinline__ float2 value(float eps) const {
-        const float count = (float)p.positions, per = (float)p.per_group.d;
-        if (!STATS) return make_float2(a / (count * per), q / (count * per));
-        const float off = a / count, m2 = fmaf(per, fmaf(-off, a, r), q);  // (off: the mean's distance from the shift)
-        return make_float2(shift + off, 1.0f / sqrtf((m2 < 0.0f ? 0.0f : m2) / (count * per) + eps));
+// Mean and squared deviations of `weight` positions of a group of `per` channels.
+struct PartMoments {
+    float weight = 0.0f, mean = 0.0f, m2 = 0.0f;
+    __device__ __forceinline__ void join(const PartMoments &o, float per) {
+        const float both = weight + o.weight, share = weight > 0.0f ? o.weight * __builtin_amdgcn_rcpf(both) : 1.0f, d = o.mean - mean;
+        m2 += fmaf(per * weight * share * d, d, o.m2);
+        mean = fmaf(share, d, mean);
+        weight = both;
     }
 };
 
-// By the 32 lanes of every half wavefront, one a group; they share the slices.  red: [blockDim / 64][3][32].
+// A lane's part of a group's slices, slices first, first + step, ...: kBatch requests under way at a time.  Statistics: the mean of
+// a batch, by the distance from its first, the squared deviations from that mean, and then the batches are joined; no sum has
+// another subtracted from it.  Sums (of a gradient): added up.
+constexpr uint32_t kBatch = 12;
+__device__ __forceinline__ void part_batch(const ClPlan &p, const ClParts &parts, const float2 *at, uint32_t s, uint32_t step, float2 *v) {
+#pragma unroll
+    for (uint32_t k = 0; k < kBatch; k++) v[k] = at[(size_t)min(s + k * step, parts.slices - 1) * p.groups];
+}
+__device__ __forceinline__ PartMoments part_moments(const ClPlan &p, const ClParts &parts, const float2 *at, uint32_t first, uint32_t step) {
+    const SliceRows rows(p.positions, parts.slices, parts.ty);
+    const float per = (float)p.per_group.d;
+    PartMoments all;
+    for (uint32_t s = first; s < parts.slices; s += kBatch * step) {
+        float2 v[kBatch];
+        float w[kBatch], off = 0.0f;
+        part_batch(p, parts, at, s, step, v);
+        PartMoments batch;
+#pragma unroll
+        for (uint32_t k = 0; k < kBatch; k++) {
+            w[k] = s + k * step < parts.slices ? (float)rows.of(s + k * step) : 0.0f;
+            batch.weight += w[k];
+            off = fmaf(w[k], v[k].x - v[0].x, off);
+        }
+        batch.mean = fmaf(off, __builtin_amdgcn_rcpf(batch.weight), v[0].x);  // (every slice has a row)
+#pragma unroll
+        for (uint32_t k = 0; k < kBatch; k++) {
+            const float d = v[k].x - batch.mean;
+            batch.m2 += s + k * step < parts.slices ? fmaf(per * w[k] * d, d, v[k].y) : 0.0f;
+        }
+        all.join(batch, per);
+    }
+    return all;
+}
+__device__ __forceinline__ float2 part_sums(const ClPlan &p, const ClParts &parts, const float2 *at, uint32_t first, uint32_t step) {
+    float2 all = make_float2(0.0f, 0.0f);
+    for (uint32_t s = first; s < parts.slices; s += kBatch * step) {
+        float2 v[kBatch];
+        part_batch(p, parts, at, s, step, v);
+#pragma unroll
+        for (uint32_t k = 0; k < kBatch; k++) {
+            all.x += s + k * step < parts.slices ? v[k].x : 0.0f;
+            all.y += s + k * step < parts.slices ? v[k].y : 0.0f;
+        }
+    }
+    return all;
+}
+
+// By the 32 lanes of every half wavefront, one a group; they share the slices.  red: [kClThreads / 64][3][32].
 template <bool STATS>
 __device__ __forceinline__ void join_whole_groups(const ClPlan &p, const ClParts &parts, uint32_t b, const ClGroups &groups, float eps,
                                                   float2 *of_group, float (*red)[3][32]) {
-    const uint32_t lane = threadIdx.x % 32, half = threadIdx.x / 32, halves = blockDim.x / 32;
+    constexpr uint32_t kWaves = kClThreads / kWave;
+    const uint32_t lane = threadIdx.x % 32, half = threadIdx.x / 32, halves = blockDim.x / 32, wave = threadIdx.x / kWave;
+    const float count = (float)p.positions, per = (float)p.per_group.d;
     for (uint32_t g0 = 0; g0 < groups.count; g0 += 32) {
         const float2 *at = parts.at + (size_t)b * parts.slices * p.groups + groups.first + min(g0 + lane, groups.count - 1);
-        PartSum<STATS> sum(p, parts, at);
-        sum.add_all(at, half, halves);
-        sum.a = half_pair_sum(sum.a);
-        sum.q = half_pair_sum(sum.q);
-        if (STATS) sum.r = half_pair_sum(sum.r);
-        if (threadIdx.x % kWave < 32) {
-            red[threadIdx.x / kWave][0][lane] = sum.a;
-            red[threadIdx.x / kWave][1][lane] = sum.q;
-            red[threadIdx.x / kWave][2][lane] = sum.r;
+        if constexpr (STATS) {
+            PartMoments mine = part_moments(p, parts, at, half, halves), other;
+            other.weight = half_swap(mine.weight);
+            other.mean = half_swap(mine.mean);
+            other.m2 = half_swap(mine.m2);
+            mine.join(other, per);
+            if (threadIdx.x % kWave < 32) {
+                red[wave][0][lane] = mine.weight;
+                red[wave][1][lane] = mine.mean;
+                red[wave][2][lane] = mine.m2;
+            }
+        } else {
+            const float2 mine = part_sums(p, parts, at, half, halves);
+            const float a = half_pair_sum(mine.x), q = half_pair_sum(mine.y);
+            if (threadIdx.x % kWave < 32) {
+                red[wave][0][lane] = a;
+                red[wave][1][lane] = q;
+            }
         }
         __syncthreads();
         if (threadIdx.x < 32 && g0 + lane < groups.count) {
-            for (uint32_t w = 1; w < blockDim.x / kWave; w++) {
-                sum.a += red[w][0][lane];
-                sum.q += red[w][1][lane];
-                sum.r += red[w][2][lane];
+            const uint32_t waves = blockDim.x / kWave;
+            if constexpr (STATS) {  // as in part_moments; wavefronts without slices have the weight 0
+                float w[kWaves], mean[kWaves], m2[kWaves], off = 0.0f, sum = 0.0f;
+#pragma unroll
+                for (uint32_t k = 0; k < kWaves; k++) {
+                    const uint32_t from = min(k, waves - 1);
+                    w[k] = k < waves ? red[from][0][lane] : 0.0f;
+                    mean[k] = red[from][1][lane];
+                    m2[k] = red[from][2][lane];
+                }
+#pragma unroll
+                for (uint32_t k = 0; k < kWaves; k++) off = fmaf(w[k], mean[k] - mean[0], off);
+                const float whole = mean[0] + off / count;
+#pragma unroll
+                for (uint32_t k = 0; k < kWaves; k++) {
+                    const float d = mean[k] - whole;
+                    sum += k < waves ? fmaf(per * w[k] * d, d, m2[k]) : 0.0f;
+                }
+                of_group[g0 + lane] = make_float2(whole, 1.0f / sqrtf(sum / (count * per) + eps));
+            } else {
+                float a = 0.0f, q = 0.0f;
+                for (uint32_t w = 0; w < waves; w++) {
+                    a += red[w][0][lane];
+                    q += red[w][1][lane];
+                }
+                of_group[g0 + lane] = make_float2(a / (count * per), q / (count * per));
             }
-            of_group[g0 + lane] = sum.value(eps);
         }
         __syncthreads();
     }
@@ -516,12 +731,13 @@ __device__ __forceinline__ float2 join_spread_group(const ClPlan &p, const ClPar
         return (float)rows.of(s) * (float)(min(hi, c0 + chunk_channels) - max(lo, c0));
     };
     float a = 0.0f, q = 0.0f;
+    const float pivot = STATS ? part(0).x : 0.0f;
     for (uint32_t i = lane; i < count; i += TEAM) {
         const float2 v = part(i);
-        a = STATS ? fmaf(v.x, size(i) / total, a) : a + v.x;
+        a = STATS ? fmaf(v.x - pivot, size(i) / total, a) : a + v.x;
         q += v.y;
     }
-    a = sum_over<TEAM>(a);
+    a = pivot + sum_over<TEAM>(a);
     if (STATS) {
         q = 0.0f;
         for (uint32_t i = lane; i < count; i += TEAM) {
@@ -632,10 +848,12 @@ __global__ __launch_bounds__(kClThreads) void cl_apply_kernel(const T *x, const 
     });
 }
 
-// LDS of cl_unit_kernel, in floats: two sums [ty][cc] and the first row [cc]; then, where a float2 may begin, the groups' statistics.
+// LDS of cl_unit_kernel, in floats: the lanes' means and squared deviations [2][ty][cc], what join_lanes needs, and the groups'
+// statistics, where a float2 may begin.
 struct UnitLds {
-    uint32_t first_row, of_group;
-    __host__ __device__ constexpr UnitLds(uint32_t ty, uint32_t cc) : first_row(2 * ty * cc), of_group((first_row + cc + 1) / 2 * 2) {}
+    uint32_t parts, of_group;
+    __host__ __device__ constexpr UnitLds(uint32_t block, uint32_t ty, uint32_t cc)
+        : parts(2 * ty * cc), of_group(parts + 2 * block) {}
     constexpr size_t bytes(size_t groups) const { return of_group * sizeof(float) + groups * sizeof(float2); }
 };
 
@@ -650,44 +868,43 @@ __global__ __launch_bounds__(kClUnitThreads) void cl_unit_kernel(const T *x, con
     const ClTile t = CL_TILE(VEC, blockIdx.x);
     const uint32_t c0 = t.col0 * VEC, cc = t.cols * VEC, c = c0 + t.tx * VEC;
     const size_t base = (size_t)t.b * positions * channels + c;
-    Row<T, VEC> r[K], first;
+    Row<T, VEC> r[K];
     Affine<VEC> affine;
-    float s1[VEC], s2[VEC], shift[VEC];
+    uint32_t each = 0;
 #pragma unroll
-    for (int e = 0; e < VEC; e++) s1[e] = s2[e] = 0.0f;
+    for (int i = 1; i <= K; i++) each += i * ty <= positions ? 1 : 0;
+    const LaneRows rows(each, positions - each * ty, ty);
+    Moments<VEC> m;
     if (t.live) {
 #pragma unroll
         for (int i = 0; i < K; i++) r[i].load(x + base + min(t.ty + i * ty, positions - 1) * channels);
-        first.load(x + base);
         if (chunk != nullptr) {
             Row<T, VEC> add;
             add.load(chunk + (size_t)t.b * channels + c);
             affine.request(gamma, beta, c);
-            first.add(add);
 #pragma unroll
             for (int i = 0; i < K; i++) r[i].add(add);
         } else {
             affine.request(gamma, beta, c);
         }
-        first.floats(shift);
+        r[0].floats(m.pivot);  // (every lane has a row)
 #pragma unroll
-        for (int i = 0; i < K; i++) {
+        for (int i = 1; i < K; i++) {
             if (t.ty + i * ty < positions) {
                 float f[VEC];
                 r[i].floats(f);
-                add_moments<VEC>(f, shift, s1, s2);
+                m.add(f);
             }
         }
     }
-    const UnitLds at_lds(ty, cc);
-    float *first_row = lds + at_lds.first_row;
+    m.finish(rows.of(t.ty));
+    const UnitLds at_lds(blockDim.x, ty, cc);
     float2 *of_group = reinterpret_cast<float2 *>(lds + at_lds.of_group);
-    put_channels<VEC>(lds, t, s1);
-    put_channels<VEC>(lds + ty * cc, t, s2);
-    if (t.ty == 0) put_channels<VEC>(first_row, t, shift);
+    put_channels<VEC>(lds, t, m.s1);
+    if (K > 1) put_channels<VEC>(lds + ty * cc, t, m.s2);
     const ClGroups groups(p, c0, c0 + cc);
     const float n = (float)positions;
-    group_moments(lds, first_row, ty, cc, c0, n, p, groups, [&](uint32_t i, float mean, float m2, float members) {
+    group_moments<(K > 1), 8>(lds, lds + at_lds.parts, ty, cc, c0, rows, p, groups, [&](uint32_t i, float mean, float m2, float members) {
         const float2 v = make_float2(mean, 1.0f / sqrtf(m2 / (n * members) + eps));
         of_group[i] = v;
         if (stats != nullptr) stats[(size_t)t.b * p.groups + groups.first + i] = v;
@@ -1149,7 +1366,7 @@ size_t chunk_channels(const ClPlan &p, uint32_t vec) { return (size_t)std::min(p
 size_t unit_lds(const ClPlan &p, uint32_t vec, bool backward) {
     const uint32_t cc = (uint32_t)chunk_channels(p, vec);
     const size_t groups = cc / p.per_group.d;
-    return backward ? UnitGradsLds(p.ty, cc).bytes(groups) : UnitLds(p.ty, cc).bytes(groups);
+    return backward ? UnitGradsLds(p.ty, cc).bytes(groups) : UnitLds(cl_lanes(p), p.ty, cc).bytes(groups);
 }
 
 // (a gradient holds two rows for one: of 8 channels each, no more than two fit the registers)
@@ -1240,7 +1457,7 @@ int cl_forward(ClPlan p, const ClForward &a, size_t batch, float eps, bool silu,
     const dim3 grid((uint32_t)(batch * p.chunks * p.slices)), block(cl_lanes(p));
     const size_t cc = chunk_channels(p, VEC);
     with_flag(chunk != nullptr, [&](auto add) {
-        launch(cl_stats_kernel<T, VEC, add.value>, grid, block, (2 * p.ty + 1) * cc * sizeof(float), stream, x, chunk, CL_GEOMETRY_OF(p),
+        launch(cl_stats_kernel<T, VEC, add.value>, grid, block, 2 * (p.ty * cc + block.x) * sizeof(float), stream, x, chunk, CL_GEOMETRY_OF(p),
                partials, p);
     });
     if (joins(p)) {

@@ -141,6 +141,11 @@ __device__ __forceinline__ float row_pair_sum(float v) {
     const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
+// The value of the lane 32 away.
+__device__ __forceinline__ float half_swap(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(threadIdx.x % 64 < 32 ? r[1] : r[0]);
+}
 __device__ __forceinline__ float half_pair_sum(float v) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
