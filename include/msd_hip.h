@@ -371,9 +371,11 @@ int msd_linear_rows_grouped(const void *x, const void *const *weights, const flo
  *   packed  [n, k / 2] bytes, the code (0 ... 15) of an even k in the low half of its byte and that
  *           of the next k in the high half
  *   scales  [n, k / group] in the storage type `dtype`; group is 32, 64 or 128 and divides k
- * Everything else as for msd_linear_rows and msd_linear_rows_grouped, m <= 8 included; products and
- * sums are float32, and a row has the same bits whatever rows and whatever layers come with it, as
- * long as the operands' alignment is the same (16 bytes for x and packed is the fast one).
+ * Everything else as for msd_linear_rows and msd_linear_rows_grouped, m <= 8 included; a row has the
+ * same bits whatever rows and whatever layers come with it, as long as the operands' alignment is the
+ * same.  Sums are float32.  With x and packed at multiples of 16 bytes (the fast alignment) and k from 128
+ * to 2^22, a float32 or activated x enters the products as two float16, off by at most 2^-23 of its value
+ * whatever the sizes of the values beside it; otherwise as it is.
  *   msd_q4_pack  makes codes and scales of a weight w [n, k] in the storage type: with a = the
  *           largest finite |w| of a group, scale = a / 7 rounded to the storage type and code =
  *           round(w * (1 / scale)) (to even, clamped to +-7) + 8; a < 1e-30 or a scale of 0: the

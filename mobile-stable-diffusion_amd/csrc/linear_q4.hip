@@ -79,8 +79,9 @@ __global__ __launch_bounds__(kQ4Threads) void linear_q4_generic_kernel(const T *
 // float16, and so are the products and, to float32, their sums; the scale of a group multiplies the sum of its products, not
 // the weights.  Of the 16 rows 8 are those of x; where x is float32, or activated, they hold its upper 11 bits and the other
 // 8 rows, which would stand empty, the next 11, the 128 values of a row and step being brought to the range of float16 by a
-// power of two.  What is left out is at most 2^-22 of a value, to either side alike: less than the roundings of a float32 sum
-// of k products leave (against 64 bits, k = 2048: 1.3e-7, torch's float32 product 4e-7).
+// power of two.  What is left out of a value is at most 2^-23 of it, as two roundings of float32 would leave out, down to 2^-26 of the
+// largest of the 128 (Q4Scale); what the float16 of smaller ones lack is found again behind the steps and summed up in float32.  The sums
+// are closer than a float32 sum of k products (against 64 bits, k = 2048: 1.3e-7, torch's float32 product 4e-7).
 //
 // Weights: a lane loads 16 bytes, 32 of its column's weights; the four lanes of a column then swap 4-byte pieces so that each
 // instruction gets 32 neighbouring ones, which never mix two scales.  Within a piece, codes come out in pairs (0, 4), (1, 5),
@@ -147,8 +148,6 @@ struct XPair<__half> {
     }
 };
 
-__device__ __forceinline__ uint32_t half_pair(_Float16 lo, _Float16 hi) { return __builtin_bit_cast(uint32_t, f16x2{lo, hi}); }
-
 // Between LDS accesses of some lanes of a wavefront and those of others to the same place: the hardware keeps their order, this
 // makes the compiler keep it.  (Fences of the wavefront's scope and its barrier cost 3 % at 16384 x 8192, 8 rows float16: they end what
 // can be scheduled together.)
@@ -170,6 +169,80 @@ struct Q4Stage {
     T scale[CT][NS];
     XPair<T> raw[PAIRS][2];
 };
+
+// Maximum over 32 lanes of values that are not less than zero, whose order is that of their bits: as floats, the compiler makes each of
+// them canonical before it compares (22 instructions in place of 9).
+__device__ __forceinline__ float half_wave_max(float v) {
+    uint32_t u = __float_as_uint(v);
+    u = max(u, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, kDppXor1, 0xF, 0xF, true));
+    u = max(u, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, kDppXor2, 0xF, 0xF, true));
+    u = max(u, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, kDppHalfMirror, 0xF, 0xF, true));
+    u = max(u, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, kDppRowMirror, 0xF, 0xF, true));
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    return __uint_as_float(max(r[0], r[1]));
+}
+
+// How a row's 128 values of a step become two float16 each, from the largest of them: times 2^(141 - exponent), which brings that to
+// 2^14 ... 2^15.  From 2^26 times less on a value is off by 2^-23 of itself at most; below `smallest` the float16 run out of digits.
+struct Q4Scale {
+    float up, factor, smallest;  // factor: 1 / up, of which the products are multiples
+    __device__ __forceinline__ explicit Q4Scale(float most) {
+        constexpr uint32_t kBand = 26;
+        const uint32_t exponent = max(__float_as_uint(most) >> 23, 20u);
+        up = __uint_as_float((268u - exponent) << 23);
+        factor = __uint_as_float((exponent - 14u) << 23);
+        smallest = __uint_as_float((max(exponent, kBand) - kBand) << 23);
+    }
+    // of two values; lo times 2048
+    __device__ __forceinline__ void split(float f, float g, f16x2 &hi, f16x2 &lo) const {
+        hi = f16x2{(_Float16)(f * up), (_Float16)(g * up)};
+        const float r = fmaf(f, up, -(float)hi[0]), s = fmaf(g, up, -(float)hi[1]);
+        lo = f16x2{(_Float16)(r * 2048.0f), (_Float16)(s * 2048.0f)};
+        lo = __builtin_elementwise_max(lo, f16x2{-16384.0f, -16384.0f});  // (never less than that; of an infinity: not NaN)
+    }
+    // what the two float16 of values below `smallest` lack of them (exactly: they have the upper digits), else 0
+    __device__ __forceinline__ void lacks(float &f, float &g) const {
+        f16x2 hi, lo;
+        split(f, g, hi, lo);
+        f = fabsf(f) < smallest ? f - fmaf((float)lo[0], 1.0f / 2048.0f, (float)hi[0]) * factor : 0.0f;
+        g = fabsf(g) < smallest ? g - fmaf((float)lo[1], 1.0f / 2048.0f, (float)hi[1]) * factor : 0.0f;
+    }
+};
+
+// What the two float16 of the smaller ones of a row's 128 values of a step lack, times a column's weights, in float32; x: the lane's 32 of
+// them (`none`: of none).
+template <typename T, int NS, int CT>
+__device__ __forceinline__ void q4_small_values(const T *x, bool none, int act_in, const Q4Scale &to_halves, const uint8_t *packed,
+                                                const uint32_t *code_at, const char *scales, const uint32_t *scale_at, float *sum) {
+    auto value = [&](uint32_t e) {
+        const float v = none ? 0.0f : Store<T>::load1(x + e);
+        return act_in ? silu_f(v) : v;
+    };
+#pragma unroll
+    for (int c = 0; c < CT; c++) sum[c] = 0.0f;
+#pragma unroll 1
+    for (uint32_t e0 = 0; e0 < 32; e0 += 8) {
+        float f[8];
+#pragma unroll
+        for (uint32_t e = 0; e < 8; e += 2) {
+            f[e] = value(e0 + e);
+            f[e + 1] = value(e0 + e + 1);
+            to_halves.lacks(f[e], f[e + 1]);
+        }
+#pragma unroll
+        for (int c = 0; c < CT; c++) {
+            const uint32_t codes = *reinterpret_cast<const uint32_t *>(packed + code_at[c] + e0 / 2);
+            const float scale = Store<T>::load1(reinterpret_cast<const T *>(scales + scale_at[c]));
+#pragma unroll
+            for (uint32_t e = 0; e < 8; e++) sum[c] = fmaf(f[e], (float)((int)((codes >> (4 * e)) & 15u) - 8) * scale, sum[c]);
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < CT; c++) {  // of the four lanes of the column
+        sum[c] += __shfl_xor(sum[c], 16);
+        sum[c] += __shfl_xor(sum[c], 32);
+    }
+}
 
 // SPLIT: two float16 for a value of x.  NS: scales per step (128 / group).  PAIRS: of rows of x that there is room for.
 template <typename T, bool SPLIT, int NS, int CT, int PAIRS>
@@ -229,9 +302,12 @@ __device__ __forceinline__ void linear_q4_body(const T *x, const Q4Layer &layer,
     f32x4 acc[CT];
 #pragma unroll
     for (int c = 0; c < CT; c++) acc[c] = f32x4{0, 0, 0, 0};
+    uint64_t lost = 0;  // bit i: in the wavefront's steps i, i + 64, ... are values whose float16 lack digits
+    uint32_t turn = 0;
     auto multiply = [&](Stage &from, uint32_t step) {
         const uint32_t had = step * kMmStep - start(step);  // values of the step that count as zeros
         uint2 *to = reinterpret_cast<uint2 *>(mine);
+        uint64_t met = 0;  // lanes that have met such values
 #pragma unroll
         for (int u = 0; u < PAIRS; u++) {
             if (2 * u >= (int)m) break;
@@ -240,34 +316,32 @@ __device__ __forceinline__ void linear_q4_body(const T *x, const Q4Layer &layer,
             if constexpr (SPLIT) {
                 const float2 first = from.raw[u][0].floats(), second = from.raw[u][1].floats();
                 float f[4] = {first.x, first.y, second.x, second.y};
-                if (had != 0) {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) f[e] = none ? 0.0f : f[e];
-                }
+                for (int e = 0; e < 4; e++) f[e] = none ? 0.0f : f[e];
                 if (act_in) {
 #pragma unroll
                     for (int e = 0; e < 4; e++) f[e] = silu_f(f[e]);
                 }
                 // (an infinity here leaves nothing but infinities and NaN of its row, which it gives whatever the others are)
-                const float most = team_max<32>(fmaxf(fmaxf(fabsf(f[0]), fabsf(f[1])), fmaxf(fabsf(f[2]), fabsf(f[3]))));
-                const uint32_t exponent = max(__float_as_uint(most) >> 23, 20u);  // most * 2^(141 - exponent) < 2^15
-                const float up = __uint_as_float((268u - exponent) << 23);
-                _Float16 hi[4], lo[4];
+                const float most = half_wave_max(fmaxf(fmaxf(fabsf(f[0]), fabsf(f[1])), fmaxf(fabsf(f[2]), fabsf(f[3]))));
+                const Q4Scale scale(most);
+                uint32_t least = ~0u;  // of twice the bits less one, of which zeros have the largest
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float s = f[e] * up;
-                    hi[e] = (_Float16)s;
-                    lo[e] = (_Float16)(fmaxf(s - (float)hi[e], -8.0f) * 2048.0f);  // (never less than -8; of an infinity: not NaN)
-                }
-                to[at] = make_uint2(half_pair(hi[0], hi[2]), half_pair(hi[1], hi[3]));
-                to[at + 2 * m] = make_uint2(half_pair(lo[0], lo[2]), half_pair(lo[1], lo[3]));
-                if (tl == 0) factors[row] = __uint_as_float((exponent - 14u) << 23);
+                for (int e = 0; e < 4; e++) least = min(least, (__float_as_uint(f[e]) << 1) - 1);
+                f16x2 hi[2], lo[2];  // (0, 2) and (1, 3): the order of the codes
+                scale.split(f[0], f[2], hi[0], lo[0]);
+                scale.split(f[1], f[3], hi[1], lo[1]);
+                met |= __ballot(least < __float_as_uint(scale.smallest) << 1);
+                to[at] = make_uint2(__builtin_bit_cast(uint32_t, hi[0]), __builtin_bit_cast(uint32_t, hi[1]));
+                to[at + 2 * m] = make_uint2(__builtin_bit_cast(uint32_t, lo[0]), __builtin_bit_cast(uint32_t, lo[1]));
+                if (tl == 0) factors[row] = scale.factor;
             } else {
                 const uint32_t v = __builtin_amdgcn_perm(from.raw[u][1].v, from.raw[u][0].v, 0x05040100u);
                 const uint32_t w = __builtin_amdgcn_perm(from.raw[u][1].v, from.raw[u][0].v, 0x07060302u);
                 to[at] = none ? make_uint2(0, 0) : make_uint2(v, w);
             }
         }
+        lost |= (uint64_t)(met != 0) << (turn++ % 64);
         lanes_in_step();
         f16x8 a[4];
 #pragma unroll
@@ -307,6 +381,33 @@ __device__ __forceinline__ void linear_q4_body(const T *x, const Q4Layer &layer,
             const uint32_t step = first + d * waves;
             if (step < steps) multiply(stage[d], step);
             request(stage[d], min(step + kAhead * waves, last));  // (past the end: what is in the cache)
+        }
+    }
+
+    if constexpr (SPLIT) {
+        // Rarely: steps once more, for the rows that have such values there (16384 x 8192, 8 rows float32: 2.7 us more for one value, and
+        // 379 in place of 28 where every row has them in every step).
+        turn = 0;
+        for (uint32_t step = wave; lost != 0 && step < steps; step += waves) {
+            if ((lost >> (turn++ % 64) & 1) == 0) continue;
+            const uint32_t at = start(step), had = step * kMmStep - at;
+            for (uint32_t row = 0; row < m; row++) {
+                XPair<T> raw;
+                raw.load(x + (size_t)row * k + at + 2 * lane);
+                float2 f = 2 * lane < had ? make_float2(0.0f, 0.0f) : raw.floats();
+                if (act_in) f = make_float2(silu_f(f.x), silu_f(f.y));
+                const float most = half_wave_max(fmaxf(fabsf(f.x), fabsf(f.y)));
+                const Q4Scale to_halves(fmaxf(most, __shfl_xor(most, 32)));
+                auto small = [&](float v) { return v != 0.0f && fabsf(v) < to_halves.smallest; };
+                if (__ballot(small(f.x) || small(f.y)) == 0) continue;
+                float sum[CT];
+                q4_small_values<T, NS, CT>(x + (size_t)row * k + at + q * 32, q * 32 < had, act_in, to_halves, packed + at / 2, code_at,
+                                           scales + (size_t)(at / kGroup + q * 32 / kGroup) * sizeof(T), scale_at, sum);
+#pragma unroll
+                for (int c = 0; c < CT; c++)
+#pragma unroll
+                    for (uint32_t r = 0; r < 4; r++) acc[c][r] += row == 4 * q + r ? sum[c] : 0.0f;
+            }
         }
     }
 
