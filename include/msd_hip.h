@@ -200,8 +200,8 @@ int msd_groupnorm_tokens_workspace(const void *x, void *y, const float *gamma, c
  *   code_scales  MSD_CODE_BLOCK)] float: the normalised tensor (x, or x + chunk) in 8 bits.  The
  *                channels of a position are cut into blocks of MSD_CODE_BLOCK; with a = the
  *                largest finite |value| of a block, code = round(value * (127 * (1 / a))) (to
- *                even, clamped to +-127) and scale = a * (1 / 127), every step rounded to
- *                float32; a < 1e-30: all zero.
+ *                even, clamped to +-127; NaN: -127) and scale = a * (1 / 127), every step
+ *                rounded to float32; a < 1e-30: all zero, whatever else is in the block.
  * workspace: 8-byte aligned device memory of at least the bytes that
  * msd_groupnorm_channels_last_workspace reports (backward = 0), apart from all else; its contents need
  * not be set, are left undefined, and belong to this call until it (or every replay of it) is

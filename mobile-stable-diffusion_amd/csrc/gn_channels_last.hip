@@ -183,6 +183,7 @@ __device__ __forceinline__ float finite_abs(float v) {
 __device__ __forceinline__ float code_inverse(float most) { return most < kCodeTiny ? 0.0f : 127.0f * (1.0f / most); }
 __device__ __forceinline__ float code_scale(float most) { return most < kCodeTiny ? 0.0f : most * (1.0f / 127.0f); }
 __device__ __forceinline__ int code_of(float h, float inv) {
+    if (inv == 0.0f) return 0;  // (of infinities and NaN too)
     return (int)fminf(fmaxf(__builtin_rintf(h * inv), -127.0f), 127.0f);
 }
 

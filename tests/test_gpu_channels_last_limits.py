@@ -41,3 +41,20 @@ def test_groups_that_fill_a_workgroups_lds(msd, cuda, b, p, c, groups, half):
 def test_groups_over_more_chunks_than_a_workgroup_joins(msd, cuda, b, p, c, groups, half):
     for act, chunk, keep8 in ((True, True, False), (False, False, True)):
         _check(msd, cuda, b, p, c, groups, half, act, chunk, keep8)
+
+
+@pytest.mark.parametrize("half", [False, True], ids=["f32", "f16"])
+@pytest.mark.parametrize("c", [64, 72])
+def test_blocks_of_nothing_but_zeros_infinities_and_nan_have_codes_of_zero(msd, cuda, c, half):
+    import torch
+    x, _, gamma, beta, _ = _inputs(torch, 2, 5, c, half, False)
+    x[0, 1, 32:64], x[1, 2, 32:64], x[1, 3, 32:64] = 0.0, 0.0, 0.0
+    x[0, 1, 40], x[1, 2, 33], x[1, 3, 63] = float("inf"), float("nan"), float("-inf")
+    _, kept = msd.groupnorm_channels_last_kept(x.to(cuda), gamma.to(cuda), beta.to(cuda), c // 8, keep8=True)
+    codes, scales = kept.codes.cpu(), kept.scales.cpu()
+    for b, p in ((0, 1), (1, 2), (1, 3)):
+        assert not bool(codes[b, p, 32:64].any()) and float(scales[b, p, 1]) == 0.0
+    want = plain.checkpoint(x.double())
+    others = torch.ones((2, 5, c), dtype=torch.bool)
+    others[0, 1, 32:64] = others[1, 2:4, 32:64] = False
+    assert torch.equal(codes[others], want[0][others]) and torch.equal(scales, want[1])
