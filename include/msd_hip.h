@@ -378,8 +378,8 @@ int msd_linear_rows_grouped(const void *x, const void *const *weights, const flo
  * whatever the sizes of the values beside it; otherwise as it is.
  *   msd_q4_pack  makes codes and scales of a weight w [n, k] in the storage type: with a = the
  *           largest finite |w| of a group, scale = a / 7 rounded to the storage type and code =
- *           round(w * (1 / scale)) (to even, clamped to +-7) + 8; a < 1e-30 or a scale of 0: the
- *           scale is 0 and the codes are 8.  packed and scales lie apart from w and each other.
+ *           round(w * (1 / scale)) (to even, clamped to +-7; NaN: -7) + 8; a < 1e-30 or a scale of 0:
+ *           the scale is 0 and the codes are 8, infinities and NaN among them or not.  packed and scales lie apart from w and each other.
  * n and k are at most 2^28 (a launch of 2^32 lanes is refused).  No counterpart in the reference, whose
  * weights are float32.
  */

@@ -27,7 +27,9 @@ __global__ __launch_bounds__(kPackThreads) void q4_pack_kernel(const T *w, uint8
         const float most = team_max<kLanes>(fmaxf(fa < inf ? fa : 0.0f, fb < inf ? fb : 0.0f));
         const float scale = most < kPackTiny ? 0.0f : round_to_storage<T>(most / 7.0f);
         const float inv = scale > 0.0f ? 1.0f / scale : 0.0f;
-        auto code = [inv](float v) { return (uint32_t)((int)fminf(fmaxf(__builtin_rintf(v * inv), -7.0f), 7.0f) + 8); };
+        auto code = [inv](float v) {  // (a scale of 0: 8, of infinities and NaN too)
+            return inv > 0.0f ? (uint32_t)((int)fminf(fmaxf(__builtin_rintf(v * inv), -7.0f), 7.0f) + 8) : 8u;
+        };
         packed[i] = (uint8_t)(code(a) | code(b) << 4);
         if (threadIdx.x % kLanes == 0) Store<T>::store1(scales + i / kLanes, scale);
     }

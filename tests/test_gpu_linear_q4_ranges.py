@@ -90,3 +90,16 @@ def test_small_values_in_one_step_of_one_row(msd, cuda, k):
         mine[:, at] = 8
         layer = (mine, scales, None)
         _check(_call(msd, cuda, x, layer), x, layer, 0, 0, "part %d" % part)
+
+
+@pytest.mark.parametrize("half", [False, True], ids=["f32", "f16"])
+def test_packing_groups_of_nothing_but_zeros_infinities_and_nan(msd, cuda, half):
+    import torch
+    w = _rows(torch, 5, 128, half, 70)
+    w[1:4, 32:64] = 0.0
+    w[1, 40], w[2, 33], w[3, 63] = float("inf"), float("nan"), float("-inf")
+    packed, scales = msd.q4_pack(w.to(cuda), 32)
+    assert bool((packed.cpu()[1:4, 16:32] == 0x88).all()) and not bool(scales.cpu()[1:4, 1].any())
+    codes, want = plain.pack(w, 32)
+    codes[1:4, 32:64] = 8
+    assert torch.equal(packed.cpu(), plain.bytes_of(codes)) and torch.equal(scales.cpu(), want)
