@@ -372,8 +372,8 @@ int msd_linear_rows_grouped(const void *x, const void *const *weights, const flo
  *           of the next k in the high half
  *   scales  [n, k / group] in the storage type `dtype`; group is 32, 64 or 128 and divides k
  * Everything else as for msd_linear_rows and msd_linear_rows_grouped, m <= 8 included; a row has the
- * same bits whatever rows and whatever layers come with it, as long as the operands' alignment is the
- * same.  Sums are float32.  With x and packed at multiples of 16 bytes (the fast alignment) and k from 128
+ * same bits whatever rows and whatever layers come with it, as long as the alignment of x and of its own
+ * layer is the same.  Sums are float32.  With x and packed at multiples of 16 bytes (the fast alignment) and k from 128
  * to 2^22, a float32 or activated x enters the products as two float16, off by at most 2^-23 of its value
  * whatever the sizes of the values beside it; otherwise as it is.
  *   msd_q4_pack  makes codes and scales of a weight w [n, k] in the storage type: with a = the

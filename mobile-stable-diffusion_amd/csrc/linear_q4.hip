@@ -518,21 +518,11 @@ int linear_q4_dispatch(const void *x, const uint8_t *const *packed, const void *
     if (m == 0) return MSD_OK;
     const T *rows = static_cast<const T *>(x);
     auto bias_of = [&](size_t i) { return biases != nullptr ? biases[i] : nullptr; };
+    // Each layer by its own alignment, so that its bits and its time are the same whatever layers come with it.
+    const bool fast_rows = aligned16(x) && k >= kMmStep && k <= (size_t)1 << 22;  // (offsets within a workgroup's columns: 32 bits)
+    auto fast = [&](size_t i) { return ns[i] != 0 && fast_rows && aligned16(packed[i]); };
     size_t tiles = 0;
-    bool aligned = aligned16(x) && k >= kMmStep && k <= (size_t)1 << 22;  // (offsets within a workgroup's columns: 32 bits)
-    for (size_t i = 0; i < count; i++) {
-        if (ns[i] == 0) continue;
-        tiles += (ns[i] + kMmTile - 1) / kMmTile;
-        aligned = aligned && aligned16(packed[i]);
-    }
-    if (!aligned) {
-        for (size_t i = 0; i < count; i++)
-            if (ns[i] != 0)
-                launch(linear_q4_generic_kernel<T>, dim3((uint32_t)std::min<size_t>(kQ4MaxBlocks, (ns[i] + kQ4Threads / kWave - 1) / (kQ4Threads / kWave))),
-                       dim3(kQ4Threads), 0, stream, rows, packed[i], static_cast<const T *>(scales[i]), bias_of(i),
-                       static_cast<T *>(ys[i]), (uint32_t)m, (uint32_t)ns[i], (uint32_t)k, (uint32_t)group, act_in, act_out);
-        return launch_status();
-    }
+    for (size_t i = 0; i < count; i++) tiles += fast(i) ? (ns[i] + kMmTile - 1) / kMmTile : 0;
     // Wavefronts: as many as share the steps evenly, eight at most, so that several workgroups share a CU.  Tiles per workgroup: more
     // of them share the work on x, as long as 160 workgroups are left; of one or two rows that work is little.  us, one tile / two /
     // four, fp16, k = 1280: 2560 columns, 1 row 2.5 3.0 3.9, 8 rows 3.2 3.8 4.6; 5120, 8 rows 3.9 3.5 4.8; 10240, 1 row 3.8 4.1 4.0,
@@ -543,7 +533,7 @@ int linear_q4_dispatch(const void *x, const uint8_t *const *packed, const void *
     const size_t columns = (size_t)kMmTile * ct;
     auto blocks_of = [&](size_t i) { return (ns[i] + columns - 1) / columns; };
     for (size_t i = 0; i < count; i++)
-        if (blocks_of(i) > kQ4MaxBlocks) return MSD_ERR_INVALID_VALUE;
+        if (fast(i) && blocks_of(i) > kQ4MaxBlocks) return MSD_ERR_INVALID_VALUE;
     Q4Layers layers{};
     uint32_t held = 0;
     auto send = [&] {
@@ -555,6 +545,12 @@ int linear_q4_dispatch(const void *x, const uint8_t *const *packed, const void *
     };
     for (size_t i = 0; i < count; i++) {
         if (ns[i] == 0) continue;
+        if (!fast(i)) {
+            launch(linear_q4_generic_kernel<T>, dim3((uint32_t)std::min<size_t>(kQ4MaxBlocks, (ns[i] + kQ4Threads / kWave - 1) / (kQ4Threads / kWave))),
+                   dim3(kQ4Threads), 0, stream, rows, packed[i], static_cast<const T *>(scales[i]), bias_of(i),
+                   static_cast<T *>(ys[i]), (uint32_t)m, (uint32_t)ns[i], (uint32_t)k, (uint32_t)group, act_in, act_out);
+            continue;
+        }
         if (held == kQ4GroupMax || layers.first_block[held] + blocks_of(i) > kQ4MaxBlocks) send();
         const uint32_t blocks = layers.first_block[held] + (uint32_t)blocks_of(i);
         layers.layer[held++] = {packed[i], scales[i], bias_of(i), ys[i], (uint32_t)ns[i]};

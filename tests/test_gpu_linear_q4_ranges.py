@@ -103,3 +103,19 @@ def test_packing_groups_of_nothing_but_zeros_infinities_and_nan(msd, cuda, half)
     codes, want = plain.pack(w, 32)
     codes[1:4, 32:64] = 8
     assert torch.equal(packed.cpu(), plain.bytes_of(codes)) and torch.equal(scales.cpu(), want)
+
+
+@pytest.mark.parametrize("half", [False, True], ids=["f32", "f16"])
+def test_a_layer_of_another_alignment_leaves_the_others_as_they_are(msd, cuda, half):
+    import torch
+    layers = [_layer(torch, n, 640, 64, half, 80 + n, False) for n in (320, 33, 640)]
+    x = _rows(torch, 5, 640, half, 81).to(cuda)
+    packed, scales = [plain.bytes_of(c).to(cuda) for c, _, _ in layers], [s.to(cuda) for _, s, _ in layers]
+    alone = [msd.linear_rows_q4(x, p, s) for p, s in zip(packed, scales)]
+    for i in range(3):
+        moved = list(packed)
+        moved[i] = torch.empty(packed[i].numel() + 1, dtype=torch.uint8, device=cuda)[1:].view(packed[i].shape).copy_(packed[i])
+        got = msd.linear_rows_q4_grouped(x, moved, scales)
+        assert all(torch.equal(a, b) for k, (a, b) in enumerate(zip(got, alone)) if k != i), i
+        assert torch.equal(got[i], msd.linear_rows_q4(x, moved[i], scales[i]))
+        _check(got[i], x.cpu(), layers[i], 0, 0, "moved %d" % i)
