@@ -462,7 +462,7 @@ def groupnorm_channels_last_backward(dy, kept, affine=True, out=None):
     tp = _affine(kept.stats, 2 * batch * kept.groups, dy, "stats")
     dgamma = dbeta = dchunk = None
     if affine:
-        dgamma, dbeta = _torch.empty_like(kept.gamma), _torch.empty_like(kept.beta)
+        dgamma, dbeta = (dy.new_empty(channels, dtype=_torch.float32) for _ in range(2))
     if kept.with_chunk:
         dchunk = dy.new_empty((batch, channels))
     size = _channels_last_workspace(batch, positions, channels, kept.groups, code, 1)

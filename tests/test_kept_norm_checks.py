@@ -90,3 +90,20 @@ def test_refused_on_the_device_too(msd, cuda):
                    dict(codes=kept.codes.cpu())):
         with pytest.raises(msd.MsdError):
             msd.groupnorm_channels_last_backward(x, kept._replace(**change))
+
+
+def test_gradients_of_gamma_and_beta_are_vectors_whatever_theirs_are(msd, library):
+    kept = _kept(msd, 2, 5, 48, 8, False)
+    kept = kept._replace(gamma=kept.gamma.view(1, 48, 1), beta=kept.beta.view(48, 1))
+    _, dgamma, dbeta, _ = msd.groupnorm_channels_last_backward(_on(torch.zeros(2, 5, 48)), kept)
+    assert dgamma.shape == dbeta.shape == (48,) and dgamma.dtype == dbeta.dtype == torch.float32
+
+
+@pytest.mark.gpu
+def test_gradients_of_gamma_and_beta_are_vectors_on_both_paths(msd, cuda, monkeypatch):
+    x, g = torch.randn(2, 5, 48, device=cuda), torch.ones(1, 48, 1, device=cuda)
+    _, kept = msd.groupnorm_channels_last_kept(x, g, g, 8)
+    first = msd.groupnorm_channels_last_backward(x, kept)
+    monkeypatch.setattr(msd, "_native_cl_q4", msd._NoNative())
+    second = msd.groupnorm_channels_last_backward(x, kept)
+    assert all(a.shape == b.shape and torch.equal(a, b) for a, b in zip(first[:3], second[:3])) and first[1].shape == (48,)
