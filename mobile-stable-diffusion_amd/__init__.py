@@ -356,6 +356,11 @@ def _channels_last(x, what="x"):
     raise MsdError("%s must be [batch, C, H, W] in torch.channels_last order or a contiguous [batch, positions, C]" % what)
 
 
+def _groups_fit(groups, channels):
+    if groups <= 0 or channels % groups:
+        raise MsdError("groups must divide the channels (got %d, %d)" % (groups, channels))
+
+
 def _same_layout(t, like, what):
     """An operand laid out as `like`, which _channels_last has checked."""
     if t.shape != like.shape or t.dtype != like.dtype:
@@ -391,8 +396,7 @@ def _channels_last_forward(x, gamma, beta, groups, eps, fuse_silu, chunk, out, s
     yp = _same_layout(out, x, "out")
     cp = _same(chunk, x, batch * channels, "chunk") if chunk is not None else None
     gp, bp = _affine(gamma, channels, x, "gamma"), _affine(beta, channels, x, "beta")
-    if groups <= 0 or channels % groups:
-        raise MsdError("groups must divide the channels (got %d, %d)" % (groups, channels))
+    _groups_fit(groups, channels)
     size = _channels_last_workspace(batch, positions, channels, groups, code, 0)
     workspace = x.new_empty(size, dtype=_torch.uint8)
     check(lib.msd_groupnorm_channels_last(x.data_ptr(), cp, yp, gp, bp, batch, positions, channels, groups, eps, int(fuse_silu), code,
@@ -423,8 +427,7 @@ def groupnorm_channels_last_kept(x, gamma, beta, groups, eps=1e-5, fuse_silu=Fal
     if out is not None and not keep8 and out.data_ptr() == x.data_ptr() and x.numel():
         raise MsdError("out must not be x unless keep8: the gradient needs x")
     torch = _torch
-    if groups <= 0:
-        raise MsdError("groups must be positive")
+    _groups_fit(groups, channels)
     stats = x.new_empty((batch, groups, 2), dtype=torch.float32)
     codes = scales = None
     if keep8:

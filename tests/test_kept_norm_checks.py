@@ -107,3 +107,12 @@ def test_gradients_of_gamma_and_beta_are_vectors_on_both_paths(msd, cuda, monkey
     monkeypatch.setattr(msd, "_native_cl_q4", msd._NoNative())
     second = msd.groupnorm_channels_last_backward(x, kept)
     assert all(a.shape == b.shape and torch.equal(a, b) for a, b in zip(first[:3], second[:3])) and first[1].shape == (48,)
+
+
+@pytest.mark.parametrize("groups", [0, -8, 7, 96, 10 ** 13])
+def test_groups_that_do_not_divide_the_channels_are_refused_before_anything_is_allocated(msd, library, groups):
+    x, g = _on(torch.zeros(2, 5, 48)), _on(torch.ones(48))
+    for call in (lambda: msd.groupnorm_channels_last_kept(x, g, g, groups), lambda: msd.groupnorm_channels_last_kept(x, g, g, groups, keep8=True),
+                 lambda: msd.groupnorm_channels_last(x, g, g, groups)):
+        with pytest.raises(msd.MsdError):
+            call()
