@@ -415,9 +415,9 @@ def groupnorm_channels_last(x, gamma, beta, groups, eps=1e-5, fuse_silu=False, c
 
 
 def groupnorm_channels_last_kept(x, gamma, beta, groups, eps=1e-5, fuse_silu=False, chunk=None, keep8=False, out=None):
-    """groupnorm_channels_last, and a KeptNorm for groupnorm_channels_last_backward.  It holds x and chunk, which must not
-    change until then (out must not be x), or with keep8 their sum in 8 bits, a quarter of float32 and a half of float16
-    (out may be x)."""
+    """groupnorm_channels_last, and a KeptNorm for groupnorm_channels_last_backward.  It holds gamma and beta, and x and chunk (out
+    must not be x) or, with keep8, the sum of these two in 8 bits, a quarter of float32 and a half of float16 (out may be x).
+    What it holds must not change until then."""
     done = _native_cl_q4.groupnorm_channels_last_kept(x, gamma, beta, groups, eps, fuse_silu, chunk, out, keep8)
     if done is not None:
         y, codes, scales, stats = done

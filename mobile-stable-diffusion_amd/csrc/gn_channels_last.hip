@@ -17,8 +17,8 @@
 // over slices of the positions and a launch that joins them and applies them.
 //
 // What bounds it: the memory, whose copies reach 6.7 TB/s here (1 GiB), and for halves with SiLU the vector instructions.  Passes
-// in a captured graph, us: 320 channels at 64 x 64 float16, 2 samples 11.6, 16 samples 26.6 (read twice, written once: 4.7 TB/s);
-// 128 at 512 x 512 float32 67 (6.0 TB/s); forward and gradient of 320 at 64 x 64, 8 samples float16 43, 16 samples by way of the 8-bit
+// in a captured graph, us: 320 channels at 64 x 64 float16, 2 samples 11.5, 16 samples 27.0 (read twice, written once: 4.7 TB/s);
+// 128 at 512 x 512 float32 67.7 (5.9 TB/s); forward and gradient of 320 at 64 x 64, 8 samples float16 43, 16 samples by way of the 8-bit
 // codes 77; of 640 at 32 x 32, 4 samples float32, codes, 31.  No atomics: sums have one order.
 #include "msd_device.h"
 #include "msd_internal.h"
@@ -33,7 +33,7 @@ namespace msd {
 namespace {
 
 // Slices, as passes in a graph, us: 320 channels at 64 x 64 float16, 2 samples / the same, forward and gradient, 8 samples / 128 at
-// 512 x 512 float32.  512 lanes, 256 workgroups, 2 rows: 11.6, 43, 67.  512 workgroups 14.1, 50, 74; 1024 lanes 14.6, 51, 71: more
+// 512 x 512 float32 (when channels were joined in one sum).  512 lanes, 256 workgroups, 2 rows: 11.6, 43, 67.  512 workgroups 14.1, 50, 74; 1024 lanes 14.6, 51, 71: more
 // of either pay for more sums to join and for rows in flight that the memory does not need.  1 row at a time 11.6, 43, 69; with
 // codes 1 row is 4 % faster in float32 (29.3 against 30.6 at 640 channels) and 4 % slower in float16 (79.6 against 76.7).
 constexpr uint32_t kClThreads = 512;    // most lanes of a workgroup that has a slice of the positions
@@ -503,7 +503,9 @@ struct Moments {
 
 // ---------------------------------------------------------------------------
 // Statistics of a slice of positions: partials [batch][slices][spans][groups], (mean, M2).
-// A read of x: 134 MB of float32 (128 channels at 512 x 512) in 22.8 us, 5.9 TB/s, against 6.1 to 7.1 of a plain read.
+// A read of x: 134 MB of float32 (128 channels at 512 x 512) in 23.8 us, 5.6 TB/s, against 6.1 to 7.1 of a plain read; three quarters of
+// a wavefront's cycles are waits for it.  The joining at the end counts where there are many channels: 320 at 64 x 64 float16, 16
+// samples in 10 us, of which its second sum is 0.4.
 // ---------------------------------------------------------------------------
 // A lane's walk over its rows first, first + step, ... below `rows`, kClRows at a time and as many on their way.  Requests are made
 // without a branch (behind the last row: the last row again, which is in the cache) and stay in order, so that a use waits for
@@ -780,8 +782,8 @@ __global__ __launch_bounds__(kWave) void cl_join_kernel(ClParts parts, float2 *j
 // `joined`: the statistics, where cl_join_kernel has been there.  `stats`: receives them, or null.
 // The first rows are on their way while a workgroup joins the slices for itself, which saves a launch for that.
 // 134 MB of float32 in and out in 42.9 us, 6.3 TB/s; results leave past the caches, where x stays (a pass of 128 channels at
-// 512 x 512: 73 us in place of 86, in a state of the kernels before the 67).  With codes the vector instructions bound it: some 20 an element, of which SiLU's exponential and reciprocal
-// count four each; 16 samples of 320 at 64 x 64 float16 in 21.4 us, 4.9 TB/s.
+// 512 x 512: 73 us in place of 86, in a state of the kernels before the 67).  With codes the vector instructions bound it, four fifths of the SIMDs' cycles: some 20 an element, of which
+// SiLU's exponential and reciprocal count four each; 16 samples of 320 at 64 x 64 float16 in 21.4 us, 4.9 TB/s.
 // ---------------------------------------------------------------------------
 // A lane's constants, channel by channel: z = (h - mean) mul + off.
 template <int VEC>
@@ -859,8 +861,8 @@ struct UnitLds {
 };
 
 // The whole of it where a workgroup has all positions of its chunk (whole groups): K rows a lane.  Latency bounds it: a load, the
-// sums through LDS, a store.  Passes in a graph, us, so and in slices: 1280 channels at 8 x 8 float16 5.6 and 9.9, at 16 x 16, 2
-// samples (K = 4) 7.5 and 10.9; with the gradient 19.1 and 24.0, of 2560 at 9 x 7 float32 (K = 2) 12.9 and 19.7.
+// sums through LDS, a store.  Passes in a graph, us, so and in slices: 1280 channels at 8 x 8 float16 5.4 and 10.4, at 16 x 16, 2
+// samples (K = 2) 7.8 and 11.1; with the gradient 19.2 and 23.9, of 2560 at 9 x 7 float32 (K = 2) 13.1 and 19.4.
 template <typename T, int VEC, int K, bool KEEP>
 __global__ __launch_bounds__(kClUnitThreads) void cl_unit_kernel(const T *x, const T *chunk, CL_GEOMETRY, const float *gamma,
                                                                  const float *beta, T *y, float2 *stats, int8_t *codes, float *scales,
@@ -1042,7 +1044,8 @@ __device__ __forceinline__ float chunk_gradient(float2 stat, float gamma, float 
 
 // Sums over a slice of positions: per channel S1, S2 and sum_p u (channel_sums [batch][slices][3][channels]), per group
 // sum gamma dz and sum gamma dz u (partials, as in cl_stats_kernel).  z is computed again, not kept: it costs instructions, 16 an
-// element of which two count four, and they bound it (16 samples of 320 at 64 x 64, float16 from codes: 20 us, 63 MB).
+// element of which two count four.  16 samples of 320 at 64 x 64, float16 from codes: 63 MB in 20 us, of which the SIMDs issue vector
+// instructions three quarters; the rest both wavefronts of a SIMD wait, for memory or a result.
 template <typename T, int VEC, int FROM, bool SILU>
 __global__ __launch_bounds__(kClThreads) void cl_sums_kernel(const T *dy, const void *h, const void *more, CL_GEOMETRY, const float2 *stats,
                                                              const float *gamma, const float *beta, float2 *partials,
@@ -1167,7 +1170,7 @@ __device__ __forceinline__ void channel_grads(const ClChannelGrads &a, uint32_t 
 
 // dx of a slice, after the join of the sums as in cl_apply_kernel, and in its first workgroups the channels' gradients (a launch of
 // their own took 31 us at 8 samples of 320 channels; here they run beside the rest).  16 samples of 320 at 64 x 64, float16 from codes:
-// 105 MB in 21.6 us, the instructions (16 an element) again.
+// 105 MB in 21.6 us, for the same instructions (16 an element) and waits.
 template <typename T, int VEC, int FROM, bool SILU>
 __global__ __launch_bounds__(kClThreads) void cl_dx_kernel(const T *dy, const void *h, const void *more, CL_GEOMETRY, uint32_t channel_blocks,
                                                            const float2 *stats, const float *gamma, const float *beta, T *dx,
