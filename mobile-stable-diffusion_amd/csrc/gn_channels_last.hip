@@ -300,7 +300,7 @@ struct ChannelLanes {
 
     __device__ __forceinline__ ChannelLanes(const float *red, uint32_t stride, uint32_t ty, uint32_t cc, uint32_t j, uint32_t log_lanes, const LaneRows &rows)
         : red(red + j * cc), stride(stride), ty(ty), cc(cc), j(j), log_lanes(log_lanes), whole(ty >> log_lanes), rows(rows) {}
-    // f(row, mean, M2) for this lane's rows; `held`: the first are in registers
+    // f(i, row, mean, M2) for this lane's rows, i = 0 ... 3 in turn; `held`: the first are in registers
     template <typename F>
     __device__ __forceinline__ void each_row(bool held, F f) {
         const uint32_t step = cc << log_lanes;
@@ -315,7 +315,7 @@ struct ChannelLanes {
         }
 #pragma unroll
         for (uint32_t k = 0; k < HELD; k++)
-            if (k < whole) f(j + (k << log_lanes), means[k], SQUARES ? m2s[k] : 0.0f);
+            if (k < whole) f(k % 4, j + (k << log_lanes), means[k], SQUARES ? m2s[k] : 0.0f);
         at = red + HELD * step;
         for (uint32_t k = HELD; k < whole; k += 4) {
             float mean[4], m2[4];
@@ -327,28 +327,29 @@ struct ChannelLanes {
             }
 #pragma unroll
             for (uint32_t i = 0; i < 4; i++)
-                if (k + i < whole) f(j + ((k + i) << log_lanes), mean[i], m2[i]);
+                if (k + i < whole) f(i, j + ((k + i) << log_lanes), mean[i], m2[i]);
             at += 4 * step;
         }
         const uint32_t last = j + (whole << log_lanes);
         if (last < ty) {
             const float *from = red + whole * step;
-            f(last, from[0], SQUARES ? from[stride] : 0.0f);
+            f(0, last, from[0], SQUARES ? from[stride] : 0.0f);
         }
     }
+    // (four sums: an addition in four waits for the one before, and has that much fewer roundings in front of it)
     __device__ __forceinline__ float offsets(float pivot) {
-        float sum = 0.0f;
-        each_row(false, [&](uint32_t row, float mean, float) { sum = fmaf(rows.of(row), mean - pivot, sum); });
-        return sum;
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        each_row(false, [&](uint32_t i, uint32_t row, float mean, float) { sum[i] = fmaf(rows.of(row), mean - pivot, sum[i]); });
+        return (sum[0] + sum[1]) + (sum[2] + sum[3]);
     }
     __device__ __forceinline__ float squares(float whole_mean) {
-        float sum = 0.0f;
-        each_row(true, [&](uint32_t row, float mean, float m2) {
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        each_row(true, [&](uint32_t i, uint32_t row, float mean, float m2) {
             const float d = mean - whole_mean;
-            sum = fmaf(rows.of(row) * d, d, sum);
-            if (SQUARES) sum += m2;
+            sum[i] = fmaf(rows.of(row) * d, d, sum[i]);
+            if (SQUARES) sum[i] += m2;
         });
-        return sum;
+        return (sum[0] + sum[1]) + (sum[2] + sum[3]);
     }
 };
 
@@ -366,7 +367,7 @@ __device__ __forceinline__ void join_lanes(float *red, float *parts, uint32_t ty
         }
     } else {
         auto sum_parts = [&](const float *from) {  // [lanes][cc]
-            float v[kMostLanes], sum = 0.0f;
+            float v[kMostLanes], sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (uint32_t k = 0; k < kMostLanes; k++) {
                 if (k >= lanes) break;
@@ -375,9 +376,9 @@ __device__ __forceinline__ void join_lanes(float *red, float *parts, uint32_t ty
 #pragma unroll
             for (uint32_t k = 0; k < kMostLanes; k++) {
                 if (k >= lanes) break;
-                sum += v[k];
+                sum[k % 4] += v[k];
             }
-            return sum;
+            return (sum[0] + sum[1]) + (sum[2] + sum[3]);
         };
         const uint32_t j = threadIdx.x / cc, c = threadIdx.x - j * cc;
         ChannelLanes<SQUARES, HELD> channel(red + c, stride, ty, cc, j, log_lanes, rows);
