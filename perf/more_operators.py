@@ -309,13 +309,13 @@ def _own(s):
             out["dpositions"] = d_positions
         return out
     if kind == "norm_train":
-        out, d_sum = {}, None
+        out, x, d_sum = {}, s["x"], None
         if case["add"]:
-            d_sum = s["dsum"]
-            out["sum"], out["y"], kept = msd.add_layernorm_kept(s["x"], s["residual"], s["gamma"], s["beta"], EPS)
+            x, out["y"] = msd.add_layernorm(x, s["residual"], s["gamma"], s["beta"], EPS)
+            out["sum"], d_sum = x, s["dsum"]
         else:
-            out["y"], kept = msd.layernorm_kept(s["x"], s["gamma"], s["beta"], EPS)
-        out["dx"], out["dgamma"], out["dbeta"] = msd.layernorm_backward(s["dy"], kept, d_sum)
+            out["y"] = msd.layernorm(x, s["gamma"], s["beta"], EPS)
+        out["dx"], out["dgamma"], out["dbeta"] = msd.layernorm_backward(s["dy"], x, s["gamma"], EPS, d_sum)
         return out
     args = (s["q"], s["k"], s["v"], case["causal"], _scale(case), s["offsets"], s["offsets_k"])
     if kind == "attend":
