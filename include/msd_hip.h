@@ -255,6 +255,44 @@ int msd_layernorm(const void *x, void *y, const float *gamma, const float *beta,
                   size_t dim, float eps, int dtype, void *stream);
 
 /*
+ * Gradient of msd_layernorm, or of the norm in msd_add_layernorm (x is then the sum that it stored): with
+ * u = (x - mean) / sqrt(var + eps) and w = dy gamma, both over a row,
+ *   dx = (w - mean(w) - u mean(w u)) / sqrt(var + eps) (+ dsum), rounded once to the storage type;
+ *   dgamma = sum over the rows of dy u, dbeta = sum of dy: [dim] float32, both or both NULL.
+ * dsum [rows, dim] (or NULL) is the gradient that comes back to x past the norm: that of msd_add_layernorm's
+ * `sum`; dx is then the gradient of both of its addends.  dx may alias dy or dsum exactly.  mean and var are formed
+ * from x again, so x is all that the forward call leaves behind.  Sums are float32, added in a fixed order without atomics:
+ * the same bits every time, in a capture too.  No rows: dgamma and dbeta are set to zero.
+ * workspace: 16-byte aligned device memory of at least the bytes that msd_layernorm_backward_workspace reports (host
+ * only), apart from all else; its contents need not be set, are left undefined, and belong to this call until it (or every
+ * replay of it) is done.  No counterpart in the reference, which has no gradients.
+ */
+int msd_layernorm_backward_workspace(size_t rows, size_t dim, int dtype, size_t *bytes);
+int msd_layernorm_backward(const void *dy, const void *x, const void *dsum, const float *gamma, void *dx, float *dgamma,
+                           float *dbeta, size_t rows, size_t dim, float eps, int dtype, void *workspace, size_t workspace_bytes,
+                           void *stream);
+
+/*
+ * Token embedding, the input of a text encoder (the gather and the positional add of M/TextEncoder.cpp:127 in
+ * one launch): y[i] = scale * table[ids[i]] + positions[i % length] for i < tokens, rounded once.  ids int64, table [vocab, dim]
+ * and y [tokens, dim] in the storage type; positions [length, dim] (more rows may follow) or NULL; length divides tokens.  A token
+ * outside [0, vocab) stands for a row of zeros.  y lies apart from all inputs.
+ *   msd_token_embedding_backward  dtable[v] = scale * sum of dy[i] over the tokens with ids[i] = v, every row of
+ *           [vocab, dim] written (zeros where no token names it); dpositions [positions, dim] = sum of dy[i] over the tokens at a
+ *           position, zeros from `length` on; positions = 0 and dpositions = NULL: not wanted.  Tokens outside [0, vocab) add
+ *           nothing to dtable.  Sums are float32, a token's rows added in a fixed order, and rounded once to the storage type: the
+ *           same bits every time.  workspace as for msd_layernorm_backward.
+ * At most 2^25 tokens, 2^28 rows, 2^20 columns, and fewer than 2^31 values in `length` (and in `positions`) rows.
+ */
+int msd_token_embedding(const int64_t *ids, const void *table, const void *positions, void *y, size_t tokens, size_t length,
+                        size_t vocab, size_t dim, float scale, int dtype, void *stream);
+int msd_token_embedding_backward_workspace(size_t tokens, size_t length, size_t vocab, size_t positions, size_t dim, int dtype,
+                                           size_t *bytes);
+int msd_token_embedding_backward(const int64_t *ids, const void *dy, void *dtable, void *dpositions, size_t tokens, size_t length,
+                                 size_t vocab, size_t positions, size_t dim, float scale, int dtype, void *workspace,
+                                 size_t workspace_bytes, void *stream);
+
+/*
  * The two additions the reference runs right before its norms, and their fusions.
  *   msd_elemwise_add   c[i] = a[i] + b[i]                 K/util.cl:1-12 (the residual adds
  *                      of M/nn/BasicTransformerBlock.cpp:126-134,149-156,170-177)
@@ -403,6 +441,49 @@ int msd_linear_rows_q4_grouped(const void *x, const uint8_t *const *packed, cons
  */
 int msd_softmax(const void *x, void *y, size_t rows, size_t cols, int stable, int dtype,
                 void *stream);
+
+/*
+ * Attention: out_i = sum_j p_ij v_j with p_i = softmax over the keys j that query i sees of scale * q_i . k_j.  Replaces the
+ * products and the softmax of CrossAttention::forward (M/nn/CrossAttention.cpp:362-377 and the matmuls around it) in one
+ * launch (two where few rows read many keys) that stores no scores.
+ *   q, out [batch][q_rows][heads][dim], k, v [batch][k_rows][kv_heads][dim] in the storage type, dim from 1 to 128, heads a
+ *   multiple of kv_heads: heads / kv_heads neighbouring query heads share a key head.
+ *   strides: host array of (batch, row, head) strides in elements for q, k, v, out in turn (the values of a head lie together),
+ *   or NULL: as listed, without gaps.  Views of one projection are fine, also for outputs: one is apart from an input or from another
+ *   output too where both have the same batch and row strides and their heads lie beside each other in a row.
+ *   Packed sequences: q_offsets and k_offsets, device arrays of batch + 1 ascending int32 (both or neither): sequence b has
+ *   the rows offsets[b] ... offsets[b + 1] - 1; q_rows and k_rows are then all rows, batch strides do not count, and rows
+ *   of no sequence stay as they were.  Lengths may be zero and differ between queries and keys.  Offsets are read on the device:
+ *   what lies outside the tensors is cut off, sequences that overlap give undefined values.
+ *   causal != 0: the last query sees every key, the one before all but the last, ...: i sees j <= i + (keys - queries).
+ *   scale: positive and finite.
+ * A row that sees no key, or whose scores are all -infinity, gives zeros.  What a row does not see has no part in it, infinities
+ * and NaN included.  Scores, maxima and sums are float32; float16 weights are rounded to float16 for the product with v.
+ *   lse    NULL, or float32 [rows of q][heads]: log2 of the sum of exp(scale q . k) (-infinity for a row that sees nothing),
+ *          kept for msd_attention_backward.
+ * workspace: 16-byte aligned device memory of at least the bytes that msd_attention_workspace reports (host only; dtype as for
+ * the call; backward = 0), apart from all else; its contents need not be set, are left undefined, and belong to this call until it (or every
+ * replay of it) is done.  The call allocates nothing and gives the same bits every time, in a capture too.
+ * At most 2^27 rows times heads of queries and of keys, and 2^22 sequences times kv_heads.
+ */
+int msd_attention_workspace(size_t batch, size_t q_rows, size_t k_rows, size_t heads, size_t kv_heads, size_t dim, int packed,
+                            int backward, int dtype, size_t *bytes);
+int msd_attention(const void *q, const void *k, const void *v, void *out, float *lse, const int32_t *q_offsets,
+                  const int32_t *k_offsets, size_t batch, size_t q_rows, size_t k_rows, size_t heads, size_t kv_heads, size_t dim,
+                  const size_t *strides, float scale, int causal, int dtype, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * Gradient of msd_attention: from dout (as out), the forward call's q, k, v, out and lse: dq (as q), dk and dv (as k), the
+ * gradients of shared key heads summed over their query heads.  strides: as above for q, k, v, out, dout, dq, dk, dv in turn.
+ * Rows that see nothing give zeros and add nothing, rows of no sequence stay as they were.  Sums are float32 in a fixed order
+ * without atomics, the same bits every time; float16 weights and score gradients are rounded to float16 for their products,
+ * the latter scaled by a power of two that keeps small gradients' digits.  workspace as above (backward = 1).
+ * No counterpart in the reference, which has no gradients.
+ */
+int msd_attention_backward(const void *dout, const void *q, const void *k, const void *v, const void *out, const float *lse,
+                           void *dq, void *dk, void *dv, const int32_t *q_offsets, const int32_t *k_offsets, size_t batch,
+                           size_t q_rows, size_t k_rows, size_t heads, size_t kv_heads, size_t dim, const size_t *strides,
+                           float scale, int causal, int dtype, void *workspace, size_t workspace_bytes, void *stream);
 
 /*
  * DDIM sampler arithmetic (M/DDIMSampler.cpp).  Host only:

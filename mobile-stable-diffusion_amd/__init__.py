@@ -39,7 +39,10 @@ C_ABI_SYMBOLS = (
     "msd_elemwise_add", "msd_chunkwise_add", "msd_chunk_add_groupnorm", "msd_add_layernorm", "msd_copy",
     "msd_groupnorm_tokens", "msd_groupnorm_tokens_workspace", "msd_permute_0_2_1",
     "msd_groupnorm_channels_last", "msd_groupnorm_channels_last_workspace", "msd_groupnorm_channels_last_backward",
-    "msd_linear_rows", "msd_linear_rows_grouped", "msd_q4_pack", "msd_linear_rows_q4", "msd_linear_rows_q4_grouped", "msd_softmax", "msd_alphas_cumprod", "msd_ddim_schedule", "msd_ddim_update",
+    "msd_linear_rows", "msd_linear_rows_grouped", "msd_q4_pack", "msd_linear_rows_q4", "msd_linear_rows_q4_grouped",
+    "msd_layernorm_backward", "msd_layernorm_backward_workspace", "msd_token_embedding", "msd_token_embedding_backward",
+    "msd_token_embedding_backward_workspace", "msd_attention", "msd_attention_backward", "msd_attention_workspace",
+    "msd_softmax", "msd_alphas_cumprod", "msd_ddim_schedule", "msd_ddim_update",
 )
 ACT_NONE, ACT_SILU = 0, 1
 
@@ -98,6 +101,14 @@ def load_library(path=None):
     lib.msd_q4_pack.argtypes = [vp, vp, vp, sz, sz, sz, it, vp]
     lib.msd_linear_rows_q4.argtypes = [vp, vp, vp, vp, vp, sz, sz, sz, sz, it, it, it, vp]
     lib.msd_linear_rows_q4_grouped.argtypes = [vp] + [ctypes.POINTER(vp)] * 4 + [ctypes.POINTER(sz), sz, sz, sz, sz, it, it, it, vp]
+    lib.msd_layernorm_backward_workspace.argtypes = [sz, sz, it, ctypes.POINTER(sz)]
+    lib.msd_layernorm_backward.argtypes = [vp] * 7 + [sz, sz, fl, it, vp, sz, vp]
+    lib.msd_token_embedding.argtypes = [vp, vp, vp, vp, sz, sz, sz, sz, fl, it, vp]
+    lib.msd_token_embedding_backward_workspace.argtypes = [sz] * 5 + [it, ctypes.POINTER(sz)]
+    lib.msd_token_embedding_backward.argtypes = [vp] * 4 + [sz] * 5 + [fl, it, vp, sz, vp]
+    lib.msd_attention_workspace.argtypes = [sz] * 6 + [it, it, it, ctypes.POINTER(sz)]
+    lib.msd_attention.argtypes = [vp] * 7 + [sz] * 6 + [ctypes.POINTER(sz), fl, it, it, vp, sz, vp]
+    lib.msd_attention_backward.argtypes = [vp] * 11 + [sz] * 6 + [ctypes.POINTER(sz), fl, it, it, vp, sz, vp]
     flp, inp = ctypes.POINTER(ctypes.c_float), ctypes.POINTER(ctypes.c_int)
     lib.msd_alphas_cumprod.argtypes = [flp]
     lib.msd_ddim_schedule.argtypes = [it, inp, flp, flp, flp, it]
@@ -560,6 +571,88 @@ def layernorm(x, gamma, beta, eps=1e-5, out=None):
     return out
 
 
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(name, *args):
+    size = ctypes.c_size_t(0)
+    check(getattr(load_library(), name)(*args, ctypes.byref(size)))
+    return size.value
+
+
+def _workspace(like, name, *args):
+    """(tensor to keep until the call is made, its pointer, its bytes)."""
+    size = _workspace_bytes(name, *args)
+    t = like.new_empty(size, dtype=_torch.uint8)
+    return t, t.data_ptr(), size
+
+
+def layernorm_backward(dy, x, gamma, eps=1e-5, dsum=None, affine=True, out=None):
+    """Gradient of layernorm(x, gamma, beta, eps), or of add_layernorm's norm (x is then the sum it returned) -> (dx, dgamma, dbeta).
+    dsum: what comes back to x past the norm (the gradient of add_layernorm's sum), added to dx.  dgamma and dbeta are float32 [dim]
+    (None unless affine).  out: receives dx; may be dy or dsum."""
+    lib = _lib or load_library()
+    dp = _on_current_device(dy, "dy")
+    n, dim = dy.numel(), dy.shape[-1]
+    rows = n // dim if dim else 0
+    xp, sp = _same(x, dy, n, "x"), _same(dsum, dy, n, "dsum") if dsum is not None else None
+    gp = _affine(gamma, dim, dy, "gamma")
+    out, op = _out_like(dy, out)
+    dgamma = dbeta = None
+    if affine:
+        dgamma, dbeta = (dy.new_empty(dim, dtype=_torch.float32) for _ in range(2))
+    code = _dtype_code(dy)
+    workspace, wp, size = _workspace(dy, "msd_layernorm_backward_workspace", rows, dim, code)
+    check(lib.msd_layernorm_backward(dp, xp, sp, gp, op, _pointer(dgamma), _pointer(dbeta), rows, dim, eps, code, wp, size, _stream()))
+    return out, dgamma, dbeta
+
+
+def _token_ids(ids):
+    """(pointer, tokens, tokens per row) of int64 ids [..., length] on the current device."""
+    ip = _on_current_device(ids, "ids")
+    if ids.dtype != _torch.int64 or ids.dim() == 0:
+        raise MsdError("ids must be int64 [..., length] (got %s, %s)" % (ids.dtype, tuple(ids.shape)))
+    return ip, ids.numel(), ids.shape[-1]
+
+
+def token_embedding(ids, table, positions=None, scale=1.0, out=None):
+    """scale * table[ids] + positions[:length]: ids int64 [..., length], table [vocab, dim], positions [length or more, dim] in its dtype
+    or None -> [..., length, dim].  An id outside [0, vocab) stands for a row of zeros."""
+    lib = _lib or load_library()
+    ip, tokens, length = _token_ids(ids)
+    tp = _on_current_device(table, "table")
+    if table.dim() != 2:
+        raise MsdError("table must be [vocab, dim] (got %s)" % (tuple(table.shape),))
+    vocab, dim = table.shape
+    pp = None
+    if positions is not None:
+        if positions.dim() != 2 or positions.shape[1] != dim or positions.shape[0] < length:
+            raise MsdError("positions must be [%d or more, %d] (got %s)" % (length, dim, tuple(positions.shape)))
+        pp = _same(positions, table, positions.numel(), "positions")
+    if out is None:
+        out = table.new_empty(ids.shape + (dim,))
+    check(lib.msd_token_embedding(ip, tp, pp, _same(out, table, tokens * dim, "out"), tokens, length, vocab, dim, scale,
+                                  _dtype_code(table), _stream()))
+    return out
+
+
+def token_embedding_backward(dy, ids, vocab, positions=0, scale=1.0):
+    """Gradients of token_embedding's table of `vocab` rows and of its `positions` rows (0: not wanted) from dy [..., length, dim]
+    -> (dtable [vocab, dim], dpositions [positions, dim] or None) in dy's dtype, every row written."""
+    lib = _lib or load_library()
+    dp = _on_current_device(dy, "dy")
+    ip, tokens, length = _token_ids(ids)
+    if dy.shape[:-1] != ids.shape:
+        raise MsdError("dy must be %s + (dim,) (got %s)" % (tuple(ids.shape), tuple(dy.shape)))
+    dim, code = dy.shape[-1], _dtype_code(dy)
+    if positions and positions < length:
+        raise MsdError("positions must be 0 or at least %d (got %d)" % (length, positions))
+    dtable = dy.new_empty((vocab, dim))
+    dpositions = dy.new_empty((positions, dim)) if positions else None
+    workspace, wp, size = _workspace(dy, "msd_token_embedding_backward_workspace", tokens, length, vocab, positions, dim, code)
+    check(lib.msd_token_embedding_backward(ip, dp, dtable.data_ptr(), _pointer(dpositions), tokens, length, vocab, positions, dim, scale,
+                                           code, wp, size, _stream()))
+    return dtable, dpositions
+
+
 def geglu(proj, out=None):
     """proj: [..., 2*inner] (value | gate) -> [..., inner]."""
     done = _native.geglu(proj, out)
@@ -777,6 +870,105 @@ def softmax(x, stable=False, out=None):
     out, yp = _out_like(x, out)
     check(lib.msd_softmax(xp, yp, rows, cols, int(stable), _dtype_code(x), _stream()))
     return out
+
+
+KeptAttention = collections.namedtuple("KeptAttention", "q k v out lse causal scale offsets offsets_k")
+KeptAttention.__doc__ = """What attention_kept keeps for the gradient: the call's tensors and lse, float32 [rows of q, heads], the log2 of the
+weights' sums."""
+
+
+def _heads(t, what, like=None):
+    """The strides of a [batch, rows, heads, dim] or packed [rows, heads, dim] tensor on the current device."""
+    torch = _torch or _bind_torch()
+    if not t.is_cuda or t.get_device() != torch.cuda.current_device() or t.dim() not in (3, 4) or (t.shape[-1] > 1 and t.stride(-1) != 1):
+        raise MsdError("%s must be [batch, rows, heads, dim] or [rows, heads, dim] on the current device, the values of a head together "
+                       "(got %s, strides %s, %s)" % (what, tuple(t.shape), t.stride(), t.device))
+    if like is not None and (t.dtype != like.dtype or t.dim() != like.dim()):
+        raise MsdError("%s must be %s with %d dimensions (got %s, %d)" % (what, like.dtype, like.dim(), t.dtype, t.dim()))
+    strides = t.stride()[:-1]
+    return strides if t.dim() == 4 else (0,) + strides
+
+
+def _attention_sizes(q, k, v, offsets, offsets_k):
+    """(batch, q_rows, k_rows, heads, kv_heads, dim), pointers of the offsets, checked."""
+    if k.shape != v.shape or q.dim() != k.dim() or q.shape[-1] != k.shape[-1] or (q.dim() == 4 and q.shape[0] != k.shape[0]):
+        raise MsdError("k and v must have one shape that fits q (got %s, %s, %s)" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+    heads, kv_heads = q.shape[-2], k.shape[-2]
+    if kv_heads == 0 or heads == 0 or heads % kv_heads:
+        raise MsdError("heads must be a multiple of the key heads (got %d, %d)" % (heads, kv_heads))
+    if q.dim() == 4:
+        if offsets is not None or offsets_k is not None:
+            raise MsdError("offsets go with packed [rows, heads, dim] tensors")
+        return (q.shape[0], q.shape[1], k.shape[1], heads, kv_heads, q.shape[-1]), None, None
+    if offsets is None:
+        raise MsdError("packed [rows, heads, dim] tensors need offsets")
+    if offsets_k is None:
+        if k.shape[0] != q.shape[0]:
+            raise MsdError("k has %d rows, q %d: pass offsets_k" % (k.shape[0], q.shape[0]))
+        offsets_k = offsets
+    pointers = []
+    for o, what in ((offsets, "offsets"), (offsets_k, "offsets_k")):
+        pointers.append(_on_current_device(o, what))
+        if o.dtype != _torch.int32 or o.dim() != 1 or o.numel() != offsets.numel() or o.numel() == 0:
+            raise MsdError("%s must be int32 [sequences + 1] (got %s, %s)" % (what, o.dtype, tuple(o.shape)))
+    return (offsets.numel() - 1, q.shape[0], k.shape[0], heads, kv_heads, q.shape[-1]), pointers[0], pointers[1]
+
+
+def _attention_forward(q, k, v, causal, scale, offsets, offsets_k, out, keep):
+    lib = _lib or load_library()
+    strides = _heads(q, "q") + _heads(k, "k", q) + _heads(v, "v", q)
+    sizes, qo, ko = _attention_sizes(q, k, v, offsets, offsets_k)
+    code = _dtype_code(q)
+    if scale is None:
+        scale = sizes[5] ** -0.5 if sizes[5] else 1.0
+    if out is None:
+        out = q.new_empty(q.shape)
+    elif out.shape != q.shape:
+        raise MsdError("out must be %s (got %s)" % (tuple(q.shape), tuple(out.shape)))
+    strides += _heads(out, "out", q)
+    lse = q.new_empty(q.shape[:-1], dtype=_torch.float32) if keep else None
+    workspace, wp, size = _workspace(q, "msd_attention_workspace", *sizes, int(qo is not None), 0, code)
+    check(lib.msd_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _pointer(lse), qo, ko, *sizes,
+                            (ctypes.c_size_t * 12)(*strides), scale, int(causal), code, wp, size, _stream()))
+    return out, lse, scale
+
+
+def attention(q, k, v, causal=False, scale=None, offsets=None, offsets_k=None, out=None):
+    """softmax(scale q k^T) v: q [batch, rows, heads, dim], k and v [batch, keys, kv_heads, dim], heads a multiple of kv_heads, dim up
+    to 128; views are fine as long as a head's values lie together.  scale: 1 / sqrt(dim) unless given.  causal: the last query sees
+    every key, the one before all but the last, ...  Packed sequences: [rows, heads, dim] tensors with offsets (and offsets_k for the
+    keys, if they differ), int32 [sequences + 1] on the device; rows of no sequence stay as they were (in a new `out`: undefined).
+    A row that sees no key gives zeros."""
+    return _attention_forward(q, k, v, causal, scale, offsets, offsets_k, out, False)[0]
+
+
+def attention_kept(q, k, v, causal=False, scale=None, offsets=None, offsets_k=None, out=None):
+    """attention, and a KeptAttention for attention_backward.  What it holds must not change until then."""
+    out, lse, scale = _attention_forward(q, k, v, causal, scale, offsets, offsets_k, out, True)
+    return out, KeptAttention(q, k, v, out, lse, bool(causal), scale, offsets, offsets_k)
+
+
+def attention_backward(dout, kept, out=None):
+    """-> (dq, dk, dv) from dout (as the forward call's out) and what that call kept.  out: three tensors (views of one are fine) that
+    receive them."""
+    lib = _lib or load_library()
+    q, k, v = kept.q, kept.k, kept.v
+    sizes, qo, ko = _attention_sizes(q, k, v, kept.offsets, kept.offsets_k)
+    if out is None:
+        out = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+    tensors = (q, k, v, kept.out, dout) + tuple(out)
+    strides = ()
+    for t, like, what in zip(tensors, (q, k, k, q, q, q, k, k), ("q", "k", "v", "out", "dout", "dq", "dk", "dv")):
+        if t.shape != like.shape:
+            raise MsdError("%s must be %s (got %s)" % (what, tuple(like.shape), tuple(t.shape)))
+        strides += _heads(t, what, q)
+    code = _dtype_code(q)
+    lp = _affine(kept.lse, q.numel() // sizes[5] if sizes[5] else 0, q, "lse")
+    workspace, wp, size = _workspace(q, "msd_attention_workspace", *sizes, int(qo is not None), 1, code)
+    check(lib.msd_attention_backward(dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), kept.out.data_ptr(), lp,
+                                     *[t.data_ptr() for t in out], qo, ko, *sizes, (ctypes.c_size_t * 24)(*strides), kept.scale,
+                                     int(kept.causal), code, wp, size, _stream()))
+    return tuple(out)
 
 
 def alphas_cumprod():

@@ -53,7 +53,7 @@ def _run(cmd):
 
 
 HIP_SOURCES = ["api.hip", "gn_plan.hip", "groupnorm.hip", "gn_channels_last.hip", "layernorm.hip", "stream_ops.hip", "embed_ops.hip",
-               "linear_q4.hip"]
+               "linear_q4.hip", "layernorm_grad.hip", "token_embedding.hip", "attention.hip", "attention_grad.hip"]
 
 
 def build_hip():

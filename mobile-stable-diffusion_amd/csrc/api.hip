@@ -557,6 +557,92 @@ int msd_add_layernorm(const void *a, const void *b, void *sum, void *y, const fl
     return layernorm_entry(a, b, sum, y, gamma, beta, rows, dim, eps, dtype, stream);
 }
 
+int msd_layernorm_backward_workspace(size_t rows, size_t dim, int dtype, size_t *bytes) {
+    if (bytes == nullptr || (dtype != MSD_DTYPE_F32 && dtype != MSD_DTYPE_F16)) return MSD_ERR_INVALID_VALUE;
+    const size_t need = ln_grad_workspace_bytes(elt_bytes(dtype), rows, dim);
+    if (need == SIZE_MAX) return MSD_ERR_INVALID_VALUE;
+    *bytes = need;
+    return MSD_OK;
+}
+
+int msd_layernorm_backward(const void *dy, const void *x, const void *dsum, const float *gamma, void *dx, float *dgamma,
+                           float *dbeta, size_t rows, size_t dim, float eps, int dtype, void *workspace, size_t workspace_bytes,
+                           void *stream) {
+    size_t need, count;
+    const int rc = msd_layernorm_backward_workspace(rows, dim, dtype, &need);
+    if (rc != MSD_OK) return rc;
+    if ((dgamma == nullptr) != (dbeta == nullptr)) return MSD_ERR_INVALID_VALUE;
+    if (__builtin_mul_overflow(rows, dim, &count) || count > (SIZE_MAX >> 3)) return MSD_ERR_INVALID_VALUE;
+    if (count != 0 && (!dy || !x || !gamma || !dx || !workspace || !aligned16(workspace) || workspace_bytes < need))
+        return MSD_ERR_INVALID_VALUE;
+    const size_t bytes = count * elt_bytes(dtype), affine = dim * sizeof(float);
+    const Range d = {dy, bytes}, in = {x, bytes}, s = {dsum, bytes}, g = {gamma, affine}, w = {workspace, need};
+    const Range to = {dx, bytes}, dg = {dgamma, affine}, db = {dbeta, affine};
+    if ((dx != dy && overlaps_any(dx, bytes, {d})) || (dx != dsum && overlaps_any(dx, bytes, {s})) ||
+        overlaps_any(dx, bytes, {in, g, w, dg, db}) || overlaps_any(dgamma, affine, {d, in, s, g, w, db}) ||
+        overlaps_any(dbeta, affine, {d, in, s, g, w}) || overlaps_any(workspace, need, {d, in, s, g}))
+        return MSD_ERR_INVALID_VALUE;
+    const LnGrad a = {dy, x, dsum, gamma, dx, dgamma, dbeta, workspace};
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    if (dtype == MSD_DTYPE_F32) return ln_grad_dispatch<float>(a, rows, dim, eps, st);
+    return ln_grad_dispatch<__half>(a, rows, dim, eps, st);
+}
+
+// Checks of a token embedding's sizes: what the kernels count in 32 bits and launch.
+static int embedding_checks(size_t tokens, size_t length, size_t vocab, size_t positions, size_t dim, int dtype) {
+    constexpr size_t kMost = size_t(1) << 31;
+    if (dtype != MSD_DTYPE_F32 && dtype != MSD_DTYPE_F16) return MSD_ERR_INVALID_VALUE;
+    if (tokens > (size_t(1) << 25) || vocab > (size_t(1) << 28) || dim > (size_t(1) << 20) || length > kMost || positions > kMost ||
+        length * dim >= kMost || positions * dim >= kMost)
+        return MSD_ERR_INVALID_VALUE;
+    if (tokens != 0 && (length == 0 || tokens % length != 0 || (positions != 0 && positions < length))) return MSD_ERR_INVALID_VALUE;
+    return MSD_OK;
+}
+
+int msd_token_embedding(const int64_t *ids, const void *table, const void *positions, void *y, size_t tokens, size_t length,
+                        size_t vocab, size_t dim, float scale, int dtype, void *stream) {
+    const int rc = embedding_checks(tokens, length, vocab, positions != nullptr ? length : 0, dim, dtype);
+    if (rc != MSD_OK) return rc;
+    if (tokens == 0 || dim == 0) return MSD_OK;
+    if (!ids || !table || !y || vocab == 0) return MSD_ERR_INVALID_VALUE;
+    const size_t bytes = tokens * dim * elt_bytes(dtype);
+    if (overlaps_any(y, bytes, {{ids, tokens * sizeof(int64_t)}, {table, vocab * dim * elt_bytes(dtype)},
+                                {positions, length * dim * elt_bytes(dtype)}}))
+        return MSD_ERR_INVALID_VALUE;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (dtype == MSD_DTYPE_F32) return embed_dispatch<float>(ids, table, positions, y, tokens, length, vocab, dim, scale, s);
+    return embed_dispatch<__half>(ids, table, positions, y, tokens, length, vocab, dim, scale, s);
+}
+
+int msd_token_embedding_backward_workspace(size_t tokens, size_t length, size_t vocab, size_t positions, size_t dim, int dtype,
+                                           size_t *bytes) {
+    if (bytes == nullptr) return MSD_ERR_INVALID_VALUE;
+    const int rc = embedding_checks(tokens, length, vocab, positions, dim, dtype);
+    if (rc == MSD_OK) *bytes = embed_grad_workspace_bytes(tokens, length, vocab, positions, dim);
+    return rc;
+}
+
+int msd_token_embedding_backward(const int64_t *ids, const void *dy, void *dtable, void *dpositions, size_t tokens, size_t length,
+                                 size_t vocab, size_t positions, size_t dim, float scale, int dtype, void *workspace,
+                                 size_t workspace_bytes, void *stream) {
+    size_t need;
+    const int rc = msd_token_embedding_backward_workspace(tokens, length, vocab, positions, dim, dtype, &need);
+    if (rc != MSD_OK) return rc;
+    if (dim == 0 || (vocab == 0 && positions == 0)) return MSD_OK;
+    if ((dtable == nullptr && vocab != 0) || (positions != 0) != (dpositions != nullptr)) return MSD_ERR_INVALID_VALUE;
+    if (tokens != 0 && (!ids || !dy)) return MSD_ERR_INVALID_VALUE;
+    if (need != 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return MSD_ERR_INVALID_VALUE;
+    const size_t elt = elt_bytes(dtype), table_bytes = vocab * dim * elt, place_bytes = positions * dim * elt;
+    const Range i = {ids, tokens * sizeof(int64_t)}, d = {dy, tokens * dim * elt}, w = {workspace, need}, p = {dpositions, place_bytes};
+    if (overlaps_any(dtable, table_bytes, {i, d, w, p}) || overlaps_any(dpositions, place_bytes, {i, d, w}) ||
+        overlaps_any(workspace, need, {i, d}))
+        return MSD_ERR_INVALID_VALUE;
+    const EmbedGrad g = {ids, dy, dtable, dpositions, workspace};
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (dtype == MSD_DTYPE_F32) return embed_grad_dispatch<float>(g, tokens, length, vocab, positions, dim, scale, s);
+    return embed_grad_dispatch<__half>(g, tokens, length, vocab, positions, dim, scale, s);
+}
+
 int msd_elemwise_add(const void *a, const void *b, void *c, size_t n, int dtype, void *stream) {
     if (dtype != MSD_DTYPE_F32 && dtype != MSD_DTYPE_F16) return MSD_ERR_INVALID_VALUE;
     if (n != 0 && (!a || !b || !c)) return MSD_ERR_INVALID_VALUE;
@@ -764,6 +850,160 @@ int msd_softmax(const void *x, void *y, size_t rows, size_t cols, int stable, in
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (dtype == MSD_DTYPE_F32) return softmax_dispatch<float>(x, y, rows, cols, stable != 0, s);
     return softmax_dispatch<__half>(x, y, rows, cols, stable != 0, s);
+}
+
+// ---- attention: sizes, strides, what may overlap ----
+
+static int attention_checks(size_t batch, size_t q_rows, size_t k_rows, size_t heads, size_t kv_heads, size_t dim, bool packed, int dtype,
+                            size_t *all_q, size_t *all_k) {
+    constexpr size_t kMost = size_t(1) << 27;
+    if (dtype != MSD_DTYPE_F32 && dtype != MSD_DTYPE_F16) return MSD_ERR_INVALID_VALUE;
+    if (heads == 0 || kv_heads == 0 || heads % kv_heads != 0 || dim == 0 || dim > 128) return MSD_ERR_INVALID_VALUE;
+    if (batch > kMost || q_rows > kMost || k_rows > kMost || heads > kMost || batch * kv_heads > (size_t(1) << 22))
+        return MSD_ERR_INVALID_VALUE;
+    *all_q = packed ? (batch != 0 ? q_rows : 0) : batch * q_rows;
+    *all_k = packed ? (batch != 0 ? k_rows : 0) : batch * k_rows;
+    if (*all_q > kMost || *all_k > kMost || *all_q * heads > kMost || *all_k * kv_heads > kMost) return MSD_ERR_INVALID_VALUE;
+    return MSD_OK;
+}
+
+static AttnProblem attention_problem(const int32_t *q_offsets, const int32_t *k_offsets, size_t batch, size_t q_rows, size_t k_rows,
+                                     size_t heads, size_t kv_heads, size_t dim, float scale, int causal) {
+    return AttnProblem{q_offsets, k_offsets, batch, q_rows, k_rows, heads, kv_heads, dim, scale, causal != 0};
+}
+
+// A strided tensor of an attention call: its view, and from where to where it reaches.
+struct Strided {
+    AttnView view;
+    size_t heads_bytes, row_bytes, bytes;  // heads of a row from the first value to the last; stride of rows; the whole tensor
+    size_t batch_bytes;
+};
+
+static bool make_strided(const void *at, size_t batch, size_t rows, size_t heads, size_t dim, size_t elt, bool packed, const size_t *strides,
+                         bool output, Strided *to) {
+    if (packed) batch = 1;
+    size_t s[3] = {rows * heads * dim, heads * dim, dim};
+    if (strides != nullptr)
+        for (int i = 0; i < 3; i++) s[i] = strides[i];
+    const size_t counts[3] = {batch, rows, heads};
+    for (int i = 0; i < 3; i++)
+        if (counts[i] <= 1) s[i] = 0;  // (the stride of a single one is never taken)
+    *to = Strided{AttnView{at, s[0], s[1], s[2]}, 0, s[1] * elt, 0, s[0] * elt};
+    if (batch == 0 || rows == 0 || heads == 0) return true;
+    if (at == nullptr) return false;
+    size_t reach[3], end = dim;
+    for (int i = 0; i < 3; i++) {
+        if (s[i] > (SIZE_MAX >> 4) || __builtin_mul_overflow(s[i], counts[i] - 1, &reach[i]) || reach[i] > (SIZE_MAX >> 4) ||
+            __builtin_add_overflow(end, reach[i], &end) || end > (SIZE_MAX >> 4))
+            return false;
+    }
+    to->heads_bytes = (reach[2] + dim) * elt;
+    to->bytes = end * elt;
+    if (!output) return true;
+    // an output's values are all different ones: taken by size, each stride passes what the smaller ones reach
+    size_t order[3] = {0, 1, 2}, covered = dim;
+    std::sort(order, order + 3, [&](size_t a, size_t b) { return s[a] < s[b]; });
+    for (const size_t i : order) {
+        if (counts[i] <= 1) continue;
+        if (s[i] < covered) return false;
+        covered = s[i] * (counts[i] - 1) + covered;
+    }
+    return true;
+}
+
+static bool strided_apart(const Strided &a, const Strided &b) {
+    if (a.bytes == 0 || b.bytes == 0 || !ranges_overlap(a.view.at, a.bytes, b.view.at, b.bytes)) return true;
+    if (a.row_bytes != b.row_bytes || a.row_bytes == 0) return false;
+    if (a.batch_bytes != b.batch_bytes && a.batch_bytes != 0 && b.batch_bytes != 0) return false;
+    // every row of one lies in the gaps between the rows of the other
+    const Strided &low = a.view.at < b.view.at ? a : b, &high = a.view.at < b.view.at ? b : a;
+    const size_t step = (const char *)high.view.at - (const char *)low.view.at;
+    return low.heads_bytes <= step && step + high.heads_bytes <= low.row_bytes &&
+           (low.batch_bytes == 0 || low.batch_bytes % low.row_bytes == 0) && (high.batch_bytes == 0 || high.batch_bytes % high.row_bytes == 0);
+}
+
+int msd_attention_workspace(size_t batch, size_t q_rows, size_t k_rows, size_t heads, size_t kv_heads, size_t dim, int packed, int backward,
+                            int dtype, size_t *bytes) {
+    size_t all_q, all_k;
+    if (bytes == nullptr) return MSD_ERR_INVALID_VALUE;
+    const int rc = attention_checks(batch, q_rows, k_rows, heads, kv_heads, dim, packed != 0, dtype, &all_q, &all_k);
+    if (rc != MSD_OK) return rc;
+    static const int32_t any = 0;  // (only whether there are offsets counts)
+    const int32_t *offsets = packed ? &any : nullptr;
+    const AttnProblem p = attention_problem(offsets, offsets, batch, q_rows, k_rows, heads, kv_heads, dim, 1.0f, 0);
+    *bytes = all_q == 0 && (backward == 0 || all_k == 0) ? 0 : backward ? attn_grad_workspace_bytes(p) : attn_workspace_bytes(p);
+    return MSD_OK;
+}
+
+int msd_attention(const void *q, const void *k, const void *v, void *out, float *lse, const int32_t *q_offsets, const int32_t *k_offsets,
+                  size_t batch, size_t q_rows, size_t k_rows, size_t heads, size_t kv_heads, size_t dim, const size_t *strides, float scale,
+                  int causal, int dtype, void *workspace, size_t workspace_bytes, void *stream) {
+    size_t all_q, all_k, need;
+    const bool packed = q_offsets != nullptr;
+    if (packed != (k_offsets != nullptr) || !(scale > 0.0f) || !std::isfinite(scale)) return MSD_ERR_INVALID_VALUE;
+    int rc = attention_checks(batch, q_rows, k_rows, heads, kv_heads, dim, packed, dtype, &all_q, &all_k);
+    if (rc == MSD_OK) rc = msd_attention_workspace(batch, q_rows, k_rows, heads, kv_heads, dim, packed, 0, dtype, &need);
+    if (rc != MSD_OK) return rc;
+    if (all_q == 0) return MSD_OK;
+    if (need != 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return MSD_ERR_INVALID_VALUE;
+    const size_t elt = elt_bytes(dtype);
+    const size_t *s = strides;
+    Strided t[4];
+    if (!make_strided(q, batch, q_rows, heads, dim, elt, packed, s, false, &t[0]) ||
+        !make_strided(k, batch, k_rows, kv_heads, dim, elt, packed, s ? s + 3 : s, false, &t[1]) ||
+        !make_strided(v, batch, k_rows, kv_heads, dim, elt, packed, s ? s + 6 : s, false, &t[2]) ||
+        !make_strided(out, batch, q_rows, heads, dim, elt, packed, s ? s + 9 : s, true, &t[3]))
+        return MSD_ERR_INVALID_VALUE;
+    for (int i = 0; i < 3; i++)
+        if (!strided_apart(t[3], t[i])) return MSD_ERR_INVALID_VALUE;
+    const size_t offset_bytes = packed ? (batch + 1) * sizeof(int32_t) : 0, lse_bytes = all_q * heads * sizeof(float);
+    const Range qo = {q_offsets, offset_bytes}, ko = {k_offsets, offset_bytes}, l = {lse, lse_bytes};
+    const Range in[3] = {{q, t[0].bytes}, {k, t[1].bytes}, {v, t[2].bytes}};
+    if (overlaps_any(out, t[3].bytes, {qo, ko, l}) || overlaps_any(lse, lse_bytes, {qo, ko, in[0], in[1], in[2]}) ||
+        overlaps_any(workspace, need, {qo, ko, l, in[0], in[1], in[2], {out, t[3].bytes}}))
+        return MSD_ERR_INVALID_VALUE;
+    const AttnProblem p = attention_problem(q_offsets, k_offsets, batch, q_rows, k_rows, heads, kv_heads, dim, scale, causal);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    if (dtype == MSD_DTYPE_F32) return attn_dispatch<float>(p, t[0].view, t[1].view, t[2].view, t[3].view, lse, workspace, st);
+    return attn_dispatch<__half>(p, t[0].view, t[1].view, t[2].view, t[3].view, lse, workspace, st);
+}
+
+int msd_attention_backward(const void *dout, const void *q, const void *k, const void *v, const void *out, const float *lse, void *dq,
+                           void *dk, void *dv, const int32_t *q_offsets, const int32_t *k_offsets, size_t batch, size_t q_rows,
+                           size_t k_rows, size_t heads, size_t kv_heads, size_t dim, const size_t *strides, float scale, int causal,
+                           int dtype, void *workspace, size_t workspace_bytes, void *stream) {
+    size_t all_q, all_k, need;
+    const bool packed = q_offsets != nullptr;
+    if (packed != (k_offsets != nullptr) || !(scale > 0.0f) || !std::isfinite(scale)) return MSD_ERR_INVALID_VALUE;
+    int rc = attention_checks(batch, q_rows, k_rows, heads, kv_heads, dim, packed, dtype, &all_q, &all_k);
+    if (rc == MSD_OK) rc = msd_attention_workspace(batch, q_rows, k_rows, heads, kv_heads, dim, packed, 1, dtype, &need);
+    if (rc != MSD_OK) return rc;
+    if (all_q == 0 && all_k == 0) return MSD_OK;
+    if (need != 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return MSD_ERR_INVALID_VALUE;
+    if (all_q != 0 && lse == nullptr) return MSD_ERR_INVALID_VALUE;
+    const size_t elt = elt_bytes(dtype);
+    const void *const at[8] = {q, k, v, out, dout, dq, dk, dv};
+    Strided t[8];
+    for (int i = 0; i < 8; i++) {
+        const bool keys = i == 1 || i == 2 || i >= 6;
+        if (!make_strided(at[i], batch, keys ? k_rows : q_rows, keys ? kv_heads : heads, dim, elt, packed,
+                          strides != nullptr ? strides + 3 * i : nullptr, i >= 5, &t[i]))
+            return MSD_ERR_INVALID_VALUE;
+    }
+    for (int to = 5; to < 8; to++)
+        for (int i = 0; i < to; i++)
+            if (!strided_apart(t[to], t[i])) return MSD_ERR_INVALID_VALUE;
+    const size_t offset_bytes = packed ? (batch + 1) * sizeof(int32_t) : 0;
+    const Range qo = {q_offsets, offset_bytes}, ko = {k_offsets, offset_bytes}, l = {lse, all_q * heads * sizeof(float)};
+    for (int i = 0; i < 8; i++)
+        if ((i >= 5 && overlaps_any(at[i], t[i].bytes, {qo, ko, l})) || overlaps_any(workspace, need, {{at[i], t[i].bytes}}))
+            return MSD_ERR_INVALID_VALUE;
+    if (overlaps_any(workspace, need, {qo, ko, l})) return MSD_ERR_INVALID_VALUE;
+    const AttnProblem p = attention_problem(q_offsets, k_offsets, batch, q_rows, k_rows, heads, kv_heads, dim, scale, causal);
+    const AttnGradViews g = {t[0].view, t[1].view, t[2].view, t[3].view, t[4].view, t[5].view, t[6].view, t[7].view};
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    if (dtype == MSD_DTYPE_F32) return attn_grad_dispatch<float>(p, g, lse, workspace, st);
+    return attn_grad_dispatch<__half>(p, g, lse, workspace, st);
 }
 
 int msd_alphas_cumprod(float *out_1000) {

@@ -1,0 +1,302 @@
+// Attention for gfx950: out_i = sum_j p_ij v_j, p_ij = softmax over the visible j of scale q_i . k_j, in one pass over the keys with
+// a running maximum and sum.  The query heads of a key head are rows of one tile (row = query * group + head in the group), so keys
+// and values are read once for all of them, and a single query still has `group` rows.  A wavefront owns 32 rows as the columns of
+// S^T = K Q^T: a lane has one row, its maximum and sum need one exchange between the halves, and P^T stays in registers as the
+// operand of O^T = V^T P^T.  K and V tiles go through LDS, twice buffered.  Where rows are too few to fill the chip, the keys are
+// cut into parts, each with a workgroup of its own, and a second launch joins them.
+#include <algorithm>
+
+#include "attention_tiles.h"
+
+namespace msd {
+namespace {
+
+struct Forward {
+    AttnShape s;
+    AttnView q, k, v, out;
+    float *lse;        // [rows of queries][heads] log2 of the weights' sum, or null
+    float *part;       // parts > 1: [parts][rows of queries][heads][dim] and behind it their log2 sums [parts][rows][heads]
+    float *part_lse;
+    uint32_t parts, total_rows;
+    bool vec;
+};
+
+// A lane's maximum may lag by this much (in powers of two) before the sums are scaled down to it, and float16 weights are
+// kept kShift larger, so that they use the type's range: at most 2^(kLag + kShift) = 2^15.
+constexpr float kLag = 8.0f;
+template <typename T>
+constexpr float kShift = Frag<T>::kFloat ? 0.0f : 7.0f;
+
+template <typename T, int D>
+__global__ __launch_bounds__(kAttnThreads) void attn_kernel(const Forward a) {
+    typedef typename Frag<T>::type frag;
+    typedef Tile<T, D> KvTile;
+    constexpr int R = KvTile::kRows, KD = D / 16, DB = D / 32, PER = KvTile::kPerThread, CH = KvTile::kChunks, E = 16 / (int)sizeof(T);
+    __shared__ KvTile tiles[2][2];  // [buffer][K, V]
+    const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, h = lane / 32;
+    const uint32_t head = blockIdx.x % a.s.kv_heads, rest = blockIdx.x / a.s.kv_heads;
+    const uint32_t part = rest % a.parts;
+    uint32_t b, tile, q0, lq, k0, lk;
+    if (!find_tile(a.s.q_offsets, a.s.batch, a.s.q_rows, a.s.group, kAttnRows, rest / a.parts, b, tile)) return;
+    span(a.s.q_offsets, b, a.s.q_rows, q0, lq);
+    span(a.s.k_offsets, b, a.s.k_rows, k0, lk);
+    const uint32_t rows = lq * a.s.group;
+    if (a.s.causal) tile = (rows + kAttnRows - 1) / kAttnRows - 1 - tile;  // (those that see most keys first)
+
+    const bool packed_q = a.s.q_offsets != nullptr, packed_k = a.s.k_offsets != nullptr;
+    // the lane's row: query i of head `qh`; it sees the keys [0, limit)
+    const uint32_t row = tile * kAttnRows + wave * 32 + lane % 32;
+    const uint32_t i = row / a.s.group, qh = head * a.s.group + row % a.s.group;
+    const bool live = row < rows;
+    auto seen_by = [&](uint32_t query) -> uint32_t {
+        return a.s.causal ? (uint32_t)max((int64_t)0, min((int64_t)lk, (int64_t)query + 1 + lk - lq)) : lk;
+    };
+    const uint32_t limit = live ? seen_by(i) : 0;
+    const T *qrow = static_cast<const T *>(a.q.at) + (packed_q ? 0 : b * a.q.batch) + (size_t)(q0 + i) * a.q.row + qh * a.q.head;
+    const T *kbase = static_cast<const T *>(a.k.at) + (packed_k ? 0 : b * a.k.batch) + (size_t)k0 * a.k.row + head * a.k.head;
+    const T *vbase = static_cast<const T *>(a.v.at) + (packed_k ? 0 : b * a.v.batch) + (size_t)k0 * a.v.row + head * a.v.head;
+    frag q[KD];
+    load_frags<T, D>(live ? qrow : nullptr, a.s.dim, a.vec, q);
+
+    // tiles of keys: what the workgroup's last row sees, this part's share of it
+    const uint32_t last_row = min(rows, (tile + 1) * kAttnRows) - 1;
+    const uint32_t all = (seen_by(last_row / a.s.group) + R - 1) / R, each = (all + a.parts - 1) / a.parts;
+    const uint32_t t0 = min(all, part * each), t1 = min(all, t0 + each);
+    const uint32_t wave_row = tile * kAttnRows + wave * 32;
+    const uint32_t wave_limit = wave_row < rows ? seen_by(min(rows - 1, wave_row + 31) / a.s.group) : 0;  // the most any row sees
+    const uint32_t wave_full = wave_row < rows ? seen_by(wave_row / a.s.group) : 0;                       // what every row sees
+
+    u32x4 next[2][PER];
+    auto fetch = [&](uint32_t t) {
+#pragma unroll
+        for (int p = 0; p < PER; p++) {
+            const uint32_t c = p * kAttnThreads + threadIdx.x, r = c / CH, key = t * R + r, d = c % CH * E;
+            const bool in = key < lk;
+            next[0][p] = in ? load_chunk<T>(kbase + (size_t)key * a.k.row, d, a.s.dim, a.vec) : u32x4{0, 0, 0, 0};
+            next[1][p] = in ? load_chunk<T>(vbase + (size_t)key * a.v.row, d, a.s.dim, a.vec) : u32x4{0, 0, 0, 0};
+        }
+    };
+    auto put = [&](uint32_t buffer) {
+#pragma unroll
+        for (int p = 0; p < PER; p++) {
+            const uint32_t c = p * kAttnThreads + threadIdx.x, r = c / CH, at = r * CH + (c % CH ^ (r & 7));
+            tiles[buffer][0].data[at] = next[0][p];
+            tiles[buffer][1].data[at] = next[1][p];
+        }
+    };
+
+    f32x16 o[DB];
+#pragma unroll
+    for (int d = 0; d < DB; d++) o[d] = zero16();
+    float top = -__builtin_inff(), sum = 0.0f;
+    if (t0 < t1) {
+        fetch(t0);
+        put(0);
+    }
+    for (uint32_t t = t0; t < t1; t++) {
+        __syncthreads();
+        if (t + 1 < t1) fetch(t + 1);
+        const KvTile &kt = tiles[(t - t0) & 1][0], &vt = tiles[(t - t0) & 1][1];
+        const uint32_t first = t * R;
+        if (first < wave_limit) {
+            f32x16 s[R / 32];
+#pragma unroll
+            for (int n = 0; n < R / 32; n++) {
+                s[n] = zero16();
+#pragma unroll
+                for (int k = 0; k < KD; k++) s[n] = mma(kt.rows(32 * n, k), q[k], s[n]);
+            }
+            const bool masked = first + R > wave_full;
+            bool odd = false;
+            if (masked) {
+#pragma unroll
+                for (int n = 0; n < R / 32; n++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++)
+                        if (first + 32 * n + 8 * (r / 4) + 4 * h + r % 4 >= limit) s[n][r] = -__builtin_inff();
+            }
+            float most = s[0][0];
+#pragma unroll
+            for (int n = 0; n < R / 32; n++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) most = fmaxf(most, s[n][r]);
+            const float now = fmaxf(top, halves_max(most) * a.s.scale2);
+            if (__builtin_amdgcn_ballot_w64(now > top + kLag) != 0) {
+                const float down = __builtin_amdgcn_exp2f(top - (now == -__builtin_inff() ? 0.0f : now));
+                sum *= down;
+#pragma unroll
+                for (int d = 0; d < DB; d++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) o[d][r] *= down;
+                top = now;
+            }
+            const float base = kShift<T> - (top == -__builtin_inff() ? 0.0f : top);
+#pragma unroll
+            for (int n = 0; n < R / 32; n++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    s[n][r] = __builtin_amdgcn_exp2f(fmaf(s[n][r], a.s.scale2, base));
+                    sum += s[n][r];
+                }
+#pragma unroll
+            for (int n = 0; n < R / 32; n++)
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    frag p;
+                    to_frag(s[n], u, p);
+#pragma unroll
+                    for (int d = 0; d < DB; d++) {
+                        frag v = vt.columns(32 * n + 16 * u, d);
+                        if (masked) leave_out_odd(v, odd);
+                        o[d] = mma(v, p, o[d]);
+                    }
+                    step_end<T>();
+                }
+            if (odd) add_odd<T, D, R>(vt, o, [&](uint32_t r) { return first + r < limit; });
+        }
+        if (t + 1 < t1) put((t + 1 - t0) & 1);
+    }
+    sum += half_swap(sum);
+    if (!live) return;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // (a row that sees nothing is zero)
+    const float lse = sum == 0.0f ? -__builtin_inff() : top - kShift<T> + __builtin_amdgcn_logf(sum);
+    const size_t place = ((size_t)(packed_q ? 0 : b) * lq + q0 + i) * a.s.heads + qh;
+    if (a.parts > 1) {
+        float *const to = a.part + (part * (size_t)a.total_rows * a.s.heads + place) * a.s.dim;
+#pragma unroll
+        for (int d = 0; d < DB; d++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const uint32_t col = 32 * d + 8 * (r / 4) + 4 * h + r % 4;
+                if (col < a.s.dim) to[col] = o[d][r] * inv;
+            }
+        if (h == 0) a.part_lse[part * (size_t)a.total_rows * a.s.heads + place] = lse;
+        return;
+    }
+    T *const to = static_cast<T *>(const_cast<void *>(a.out.at)) + (packed_q ? 0 : b * a.out.batch) + (size_t)(q0 + i) * a.out.row + qh * a.out.head;
+#pragma unroll
+    for (int d = 0; d < DB; d++)
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            const uint32_t col = 32 * d + 8 * g + 4 * h;
+            T v[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) Store<T>::store1(v + j, o[d][4 * g + j] * inv);
+            if (a.vec) {
+                if (col < a.s.dim) __builtin_memcpy(__builtin_assume_aligned(to + col, 4 * sizeof(T)), v, sizeof(v));
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (col + j < a.s.dim) to[col + j] = v[j];
+            }
+        }
+    if (a.lse != nullptr && h == 0) a.lse[place] = lse;
+}
+
+// out = sum of the parts, each weighted by its share of the weights' sum: a wavefront for a row of a head.
+template <typename T>
+__global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(const Forward a) {
+    const size_t at = (size_t)blockIdx.x * kAttnWaves + threadIdx.x / kWave;
+    const size_t count = (size_t)a.total_rows * a.s.heads;
+    if (at >= count) return;
+    const uint32_t row = (uint32_t)(at / a.s.heads), head = (uint32_t)(at % a.s.heads), lane = threadIdx.x % kWave;
+    uint32_t b = 0, i = row;
+    if (a.s.q_offsets == nullptr) {
+        b = row / a.s.q_rows;
+        i = row - b * a.s.q_rows;
+    } else {  // rows of no sequence stay as they were
+        bool inside = false;
+        for (uint32_t s = lane; s < a.s.batch; s += kWave) {
+            uint32_t first, n;
+            span(a.s.q_offsets, s, a.s.q_rows, first, n);
+            inside |= row >= first && row - first < n;
+        }
+        if (__builtin_amdgcn_ballot_w64(inside) == 0) return;
+    }
+    float most = -__builtin_inff();
+    for (uint32_t p = 0; p < a.parts; p++) most = fmaxf(most, a.part_lse[p * count + at]);
+    const float base = most == -__builtin_inff() ? 0.0f : most;
+    float sum = 0.0f;
+    bool bad = false;  // (a NaN is no maximum)
+    for (uint32_t p = 0; p < a.parts; p++) {
+        const float l = a.part_lse[p * count + at];
+        bad |= l != l;
+        sum += __builtin_amdgcn_exp2f(l - base);
+    }
+    const float inv = bad ? __builtin_nanf("") : sum == 0.0f ? 0.0f : 1.0f / sum;
+    T *const to = static_cast<T *>(const_cast<void *>(a.out.at)) + b * a.out.batch + (size_t)i * a.out.row + head * a.out.head;
+    for (uint32_t d = lane; d < a.s.dim; d += kWave) {
+        float t = 0.0f;
+        for (uint32_t p = 0; p < a.parts; p++) {
+            const float w = __builtin_amdgcn_exp2f(a.part_lse[p * count + at] - base);
+            if (w != 0.0f) t = fmaf(w * inv, a.part[(p * count + at) * a.s.dim + d], t);
+        }
+        Store<T>::store1(to + d, t);
+    }
+    if (a.lse != nullptr && lane == 0) a.lse[at] = sum == 0.0f ? -__builtin_inff() : base + __builtin_amdgcn_logf(sum);
+}
+
+// Tiles of rows: the sequences' own where they are equal, at most this many where only their sum is known here.
+size_t row_tiles(const AttnProblem &p) {
+    const size_t group = p.heads / p.kv_heads;
+    if (p.q_offsets == nullptr) return p.batch * ((p.q_rows * group + kAttnRows - 1) / kAttnRows);
+    return p.q_rows * group / kAttnRows + p.batch;
+}
+
+// Parts of the keys: workgroups for two of the chip's CUs each, at least 256 keys in a part on average.
+uint32_t key_parts(const AttnProblem &p) {
+    const size_t keys = p.k_offsets == nullptr ? p.k_rows : p.k_rows / std::max<size_t>(1, p.batch);
+    const size_t blocks = std::max<size_t>(1, row_tiles(p) * p.kv_heads), want = 2 * (size_t)chip_info().cus;
+    if (blocks * 2 > want) return 1;
+    return (uint32_t)std::max<size_t>(1, std::min<size_t>(want / blocks, keys / 256));
+}
+
+size_t total_rows(const AttnProblem &p) { return p.q_offsets == nullptr ? p.batch * p.q_rows : p.q_rows; }
+
+}  // namespace
+
+size_t attn_workspace_bytes(const AttnProblem &p) {
+    const uint32_t parts = key_parts(p);
+    return parts <= 1 ? 0 : parts * total_rows(p) * p.heads * (p.dim + 1) * sizeof(float);
+}
+
+AttnShape attn_shape(const AttnProblem &p) {
+    return AttnShape{p.q_offsets, p.k_offsets, (uint32_t)p.batch, (uint32_t)p.q_rows, (uint32_t)p.k_rows, (uint32_t)p.heads,
+                     (uint32_t)p.kv_heads, (uint32_t)(p.heads / p.kv_heads), (uint32_t)p.dim, p.scale * kLog2e, p.causal};
+}
+
+bool attn_vectors(size_t elt, size_t dim, std::initializer_list<AttnView> views) {
+    bool vec = dim * elt % 16 == 0;
+    for (const AttnView &v : views)
+        vec = vec && aligned16(v.at) && v.row * elt % 16 == 0 && v.head * elt % 16 == 0 && v.batch * elt % 16 == 0;
+    return vec;
+}
+
+template <typename T>
+int attn_dispatch(const AttnProblem &p, const AttnView &q, const AttnView &k, const AttnView &v, const AttnView &out, float *lse,
+                  void *workspace, hipStream_t stream) {
+    const size_t tiles = row_tiles(p);
+    if (tiles == 0) return MSD_OK;
+    Forward a{attn_shape(p), q, k, v, out, lse, nullptr, nullptr, key_parts(p), (uint32_t)total_rows(p),
+              attn_vectors(sizeof(T), p.dim, {q, k, v, out})};
+    if (a.parts > 1) {
+        a.part = static_cast<float *>(workspace);
+        a.part_lse = a.part + (size_t)a.parts * a.total_rows * p.heads * p.dim;
+    }
+    const dim3 grid((uint32_t)(tiles * a.parts * p.kv_heads));
+    if (p.dim <= 64)
+        launch((attn_kernel<T, 64>), grid, dim3(kAttnThreads), 0, stream, a);
+    else
+        launch((attn_kernel<T, 128>), grid, dim3(kAttnThreads), 0, stream, a);
+    if (a.parts > 1)
+        launch((attn_join_kernel<T>), dim3((uint32_t)((total_rows(p) * p.heads + kAttnWaves - 1) / kAttnWaves)), dim3(kAttnThreads), 0,
+               stream, a);
+    return launch_status();
+}
+
+template int attn_dispatch<float>(const AttnProblem &, const AttnView &, const AttnView &, const AttnView &, const AttnView &, float *,
+                                  void *, hipStream_t);
+template int attn_dispatch<__half>(const AttnProblem &, const AttnView &, const AttnView &, const AttnView &, const AttnView &, float *,
+                                   void *, hipStream_t);
+
+}  // namespace msd

@@ -1,0 +1,444 @@
+// Gradient of attention for gfx950.  With p as in the forward call (formed again from its log2 sums) and D_i = do_i . out_i,
+//     dS_ij = p_ij (do_i . v_j - D_i),   dq_i = scale sum_j dS_ij k_j,   dk_j = scale sum_i dS_ij q_i,   dv_j = sum_i p_ij do_i.
+// Three launches: D (and row norms); dq with a workgroup for rows, over the keys, as the forward call; dk and dv with a
+// workgroup for keys, over the rows.  Each gradient is owned by one workgroup, so nothing is added by atomics, at the price of
+// forming S and dO V^T twice (7 products for 5).  The heads of a key head are rows of the same tiles, so their gradients
+// add up in the accumulators.
+//
+// float16: dS is rounded to float16 for its product, after a power of two that brings the largest it can be,
+// |do_i| max |v_j| + |D_i|, next to 2^14: it keeps 11 bits down to 2^-28 of that, whatever the gradients' size.  The power
+// follows the largest bound so far, and the sums are scaled down where it moves.
+#include <algorithm>
+
+#include "attention_tiles.h"
+
+namespace msd {
+namespace {
+
+struct Backward {
+    AttnShape s;
+    AttnView q, k, v, out, dout, dq, dk, dv;
+    const float *lse;
+    float *delta, *norm, *v_norm;  // [rows][heads] D and |do|, [keys][kv_heads] |v|; the norms null for float32
+    uint32_t total_rows, total_keys;
+    bool vec;
+};
+
+// 16 lanes to a row of a head.
+template <typename T>
+__global__ __launch_bounds__(kAttnThreads) void attn_grad_rows_kernel(const Backward a) {
+    constexpr uint32_t E = 16 / sizeof(T), kTeam = 16;
+    const size_t at = (size_t)blockIdx.x * (kAttnThreads / kTeam) + threadIdx.x / kTeam;
+    const size_t rows = (size_t)a.total_rows * a.s.heads, keys = a.v_norm != nullptr ? (size_t)a.total_keys * a.s.kv_heads : 0;
+    if (at >= rows + keys) return;
+    const bool of_keys = at >= rows;
+    const size_t item = of_keys ? at - rows : at;
+    const uint32_t heads = of_keys ? a.s.kv_heads : a.s.heads;
+    const uint32_t row = (uint32_t)(item / heads), head = (uint32_t)(item % heads);
+    auto address = [&](const AttnView &v, const int32_t *offsets, uint32_t each) {
+        const uint32_t b = offsets != nullptr ? 0 : row / each, i = offsets != nullptr ? row : row % each;
+        return static_cast<const T *>(v.at) + b * v.batch + (size_t)i * v.row + head * v.head;
+    };
+    const T *first, *second;
+    if (of_keys) {
+        first = second = address(a.v, a.s.k_offsets, a.s.k_rows);
+    } else {
+        first = address(a.dout, a.s.q_offsets, a.s.q_rows);
+        second = address(a.out, a.s.q_offsets, a.s.q_rows);
+    }
+    float dot = 0.0f, square = 0.0f;
+    for (uint32_t d = threadIdx.x % kTeam * E; d < a.s.dim; d += kTeam * E) {
+        float x[E], y[E];
+        Store<T>::unpack(load_chunk<T>(first, d, a.s.dim, a.vec), x);
+        Store<T>::unpack(load_chunk<T>(second, d, a.s.dim, a.vec), y);
+#pragma unroll
+        for (uint32_t e = 0; e < E; e++) {
+            dot = fmaf(x[e], y[e], dot);
+            square = fmaf(x[e], x[e], square);
+        }
+    }
+    dot = team_sum<16>(dot);
+    square = team_sum<16>(square);
+    if (threadIdx.x % kTeam != 0) return;
+    if (of_keys) {
+        a.v_norm[item] = sqrtf(square);
+    } else {
+        a.delta[item] = dot;
+        if (a.norm != nullptr) a.norm[item] = sqrtf(square);
+    }
+}
+
+// The power of two for dS up to `bound`, and the sums' way there.
+struct DsScale {
+    int power = 100;
+    __device__ __forceinline__ bool lower(float bound, float &down) {
+        const int p = max(-100, min(100, 14 - __builtin_amdgcn_frexp_expf(bound)));
+        if (p >= power) return false;
+        down = ldexpf(1.0f, max(-126, p - power));
+        power = p;
+        return true;
+    }
+};
+
+// kPShift: float16 weights are kept that many powers of two larger where they are an operand themselves (they are at most 1).
+template <typename T>
+constexpr int kPShift = Frag<T>::kFloat ? 0 : 15;
+
+// Stores an accumulator's columns: row `to` gets the lane's column times `by`.
+template <typename T, int D>
+__device__ __forceinline__ void store_rows(T *to, const f32x16 (&acc)[D / 32], float by, uint32_t dim, bool vec) {
+    const uint32_t h = threadIdx.x % kWave / 32;
+#pragma unroll
+    for (int d = 0; d < D / 32; d++)
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            const uint32_t col = 32 * d + 8 * g + 4 * h;
+            T v[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) Store<T>::store1(v + j, acc[d][4 * g + j] * by);
+            if (vec) {
+                if (col < dim) __builtin_memcpy(__builtin_assume_aligned(to + col, 4 * sizeof(T)), v, sizeof(v));
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (col + j < dim) to[col + j] = v[j];
+            }
+        }
+}
+
+// dq: the forward kernel's tiles of rows over tiles of keys.
+template <typename T, int D>
+__global__ __launch_bounds__(kAttnThreads) void attn_grad_q_kernel(const Backward a) {
+    typedef typename Frag<T>::type frag;
+    typedef Tile<T, D> KvTile;
+    constexpr bool kHalf = !Frag<T>::kFloat;
+    constexpr int R = KvTile::kRows, KD = D / 16, DB = D / 32, PER = KvTile::kPerThread, CH = KvTile::kChunks, E = 16 / (int)sizeof(T);
+    __shared__ KvTile tiles[2][2];
+    const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, h = lane / 32;
+    const uint32_t head = blockIdx.x % a.s.kv_heads;
+    uint32_t b, tile, q0, lq, k0, lk;
+    if (!find_tile(a.s.q_offsets, a.s.batch, a.s.q_rows, a.s.group, kAttnRows, blockIdx.x / a.s.kv_heads, b, tile)) return;
+    span(a.s.q_offsets, b, a.s.q_rows, q0, lq);
+    span(a.s.k_offsets, b, a.s.k_rows, k0, lk);
+    const uint32_t rows = lq * a.s.group;
+    if (a.s.causal) tile = (rows + kAttnRows - 1) / kAttnRows - 1 - tile;
+    const bool packed = a.s.q_offsets != nullptr;
+    const uint32_t row = tile * kAttnRows + wave * 32 + lane % 32;
+    const uint32_t i = row / a.s.group, qh = head * a.s.group + row % a.s.group;
+    const bool live = row < rows;
+    auto seen_by = [&](uint32_t query) -> uint32_t {
+        return a.s.causal ? (uint32_t)max((int64_t)0, min((int64_t)lk, (int64_t)query + 1 + lk - lq)) : lk;
+    };
+    const uint32_t limit = live ? seen_by(i) : 0;
+    auto at_row = [&](const AttnView &v) {
+        return static_cast<const T *>(v.at) + (packed ? 0 : b * v.batch) + (size_t)(q0 + i) * v.row + qh * v.head;
+    };
+    const T *kbase = static_cast<const T *>(a.k.at) + (packed ? 0 : b * a.k.batch) + (size_t)k0 * a.k.row + head * a.k.head;
+    const T *vbase = static_cast<const T *>(a.v.at) + (packed ? 0 : b * a.v.batch) + (size_t)k0 * a.v.row + head * a.v.head;
+    frag q[KD], g[KD];
+    load_frags<T, D>(live ? at_row(a.q) : nullptr, a.s.dim, a.vec, q);
+    load_frags<T, D>(live ? at_row(a.dout) : nullptr, a.s.dim, a.vec, g);
+    const size_t place = ((size_t)(packed ? 0 : b) * lq + q0 + i) * a.s.heads + qh;
+    const float lse = live ? a.lse[place] : 0.0f, delta = live ? a.delta[place] : 0.0f;
+    const float base = lse == -__builtin_inff() ? lse : -lse;  // (a row that sees nothing: weights of zero)
+    float most_norm = 0.0f, most_delta = 0.0f;
+    if (kHalf) {
+        most_norm = team_max<64>(live ? a.norm[place] : 0.0f);
+        most_delta = team_max<64>(fabsf(delta));
+    }
+    const float *const v_norm = kHalf ? a.v_norm + ((size_t)(packed ? 0 : b) * lk + k0) * a.s.kv_heads + head : nullptr;
+
+    const uint32_t last_row = min(rows, (tile + 1) * kAttnRows) - 1;
+    const uint32_t t1 = (seen_by(last_row / a.s.group) + R - 1) / R;
+    const uint32_t wave_row = tile * kAttnRows + wave * 32;
+    const uint32_t wave_limit = wave_row < rows ? seen_by(min(rows - 1, wave_row + 31) / a.s.group) : 0;
+    const uint32_t wave_full = wave_row < rows ? seen_by(wave_row / a.s.group) : 0;
+
+    u32x4 next[2][PER];
+    float next_norm = 0.0f;
+    auto fetch = [&](uint32_t t) {
+#pragma unroll
+        for (int p = 0; p < PER; p++) {
+            const uint32_t c = p * kAttnThreads + threadIdx.x, r = c / CH, key = t * R + r, d = c % CH * E;
+            const bool in = key < lk;
+            next[0][p] = in ? load_chunk<T>(kbase + (size_t)key * a.k.row, d, a.s.dim, a.vec) : u32x4{0, 0, 0, 0};
+            next[1][p] = in ? load_chunk<T>(vbase + (size_t)key * a.v.row, d, a.s.dim, a.vec) : u32x4{0, 0, 0, 0};
+        }
+        if (kHalf) next_norm = t * R + lane < lk ? v_norm[(size_t)(t * R + lane) * a.s.kv_heads] : 0.0f;
+    };
+    auto put = [&](uint32_t buffer) {
+#pragma unroll
+        for (int p = 0; p < PER; p++) {
+            const uint32_t c = p * kAttnThreads + threadIdx.x, r = c / CH, at = r * CH + (c % CH ^ (r & 7));
+            tiles[buffer][0].data[at] = next[0][p];
+            tiles[buffer][1].data[at] = next[1][p];
+        }
+    };
+    f32x16 dq[DB];
+#pragma unroll
+    for (int d = 0; d < DB; d++) dq[d] = zero16();
+    DsScale scale;
+    if (t1 != 0) {
+        fetch(0);
+        put(0);
+    }
+    for (uint32_t t = 0; t < t1; t++) {
+        const float v_most = kHalf ? team_max<64>(next_norm) : 0.0f;
+        __syncthreads();
+        if (t + 1 < t1) fetch(t + 1);
+        const KvTile &kt = tiles[t & 1][0], &vt = tiles[t & 1][1];
+        const uint32_t first = t * R;
+        if (first < wave_limit) {
+            float by = 1.0f;
+            if (kHalf) {
+                float down;
+                if (scale.lower(fmaf(most_norm, v_most, most_delta), down)) {
+#pragma unroll
+                    for (int d = 0; d < DB; d++)
+#pragma unroll
+                        for (int r = 0; r < 16; r++) dq[d][r] *= down;
+                }
+                by = ldexpf(1.0f, scale.power);
+            }
+            const float delta_by = delta * by;
+            const bool masked = first + R > wave_full;
+            bool odd = false;
+#pragma unroll
+            for (int n = 0; n < R / 32; n++) {
+                f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+                for (int k = 0; k < KD; k++) {
+                    s = mma(kt.rows(32 * n, k), q[k], s);
+                    dp = mma(vt.rows(32 * n, k), g[k], dp);
+                    step_end<T>();
+                }
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+                    s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.s.scale2, base)) * fmaf(dp[r], by, -delta_by);
+                if (masked) {
+#pragma unroll
+                    for (int r = 0; r < 16; r++)
+                        if (first + 32 * n + 8 * (r / 4) + 4 * h + r % 4 >= limit) s[r] = 0.0f;
+                }
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    frag ds;
+                    to_frag(s, u, ds);
+#pragma unroll
+                    for (int d = 0; d < DB; d++) {
+                        frag k = kt.columns(32 * n + 16 * u, d);
+                        if (masked) leave_out_odd(k, odd);
+                        dq[d] = mma(k, ds, dq[d]);
+                    }
+                    step_end<T>();
+                }
+            }
+            if (odd) add_odd<T, D, R>(kt, dq, [&](uint32_t r) { return first + r < limit; });
+        }
+        if (t + 1 < t1) put((t + 1) & 1);
+    }
+    if (!live) return;
+    T *const to = static_cast<T *>(const_cast<void *>(a.dq.at)) + (packed ? 0 : b * a.dq.batch) + (size_t)(q0 + i) * a.dq.row + qh * a.dq.head;
+    const float natural = a.s.scale2 * (1.0f / kLog2e);
+    store_rows<T, D>(to, dq, kHalf ? ldexpf(natural, -scale.power) : natural, a.s.dim, a.vec);
+}
+
+// dk and dv: a wavefront owns 32 keys as the columns of S = Q K^T; the rows that see them pass by.
+template <typename T, int D>
+__global__ __launch_bounds__(kAttnThreads) void attn_grad_kv_kernel(const Backward a) {
+    typedef typename Frag<T>::type frag;
+    typedef Tile<T, D, D == 128 ? 32 : Frag<T>::kTile> RowTile;  // (64 rows of 128 columns on their way leave too few registers)
+    constexpr bool kHalf = !Frag<T>::kFloat;
+    constexpr int R = RowTile::kRows, KD = D / 16, DB = D / 32, PER = RowTile::kPerThread, CH = RowTile::kChunks, E = 16 / (int)sizeof(T);
+    __shared__ RowTile tiles[2][2];                // [buffer][Q, dO]
+    __shared__ __align__(16) float stats[2][3][R]; // [buffer][- log2 sum, D, |do|]
+    const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, h = lane / 32;
+    const uint32_t head = blockIdx.x % a.s.kv_heads;
+    uint32_t b, tile, q0, lq, k0, lk;
+    if (!find_tile(a.s.k_offsets, a.s.batch, a.s.k_rows, 1, kAttnRows, blockIdx.x / a.s.kv_heads, b, tile)) return;
+    span(a.s.q_offsets, b, a.s.q_rows, q0, lq);
+    span(a.s.k_offsets, b, a.s.k_rows, k0, lk);
+    const bool packed = a.s.q_offsets != nullptr;
+    const uint32_t rows = lq * a.s.group, key = tile * kAttnRows + wave * 32 + lane % 32;
+    const bool live = key < lk;
+    // the first row that sees a key
+    auto first_row = [&](uint32_t j) -> uint32_t {
+        const int64_t query = a.s.causal ? max((int64_t)0, (int64_t)j + lq - lk) : 0;
+        return query >= lq ? rows : (uint32_t)query * a.s.group;
+    };
+    const T *kbase = static_cast<const T *>(a.k.at) + (packed ? 0 : b * a.k.batch) + (size_t)(k0 + key) * a.k.row + head * a.k.head;
+    const T *vbase = static_cast<const T *>(a.v.at) + (packed ? 0 : b * a.v.batch) + (size_t)(k0 + key) * a.v.row + head * a.v.head;
+    const T *qbase = static_cast<const T *>(a.q.at) + (packed ? 0 : b * a.q.batch) + (size_t)q0 * a.q.row + head * a.s.group * a.q.head;
+    const T *gbase = static_cast<const T *>(a.dout.at) + (packed ? 0 : b * a.dout.batch) + (size_t)q0 * a.dout.row + head * a.s.group * a.dout.head;
+    const size_t place0 = ((size_t)(packed ? 0 : b) * lq + q0) * a.s.heads + head * a.s.group;
+    frag k[KD], v[KD];
+    load_frags<T, D>(live ? kbase : nullptr, a.s.dim, a.vec, k);
+    load_frags<T, D>(live ? vbase : nullptr, a.s.dim, a.vec, v);
+    float v_most = 0.0f;
+    if (kHalf) v_most = team_max<64>(live ? a.v_norm[(((size_t)(packed ? 0 : b) * lk + k0) + key) * a.s.kv_heads + head] : 0.0f);
+
+    const uint32_t wave_key = tile * kAttnRows + wave * 32;
+    const uint32_t from = live ? first_row(key) : rows;                                  // the lane's rows: [from, rows)
+    const uint32_t wave_from = wave_key < lk ? first_row(wave_key) : rows;               // the first any key is seen by
+    const uint32_t wave_full = wave_key < lk ? first_row(min(lk - 1, wave_key + 31)) : rows; // from here on all are
+    const uint32_t t0 = first_row(tile * kAttnRows) / R, t1 = (rows + R - 1) / R;
+
+    u32x4 next[2][PER];
+    float next_stat[3] = {0.0f, 0.0f, 0.0f};
+    auto fetch = [&](uint32_t t) {
+#pragma unroll
+        for (int p = 0; p < PER; p++) {
+            const uint32_t c = p * kAttnThreads + threadIdx.x, r = t * R + c / CH, d = c % CH * E;
+            const bool in = r < rows;
+            const uint32_t i = r / a.s.group, gh = r - i * a.s.group;
+            next[0][p] = in ? load_chunk<T>(qbase + (size_t)i * a.q.row + gh * a.q.head, d, a.s.dim, a.vec) : u32x4{0, 0, 0, 0};
+            next[1][p] = in ? load_chunk<T>(gbase + (size_t)i * a.dout.row + gh * a.dout.head, d, a.s.dim, a.vec) : u32x4{0, 0, 0, 0};
+        }
+        if (threadIdx.x < R) {
+            const uint32_t r = t * R + threadIdx.x, i = r / a.s.group;
+            const bool in = r < rows;
+            const size_t at = place0 + (size_t)i * a.s.heads + (r - i * a.s.group);
+            const float lse = in ? a.lse[at] : -__builtin_inff();
+            next_stat[0] = lse == -__builtin_inff() ? lse : (float)kPShift<T> - lse;  // (rows that see nothing: weights of zero)
+            next_stat[1] = in ? a.delta[at] : 0.0f;
+            if (kHalf) next_stat[2] = in ? a.norm[at] : 0.0f;
+        }
+    };
+    auto put = [&](uint32_t buffer) {
+#pragma unroll
+        for (int p = 0; p < PER; p++) {
+            const uint32_t c = p * kAttnThreads + threadIdx.x, r = c / CH, at = r * CH + (c % CH ^ (r & 7));
+            tiles[buffer][0].data[at] = next[0][p];
+            tiles[buffer][1].data[at] = next[1][p];
+        }
+        if (threadIdx.x < R) {
+#pragma unroll
+            for (int i = 0; i < 3; i++) stats[buffer][i][threadIdx.x] = next_stat[i];
+        }
+    };
+    f32x16 dk[DB], dv[DB];
+#pragma unroll
+    for (int d = 0; d < DB; d++) dk[d] = dv[d] = zero16();
+    DsScale scale;
+    if (t0 < t1) {
+        fetch(t0);
+        put(0);
+    }
+    for (uint32_t t = t0; t < t1; t++) {
+        __syncthreads();
+        if (t + 1 < t1) fetch(t + 1);
+        const uint32_t buffer = (t - t0) & 1, first = t * R;
+        const RowTile &qt = tiles[buffer][0], &gt = tiles[buffer][1];
+        if (first + R > wave_from && wave_from < rows) {
+            float by = 1.0f;
+            if (kHalf) {
+                float down;
+                if (scale.lower(team_max<64>(fmaf(stats[buffer][2][lane % R], v_most, fabsf(stats[buffer][1][lane % R]))), down)) {
+#pragma unroll
+                    for (int d = 0; d < DB; d++)
+#pragma unroll
+                        for (int r = 0; r < 16; r++) dk[d][r] *= down;
+                }
+                by = ldexpf(1.0f, scale.power - kPShift<T>);
+            }
+            const bool masked = first < wave_full;
+            bool odd = false;
+#pragma unroll
+            for (int n = 0; n < R / 32; n++) {
+                f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+                for (int c = 0; c < KD; c++) {
+                    s = mma(qt.rows(32 * n, c), k[c], s);
+                    dp = mma(gt.rows(32 * n, c), v[c], dp);
+                    step_end<T>();
+                }
+#pragma unroll
+                for (int g = 0; g < 4; g++) {
+                    const f32x4 base = *reinterpret_cast<const f32x4 *>(&stats[buffer][0][32 * n + 8 * g + 4 * h]);
+                    const f32x4 delta = *reinterpret_cast<const f32x4 *>(&stats[buffer][1][32 * n + 8 * g + 4 * h]);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const int r = 4 * g + j;
+                        s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.s.scale2, base[j]));
+                        dp[r] = s[r] * (kHalf ? fmaf(dp[r], by, -delta[j] * by) : dp[r] - delta[j]);
+                    }
+                }
+                if (masked) {
+#pragma unroll
+                    for (int r = 0; r < 16; r++)
+                        if (first + 32 * n + 8 * (r / 4) + 4 * h + r % 4 < from) s[r] = dp[r] = 0.0f;
+                }
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    frag p, ds;
+                    to_frag(s, u, p);
+                    to_frag(dp, u, ds);
+#pragma unroll
+                    for (int d = 0; d < DB; d++) {
+                        frag gc = gt.columns(32 * n + 16 * u, d), qc = qt.columns(32 * n + 16 * u, d);
+                        if (masked) {
+                            leave_out_odd(gc, odd);
+                            leave_out_odd(qc, odd);
+                        }
+                        dv[d] = mma(gc, p, dv[d]);
+                        dk[d] = mma(qc, ds, dk[d]);
+                        step_end<T>();
+                    }
+                }
+            }
+            if (odd) {
+                auto visible = [&](uint32_t r) { return first + r >= from; };
+                add_odd<T, D, R>(gt, dv, visible);
+                add_odd<T, D, R>(qt, dk, visible);
+            }
+        }
+        if (t + 1 < t1) put((t + 1 - t0) & 1);
+    }
+    if (!live) return;
+    auto out = [&](const AttnView &to) {
+        return static_cast<T *>(const_cast<void *>(to.at)) + (packed ? 0 : b * to.batch) + (size_t)(k0 + key) * to.row + head * to.head;
+    };
+    const float natural = a.s.scale2 * (1.0f / kLog2e);
+    store_rows<T, D>(out(a.dk), dk, kHalf ? ldexpf(natural, -scale.power) : natural, a.s.dim, a.vec);
+    store_rows<T, D>(out(a.dv), dv, ldexpf(1.0f, -kPShift<T>), a.s.dim, a.vec);
+}
+
+size_t tiles_of(const int32_t *offsets, size_t batch, size_t rows, size_t times) {
+    if (offsets == nullptr) return batch * ((rows * times + kAttnRows - 1) / kAttnRows);
+    return rows * times / kAttnRows + batch;
+}
+
+}  // namespace
+
+size_t attn_grad_workspace_bytes(const AttnProblem &p) {
+    const size_t rows = p.q_offsets == nullptr ? p.batch * p.q_rows : p.q_rows, keys = p.k_offsets == nullptr ? p.batch * p.k_rows : p.k_rows;
+    return (2 * rows * p.heads + keys * p.kv_heads) * sizeof(float);
+}
+
+template <typename T>
+int attn_grad_dispatch(const AttnProblem &p, const AttnGradViews &g, const float *lse, void *workspace, hipStream_t stream) {
+    const size_t rows = p.q_offsets == nullptr ? p.batch * p.q_rows : p.q_rows, keys = p.k_offsets == nullptr ? p.batch * p.k_rows : p.k_rows;
+    float *const delta = static_cast<float *>(workspace);
+    constexpr bool kHalf = !Frag<T>::kFloat;
+    const Backward a{attn_shape(p), g.q, g.k, g.v, g.out, g.dout, g.dq, g.dk, g.dv, lse, delta,
+                     kHalf ? delta + rows * p.heads : nullptr, kHalf ? delta + 2 * rows * p.heads : nullptr, (uint32_t)rows, (uint32_t)keys,
+                     attn_vectors(sizeof(T), p.dim, {g.q, g.k, g.v, g.out, g.dout, g.dq, g.dk, g.dv})};
+    const size_t items = rows * p.heads + (kHalf ? keys * p.kv_heads : 0);
+    if (items != 0)
+        launch((attn_grad_rows_kernel<T>), dim3((uint32_t)((items + 15) / 16)), dim3(kAttnThreads), 0, stream, a);
+    const dim3 of_rows((uint32_t)(tiles_of(p.q_offsets, p.batch, p.q_rows, p.heads / p.kv_heads) * p.kv_heads));
+    const dim3 of_keys((uint32_t)(tiles_of(p.k_offsets, p.batch, p.k_rows, 1) * p.kv_heads));
+    if (p.dim <= 64) {
+        if (of_keys.x != 0) launch((attn_grad_kv_kernel<T, 64>), of_keys, dim3(kAttnThreads), 0, stream, a);
+        if (of_rows.x != 0) launch((attn_grad_q_kernel<T, 64>), of_rows, dim3(kAttnThreads), 0, stream, a);
+    } else {
+        if (of_keys.x != 0) launch((attn_grad_kv_kernel<T, 128>), of_keys, dim3(kAttnThreads), 0, stream, a);
+        if (of_rows.x != 0) launch((attn_grad_q_kernel<T, 128>), of_rows, dim3(kAttnThreads), 0, stream, a);
+    }
+    return launch_status();
+}
+
+template int attn_grad_dispatch<float>(const AttnProblem &, const AttnGradViews &, const float *, void *, hipStream_t);
+template int attn_grad_dispatch<__half>(const AttnProblem &, const AttnGradViews &, const float *, void *, hipStream_t);
+
+}  // namespace msd

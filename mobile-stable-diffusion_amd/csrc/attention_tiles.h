@@ -1,0 +1,263 @@
+// What the attention kernels share (attention.hip, attention_grad.hip): fragments of the 32 x 32 x 16 matrix products, tiles of
+// rows in LDS that are read by rows and by columns, the way from a workgroup to its sequence.
+//
+// Products are formed transposed, so that what one leaves in registers is what the next one takes.  With A's rows and B's
+// columns both indexed by lane & 31, the accumulator's lane has column lane & 31 and, in register 4 i + j, row 8 i + 4 h + j
+// with h = lane / 32.  Registers 8 t ... 8 t + 7 are then, rounded to the storage type, the B operand of the product over
+// rows 16 t ... 16 t + 15, if its A operand takes the same rows in the same order.  float32 goes through the same fragments,
+// eight values a lane, as eight products of 32 x 32 x 2.
+#pragma once
+
+#include <initializer_list>
+
+#include "msd_device.h"
+#include "msd_internal.h"
+
+namespace msd {
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef __fp16 fp16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+
+constexpr uint32_t kAttnThreads = 256, kAttnWaves = kAttnThreads / kWave;
+constexpr uint32_t kAttnRows = 32 * kAttnWaves;  // rows that a workgroup owns, 32 to a wavefront
+
+template <typename T>
+struct Frag;
+template <>
+struct Frag<__half> {
+    typedef half8 type;
+    static constexpr int kTile = 64;  // rows of a tile in LDS
+    static constexpr bool kFloat = false;
+};
+template <>
+struct Frag<float> {
+    typedef f32x8 type;
+    static constexpr int kTile = 32;
+    static constexpr bool kFloat = true;
+};
+
+__device__ __forceinline__ f32x16 mma(const half8 &a, const half8 &b, const f32x16 &c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma(const f32x8 &a, const f32x8 &b, f32x16 c) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+    return c;
+}
+
+// Between steps of products of float32, whose operands are twice as large: none is read from LDS ahead of its step (with
+// all of them there was no room in registers), and a step takes long enough to hide the next one's reads.
+template <typename T>
+__device__ __forceinline__ void step_end() {
+    if (Frag<T>::kFloat) __builtin_amdgcn_sched_barrier(0);
+}
+
+// Registers 8 t ... 8 t + 7 of an accumulator as a B operand (float16: rounded to nearest).
+__device__ __forceinline__ void to_frag(const f32x16 &c, int t, half8 &b) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const __half2 h = __floats2half2_rn(c[8 * t + 2 * j], c[8 * t + 2 * j + 1]);
+        typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+        const half2_t v = __builtin_bit_cast(half2_t, h);
+        b[2 * j] = v[0];
+        b[2 * j + 1] = v[1];
+    }
+}
+__device__ __forceinline__ void to_frag(const f32x16 &c, int t, f32x8 &b) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) b[j] = c[8 * t + j];
+}
+
+__device__ __forceinline__ f32x16 zero16() {
+    f32x16 z;
+#pragma unroll
+    for (int i = 0; i < 16; i++) z[i] = 0.0f;
+    return z;
+}
+
+// A masked pair's weight is zero, but zero times an infinity or NaN is not.  Where a tile has masked pairs, what its A operands
+// hold of those is left out of the product, and `add_odd` puts it back for the pairs that are visible.
+template <typename F>
+__device__ __forceinline__ bool any_odd(const F &a) {
+    uint32_t w[sizeof(F) / 4], found = 0;
+    __builtin_memcpy(w, &a, sizeof(F));
+#pragma unroll
+    for (uint32_t i = 0; i < sizeof(F) / 4; i++)  // (an exponent of ones, and one more, is the sign's bit)
+        found |= sizeof(F) == 16 ? (w[i] & 0x7C007C00u) + 0x04000400u : (w[i] & 0x7F800000u) + 0x00800000u;
+    return __builtin_amdgcn_ballot_w64((found & (sizeof(F) == 16 ? 0x80008000u : 0x80000000u)) != 0) != 0;
+}
+template <typename F>
+__device__ __forceinline__ void leave_out_odd(F &a, bool &odd) {
+    if (!any_odd(a)) return;
+    odd = true;
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+        if (!(__builtin_fabsf((float)a[j]) < __builtin_inff())) a[j] = 0;
+}
+// The infinities and NaN of a tile's columns, one kind at a time as ones against ones at the visible pairs (`visible(row)`: of
+// the lane's column and that row of the tile): a positive count puts the value into the sum.
+template <typename T, int D, int ROWS, typename Tile, typename Visible>
+__device__ __forceinline__ void add_odd(const Tile &tile, f32x16 (&acc)[D / 32], Visible visible) {
+    typedef typename Frag<T>::type frag;
+    const uint32_t h = threadIdx.x % kWave / 32;
+#pragma unroll 1
+    for (int r0 = 0; r0 < ROWS; r0 += 16) {
+        frag seen;
+#pragma unroll
+        for (int j = 0; j < 8; j++) seen[j] = visible(r0 + 8 * (j / 4) + 4 * h + j % 4) ? 1 : 0;
+#pragma unroll
+        for (int d = 0; d < D / 32; d++) {
+            const frag a = tile.columns(r0, d);
+            if (!any_odd(a)) continue;
+#pragma unroll 1
+            for (int kind = 0; kind < 3; kind++) {
+                const float value = kind == 0 ? __builtin_inff() : kind == 1 ? -__builtin_inff() : __builtin_nanf("");
+                frag is;
+#pragma unroll
+                for (int j = 0; j < 8; j++) is[j] = (kind == 2 ? a[j] != a[j] : (float)a[j] == value) ? 1 : 0;
+                const f32x16 count = mma(is, seen, zero16());
+#pragma unroll
+                for (int i = 0; i < 16; i++)
+                    if (count[i] > 0.0f) acc[d][i] += value;
+            }
+        }
+    }
+}
+
+// 16 bytes of a row from column d on, zeros behind its end.  vec: rows are whole aligned 16-byte vectors.
+template <typename T>
+__device__ __forceinline__ u32x4 load_chunk(const T *row, uint32_t d, uint32_t dim, bool vec) {
+    constexpr int E = 16 / sizeof(T);
+    if (vec) return d < dim ? *reinterpret_cast<const u32x4 *>(row + d) : u32x4{0, 0, 0, 0};
+    T v[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) v[e] = d + e < dim ? row[d + e] : T(0.0f);
+    u32x4 out;
+    __builtin_memcpy(&out, v, 16);
+    return out;
+}
+
+// Operands that a wavefront keeps: 32 rows (its lane's row, or null) as KD fragments.
+template <typename T, int D>
+__device__ __forceinline__ void load_frags(const T *row, uint32_t dim, bool vec, typename Frag<T>::type (&f)[D / 16]) {
+    const uint32_t h = threadIdx.x % kWave / 32;
+#pragma unroll
+    for (int k = 0; k < D / 16; k++) {
+        u32x4 v[sizeof(T) / 2];
+#pragma unroll
+        for (uint32_t i = 0; i < sizeof(T) / 2; i++)
+            v[i] = row != nullptr ? load_chunk<T>(row, 16 * k + 8 * h + i * (16 / sizeof(T)), dim, vec) : u32x4{0, 0, 0, 0};
+        __builtin_memcpy(&f[k], v, sizeof(f[k]));
+    }
+}
+
+// A tile in LDS: ROWS rows of D values as 16-byte chunks, chunk c of row r at place c ^ (r & 7), so that lanes that read one
+// chunk of neighbouring rows, or neighbouring chunks of four rows, meet different banks.
+template <typename T, int D, int ROWS = Frag<T>::kTile>
+struct Tile {
+    static constexpr int kRows = ROWS, kChunks = D * (int)sizeof(T) / 16;
+    static constexpr int kPerThread = kRows * kChunks / (int)kAttnThreads;
+    typedef typename Frag<T>::type frag;
+    u32x4 data[kRows * kChunks];
+
+    // A operand by rows: row r0 + (lane & 31), columns 16 k + 8 h ...
+    __device__ __forceinline__ frag rows(int r0, int k) const {
+        const uint32_t lane = threadIdx.x % kWave, r = r0 + lane % 32, h = lane / 32;
+        frag f;
+        u32x4 v[sizeof(T) / 2];
+#pragma unroll
+        for (uint32_t i = 0; i < sizeof(T) / 2; i++) v[i] = data[r * kChunks + (((2 * k + h) * (sizeof(T) / 2) + i) ^ (r & 7))];
+        __builtin_memcpy(&f, v, sizeof(f));
+        return f;
+    }
+    // A operand by columns: column 32 db + (lane & 31), the 16 rows from r0 on in the accumulators' order
+    __device__ __forceinline__ frag columns(int r0, int db) const {
+        const uint32_t lane = threadIdx.x % kWave, h = lane / 32;
+        frag f;
+        if constexpr (!Frag<T>::kFloat) {
+            // 16 lanes read 4 rows of 16 columns, 8 bytes a lane, and each gets a column of 4
+            const uint32_t i = lane % 16, col = 32 * db + 16 * (lane / 16 % 2) + 4 * (i % 4);
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const uint32_t r = r0 + 8 * u + 4 * h + i / 4;
+                const char *p = reinterpret_cast<const char *>(data) + (r * kChunks + ((col / 8) ^ (r & 7))) * 16 + col % 8 * 2;
+                const fp16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4f16(
+                    (fp16x4 __attribute__((address_space(3))) *)(__attribute__((address_space(3))) const char *)p);
+#pragma unroll
+                for (int j = 0; j < 4; j++) f[4 * u + j] = (_Float16)v[j];
+            }
+        } else {
+            const uint32_t col = 32 * db + lane % 32;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const uint32_t r = r0 + 8 * (j / 4) + 4 * h + j % 4;
+                f[j] = reinterpret_cast<const float *>(data)[(r * kChunks + ((col / 4) ^ (r & 7))) * 4 + col % 4];
+            }
+        }
+        return f;
+    }
+};
+
+// Maximum with the lane of the other half.
+__device__ __forceinline__ float halves_max(float v) { return fmaxf(v, half_swap(v)); }
+
+struct AttnShape {
+    const int32_t *q_offsets, *k_offsets;  // [batch + 1] or null: sequences of equal length
+    uint32_t batch, q_rows, k_rows;        // rows of all sequences (of one, without offsets)
+    uint32_t heads, kv_heads, group, dim;
+    float scale2;  // scale * log2(e)
+    bool causal;
+};
+
+AttnShape attn_shape(const AttnProblem &p);
+// Whether every row of the views is whole aligned 16-byte vectors.
+bool attn_vectors(size_t elt, size_t dim, std::initializer_list<AttnView> views);
+
+// [first, last) of sequence b: within the rows there are, whatever the offsets say.
+__device__ __forceinline__ void span(const int32_t *offsets, uint32_t b, uint32_t rows, uint32_t &first, uint32_t &count) {
+    if (offsets == nullptr) {
+        first = 0;
+        count = rows;
+        return;
+    }
+    const int32_t from = max(0, min(offsets[b], (int32_t)rows)), to = max(from, min(offsets[b + 1], (int32_t)rows));
+    first = (uint32_t)from;
+    count = (uint32_t)(to - from);
+}
+
+// Tile number `index` of all sequences' tiles, `per` rows each: a sequence has `times` rows for each of its offsets' rows.
+// False where there are fewer tiles.  Whole wavefronts look, 64 sequences at a time.
+__device__ __forceinline__ bool find_tile(const int32_t *offsets, uint32_t batch, uint32_t rows, uint32_t times, uint32_t per, uint32_t index,
+                                          uint32_t &b, uint32_t &tile) {
+    if (offsets == nullptr) {
+        const uint32_t tiles = (rows * times + per - 1) / per;
+        b = index / tiles;
+        tile = index - b * tiles;
+        return b < batch;
+    }
+    const uint32_t lane = threadIdx.x % kWave;
+    for (uint32_t b0 = 0; b0 < batch; b0 += kWave) {
+        uint32_t first, count = 0;
+        if (b0 + lane < batch) span(offsets, b0 + lane, rows, first, count);
+        const uint32_t tiles = (count * times + per - 1) / per;
+        uint32_t upto = tiles;
+#pragma unroll
+        for (uint32_t d = 1; d < kWave; d *= 2) {
+            const uint32_t o = __shfl_up(upto, d, kWave);
+            if (lane >= d) upto += o;
+        }
+        const uint64_t after = __builtin_amdgcn_ballot_w64(upto > index);
+        if (after != 0) {
+            const uint32_t at = (uint32_t)__builtin_ctzll(after);
+            b = b0 + at;
+            tile = index - (uint32_t)__builtin_amdgcn_readlane(upto - tiles, at);
+            return true;
+        }
+        index -= (uint32_t)__builtin_amdgcn_readlane(upto, kWave - 1);
+    }
+    return false;
+}
+
+}  // namespace msd

@@ -171,6 +171,55 @@ int cl_backward_dispatch(const ClBackward &a, size_t batch, size_t positions, si
 template <typename T>
 int ln_dispatch(const void *x, const void *res, void *sum, void *y, const float *gamma,
                 const float *beta, size_t rows, size_t dim, float eps, hipStream_t stream);
+// Gradient of LayerNorm (layernorm_grad.hip)
+struct LnGrad {
+    const void *dy, *x, *dsum;  // dsum or null
+    const float *gamma;
+    void *dx;
+    float *dgamma, *dbeta;  // both or neither
+    void *workspace;
+};
+// SIZE_MAX for a shape beyond what the kernels count in 32 bits
+size_t ln_grad_workspace_bytes(size_t elt, size_t rows, size_t dim);
+template <typename T>
+int ln_grad_dispatch(const LnGrad &g, size_t rows, size_t dim, float eps, hipStream_t stream);
+// Token embedding and its gradient (token_embedding.hip): y, dy [tokens, dim], token i at position i % length
+template <typename T>
+int embed_dispatch(const int64_t *ids, const void *table, const void *positions, void *y, size_t tokens, size_t length, size_t vocab,
+                   size_t dim, float scale, hipStream_t stream);
+struct EmbedGrad {
+    const int64_t *ids;
+    const void *dy;
+    void *dtable, *dpositions;  // [vocab, dim]; [positions, dim] or null
+    void *workspace;
+};
+size_t embed_grad_workspace_bytes(size_t tokens, size_t length, size_t vocab, size_t positions, size_t dim);
+template <typename T>
+int embed_grad_dispatch(const EmbedGrad &g, size_t tokens, size_t length, size_t vocab, size_t positions, size_t dim, float scale,
+                        hipStream_t stream);
+// Rows of a tensor [sequence][row][head][d], as strides in elements; packed sequences have no stride of their own.
+struct AttnView {
+    const void *at;
+    size_t batch, row, head;
+};
+
+struct AttnProblem {
+    const int32_t *q_offsets, *k_offsets;  // packed sequences: [batch + 1] first rows; both or neither
+    size_t batch, q_rows, k_rows;          // packed: rows of all sequences; otherwise of one
+    size_t heads, kv_heads, dim;
+    float scale;
+    bool causal;
+};
+size_t attn_workspace_bytes(const AttnProblem &p);
+template <typename T>
+int attn_dispatch(const AttnProblem &p, const AttnView &q, const AttnView &k, const AttnView &v, const AttnView &out, float *lse,
+                  void *workspace, hipStream_t stream);
+struct AttnGradViews {
+    AttnView q, k, v, out, dout, dq, dk, dv;
+};
+size_t attn_grad_workspace_bytes(const AttnProblem &p);
+template <typename T>
+int attn_grad_dispatch(const AttnProblem &p, const AttnGradViews &g, const float *lse, void *workspace, hipStream_t stream);
 template <typename T>
 int add_dispatch(const void *a, const void *b, void *c, size_t n, size_t chunk_size,
                  hipStream_t stream);  // chunk_size 0: elementwise; else b holds one value per chunk
