@@ -6,8 +6,9 @@
 // add up in the accumulators.
 //
 // float16: dS is rounded to float16 for its product, after a power of two that brings the largest it can be,
-// |do_i| max |v_j| + |D_i|, next to 2^14: it keeps 11 bits down to 2^-28 of that, whatever the gradients' size.  The power
-// follows the largest bound so far, and the sums are scaled down where it moves.
+// |do_i| max |v_j| + |D_i|, next to 2^14: it keeps 11 bits down to 2^-28 of that, whatever the gradients' size.  Each row of dq
+// and each key of dk and dv has a power of its own, from what it sees alone; it follows the largest bound so far, and the sums
+// are scaled down where it moves.
 #include <algorithm>
 
 #include "attention_tiles.h"
@@ -68,12 +69,30 @@ __global__ __launch_bounds__(kAttnThreads) void attn_grad_rows_kernel(const Back
     }
 }
 
-// The power of two for dS up to `bound`, and the sums' way there.
+// Largest value of the lanes up to this one, and from this one on.
+__device__ __forceinline__ float max_up_to(float v) {
+#pragma unroll
+    for (uint32_t d = 1; d < kWave; d *= 2) {
+        const float o = __shfl_up(v, d, kWave);
+        if (threadIdx.x % kWave >= d) v = fmaxf(v, o);
+    }
+    return v;
+}
+__device__ __forceinline__ float max_from(float v) {
+#pragma unroll
+    for (uint32_t d = 1; d < kWave; d *= 2) {
+        const float o = __shfl_down(v, d, kWave);
+        if (threadIdx.x % kWave + d < kWave) v = fmaxf(v, o);
+    }
+    return v;
+}
+
+// A lane's power of two for dS of up to `bound`; where that lowers any lane's, its sums are to be scaled by `down`.
 struct DsScale {
     int power = 100;
     __device__ __forceinline__ bool lower(float bound, float &down) {
-        const int p = max(-100, min(100, 14 - __builtin_amdgcn_frexp_expf(bound)));
-        if (p >= power) return false;
+        const int p = min(power, max(-100, min(100, 14 - __builtin_amdgcn_frexp_expf(bound))));
+        if (__builtin_amdgcn_ballot_w64(p < power) == 0) return false;
         down = ldexpf(1.0f, max(-126, p - power));
         power = p;
         return true;
@@ -141,11 +160,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_grad_q_kernel(const Backwar
     const size_t place = ((size_t)(packed ? 0 : b) * lq + q0 + i) * a.s.heads + qh;
     const float lse = live ? a.lse[place] : 0.0f, delta = live ? a.delta[place] : 0.0f;
     const float base = lse == -__builtin_inff() ? lse : -lse;  // (a row that sees nothing: weights of zero)
-    float most_norm = 0.0f, most_delta = 0.0f;
-    if (kHalf) {
-        most_norm = team_max<64>(live ? a.norm[place] : 0.0f);
-        most_delta = team_max<64>(fabsf(delta));
-    }
+    const float norm = kHalf && live ? a.norm[place] : 0.0f;
     const float *const v_norm = kHalf ? a.v_norm + ((size_t)(packed ? 0 : b) * lk + k0) * a.s.kv_heads + head : nullptr;
 
     const uint32_t last_row = min(rows, (tile + 1) * kAttnRows) - 1;
@@ -183,16 +198,24 @@ __global__ __launch_bounds__(kAttnThreads) void attn_grad_q_kernel(const Backwar
         put(0);
     }
     for (uint32_t t = 0; t < t1; t++) {
-        const float v_most = kHalf ? team_max<64>(next_norm) : 0.0f;
+        const float v_norms = next_norm;  // (of the tile's keys, one to a lane)
         __syncthreads();
         if (t + 1 < t1) fetch(t + 1);
         const KvTile &kt = tiles[t & 1][0], &vt = tiles[t & 1][1];
         const uint32_t first = t * R;
         if (first < wave_limit) {
             float by = 1.0f;
+            const bool masked = first + R > wave_full;
+            bool odd = false;
             if (kHalf) {
-                float down;
-                if (scale.lower(fmaf(most_norm, v_most, most_delta), down)) {
+                float down, v_most;
+                if (masked) {
+                    const float upto = __shfl(max_up_to(v_norms), (int)min(limit - first - 1, (uint32_t)R - 1), kWave);
+                    v_most = first < limit ? upto : 0.0f;
+                } else {
+                    v_most = team_max<64>(v_norms);
+                }
+                if (scale.lower(fmaf(norm, v_most, fabsf(delta)), down)) {
 #pragma unroll
                     for (int d = 0; d < DB; d++)
 #pragma unroll
@@ -201,8 +224,6 @@ __global__ __launch_bounds__(kAttnThreads) void attn_grad_q_kernel(const Backwar
                 by = ldexpf(1.0f, scale.power);
             }
             const float delta_by = delta * by;
-            const bool masked = first + R > wave_full;
-            bool odd = false;
 #pragma unroll
             for (int n = 0; n < R / 32; n++) {
                 f32x16 s = zero16(), dp = zero16();
@@ -274,8 +295,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_grad_kv_kernel(const Backwa
     frag k[KD], v[KD];
     load_frags<T, D>(live ? kbase : nullptr, a.s.dim, a.vec, k);
     load_frags<T, D>(live ? vbase : nullptr, a.s.dim, a.vec, v);
-    float v_most = 0.0f;
-    if (kHalf) v_most = team_max<64>(live ? a.v_norm[(((size_t)(packed ? 0 : b) * lk + k0) + key) * a.s.kv_heads + head] : 0.0f);
+    const float v_norm = kHalf && live ? a.v_norm[(((size_t)(packed ? 0 : b) * lk + k0) + key) * a.s.kv_heads + head] : 0.0f;
 
     const uint32_t wave_key = tile * kAttnRows + wave * 32;
     const uint32_t from = live ? first_row(key) : rows;                                  // the lane's rows: [from, rows)
@@ -331,9 +351,22 @@ __global__ __launch_bounds__(kAttnThreads) void attn_grad_kv_kernel(const Backwa
         const RowTile &qt = tiles[buffer][0], &gt = tiles[buffer][1];
         if (first + R > wave_from && wave_from < rows) {
             float by = 1.0f;
+            const bool masked = first < wave_full;
+            bool odd = false;
             if (kHalf) {
-                float down;
-                if (scale.lower(team_max<64>(fmaf(stats[buffer][2][lane % R], v_most, fabsf(stats[buffer][1][lane % R]))), down)) {
+                float down, norms = stats[buffer][2][lane % R], deltas = fabsf(stats[buffer][1][lane % R]);
+                if (masked) {
+                    norms = max_from(lane < R ? norms : 0.0f);
+                    deltas = max_from(lane < R ? deltas : 0.0f);
+                    const uint32_t behind = from > first ? min(from - first, (uint32_t)R) : 0;  // the tile's rows that do not see the key
+                    norms = __shfl(norms, (int)min(behind, (uint32_t)R - 1), kWave);
+                    deltas = __shfl(deltas, (int)min(behind, (uint32_t)R - 1), kWave);
+                    if (behind == R) norms = deltas = 0.0f;
+                } else {
+                    norms = team_max<64>(norms);
+                    deltas = team_max<64>(deltas);
+                }
+                if (scale.lower(fmaf(norms, v_norm, deltas), down)) {
 #pragma unroll
                     for (int d = 0; d < DB; d++)
 #pragma unroll
@@ -341,8 +374,6 @@ __global__ __launch_bounds__(kAttnThreads) void attn_grad_kv_kernel(const Backwa
                 }
                 by = ldexpf(1.0f, scale.power - kPShift<T>);
             }
-            const bool masked = first < wave_full;
-            bool odd = false;
 #pragma unroll
             for (int n = 0; n < R / 32; n++) {
                 f32x16 s = zero16(), dp = zero16();
