@@ -282,7 +282,7 @@ int msd_layernorm_backward(const void *dy, const void *x, const void *dsum, cons
  *           position, zeros from `length` on; positions = 0 and dpositions = NULL: not wanted.  Tokens outside [0, vocab) add
  *           nothing to dtable.  Sums are float32, a token's rows added in a fixed order, and rounded once to the storage type: the
  *           same bits every time.  workspace as for msd_layernorm_backward.
- * At most 2^25 tokens, 2^28 rows, 2^20 columns, and fewer than 2^31 values in `length` (and in `positions`) rows.
+ * At most 2^25 tokens, 2^28 rows, 2^20 columns, 2^35 values of dy, and fewer than 2^31 values in `length` (and in `positions`) rows.
  */
 int msd_token_embedding(const int64_t *ids, const void *table, const void *positions, void *y, size_t tokens, size_t length,
                         size_t vocab, size_t dim, float scale, int dtype, void *stream);
@@ -461,6 +461,8 @@ int msd_softmax(const void *x, void *y, size_t rows, size_t cols, int stable, in
  * and NaN included.  Scores, maxima and sums are float32; float16 weights are rounded to float16 for the product with v.
  *   lse    NULL, or float32 [rows of q][heads]: log2 of the sum of exp(scale q . k) (-infinity for a row that sees nothing),
  *          kept for msd_attention_backward.
+ *   rest   NULL, or with float16 [rows of q][heads][dim] float16 without gaps: what the rounding of out took away, kept for
+ *          msd_attention_backward, whose dq and dk are then a third nearer (out alone gives do_i . out_i to 11 bits).
  * workspace: 16-byte aligned device memory of at least the bytes that msd_attention_workspace reports (host only; dtype as for
  * the call; backward = 0), apart from all else; its contents need not be set, are left undefined, and belong to this call until it (or every
  * replay of it) is done.  The call allocates nothing and gives the same bits every time, in a capture too.
@@ -468,12 +470,12 @@ int msd_softmax(const void *x, void *y, size_t rows, size_t cols, int stable, in
  */
 int msd_attention_workspace(size_t batch, size_t q_rows, size_t k_rows, size_t heads, size_t kv_heads, size_t dim, int packed,
                             int backward, int dtype, size_t *bytes);
-int msd_attention(const void *q, const void *k, const void *v, void *out, float *lse, const int32_t *q_offsets,
+int msd_attention(const void *q, const void *k, const void *v, void *out, float *lse, void *rest, const int32_t *q_offsets,
                   const int32_t *k_offsets, size_t batch, size_t q_rows, size_t k_rows, size_t heads, size_t kv_heads, size_t dim,
                   const size_t *strides, float scale, int causal, int dtype, void *workspace, size_t workspace_bytes, void *stream);
 
 /*
- * Gradient of msd_attention: from dout (as out), the forward call's q, k, v, out and lse: dq (as q), dk and dv (as k), the
+ * Gradient of msd_attention: from dout (as out), the forward call's q, k, v, out, lse and rest (or NULL): dq (as q), dk and dv (as k), the
  * gradients of shared key heads summed over their query heads.  strides: as above for q, k, v, out, dout, dq, dk, dv in turn.
  * Rows that see nothing give zeros and add nothing, rows of no sequence stay as they were.  Sums are float32 in a fixed order
  * without atomics, the same bits every time; float16 weights and score gradients are rounded to float16 for their products,
@@ -481,7 +483,7 @@ int msd_attention(const void *q, const void *k, const void *v, void *out, float 
  * No counterpart in the reference, which has no gradients.
  */
 int msd_attention_backward(const void *dout, const void *q, const void *k, const void *v, const void *out, const float *lse,
-                           void *dq, void *dk, void *dv, const int32_t *q_offsets, const int32_t *k_offsets, size_t batch,
+                           const void *rest, void *dq, void *dk, void *dv, const int32_t *q_offsets, const int32_t *k_offsets, size_t batch,
                            size_t q_rows, size_t k_rows, size_t heads, size_t kv_heads, size_t dim, const size_t *strides,
                            float scale, int causal, int dtype, void *workspace, size_t workspace_bytes, void *stream);
 

@@ -21,6 +21,7 @@ LIB_HIP_PATH = os.path.join(CSRC_DIR, "libmsd_hip.so")
 LIB_NN_PATH = os.path.join(CSRC_DIR, "libmsd_nn.so")
 TORCH_CALLS_PATH = os.path.join(CSRC_DIR, "msd_torch_calls.so")
 TORCH_CALLS_CL_Q4_PATH = os.path.join(CSRC_DIR, "msd_torch_calls_cl_q4.so")  # channels-last norms, 4-bit weights
+TORCH_CALLS_TEXT_PATH = os.path.join(CSRC_DIR, "msd_torch_calls_text.so")  # token embedding, LayerNorm's gradient, attention
 
 DTYPE_F32 = 0
 DTYPE_F16 = 1
@@ -107,8 +108,8 @@ def load_library(path=None):
     lib.msd_token_embedding_backward_workspace.argtypes = [sz] * 5 + [it, ctypes.POINTER(sz)]
     lib.msd_token_embedding_backward.argtypes = [vp] * 4 + [sz] * 5 + [fl, it, vp, sz, vp]
     lib.msd_attention_workspace.argtypes = [sz] * 6 + [it, it, it, ctypes.POINTER(sz)]
-    lib.msd_attention.argtypes = [vp] * 7 + [sz] * 6 + [ctypes.POINTER(sz), fl, it, it, vp, sz, vp]
-    lib.msd_attention_backward.argtypes = [vp] * 11 + [sz] * 6 + [ctypes.POINTER(sz), fl, it, it, vp, sz, vp]
+    lib.msd_attention.argtypes = [vp] * 8 + [sz] * 6 + [ctypes.POINTER(sz), fl, it, it, vp, sz, vp]
+    lib.msd_attention_backward.argtypes = [vp] * 12 + [sz] * 6 + [ctypes.POINTER(sz), fl, it, it, vp, sz, vp]
     flp, inp = ctypes.POINTER(ctypes.c_float), ctypes.POINTER(ctypes.c_int)
     lib.msd_alphas_cumprod.argtypes = [flp]
     lib.msd_ddim_schedule.argtypes = [it, inp, flp, flp, flp, it]
@@ -117,7 +118,7 @@ def load_library(path=None):
         if name != "msd_error_string":
             getattr(lib, name).restype = it
     _lib = lib
-    for native in (_native, _native_cl_q4):
+    for native in (_native, _native_cl_q4, _native_text):
         if not isinstance(native, _Unbound):
             _bind_addresses(native)
     return lib
@@ -147,6 +148,11 @@ class _UnboundClQ4(_Unbound):
         return getattr(_bind_native_cl_q4(), name)
 
 
+class _UnboundText(_Unbound):
+    def __getattr__(self, name):
+        return getattr(_bind_native_text(), name)
+
+
 class _NoNative:
     """Stands for the native calls where there are none: every call takes its general path."""
 
@@ -160,7 +166,8 @@ class _NoNative:
         pass
 
 
-_native, _native_cl_q4 = _Unbound(), _UnboundClQ4()  # (two extensions: csrc/torch_calls.cpp, csrc/torch_calls_cl_q4.cpp)
+# (three extensions: csrc/torch_calls.cpp, csrc/torch_calls_cl_q4.cpp, csrc/torch_calls_text.cpp)
+_native, _native_cl_q4, _native_text = _Unbound(), _UnboundClQ4(), _UnboundText()
 
 
 def _bind_addresses(native):
@@ -211,6 +218,17 @@ def _bind_native_cl_q4():
         _bind_addresses(native)
         _native_cl_q4 = native
     return _native_cl_q4
+
+
+def _bind_native_text():
+    global _native_text
+    load_library()
+    torch = _bind_torch()
+    if isinstance(_native_text, _Unbound):
+        native = _load_native(torch, TORCH_CALLS_TEXT_PATH)
+        _bind_addresses(native)
+        _native_text = native
+    return _native_text
 
 
 _torch = None
@@ -589,6 +607,9 @@ def layernorm_backward(dy, x, gamma, eps=1e-5, dsum=None, affine=True, out=None)
     """Gradient of layernorm(x, gamma, beta, eps), or of add_layernorm's norm (x is then the sum it returned) -> (dx, dgamma, dbeta).
     dsum: what comes back to x past the norm (the gradient of add_layernorm's sum), added to dx.  dgamma and dbeta are float32 [dim]
     (None unless affine).  out: receives dx; may be dy or dsum."""
+    done = _native_text.layernorm_backward(dy, x, gamma, eps, dsum, affine, out)
+    if done is not None:
+        return done
     lib = _lib or load_library()
     dp = _on_current_device(dy, "dy")
     n, dim = dy.numel(), dy.shape[-1]
@@ -616,6 +637,9 @@ def _token_ids(ids):
 def token_embedding(ids, table, positions=None, scale=1.0, out=None):
     """scale * table[ids] + positions[:length]: ids int64 [..., length], table [vocab, dim], positions [length or more, dim] in its dtype
     or None -> [..., length, dim].  An id outside [0, vocab) stands for a row of zeros."""
+    done = _native_text.token_embedding(ids, table, positions, scale, out)
+    if done is not None:
+        return done
     lib = _lib or load_library()
     ip, tokens, length = _token_ids(ids)
     tp = _on_current_device(table, "table")
@@ -637,6 +661,9 @@ def token_embedding(ids, table, positions=None, scale=1.0, out=None):
 def token_embedding_backward(dy, ids, vocab, positions=0, scale=1.0):
     """Gradients of token_embedding's table of `vocab` rows and of its `positions` rows (0: not wanted) from dy [..., length, dim]
     -> (dtable [vocab, dim], dpositions [positions, dim] or None) in dy's dtype, every row written."""
+    done = _native_text.token_embedding_backward(dy, ids, vocab, positions, scale)
+    if done is not None:
+        return done
     lib = _lib or load_library()
     dp = _on_current_device(dy, "dy")
     ip, tokens, length = _token_ids(ids)
@@ -872,9 +899,9 @@ def softmax(x, stable=False, out=None):
     return out
 
 
-KeptAttention = collections.namedtuple("KeptAttention", "q k v out lse causal scale offsets offsets_k")
-KeptAttention.__doc__ = """What attention_kept keeps for the gradient: the call's tensors and lse, float32 [rows of q, heads], the log2 of the
-weights' sums."""
+KeptAttention = collections.namedtuple("KeptAttention", "q k v out lse rest causal scale offsets offsets_k")
+KeptAttention.__doc__ = """What attention_kept keeps for the gradient: the call's tensors, lse, float32 [rows of q, heads], the log2 of the weights'
+sums, and for float16 rest, what the rounding of out took away."""
 
 
 def _heads(t, what, like=None):
@@ -927,10 +954,11 @@ def _attention_forward(q, k, v, causal, scale, offsets, offsets_k, out, keep):
         raise MsdError("out must be %s (got %s)" % (tuple(q.shape), tuple(out.shape)))
     strides += _heads(out, "out", q)
     lse = q.new_empty(q.shape[:-1], dtype=_torch.float32) if keep else None
+    rest = q.new_empty(q.shape) if keep and code == DTYPE_F16 else None
     workspace, wp, size = _workspace(q, "msd_attention_workspace", *sizes, int(qo is not None), 0, code)
-    check(lib.msd_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _pointer(lse), qo, ko, *sizes,
+    check(lib.msd_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _pointer(lse), _pointer(rest), qo, ko, *sizes,
                             (ctypes.c_size_t * 12)(*strides), scale, int(causal), code, wp, size, _stream()))
-    return out, lse, scale
+    return out, lse, rest, scale
 
 
 def attention(q, k, v, causal=False, scale=None, offsets=None, offsets_k=None, out=None):
@@ -939,18 +967,27 @@ def attention(q, k, v, causal=False, scale=None, offsets=None, offsets_k=None, o
     every key, the one before all but the last, ...  Packed sequences: [rows, heads, dim] tensors with offsets (and offsets_k for the
     keys, if they differ), int32 [sequences + 1] on the device; rows of no sequence stay as they were (in a new `out`: undefined).
     A row that sees no key gives zeros."""
+    done = _native_text.attention(q, k, v, causal, scale, offsets, offsets_k, out, False)
+    if done is not None:
+        return done
     return _attention_forward(q, k, v, causal, scale, offsets, offsets_k, out, False)[0]
 
 
 def attention_kept(q, k, v, causal=False, scale=None, offsets=None, offsets_k=None, out=None):
     """attention, and a KeptAttention for attention_backward.  What it holds must not change until then."""
-    out, lse, scale = _attention_forward(q, k, v, causal, scale, offsets, offsets_k, out, True)
-    return out, KeptAttention(q, k, v, out, lse, bool(causal), scale, offsets, offsets_k)
+    done = _native_text.attention(q, k, v, causal, scale, offsets, offsets_k, out, True)
+    if done is None:
+        done = _attention_forward(q, k, v, causal, scale, offsets, offsets_k, out, True)
+    out, lse, rest, scale = done
+    return out, KeptAttention(q, k, v, out, lse, rest, bool(causal), scale, offsets, offsets_k)
 
 
 def attention_backward(dout, kept, out=None):
     """-> (dq, dk, dv) from dout (as the forward call's out) and what that call kept.  out: three tensors (views of one are fine) that
     receive them."""
+    done = _native_text.attention_backward(dout, out, *kept)
+    if done is not None:
+        return done
     lib = _lib or load_library()
     q, k, v = kept.q, kept.k, kept.v
     sizes, qo, ko = _attention_sizes(q, k, v, kept.offsets, kept.offsets_k)
@@ -964,8 +1001,9 @@ def attention_backward(dout, kept, out=None):
         strides += _heads(t, what, q)
     code = _dtype_code(q)
     lp = _affine(kept.lse, q.numel() // sizes[5] if sizes[5] else 0, q, "lse")
+    rp = _same(kept.rest, q, q.numel(), "rest") if kept.rest is not None else None
     workspace, wp, size = _workspace(q, "msd_attention_workspace", *sizes, int(qo is not None), 1, code)
-    check(lib.msd_attention_backward(dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), kept.out.data_ptr(), lp,
+    check(lib.msd_attention_backward(dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), kept.out.data_ptr(), lp, rp,
                                      *[t.data_ptr() for t in out], qo, ko, *sizes, (ctypes.c_size_t * 24)(*strides), kept.scale,
                                      int(kept.causal), code, wp, size, _stream()))
     return tuple(out)

@@ -2,7 +2,7 @@
 
     libmsd_hip.so   HIP kernels + the C ABI declared in include/msd_hip.h
     libmsd_nn.so    C++ host layer objects (GroupNorm / LayerNorm / GEGLU / ...) on top of it
-    msd_torch_calls.so, msd_torch_calls_cl_q4.so  the package's calls for plain torch tensors (CPython extensions, host only)
+    msd_torch_calls.so, msd_torch_calls_cl_q4.so, msd_torch_calls_text.so  the package's calls for plain torch tensors (CPython extensions, host only)
     cli/msd_compare golden-file comparison tool (host only)
     cli/msd_layer_check  runs the layer objects against golden .npy files (needs a GPU)
 
@@ -38,7 +38,7 @@ DEVICE_FLAGS = [
 
 LIB_HIP = os.path.join(CSRC, "libmsd_hip.so")
 LIB_NN = os.path.join(CSRC, "libmsd_nn.so")
-TORCH_CALLS = [os.path.join(CSRC, name) for name in ("msd_torch_calls.so", "msd_torch_calls_cl_q4.so")]
+TORCH_CALLS = [os.path.join(CSRC, name) for name in ("msd_torch_calls.so", "msd_torch_calls_cl_q4.so", "msd_torch_calls_text.so")]
 CLI_COMPARE = os.path.join(CSRC, "cli", "msd_compare")
 CLI_LAYER_CHECK = os.path.join(CSRC, "cli", "msd_layer_check")
 
@@ -111,7 +111,7 @@ def build_torch_calls():
     torch_dir = torch_with_hip_headers()
     if torch_dir is None:
         return []
-    for path in TORCH_CALLS:
+    def build_one(path):
         source = os.path.basename(path)[len("msd_"):].replace(".so", ".cpp")
         _run([os.environ.get("CXX", "g++"), "-O2", "-DNDEBUG", "-std=c++17", "-fPIC", "-shared", "-DUSE_ROCM", "-D__HIP_PLATFORM_AMD__",
               '-DMSD_BUILT_FOR="%s"' % _runs_with(torch_dir),
@@ -119,6 +119,9 @@ def build_torch_calls():
               "-isystem", "/opt/rocm/include", "-isystem", sysconfig.get_paths()["include"],
               os.path.join(CSRC, source), "-o", path, "-L", os.path.join(torch_dir, "lib"), "-ltorch_python",
               "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip", "-L/opt/rocm/lib", "-lamdhip64"])
+    from concurrent.futures import ThreadPoolExecutor
+    with ThreadPoolExecutor(max_workers=len(TORCH_CALLS)) as pool:
+        list(pool.map(build_one, TORCH_CALLS))
     return TORCH_CALLS
 
 

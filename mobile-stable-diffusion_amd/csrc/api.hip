@@ -577,7 +577,7 @@ int msd_layernorm_backward(const void *dy, const void *x, const void *dsum, cons
         return MSD_ERR_INVALID_VALUE;
     const size_t bytes = count * elt_bytes(dtype), affine = dim * sizeof(float);
     const Range d = {dy, bytes}, in = {x, bytes}, s = {dsum, bytes}, g = {gamma, affine}, w = {workspace, need};
-    const Range to = {dx, bytes}, dg = {dgamma, affine}, db = {dbeta, affine};
+    const Range dg = {dgamma, affine}, db = {dbeta, affine};
     if ((dx != dy && overlaps_any(dx, bytes, {d})) || (dx != dsum && overlaps_any(dx, bytes, {s})) ||
         overlaps_any(dx, bytes, {in, g, w, dg, db}) || overlaps_any(dgamma, affine, {d, in, s, g, w, db}) ||
         overlaps_any(dbeta, affine, {d, in, s, g, w}) || overlaps_any(workspace, need, {d, in, s, g}))
@@ -593,7 +593,7 @@ static int embedding_checks(size_t tokens, size_t length, size_t vocab, size_t p
     constexpr size_t kMost = size_t(1) << 31;
     if (dtype != MSD_DTYPE_F32 && dtype != MSD_DTYPE_F16) return MSD_ERR_INVALID_VALUE;
     if (tokens > (size_t(1) << 25) || vocab > (size_t(1) << 28) || dim > (size_t(1) << 20) || length > kMost || positions > kMost ||
-        length * dim >= kMost || positions * dim >= kMost)
+        length * dim >= kMost || positions * dim >= kMost || tokens * dim > (size_t(1) << 35))
         return MSD_ERR_INVALID_VALUE;
     if (tokens != 0 && (length == 0 || tokens % length != 0 || (positions != 0 && positions < length))) return MSD_ERR_INVALID_VALUE;
     return MSD_OK;
@@ -935,7 +935,7 @@ int msd_attention_workspace(size_t batch, size_t q_rows, size_t k_rows, size_t h
     return MSD_OK;
 }
 
-int msd_attention(const void *q, const void *k, const void *v, void *out, float *lse, const int32_t *q_offsets, const int32_t *k_offsets,
+int msd_attention(const void *q, const void *k, const void *v, void *out, float *lse, void *rest, const int32_t *q_offsets, const int32_t *k_offsets,
                   size_t batch, size_t q_rows, size_t k_rows, size_t heads, size_t kv_heads, size_t dim, const size_t *strides, float scale,
                   int causal, int dtype, void *workspace, size_t workspace_bytes, void *stream) {
     size_t all_q, all_k, need;
@@ -958,17 +958,21 @@ int msd_attention(const void *q, const void *k, const void *v, void *out, float 
         if (!strided_apart(t[3], t[i])) return MSD_ERR_INVALID_VALUE;
     const size_t offset_bytes = packed ? (batch + 1) * sizeof(int32_t) : 0, lse_bytes = all_q * heads * sizeof(float);
     const Range qo = {q_offsets, offset_bytes}, ko = {k_offsets, offset_bytes}, l = {lse, lse_bytes};
-    const Range in[3] = {{q, t[0].bytes}, {k, t[1].bytes}, {v, t[2].bytes}};
+    const size_t rest_bytes = all_q * heads * dim * elt;
+    if (dtype == MSD_DTYPE_F32) rest = nullptr;  // (nothing is rounded away)
+    const Range in[3] = {{q, t[0].bytes}, {k, t[1].bytes}, {v, t[2].bytes}}, r = {rest, rest_bytes};
+    if (overlaps_any(rest, rest_bytes, {qo, ko, l, in[0], in[1], in[2], {out, t[3].bytes}}) || overlaps_any(workspace, need, {r}))
+        return MSD_ERR_INVALID_VALUE;
     if (overlaps_any(out, t[3].bytes, {qo, ko, l}) || overlaps_any(lse, lse_bytes, {qo, ko, in[0], in[1], in[2]}) ||
         overlaps_any(workspace, need, {qo, ko, l, in[0], in[1], in[2], {out, t[3].bytes}}))
         return MSD_ERR_INVALID_VALUE;
     const AttnProblem p = attention_problem(q_offsets, k_offsets, batch, q_rows, k_rows, heads, kv_heads, dim, scale, causal);
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (dtype == MSD_DTYPE_F32) return attn_dispatch<float>(p, t[0].view, t[1].view, t[2].view, t[3].view, lse, workspace, st);
-    return attn_dispatch<__half>(p, t[0].view, t[1].view, t[2].view, t[3].view, lse, workspace, st);
+    if (dtype == MSD_DTYPE_F32) return attn_dispatch<float>(p, t[0].view, t[1].view, t[2].view, t[3].view, lse, rest, workspace, st);
+    return attn_dispatch<__half>(p, t[0].view, t[1].view, t[2].view, t[3].view, lse, rest, workspace, st);
 }
 
-int msd_attention_backward(const void *dout, const void *q, const void *k, const void *v, const void *out, const float *lse, void *dq,
+int msd_attention_backward(const void *dout, const void *q, const void *k, const void *v, const void *out, const float *lse, const void *rest, void *dq,
                            void *dk, void *dv, const int32_t *q_offsets, const int32_t *k_offsets, size_t batch, size_t q_rows,
                            size_t k_rows, size_t heads, size_t kv_heads, size_t dim, const size_t *strides, float scale, int causal,
                            int dtype, void *workspace, size_t workspace_bytes, void *stream) {
@@ -995,15 +999,17 @@ int msd_attention_backward(const void *dout, const void *q, const void *k, const
             if (!strided_apart(t[to], t[i])) return MSD_ERR_INVALID_VALUE;
     const size_t offset_bytes = packed ? (batch + 1) * sizeof(int32_t) : 0;
     const Range qo = {q_offsets, offset_bytes}, ko = {k_offsets, offset_bytes}, l = {lse, all_q * heads * sizeof(float)};
+    if (dtype == MSD_DTYPE_F32) rest = nullptr;
+    const Range r = {rest, all_q * heads * dim * elt};
     for (int i = 0; i < 8; i++)
-        if ((i >= 5 && overlaps_any(at[i], t[i].bytes, {qo, ko, l})) || overlaps_any(workspace, need, {{at[i], t[i].bytes}}))
+        if ((i >= 5 && overlaps_any(at[i], t[i].bytes, {qo, ko, l, r})) || overlaps_any(workspace, need, {{at[i], t[i].bytes}}))
             return MSD_ERR_INVALID_VALUE;
-    if (overlaps_any(workspace, need, {qo, ko, l})) return MSD_ERR_INVALID_VALUE;
+    if (overlaps_any(workspace, need, {qo, ko, l, r})) return MSD_ERR_INVALID_VALUE;
     const AttnProblem p = attention_problem(q_offsets, k_offsets, batch, q_rows, k_rows, heads, kv_heads, dim, scale, causal);
     const AttnGradViews g = {t[0].view, t[1].view, t[2].view, t[3].view, t[4].view, t[5].view, t[6].view, t[7].view};
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (dtype == MSD_DTYPE_F32) return attn_grad_dispatch<float>(p, g, lse, workspace, st);
-    return attn_grad_dispatch<__half>(p, g, lse, workspace, st);
+    if (dtype == MSD_DTYPE_F32) return attn_grad_dispatch<float>(p, g, lse, rest, workspace, st);
+    return attn_grad_dispatch<__half>(p, g, lse, rest, workspace, st);
 }
 
 int msd_alphas_cumprod(float *out_1000) {

@@ -15,6 +15,7 @@ struct Forward {
     AttnShape s;
     AttnView q, k, v, out;
     float *lse;        // [rows of queries][heads] log2 of the weights' sum, or null
+    void *rest;        // [rows of queries][heads][dim] what rounding takes from out, or null
     float *part;       // parts > 1: [parts][rows of queries][heads][dim] and behind it their log2 sums [parts][rows][heads]
     float *part_lse;
     uint32_t parts, total_rows;
@@ -28,7 +29,7 @@ template <typename T>
 constexpr float kShift = Frag<T>::kFloat ? 0.0f : 7.0f;
 
 template <typename T, int D>
-__global__ __launch_bounds__(kAttnThreads) void attn_kernel(const Forward a) {
+__global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_kernel(const Forward a) {
     typedef typename Frag<T>::type frag;
     typedef Tile<T, D> KvTile;
     constexpr int R = KvTile::kRows, KD = D / 16, DB = D / 32, PER = KvTile::kPerThread, CH = KvTile::kChunks, E = 16 / (int)sizeof(T);
@@ -190,6 +191,28 @@ __global__ __launch_bounds__(kAttnThreads) void attn_kernel(const Forward a) {
                     if (col + j < a.s.dim) to[col + j] = v[j];
             }
         }
+    if (!Frag<T>::kFloat && a.rest != nullptr) {
+        T *const left = static_cast<T *>(a.rest) + place * a.s.dim;
+#pragma unroll
+        for (int d = 0; d < DB; d++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const uint32_t col = 32 * d + 8 * g + 4 * h;
+                T v[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const float value = o[d][4 * g + j] * inv;
+                    Store<T>::store1(v + j, value - round_to_storage<T>(value));
+                }
+                if (a.vec) {
+                    if (col < a.s.dim) __builtin_memcpy(__builtin_assume_aligned(left + col, 4 * sizeof(T)), v, sizeof(v));
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        if (col + j < a.s.dim) left[col + j] = v[j];
+                }
+            }
+    }
     if (a.lse != nullptr && h == 0) a.lse[place] = lse;
 }
 
@@ -232,6 +255,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(const Forward a
             if (w != 0.0f) t = fmaf(w * inv, a.part[(p * count + at) * a.s.dim + d], t);
         }
         Store<T>::store1(to + d, t);
+        if (!Frag<T>::kFloat && a.rest != nullptr) Store<T>::store1(static_cast<T *>(a.rest) + at * a.s.dim + d, t - round_to_storage<T>(t));
     }
     if (a.lse != nullptr && lane == 0) a.lse[at] = sum == 0.0f ? -__builtin_inff() : base + __builtin_amdgcn_logf(sum);
 }
@@ -274,11 +298,11 @@ bool attn_vectors(size_t elt, size_t dim, std::initializer_list<AttnView> views)
 
 template <typename T>
 int attn_dispatch(const AttnProblem &p, const AttnView &q, const AttnView &k, const AttnView &v, const AttnView &out, float *lse,
-                  void *workspace, hipStream_t stream) {
+                  void *rest, void *workspace, hipStream_t stream) {
     const size_t tiles = row_tiles(p);
     if (tiles == 0) return MSD_OK;
-    Forward a{attn_shape(p), q, k, v, out, lse, nullptr, nullptr, key_parts(p), (uint32_t)total_rows(p),
-              attn_vectors(sizeof(T), p.dim, {q, k, v, out})};
+    Forward a{attn_shape(p), q, k, v, out, lse, rest, nullptr, nullptr, key_parts(p), (uint32_t)total_rows(p),
+              attn_vectors(sizeof(T), p.dim, {q, k, v, out, AttnView{rest, 0, 0, 0}})};
     if (a.parts > 1) {
         a.part = static_cast<float *>(workspace);
         a.part_lse = a.part + (size_t)a.parts * a.total_rows * p.heads * p.dim;
@@ -295,8 +319,8 @@ int attn_dispatch(const AttnProblem &p, const AttnView &q, const AttnView &k, co
 }
 
 template int attn_dispatch<float>(const AttnProblem &, const AttnView &, const AttnView &, const AttnView &, const AttnView &, float *,
-                                  void *, hipStream_t);
+                                  void *, void *, hipStream_t);
 template int attn_dispatch<__half>(const AttnProblem &, const AttnView &, const AttnView &, const AttnView &, const AttnView &, float *,
-                                   void *, hipStream_t);
+                                   void *, void *, hipStream_t);
 
 }  // namespace msd

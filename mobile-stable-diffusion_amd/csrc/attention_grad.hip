@@ -20,6 +20,7 @@ struct Backward {
     AttnShape s;
     AttnView q, k, v, out, dout, dq, dk, dv;
     const float *lse;
+    const void *rest;  // [rows][heads][dim] what rounding took from out, or null
     float *delta, *norm, *v_norm;  // [rows][heads] D and |do|, [keys][kv_heads] |v|; the norms null for float32
     uint32_t total_rows, total_keys;
     bool vec;
@@ -47,6 +48,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_grad_rows_kernel(const Back
         first = address(a.dout, a.s.q_offsets, a.s.q_rows);
         second = address(a.out, a.s.q_offsets, a.s.q_rows);
     }
+    const T *const rest = !of_keys && a.rest != nullptr ? static_cast<const T *>(a.rest) + item * a.s.dim : nullptr;
     float dot = 0.0f, square = 0.0f;
     for (uint32_t d = threadIdx.x % kTeam * E; d < a.s.dim; d += kTeam * E) {
         float x[E], y[E];
@@ -56,6 +58,11 @@ __global__ __launch_bounds__(kAttnThreads) void attn_grad_rows_kernel(const Back
         for (uint32_t e = 0; e < E; e++) {
             dot = fmaf(x[e], y[e], dot);
             square = fmaf(x[e], x[e], square);
+        }
+        if (rest != nullptr) {
+            Store<T>::unpack(load_chunk<T>(rest, d, a.s.dim, a.vec), y);
+#pragma unroll
+            for (uint32_t e = 0; e < E; e++) dot = fmaf(x[e], y[e], dot);
         }
     }
     dot = team_sum<16>(dot);
@@ -127,7 +134,7 @@ __device__ __forceinline__ void store_rows(T *to, const f32x16 (&acc)[D / 32], f
 
 // dq: the forward kernel's tiles of rows over tiles of keys.
 template <typename T, int D>
-__global__ __launch_bounds__(kAttnThreads) void attn_grad_q_kernel(const Backward a) {
+__global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_grad_q_kernel(const Backward a) {
     typedef typename Frag<T>::type frag;
     typedef Tile<T, D> KvTile;
     constexpr bool kHalf = !Frag<T>::kFloat;
@@ -266,7 +273,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_grad_q_kernel(const Backwar
 
 // dk and dv: a wavefront owns 32 keys as the columns of S = Q K^T; the rows that see them pass by.
 template <typename T, int D>
-__global__ __launch_bounds__(kAttnThreads) void attn_grad_kv_kernel(const Backward a) {
+__global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat || D == 128 ? 1 : 2) void attn_grad_kv_kernel(const Backward a) {
     typedef typename Frag<T>::type frag;
     typedef Tile<T, D, D == 128 ? 32 : Frag<T>::kTile> RowTile;  // (64 rows of 128 columns on their way leave too few registers)
     constexpr bool kHalf = !Frag<T>::kFloat;
@@ -447,13 +454,13 @@ size_t attn_grad_workspace_bytes(const AttnProblem &p) {
 }
 
 template <typename T>
-int attn_grad_dispatch(const AttnProblem &p, const AttnGradViews &g, const float *lse, void *workspace, hipStream_t stream) {
+int attn_grad_dispatch(const AttnProblem &p, const AttnGradViews &g, const float *lse, const void *rest, void *workspace, hipStream_t stream) {
     const size_t rows = p.q_offsets == nullptr ? p.batch * p.q_rows : p.q_rows, keys = p.k_offsets == nullptr ? p.batch * p.k_rows : p.k_rows;
     float *const delta = static_cast<float *>(workspace);
     constexpr bool kHalf = !Frag<T>::kFloat;
-    const Backward a{attn_shape(p), g.q, g.k, g.v, g.out, g.dout, g.dq, g.dk, g.dv, lse, delta,
+    const Backward a{attn_shape(p), g.q, g.k, g.v, g.out, g.dout, g.dq, g.dk, g.dv, lse, rest, delta,
                      kHalf ? delta + rows * p.heads : nullptr, kHalf ? delta + 2 * rows * p.heads : nullptr, (uint32_t)rows, (uint32_t)keys,
-                     attn_vectors(sizeof(T), p.dim, {g.q, g.k, g.v, g.out, g.dout, g.dq, g.dk, g.dv})};
+                     attn_vectors(sizeof(T), p.dim, {g.q, g.k, g.v, g.out, g.dout, g.dq, g.dk, g.dv, AttnView{rest, 0, 0, 0}})};
     const size_t items = rows * p.heads + (kHalf ? keys * p.kv_heads : 0);
     if (items != 0)
         launch((attn_grad_rows_kernel<T>), dim3((uint32_t)((items + 15) / 16)), dim3(kAttnThreads), 0, stream, a);
@@ -469,7 +476,7 @@ int attn_grad_dispatch(const AttnProblem &p, const AttnGradViews &g, const float
     return launch_status();
 }
 
-template int attn_grad_dispatch<float>(const AttnProblem &, const AttnGradViews &, const float *, void *, hipStream_t);
-template int attn_grad_dispatch<__half>(const AttnProblem &, const AttnGradViews &, const float *, void *, hipStream_t);
+template int attn_grad_dispatch<float>(const AttnProblem &, const AttnGradViews &, const float *, const void *, void *, hipStream_t);
+template int attn_grad_dispatch<__half>(const AttnProblem &, const AttnGradViews &, const float *, const void *, void *, hipStream_t);
 
 }  // namespace msd

@@ -176,20 +176,20 @@ __global__ __launch_bounds__(kThreads) void ln_grad_kernel(const T *dy, const T 
     }
 }
 
-// Columns of the partial rows, added in order: 32 columns and 8 runs of rows to a workgroup.
-constexpr uint32_t kJoinColumns = 32, kJoinRuns = kThreads / kJoinColumns;
-__global__ __launch_bounds__(kThreads) void ln_grad_join_kernel(const float *partial, float *dgamma, float *dbeta, uint32_t parts,
-                                                                uint32_t dim) {
-    __shared__ float lds[kJoinRuns][kJoinColumns];
+// Columns of the partial rows, added in order: 32 columns and 32 runs of rows to a workgroup.
+constexpr uint32_t kJoinThreads = 1024, kJoinColumns = 32, kJoinRuns = kJoinThreads / kJoinColumns;
+__global__ __launch_bounds__(kJoinThreads) void ln_grad_join_kernel(const float *partial, float *dgamma, float *dbeta, uint32_t parts,
+                                                                    uint32_t dim) {
+    __shared__ float lds[kJoinRuns][kJoinColumns + 1];
     const uint32_t lane = threadIdx.x % kJoinColumns, run = threadIdx.x / kJoinColumns;
     const uint32_t col = blockIdx.x * kJoinColumns + lane;  // of [dgamma | dbeta]
     float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     if (col < 2 * dim) {
         const uint32_t each = (parts + kJoinRuns - 1) / kJoinRuns, last = min(parts, (run + 1) * each);
         uint32_t p = run * each;
-        for (; p + 4 <= last; p += 4)
+        for (; p + 8 <= last; p += 8)
 #pragma unroll
-            for (int i = 0; i < 4; i++) t[i] += partial[(size_t)(p + i) * 2 * dim + col];
+            for (int i = 0; i < 8; i++) t[i % 4] += partial[(size_t)(p + i) * 2 * dim + col];
         for (; p < last; p++) t[0] += partial[(size_t)p * 2 * dim + col];
     }
     lds[run][lane] = (t[0] + t[1]) + (t[2] + t[3]);
@@ -292,7 +292,7 @@ Plan make_plan(size_t elt, size_t rows, size_t dim, bool aligned) {
     }
     if (p.tl == 0) return p;
     const size_t teams = kThreads / p.tl, most = (rows + teams - 1) / teams;
-    p.blocks = (uint32_t)std::max<size_t>(1, std::min<size_t>(most, 4 * (size_t)chip_info().cus));
+    p.blocks = (uint32_t)std::max<size_t>(1, std::min<size_t>(most, 2 * (size_t)chip_info().cus));
     return p;
 }
 
@@ -390,7 +390,7 @@ int ln_grad_dispatch(const LnGrad &g, size_t rows, size_t dim, float eps, hipStr
         launch_scalars<T, 256>(a, p);
     }
     if (affine)
-        launch(ln_grad_join_kernel, dim3((2 * a.dim + kJoinColumns - 1) / kJoinColumns), dim3(kThreads), 0, stream, partial, g.dgamma,
+        launch(ln_grad_join_kernel, dim3((2 * a.dim + kJoinColumns - 1) / kJoinColumns), dim3(kJoinThreads), 0, stream, partial, g.dgamma,
                g.dbeta, p.blocks, a.dim);
     return launch_status();
 }

@@ -213,13 +213,13 @@ struct AttnProblem {
 size_t attn_workspace_bytes(const AttnProblem &p);
 template <typename T>
 int attn_dispatch(const AttnProblem &p, const AttnView &q, const AttnView &k, const AttnView &v, const AttnView &out, float *lse,
-                  void *workspace, hipStream_t stream);
+                  void *rest, void *workspace, hipStream_t stream);
 struct AttnGradViews {
     AttnView q, k, v, out, dout, dq, dk, dv;
 };
 size_t attn_grad_workspace_bytes(const AttnProblem &p);
 template <typename T>
-int attn_grad_dispatch(const AttnProblem &p, const AttnGradViews &g, const float *lse, void *workspace, hipStream_t stream);
+int attn_grad_dispatch(const AttnProblem &p, const AttnGradViews &g, const float *lse, const void *rest, void *workspace, hipStream_t stream);
 template <typename T>
 int add_dispatch(const void *a, const void *b, void *c, size_t n, size_t chunk_size,
                  hipStream_t stream);  // chunk_size 0: elementwise; else b holds one value per chunk

@@ -1,11 +1,14 @@
 // Token embedding and its gradient for gfx950.
 //     y[i] = scale * table[ids[i]] + positions[i % length]
 //     dtable[v] = scale * (sum of dy[i] over the i with ids[i] = v),   dpositions[p] = sum of dy[i] over the i with i % length = p
-// Tokens are few next to what their rows hold, so the gradient first sorts them (stable, by digits of 9 bits) and then every
-// row of dtable is written once by one wavefront, which adds its token's rows of dy in ascending order in float32: no atomics,
-// the same bits every time.  A token that comes more often than kSlab times (padding; a few words are most of a text) is cut
-// into parts, whose sums a second launch adds.  Tokens outside [0, vocab) have rows of zeros and no gradient.
+// Tokens are few next to what their rows hold, so the gradient first sorts them (stable, by digits of 9 bits); a wavefront then
+// takes kSlab sorted tokens and adds their rows of dy, runs of one token in ascending order in float32.  A run that lies in one
+// slab is a row of dtable; a run over several leaves a part in each (padding; a few words are most of a text), and the last
+// launch adds those: no atomics, the same bits every time, and no token costs more than its share.  The rows that no token names,
+// and the sums over the batch for dpositions, are the work of workgroups beside the sort's, whose few ones mostly wait.
+// Tokens outside [0, vocab) have rows of zeros and no gradient.
 #include <algorithm>
+#include <initializer_list>
 
 #include "msd_device.h"
 #include "msd_internal.h"
@@ -17,20 +20,24 @@ constexpr uint32_t kThreads = 256;
 
 // ---- forward ---------------------------------------------------------------
 
-// N elements per lane: a 16-byte vector, or one element where rows are no whole vectors or not aligned to them.
+// N elements per lane: 16 or 8 bytes, or one element where rows are no whole pieces of those or not aligned to them.
 template <typename T, int N>
 __device__ __forceinline__ void load_piece(const T *p, float (&f)[N]) {
-    if constexpr (N == 1)
-        f[0] = Store<T>::load1(p);
-    else
-        Store<T>::unpack(*reinterpret_cast<const u32x4 *>(p), f);
+    T v[N];
+    __builtin_memcpy(v, __builtin_assume_aligned(p, sizeof(v)), sizeof(v));
+#pragma unroll
+    for (int e = 0; e < N; e++) f[e] = Store<T>::load1(v + e);
 }
 template <typename T, int N>
 __device__ __forceinline__ void store_piece(T *p, const float (&f)[N]) {
-    if constexpr (N == 1)
-        Store<T>::store1(p, f[0]);
-    else
-        store_stream(reinterpret_cast<u32x4 *>(p), Store<T>::pack(f));
+    T v[N];
+#pragma unroll
+    for (int e = 0; e < N; e++) Store<T>::store1(v + e, f[e]);
+    if constexpr (sizeof(v) == 16) {
+        store_stream(reinterpret_cast<u32x4 *>(p), __builtin_bit_cast(u32x4, v));
+    } else {
+        __builtin_memcpy(__builtin_assume_aligned(p, sizeof(v)), v, sizeof(v));
+    }
 }
 
 // 1 << shift adjacent lanes to a token.
@@ -60,10 +67,74 @@ __global__ __launch_bounds__(kThreads) void embed_kernel(const int64_t *ids, con
     }
 }
 
-// ---- sort --------------------------------------------------------------------
+// ---- beside the sort ---------------------------------------------------------
 constexpr uint32_t kSortThreads = 1024, kSortWaves = kSortThreads / kWave;
-constexpr uint32_t kSortRounds = 4;  // tokens per lane
-constexpr uint32_t kSortBlock = kSortThreads * kSortRounds;
+
+// Work of the workgroups behind the sort's own: zeros to dtable, and dpositions' partial sums over runs of the batch.
+struct Side {
+    char *zeros;             // (null: none in this launch)
+    size_t zero_bytes;       // (a share of dtable: whole 16-byte vectors from its beginning on, but for the last)
+    uint32_t zero_blocks;
+    const void *dy;
+    float *position_parts;   // [runs][length][dim], null: none in this launch
+    uint32_t batch, length, pieces, run_blocks, runs;
+    int piece;               // elements of a piece
+};
+
+template <typename T, int N>
+__device__ __forceinline__ void positions_parts(const Side &w, uint32_t block) {
+    const uint32_t run = block / w.run_blocks;
+    const uint64_t count = (uint64_t)w.length * w.pieces, i = (uint64_t)(block - run * w.run_blocks) * kSortThreads + threadIdx.x;
+    if (i >= count) return;
+    const T *const dy = static_cast<const T *>(w.dy) + i * N;
+    const size_t step = (size_t)w.length * w.pieces * N;
+    const uint32_t each = (w.batch + w.runs - 1) / w.runs, stop = min(w.batch, (run + 1) * each);
+    float sum[N];
+#pragma unroll
+    for (int e = 0; e < N; e++) sum[e] = 0.0f;
+    uint32_t b = run * each;
+    for (; b + 8 <= stop; b += 8) {
+        float f[8][N];
+#pragma unroll
+        for (uint32_t u = 0; u < 8; u++) load_piece<T, N>(dy + (b + u) * step, f[u]);
+#pragma unroll
+        for (uint32_t u = 0; u < 8; u++)
+#pragma unroll
+            for (int e = 0; e < N; e++) sum[e] += f[u][e];
+    }
+    for (; b < stop; b++) {
+        float f[N];
+        load_piece<T, N>(dy + b * step, f);
+#pragma unroll
+        for (int e = 0; e < N; e++) sum[e] += f[e];
+    }
+    float *const out = w.position_parts + ((size_t)run * count + i) * N;
+#pragma unroll
+    for (int e = 0; e < N; e++) out[e] = sum[e];
+}
+
+template <typename T>
+__device__ __forceinline__ void side_work(const Side &w, uint32_t block) {
+    if (block < w.zero_blocks) {
+        const size_t at = (size_t)block * kSortThreads + threadIdx.x, step = (size_t)w.zero_blocks * kSortThreads;
+        size_t vectors = w.zero_bytes / 16;
+        if ((reinterpret_cast<uintptr_t>(w.zeros) & 15u) != 0) vectors = 0;
+        for (size_t i = at; i < vectors; i += step) reinterpret_cast<u32x4 *>(w.zeros)[i] = u32x4{0, 0, 0, 0};
+        for (size_t i = vectors * (16 / sizeof(T)) + at; i < w.zero_bytes / sizeof(T); i += step)
+            Store<T>::store1(reinterpret_cast<T *>(w.zeros) + i, 0.0f);
+        return;
+    }
+    block -= w.zero_blocks;
+    constexpr int V = Store<T>::EPV;
+    if (w.piece == V)
+        positions_parts<T, V>(w, block);
+    else if (w.piece == V / 2)
+        positions_parts<T, V / 2>(w, block);
+    else
+        positions_parts<T, 1>(w, block);
+}
+
+// ---- sort --------------------------------------------------------------------
 constexpr uint32_t kDigitBits = 9, kBins = 1u << kDigitBits;
 
 struct Entry {  // a token and its place
@@ -76,16 +147,17 @@ __device__ __forceinline__ uint32_t key_of(const int64_t *ids, uint32_t i, uint3
     return id >= 0 && id < (int64_t)vocab ? (uint32_t)id : vocab;
 }
 
-// How many of a block's tokens have each digit before this one: wavefront w has the tokens [w * 256, w * 256 + 256) of the block
-// in rounds of 64.  counts[w][bin] ends as the wavefront's count; rank[r] is the token's place among those of its wavefront
+// How many of a block's tokens have each digit before this one: a wavefront has ROUNDS times 64 neighbouring tokens of the block.
+// counts[w][bin] ends as the wavefront's count; rank[r] is the token's place among those of its wavefront
 // and digit.  Lanes of a digit find each other by a ballot for each of its bits; the lowest of them moves the counter.
-__device__ __forceinline__ void rank_digits(uint16_t (*counts)[kBins], const uint32_t (&digit)[kSortRounds],
-                                            const bool (&live)[kSortRounds], uint32_t (&rank)[kSortRounds]) {
+template <uint32_t ROUNDS>
+__device__ __forceinline__ void rank_digits(uint16_t (*counts)[kBins], const uint32_t (&digit)[ROUNDS], const bool (&live)[ROUNDS],
+                                            uint32_t (&rank)[ROUNDS]) {
     const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     for (uint32_t i = lane; i < kBins; i += kWave) counts[wave][i] = 0;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-    for (uint32_t r = 0; r < kSortRounds; r++) {
+    for (uint32_t r = 0; r < ROUNDS; r++) {
         uint64_t same = __builtin_amdgcn_ballot_w64(live[r]);
 #pragma unroll
         for (uint32_t bit = 0; bit < kDigitBits; bit++) {
@@ -135,38 +207,40 @@ __device__ __forceinline__ uint32_t before_bins(uint32_t v, uint32_t *slots) {
     return base + up - v;
 }
 
-// Up to kSortBlock tokens: one workgroup, all digits, the tokens in LDS between them.
+// Up to ROUNDS * 1024 tokens: one workgroup, all digits, the tokens in LDS between them.
+template <typename T, uint32_t ROUNDS>
 __global__ __launch_bounds__(kSortThreads) void sort_small_kernel(const int64_t *ids, Entry *sorted, uint32_t tokens, uint32_t vocab,
-                                                                  uint32_t digits) {
+                                                                  uint32_t digits, const Side side) {
+    if (blockIdx.x != 0) return side_work<T>(side, blockIdx.x - 1);
     __shared__ uint16_t counts[kSortWaves][kBins];
     __shared__ uint32_t start[kBins], slots[kBins / kWave];
-    __shared__ Entry entries[kSortBlock];
+    __shared__ Entry entries[(kSortThreads * ROUNDS)];
     const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    uint32_t id[kSortRounds], at[kSortRounds], digit[kSortRounds], rank[kSortRounds];
-    bool live[kSortRounds];
+    uint32_t id[ROUNDS], at[ROUNDS], digit[ROUNDS], rank[ROUNDS];
+    bool live[ROUNDS];
 #pragma unroll
-    for (uint32_t r = 0; r < kSortRounds; r++) {
-        const uint32_t i = wave * (kWave * kSortRounds) + r * kWave + lane;
+    for (uint32_t r = 0; r < ROUNDS; r++) {
+        const uint32_t i = wave * (kWave * ROUNDS) + r * kWave + lane;
         live[r] = i < tokens;
         at[r] = i;
         id[r] = live[r] ? key_of(ids, i, vocab) : 0;
     }
     for (uint32_t pass = 0; pass < digits; pass++) {
 #pragma unroll
-        for (uint32_t r = 0; r < kSortRounds; r++) digit[r] = id[r] >> (pass * kDigitBits) & (kBins - 1);
-        rank_digits(counts, digit, live, rank);
+        for (uint32_t r = 0; r < ROUNDS; r++) digit[r] = id[r] >> (pass * kDigitBits) & (kBins - 1);
+        rank_digits<ROUNDS>(counts, digit, live, rank);
         __syncthreads();
         const uint32_t total = before_waves(counts);
         const uint32_t first = before_bins(total, slots);
         if (threadIdx.x < kBins) start[threadIdx.x] = first;
         __syncthreads();
 #pragma unroll
-        for (uint32_t r = 0; r < kSortRounds; r++)
+        for (uint32_t r = 0; r < ROUNDS; r++)
             if (live[r]) entries[start[digit[r]] + counts[wave][digit[r]] + rank[r]] = Entry{id[r], at[r]};
         __syncthreads();
 #pragma unroll
-        for (uint32_t r = 0; r < kSortRounds; r++) {
-            const uint32_t i = wave * (kWave * kSortRounds) + r * kWave + lane;
+        for (uint32_t r = 0; r < ROUNDS; r++) {
+            const uint32_t i = wave * (kWave * ROUNDS) + r * kWave + lane;
             if (live[r]) {
                 const Entry e = entries[i];
                 id[r] = e.id;
@@ -175,16 +249,17 @@ __global__ __launch_bounds__(kSortThreads) void sort_small_kernel(const int64_t 
         }
     }
 #pragma unroll
-    for (uint32_t r = 0; r < kSortRounds; r++)
-        if (live[r]) sorted[wave * (kWave * kSortRounds) + r * kWave + lane] = Entry{id[r], at[r]};
+    for (uint32_t r = 0; r < ROUNDS; r++)
+        if (live[r]) sorted[wave * (kWave * ROUNDS) + r * kWave + lane] = Entry{id[r], at[r]};
 }
 
 // A block's tokens in front of a pass: from the ids, or from the pass before.
-__device__ __forceinline__ void block_entries(const int64_t *ids, const Entry *from, uint32_t tokens, uint32_t vocab, Entry (&e)[kSortRounds],
-                                              bool (&live)[kSortRounds]) {
+template <uint32_t ROUNDS>
+__device__ __forceinline__ void block_entries(const int64_t *ids, const Entry *from, uint32_t tokens, uint32_t vocab, Entry (&e)[ROUNDS],
+                                              bool (&live)[ROUNDS]) {
 #pragma unroll
-    for (uint32_t r = 0; r < kSortRounds; r++) {
-        const uint32_t i = blockIdx.x * kSortBlock + threadIdx.x / kWave * (kWave * kSortRounds) + r * kWave + threadIdx.x % kWave;
+    for (uint32_t r = 0; r < ROUNDS; r++) {
+        const uint32_t i = blockIdx.x * (kSortThreads * ROUNDS) + threadIdx.x / kWave * (kWave * ROUNDS) + r * kWave + threadIdx.x % kWave;
         live[r] = i < tokens;
         e[r] = Entry{0, i};
         if (live[r]) e[r] = from != nullptr ? from[i] : Entry{key_of(ids, i, vocab), i};
@@ -192,38 +267,44 @@ __device__ __forceinline__ void block_entries(const int64_t *ids, const Entry *f
 }
 
 // table[block][bin]: how many of the block's tokens have that digit.
+template <typename T, uint32_t ROUNDS>
 __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(const int64_t *ids, const Entry *from, uint32_t *table, uint32_t tokens,
-                                                                  uint32_t vocab, uint32_t shift) {
+                                                                  uint32_t vocab, uint32_t shift, uint32_t blocks, const Side side) {
+    if (blockIdx.x >= blocks) return side_work<T>(side, blockIdx.x - blocks);
     __shared__ uint32_t bins[kBins];
     if (threadIdx.x < kBins) bins[threadIdx.x] = 0;
     __syncthreads();
-    Entry e[kSortRounds];
-    bool live[kSortRounds];
-    block_entries(ids, from, tokens, vocab, e, live);
+    Entry e[ROUNDS];
+    bool live[ROUNDS];
+    block_entries<ROUNDS>(ids, from, tokens, vocab, e, live);
 #pragma unroll
-    for (uint32_t r = 0; r < kSortRounds; r++)
+    for (uint32_t r = 0; r < ROUNDS; r++)
         if (live[r]) atomicAdd(&bins[e[r].id >> shift & (kBins - 1)], 1u);  // (whole numbers: any order gives the same)
     __syncthreads();
     if (threadIdx.x < kBins) table[(size_t)blockIdx.x * kBins + threadIdx.x] = bins[threadIdx.x];
 }
 
 // Every block adds the table's columns for itself: what lies before it in its bins, and the bins' totals.
+template <typename T, uint32_t ROUNDS>
 __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(const int64_t *ids, const Entry *from, const uint32_t *table, Entry *to,
-                                                                  uint32_t tokens, uint32_t vocab, uint32_t shift) {
+                                                                  uint32_t tokens, uint32_t vocab, uint32_t shift, uint32_t blocks,
+                                                                  const Side side) {
+    if (blockIdx.x >= blocks) return side_work<T>(side, blockIdx.x - blocks);
     __shared__ uint16_t counts[kSortWaves][kBins];
     __shared__ uint32_t start[kBins], half[2][kBins], slots[kBins / kWave];
     const uint32_t wave = threadIdx.x / kWave;
-    Entry e[kSortRounds];
-    bool live[kSortRounds];
-    uint32_t digit[kSortRounds], rank[kSortRounds];
-    block_entries(ids, from, tokens, vocab, e, live);
+    Entry e[ROUNDS];
+    bool live[ROUNDS];
+    uint32_t digit[ROUNDS], rank[ROUNDS];
+    block_entries<ROUNDS>(ids, from, tokens, vocab, e, live);
 #pragma unroll
-    for (uint32_t r = 0; r < kSortRounds; r++) digit[r] = e[r].id >> shift & (kBins - 1);
-    rank_digits(counts, digit, live, rank);
+    for (uint32_t r = 0; r < ROUNDS; r++) digit[r] = e[r].id >> shift & (kBins - 1);
+    rank_digits<ROUNDS>(counts, digit, live, rank);
     // two threads to a bin: the even blocks' counts and the odd ones'
     const uint32_t bin = threadIdx.x % kBins, odd = threadIdx.x / kBins;
     uint32_t all = 0, mine = 0;
-    for (uint32_t b = odd; b < gridDim.x; b += 2) {
+    #pragma unroll 8
+    for (uint32_t b = odd; b < blocks; b += 2) {
         const uint32_t c = table[(size_t)b * kBins + bin];
         all += c;
         mine += b < blockIdx.x ? c : 0;
@@ -244,13 +325,12 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(const int64_t 
     if (odd == 0) start[bin] = first + mine;
     __syncthreads();
 #pragma unroll
-    for (uint32_t r = 0; r < kSortRounds; r++)
+    for (uint32_t r = 0; r < ROUNDS; r++)
         if (live[r]) to[start[digit[r]] + counts[wave][digit[r]] + rank[r]] = e[r];
 }
 
 // ---- sums ----------------------------------------------------------------------
-constexpr uint32_t kSlab = 64;  // sorted tokens of a part; a token that comes more often is long
-constexpr uint32_t kRows = 8;   // rows of dtable per wavefront
+constexpr uint32_t kSlab = 16;  // sorted tokens of a wavefront
 
 // First place in sorted[0, tokens) whose id is at least v; the whole wavefront looks, 64 places at a time.
 __device__ __forceinline__ uint32_t first_of(const Entry *sorted, uint32_t tokens, uint32_t v) {
@@ -269,162 +349,132 @@ __device__ __forceinline__ uint32_t first_of(const Entry *sorted, uint32_t token
     return low;
 }
 
-// Adds scale * dy of sorted[from, to) into one row, in order.  A lane has the pieces lane, lane + 64, ...
-template <typename T, int N, typename Put>
-__device__ __forceinline__ void add_rows(const T *dy, const Entry *sorted, uint32_t from, uint32_t to, uint32_t pieces, Put put) {
-    const size_t dim = (size_t)pieces * N;
-    for (uint32_t p = threadIdx.x % kWave; p < pieces; p += kWave) {
-        float sum[N];
-#pragma unroll
-        for (int e = 0; e < N; e++) sum[e] = 0.0f;
-        uint32_t i = from;
-        for (; i + 4 <= to; i += 4) {
-            float f[4][N];
-#pragma unroll
-            for (int u = 0; u < 4; u++) load_piece<T, N>(dy + (size_t)sorted[i + u].at * dim + (size_t)p * N, f[u]);
-#pragma unroll
-            for (int u = 0; u < 4; u++)
-#pragma unroll
-                for (int e = 0; e < N; e++) sum[e] += f[u][e];
-        }
-        for (; i < to; i++) {
-            float f[N];
-            load_piece<T, N>(dy + (size_t)sorted[i].at * dim + (size_t)p * N, f);
-#pragma unroll
-            for (int e = 0; e < N; e++) sum[e] += f[e];
-        }
-        put(p, sum);
-    }
-}
-
-// Wavefronts [0, ceil(vocab / kRows)): the rows of dtable, long tokens' left out.  The following ceil(tokens / kSlab): the parts
-// of long tokens in the sorted tokens' slabs, parts[slab][2][dim]: what comes in from the slab before, and what starts in it.
+// A wavefront's slab and 64 of its pieces (few tokens of long rows are work for many wavefronts): parts[slab][2][dim] receives the run that comes in from the slab before, and the one that starts in it and
+// goes on in the next; runs that begin and end here are rows of dtable.
 template <typename T, int N>
-__global__ __launch_bounds__(kThreads) void embed_grad_rows_kernel(const T *dy, const Entry *sorted, T *dtable, float *parts, uint32_t tokens,
-                                                                   uint32_t pieces, uint32_t vocab, float scale) {
+__global__ __launch_bounds__(kThreads) void embed_grad_slabs_kernel(const T *dy, const Entry *sorted, T *dtable, float *parts, uint32_t tokens,
+                                                                    uint32_t pieces, uint32_t vocab, float scale, uint32_t chunks) {
     const uint32_t wave = __builtin_amdgcn_readfirstlane(blockIdx.x * (kThreads / kWave) + threadIdx.x / kWave);
-    const uint32_t owners = (vocab + kRows - 1) / kRows;
-    const size_t dim = (size_t)pieces * N;
-    if (wave < owners) {
-        uint32_t at = __builtin_amdgcn_readfirstlane(first_of(sorted, tokens, wave * kRows));
-        for (uint32_t v = wave * kRows; v < min(vocab, (wave + 1) * kRows); v++) {
-            // (the row's tokens: at most kSlab of them, or it is left to its parts)
-            const uint32_t lane = threadIdx.x % kWave;
-            const bool mine = at + lane < tokens && sorted[at + lane].id == v;
-            const uint32_t n = __builtin_popcountll(__builtin_amdgcn_ballot_w64(mine));
-            if (n == kSlab && at + kSlab < tokens && sorted[at + kSlab].id == v) {
-                at = __builtin_amdgcn_readfirstlane(first_of(sorted, tokens, v + 1));
-                continue;
-            }
-            add_rows<T, N>(dy, sorted, at, at + n, pieces, [&](uint32_t p, const float (&sum)[N]) {
-                float f[N];
-#pragma unroll
-                for (int e = 0; e < N; e++) f[e] = n != 0 ? sum[e] * scale : 0.0f;
-                store_piece<T, N>(dtable + (size_t)v * dim + (size_t)p * N, f);
-            });
-            at += n;
-        }
-        return;
-    }
-    const uint32_t slab = wave - owners, begin = slab * kSlab;
+    const uint32_t slab = wave / chunks, p0 = (wave - slab * chunks) * kWave;
+    const uint32_t begin = slab * kSlab, lane = threadIdx.x % kWave;
     if (begin >= tokens) return;
-    const uint32_t end = min(tokens, begin + kSlab);
-    auto part = [&](uint32_t from, uint32_t to, uint32_t which) {
-        float *const out = parts + ((size_t)slab * 2 + which) * dim;
-        add_rows<T, N>(dy, sorted, from, to, pieces, [&](uint32_t p, const float (&sum)[N]) {
-#pragma unroll
-            for (int e = 0; e < N; e++) out[(size_t)p * N + e] = sum[e];
-        });
-    };
-    const uint32_t lane = threadIdx.x % kWave;
-    const uint32_t id = begin + lane < end ? sorted[begin + lane].id : 0xFFFFFFFFu;
-    const uint32_t first = sorted[begin].id, last = sorted[end - 1].id;
-    if (begin != 0 && sorted[begin - 1].id == first && first < vocab) {
-        // is it long?  (it starts before this slab)
-        const uint32_t from = first_of(sorted, tokens, first);
-        if (from + kSlab < tokens && sorted[from + kSlab].id == first)
-            part(begin, begin + __builtin_popcountll(__builtin_amdgcn_ballot_w64(id == first)), 0);
-        if (first == last) return;
-    }
-    if (last < vocab) {
-        const uint32_t n = __builtin_popcountll(__builtin_amdgcn_ballot_w64(id == last && begin + lane < end));
-        const uint32_t from = end - n;
-        if (from + kSlab < tokens && sorted[from + kSlab].id == last) part(from, end, 1);
-    }
-}
-
-// A workgroup for a slab in which a long token starts, and for 64 of its columns: the four wavefronts add a quarter of its parts each.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void embed_grad_join_kernel(const Entry *sorted, const float *parts, T *dtable, uint32_t tokens,
-                                                                   uint32_t dim, uint32_t vocab, float scale) {
-    __shared__ float lds[kThreads / kWave][kWave];
-    const uint32_t begin = blockIdx.x * kSlab, end = min(tokens, begin + kSlab);
-    const uint32_t last = sorted[end - 1].id;
-    if (last >= vocab || (begin != 0 && sorted[begin - 1].id == last)) return;
-    const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    const uint32_t n = __builtin_popcountll(__builtin_amdgcn_ballot_w64(begin + lane < end && sorted[begin + lane].id == last));
-    const uint32_t from = end - n;
-    if (from + kSlab >= tokens || sorted[from + kSlab].id != last) return;
-    const uint32_t to = first_of(sorted, tokens, last + 1);
-    const uint32_t slabs = (to - 1) / kSlab - blockIdx.x;  // after this one
-    const uint32_t col = blockIdx.y * kWave + lane;
-    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (col < dim) {
-        if (wave == 0) sum[0] = parts[((size_t)blockIdx.x * 2 + 1) * dim + col];
-        const uint32_t each = (slabs + 3) / 4, stop = min(slabs, (wave + 1) * each);
-        uint32_t s = wave * each;
-        for (; s + 4 <= stop; s += 4)
-#pragma unroll
-            for (uint32_t u = 0; u < 4; u++) sum[u] += parts[((size_t)blockIdx.x + 1 + s + u) * 2 * dim + col];
-        for (; s < stop; s++) sum[0] += parts[((size_t)blockIdx.x + 1 + s) * 2 * dim + col];
-    }
-    lds[wave][lane] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-    __syncthreads();
-    if (wave != 0 || col >= dim) return;
-    Store<T>::store1(dtable + (size_t)last * dim + col, ((lds[0][lane] + lds[1][lane]) + (lds[2][lane] + lds[3][lane])) * scale);
-}
-
-// dpositions: runs of the batch to partial sums [runs][length][dim], one lane a piece of a row; the rows behind `length` are zero.
-template <typename T, int N>
-__global__ __launch_bounds__(kThreads) void positions_parts_kernel(const T *dy, float *parts, uint32_t batch, uint32_t length,
-                                                                   uint32_t pieces, uint32_t runs) {
-    const uint64_t count = (uint64_t)length * pieces, i = (uint64_t)blockIdx.x * kThreads + threadIdx.x;
-    if (i >= count) return;
+    const uint32_t n = min(kSlab, tokens - begin);
     const size_t dim = (size_t)pieces * N;
-    const uint32_t each = (batch + runs - 1) / runs, stop = min(batch, (blockIdx.y + 1) * each);
+    const Entry mine = sorted[begin + min(lane, n - 1)];
+    const uint32_t before = begin != 0 ? sorted[begin - 1].id : 0xFFFFFFFFu, after = begin + n < tokens ? sorted[begin + n].id : 0xFFFFFFFFu;
+    auto id_of = [&](uint32_t i) { return (uint32_t)__builtin_amdgcn_readlane(mine.id, i); };
+    if (id_of(0) >= vocab) return;  // (those outside the table come last)
+    const uint32_t p = min(p0 + lane, pieces - 1);
+    const bool in = p0 + lane < pieces;
     float sum[N];
 #pragma unroll
     for (int e = 0; e < N; e++) sum[e] = 0.0f;
-    uint32_t b = blockIdx.y * each;
-    for (; b + 4 <= stop; b += 4) {
-        float f[4][N];
+    auto put = [&](uint32_t id, bool first, bool last) {  // the run of `id` up to here
+        if (!in || id >= vocab) return;
+        if ((first && before == id) || (last && after == id)) {
+            float *const out = parts + ((size_t)slab * 2 + (first && before == id ? 0 : 1)) * dim + (size_t)p * N;
 #pragma unroll
-        for (uint32_t u = 0; u < 4; u++) load_piece<T, N>(dy + ((size_t)(b + u) * length) * dim + (size_t)i * N, f[u]);
+            for (int e = 0; e < N; e++) out[e] = sum[e];
+        } else {
 #pragma unroll
-        for (uint32_t u = 0; u < 4; u++)
+            for (int e = 0; e < N; e++) sum[e] *= scale;
+            store_piece<T, N>(dtable + (size_t)id * dim + (size_t)p * N, sum);
+        }
+    };
+    uint32_t id = id_of(0);
+    bool first = true;
+    for (uint32_t i0 = 0; i0 < n; i0 += 8) {
+        float f[8][N];
+#pragma unroll
+        for (uint32_t u = 0; u < 8; u++) {
+            const uint32_t at = (uint32_t)__builtin_amdgcn_readlane(mine.at, min(i0 + u, n - 1));
+            load_piece<T, N>(dy + (size_t)at * dim + (size_t)p * N, f[u]);
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < 8; u++) {
+            if (i0 + u >= n) break;
+            const uint32_t next = id_of(i0 + u);
+            if (next != id) {
+                put(id, first, false);
+#pragma unroll
+                for (int e = 0; e < N; e++) sum[e] = 0.0f;
+                id = next;
+                first = false;
+            }
 #pragma unroll
             for (int e = 0; e < N; e++) sum[e] += f[u][e];
+        }
     }
-    for (; b < stop; b++) {
-        float f[N];
-        load_piece<T, N>(dy + ((size_t)b * length) * dim + (size_t)i * N, f);
-#pragma unroll
-        for (int e = 0; e < N; e++) sum[e] += f[e];
-    }
-    float *const out = parts + ((size_t)blockIdx.y * count + i) * N;
-#pragma unroll
-    for (int e = 0; e < N; e++) out[e] = sum[e];
+    put(id, first, true);
 }
 
+constexpr uint32_t kJoinColumns = 4 * kWave;
+
+// A workgroup for kSortWaves slabs and kJoinColumns columns, a wavefront looking at each slab: of a run that starts in one and goes on, the
+// wavefronts add a share of the parts each.  The workgroups behind `blocks` add dpositions' parts.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void positions_join_kernel(const float *parts, T *dpositions, uint64_t live, uint64_t count,
-                                                                  uint32_t runs) {
-    const uint64_t i = (uint64_t)blockIdx.x * kThreads + threadIdx.x;
-    if (i >= count) return;
-    float sum = 0.0f;
-    if (i < live)
-        for (uint32_t r = 0; r < runs; r++) sum += parts[(size_t)r * live + i];
-    Store<T>::store1(dpositions + i, sum);
+__global__ __launch_bounds__(kSortThreads) void embed_grad_join_kernel(const Entry *sorted, const float *parts, T *dtable, uint32_t tokens,
+                                                                       uint32_t dim, uint32_t vocab, float scale, uint32_t columns,
+                                                                       uint32_t blocks, const float *position_parts, T *dpositions,
+                                                                       uint64_t live, uint64_t count, uint32_t runs) {
+    if (blockIdx.x >= blocks) {
+        const uint64_t i = (uint64_t)(blockIdx.x - blocks) * kSortThreads + threadIdx.x;
+        if (i >= count) return;
+        float sum = 0.0f;
+        if (i < live) {
+#pragma unroll 4
+            for (uint32_t r = 0; r < runs; r++) sum += position_parts[(size_t)r * live + i];
+        }
+        Store<T>::store1(dpositions + i, sum);
+        return;
+    }
+    __shared__ float lds[kSortWaves][kJoinColumns];
+    __shared__ uint32_t run_id[kSortWaves], run_slabs[kSortWaves];  // (slabs behind the first that the run reaches; 0: no run)
+    const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    const uint32_t slab0 = blockIdx.x / columns * kSortWaves, col0 = blockIdx.x % columns * kJoinColumns;
+    {
+        const uint32_t slab = slab0 + wave, begin = slab * kSlab;
+        uint32_t id = 0, more = 0;
+        if (begin < tokens && begin + kSlab < tokens) {
+            id = sorted[begin + kSlab - 1].id;
+            const bool here = begin == 0 || sorted[begin - 1].id != id;  // (it starts in this slab)
+            if (here && id < vocab && sorted[begin + kSlab].id == id) more = (first_of(sorted, tokens, id + 1) - 1) / kSlab - slab;
+        }
+        if (lane == 0) {
+            run_id[wave] = id;
+            run_slabs[wave] = more;
+        }
+    }
+    __syncthreads();
+    for (uint32_t s = 0; s < kSortWaves; s++) {
+        const uint32_t slabs = run_slabs[s], slab = slab0 + s;
+        if (slabs == 0) continue;
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const uint32_t each = (slabs + kSortWaves - 1) / kSortWaves, stop = min(slabs, (wave + 1) * each);
+        auto add = [&](size_t part) {
+#pragma unroll
+            for (uint32_t c = 0; c < 4; c++) {
+                const uint32_t col = col0 + c * kWave + lane;
+                sum[c] += col < dim ? parts[part * dim + col] : 0.0f;
+            }
+        };
+        if (wave == 0) add((size_t)slab * 2 + 1);
+        uint32_t i = wave * each;
+        for (; i + 4 <= stop; i += 4)
+#pragma unroll
+            for (uint32_t u = 0; u < 4; u++) add(((size_t)slab + 1 + i + u) * 2);
+        for (; i < stop; i++) add(((size_t)slab + 1 + i) * 2);
+#pragma unroll
+        for (uint32_t c = 0; c < 4; c++) lds[wave][c * kWave + lane] = sum[c];
+        __syncthreads();
+        if (threadIdx.x < kJoinColumns && col0 + threadIdx.x < dim) {
+            float total = 0.0f;
+#pragma unroll
+            for (uint32_t w = 0; w < kSortWaves; w++) total += lds[w][threadIdx.x];
+            Store<T>::store1(dtable + (size_t)run_id[s] * dim + col0 + threadIdx.x, total * scale);
+        }
+        __syncthreads();
+    }
 }
 
 uint32_t sort_digits(size_t vocab) {
@@ -433,10 +483,13 @@ uint32_t sort_digits(size_t vocab) {
     return (bits + kDigitBits - 1) / kDigitBits;
 }
 
-// Workspace: the sorted tokens twice (passes go from one to the other), the digits' table, the parts of long tokens, those of positions.
+// Tokens per lane of the sort: four where one would make more workgroups than a chip has CUs by far, whose counts each adds for itself.
+uint32_t sort_rounds(size_t tokens) { return tokens <= kSortThreads || (tokens > 4 * kSortThreads && tokens <= 128 * kSortThreads) ? 1 : 4; }
+
+// Workspace: the sorted tokens twice (passes go from one to the other), the digits' table, the parts of runs, those of positions.
 struct Layout {
     size_t entries[2], table, parts, position_parts, bytes;
-    uint32_t blocks, digits, runs;
+    uint32_t blocks, rounds, digits, runs;
 };
 Layout layout(size_t tokens, size_t length, size_t vocab, size_t positions, size_t dim) {
     Layout l{};
@@ -445,7 +498,8 @@ Layout layout(size_t tokens, size_t length, size_t vocab, size_t positions, size
         l.bytes += (bytes + 255) & ~(size_t)255;
         return at;
     };
-    l.blocks = (uint32_t)((tokens + kSortBlock - 1) / kSortBlock);
+    l.rounds = sort_rounds(tokens);
+    l.blocks = (uint32_t)((tokens + kSortThreads * l.rounds - 1) / (kSortThreads * l.rounds));
     l.digits = sort_digits(vocab);
     l.entries[0] = take(tokens * sizeof(Entry));
     if (l.blocks > 1) {
@@ -463,83 +517,133 @@ Layout layout(size_t tokens, size_t length, size_t vocab, size_t positions, size
     return l;
 }
 
+template <typename T, uint32_t ROUNDS>
+void sort_tokens(const EmbedGrad &g, const Layout &l, Entry *const (&entries)[2], uint32_t *table, const Entry **sorted, uint32_t tokens,
+                 uint32_t vocab, size_t table_bytes, Side side, hipStream_t stream) {
+    const uint32_t launches = l.blocks > 1 ? 2 * l.digits : 1;
+    // a share of the zeros to every launch, positions' sums to the first
+    const size_t share = (table_bytes / 16 + launches - 1) / launches * 16;
+    auto next = [&](uint32_t launch) {
+        const size_t from = std::min(table_bytes, launch * share);
+        side.zeros = static_cast<char *>(g.dtable) + from;
+        side.zero_bytes = launch + 1 == launches ? table_bytes - from : std::min(share, table_bytes - from);
+        side.zero_blocks = (uint32_t)std::min<size_t>((side.zero_bytes / 16 + 4 * kSortThreads - 1) / (4 * kSortThreads) + 1, 1024);
+        if (launch != 0) side.position_parts = nullptr;
+        return l.blocks + side.zero_blocks + (side.position_parts != nullptr ? side.run_blocks * side.runs : 0);
+    };
+    if (l.blocks <= 1) {
+        const uint32_t blocks = next(0) + 1 - l.blocks;  // (no tokens: the sort's workgroup finds none)
+        launch((sort_small_kernel<T, ROUNDS>), dim3(blocks), dim3(kSortThreads), 0, stream, g.ids, entries[0], tokens, vocab, l.digits, side);
+        *sorted = entries[0];
+        return;
+    }
+    const Entry *from = nullptr;
+    for (uint32_t pass = 0; pass < l.digits; pass++) {
+        Entry *const to = entries[pass % 2];
+        const uint32_t counting = next(2 * pass);
+        launch((sort_count_kernel<T, ROUNDS>), dim3(counting), dim3(kSortThreads), 0, stream, g.ids, from, table, tokens, vocab,
+               pass * kDigitBits, l.blocks, side);
+        const uint32_t placing = next(2 * pass + 1);
+        launch((sort_place_kernel<T, ROUNDS>), dim3(placing), dim3(kSortThreads), 0, stream, g.ids, from, table, to, tokens, vocab,
+               pass * kDigitBits, l.blocks, side);
+        from = to;
+    }
+    *sorted = from;
+}
+
 }  // namespace
 
 size_t embed_grad_workspace_bytes(size_t tokens, size_t length, size_t vocab, size_t positions, size_t dim) {
     return layout(tokens, length, vocab, positions, dim).bytes;
 }
 
+// Elements per piece: the widest of 16 and 8 bytes that rows are whole ones of, aligned, or 1.
+template <typename T>
+static int piece_of(size_t dim, std::initializer_list<const void *> at) {
+    for (int n = Store<T>::EPV; n >= Store<T>::EPV / 2; n /= 2) {
+        bool fits = dim % n == 0;
+        for (const void *p : at) fits = fits && reinterpret_cast<uintptr_t>(p) % (n * sizeof(T)) == 0;
+        if (fits) return n;
+    }
+    return 1;
+}
+
+template <typename T, int N>
+static void embed_rows(const int64_t *ids, const void *table, const void *positions, void *y, size_t tokens, size_t length, size_t vocab,
+                       size_t dim, float scale, hipStream_t stream) {
+    const size_t pieces = dim / N;
+    uint32_t shift = 0;
+    while (shift < 6 && (size_t(1) << shift) < pieces) shift++;
+    launch((embed_kernel<T, N>), dim3((uint32_t)(((tokens << shift) + kThreads - 1) / kThreads)), dim3(kThreads), 0, stream, ids,
+           static_cast<const T *>(table), static_cast<const T *>(positions), static_cast<T *>(y), (uint32_t)tokens, (uint32_t)pieces,
+           (uint32_t)length, (uint32_t)vocab, scale, shift);
+}
+
 template <typename T>
 int embed_dispatch(const int64_t *ids, const void *table, const void *positions, void *y, size_t tokens, size_t length, size_t vocab,
                    size_t dim, float scale, hipStream_t stream) {
-    constexpr int N = Store<T>::EPV;
-    const T *t = static_cast<const T *>(table), *p = static_cast<const T *>(positions);
-    const bool vectors = dim % N == 0 && aligned16(table) && aligned16(positions) && aligned16(y);
-    const size_t pieces = vectors ? dim / N : dim;
-    uint32_t shift = 0;
-    while (shift < 6 && (size_t(1) << shift) < pieces) shift++;
-    const dim3 grid((uint32_t)(((tokens << shift) + kThreads - 1) / kThreads));
-    if (vectors)
-        launch((embed_kernel<T, N>), grid, dim3(kThreads), 0, stream, ids, t, p, static_cast<T *>(y), (uint32_t)tokens,
-               (uint32_t)pieces, (uint32_t)length, (uint32_t)vocab, scale, shift);
-    else
-        launch((embed_kernel<T, 1>), grid, dim3(kThreads), 0, stream, ids, t, p, static_cast<T *>(y), (uint32_t)tokens,
-               (uint32_t)pieces, (uint32_t)length, (uint32_t)vocab, scale, shift);
+    constexpr int V = Store<T>::EPV;
+    switch (piece_of<T>(dim, {table, positions, y})) {
+        case V: embed_rows<T, V>(ids, table, positions, y, tokens, length, vocab, dim, scale, stream); break;
+        case V / 2: embed_rows<T, V / 2>(ids, table, positions, y, tokens, length, vocab, dim, scale, stream); break;
+        default: embed_rows<T, 1>(ids, table, positions, y, tokens, length, vocab, dim, scale, stream); break;
+    }
     return launch_status();
 }
 
 template <typename T, int N>
-static void embed_grad_rows(const EmbedGrad &g, const Entry *sorted, float *parts, const Layout &l, size_t tokens, size_t length, size_t dim,
-                            size_t vocab, float *position_parts, float scale, hipStream_t stream) {
-    const T *dy = static_cast<const T *>(g.dy);
-    const uint32_t pieces = (uint32_t)(dim / N);
-    const size_t waves = (vocab + kRows - 1) / kRows + (tokens + kSlab - 1) / kSlab, per = kThreads / kWave;
-    launch((embed_grad_rows_kernel<T, N>), dim3((uint32_t)((waves + per - 1) / per)), dim3(kThreads), 0, stream, dy, sorted,
-           static_cast<T *>(g.dtable), parts, (uint32_t)tokens, pieces, (uint32_t)vocab, scale);
-    if (g.dpositions != nullptr && tokens != 0)
-        launch((positions_parts_kernel<T, N>), dim3((uint32_t)((length * pieces + kThreads - 1) / kThreads), l.runs), dim3(kThreads), 0,
-               stream, dy, position_parts, (uint32_t)(tokens / length), (uint32_t)length, pieces, l.runs);
+static void embed_grad_slabs(const EmbedGrad &g, const Entry *sorted, float *parts, uint32_t tokens, size_t dim, uint32_t vocab, float scale,
+                             hipStream_t stream) {
+    const uint32_t chunks = (uint32_t)((dim / N + kWave - 1) / kWave), per = kThreads / kWave;
+    const size_t waves = (size_t)((tokens + kSlab - 1) / kSlab) * chunks;
+    launch((embed_grad_slabs_kernel<T, N>), dim3((uint32_t)((waves + per - 1) / per)), dim3(kThreads), 0, stream, static_cast<const T *>(g.dy), sorted,
+           static_cast<T *>(g.dtable), parts, tokens, (uint32_t)(dim / N), vocab, scale, chunks);
 }
 
 template <typename T>
 int embed_grad_dispatch(const EmbedGrad &g, size_t tokens, size_t length, size_t vocab, size_t positions, size_t dim, float scale,
                         hipStream_t stream) {
+    constexpr int V = Store<T>::EPV;
     const Layout l = layout(tokens, length, vocab, positions, dim);
     char *const base = static_cast<char *>(g.workspace);
-    Entry *entries[2] = {reinterpret_cast<Entry *>(base + l.entries[0]), reinterpret_cast<Entry *>(base + l.entries[1])};
+    Entry *const entries[2] = {reinterpret_cast<Entry *>(base + l.entries[0]), reinterpret_cast<Entry *>(base + l.entries[1])};
     uint32_t *const table = reinterpret_cast<uint32_t *>(base + l.table);
     float *const parts = reinterpret_cast<float *>(base + l.parts);
     float *const position_parts = reinterpret_cast<float *>(base + l.position_parts);
-    const Entry *sorted = entries[0];
-    if (l.blocks == 1) {
-        launch(sort_small_kernel, dim3(1), dim3(kSortThreads), 0, stream, g.ids, entries[0], (uint32_t)tokens, (uint32_t)vocab, l.digits);
-    } else if (l.blocks > 1) {
-        const Entry *from = nullptr;
-        for (uint32_t pass = 0; pass < l.digits; pass++) {
-            Entry *const to = entries[pass % 2];
-            launch(sort_count_kernel, dim3(l.blocks), dim3(kSortThreads), 0, stream, g.ids, from, table, (uint32_t)tokens,
-                   (uint32_t)vocab, pass * kDigitBits);
-            launch(sort_place_kernel, dim3(l.blocks), dim3(kSortThreads), 0, stream, g.ids, from, table, to, (uint32_t)tokens,
-                   (uint32_t)vocab, pass * kDigitBits);
-            from = to;
-        }
-        sorted = from;
+    const int piece = piece_of<T>(dim, {g.dy, g.dtable});
+    Side side{};
+    side.dy = g.dy;
+    side.piece = piece;
+    side.pieces = (uint32_t)(dim / piece);
+    if (l.runs != 0) {
+        side.position_parts = position_parts;
+        side.batch = (uint32_t)(tokens / length);
+        side.length = (uint32_t)length;
+        side.runs = l.runs;
+        side.run_blocks = (uint32_t)((length * side.pieces + kSortThreads - 1) / kSortThreads);
     }
-    constexpr int N = Store<T>::EPV;
-    const bool vectors = dim % N == 0 && aligned16(g.dy) && aligned16(g.dtable);
-    if (vectors)
-        embed_grad_rows<T, N>(g, sorted, parts, l, tokens, length, dim, vocab, position_parts, scale, stream);
+    const Entry *sorted = nullptr;
+    const size_t table_bytes = vocab * dim * sizeof(T);
+    if (l.rounds == 1)
+        sort_tokens<T, 1>(g, l, entries, table, &sorted, (uint32_t)tokens, (uint32_t)vocab, table_bytes, side, stream);
     else
-        embed_grad_rows<T, 1>(g, sorted, parts, l, tokens, length, dim, vocab, position_parts, scale, stream);
-    if (tokens > kSlab)  // (fewer: no token is long)
-        launch((embed_grad_join_kernel<T>), dim3((uint32_t)((tokens + kSlab - 1) / kSlab), (uint32_t)((dim + kWave - 1) / kWave)),
-               dim3(kThreads), 0, stream, sorted, parts, static_cast<T *>(g.dtable), (uint32_t)tokens, (uint32_t)dim, (uint32_t)vocab,
-               scale);
-    if (g.dpositions != nullptr) {
-        const uint64_t count = (uint64_t)positions * dim, live = tokens != 0 ? (uint64_t)length * dim : 0;
-        launch((positions_join_kernel<T>), dim3((uint32_t)((count + kThreads - 1) / kThreads)), dim3(kThreads), 0, stream, position_parts,
-               static_cast<T *>(g.dpositions), live, count, l.runs);
+        sort_tokens<T, 4>(g, l, entries, table, &sorted, (uint32_t)tokens, (uint32_t)vocab, table_bytes, side, stream);
+    if (tokens != 0 && vocab != 0) {
+        if (piece == V)
+            embed_grad_slabs<T, V>(g, sorted, parts, (uint32_t)tokens, dim, (uint32_t)vocab, scale, stream);
+        else if (piece == V / 2)
+            embed_grad_slabs<T, V / 2>(g, sorted, parts, (uint32_t)tokens, dim, (uint32_t)vocab, scale, stream);
+        else
+            embed_grad_slabs<T, 1>(g, sorted, parts, (uint32_t)tokens, dim, (uint32_t)vocab, scale, stream);
     }
+    const uint64_t count = g.dpositions != nullptr ? (uint64_t)positions * dim : 0, live = tokens != 0 ? (uint64_t)length * dim : 0;
+    const uint32_t slabs = (uint32_t)((tokens + kSlab - 1) / kSlab), columns = (uint32_t)((dim + kJoinColumns - 1) / kJoinColumns);
+    const uint32_t blocks = slabs > 1 && vocab != 0 ? (slabs + kSortWaves - 1) / kSortWaves * columns : 0;  // (one slab has no run that goes on)
+    const uint32_t more = (uint32_t)((count + kSortThreads - 1) / kSortThreads);
+    if (blocks + more != 0)
+        launch((embed_grad_join_kernel<T>), dim3(blocks + more), dim3(kSortThreads), 0, stream, sorted, parts, static_cast<T *>(g.dtable),
+               (uint32_t)tokens, (uint32_t)dim, (uint32_t)vocab, scale, columns, blocks, position_parts, static_cast<T *>(g.dpositions), live,
+               count, l.runs);
     return launch_status();
 }
 
