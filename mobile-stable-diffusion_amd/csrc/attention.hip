@@ -32,7 +32,7 @@ template <typename T, int D>
 __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_kernel(const Forward a) {
     typedef typename Frag<T>::type frag;
     typedef Tile<T, D> KvTile;
-    constexpr int R = KvTile::kRows, KD = D / 16, DB = D / 32, PER = KvTile::kPerThread, CH = KvTile::kChunks, E = 16 / (int)sizeof(T);
+    constexpr int R = KvTile::kRows, KD = D / 16, DB = D / 32;
     __shared__ KvTile tiles[2][2];  // [buffer][K, V]
     const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, h = lane / 32;
     const uint32_t head = blockIdx.x % a.s.kv_heads, rest = blockIdx.x / a.s.kv_heads;
@@ -67,22 +67,22 @@ __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_ke
     const uint32_t wave_limit = wave_row < rows ? seen_by(min(rows - 1, wave_row + 31) / a.s.group) : 0;  // the most any row sees
     const uint32_t wave_full = wave_row < rows ? seen_by(wave_row / a.s.group) : 0;                       // what every row sees
 
-    u32x4 next[2][PER];
-    auto fetch = [&](uint32_t t) {
+    uint32_t k_offset[KvTile::kPerThread], v_offset[KvTile::kPerThread];
 #pragma unroll
-        for (int p = 0; p < PER; p++) {
-            const uint32_t c = p * kAttnThreads + threadIdx.x, r = c / CH, key = t * R + r, d = c % CH * E;
-            const bool in = key < lk;
-            next[0][p] = in ? load_chunk<T>(kbase + (size_t)key * a.k.row, d, a.s.dim, a.vec) : u32x4{0, 0, 0, 0};
-            next[1][p] = in ? load_chunk<T>(vbase + (size_t)key * a.v.row, d, a.s.dim, a.vec) : u32x4{0, 0, 0, 0};
-        }
-    };
-    auto put = [&](uint32_t buffer) {
-#pragma unroll
-        for (int p = 0; p < PER; p++) {
-            const uint32_t c = p * kAttnThreads + threadIdx.x, r = c / CH, at = r * CH + (c % CH ^ (r & 7));
-            tiles[buffer][0].data[at] = next[0][p];
-            tiles[buffer][1].data[at] = next[1][p];
+    for (int p = 0; p < KvTile::kPerThread; p++) {
+        const uint32_t r = KvTile::row_of(p), d = KvTile::column_of(p);
+        k_offset[p] = d < a.s.dim ? (uint32_t)((r * a.k.row + d) * sizeof(T)) : kNowhere;
+        v_offset[p] = d < a.s.dim ? (uint32_t)((r * a.v.row + d) * sizeof(T)) : kNowhere;
+    }
+    auto fetch = [&](uint32_t t, uint32_t buffer) {
+        const T *const kt = kbase + (size_t)t * R * a.k.row, *const vt = vbase + (size_t)t * R * a.v.row;
+        const uint32_t n = min(lk - t * R, (uint32_t)R);
+        if (a.vec) {
+            tiles[buffer][0].request(kt, (uint32_t)(((n - 1) * a.k.row + a.s.dim) * sizeof(T)), k_offset);
+            tiles[buffer][1].request(vt, (uint32_t)(((n - 1) * a.v.row + a.s.dim) * sizeof(T)), v_offset);
+        } else {
+            tiles[buffer][0].copy([&](uint32_t r) -> const T * { return r < n ? kt + r * a.k.row : nullptr; }, a.s.dim);
+            tiles[buffer][1].copy([&](uint32_t r) -> const T * { return r < n ? vt + r * a.v.row : nullptr; }, a.s.dim);
         }
     };
 
@@ -90,13 +90,11 @@ __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_ke
 #pragma unroll
     for (int d = 0; d < DB; d++) o[d] = zero16();
     float top = -__builtin_inff(), sum = 0.0f;
-    if (t0 < t1) {
-        fetch(t0);
-        put(0);
-    }
+    if (t0 < t1) fetch(t0, 0);
     for (uint32_t t = t0; t < t1; t++) {
+        wait_tiles();
         __syncthreads();
-        if (t + 1 < t1) fetch(t + 1);
+        if (t + 1 < t1) fetch(t + 1, (t + 1 - t0) & 1);
         const KvTile &kt = tiles[(t - t0) & 1][0], &vt = tiles[(t - t0) & 1][1];
         const uint32_t first = t * R;
         if (first < wave_limit) {
@@ -155,7 +153,6 @@ __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_ke
                 }
             if (odd) add_odd<T, D, R>(vt, o, [&](uint32_t r) { return first + r < limit; });
         }
-        if (t + 1 < t1) put((t + 1 - t0) & 1);
     }
     sum += half_swap(sum);
     if (!live) return;
@@ -289,10 +286,11 @@ AttnShape attn_shape(const AttnProblem &p) {
                      (uint32_t)p.kv_heads, (uint32_t)(p.heads / p.kv_heads), (uint32_t)p.dim, p.scale * kLog2e, p.causal};
 }
 
-bool attn_vectors(size_t elt, size_t dim, std::initializer_list<AttnView> views) {
-    bool vec = dim * elt % 16 == 0;
+bool attn_vectors(size_t elt, const AttnProblem &p, std::initializer_list<AttnView> views) {
+    bool vec = p.dim * elt % 16 == 0;
     for (const AttnView &v : views)
-        vec = vec && aligned16(v.at) && v.row * elt % 16 == 0 && v.head * elt % 16 == 0 && v.batch * elt % 16 == 0;
+        vec = vec && aligned16(v.at) && v.row * elt % 16 == 0 && v.head * elt % 16 == 0 && v.batch * elt % 16 == 0 &&
+              v.row * elt < (size_t(1) << 23) && v.head * elt < (size_t(1) << 29) / p.heads;
     return vec;
 }
 
@@ -302,7 +300,7 @@ int attn_dispatch(const AttnProblem &p, const AttnView &q, const AttnView &k, co
     const size_t tiles = row_tiles(p);
     if (tiles == 0) return MSD_OK;
     Forward a{attn_shape(p), q, k, v, out, lse, rest, nullptr, nullptr, key_parts(p), (uint32_t)total_rows(p),
-              attn_vectors(sizeof(T), p.dim, {q, k, v, out, AttnView{rest, 0, 0, 0}})};
+              attn_vectors(sizeof(T), p, {q, k, v, out, AttnView{rest, 0, 0, 0}})};
     if (a.parts > 1) {
         a.part = static_cast<float *>(workspace);
         a.part_lse = a.part + (size_t)a.parts * a.total_rows * p.heads * p.dim;

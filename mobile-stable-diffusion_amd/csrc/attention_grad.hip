@@ -23,6 +23,7 @@ struct Backward {
     const void *rest;  // [rows][heads][dim] what rounding took from out, or null
     float *delta, *norm, *v_norm;  // [rows][heads] D and |do|, [keys][kv_heads] |v|; the norms null for float32
     uint32_t total_rows, total_keys;
+    FastDiv by_group;
     bool vec;
 };
 
@@ -138,7 +139,7 @@ __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_gr
     typedef typename Frag<T>::type frag;
     typedef Tile<T, D> KvTile;
     constexpr bool kHalf = !Frag<T>::kFloat;
-    constexpr int R = KvTile::kRows, KD = D / 16, DB = D / 32, PER = KvTile::kPerThread, CH = KvTile::kChunks, E = 16 / (int)sizeof(T);
+    constexpr int R = KvTile::kRows, KD = D / 16, DB = D / 32;
     __shared__ KvTile tiles[2][2];
     const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, h = lane / 32;
     const uint32_t head = blockIdx.x % a.s.kv_heads;
@@ -176,38 +177,36 @@ __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_gr
     const uint32_t wave_limit = wave_row < rows ? seen_by(min(rows - 1, wave_row + 31) / a.s.group) : 0;
     const uint32_t wave_full = wave_row < rows ? seen_by(wave_row / a.s.group) : 0;
 
-    u32x4 next[2][PER];
+    uint32_t k_offset[KvTile::kPerThread], v_offset[KvTile::kPerThread];
+#pragma unroll
+    for (int p = 0; p < KvTile::kPerThread; p++) {
+        const uint32_t r = KvTile::row_of(p), d = KvTile::column_of(p);
+        k_offset[p] = d < a.s.dim ? (uint32_t)((r * a.k.row + d) * sizeof(T)) : kNowhere;
+        v_offset[p] = d < a.s.dim ? (uint32_t)((r * a.v.row + d) * sizeof(T)) : kNowhere;
+    }
     float next_norm = 0.0f;
-    auto fetch = [&](uint32_t t) {
-#pragma unroll
-        for (int p = 0; p < PER; p++) {
-            const uint32_t c = p * kAttnThreads + threadIdx.x, r = c / CH, key = t * R + r, d = c % CH * E;
-            const bool in = key < lk;
-            next[0][p] = in ? load_chunk<T>(kbase + (size_t)key * a.k.row, d, a.s.dim, a.vec) : u32x4{0, 0, 0, 0};
-            next[1][p] = in ? load_chunk<T>(vbase + (size_t)key * a.v.row, d, a.s.dim, a.vec) : u32x4{0, 0, 0, 0};
-        }
+    auto fetch = [&](uint32_t t, uint32_t buffer) {
         if (kHalf) next_norm = t * R + lane < lk ? v_norm[(size_t)(t * R + lane) * a.s.kv_heads] : 0.0f;
-    };
-    auto put = [&](uint32_t buffer) {
-#pragma unroll
-        for (int p = 0; p < PER; p++) {
-            const uint32_t c = p * kAttnThreads + threadIdx.x, r = c / CH, at = r * CH + (c % CH ^ (r & 7));
-            tiles[buffer][0].data[at] = next[0][p];
-            tiles[buffer][1].data[at] = next[1][p];
+        const T *const kt = kbase + (size_t)t * R * a.k.row, *const vt = vbase + (size_t)t * R * a.v.row;
+        const uint32_t n = min(lk - t * R, (uint32_t)R);
+        if (a.vec) {
+            tiles[buffer][0].request(kt, (uint32_t)(((n - 1) * a.k.row + a.s.dim) * sizeof(T)), k_offset);
+            tiles[buffer][1].request(vt, (uint32_t)(((n - 1) * a.v.row + a.s.dim) * sizeof(T)), v_offset);
+        } else {
+            tiles[buffer][0].copy([&](uint32_t r) -> const T * { return r < n ? kt + r * a.k.row : nullptr; }, a.s.dim);
+            tiles[buffer][1].copy([&](uint32_t r) -> const T * { return r < n ? vt + r * a.v.row : nullptr; }, a.s.dim);
         }
     };
     f32x16 dq[DB];
 #pragma unroll
     for (int d = 0; d < DB; d++) dq[d] = zero16();
     DsScale scale;
-    if (t1 != 0) {
-        fetch(0);
-        put(0);
-    }
+    if (t1 != 0) fetch(0, 0);
     for (uint32_t t = 0; t < t1; t++) {
         const float v_norms = next_norm;  // (of the tile's keys, one to a lane)
+        wait_tiles();
         __syncthreads();
-        if (t + 1 < t1) fetch(t + 1);
+        if (t + 1 < t1) fetch(t + 1, (t + 1) & 1);
         const KvTile &kt = tiles[t & 1][0], &vt = tiles[t & 1][1];
         const uint32_t first = t * R;
         if (first < wave_limit) {
@@ -263,7 +262,6 @@ __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_gr
             }
             if (odd) add_odd<T, D, R>(kt, dq, [&](uint32_t r) { return first + r < limit; });
         }
-        if (t + 1 < t1) put((t + 1) & 1);
     }
     if (!live) return;
     T *const to = static_cast<T *>(const_cast<void *>(a.dq.at)) + (packed ? 0 : b * a.dq.batch) + (size_t)(q0 + i) * a.dq.row + qh * a.dq.head;
@@ -277,7 +275,7 @@ __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat || D == 128 ? 1 : 2) 
     typedef typename Frag<T>::type frag;
     typedef Tile<T, D, D == 128 ? 32 : Frag<T>::kTile> RowTile;  // (64 rows of 128 columns on their way leave too few registers)
     constexpr bool kHalf = !Frag<T>::kFloat;
-    constexpr int R = RowTile::kRows, KD = D / 16, DB = D / 32, PER = RowTile::kPerThread, CH = RowTile::kChunks, E = 16 / (int)sizeof(T);
+    constexpr int R = RowTile::kRows, KD = D / 16, DB = D / 32;
     __shared__ RowTile tiles[2][2];                // [buffer][Q, dO]
     __shared__ __align__(16) float stats[2][3][R]; // [buffer][- log2 sum, D, |do|]
     const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, h = lane / 32;
@@ -310,19 +308,35 @@ __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat || D == 128 ? 1 : 2) 
     const uint32_t wave_full = wave_key < lk ? first_row(min(lk - 1, wave_key + 31)) : rows; // from here on all are
     const uint32_t t0 = first_row(tile * kAttnRows) / R, t1 = (rows + R - 1) / R;
 
-    u32x4 next[2][PER];
     float next_stat[3] = {0.0f, 0.0f, 0.0f};
-    auto fetch = [&](uint32_t t) {
+    auto fetch = [&](uint32_t t, uint32_t buffer) {
+        const uint32_t i0 = t * R / a.s.group;  // the query of the tile's first row
+        const T *const q = qbase + (size_t)i0 * a.q.row, *const g = gbase + (size_t)i0 * a.dout.row;
+        const uint32_t last = min(rows, (t + 1) * R) - 1, n = last / a.s.group - i0;
+        if (a.vec) {
+            uint32_t q_offset[RowTile::kPerThread], g_offset[RowTile::kPerThread];
 #pragma unroll
-        for (int p = 0; p < PER; p++) {
-            const uint32_t c = p * kAttnThreads + threadIdx.x, r = t * R + c / CH, d = c % CH * E;
-            const bool in = r < rows;
-            const uint32_t i = r / a.s.group, gh = r - i * a.s.group;
-            next[0][p] = in ? load_chunk<T>(qbase + (size_t)i * a.q.row + gh * a.q.head, d, a.s.dim, a.vec) : u32x4{0, 0, 0, 0};
-            next[1][p] = in ? load_chunk<T>(gbase + (size_t)i * a.dout.row + gh * a.dout.head, d, a.s.dim, a.vec) : u32x4{0, 0, 0, 0};
+            for (int p = 0; p < RowTile::kPerThread; p++) {
+                const uint32_t r = t * R + RowTile::row_of(p), d = RowTile::column_of(p), i = fast_div(r, a.by_group), gh = r - i * a.s.group;
+                const bool in = r < rows && d < a.s.dim;
+                q_offset[p] = in ? (uint32_t)(((i - i0) * a.q.row + gh * a.q.head + d) * sizeof(T)) : kNowhere;
+                g_offset[p] = in ? (uint32_t)(((i - i0) * a.dout.row + gh * a.dout.head + d) * sizeof(T)) : kNowhere;
+            }
+            const uint32_t heads = a.s.group - 1;
+            tiles[buffer][0].request(q, (uint32_t)((n * a.q.row + heads * a.q.head + a.s.dim) * sizeof(T)), q_offset);
+            tiles[buffer][1].request(g, (uint32_t)((n * a.dout.row + heads * a.dout.head + a.s.dim) * sizeof(T)), g_offset);
+        } else {
+            auto from = [&](const T *base, const AttnView &v) {
+                return [=](uint32_t r) -> const T * {
+                    const uint32_t i = (t * R + r) / a.s.group, gh = t * R + r - i * a.s.group;
+                    return t * R + r < rows ? base + (i - i0) * v.row + gh * v.head : nullptr;
+                };
+            };
+            tiles[buffer][0].copy(from(q, a.q), a.s.dim);
+            tiles[buffer][1].copy(from(g, a.dout), a.s.dim);
         }
         if (threadIdx.x < R) {
-            const uint32_t r = t * R + threadIdx.x, i = r / a.s.group;
+            const uint32_t r = t * R + threadIdx.x, i = fast_div(r, a.by_group);
             const bool in = r < rows;
             const size_t at = place0 + (size_t)i * a.s.heads + (r - i * a.s.group);
             const float lse = in ? a.lse[at] : -__builtin_inff();
@@ -331,13 +345,7 @@ __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat || D == 128 ? 1 : 2) 
             if (kHalf) next_stat[2] = in ? a.norm[at] : 0.0f;
         }
     };
-    auto put = [&](uint32_t buffer) {
-#pragma unroll
-        for (int p = 0; p < PER; p++) {
-            const uint32_t c = p * kAttnThreads + threadIdx.x, r = c / CH, at = r * CH + (c % CH ^ (r & 7));
-            tiles[buffer][0].data[at] = next[0][p];
-            tiles[buffer][1].data[at] = next[1][p];
-        }
+    auto put = [&](uint32_t buffer) {  // (what the next tile's rows have beside their values)
         if (threadIdx.x < R) {
 #pragma unroll
             for (int i = 0; i < 3; i++) stats[buffer][i][threadIdx.x] = next_stat[i];
@@ -348,12 +356,13 @@ __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat || D == 128 ? 1 : 2) 
     for (int d = 0; d < DB; d++) dk[d] = dv[d] = zero16();
     DsScale scale;
     if (t0 < t1) {
-        fetch(t0);
+        fetch(t0, 0);
         put(0);
     }
     for (uint32_t t = t0; t < t1; t++) {
+        wait_tiles();
         __syncthreads();
-        if (t + 1 < t1) fetch(t + 1);
+        if (t + 1 < t1) fetch(t + 1, (t + 1 - t0) & 1);
         const uint32_t buffer = (t - t0) & 1, first = t * R;
         const RowTile &qt = tiles[buffer][0], &gt = tiles[buffer][1];
         if (first + R > wave_from && wave_from < rows) {
@@ -460,7 +469,7 @@ int attn_grad_dispatch(const AttnProblem &p, const AttnGradViews &g, const float
     constexpr bool kHalf = !Frag<T>::kFloat;
     const Backward a{attn_shape(p), g.q, g.k, g.v, g.out, g.dout, g.dq, g.dk, g.dv, lse, rest, delta,
                      kHalf ? delta + rows * p.heads : nullptr, kHalf ? delta + 2 * rows * p.heads : nullptr, (uint32_t)rows, (uint32_t)keys,
-                     attn_vectors(sizeof(T), p.dim, {g.q, g.k, g.v, g.out, g.dout, g.dq, g.dk, g.dv, AttnView{rest, 0, 0, 0}})};
+                     make_fast_div((uint32_t)(p.heads / p.kv_heads)), attn_vectors(sizeof(T), p, {g.q, g.k, g.v, g.out, g.dout, g.dq, g.dk, g.dv, AttnView{rest, 0, 0, 0}})};
     const size_t items = rows * p.heads + (kHalf ? keys * p.kv_heads : 0);
     if (items != 0)
         launch((attn_grad_rows_kernel<T>), dim3((uint32_t)((items + 15) / 16)), dim3(kAttnThreads), 0, stream, a);

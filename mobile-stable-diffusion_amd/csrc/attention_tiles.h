@@ -153,6 +153,11 @@ __device__ __forceinline__ void load_frags(const T *row, uint32_t dim, bool vec,
     }
 }
 
+constexpr uint32_t kNowhere = 0x80000000u;  // an offset behind the end of any rows of a tile (attn_vectors)
+
+// Until what Tile::request asked for is in LDS (this wavefront's part; a barrier makes it everyone's).
+__device__ __forceinline__ void wait_tiles() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
 // A tile in LDS: ROWS rows of D values as 16-byte chunks, chunk c of row r at place c ^ (r & 7), so that lanes that read one
 // chunk of neighbouring rows, or neighbouring chunks of four rows, meet different banks.
 template <typename T, int D, int ROWS = Frag<T>::kTile>
@@ -161,6 +166,37 @@ struct Tile {
     static constexpr int kPerThread = kRows * kChunks / (int)kAttnThreads;
     typedef typename Frag<T>::type frag;
     u32x4 data[kRows * kChunks];
+
+    // Row and column of the chunk that belongs at this thread's place number p.
+    static __device__ __forceinline__ uint32_t row_of(int p) { return (p * kAttnThreads + threadIdx.x) / kChunks; }
+    static __device__ __forceinline__ uint32_t column_of(int p) {
+        return ((p * kAttnThreads + threadIdx.x) % kChunks ^ (row_of(p) & 7)) * (16 / (uint32_t)sizeof(T));
+    }
+    // Asks for this thread's chunks, `offset[p]` bytes behind `from` (the same in the whole wavefront), straight from memory to
+    // LDS; from byte `bytes` on there are zeros.  wait_tiles() and a barrier later they are there.  Written as assembly because
+    // the compiler, which knows no more than that these write LDS, would wait for them in front of every read by columns.
+    __device__ __forceinline__ void request(const void *from, uint32_t bytes, const uint32_t (&offset)[kPerThread]) {
+        const uintptr_t at = reinterpret_cast<uintptr_t>(from);
+        const u32x4 resource = {(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)at), (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(at >> 32)),
+                                (uint32_t)__builtin_amdgcn_readfirstlane(bytes), 0x00020000u};
+        const uint32_t first = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) * kWave;
+        const uint32_t lds = (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char *)data) + first * 16;
+#pragma unroll
+        for (int p = 0; p < kPerThread; p++)
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                         :
+                         : "s"(lds + p * kAttnThreads * 16), "v"(offset[p]), "s"(resource)
+                         : "memory", "m0");
+    }
+    // The same through registers, for rows that are no whole aligned vectors: `row(r)` is a row's first value, or null for zeros.
+    template <typename Row>
+    __device__ __forceinline__ void copy(Row row, uint32_t dim) {
+#pragma unroll 1
+        for (int p = 0; p < kPerThread; p++) {
+            const T *const from = row(row_of(p));
+            data[p * kAttnThreads + threadIdx.x] = from != nullptr ? load_chunk<T>(from, column_of(p), dim, false) : u32x4{0, 0, 0, 0};
+        }
+    }
 
     // A operand by rows: row r0 + (lane & 31), columns 16 k + 8 h ...
     __device__ __forceinline__ frag rows(int r0, int k) const {
@@ -212,8 +248,8 @@ struct AttnShape {
 };
 
 AttnShape attn_shape(const AttnProblem &p);
-// Whether every row of the views is whole aligned 16-byte vectors.
-bool attn_vectors(size_t elt, size_t dim, std::initializer_list<AttnView> views);
+// Whether every row of the views is whole aligned 16-byte vectors, and a tile's reach fits 31 bits.
+bool attn_vectors(size_t elt, const AttnProblem &p, std::initializer_list<AttnView> views);
 
 // [first, last) of sequence b: within the rows there are, whatever the offsets say.
 __device__ __forceinline__ void span(const int32_t *offsets, uint32_t b, uint32_t rows, uint32_t &first, uint32_t &count) {
