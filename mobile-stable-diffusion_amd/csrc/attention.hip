@@ -5,6 +5,7 @@
 // operand of O^T = V^T P^T.  K and V tiles go through LDS, twice buffered.  Where rows are too few to fill the chip, the keys are
 // cut into parts, each with a workgroup of its own, and a second launch joins them.
 #include <algorithm>
+#include <type_traits>
 
 #include "attention_tiles.h"
 
@@ -35,6 +36,7 @@ __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_ke
     constexpr int R = KvTile::kRows, KD = D / 16, DB = D / 32;
     __shared__ KvTile tiles[2][2];  // [buffer][K, V]
     const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, h = lane / 32;
+    const TileLanes<T, D> lanes;
     const uint32_t head = blockIdx.x % a.s.kv_heads, rest = blockIdx.x / a.s.kv_heads;
     const uint32_t part = rest % a.parts;
     uint32_t b, tile, q0, lq, k0, lk;
@@ -98,60 +100,67 @@ __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_ke
         const KvTile &kt = tiles[(t - t0) & 1][0], &vt = tiles[(t - t0) & 1][1];
         const uint32_t first = t * R;
         if (first < wave_limit) {
-            f32x16 s[R / 32];
+            // (apart for tiles with masked pairs: the tests between their products would keep the others' from overlapping)
+            auto work = [&](auto with_masked) {
+                constexpr bool MASKED = decltype(with_masked)::value;
+                f32x16 s[R / 32];
 #pragma unroll
-            for (int n = 0; n < R / 32; n++) {
-                s[n] = zero16();
+                for (int n = 0; n < R / 32; n++) {
+                    s[n] = zero16();
 #pragma unroll
-                for (int k = 0; k < KD; k++) s[n] = mma(kt.rows(32 * n, k), q[k], s[n]);
-            }
-            const bool masked = first + R > wave_full;
-            bool odd = false;
-            if (masked) {
+                    for (int k = 0; k < KD; k++) s[n] = mma(kt.rows(lanes, 32 * n, k), q[k], s[n]);
+                }
+                bool odd = false;
+                if constexpr (MASKED) {
+#pragma unroll
+                    for (int n = 0; n < R / 32; n++)
+#pragma unroll
+                        for (int r = 0; r < 16; r++)
+                            if (first + 32 * n + 8 * (r / 4) + 4 * h + r % 4 >= limit) s[n][r] = -__builtin_inff();
+                }
+                float most = s[0][0];
 #pragma unroll
                 for (int n = 0; n < R / 32; n++)
 #pragma unroll
-                    for (int r = 0; r < 16; r++)
-                        if (first + 32 * n + 8 * (r / 4) + 4 * h + r % 4 >= limit) s[n][r] = -__builtin_inff();
-            }
-            float most = s[0][0];
+                    for (int r = 0; r < 16; r++) most = fmaxf(most, s[n][r]);
+                const float now = fmaxf(top, halves_max(most) * a.s.scale2);
+                if (__builtin_amdgcn_ballot_w64(now > top + kLag) != 0) {
+                    const float down = __builtin_amdgcn_exp2f(top - (now == -__builtin_inff() ? 0.0f : now));
+                    sum *= down;
 #pragma unroll
-            for (int n = 0; n < R / 32; n++)
+                    for (int d = 0; d < DB; d++)
 #pragma unroll
-                for (int r = 0; r < 16; r++) most = fmaxf(most, s[n][r]);
-            const float now = fmaxf(top, halves_max(most) * a.s.scale2);
-            if (__builtin_amdgcn_ballot_w64(now > top + kLag) != 0) {
-                const float down = __builtin_amdgcn_exp2f(top - (now == -__builtin_inff() ? 0.0f : now));
-                sum *= down;
-#pragma unroll
-                for (int d = 0; d < DB; d++)
-#pragma unroll
-                    for (int r = 0; r < 16; r++) o[d][r] *= down;
-                top = now;
-            }
-            const float base = kShift<T> - (top == -__builtin_inff() ? 0.0f : top);
-#pragma unroll
-            for (int n = 0; n < R / 32; n++)
-#pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    s[n][r] = __builtin_amdgcn_exp2f(fmaf(s[n][r], a.s.scale2, base));
-                    sum += s[n][r];
+                        for (int r = 0; r < 16; r++) o[d][r] *= down;
+                    top = now;
                 }
+                const float base = kShift<T> - (top == -__builtin_inff() ? 0.0f : top);
 #pragma unroll
-            for (int n = 0; n < R / 32; n++)
+                for (int n = 0; n < R / 32; n++)
 #pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    frag p;
-                    to_frag(s[n], u, p);
-#pragma unroll
-                    for (int d = 0; d < DB; d++) {
-                        frag v = vt.columns(32 * n + 16 * u, d);
-                        if (masked) leave_out_odd(v, odd);
-                        o[d] = mma(v, p, o[d]);
+                    for (int r = 0; r < 16; r++) {
+                        s[n][r] = __builtin_amdgcn_exp2f(fmaf(s[n][r], a.s.scale2, base));
+                        sum += s[n][r];
                     }
-                    step_end<T>();
-                }
-            if (odd) add_odd<T, D, R>(vt, o, [&](uint32_t r) { return first + r < limit; });
+#pragma unroll
+                for (int n = 0; n < R / 32; n++)
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        frag p;
+                        to_frag(s[n], u, p);
+#pragma unroll
+                        for (int d = 0; d < DB; d++) {
+                            frag v = vt.columns(lanes, 32 * n + 16 * u, d);
+                            if constexpr (MASKED) leave_out_odd(v, odd);
+                            o[d] = mma(v, p, o[d]);
+                        }
+                        step_end<Frag<T>::kFloat>();
+                    }
+                if (MASKED && odd) add_odd<T, D, R>(vt, lanes, o, [&](uint32_t r) { return first + r < limit; });
+            };
+            if (first + R > wave_full)
+                work(std::true_type{});
+            else
+                work(std::false_type{});
         }
     }
     sum += half_swap(sum);

@@ -10,6 +10,7 @@
 // and each key of dk and dv has a power of its own, from what it sees alone; it follows the largest bound so far, and the sums
 // are scaled down where it moves.
 #include <algorithm>
+#include <type_traits>
 
 #include "attention_tiles.h"
 
@@ -142,6 +143,7 @@ __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_gr
     constexpr int R = KvTile::kRows, KD = D / 16, DB = D / 32;
     __shared__ KvTile tiles[2][2];
     const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, h = lane / 32;
+    const TileLanes<T, D> lanes;
     const uint32_t head = blockIdx.x % a.s.kv_heads;
     uint32_t b, tile, q0, lq, k0, lk;
     if (!find_tile(a.s.q_offsets, a.s.batch, a.s.q_rows, a.s.group, kAttnRows, blockIdx.x / a.s.kv_heads, b, tile)) return;
@@ -210,57 +212,63 @@ __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_gr
         const KvTile &kt = tiles[t & 1][0], &vt = tiles[t & 1][1];
         const uint32_t first = t * R;
         if (first < wave_limit) {
-            float by = 1.0f;
-            const bool masked = first + R > wave_full;
-            bool odd = false;
-            if (kHalf) {
-                float down, v_most;
-                if (masked) {
-                    const float upto = __shfl(max_up_to(v_norms), (int)min(limit - first - 1, (uint32_t)R - 1), kWave);
-                    v_most = first < limit ? upto : 0.0f;
-                } else {
-                    v_most = team_max<64>(v_norms);
+            auto work = [&](auto with_masked) {  // (apart for tiles with masked pairs, as in the forward call)
+                constexpr bool MASKED = decltype(with_masked)::value;
+                float by = 1.0f;
+                bool odd = false;
+                if (kHalf) {
+                    float down, v_most;
+                    if constexpr (MASKED) {
+                        const float upto = __shfl(max_up_to(v_norms), (int)min(limit - first - 1, (uint32_t)R - 1), kWave);
+                        v_most = first < limit ? upto : 0.0f;
+                    } else {
+                        v_most = team_max<64>(v_norms);
+                    }
+                    if (scale.lower(fmaf(norm, v_most, fabsf(delta)), down)) {
+#pragma unroll
+                        for (int d = 0; d < DB; d++)
+#pragma unroll
+                            for (int r = 0; r < 16; r++) dq[d][r] *= down;
+                    }
+                    by = ldexpf(1.0f, scale.power);
                 }
-                if (scale.lower(fmaf(norm, v_most, fabsf(delta)), down)) {
+                const float delta_by = delta * by;
 #pragma unroll
-                    for (int d = 0; d < DB; d++)
+                for (int n = 0; n < R / 32; n++) {
+                    f32x16 s = zero16(), dp = zero16();
 #pragma unroll
-                        for (int r = 0; r < 16; r++) dq[d][r] *= down;
-                }
-                by = ldexpf(1.0f, scale.power);
-            }
-            const float delta_by = delta * by;
-#pragma unroll
-            for (int n = 0; n < R / 32; n++) {
-                f32x16 s = zero16(), dp = zero16();
-#pragma unroll
-                for (int k = 0; k < KD; k++) {
-                    s = mma(kt.rows(32 * n, k), q[k], s);
-                    dp = mma(vt.rows(32 * n, k), g[k], dp);
-                    step_end<T>();
-                }
-#pragma unroll
-                for (int r = 0; r < 16; r++)
-                    s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.s.scale2, base)) * fmaf(dp[r], by, -delta_by);
-                if (masked) {
+                    for (int k = 0; k < KD; k++) {
+                        s = mma(kt.rows(lanes, 32 * n, k), q[k], s);
+                        dp = mma(vt.rows(lanes, 32 * n, k), g[k], dp);
+                        step_end<Frag<T>::kFloat>();
+                    }
 #pragma unroll
                     for (int r = 0; r < 16; r++)
-                        if (first + 32 * n + 8 * (r / 4) + 4 * h + r % 4 >= limit) s[r] = 0.0f;
-                }
+                        s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.s.scale2, base)) * fmaf(dp[r], by, -delta_by);
+                    if constexpr (MASKED) {
 #pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    frag ds;
-                    to_frag(s, u, ds);
-#pragma unroll
-                    for (int d = 0; d < DB; d++) {
-                        frag k = kt.columns(32 * n + 16 * u, d);
-                        if (masked) leave_out_odd(k, odd);
-                        dq[d] = mma(k, ds, dq[d]);
+                        for (int r = 0; r < 16; r++)
+                            if (first + 32 * n + 8 * (r / 4) + 4 * h + r % 4 >= limit) s[r] = 0.0f;
                     }
-                    step_end<T>();
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        frag ds;
+                        to_frag(s, u, ds);
+#pragma unroll
+                        for (int d = 0; d < DB; d++) {
+                            frag k = kt.columns(lanes, 32 * n + 16 * u, d);
+                            if constexpr (MASKED) leave_out_odd(k, odd);
+                            dq[d] = mma(k, ds, dq[d]);
+                        }
+                        step_end<Frag<T>::kFloat || D == 128>();
+                    }
                 }
-            }
-            if (odd) add_odd<T, D, R>(kt, dq, [&](uint32_t r) { return first + r < limit; });
+                if (MASKED && odd) add_odd<T, D, R>(kt, lanes, dq, [&](uint32_t r) { return first + r < limit; });
+            };
+            if (first + R > wave_full)
+                work(std::true_type{});
+            else
+                work(std::false_type{});
         }
     }
     if (!live) return;
@@ -269,16 +277,28 @@ __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_gr
     store_rows<T, D>(to, dq, kHalf ? ldexpf(natural, -scale.power) : natural, a.s.dim, a.vec);
 }
 
+template <typename T, int D, bool IN_LDS>
+struct KeptValues {
+    typedef Tile<T, D, (int)kAttnRows> type;
+};
+template <typename T, int D>
+struct KeptValues<T, D, false> {
+    struct type {};
+};
+
 // dk and dv: a wavefront owns 32 keys as the columns of S = Q K^T; the rows that see them pass by.
 template <typename T, int D>
-__global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat || D == 128 ? 1 : 2) void attn_grad_kv_kernel(const Backward a) {
+__global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_grad_kv_kernel(const Backward a) {
     typedef typename Frag<T>::type frag;
     typedef Tile<T, D, D == 128 ? 32 : Frag<T>::kTile> RowTile;  // (64 rows of 128 columns on their way leave too few registers)
     constexpr bool kHalf = !Frag<T>::kFloat;
     constexpr int R = RowTile::kRows, KD = D / 16, DB = D / 32;
     __shared__ RowTile tiles[2][2];                // [buffer][Q, dO]
+    constexpr bool kVInLds = kHalf && D == 128;
+    __shared__ typename KeptValues<T, D, kVInLds>::type values;
     __shared__ __align__(16) float stats[2][3][R]; // [buffer][- log2 sum, D, |do|]
     const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, h = lane / 32;
+    const TileLanes<T, D> lanes;
     const uint32_t head = blockIdx.x % a.s.kv_heads;
     uint32_t b, tile, q0, lq, k0, lk;
     if (!find_tile(a.s.k_offsets, a.s.batch, a.s.k_rows, 1, kAttnRows, blockIdx.x / a.s.kv_heads, b, tile)) return;
@@ -297,9 +317,30 @@ __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat || D == 128 ? 1 : 2) 
     const T *qbase = static_cast<const T *>(a.q.at) + (packed ? 0 : b * a.q.batch) + (size_t)q0 * a.q.row + head * a.s.group * a.q.head;
     const T *gbase = static_cast<const T *>(a.dout.at) + (packed ? 0 : b * a.dout.batch) + (size_t)q0 * a.dout.row + head * a.s.group * a.dout.head;
     const size_t place0 = ((size_t)(packed ? 0 : b) * lq + q0) * a.s.heads + head * a.s.group;
-    frag k[KD], v[KD];
+    frag k[KD], v[kVInLds ? 1 : KD];
     load_frags<T, D>(live ? kbase : nullptr, a.s.dim, a.vec, k);
-    load_frags<T, D>(live ? vbase : nullptr, a.s.dim, a.vec, v);
+    if constexpr (kVInLds) {
+        typedef typename KeptValues<T, D, true>::type Values;
+        const uint32_t key0 = tile * kAttnRows, n = min(lk - key0, kAttnRows);
+        const T *const from = static_cast<const T *>(a.v.at) + (packed ? 0 : b * a.v.batch) + (size_t)(k0 + key0) * a.v.row + head * a.v.head;
+        if (a.vec) {
+            uint32_t offset[Values::kPerThread];
+#pragma unroll
+            for (int p = 0; p < Values::kPerThread; p++)
+                offset[p] = Values::column_of(p) < a.s.dim ? (uint32_t)((Values::row_of(p) * a.v.row + Values::column_of(p)) * sizeof(T)) : kNowhere;
+            values.request(from, (uint32_t)(((n - 1) * a.v.row + a.s.dim) * sizeof(T)), offset);
+        } else {
+            values.copy([&](uint32_t r) -> const T * { return r < n ? from + r * a.v.row : nullptr; }, a.s.dim);
+        }
+    } else {
+        load_frags<T, D>(live ? vbase : nullptr, a.s.dim, a.vec, v);
+    }
+    auto value = [&](int c) -> frag {
+        if constexpr (kVInLds)
+            return values.rows(lanes, wave * 32, c);
+        else
+            return v[c];
+    };
     const float v_norm = kHalf && live ? a.v_norm[(((size_t)(packed ? 0 : b) * lk + k0) + key) * a.s.kv_heads + head] : 0.0f;
 
     const uint32_t wave_key = tile * kAttnRows + wave * 32;
@@ -366,78 +407,91 @@ __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat || D == 128 ? 1 : 2) 
         const uint32_t buffer = (t - t0) & 1, first = t * R;
         const RowTile &qt = tiles[buffer][0], &gt = tiles[buffer][1];
         if (first + R > wave_from && wave_from < rows) {
-            float by = 1.0f;
-            const bool masked = first < wave_full;
-            bool odd = false;
-            if (kHalf) {
-                float down, norms = stats[buffer][2][lane % R], deltas = fabsf(stats[buffer][1][lane % R]);
-                if (masked) {
-                    norms = max_from(lane < R ? norms : 0.0f);
-                    deltas = max_from(lane < R ? deltas : 0.0f);
-                    const uint32_t behind = from > first ? min(from - first, (uint32_t)R) : 0;  // the tile's rows that do not see the key
-                    norms = __shfl(norms, (int)min(behind, (uint32_t)R - 1), kWave);
-                    deltas = __shfl(deltas, (int)min(behind, (uint32_t)R - 1), kWave);
-                    if (behind == R) norms = deltas = 0.0f;
-                } else {
-                    norms = team_max<64>(norms);
-                    deltas = team_max<64>(deltas);
-                }
-                if (scale.lower(fmaf(norms, v_norm, deltas), down)) {
-#pragma unroll
-                    for (int d = 0; d < DB; d++)
-#pragma unroll
-                        for (int r = 0; r < 16; r++) dk[d][r] *= down;
-                }
-                by = ldexpf(1.0f, scale.power - kPShift<T>);
-            }
-#pragma unroll
-            for (int n = 0; n < R / 32; n++) {
-                f32x16 s = zero16(), dp = zero16();
-#pragma unroll
-                for (int c = 0; c < KD; c++) {
-                    s = mma(qt.rows(32 * n, c), k[c], s);
-                    dp = mma(gt.rows(32 * n, c), v[c], dp);
-                    step_end<T>();
-                }
-#pragma unroll
-                for (int g = 0; g < 4; g++) {
-                    const f32x4 base = *reinterpret_cast<const f32x4 *>(&stats[buffer][0][32 * n + 8 * g + 4 * h]);
-                    const f32x4 delta = *reinterpret_cast<const f32x4 *>(&stats[buffer][1][32 * n + 8 * g + 4 * h]);
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const int r = 4 * g + j;
-                        s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.s.scale2, base[j]));
-                        dp[r] = s[r] * (kHalf ? fmaf(dp[r], by, -delta[j] * by) : dp[r] - delta[j]);
+            auto work = [&](auto with_masked) {
+                constexpr bool MASKED = decltype(with_masked)::value;
+                float by = 1.0f;
+                bool odd = false;
+                if (kHalf) {
+                    float down, norms = stats[buffer][2][lane % R], deltas = fabsf(stats[buffer][1][lane % R]);
+                    if constexpr (MASKED) {
+                        norms = max_from(lane < R ? norms : 0.0f);
+                        deltas = max_from(lane < R ? deltas : 0.0f);
+                        const uint32_t behind = from > first ? min(from - first, (uint32_t)R) : 0;  // the tile's rows that do not see the key
+                        norms = __shfl(norms, (int)min(behind, (uint32_t)R - 1), kWave);
+                        deltas = __shfl(deltas, (int)min(behind, (uint32_t)R - 1), kWave);
+                        if (behind == R) norms = deltas = 0.0f;
+                    } else {
+                        norms = team_max<64>(norms);
+                        deltas = team_max<64>(deltas);
                     }
+                    if (scale.lower(fmaf(norms, v_norm, deltas), down)) {
+#pragma unroll
+                        for (int d = 0; d < DB; d++)
+#pragma unroll
+                            for (int r = 0; r < 16; r++) dk[d][r] *= down;
+                    }
+                    by = ldexpf(1.0f, scale.power - kPShift<T>);
                 }
-                if (masked) {
 #pragma unroll
-                    for (int r = 0; r < 16; r++)
-                        if (first + 32 * n + 8 * (r / 4) + 4 * h + r % 4 < from) s[r] = dp[r] = 0.0f;
-                }
+                for (int n = 0; n < R / 32; n++) {
+                    f32x16 s = zero16(), dp = zero16();
 #pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    frag p, ds;
-                    to_frag(s, u, p);
-                    to_frag(dp, u, ds);
+                    for (int c = 0; c < KD; c++) {
+                        s = mma(qt.rows(lanes, 32 * n, c), k[c], s);
+                        dp = mma(gt.rows(lanes, 32 * n, c), value(c), dp);
+                        step_end<Frag<T>::kFloat>();
+                    }
 #pragma unroll
-                    for (int d = 0; d < DB; d++) {
-                        frag gc = gt.columns(32 * n + 16 * u, d), qc = qt.columns(32 * n + 16 * u, d);
-                        if (masked) {
-                            leave_out_odd(gc, odd);
-                            leave_out_odd(qc, odd);
+                    for (int g = 0; g < 4; g++) {
+                        const f32x4 base = *reinterpret_cast<const f32x4 *>(&stats[buffer][0][32 * n + 8 * g + 4 * h]);
+                        const f32x4 delta = *reinterpret_cast<const f32x4 *>(&stats[buffer][1][32 * n + 8 * g + 4 * h]);
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            const int r = 4 * g + j;
+                            s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.s.scale2, base[j]));
+                            dp[r] = s[r] * (kHalf ? fmaf(dp[r], by, -delta[j] * by) : dp[r] - delta[j]);
                         }
-                        dv[d] = mma(gc, p, dv[d]);
-                        dk[d] = mma(qc, ds, dk[d]);
-                        step_end<T>();
+                    }
+                    if constexpr (MASKED) {
+#pragma unroll
+                        for (int r = 0; r < 16; r++)
+                            if (first + 32 * n + 8 * (r / 4) + 4 * h + r % 4 < from) s[r] = dp[r] = 0.0f;
+                    }
+                    frag p[2], ds[2];
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        to_frag(s, u, p[u]);
+                        to_frag(dp, u, ds[u]);
+                        if constexpr (MASKED) {
+                            keep_here(p[u]);
+                            keep_here(ds[u]);
+                        }
+                    }
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+#pragma unroll
+                        for (int d = 0; d < DB; d++) {
+                            frag gc = gt.columns(lanes, 32 * n + 16 * u, d), qc = qt.columns(lanes, 32 * n + 16 * u, d);
+                            if constexpr (MASKED) {
+                                leave_out_odd(gc, odd);
+                                leave_out_odd(qc, odd);
+                            }
+                            dv[d] = mma(gc, p[u], dv[d]);
+                            dk[d] = mma(qc, ds[u], dk[d]);
+                            step_end<Frag<T>::kFloat || D == 128>();
+                        }
                     }
                 }
-            }
-            if (odd) {
-                auto visible = [&](uint32_t r) { return first + r >= from; };
-                add_odd<T, D, R>(gt, dv, visible);
-                add_odd<T, D, R>(qt, dk, visible);
-            }
+                if (MASKED && odd) {
+                    auto visible = [&](uint32_t r) { return first + r >= from; };
+                    add_odd<T, D, R>(gt, lanes, dv, visible);
+                    add_odd<T, D, R>(qt, lanes, dk, visible);
+                }
+            };
+            if (first < wave_full)
+                work(std::true_type{});
+            else
+                work(std::false_type{});
         }
         if (t + 1 < t1) put((t + 1 - t0) & 1);
     }

@@ -47,11 +47,11 @@ __device__ __forceinline__ f32x16 mma(const f32x8 &a, const f32x8 &b, f32x16 c) 
     return c;
 }
 
-// Between steps of products of float32, whose operands are twice as large: none is read from LDS ahead of its step (with
-// all of them there was no room in registers), and a step takes long enough to hide the next one's reads.
-template <typename T>
+// Between steps of products whose operands fill the registers: none is read from LDS ahead of its step (with all of them read
+// first there is no room).
+template <bool FULL>
 __device__ __forceinline__ void step_end() {
-    if (Frag<T>::kFloat) __builtin_amdgcn_sched_barrier(0);
+    if (FULL) __builtin_amdgcn_sched_barrier(0);
 }
 
 // Registers 8 t ... 8 t + 7 of an accumulator as a B operand (float16: rounded to nearest).
@@ -77,6 +77,15 @@ __device__ __forceinline__ f32x16 zero16() {
     return z;
 }
 
+// Keeps the compiler from moving what gives a fragment behind the branches that follow.
+__device__ __forceinline__ void keep_here(half8 &f) {
+    u32x4 v = __builtin_bit_cast(u32x4, f);
+    asm volatile("" : "+v"(v));
+    f = __builtin_bit_cast(half8, v);
+}
+
+__device__ __forceinline__ void keep_here(f32x8 &) {}
+
 // A masked pair's weight is zero, but zero times an infinity or NaN is not.  Where a tile has masked pairs, what its A operands
 // hold of those is left out of the product, and `add_odd` puts it back for the pairs that are visible.
 template <typename F>
@@ -96,10 +105,13 @@ __device__ __forceinline__ void leave_out_odd(F &a, bool &odd) {
     for (int j = 0; j < 8; j++)
         if (!(__builtin_fabsf((float)a[j]) < __builtin_inff())) a[j] = 0;
 }
+template <typename T, int D>
+struct TileLanes;
+
 // The infinities and NaN of a tile's columns, one kind at a time as ones against ones at the visible pairs (`visible(row)`: of
 // the lane's column and that row of the tile): a positive count puts the value into the sum.
 template <typename T, int D, int ROWS, typename Tile, typename Visible>
-__device__ __forceinline__ void add_odd(const Tile &tile, f32x16 (&acc)[D / 32], Visible visible) {
+__device__ __forceinline__ void add_odd(const Tile &tile, const TileLanes<T, D> &lanes, f32x16 (&acc)[D / 32], Visible visible) {
     typedef typename Frag<T>::type frag;
     const uint32_t h = threadIdx.x % kWave / 32;
 #pragma unroll 1
@@ -109,7 +121,7 @@ __device__ __forceinline__ void add_odd(const Tile &tile, f32x16 (&acc)[D / 32],
         for (int j = 0; j < 8; j++) seen[j] = visible(r0 + 8 * (j / 4) + 4 * h + j % 4) ? 1 : 0;
 #pragma unroll
         for (int d = 0; d < D / 32; d++) {
-            const frag a = tile.columns(r0, d);
+            const frag a = tile.columns(lanes, r0, d);
             if (!any_odd(a)) continue;
 #pragma unroll 1
             for (int kind = 0; kind < 3; kind++) {
@@ -158,6 +170,26 @@ constexpr uint32_t kNowhere = 0x80000000u;  // an offset behind the end of any r
 // Until what Tile::request asked for is in LDS (this wavefront's part; a barrier makes it everyone's).
 __device__ __forceinline__ void wait_tiles() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
+// Where a lane reads in a tile (below), in bytes from its beginning.  The places differ by more than a constant only in the three
+// bits of the chunk's number that the row's number goes into: a few registers, and the rest is in the instructions.
+template <typename T, int D>
+struct TileLanes {
+    static constexpr uint32_t kRowBytes = D * sizeof(T);
+    uint32_t row[4], column[Frag<T>::kFloat ? 4 : 2];
+    __device__ __forceinline__ TileLanes() {
+        const uint32_t lane = threadIdx.x % kWave, h = lane / 32, i = lane % 16;
+        for (uint32_t j = 0; j < 4; j++)
+            row[j] = lane % 32 * kRowBytes + (((Frag<T>::kFloat ? 4 * (j / 2) + 2 * h + j % 2 : 2 * j + h) ^ lane % 8) * 16);
+        if constexpr (Frag<T>::kFloat) {
+            for (uint32_t j = 0; j < 4; j++)
+                column[j] = (4 * h + j) * kRowBytes + (lane % 32 / 4 ^ (4 * h + j)) * 16 + lane % 4 * 4;
+        } else {
+            for (uint32_t j = 0; j < 2; j++)
+                column[j] = (4 * h + i / 4) * kRowBytes + ((4 * j + 2 * (lane / 16 % 2) + i % 4 / 2) ^ (4 * h + i / 4)) * 16 + i % 2 * 8;
+        }
+    }
+};
+
 // A tile in LDS: ROWS rows of D values as 16-byte chunks, chunk c of row r at place c ^ (r & 7), so that lanes that read one
 // chunk of neighbouring rows, or neighbouring chunks of four rows, meet different banks.
 template <typename T, int D, int ROWS = Frag<T>::kTile>
@@ -180,13 +212,16 @@ struct Tile {
         const u32x4 resource = {(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)at), (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(at >> 32)),
                                 (uint32_t)__builtin_amdgcn_readfirstlane(bytes), 0x00020000u};
         const uint32_t first = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) * kWave;
-        const uint32_t lds = (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char *)data) + first * 16;
+        const uint32_t lds = __builtin_amdgcn_readfirstlane(
+            (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char *)data) + first * 16);
 #pragma unroll
-        for (int p = 0; p < kPerThread; p++)
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                         :
+        for (int p = 0; p < kPerThread; p++) {
+            uint32_t m0;  // (the compiler's own; a load takes it when it is issued)
+            asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
+                         : "=&s"(m0)
                          : "s"(lds + p * kAttnThreads * 16), "v"(offset[p]), "s"(resource)
-                         : "memory", "m0");
+                         : "memory");
+        }
     }
     // The same through registers, for rows that are no whole aligned vectors: `row(r)` is a row's first value, or null for zeros.
     template <typename Row>
@@ -198,39 +233,39 @@ struct Tile {
         }
     }
 
+    typedef __attribute__((address_space(3))) const char *lds_t;
     // A operand by rows: row r0 + (lane & 31), columns 16 k + 8 h ...
-    __device__ __forceinline__ frag rows(int r0, int k) const {
-        const uint32_t lane = threadIdx.x % kWave, r = r0 + lane % 32, h = lane / 32;
+    __device__ __forceinline__ frag rows(const TileLanes<T, D> &l, int r0, int k) const {
+        const lds_t at = (lds_t)data;
         frag f;
         u32x4 v[sizeof(T) / 2];
+        if constexpr (!Frag<T>::kFloat) {
+            v[0] = *(__attribute__((address_space(3))) const u32x4 *)(at + l.row[k % 4] + (r0 * kChunks * 16 + k / 4 * 128));
+        } else {
 #pragma unroll
-        for (uint32_t i = 0; i < sizeof(T) / 2; i++) v[i] = data[r * kChunks + (((2 * k + h) * (sizeof(T) / 2) + i) ^ (r & 7))];
+            for (int i = 0; i < 2; i++)
+                v[i] = *(__attribute__((address_space(3))) const u32x4 *)(at + l.row[k % 2 * 2 + i] + (r0 * kChunks * 16 + k / 2 * 128));
+        }
         __builtin_memcpy(&f, v, sizeof(f));
         return f;
     }
     // A operand by columns: column 32 db + (lane & 31), the 16 rows from r0 on in the accumulators' order
-    __device__ __forceinline__ frag columns(int r0, int db) const {
-        const uint32_t lane = threadIdx.x % kWave, h = lane / 32;
+    __device__ __forceinline__ frag columns(const TileLanes<T, D> &l, int r0, int db) const {
+        const lds_t at = (lds_t)data;
         frag f;
         if constexpr (!Frag<T>::kFloat) {
             // 16 lanes read 4 rows of 16 columns, 8 bytes a lane, and each gets a column of 4
-            const uint32_t i = lane % 16, col = 32 * db + 16 * (lane / 16 % 2) + 4 * (i % 4);
 #pragma unroll
             for (int u = 0; u < 2; u++) {
-                const uint32_t r = r0 + 8 * u + 4 * h + i / 4;
-                const char *p = reinterpret_cast<const char *>(data) + (r * kChunks + ((col / 8) ^ (r & 7))) * 16 + col % 8 * 2;
                 const fp16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4f16(
-                    (fp16x4 __attribute__((address_space(3))) *)(__attribute__((address_space(3))) const char *)p);
+                    (fp16x4 __attribute__((address_space(3))) *)(at + l.column[db % 2] + ((r0 + 8 * u) * kChunks * 16 + db / 2 * 128)));
 #pragma unroll
                 for (int j = 0; j < 4; j++) f[4 * u + j] = (_Float16)v[j];
             }
         } else {
-            const uint32_t col = 32 * db + lane % 32;
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const uint32_t r = r0 + 8 * (j / 4) + 4 * h + j % 4;
-                f[j] = reinterpret_cast<const float *>(data)[(r * kChunks + ((col / 4) ^ (r & 7))) * 4 + col % 4];
-            }
+            for (int j = 0; j < 8; j++)
+                f[j] = *(__attribute__((address_space(3))) const float *)(at + l.column[j % 4] + ((r0 + j / 4 * 8) * kChunks * 16 + db * 128));
         }
         return f;
     }
