@@ -40,7 +40,7 @@ __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_ke
     const uint32_t head = blockIdx.x % a.s.kv_heads, rest = blockIdx.x / a.s.kv_heads;
     const uint32_t part = rest % a.parts;
     uint32_t b, tile, q0, lq, k0, lk;
-    if (!find_tile(a.s.q_offsets, a.s.batch, a.s.q_rows, a.s.group, kAttnRows, rest / a.parts, b, tile)) return;
+    if (!find_tile(a.s.q_offsets, a.s.batch, a.s.q_rows, a.s.group, kAttnRows, rest / a.parts, a.s.q_by_tile, b, tile)) return;
     span(a.s.q_offsets, b, a.s.q_rows, q0, lq);
     span(a.s.k_offsets, b, a.s.k_rows, k0, lk);
     const uint32_t rows = lq * a.s.group;
@@ -291,8 +291,11 @@ size_t attn_workspace_bytes(const AttnProblem &p) {
 }
 
 AttnShape attn_shape(const AttnProblem &p) {
+    const size_t few = 8 * (size_t)chip_info().cus, once = 2 * (size_t)chip_info().cus;
+    const size_t k_blocks = p.batch * ((p.k_rows + kAttnRows - 1) / kAttnRows) * p.kv_heads;
     return AttnShape{p.q_offsets, p.k_offsets, (uint32_t)p.batch, (uint32_t)p.q_rows, (uint32_t)p.k_rows, (uint32_t)p.heads,
-                     (uint32_t)p.kv_heads, (uint32_t)(p.heads / p.kv_heads), (uint32_t)p.dim, p.scale * kLog2e, p.causal};
+                     (uint32_t)p.kv_heads, (uint32_t)(p.heads / p.kv_heads), (uint32_t)p.dim, p.scale * kLog2e, p.causal,
+                     p.causal && row_tiles(p) * p.kv_heads <= few, p.causal && k_blocks <= few, p.causal && k_blocks <= once};
 }
 
 bool attn_vectors(size_t elt, const AttnProblem &p, std::initializer_list<AttnView> views) {

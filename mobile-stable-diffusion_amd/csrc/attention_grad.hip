@@ -146,7 +146,7 @@ __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_gr
     const TileLanes<T, D> lanes;
     const uint32_t head = blockIdx.x % a.s.kv_heads;
     uint32_t b, tile, q0, lq, k0, lk;
-    if (!find_tile(a.s.q_offsets, a.s.batch, a.s.q_rows, a.s.group, kAttnRows, blockIdx.x / a.s.kv_heads, b, tile)) return;
+    if (!find_tile(a.s.q_offsets, a.s.batch, a.s.q_rows, a.s.group, kAttnRows, blockIdx.x / a.s.kv_heads, a.s.q_by_tile, b, tile)) return;
     span(a.s.q_offsets, b, a.s.q_rows, q0, lq);
     span(a.s.k_offsets, b, a.s.k_rows, k0, lk);
     const uint32_t rows = lq * a.s.group;
@@ -301,7 +301,11 @@ __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_gr
     const TileLanes<T, D> lanes;
     const uint32_t head = blockIdx.x % a.s.kv_heads;
     uint32_t b, tile, q0, lq, k0, lk;
-    if (!find_tile(a.s.k_offsets, a.s.batch, a.s.k_rows, 1, kAttnRows, blockIdx.x / a.s.kv_heads, b, tile)) return;
+    if (!find_tile(a.s.k_offsets, a.s.batch, a.s.k_rows, 1, kAttnRows, blockIdx.x / a.s.kv_heads, a.s.k_by_tile, b, tile)) return;
+    if (a.s.k_offsets == nullptr && a.s.k_folded) {
+        const uint32_t tiles = (a.s.k_rows + kAttnRows - 1) / kAttnRows, half = (tiles + 1) / 2;
+        if (tile >= half) tile = tiles - 1 - (tile - half);
+    }
     span(a.s.q_offsets, b, a.s.q_rows, q0, lq);
     span(a.s.k_offsets, b, a.s.k_rows, k0, lk);
     const bool packed = a.s.q_offsets != nullptr;

@@ -280,6 +280,10 @@ struct AttnShape {
     uint32_t heads, kv_heads, group, dim;
     float scale2;  // scale * log2(e)
     bool causal;
+    // Order of equal sequences' tiles.  Tile by tile (of all sequences, the longest first) where the work of tiles differs and a
+    // launch is few rounds of the chip's workgroups; otherwise sequence by sequence, which keeps fewer keys in an L2 at a time.
+    bool q_by_tile, k_by_tile;
+    bool k_folded;  // one round: the long tiles' half, then the short ones' backwards, so that a CU's two together are as long as others'
 };
 
 AttnShape attn_shape(const AttnProblem &p);
@@ -299,11 +303,16 @@ __device__ __forceinline__ void span(const int32_t *offsets, uint32_t b, uint32_
 }
 
 // Tile number `index` of all sequences' tiles, `per` rows each: a sequence has `times` rows for each of its offsets' rows.
-// False where there are fewer tiles.  Whole wavefronts look, 64 sequences at a time.
+// `by_tile`: see AttnShape.  False where there are fewer tiles.  Whole wavefronts look, 64 sequences at a time.
 __device__ __forceinline__ bool find_tile(const int32_t *offsets, uint32_t batch, uint32_t rows, uint32_t times, uint32_t per, uint32_t index,
-                                          uint32_t &b, uint32_t &tile) {
+                                          bool by_tile, uint32_t &b, uint32_t &tile) {
     if (offsets == nullptr) {
         const uint32_t tiles = (rows * times + per - 1) / per;
+        if (by_tile) {
+            tile = index / batch;
+            b = index - tile * batch;
+            return tile < tiles;
+        }
         b = index / tiles;
         tile = index - b * tiles;
         return b < batch;

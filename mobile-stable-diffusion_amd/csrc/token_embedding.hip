@@ -409,9 +409,10 @@ __global__ __launch_bounds__(kThreads) void embed_grad_slabs_kernel(const T *dy,
 }
 
 constexpr uint32_t kJoinColumns = 4 * kWave;
+constexpr uint32_t kJoinAlone = 16;  // slabs behind the first up to which a run is one wavefront's work
 
-// A workgroup for kSortWaves slabs and kJoinColumns columns, a wavefront looking at each slab: of a run that starts in one and goes on, the
-// wavefronts add a share of the parts each.  The workgroups behind `blocks` add dpositions' parts.
+// A workgroup for kSortWaves slabs and kJoinColumns columns, a wavefront looking at each slab: it adds the parts of a run that starts
+// in its slab and goes on, or, of a long one, all wavefronts a share each.  The workgroups behind `blocks` add dpositions' parts.
 template <typename T>
 __global__ __launch_bounds__(kSortThreads) void embed_grad_join_kernel(const Entry *sorted, const float *parts, T *dtable, uint32_t tokens,
                                                                        uint32_t dim, uint32_t vocab, float scale, uint32_t columns,
@@ -429,9 +430,17 @@ __global__ __launch_bounds__(kSortThreads) void embed_grad_join_kernel(const Ent
         return;
     }
     __shared__ float lds[kSortWaves][kJoinColumns];
-    __shared__ uint32_t run_id[kSortWaves], run_slabs[kSortWaves];  // (slabs behind the first that the run reaches; 0: no run)
+    __shared__ uint32_t run_id[kSortWaves], run_slabs[kSortWaves];  // (slabs behind the first that a long run reaches; 0: none)
     const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     const uint32_t slab0 = blockIdx.x / columns * kSortWaves, col0 = blockIdx.x % columns * kJoinColumns;
+    float sum[4];
+    auto add = [&](size_t part) {
+#pragma unroll
+        for (uint32_t c = 0; c < 4; c++) {
+            const uint32_t col = col0 + c * kWave + lane;
+            sum[c] += col < dim ? parts[part * dim + col] : 0.0f;
+        }
+    };
     {
         const uint32_t slab = slab0 + wave, begin = slab * kSlab;
         uint32_t id = 0, more = 0;
@@ -440,29 +449,37 @@ __global__ __launch_bounds__(kSortThreads) void embed_grad_join_kernel(const Ent
             const bool here = begin == 0 || sorted[begin - 1].id != id;  // (it starts in this slab)
             if (here && id < vocab && sorted[begin + kSlab].id == id) more = (first_of(sorted, tokens, id + 1) - 1) / kSlab - slab;
         }
+        more = __builtin_amdgcn_readfirstlane(more);
+        const bool is_long = more > kJoinAlone;
         if (lane == 0) {
             run_id[wave] = id;
-            run_slabs[wave] = more;
+            run_slabs[wave] = is_long ? more : 0;
+        }
+        if (more != 0 && !is_long) {  // most runs: the wavefront's own
+#pragma unroll
+            for (uint32_t c = 0; c < 4; c++) sum[c] = 0.0f;
+            add((size_t)slab * 2 + 1);
+#pragma unroll 4
+            for (uint32_t i = 0; i < more; i++) add(((size_t)slab + 1 + i) * 2);
+#pragma unroll
+            for (uint32_t c = 0; c < 4; c++) {
+                const uint32_t col = col0 + c * kWave + lane;
+                if (col < dim) Store<T>::store1(dtable + (size_t)id * dim + col, sum[c] * scale);
+            }
         }
     }
     __syncthreads();
     for (uint32_t s = 0; s < kSortWaves; s++) {
         const uint32_t slabs = run_slabs[s], slab = slab0 + s;
         if (slabs == 0) continue;
-        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         const uint32_t each = (slabs + kSortWaves - 1) / kSortWaves, stop = min(slabs, (wave + 1) * each);
-        auto add = [&](size_t part) {
 #pragma unroll
-            for (uint32_t c = 0; c < 4; c++) {
-                const uint32_t col = col0 + c * kWave + lane;
-                sum[c] += col < dim ? parts[part * dim + col] : 0.0f;
-            }
-        };
+        for (uint32_t c = 0; c < 4; c++) sum[c] = 0.0f;
         if (wave == 0) add((size_t)slab * 2 + 1);
         uint32_t i = wave * each;
-        for (; i + 4 <= stop; i += 4)
+        for (; i + 8 <= stop; i += 8)
 #pragma unroll
-            for (uint32_t u = 0; u < 4; u++) add(((size_t)slab + 1 + i + u) * 2);
+            for (uint32_t u = 0; u < 8; u++) add(((size_t)slab + 1 + i + u) * 2);
         for (; i < stop; i++) add(((size_t)slab + 1 + i) * 2);
 #pragma unroll
         for (uint32_t c = 0; c < 4; c++) lds[wave][c * kWave + lane] = sum[c];
