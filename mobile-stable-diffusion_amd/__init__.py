@@ -589,18 +589,12 @@ def layernorm(x, gamma, beta, eps=1e-5, out=None):
     return out
 
 
-@functools.lru_cache(maxsize=1024)
-def _workspace_bytes(name, *args):
-    size = ctypes.c_size_t(0)
-    check(getattr(load_library(), name)(*args, ctypes.byref(size)))
-    return size.value
-
-
 def _workspace(like, name, *args):
     """(tensor to keep until the call is made, its pointer, its bytes)."""
-    size = _workspace_bytes(name, *args)
-    t = like.new_empty(size, dtype=_torch.uint8)
-    return t, t.data_ptr(), size
+    size = ctypes.c_size_t(0)
+    check(getattr(load_library(), name)(*args, ctypes.byref(size)))
+    t = like.new_empty(size.value, dtype=_torch.uint8)
+    return t, t.data_ptr(), size.value
 
 
 def layernorm_backward(dy, x, gamma, eps=1e-5, dsum=None, affine=True, out=None):

@@ -582,7 +582,7 @@ int msd_layernorm_backward(const void *dy, const void *x, const void *dsum, cons
         overlaps_any(dx, bytes, {in, g, w, dg, db}) || overlaps_any(dgamma, affine, {d, in, s, g, w, db}) ||
         overlaps_any(dbeta, affine, {d, in, s, g, w}) || overlaps_any(workspace, need, {d, in, s, g}))
         return MSD_ERR_INVALID_VALUE;
-    const LnGrad a = {dy, x, dsum, gamma, dx, dgamma, dbeta, workspace};
+    const LnGrad a = {dy, x, dsum, gamma, dx, dgamma, dbeta, workspace, workspace_bytes};
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (dtype == MSD_DTYPE_F32) return ln_grad_dispatch<float>(a, rows, dim, eps, st);
     return ln_grad_dispatch<__half>(a, rows, dim, eps, st);
@@ -637,7 +637,7 @@ int msd_token_embedding_backward(const int64_t *ids, const void *dy, void *dtabl
     if (overlaps_any(dtable, table_bytes, {i, d, w, p}) || overlaps_any(dpositions, place_bytes, {i, d, w}) ||
         overlaps_any(workspace, need, {i, d}))
         return MSD_ERR_INVALID_VALUE;
-    const EmbedGrad g = {ids, dy, dtable, dpositions, workspace};
+    const EmbedGrad g = {ids, dy, dtable, dpositions, workspace, workspace_bytes};
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (dtype == MSD_DTYPE_F32) return embed_grad_dispatch<float>(g, tokens, length, vocab, positions, dim, scale, s);
     return embed_grad_dispatch<__half>(g, tokens, length, vocab, positions, dim, scale, s);
@@ -968,8 +968,8 @@ int msd_attention(const void *q, const void *k, const void *v, void *out, float 
         return MSD_ERR_INVALID_VALUE;
     const AttnProblem p = attention_problem(q_offsets, k_offsets, batch, q_rows, k_rows, heads, kv_heads, dim, scale, causal);
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (dtype == MSD_DTYPE_F32) return attn_dispatch<float>(p, t[0].view, t[1].view, t[2].view, t[3].view, lse, rest, workspace, st);
-    return attn_dispatch<__half>(p, t[0].view, t[1].view, t[2].view, t[3].view, lse, rest, workspace, st);
+    if (dtype == MSD_DTYPE_F32) return attn_dispatch<float>(p, t[0].view, t[1].view, t[2].view, t[3].view, lse, rest, workspace, workspace_bytes, st);
+    return attn_dispatch<__half>(p, t[0].view, t[1].view, t[2].view, t[3].view, lse, rest, workspace, workspace_bytes, st);
 }
 
 int msd_attention_backward(const void *dout, const void *q, const void *k, const void *v, const void *out, const float *lse, const void *rest, void *dq,
@@ -1008,8 +1008,8 @@ int msd_attention_backward(const void *dout, const void *q, const void *k, const
     const AttnProblem p = attention_problem(q_offsets, k_offsets, batch, q_rows, k_rows, heads, kv_heads, dim, scale, causal);
     const AttnGradViews g = {t[0].view, t[1].view, t[2].view, t[3].view, t[4].view, t[5].view, t[6].view, t[7].view};
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (dtype == MSD_DTYPE_F32) return attn_grad_dispatch<float>(p, g, lse, rest, workspace, st);
-    return attn_grad_dispatch<__half>(p, g, lse, rest, workspace, st);
+    if (dtype == MSD_DTYPE_F32) return attn_grad_dispatch<float>(p, g, lse, rest, workspace, workspace_bytes, st);
+    return attn_grad_dispatch<__half>(p, g, lse, rest, workspace, workspace_bytes, st);
 }
 
 int msd_alphas_cumprod(float *out_1000) {

@@ -147,12 +147,12 @@ __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_ke
                     for (int u = 0; u < 2; u++) {
                         frag p;
                         to_frag(s[n], u, p);
+                        frag v[DB];
 #pragma unroll
-                        for (int d = 0; d < DB; d++) {
-                            frag v = vt.columns(lanes, 32 * n + 16 * u, d);
-                            if constexpr (MASKED) leave_out_odd(v, odd);
-                            o[d] = mma(v, p, o[d]);
-                        }
+                        for (int d = 0; d < DB; d++) v[d] = vt.columns(lanes, 32 * n + 16 * u, d);
+                        if constexpr (MASKED) leave_out_odd<DB>(v, odd);
+#pragma unroll
+                        for (int d = 0; d < DB; d++) o[d] = mma(v[d], p, o[d]);
                         step_end<Frag<T>::kFloat>();
                     }
                 if (MASKED && odd) add_odd<T, D, R>(vt, lanes, o, [&](uint32_t r) { return first + r < limit; });
@@ -242,26 +242,29 @@ __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(const Forward a
         }
         if (__builtin_amdgcn_ballot_w64(inside) == 0) return;
     }
-    float most = -__builtin_inff();
-    for (uint32_t p = 0; p < a.parts; p++) most = fmaxf(most, a.part_lse[p * count + at]);
-    const float base = most == -__builtin_inff() ? 0.0f : most;
-    float sum = 0.0f;
-    bool bad = false;  // (a NaN is no maximum)
-    for (uint32_t p = 0; p < a.parts; p++) {
-        const float l = a.part_lse[p * count + at];
-        bad |= l != l;
-        sum += __builtin_amdgcn_exp2f(l - base);
-    }
-    const float inv = bad ? __builtin_nanf("") : sum == 0.0f ? 0.0f : 1.0f / sum;
+    // a part's share of the weights, one to a lane
+    const float l = lane < a.parts ? a.part_lse[lane * count + at] : -__builtin_inff();
+    const float most = team_max<64>(l), base = most == -__builtin_inff() ? 0.0f : most;
+    const float weight = __builtin_amdgcn_exp2f(l - base), sum = wave_sum(weight);  // (NaN where any is)
+    const float share = sum == 0.0f ? 0.0f : weight / sum;
     T *const to = static_cast<T *>(const_cast<void *>(a.out.at)) + b * a.out.batch + (size_t)i * a.out.row + head * a.out.head;
-    for (uint32_t d = lane; d < a.s.dim; d += kWave) {
+    for (uint32_t d = lane; d < a.s.dim + lane; d += kWave) {  // (all lanes take every turn: each hands out its share)
         float t = 0.0f;
-        for (uint32_t p = 0; p < a.parts; p++) {
-            const float w = __builtin_amdgcn_exp2f(a.part_lse[p * count + at] - base);
-            if (w != 0.0f) t = fmaf(w * inv, a.part[(p * count + at) * a.s.dim + d], t);
+        for (uint32_t p0 = 0; p0 < a.parts; p0 += 8) {
+            float f[8];
+#pragma unroll
+            for (uint32_t u = 0; u < 8; u++)
+                f[u] = p0 + u < a.parts && d < a.s.dim ? a.part[((p0 + u) * count + at) * a.s.dim + d] : 0.0f;
+#pragma unroll
+            for (uint32_t u = 0; u < 8; u++) {
+                const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(share), min(p0 + u, kWave - 1)));
+                if (w != 0.0f) t = fmaf(w, f[u], t);
+            }
         }
-        Store<T>::store1(to + d, t);
-        if (!Frag<T>::kFloat && a.rest != nullptr) Store<T>::store1(static_cast<T *>(a.rest) + at * a.s.dim + d, t - round_to_storage<T>(t));
+        if (d < a.s.dim) {
+            Store<T>::store1(to + d, t);
+            if (!Frag<T>::kFloat && a.rest != nullptr) Store<T>::store1(static_cast<T *>(a.rest) + at * a.s.dim + d, t - round_to_storage<T>(t));
+        }
     }
     if (a.lse != nullptr && lane == 0) a.lse[at] = sum == 0.0f ? -__builtin_inff() : base + __builtin_amdgcn_logf(sum);
 }
@@ -273,12 +276,14 @@ size_t row_tiles(const AttnProblem &p) {
     return p.q_rows * group / kAttnRows + p.batch;
 }
 
-// Parts of the keys: workgroups for two of the chip's CUs each, at least 256 keys in a part on average.
+// Parts of the keys: workgroups for eight rounds of the chip where the sequences' lengths may differ, for two otherwise, with at
+// least 256 keys in a part on average; one wavefront joins at most kWave of them.
 uint32_t key_parts(const AttnProblem &p) {
-    const size_t keys = p.k_offsets == nullptr ? p.k_rows : p.k_rows / std::max<size_t>(1, p.batch);
-    const size_t blocks = std::max<size_t>(1, row_tiles(p) * p.kv_heads), want = 2 * (size_t)chip_info().cus;
-    if (blocks * 2 > want) return 1;
-    return (uint32_t)std::max<size_t>(1, std::min<size_t>(want / blocks, keys / 256));
+    const bool packed = p.k_offsets != nullptr;
+    const size_t keys = packed ? p.k_rows / std::max<size_t>(1, p.batch) : p.k_rows;
+    const size_t blocks = std::max<size_t>(1, row_tiles(p) * p.kv_heads), cus = chip_info().cus;
+    if (blocks > cus) return 1;
+    return (uint32_t)std::max<size_t>(1, std::min<size_t>({(packed ? 8 : 2) * cus / blocks, keys / 256, (size_t)kWave}));
 }
 
 size_t total_rows(const AttnProblem &p) { return p.q_offsets == nullptr ? p.batch * p.q_rows : p.q_rows; }
@@ -291,11 +296,11 @@ size_t attn_workspace_bytes(const AttnProblem &p) {
 }
 
 AttnShape attn_shape(const AttnProblem &p) {
-    const size_t few = 8 * (size_t)chip_info().cus, once = 2 * (size_t)chip_info().cus;
+    const size_t few = 8 * (size_t)chip_info().cus;
     const size_t k_blocks = p.batch * ((p.k_rows + kAttnRows - 1) / kAttnRows) * p.kv_heads;
     return AttnShape{p.q_offsets, p.k_offsets, (uint32_t)p.batch, (uint32_t)p.q_rows, (uint32_t)p.k_rows, (uint32_t)p.heads,
                      (uint32_t)p.kv_heads, (uint32_t)(p.heads / p.kv_heads), (uint32_t)p.dim, p.scale * kLog2e, p.causal,
-                     p.causal && row_tiles(p) * p.kv_heads <= few, p.causal && k_blocks <= few, p.causal && k_blocks <= once};
+                     p.causal && row_tiles(p) * p.kv_heads <= few, p.causal && k_blocks <= few};
 }
 
 bool attn_vectors(size_t elt, const AttnProblem &p, std::initializer_list<AttnView> views) {
@@ -308,11 +313,12 @@ bool attn_vectors(size_t elt, const AttnProblem &p, std::initializer_list<AttnVi
 
 template <typename T>
 int attn_dispatch(const AttnProblem &p, const AttnView &q, const AttnView &k, const AttnView &v, const AttnView &out, float *lse,
-                  void *rest, void *workspace, hipStream_t stream) {
+                  void *rest, void *workspace, size_t workspace_bytes, hipStream_t stream) {
     const size_t tiles = row_tiles(p);
     if (tiles == 0) return MSD_OK;
     Forward a{attn_shape(p), q, k, v, out, lse, rest, nullptr, nullptr, key_parts(p), (uint32_t)total_rows(p),
               attn_vectors(sizeof(T), p, {q, k, v, out, AttnView{rest, 0, 0, 0}})};
+    a.parts = (uint32_t)std::max<size_t>(1, std::min<size_t>(a.parts, workspace_bytes / (total_rows(p) * p.heads * (p.dim + 1) * sizeof(float))));
     if (a.parts > 1) {
         a.part = static_cast<float *>(workspace);
         a.part_lse = a.part + (size_t)a.parts * a.total_rows * p.heads * p.dim;
@@ -329,8 +335,8 @@ int attn_dispatch(const AttnProblem &p, const AttnView &q, const AttnView &k, co
 }
 
 template int attn_dispatch<float>(const AttnProblem &, const AttnView &, const AttnView &, const AttnView &, const AttnView &, float *,
-                                  void *, void *, hipStream_t);
+                                  void *, void *, size_t, hipStream_t);
 template int attn_dispatch<__half>(const AttnProblem &, const AttnView &, const AttnView &, const AttnView &, const AttnView &, float *,
-                                   void *, void *, hipStream_t);
+                                   void *, void *, size_t, hipStream_t);
 
 }  // namespace msd

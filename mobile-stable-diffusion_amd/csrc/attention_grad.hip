@@ -23,7 +23,8 @@ struct Backward {
     const float *lse;
     const void *rest;  // [rows][heads][dim] what rounding took from out, or null
     float *delta, *norm, *v_norm;  // [rows][heads] D and |do|, [keys][kv_heads] |v|; the norms null for float32
-    uint32_t total_rows, total_keys;
+    float *part;  // parts > 1: [parts][keys][kv_heads][dk, dv][dim]
+    uint32_t total_rows, total_keys, parts;
     FastDiv by_group;
     bool vec;
 };
@@ -254,12 +255,12 @@ __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_gr
                     for (int u = 0; u < 2; u++) {
                         frag ds;
                         to_frag(s, u, ds);
+                        frag k[DB];
 #pragma unroll
-                        for (int d = 0; d < DB; d++) {
-                            frag k = kt.columns(lanes, 32 * n + 16 * u, d);
-                            if constexpr (MASKED) leave_out_odd(k, odd);
-                            dq[d] = mma(k, ds, dq[d]);
-                        }
+                        for (int d = 0; d < DB; d++) k[d] = kt.columns(lanes, 32 * n + 16 * u, d);
+                        if constexpr (MASKED) leave_out_odd<DB>(k, odd);
+#pragma unroll
+                        for (int d = 0; d < DB; d++) dq[d] = mma(k[d], ds, dq[d]);
                         step_end<Frag<T>::kFloat || D == 128>();
                     }
                 }
@@ -301,11 +302,8 @@ __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_gr
     const TileLanes<T, D> lanes;
     const uint32_t head = blockIdx.x % a.s.kv_heads;
     uint32_t b, tile, q0, lq, k0, lk;
-    if (!find_tile(a.s.k_offsets, a.s.batch, a.s.k_rows, 1, kAttnRows, blockIdx.x / a.s.kv_heads, a.s.k_by_tile, b, tile)) return;
-    if (a.s.k_offsets == nullptr && a.s.k_folded) {
-        const uint32_t tiles = (a.s.k_rows + kAttnRows - 1) / kAttnRows, half = (tiles + 1) / 2;
-        if (tile >= half) tile = tiles - 1 - (tile - half);
-    }
+    if (!find_tile(a.s.k_offsets, a.s.batch, a.s.k_rows, 1, kAttnRows, blockIdx.x / a.s.kv_heads / a.parts, a.s.k_by_tile, b, tile)) return;
+    const uint32_t part = blockIdx.x / a.s.kv_heads % a.parts;
     span(a.s.q_offsets, b, a.s.q_rows, q0, lq);
     span(a.s.k_offsets, b, a.s.k_rows, k0, lk);
     const bool packed = a.s.q_offsets != nullptr;
@@ -351,7 +349,8 @@ __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_gr
     const uint32_t from = live ? first_row(key) : rows;                                  // the lane's rows: [from, rows)
     const uint32_t wave_from = wave_key < lk ? first_row(wave_key) : rows;               // the first any key is seen by
     const uint32_t wave_full = wave_key < lk ? first_row(min(lk - 1, wave_key + 31)) : rows; // from here on all are
-    const uint32_t t0 = first_row(tile * kAttnRows) / R, t1 = (rows + R - 1) / R;
+    const uint32_t from_tile = min(first_row(tile * kAttnRows), rows) / R, all = (rows + R - 1) / R - from_tile;
+    const uint32_t each = (all + a.parts - 1) / a.parts, t0 = from_tile + min(all, part * each), t1 = min(from_tile + all, t0 + each);
 
     float next_stat[3] = {0.0f, 0.0f, 0.0f};
     auto fetch = [&](uint32_t t, uint32_t buffer) {
@@ -475,13 +474,13 @@ __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_gr
                     for (int u = 0; u < 2; u++) {
 #pragma unroll
                         for (int d = 0; d < DB; d++) {
-                            frag gc = gt.columns(lanes, 32 * n + 16 * u, d), qc = qt.columns(lanes, 32 * n + 16 * u, d);
+                            frag gc[1] = {gt.columns(lanes, 32 * n + 16 * u, d)}, qc[1] = {qt.columns(lanes, 32 * n + 16 * u, d)};
                             if constexpr (MASKED) {
-                                leave_out_odd(gc, odd);
-                                leave_out_odd(qc, odd);
+                                leave_out_odd<1>(gc, odd);
+                                leave_out_odd<1>(qc, odd);
                             }
-                            dv[d] = mma(gc, p[u], dv[d]);
-                            dk[d] = mma(qc, ds[u], dk[d]);
+                            dv[d] = mma(gc[0], p[u], dv[d]);
+                            dk[d] = mma(qc[0], ds[u], dk[d]);
                             step_end<Frag<T>::kFloat || D == 128>();
                         }
                     }
@@ -499,13 +498,53 @@ __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_gr
         }
         if (t + 1 < t1) put((t + 1 - t0) & 1);
     }
-    if (!live) return;
+    uint32_t thread = threadIdx.x;  // (the key's number is formed again: over the loop there is no register for it)
+    asm volatile("" : "+v"(thread));
+    const uint32_t own_key = tile * kAttnRows + thread / kWave * 32 + thread % 32;
+    if (own_key >= lk) return;
     auto out = [&](const AttnView &to) {
-        return static_cast<T *>(const_cast<void *>(to.at)) + (packed ? 0 : b * to.batch) + (size_t)(k0 + key) * to.row + head * to.head;
+        return static_cast<T *>(const_cast<void *>(to.at)) + (packed ? 0 : b * to.batch) + (size_t)(k0 + own_key) * to.row + head * to.head;
     };
     const float natural = a.s.scale2 * (1.0f / kLog2e);
-    store_rows<T, D>(out(a.dk), dk, kHalf ? ldexpf(natural, -scale.power) : natural, a.s.dim, a.vec);
-    store_rows<T, D>(out(a.dv), dv, ldexpf(1.0f, -kPShift<T>), a.s.dim, a.vec);
+    const float by_k = kHalf ? ldexpf(natural, -scale.power) : natural, by_v = ldexpf(1.0f, -kPShift<T>);
+    if (a.parts > 1) {
+        const size_t place = ((size_t)(packed ? 0 : b) * lk + k0 + own_key) * a.s.kv_heads + head;
+        float *const to = a.part + (part * (size_t)a.total_keys * a.s.kv_heads + place) * 2 * a.s.dim;
+        const bool whole = a.s.dim % 4 == 0;
+        store_rows<float, D>(to, dk, by_k, a.s.dim, whole);
+        store_rows<float, D>(to + a.s.dim, dv, by_v, a.s.dim, whole);
+        return;
+    }
+    store_rows<T, D>(out(a.dk), dk, by_k, a.s.dim, a.vec);
+    store_rows<T, D>(out(a.dv), dv, by_v, a.s.dim, a.vec);
+}
+
+// dk and dv from the parts, for a tile of keys of a head, in the parts' order.
+template <typename T>
+__global__ __launch_bounds__(kAttnThreads) void attn_grad_join_kernel(const Backward a) {
+    const uint32_t head = blockIdx.x % a.s.kv_heads;
+    uint32_t b, tile, k0, lk;
+    if (!find_tile(a.s.k_offsets, a.s.batch, a.s.k_rows, 1, kAttnRows, blockIdx.x / a.s.kv_heads, false, b, tile)) return;
+    span(a.s.k_offsets, b, a.s.k_rows, k0, lk);
+    const bool packed = a.s.k_offsets != nullptr;
+    const uint32_t n = min(kAttnRows, lk - tile * kAttnRows), row = 2 * a.s.dim;
+    const size_t step = (size_t)a.total_keys * a.s.kv_heads * row;
+    for (uint32_t at = threadIdx.x; at < n * row; at += kAttnThreads) {
+        const uint32_t r = at / row, c = at - r * row, key = tile * kAttnRows + r;
+        const float *from = a.part + (((size_t)(packed ? 0 : b) * lk + k0 + key) * a.s.kv_heads + head) * row + c;
+        float sum = 0.0f;
+        for (uint32_t p0 = 0; p0 < a.parts; p0 += 8) {
+            float f[8];
+#pragma unroll
+            for (uint32_t u = 0; u < 8; u++) f[u] = p0 + u < a.parts ? from[(p0 + u) * step] : 0.0f;
+#pragma unroll
+            for (uint32_t u = 0; u < 8; u++) sum += f[u];
+        }
+        const bool of_k = c < a.s.dim;
+        const AttnView &to = of_k ? a.dk : a.dv;
+        Store<T>::store1(static_cast<T *>(const_cast<void *>(to.at)) + (packed ? 0 : b * to.batch) + (size_t)(k0 + key) * to.row +
+                             head * to.head + (of_k ? c : c - a.s.dim), sum);
+    }
 }
 
 size_t tiles_of(const int32_t *offsets, size_t batch, size_t rows, size_t times) {
@@ -513,26 +552,45 @@ size_t tiles_of(const int32_t *offsets, size_t batch, size_t rows, size_t times)
     return rows * times / kAttnRows + batch;
 }
 
+// Parts of the rows for dk and dv.  Under a causal mask tiles of keys differ in the rows that see them: cut in two they fill up
+// a launch of few rounds.  Few keys and many rows (a prompt's keys, an image's rows) are cut until the chip is full, with
+// at least 256 rows in a part on average.
+uint32_t row_parts(const AttnProblem &p) {
+    const size_t blocks = std::max<size_t>(1, tiles_of(p.k_offsets, p.batch, p.k_rows, 1) * p.kv_heads), once = 2 * (size_t)chip_info().cus;
+    const size_t rows = (p.q_offsets != nullptr ? p.q_rows / std::max<size_t>(1, p.batch) : p.q_rows) * (p.heads / p.kv_heads);
+    size_t parts = p.causal && blocks <= 4 * once ? 2 : 1;
+    if (blocks * parts < once) parts = (once + blocks - 1) / blocks;
+    return (uint32_t)std::max<size_t>(1, std::min<size_t>(parts, rows / 256));
+}
+
 }  // namespace
 
 size_t attn_grad_workspace_bytes(const AttnProblem &p) {
     const size_t rows = p.q_offsets == nullptr ? p.batch * p.q_rows : p.q_rows, keys = p.k_offsets == nullptr ? p.batch * p.k_rows : p.k_rows;
-    return (2 * rows * p.heads + keys * p.kv_heads) * sizeof(float);
+    AttnProblem masked = p, open = p;  // (the bytes go by the sizes alone, the parts by the mask too)
+    masked.causal = true;
+    open.causal = false;
+    const size_t parts = std::max(row_parts(masked), row_parts(open)), vectors = (2 * rows * p.heads + keys * p.kv_heads + 3) / 4 * 4;
+    return (vectors + (parts > 1 ? parts * keys * p.kv_heads * 2 * p.dim : 0)) * sizeof(float);
 }
 
 template <typename T>
-int attn_grad_dispatch(const AttnProblem &p, const AttnGradViews &g, const float *lse, const void *rest, void *workspace, hipStream_t stream) {
+int attn_grad_dispatch(const AttnProblem &p, const AttnGradViews &g, const float *lse, const void *rest, void *workspace, size_t workspace_bytes,
+                       hipStream_t stream) {
     const size_t rows = p.q_offsets == nullptr ? p.batch * p.q_rows : p.q_rows, keys = p.k_offsets == nullptr ? p.batch * p.k_rows : p.k_rows;
     float *const delta = static_cast<float *>(workspace);
     constexpr bool kHalf = !Frag<T>::kFloat;
+    float *const part = delta + (2 * rows * p.heads + keys * p.kv_heads + 3) / 4 * 4;
+    const size_t vectors = (size_t)(part - delta) * sizeof(float), part_bytes = std::max<size_t>(1, keys * p.kv_heads * 2 * p.dim * sizeof(float));
+    const uint32_t parts = (uint32_t)std::max<size_t>(1, std::min<size_t>(row_parts(p), (workspace_bytes - vectors) / part_bytes));
     const Backward a{attn_shape(p), g.q, g.k, g.v, g.out, g.dout, g.dq, g.dk, g.dv, lse, rest, delta,
-                     kHalf ? delta + rows * p.heads : nullptr, kHalf ? delta + 2 * rows * p.heads : nullptr, (uint32_t)rows, (uint32_t)keys,
+                     kHalf ? delta + rows * p.heads : nullptr, kHalf ? delta + 2 * rows * p.heads : nullptr, part, (uint32_t)rows, (uint32_t)keys, parts,
                      make_fast_div((uint32_t)(p.heads / p.kv_heads)), attn_vectors(sizeof(T), p, {g.q, g.k, g.v, g.out, g.dout, g.dq, g.dk, g.dv, AttnView{rest, 0, 0, 0}})};
     const size_t items = rows * p.heads + (kHalf ? keys * p.kv_heads : 0);
     if (items != 0)
         launch((attn_grad_rows_kernel<T>), dim3((uint32_t)((items + 15) / 16)), dim3(kAttnThreads), 0, stream, a);
     const dim3 of_rows((uint32_t)(tiles_of(p.q_offsets, p.batch, p.q_rows, p.heads / p.kv_heads) * p.kv_heads));
-    const dim3 of_keys((uint32_t)(tiles_of(p.k_offsets, p.batch, p.k_rows, 1) * p.kv_heads));
+    const dim3 key_tiles((uint32_t)(tiles_of(p.k_offsets, p.batch, p.k_rows, 1) * p.kv_heads)), of_keys(key_tiles.x * parts);
     if (p.dim <= 64) {
         if (of_keys.x != 0) launch((attn_grad_kv_kernel<T, 64>), of_keys, dim3(kAttnThreads), 0, stream, a);
         if (of_rows.x != 0) launch((attn_grad_q_kernel<T, 64>), of_rows, dim3(kAttnThreads), 0, stream, a);
@@ -540,10 +598,11 @@ int attn_grad_dispatch(const AttnProblem &p, const AttnGradViews &g, const float
         if (of_keys.x != 0) launch((attn_grad_kv_kernel<T, 128>), of_keys, dim3(kAttnThreads), 0, stream, a);
         if (of_rows.x != 0) launch((attn_grad_q_kernel<T, 128>), of_rows, dim3(kAttnThreads), 0, stream, a);
     }
+    if (parts > 1 && key_tiles.x != 0) launch((attn_grad_join_kernel<T>), key_tiles, dim3(kAttnThreads), 0, stream, a);
     return launch_status();
 }
 
-template int attn_grad_dispatch<float>(const AttnProblem &, const AttnGradViews &, const float *, const void *, void *, hipStream_t);
-template int attn_grad_dispatch<__half>(const AttnProblem &, const AttnGradViews &, const float *, const void *, void *, hipStream_t);
+template int attn_grad_dispatch<float>(const AttnProblem &, const AttnGradViews &, const float *, const void *, void *, size_t, hipStream_t);
+template int attn_grad_dispatch<__half>(const AttnProblem &, const AttnGradViews &, const float *, const void *, void *, size_t, hipStream_t);
 
 }  // namespace msd

@@ -88,22 +88,28 @@ __device__ __forceinline__ void keep_here(f32x8 &) {}
 
 // A masked pair's weight is zero, but zero times an infinity or NaN is not.  Where a tile has masked pairs, what its A operands
 // hold of those is left out of the product, and `add_odd` puts it back for the pairs that are visible.
-template <typename F>
-__device__ __forceinline__ bool any_odd(const F &a) {
-    uint32_t w[sizeof(F) / 4], found = 0;
-    __builtin_memcpy(w, &a, sizeof(F));
+template <int N, typename F>
+__device__ __forceinline__ bool any_odd(const F (&a)[N]) {
+    uint32_t found = 0;
 #pragma unroll
-    for (uint32_t i = 0; i < sizeof(F) / 4; i++)  // (an exponent of ones, and one more, is the sign's bit)
-        found |= sizeof(F) == 16 ? (w[i] & 0x7C007C00u) + 0x04000400u : (w[i] & 0x7F800000u) + 0x00800000u;
+    for (int n = 0; n < N; n++) {
+        uint32_t w[sizeof(F) / 4];
+        __builtin_memcpy(w, &a[n], sizeof(F));
+#pragma unroll
+        for (uint32_t i = 0; i < sizeof(F) / 4; i++)  // (an exponent of ones, and one more, is the sign's bit)
+            found |= sizeof(F) == 16 ? (w[i] & 0x7C007C00u) + 0x04000400u : (w[i] & 0x7F800000u) + 0x00800000u;
+    }
     return __builtin_amdgcn_ballot_w64((found & (sizeof(F) == 16 ? 0x80008000u : 0x80000000u)) != 0) != 0;
 }
-template <typename F>
-__device__ __forceinline__ void leave_out_odd(F &a, bool &odd) {
-    if (!any_odd(a)) return;
+template <int N, typename F>
+__device__ __forceinline__ void leave_out_odd(F (&a)[N], bool &odd) {
+    if (!any_odd<N>(a)) return;
     odd = true;
 #pragma unroll
-    for (int j = 0; j < 8; j++)
-        if (!(__builtin_fabsf((float)a[j]) < __builtin_inff())) a[j] = 0;
+    for (int n = 0; n < N; n++)
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (!(__builtin_fabsf((float)a[n][j]) < __builtin_inff())) a[n][j] = 0;
 }
 template <typename T, int D>
 struct TileLanes;
@@ -121,8 +127,8 @@ __device__ __forceinline__ void add_odd(const Tile &tile, const TileLanes<T, D> 
         for (int j = 0; j < 8; j++) seen[j] = visible(r0 + 8 * (j / 4) + 4 * h + j % 4) ? 1 : 0;
 #pragma unroll
         for (int d = 0; d < D / 32; d++) {
-            const frag a = tile.columns(lanes, r0, d);
-            if (!any_odd(a)) continue;
+            const frag one[1] = {tile.columns(lanes, r0, d)}, &a = one[0];
+            if (!any_odd<1>(one)) continue;
 #pragma unroll 1
             for (int kind = 0; kind < 3; kind++) {
                 const float value = kind == 0 ? __builtin_inff() : kind == 1 ? -__builtin_inff() : __builtin_nanf("");
@@ -283,7 +289,6 @@ struct AttnShape {
     // Order of equal sequences' tiles.  Tile by tile (of all sequences, the longest first) where the work of tiles differs and a
     // launch is few rounds of the chip's workgroups; otherwise sequence by sequence, which keeps fewer keys in an L2 at a time.
     bool q_by_tile, k_by_tile;
-    bool k_folded;  // one round: the long tiles' half, then the short ones' backwards, so that a CU's two together are as long as others'
 };
 
 AttnShape attn_shape(const AttnProblem &p);

@@ -186,11 +186,9 @@ __global__ __launch_bounds__(kJoinThreads) void ln_grad_join_kernel(const float 
     float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     if (col < 2 * dim) {
         const uint32_t each = (parts + kJoinRuns - 1) / kJoinRuns, last = min(parts, (run + 1) * each);
-        uint32_t p = run * each;
-        for (; p + 8 <= last; p += 8)
+        for (uint32_t p = run * each; p < last; p += 8)
 #pragma unroll
-            for (int i = 0; i < 8; i++) t[i % 4] += partial[(size_t)(p + i) * 2 * dim + col];
-        for (; p < last; p++) t[0] += partial[(size_t)p * 2 * dim + col];
+            for (int i = 0; i < 8; i++) t[i % 4] += p + i < last ? partial[(size_t)(p + i) * 2 * dim + col] : 0.0f;
     }
     lds[run][lane] = (t[0] + t[1]) + (t[2] + t[3]);
     __syncthreads();
@@ -364,7 +362,9 @@ int ln_grad_dispatch(const LnGrad &g, size_t rows, size_t dim, float eps, hipStr
         return launch_status();
     }
     const bool aligned = aligned16(g.dy) && aligned16(g.x) && aligned16(g.dx) && aligned16(g.dsum);
-    const Plan p = make_plan(sizeof(T), rows, dim, aligned);
+    Plan p = make_plan(sizeof(T), rows, dim, aligned);
+    const size_t room = (g.workspace_bytes - (p.tl == 0 ? rows * sizeof(f32x4) : 0)) / (2 * dim * sizeof(float));
+    p.blocks = (uint32_t)std::min<size_t>(p.blocks, room);
     const bool affine = g.dgamma != nullptr;
     f32x4 *const stats = static_cast<f32x4 *>(g.workspace);
     float *const partial = static_cast<float *>(g.workspace) + (p.tl == 0 ? 4 * rows : 0);

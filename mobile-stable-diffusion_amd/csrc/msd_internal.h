@@ -178,6 +178,7 @@ struct LnGrad {
     void *dx;
     float *dgamma, *dbeta;  // both or neither
     void *workspace;
+    size_t workspace_bytes;  // (a launch is cut into no more parts than these hold, whatever the plan has become since they were asked for)
 };
 // SIZE_MAX for a shape beyond what the kernels count in 32 bits
 size_t ln_grad_workspace_bytes(size_t elt, size_t rows, size_t dim);
@@ -192,6 +193,7 @@ struct EmbedGrad {
     const void *dy;
     void *dtable, *dpositions;  // [vocab, dim]; [positions, dim] or null
     void *workspace;
+    size_t workspace_bytes;
 };
 size_t embed_grad_workspace_bytes(size_t tokens, size_t length, size_t vocab, size_t positions, size_t dim);
 template <typename T>
@@ -213,13 +215,14 @@ struct AttnProblem {
 size_t attn_workspace_bytes(const AttnProblem &p);
 template <typename T>
 int attn_dispatch(const AttnProblem &p, const AttnView &q, const AttnView &k, const AttnView &v, const AttnView &out, float *lse,
-                  void *rest, void *workspace, hipStream_t stream);
+                  void *rest, void *workspace, size_t workspace_bytes, hipStream_t stream);
 struct AttnGradViews {
     AttnView q, k, v, out, dout, dq, dk, dv;
 };
 size_t attn_grad_workspace_bytes(const AttnProblem &p);
 template <typename T>
-int attn_grad_dispatch(const AttnProblem &p, const AttnGradViews &g, const float *lse, const void *rest, void *workspace, hipStream_t stream);
+int attn_grad_dispatch(const AttnProblem &p, const AttnGradViews &g, const float *lse, const void *rest, void *workspace, size_t workspace_bytes,
+                       hipStream_t stream);
 template <typename T>
 int add_dispatch(const void *a, const void *b, void *c, size_t n, size_t chunk_size,
                  hipStream_t stream);  // chunk_size 0: elementwise; else b holds one value per chunk

@@ -92,21 +92,14 @@ __device__ __forceinline__ void positions_parts(const Side &w, uint32_t block) {
     float sum[N];
 #pragma unroll
     for (int e = 0; e < N; e++) sum[e] = 0.0f;
-    uint32_t b = run * each;
-    for (; b + 8 <= stop; b += 8) {
+    for (uint32_t b = run * each; b < stop; b += 8) {
         float f[8][N];
 #pragma unroll
-        for (uint32_t u = 0; u < 8; u++) load_piece<T, N>(dy + (b + u) * step, f[u]);
+        for (uint32_t u = 0; u < 8; u++) load_piece<T, N>(dy + min(b + u, stop - 1) * step, f[u]);
 #pragma unroll
         for (uint32_t u = 0; u < 8; u++)
 #pragma unroll
-            for (int e = 0; e < N; e++) sum[e] += f[u][e];
-    }
-    for (; b < stop; b++) {
-        float f[N];
-        load_piece<T, N>(dy + b * step, f);
-#pragma unroll
-        for (int e = 0; e < N; e++) sum[e] += f[e];
+            for (int e = 0; e < N; e++) sum[e] += b + u < stop ? f[u][e] : 0.0f;
     }
     float *const out = w.position_parts + ((size_t)run * count + i) * N;
 #pragma unroll
@@ -476,11 +469,20 @@ __global__ __launch_bounds__(kSortThreads) void embed_grad_join_kernel(const Ent
 #pragma unroll
         for (uint32_t c = 0; c < 4; c++) sum[c] = 0.0f;
         if (wave == 0) add((size_t)slab * 2 + 1);
-        uint32_t i = wave * each;
-        for (; i + 8 <= stop; i += 8)
+        for (uint32_t i = wave * each; i < stop; i += 16) {
+            float f[16][4];
 #pragma unroll
-            for (uint32_t u = 0; u < 8; u++) add(((size_t)slab + 1 + i + u) * 2);
-        for (; i < stop; i++) add(((size_t)slab + 1 + i) * 2);
+            for (uint32_t u = 0; u < 16; u++)
+#pragma unroll
+                for (uint32_t c = 0; c < 4; c++) {
+                    const uint32_t col = col0 + c * kWave + lane;
+                    f[u][c] = i + u < stop && col < dim ? parts[((size_t)slab + 1 + i + u) * 2 * dim + col] : 0.0f;
+                }
+#pragma unroll
+            for (uint32_t u = 0; u < 16; u++)
+#pragma unroll
+                for (uint32_t c = 0; c < 4; c++) sum[c] += f[u][c];
+        }
 #pragma unroll
         for (uint32_t c = 0; c < 4; c++) lds[wave][c * kWave + lane] = sum[c];
         __syncthreads();
@@ -621,7 +623,8 @@ template <typename T>
 int embed_grad_dispatch(const EmbedGrad &g, size_t tokens, size_t length, size_t vocab, size_t positions, size_t dim, float scale,
                         hipStream_t stream) {
     constexpr int V = Store<T>::EPV;
-    const Layout l = layout(tokens, length, vocab, positions, dim);
+    Layout l = layout(tokens, length, vocab, positions, dim);
+    if (l.runs != 0) l.runs = (uint32_t)std::min<size_t>(l.runs, (g.workspace_bytes - l.position_parts) / (length * dim * sizeof(float)));
     char *const base = static_cast<char *>(g.workspace);
     Entry *const entries[2] = {reinterpret_cast<Entry *>(base + l.entries[0]), reinterpret_cast<Entry *>(base + l.entries[1])};
     uint32_t *const table = reinterpret_cast<uint32_t *>(base + l.table);

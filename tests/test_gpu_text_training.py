@@ -248,3 +248,23 @@ def test_float16_gradients_keep_their_digits_at_any_size(msd, cuda, size):
     kept = msd.attention_kept(d[0], d[1], d[2], False, 0.125, _offsets([200], cuda))[1]
     for g, w in zip(msd.attention_backward(d[3], kept), want[1:]):
         plain.check(g, w)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("causal,lengths", [(False, [(2100, 77)]), (True, [(900, 900)]), (False, [(1500, 20), (0, 5), (3, 0), (700, 130)])])
+def test_gradients_of_keys_that_many_rows_see(msd, cuda, dtype, causal, lengths):
+    """Few keys, many rows: the rows are cut into parts that are added afterwards."""
+    q, k, v, dout = _pack(lengths, 4, 2, 48, DTYPES[dtype])
+    want = plain.attention(q, k, v, causal, 0.2, dout, lengths)
+    offsets, offsets_k = _offsets([a for a, _ in lengths], cuda), _offsets([b for _, b in lengths], cuda)
+    d = [x.to(cuda) for x in (q, k, v, dout)]
+    kept = msd.attention_kept(d[0], d[1], d[2], causal, 0.2, offsets, offsets_k)[1]
+    grads = msd.attention_backward(d[3], kept)
+    for g, w, what in zip(grads, want[1:], ("dq", "dk", "dv")):
+        plain.check(g, w, what)
+    if len(lengths) == 1:  # the same as a dense batch of one
+        dense = [x[None] for x in d]
+        kept = msd.attention_kept(dense[0], dense[1], dense[2], causal, 0.2)[1]
+        for g, w in zip(msd.attention_backward(dense[3], kept), grads):
+            plain.check(g[0], (w.cpu().double(), 2 * want[1:][[x is w for x in grads].index(True)][1]))
