@@ -113,6 +113,19 @@ struct DsScale {
 template <typename T>
 constexpr int kPShift = Frag<T>::kFloat ? 0 : 15;
 
+// Whether a sequence's float16 score gradients go into their products in two parts, the rounded value and what it left.  The
+// roundings of one part are as large as that of the result itself, 1.41 times it together, where many terms make a sum;
+// of few terms, or of few columns (dS sums to zero over the keys, and what is left of such sums is smaller), they come to 1.7 times
+// and more.  Longer sequences have the second part in the tiles that the mask cuts alone: 9 products for 7 take 1.2 times as long.
+__device__ __forceinline__ bool few_terms(uint32_t lq, uint32_t lk, uint32_t dim) { return min(lq, lk) < 512 || dim <= 48; }
+
+// The part of registers 8 u ... 8 u + 7 that their rounding to `f` left.
+__device__ __forceinline__ void left_by(const half8 &f, int u, f32x16 &c) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) c[8 * u + j] -= (float)f[j];
+}
+[[maybe_unused]] __device__ __forceinline__ void left_by(const f32x8 &, int, f32x16 &) {}
+
 // Stores an accumulator's columns: row `to` gets the lane's column times `by`.
 template <typename T, int D>
 __device__ __forceinline__ void store_rows(T *to, const f32x16 (&acc)[D / 32], float by, uint32_t dim, bool vec) {
@@ -200,6 +213,7 @@ __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_gr
             tiles[buffer][1].copy([&](uint32_t r) -> const T * { return r < n ? vt + r * a.v.row : nullptr; }, a.s.dim);
         }
     };
+    const bool few = kHalf && few_terms(lq, lk, a.s.dim);
     f32x16 dq[DB];
 #pragma unroll
     for (int d = 0; d < DB; d++) dq[d] = zero16();
@@ -252,12 +266,15 @@ __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_gr
                             if (first + 32 * n + 8 * (r / 4) + 4 * h + r % 4 >= limit) s[r] = 0.0f;
                     }
 #pragma unroll
-                    for (int u = 0; u < 2; u++) {
+                    for (int u = 0; u < (MASKED && kHalf ? 4 : 2); u++) {
                         frag ds;
-                        to_frag(s, u, ds);
+                        to_frag(s, u % 2, ds);
+                        if constexpr (MASKED && kHalf) {  // (a second time with what the rounding took away)
+                            if (u < 2) left_by(ds, u, s);
+                        }
                         frag k[DB];
 #pragma unroll
-                        for (int d = 0; d < DB; d++) k[d] = kt.columns(lanes, 32 * n + 16 * u, d);
+                        for (int d = 0; d < DB; d++) k[d] = kt.columns(lanes, 32 * n + 16 * (u % 2), d);
                         if constexpr (MASKED) leave_out_odd<DB>(k, odd);
 #pragma unroll
                         for (int d = 0; d < DB; d++) dq[d] = mma(k[d], ds, dq[d]);
@@ -266,7 +283,7 @@ __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_gr
                 }
                 if (MASKED && odd) add_odd<T, D, R>(kt, lanes, dq, [&](uint32_t r) { return first + r < limit; });
             };
-            if (first + R > wave_full)
+            if (first + R > wave_full || few)
                 work(std::true_type{});
             else
                 work(std::false_type{});
@@ -395,6 +412,7 @@ __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_gr
             for (int i = 0; i < 3; i++) stats[buffer][i][threadIdx.x] = next_stat[i];
         }
     };
+    const bool few = kHalf && few_terms(lq, lk, a.s.dim);
     f32x16 dk[DB], dv[DB];
 #pragma unroll
     for (int d = 0; d < DB; d++) dk[d] = dv[d] = zero16();
@@ -468,6 +486,7 @@ __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_gr
                         if constexpr (MASKED) {
                             keep_here(p[u]);
                             keep_here(ds[u]);
+                            if constexpr (kHalf) left_by(ds[u], u, dp);
                         }
                     }
 #pragma unroll
@@ -484,6 +503,19 @@ __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_gr
                             step_end<Frag<T>::kFloat || D == 128>();
                         }
                     }
+                    if constexpr (MASKED && kHalf) {  // (a second time with what the rounding took away)
+#pragma unroll
+                        for (int u = 0; u < 2; u++) {
+                            to_frag(dp, u, ds[u]);
+#pragma unroll
+                            for (int d = 0; d < DB; d++) {
+                                frag qc[1] = {qt.columns(lanes, 32 * n + 16 * u, d)};
+                                leave_out_odd<1>(qc, odd);
+                                dk[d] = mma(qc[0], ds[u], dk[d]);
+                                step_end<D == 128>();
+                            }
+                        }
+                    }
                 }
                 if (MASKED && odd) {
                     auto visible = [&](uint32_t r) { return first + r >= from; };
@@ -491,7 +523,7 @@ __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_gr
                     add_odd<T, D, R>(qt, lanes, dk, visible);
                 }
             };
-            if (first < wave_full)
+            if (first < wave_full || few)
                 work(std::true_type{});
             else
                 work(std::false_type{});
@@ -559,7 +591,7 @@ uint32_t row_parts(const AttnProblem &p) {
     const size_t blocks = std::max<size_t>(1, tiles_of(p.k_offsets, p.batch, p.k_rows, 1) * p.kv_heads), once = 2 * (size_t)chip_info().cus;
     const size_t rows = (p.q_offsets != nullptr ? p.q_rows / std::max<size_t>(1, p.batch) : p.q_rows) * (p.heads / p.kv_heads);
     size_t parts = p.causal && blocks <= 4 * once ? 2 : 1;
-    if (blocks * parts < once) parts = (once + blocks - 1) / blocks;
+    parts = std::max(parts, once / blocks);
     return (uint32_t)std::max<size_t>(1, std::min<size_t>(parts, rows / 256));
 }
 
