@@ -29,10 +29,11 @@ constexpr float kLag = 8.0f;
 template <typename T>
 constexpr float kShift = Frag<T>::kFloat ? 0.0f : 7.0f;
 
-template <typename T, int D>
-__global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_kernel(const Forward a) {
+template <typename T, int D, int WAVES>
+__global__ __launch_bounds__(WAVES *kWave, Frag<T>::kFloat || WAVES == 1 ? 1 : 2) void attn_kernel(const Forward a) {
     typedef typename Frag<T>::type frag;
-    typedef Tile<T, D> KvTile;
+    typedef Tile<T, D, WAVES> KvTile;
+    constexpr uint32_t kOwn = 32 * WAVES;
     constexpr int R = KvTile::kRows, KD = D / 16, DB = D / 32;
     __shared__ KvTile tiles[2][2];  // [buffer][K, V]
     const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, h = lane / 32;
@@ -40,15 +41,15 @@ __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_ke
     const uint32_t head = blockIdx.x % a.s.kv_heads, rest = blockIdx.x / a.s.kv_heads;
     const uint32_t part = rest % a.parts;
     uint32_t b, tile, q0, lq, k0, lk;
-    if (!find_tile(a.s.q_offsets, a.s.batch, a.s.q_rows, a.s.group, kAttnRows, rest / a.parts, a.s.q_by_tile, b, tile)) return;
+    if (!find_tile(a.s.q_offsets, a.s.batch, a.s.q_rows, a.s.group, kOwn, rest / a.parts, a.s.q_by_tile, b, tile)) return;
     span(a.s.q_offsets, b, a.s.q_rows, q0, lq);
     span(a.s.k_offsets, b, a.s.k_rows, k0, lk);
     const uint32_t rows = lq * a.s.group;
-    if (a.s.causal) tile = (rows + kAttnRows - 1) / kAttnRows - 1 - tile;  // (those that see most keys first)
+    if (a.s.causal) tile = (rows + kOwn - 1) / kOwn - 1 - tile;  // (those that see most keys first)
 
     const bool packed_q = a.s.q_offsets != nullptr, packed_k = a.s.k_offsets != nullptr;
     // the lane's row: query i of head `qh`; it sees the keys [0, limit)
-    const uint32_t row = tile * kAttnRows + wave * 32 + lane % 32;
+    const uint32_t row = tile * kOwn + wave * 32 + lane % 32;
     const uint32_t i = row / a.s.group, qh = head * a.s.group + row % a.s.group;
     const bool live = row < rows;
     auto seen_by = [&](uint32_t query) -> uint32_t {
@@ -62,26 +63,25 @@ __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_ke
     load_frags<T, D>(live ? qrow : nullptr, a.s.dim, a.vec, q);
 
     // tiles of keys: what the workgroup's last row sees, this part's share of it
-    const uint32_t last_row = min(rows, (tile + 1) * kAttnRows) - 1;
+    const uint32_t last_row = min(rows, (tile + 1) * kOwn) - 1;
     const uint32_t all = (seen_by(last_row / a.s.group) + R - 1) / R, each = (all + a.parts - 1) / a.parts;
     const uint32_t t0 = min(all, part * each), t1 = min(all, t0 + each);
-    const uint32_t wave_row = tile * kAttnRows + wave * 32;
+    const uint32_t wave_row = tile * kOwn + wave * 32;
     const uint32_t wave_limit = wave_row < rows ? seen_by(min(rows - 1, wave_row + 31) / a.s.group) : 0;  // the most any row sees
     const uint32_t wave_full = wave_row < rows ? seen_by(wave_row / a.s.group) : 0;                       // what every row sees
 
-    uint32_t k_offset[KvTile::kPerThread], v_offset[KvTile::kPerThread];
-#pragma unroll
-    for (int p = 0; p < KvTile::kPerThread; p++) {
-        const uint32_t r = KvTile::row_of(p), d = KvTile::column_of(p);
-        k_offset[p] = d < a.s.dim ? (uint32_t)((r * a.k.row + d) * sizeof(T)) : kNowhere;
-        v_offset[p] = d < a.s.dim ? (uint32_t)((r * a.v.row + d) * sizeof(T)) : kNowhere;
-    }
+    uint32_t k_base[KvTile::kTurn], v_base[KvTile::kTurn];
+    const uint32_t k_row = (uint32_t)a.k.row, v_row = (uint32_t)a.v.row;
+    KvTile::offsets(k_row, a.s.dim, k_base);
+    KvTile::offsets(v_row, a.s.dim, v_base);
     auto fetch = [&](uint32_t t, uint32_t buffer) {
         const T *const kt = kbase + (size_t)t * R * a.k.row, *const vt = vbase + (size_t)t * R * a.v.row;
         const uint32_t n = min(lk - t * R, (uint32_t)R);
         if (a.vec) {
-            tiles[buffer][0].request(kt, (uint32_t)(((n - 1) * a.k.row + a.s.dim) * sizeof(T)), k_offset);
-            tiles[buffer][1].request(vt, (uint32_t)(((n - 1) * a.v.row + a.s.dim) * sizeof(T)), v_offset);
+            tiles[buffer][0].request(kt, (uint32_t)(((n - 1) * a.k.row + a.s.dim) * sizeof(T)),
+                                     [&](int p) { return KvTile::offset_of(k_base, k_row, p); });
+            tiles[buffer][1].request(vt, (uint32_t)(((n - 1) * a.v.row + a.s.dim) * sizeof(T)),
+                                     [&](int p) { return KvTile::offset_of(v_base, v_row, p); });
         } else {
             tiles[buffer][0].copy([&](uint32_t r) -> const T * { return r < n ? kt + r * a.k.row : nullptr; }, a.s.dim);
             tiles[buffer][1].copy([&](uint32_t r) -> const T * { return r < n ? vt + r * a.v.row : nullptr; }, a.s.dim);
@@ -269,11 +269,26 @@ __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(const Forward a
     if (a.lse != nullptr && lane == 0) a.lse[at] = sum == 0.0f ? -__builtin_inff() : base + __builtin_amdgcn_logf(sum);
 }
 
+}  // namespace
+
+// Whether workgroups of one wavefront do, of up to 64 columns: all of them at once are one to a SIMD, or sequences are so short that
+// of four most would have no rows.
+bool attn_few(const AttnProblem &p, size_t rows, size_t times) {
+    if (p.dim > 64) return false;
+    const size_t all = (p.q_offsets == nullptr ? p.batch : 1) * rows * times, tiles = all / 32 + p.batch;
+    return tiles * p.kv_heads <= 4 * (size_t)chip_info().cus || all / std::max<size_t>(1, p.batch) <= 48;
+}
+
+namespace {
+
+bool attn_few_rows(const AttnProblem &p) { return attn_few(p, p.q_rows, p.heads / p.kv_heads); }
+
 // Tiles of rows: the sequences' own where they are equal, at most this many where only their sum is known here.
 size_t row_tiles(const AttnProblem &p) {
     const size_t group = p.heads / p.kv_heads;
-    if (p.q_offsets == nullptr) return p.batch * ((p.q_rows * group + kAttnRows - 1) / kAttnRows);
-    return p.q_rows * group / kAttnRows + p.batch;
+    const size_t own = attn_rows(attn_few_rows(p));
+    if (p.q_offsets == nullptr) return p.batch * ((p.q_rows * group + own - 1) / own);
+    return p.q_rows * group / own + p.batch;
 }
 
 // Parts of the keys: workgroups for eight rounds of the chip where the sequences' lengths may differ, for two otherwise, with at
@@ -297,7 +312,7 @@ size_t attn_workspace_bytes(const AttnProblem &p) {
 
 AttnShape attn_shape(const AttnProblem &p) {
     const size_t few = 8 * (size_t)chip_info().cus;
-    const size_t k_blocks = p.batch * ((p.k_rows + kAttnRows - 1) / kAttnRows) * p.kv_heads;
+    const size_t own = attn_rows(attn_few(p, p.k_rows, 1)), k_blocks = p.batch * ((p.k_rows + own - 1) / own) * p.kv_heads;
     return AttnShape{p.q_offsets, p.k_offsets, (uint32_t)p.batch, (uint32_t)p.q_rows, (uint32_t)p.k_rows, (uint32_t)p.heads,
                      (uint32_t)p.kv_heads, (uint32_t)(p.heads / p.kv_heads), (uint32_t)p.dim, p.scale * kLog2e, p.causal,
                      p.causal && row_tiles(p) * p.kv_heads <= few, p.causal && k_blocks <= few};
@@ -324,10 +339,12 @@ int attn_dispatch(const AttnProblem &p, const AttnView &q, const AttnView &k, co
         a.part_lse = a.part + (size_t)a.parts * a.total_rows * p.heads * p.dim;
     }
     const dim3 grid((uint32_t)(tiles * a.parts * p.kv_heads));
-    if (p.dim <= 64)
-        launch((attn_kernel<T, 64>), grid, dim3(kAttnThreads), 0, stream, a);
+    if (attn_few_rows(p))
+        launch((attn_kernel<T, 64, 1>), grid, dim3(kWave), 0, stream, a);
+    else if (p.dim <= 64)
+        launch((attn_kernel<T, 64, kAttnWaves>), grid, dim3(kAttnThreads), 0, stream, a);
     else
-        launch((attn_kernel<T, 128>), grid, dim3(kAttnThreads), 0, stream, a);
+        launch((attn_kernel<T, 128, kAttnWaves>), grid, dim3(kAttnThreads), 0, stream, a);
     if (a.parts > 1)
         launch((attn_join_kernel<T>), dim3((uint32_t)((total_rows(p) * p.heads + kAttnWaves - 1) / kAttnWaves)), dim3(kAttnThreads), 0,
                stream, a);

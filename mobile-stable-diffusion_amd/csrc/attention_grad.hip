@@ -149,10 +149,11 @@ __device__ __forceinline__ void store_rows(T *to, const f32x16 (&acc)[D / 32], f
 }
 
 // dq: the forward kernel's tiles of rows over tiles of keys.
-template <typename T, int D>
-__global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_grad_q_kernel(const Backward a) {
+template <typename T, int D, int WAVES>
+__global__ __launch_bounds__(WAVES *kWave, Frag<T>::kFloat || WAVES == 1 ? 1 : 2) void attn_grad_q_kernel(const Backward a) {
     typedef typename Frag<T>::type frag;
-    typedef Tile<T, D> KvTile;
+    typedef Tile<T, D, WAVES> KvTile;
+    constexpr uint32_t kOwn = 32 * WAVES;
     constexpr bool kHalf = !Frag<T>::kFloat;
     constexpr int R = KvTile::kRows, KD = D / 16, DB = D / 32;
     __shared__ KvTile tiles[2][2];
@@ -160,13 +161,13 @@ __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_gr
     const TileLanes<T, D> lanes;
     const uint32_t head = blockIdx.x % a.s.kv_heads;
     uint32_t b, tile, q0, lq, k0, lk;
-    if (!find_tile(a.s.q_offsets, a.s.batch, a.s.q_rows, a.s.group, kAttnRows, blockIdx.x / a.s.kv_heads, a.s.q_by_tile, b, tile)) return;
+    if (!find_tile(a.s.q_offsets, a.s.batch, a.s.q_rows, a.s.group, kOwn, blockIdx.x / a.s.kv_heads, a.s.q_by_tile, b, tile)) return;
     span(a.s.q_offsets, b, a.s.q_rows, q0, lq);
     span(a.s.k_offsets, b, a.s.k_rows, k0, lk);
     const uint32_t rows = lq * a.s.group;
-    if (a.s.causal) tile = (rows + kAttnRows - 1) / kAttnRows - 1 - tile;
+    if (a.s.causal) tile = (rows + kOwn - 1) / kOwn - 1 - tile;
     const bool packed = a.s.q_offsets != nullptr;
-    const uint32_t row = tile * kAttnRows + wave * 32 + lane % 32;
+    const uint32_t row = tile * kOwn + wave * 32 + lane % 32;
     const uint32_t i = row / a.s.group, qh = head * a.s.group + row % a.s.group;
     const bool live = row < rows;
     auto seen_by = [&](uint32_t query) -> uint32_t {
@@ -187,27 +188,26 @@ __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_gr
     const float norm = kHalf && live ? a.norm[place] : 0.0f;
     const float *const v_norm = kHalf ? a.v_norm + ((size_t)(packed ? 0 : b) * lk + k0) * a.s.kv_heads + head : nullptr;
 
-    const uint32_t last_row = min(rows, (tile + 1) * kAttnRows) - 1;
+    const uint32_t last_row = min(rows, (tile + 1) * kOwn) - 1;
     const uint32_t t1 = (seen_by(last_row / a.s.group) + R - 1) / R;
-    const uint32_t wave_row = tile * kAttnRows + wave * 32;
+    const uint32_t wave_row = tile * kOwn + wave * 32;
     const uint32_t wave_limit = wave_row < rows ? seen_by(min(rows - 1, wave_row + 31) / a.s.group) : 0;
     const uint32_t wave_full = wave_row < rows ? seen_by(wave_row / a.s.group) : 0;
 
-    uint32_t k_offset[KvTile::kPerThread], v_offset[KvTile::kPerThread];
-#pragma unroll
-    for (int p = 0; p < KvTile::kPerThread; p++) {
-        const uint32_t r = KvTile::row_of(p), d = KvTile::column_of(p);
-        k_offset[p] = d < a.s.dim ? (uint32_t)((r * a.k.row + d) * sizeof(T)) : kNowhere;
-        v_offset[p] = d < a.s.dim ? (uint32_t)((r * a.v.row + d) * sizeof(T)) : kNowhere;
-    }
+    uint32_t k_base[KvTile::kTurn], v_base[KvTile::kTurn];
+    const uint32_t k_row = (uint32_t)a.k.row, v_row = (uint32_t)a.v.row;
+    KvTile::offsets(k_row, a.s.dim, k_base);
+    KvTile::offsets(v_row, a.s.dim, v_base);
     float next_norm = 0.0f;
     auto fetch = [&](uint32_t t, uint32_t buffer) {
         if (kHalf) next_norm = t * R + lane < lk ? v_norm[(size_t)(t * R + lane) * a.s.kv_heads] : 0.0f;
         const T *const kt = kbase + (size_t)t * R * a.k.row, *const vt = vbase + (size_t)t * R * a.v.row;
         const uint32_t n = min(lk - t * R, (uint32_t)R);
         if (a.vec) {
-            tiles[buffer][0].request(kt, (uint32_t)(((n - 1) * a.k.row + a.s.dim) * sizeof(T)), k_offset);
-            tiles[buffer][1].request(vt, (uint32_t)(((n - 1) * a.v.row + a.s.dim) * sizeof(T)), v_offset);
+            tiles[buffer][0].request(kt, (uint32_t)(((n - 1) * a.k.row + a.s.dim) * sizeof(T)),
+                                     [&](int p) { return KvTile::offset_of(k_base, k_row, p); });
+            tiles[buffer][1].request(vt, (uint32_t)(((n - 1) * a.v.row + a.s.dim) * sizeof(T)),
+                                     [&](int p) { return KvTile::offset_of(v_base, v_row, p); });
         } else {
             tiles[buffer][0].copy([&](uint32_t r) -> const T * { return r < n ? kt + r * a.k.row : nullptr; }, a.s.dim);
             tiles[buffer][1].copy([&](uint32_t r) -> const T * { return r < n ? vt + r * a.v.row : nullptr; }, a.s.dim);
@@ -295,36 +295,37 @@ __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_gr
     store_rows<T, D>(to, dq, kHalf ? ldexpf(natural, -scale.power) : natural, a.s.dim, a.vec);
 }
 
-template <typename T, int D, bool IN_LDS>
+template <typename T, int D, int WAVES, bool IN_LDS>
 struct KeptValues {
-    typedef Tile<T, D, (int)kAttnRows> type;
+    typedef Tile<T, D, WAVES, 32 * WAVES> type;
 };
-template <typename T, int D>
-struct KeptValues<T, D, false> {
+template <typename T, int D, int WAVES>
+struct KeptValues<T, D, WAVES, false> {
     struct type {};
 };
 
 // dk and dv: a wavefront owns 32 keys as the columns of S = Q K^T; the rows that see them pass by.
-template <typename T, int D>
-__global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_grad_kv_kernel(const Backward a) {
+template <typename T, int D, int WAVES>
+__global__ __launch_bounds__(WAVES *kWave, Frag<T>::kFloat || WAVES == 1 ? 1 : 2) void attn_grad_kv_kernel(const Backward a) {
     typedef typename Frag<T>::type frag;
-    typedef Tile<T, D, D == 128 ? 32 : Frag<T>::kTile> RowTile;  // (64 rows of 128 columns on their way leave too few registers)
+    constexpr uint32_t kOwn = 32 * WAVES;
+    typedef Tile<T, D, WAVES, D == 128 ? 32 : Frag<T>::kTile> RowTile;  // (64 rows of 128 columns on their way leave too few registers)
     constexpr bool kHalf = !Frag<T>::kFloat;
     constexpr int R = RowTile::kRows, KD = D / 16, DB = D / 32;
     __shared__ RowTile tiles[2][2];                // [buffer][Q, dO]
     constexpr bool kVInLds = kHalf && D == 128;
-    __shared__ typename KeptValues<T, D, kVInLds>::type values;
+    __shared__ typename KeptValues<T, D, WAVES, kVInLds>::type values;
     __shared__ __align__(16) float stats[2][3][R]; // [buffer][- log2 sum, D, |do|]
     const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, h = lane / 32;
     const TileLanes<T, D> lanes;
     const uint32_t head = blockIdx.x % a.s.kv_heads;
     uint32_t b, tile, q0, lq, k0, lk;
-    if (!find_tile(a.s.k_offsets, a.s.batch, a.s.k_rows, 1, kAttnRows, blockIdx.x / a.s.kv_heads / a.parts, a.s.k_by_tile, b, tile)) return;
+    if (!find_tile(a.s.k_offsets, a.s.batch, a.s.k_rows, 1, kOwn, blockIdx.x / a.s.kv_heads / a.parts, a.s.k_by_tile, b, tile)) return;
     const uint32_t part = blockIdx.x / a.s.kv_heads % a.parts;
     span(a.s.q_offsets, b, a.s.q_rows, q0, lq);
     span(a.s.k_offsets, b, a.s.k_rows, k0, lk);
     const bool packed = a.s.q_offsets != nullptr;
-    const uint32_t rows = lq * a.s.group, key = tile * kAttnRows + wave * 32 + lane % 32;
+    const uint32_t rows = lq * a.s.group, key = tile * kOwn + wave * 32 + lane % 32;
     const bool live = key < lk;
     // the first row that sees a key
     auto first_row = [&](uint32_t j) -> uint32_t {
@@ -339,15 +340,14 @@ __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_gr
     frag k[KD], v[kVInLds ? 1 : KD];
     load_frags<T, D>(live ? kbase : nullptr, a.s.dim, a.vec, k);
     if constexpr (kVInLds) {
-        typedef typename KeptValues<T, D, true>::type Values;
-        const uint32_t key0 = tile * kAttnRows, n = min(lk - key0, kAttnRows);
+        typedef typename KeptValues<T, D, WAVES, true>::type Values;
+        const uint32_t key0 = tile * kOwn, n = min(lk - key0, kOwn);
         const T *const from = static_cast<const T *>(a.v.at) + (packed ? 0 : b * a.v.batch) + (size_t)(k0 + key0) * a.v.row + head * a.v.head;
         if (a.vec) {
-            uint32_t offset[Values::kPerThread];
-#pragma unroll
-            for (int p = 0; p < Values::kPerThread; p++)
-                offset[p] = Values::column_of(p) < a.s.dim ? (uint32_t)((Values::row_of(p) * a.v.row + Values::column_of(p)) * sizeof(T)) : kNowhere;
-            values.request(from, (uint32_t)(((n - 1) * a.v.row + a.s.dim) * sizeof(T)), offset);
+            uint32_t base[Values::kTurn];
+            Values::offsets((uint32_t)a.v.row, a.s.dim, base);
+            values.request(from, (uint32_t)(((n - 1) * a.v.row + a.s.dim) * sizeof(T)),
+                           [&](int p) { return Values::offset_of(base, (uint32_t)a.v.row, p); });
         } else {
             values.copy([&](uint32_t r) -> const T * { return r < n ? from + r * a.v.row : nullptr; }, a.s.dim);
         }
@@ -362,11 +362,11 @@ __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_gr
     };
     const float v_norm = kHalf && live ? a.v_norm[(((size_t)(packed ? 0 : b) * lk + k0) + key) * a.s.kv_heads + head] : 0.0f;
 
-    const uint32_t wave_key = tile * kAttnRows + wave * 32;
+    const uint32_t wave_key = tile * kOwn + wave * 32;
     const uint32_t from = live ? first_row(key) : rows;                                  // the lane's rows: [from, rows)
     const uint32_t wave_from = wave_key < lk ? first_row(wave_key) : rows;               // the first any key is seen by
     const uint32_t wave_full = wave_key < lk ? first_row(min(lk - 1, wave_key + 31)) : rows; // from here on all are
-    const uint32_t from_tile = min(first_row(tile * kAttnRows), rows) / R, all = (rows + R - 1) / R - from_tile;
+    const uint32_t from_tile = min(first_row(tile * kOwn), rows) / R, all = (rows + R - 1) / R - from_tile;
     const uint32_t each = (all + a.parts - 1) / a.parts, t0 = from_tile + min(all, part * each), t1 = min(from_tile + all, t0 + each);
 
     float next_stat[3] = {0.0f, 0.0f, 0.0f};
@@ -384,8 +384,8 @@ __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_gr
                 g_offset[p] = in ? (uint32_t)(((i - i0) * a.dout.row + gh * a.dout.head + d) * sizeof(T)) : kNowhere;
             }
             const uint32_t heads = a.s.group - 1;
-            tiles[buffer][0].request(q, (uint32_t)((n * a.q.row + heads * a.q.head + a.s.dim) * sizeof(T)), q_offset);
-            tiles[buffer][1].request(g, (uint32_t)((n * a.dout.row + heads * a.dout.head + a.s.dim) * sizeof(T)), g_offset);
+            tiles[buffer][0].request(q, (uint32_t)((n * a.q.row + heads * a.q.head + a.s.dim) * sizeof(T)), [&](int p) { return q_offset[p]; });
+            tiles[buffer][1].request(g, (uint32_t)((n * a.dout.row + heads * a.dout.head + a.s.dim) * sizeof(T)), [&](int p) { return g_offset[p]; });
         } else {
             auto from = [&](const T *base, const AttnView &v) {
                 return [=](uint32_t r) -> const T * {
@@ -532,7 +532,7 @@ __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_gr
     }
     uint32_t thread = threadIdx.x;  // (the key's number is formed again: over the loop there is no register for it)
     asm volatile("" : "+v"(thread));
-    const uint32_t own_key = tile * kAttnRows + thread / kWave * 32 + thread % 32;
+    const uint32_t own_key = tile * kOwn + thread / kWave * 32 + thread % 32;
     if (own_key >= lk) return;
     auto out = [&](const AttnView &to) {
         return static_cast<T *>(const_cast<void *>(to.at)) + (packed ? 0 : b * to.batch) + (size_t)(k0 + own_key) * to.row + head * to.head;
@@ -551,18 +551,19 @@ __global__ __launch_bounds__(kAttnThreads, Frag<T>::kFloat ? 1 : 2) void attn_gr
     store_rows<T, D>(out(a.dv), dv, by_v, a.s.dim, a.vec);
 }
 
-// dk and dv from the parts, for a tile of keys of a head, in the parts' order.
+// dk and dv from the parts, in their order, for a few keys of a head.
+constexpr uint32_t kJoinKeys = 8;
 template <typename T>
 __global__ __launch_bounds__(kAttnThreads) void attn_grad_join_kernel(const Backward a) {
     const uint32_t head = blockIdx.x % a.s.kv_heads;
     uint32_t b, tile, k0, lk;
-    if (!find_tile(a.s.k_offsets, a.s.batch, a.s.k_rows, 1, kAttnRows, blockIdx.x / a.s.kv_heads, false, b, tile)) return;
+    if (!find_tile(a.s.k_offsets, a.s.batch, a.s.k_rows, 1, kJoinKeys, blockIdx.x / a.s.kv_heads, false, b, tile)) return;
     span(a.s.k_offsets, b, a.s.k_rows, k0, lk);
     const bool packed = a.s.k_offsets != nullptr;
-    const uint32_t n = min(kAttnRows, lk - tile * kAttnRows), row = 2 * a.s.dim;
+    const uint32_t n = min(kJoinKeys, lk - tile * kJoinKeys), row = 2 * a.s.dim;
     const size_t step = (size_t)a.total_keys * a.s.kv_heads * row;
     for (uint32_t at = threadIdx.x; at < n * row; at += kAttnThreads) {
-        const uint32_t r = at / row, c = at - r * row, key = tile * kAttnRows + r;
+        const uint32_t r = at / row, c = at - r * row, key = tile * kJoinKeys + r;
         const float *from = a.part + (((size_t)(packed ? 0 : b) * lk + k0 + key) * a.s.kv_heads + head) * row + c;
         float sum = 0.0f;
         for (uint32_t p0 = 0; p0 < a.parts; p0 += 8) {
@@ -579,16 +580,19 @@ __global__ __launch_bounds__(kAttnThreads) void attn_grad_join_kernel(const Back
     }
 }
 
-size_t tiles_of(const int32_t *offsets, size_t batch, size_t rows, size_t times) {
-    if (offsets == nullptr) return batch * ((rows * times + kAttnRows - 1) / kAttnRows);
-    return rows * times / kAttnRows + batch;
+size_t tiles_of(const int32_t *offsets, size_t batch, size_t rows, size_t times, size_t own) {
+    if (offsets == nullptr) return batch * ((rows * times + own - 1) / own);
+    return rows * times / own + batch;
+}
+size_t tiles_of_keys(const AttnProblem &p) {
+    return tiles_of(p.k_offsets, p.batch, p.k_rows, 1, attn_rows(attn_few(p, p.k_rows, 1)));
 }
 
 // Parts of the rows for dk and dv.  Under a causal mask tiles of keys differ in the rows that see them: cut in two they fill up
 // a launch of few rounds.  Few keys and many rows (a prompt's keys, an image's rows) are cut until the chip is full, with
 // at least 256 rows in a part on average.
 uint32_t row_parts(const AttnProblem &p) {
-    const size_t blocks = std::max<size_t>(1, tiles_of(p.k_offsets, p.batch, p.k_rows, 1) * p.kv_heads), once = 2 * (size_t)chip_info().cus;
+    const size_t blocks = std::max<size_t>(1, tiles_of_keys(p) * p.kv_heads), once = 2 * (size_t)chip_info().cus;
     const size_t rows = (p.q_offsets != nullptr ? p.q_rows / std::max<size_t>(1, p.batch) : p.q_rows) * (p.heads / p.kv_heads);
     size_t parts = p.causal && blocks <= 4 * once ? 2 : 1;
     parts = std::max(parts, once / blocks);
@@ -621,16 +625,30 @@ int attn_grad_dispatch(const AttnProblem &p, const AttnGradViews &g, const float
     const size_t items = rows * p.heads + (kHalf ? keys * p.kv_heads : 0);
     if (items != 0)
         launch((attn_grad_rows_kernel<T>), dim3((uint32_t)((items + 15) / 16)), dim3(kAttnThreads), 0, stream, a);
-    const dim3 of_rows((uint32_t)(tiles_of(p.q_offsets, p.batch, p.q_rows, p.heads / p.kv_heads) * p.kv_heads));
-    const dim3 key_tiles((uint32_t)(tiles_of(p.k_offsets, p.batch, p.k_rows, 1) * p.kv_heads)), of_keys(key_tiles.x * parts);
-    if (p.dim <= 64) {
-        if (of_keys.x != 0) launch((attn_grad_kv_kernel<T, 64>), of_keys, dim3(kAttnThreads), 0, stream, a);
-        if (of_rows.x != 0) launch((attn_grad_q_kernel<T, 64>), of_rows, dim3(kAttnThreads), 0, stream, a);
-    } else {
-        if (of_keys.x != 0) launch((attn_grad_kv_kernel<T, 128>), of_keys, dim3(kAttnThreads), 0, stream, a);
-        if (of_rows.x != 0) launch((attn_grad_q_kernel<T, 128>), of_rows, dim3(kAttnThreads), 0, stream, a);
+    const size_t group = p.heads / p.kv_heads;
+    const bool few_rows = attn_few(p, p.q_rows, group), few_keys = attn_few(p, p.k_rows, 1);
+    const dim3 of_rows((uint32_t)(tiles_of(p.q_offsets, p.batch, p.q_rows, group, attn_rows(few_rows)) * p.kv_heads));
+    const dim3 of_keys((uint32_t)(tiles_of_keys(p) * p.kv_heads * parts));
+    if (of_keys.x != 0) {
+        if (few_keys)
+            launch((attn_grad_kv_kernel<T, 64, 1>), of_keys, dim3(kWave), 0, stream, a);
+        else if (p.dim <= 64)
+            launch((attn_grad_kv_kernel<T, 64, kAttnWaves>), of_keys, dim3(kAttnThreads), 0, stream, a);
+        else
+            launch((attn_grad_kv_kernel<T, 128, kAttnWaves>), of_keys, dim3(kAttnThreads), 0, stream, a);
     }
-    if (parts > 1 && key_tiles.x != 0) launch((attn_grad_join_kernel<T>), key_tiles, dim3(kAttnThreads), 0, stream, a);
+    if (of_rows.x != 0) {
+        if (few_rows)
+            launch((attn_grad_q_kernel<T, 64, 1>), of_rows, dim3(kWave), 0, stream, a);
+        else if (p.dim <= 64)
+            launch((attn_grad_q_kernel<T, 64, kAttnWaves>), of_rows, dim3(kAttnThreads), 0, stream, a);
+        else
+            launch((attn_grad_q_kernel<T, 128, kAttnWaves>), of_rows, dim3(kAttnThreads), 0, stream, a);
+    }
+    if (parts > 1) {
+        const size_t joins = tiles_of(p.k_offsets, p.batch, p.k_rows, 1, kJoinKeys) * p.kv_heads;
+        launch((attn_grad_join_kernel<T>), dim3((uint32_t)joins), dim3(kAttnThreads), 0, stream, a);
+    }
     return launch_status();
 }
 

@@ -21,7 +21,8 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 
 constexpr uint32_t kAttnThreads = 256, kAttnWaves = kAttnThreads / kWave;
-constexpr uint32_t kAttnRows = 32 * kAttnWaves;  // rows that a workgroup owns, 32 to a wavefront
+// A workgroup has 1 or 4 wavefronts, each with 32 rows of its own; the tiles that pass by are everyone's.
+constexpr uint32_t attn_rows(bool few) { return few ? 32 : 32 * kAttnWaves; }
 
 template <typename T>
 struct Frag;
@@ -198,22 +199,34 @@ struct TileLanes {
 
 // A tile in LDS: ROWS rows of D values as 16-byte chunks, chunk c of row r at place c ^ (r & 7), so that lanes that read one
 // chunk of neighbouring rows, or neighbouring chunks of four rows, meet different banks.
-template <typename T, int D, int ROWS = Frag<T>::kTile>
+template <typename T, int D, int WAVES, int ROWS = Frag<T>::kTile>
 struct Tile {
-    static constexpr int kRows = ROWS, kChunks = D * (int)sizeof(T) / 16;
-    static constexpr int kPerThread = kRows * kChunks / (int)kAttnThreads;
+    static constexpr int kThreads = WAVES * kWave, kRows = ROWS, kChunks = D * (int)sizeof(T) / 16;
+    static constexpr int kPerThread = kRows * kChunks / kThreads;
+    // places of a thread that lie kTurn apart are kTurn * kStep rows apart, in the same column
+    static constexpr int kStep = kThreads / kChunks, kTurn = kStep >= 8 ? 1 : 8 / kStep;
     typedef typename Frag<T>::type frag;
     u32x4 data[kRows * kChunks];
 
     // Row and column of the chunk that belongs at this thread's place number p.
-    static __device__ __forceinline__ uint32_t row_of(int p) { return (p * kAttnThreads + threadIdx.x) / kChunks; }
+    static __device__ __forceinline__ uint32_t row_of(int p) { return (p * kThreads + threadIdx.x) / kChunks; }
     static __device__ __forceinline__ uint32_t column_of(int p) {
-        return ((p * kAttnThreads + threadIdx.x) % kChunks ^ (row_of(p) & 7)) * (16 / (uint32_t)sizeof(T));
+        return ((p * kThreads + threadIdx.x) % kChunks ^ (row_of(p) & 7)) * (16 / (uint32_t)sizeof(T));
     }
-    // Asks for this thread's chunks, `offset[p]` bytes behind `from` (the same in the whole wavefront), straight from memory to
+    // Bytes from a tile's first row to this thread's first kTurn chunks, for rows of `row` elements; chunk p is at
+    // `offset_of(base, row, p)`.
+    static __device__ __forceinline__ void offsets(uint32_t row, uint32_t dim, uint32_t (&base)[kTurn]) {
+#pragma unroll
+        for (int p = 0; p < kTurn; p++) base[p] = column_of(p) < dim ? (row_of(p) * row + column_of(p)) * (uint32_t)sizeof(T) : kNowhere;
+    }
+    static __device__ __forceinline__ uint32_t offset_of(const uint32_t (&base)[kTurn], uint32_t row, int p) {
+        return base[p % kTurn] + p / kTurn * (kTurn * kStep * (uint32_t)sizeof(T)) * row;
+    }
+    // Asks for this thread's chunks, `offset(p)` bytes behind `from` (the same in the whole wavefront), straight from memory to
     // LDS; from byte `bytes` on there are zeros.  wait_tiles() and a barrier later they are there.  Written as assembly because
     // the compiler, which knows no more than that these write LDS, would wait for them in front of every read by columns.
-    __device__ __forceinline__ void request(const void *from, uint32_t bytes, const uint32_t (&offset)[kPerThread]) {
+    template <typename Offset>
+    __device__ __forceinline__ void request(const void *from, uint32_t bytes, Offset offset) {
         const uintptr_t at = reinterpret_cast<uintptr_t>(from);
         const u32x4 resource = {(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)at), (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(at >> 32)),
                                 (uint32_t)__builtin_amdgcn_readfirstlane(bytes), 0x00020000u};
@@ -225,7 +238,7 @@ struct Tile {
             uint32_t m0;  // (the compiler's own; a load takes it when it is issued)
             asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
                          : "=&s"(m0)
-                         : "s"(lds + p * kAttnThreads * 16), "v"(offset[p]), "s"(resource)
+                         : "s"(lds + p * kThreads * 16), "v"(offset(p)), "s"(resource)
                          : "memory");
         }
     }
@@ -235,7 +248,7 @@ struct Tile {
 #pragma unroll 1
         for (int p = 0; p < kPerThread; p++) {
             const T *const from = row(row_of(p));
-            data[p * kAttnThreads + threadIdx.x] = from != nullptr ? load_chunk<T>(from, column_of(p), dim, false) : u32x4{0, 0, 0, 0};
+            data[p * kThreads + threadIdx.x] = from != nullptr ? load_chunk<T>(from, column_of(p), dim, false) : u32x4{0, 0, 0, 0};
         }
     }
 
@@ -292,6 +305,7 @@ struct AttnShape {
 };
 
 AttnShape attn_shape(const AttnProblem &p);
+bool attn_few(const AttnProblem &p, size_t rows, size_t times);
 // Whether every row of the views is whole aligned 16-byte vectors, and a tile's reach fits 31 bits.
 bool attn_vectors(size_t elt, const AttnProblem &p, std::initializer_list<AttnView> views);
 

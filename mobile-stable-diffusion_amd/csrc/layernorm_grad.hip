@@ -46,6 +46,29 @@ __device__ __forceinline__ float row_sum(float v, float *slots) {
     }
 }
 
+// Three at once.
+template <int TL>
+__device__ __forceinline__ void row_sums(float &a, float &b, float &c, float *slots) {
+    a = team_sum<TL < (int)kThreads ? TL : kWave>(a);
+    b = team_sum<TL < (int)kThreads ? TL : kWave>(b);
+    c = team_sum<TL < (int)kThreads ? TL : kWave>(c);
+    if constexpr (TL == (int)kThreads) {
+        if (threadIdx.x % kWave == 0) {
+            slots[threadIdx.x / kWave] = a;
+            slots[kWaves + threadIdx.x / kWave] = b;
+            slots[2 * kWaves + threadIdx.x / kWave] = c;
+        }
+        __syncthreads();
+        a = b = c = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kWaves; i++) {
+            a += slots[i];
+            b += slots[kWaves + i];
+            c += slots[2 * kWaves + i];
+        }
+    }
+}
+
 // The rows of workgroup b: teams of it take rows b * teams + team, and so on by gridDim.x * teams.  Each keeps the next row's
 // loads in flight while it works on one.  partial: [gridDim.x][2][dim] or null (dgamma and dbeta not wanted).
 template <typename T, int N, int K, int TL>
@@ -126,8 +149,20 @@ __global__ __launch_bounds__(kThreads) void ln_grad_kernel(const T *dy, const T 
                 f[k][e] = in[k] ? f[k][e] - mean : 0.0f;
                 q = fmaf(f[k][e], f[k][e], q);
             }
-        const float rstd = __builtin_amdgcn_rsqf(row_sum<TL>(q, slots + kWaves) * inv_dim + eps);
         float m1 = 0.0f, m2 = 0.0f;
+#pragma unroll
+        for (int k = 0; k < K; k++)
+#pragma unroll
+            for (int e = 0; e < N; e++) {
+                const float w = d[k][e] * g[k][e];
+                m1 += w;
+                m2 = fmaf(w, f[k][e], m2);
+            }
+        // (three sums side by side: a row waits for two rounds of reductions in all)
+        row_sums<TL>(q, m1, m2, slots + kWaves);
+        const float rstd = __builtin_amdgcn_rsqf(q * inv_dim + eps);
+        m1 *= inv_dim;
+        m2 *= rstd * inv_dim;
 #pragma unroll
         for (int k = 0; k < K; k++)
 #pragma unroll
@@ -136,11 +171,7 @@ __global__ __launch_bounds__(kThreads) void ln_grad_kernel(const T *dy, const T 
                 sum_g[k][e] = fmaf(d[k][e], f[k][e], sum_g[k][e]);
                 sum_b[k][e] += d[k][e];
                 d[k][e] *= g[k][e];
-                m1 += d[k][e];
-                m2 = fmaf(d[k][e], f[k][e], m2);
             }
-        m1 = row_sum<TL>(m1, slots + 2 * kWaves) * inv_dim;
-        m2 = row_sum<TL>(m2, slots + 3 * kWaves) * inv_dim;
         if (row < rows) {
 #pragma unroll
             for (int k = 0; k < K; k++) {

@@ -323,7 +323,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(const int64_t 
 }
 
 // ---- sums ----------------------------------------------------------------------
-constexpr uint32_t kSlab = 16;  // sorted tokens of a wavefront
+constexpr uint32_t kSlab = 32;  // sorted tokens of a wavefront
 
 // First place in sorted[0, tokens) whose id is at least v; the whole wavefront looks, 64 places at a time.
 __device__ __forceinline__ uint32_t first_of(const Entry *sorted, uint32_t tokens, uint32_t v) {
@@ -401,7 +401,7 @@ __global__ __launch_bounds__(kThreads) void embed_grad_slabs_kernel(const T *dy,
     put(id, first, true);
 }
 
-constexpr uint32_t kJoinColumns = 4 * kWave;
+constexpr uint32_t kJoinLane = 2, kJoinColumns = kJoinLane * kWave;  // columns of a lane, of a workgroup
 constexpr uint32_t kJoinAlone = 16;  // slabs behind the first up to which a run is one wavefront's work
 
 // A workgroup for kSortWaves slabs and kJoinColumns columns, a wavefront looking at each slab: it adds the parts of a run that starts
@@ -426,10 +426,10 @@ __global__ __launch_bounds__(kSortThreads) void embed_grad_join_kernel(const Ent
     __shared__ uint32_t run_id[kSortWaves], run_slabs[kSortWaves];  // (slabs behind the first that a long run reaches; 0: none)
     const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     const uint32_t slab0 = blockIdx.x / columns * kSortWaves, col0 = blockIdx.x % columns * kJoinColumns;
-    float sum[4];
+    float sum[kJoinLane];
     auto add = [&](size_t part) {
 #pragma unroll
-        for (uint32_t c = 0; c < 4; c++) {
+        for (uint32_t c = 0; c < kJoinLane; c++) {
             const uint32_t col = col0 + c * kWave + lane;
             sum[c] += col < dim ? parts[part * dim + col] : 0.0f;
         }
@@ -450,12 +450,12 @@ __global__ __launch_bounds__(kSortThreads) void embed_grad_join_kernel(const Ent
         }
         if (more != 0 && !is_long) {  // most runs: the wavefront's own
 #pragma unroll
-            for (uint32_t c = 0; c < 4; c++) sum[c] = 0.0f;
+            for (uint32_t c = 0; c < kJoinLane; c++) sum[c] = 0.0f;
             add((size_t)slab * 2 + 1);
 #pragma unroll 4
             for (uint32_t i = 0; i < more; i++) add(((size_t)slab + 1 + i) * 2);
 #pragma unroll
-            for (uint32_t c = 0; c < 4; c++) {
+            for (uint32_t c = 0; c < kJoinLane; c++) {
                 const uint32_t col = col0 + c * kWave + lane;
                 if (col < dim) Store<T>::store1(dtable + (size_t)id * dim + col, sum[c] * scale);
             }
@@ -467,24 +467,24 @@ __global__ __launch_bounds__(kSortThreads) void embed_grad_join_kernel(const Ent
         if (slabs == 0) continue;
         const uint32_t each = (slabs + kSortWaves - 1) / kSortWaves, stop = min(slabs, (wave + 1) * each);
 #pragma unroll
-        for (uint32_t c = 0; c < 4; c++) sum[c] = 0.0f;
+        for (uint32_t c = 0; c < kJoinLane; c++) sum[c] = 0.0f;
         if (wave == 0) add((size_t)slab * 2 + 1);
         for (uint32_t i = wave * each; i < stop; i += 16) {
-            float f[16][4];
+            float f[16][kJoinLane];
 #pragma unroll
             for (uint32_t u = 0; u < 16; u++)
 #pragma unroll
-                for (uint32_t c = 0; c < 4; c++) {
+                for (uint32_t c = 0; c < kJoinLane; c++) {
                     const uint32_t col = col0 + c * kWave + lane;
                     f[u][c] = i + u < stop && col < dim ? parts[((size_t)slab + 1 + i + u) * 2 * dim + col] : 0.0f;
                 }
 #pragma unroll
             for (uint32_t u = 0; u < 16; u++)
 #pragma unroll
-                for (uint32_t c = 0; c < 4; c++) sum[c] += f[u][c];
+                for (uint32_t c = 0; c < kJoinLane; c++) sum[c] += f[u][c];
         }
 #pragma unroll
-        for (uint32_t c = 0; c < 4; c++) lds[wave][c * kWave + lane] = sum[c];
+        for (uint32_t c = 0; c < kJoinLane; c++) lds[wave][c * kWave + lane] = sum[c];
         __syncthreads();
         if (threadIdx.x < kJoinColumns && col0 + threadIdx.x < dim) {
             float total = 0.0f;
