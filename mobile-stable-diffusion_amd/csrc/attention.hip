@@ -32,6 +32,7 @@ constexpr float kShift = Frag<T>::kFloat ? 0.0f : 7.0f;
 template <typename T, int D, int WAVES>
 __global__ __launch_bounds__(WAVES *kWave, Frag<T>::kFloat || WAVES == 1 ? 1 : 2) void attn_kernel(const Forward a) {
     typedef typename Frag<T>::type frag;
+    typedef typename Frag<T>::operand operand_t;
     typedef Tile<T, D, WAVES> KvTile;
     constexpr uint32_t kOwn = 32 * WAVES;
     constexpr int R = KvTile::kRows, KD = D / 16, DB = D / 32;
@@ -59,7 +60,7 @@ __global__ __launch_bounds__(WAVES *kWave, Frag<T>::kFloat || WAVES == 1 ? 1 : 2
     const T *qrow = static_cast<const T *>(a.q.at) + (packed_q ? 0 : b * a.q.batch) + (size_t)(q0 + i) * a.q.row + qh * a.q.head;
     const T *kbase = static_cast<const T *>(a.k.at) + (packed_k ? 0 : b * a.k.batch) + (size_t)k0 * a.k.row + head * a.k.head;
     const T *vbase = static_cast<const T *>(a.v.at) + (packed_k ? 0 : b * a.v.batch) + (size_t)k0 * a.v.row + head * a.v.head;
-    frag q[KD];
+    operand_t q[KD];
     load_frags<T, D>(live ? qrow : nullptr, a.s.dim, a.vec, q);
 
     // tiles of keys: what the workgroup's last row sees, this part's share of it
@@ -145,7 +146,7 @@ __global__ __launch_bounds__(WAVES *kWave, Frag<T>::kFloat || WAVES == 1 ? 1 : 2
                 for (int n = 0; n < R / 32; n++)
 #pragma unroll
                     for (int u = 0; u < 2; u++) {
-                        frag p;
+                        operand_t p;
                         to_frag(s[n], u, p);
                         frag v[DB];
 #pragma unroll

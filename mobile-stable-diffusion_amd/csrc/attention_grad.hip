@@ -124,7 +124,7 @@ __device__ __forceinline__ void left_by(const half8 &f, int u, f32x16 &c) {
 #pragma unroll
     for (int j = 0; j < 8; j++) c[8 * u + j] -= (float)f[j];
 }
-[[maybe_unused]] __device__ __forceinline__ void left_by(const f32x8 &, int, f32x16 &) {}
+[[maybe_unused]] __device__ __forceinline__ void left_by(const Thirds &, int, f32x16 &) {}
 
 // Stores an accumulator's columns: row `to` gets the lane's column times `by`.
 template <typename T, int D>
@@ -152,6 +152,7 @@ __device__ __forceinline__ void store_rows(T *to, const f32x16 (&acc)[D / 32], f
 template <typename T, int D, int WAVES>
 __global__ __launch_bounds__(WAVES *kWave, Frag<T>::kFloat || WAVES == 1 ? 1 : 2) void attn_grad_q_kernel(const Backward a) {
     typedef typename Frag<T>::type frag;
+    typedef typename Frag<T>::operand operand_t;
     typedef Tile<T, D, WAVES> KvTile;
     constexpr uint32_t kOwn = 32 * WAVES;
     constexpr bool kHalf = !Frag<T>::kFloat;
@@ -179,7 +180,7 @@ __global__ __launch_bounds__(WAVES *kWave, Frag<T>::kFloat || WAVES == 1 ? 1 : 2
     };
     const T *kbase = static_cast<const T *>(a.k.at) + (packed ? 0 : b * a.k.batch) + (size_t)k0 * a.k.row + head * a.k.head;
     const T *vbase = static_cast<const T *>(a.v.at) + (packed ? 0 : b * a.v.batch) + (size_t)k0 * a.v.row + head * a.v.head;
-    frag q[KD], g[KD];
+    operand_t q[KD], g[KD];
     load_frags<T, D>(live ? at_row(a.q) : nullptr, a.s.dim, a.vec, q);
     load_frags<T, D>(live ? at_row(a.dout) : nullptr, a.s.dim, a.vec, g);
     const size_t place = ((size_t)(packed ? 0 : b) * lq + q0 + i) * a.s.heads + qh;
@@ -267,7 +268,7 @@ __global__ __launch_bounds__(WAVES *kWave, Frag<T>::kFloat || WAVES == 1 ? 1 : 2
                     }
 #pragma unroll
                     for (int u = 0; u < (MASKED && kHalf ? 4 : 2); u++) {
-                        frag ds;
+                        operand_t ds;
                         to_frag(s, u % 2, ds);
                         if constexpr (MASKED && kHalf) {  // (a second time with what the rounding took away)
                             if (u < 2) left_by(ds, u, s);
@@ -308,6 +309,7 @@ struct KeptValues<T, D, WAVES, false> {
 template <typename T, int D, int WAVES>
 __global__ __launch_bounds__(WAVES *kWave, Frag<T>::kFloat || WAVES == 1 ? 1 : 2) void attn_grad_kv_kernel(const Backward a) {
     typedef typename Frag<T>::type frag;
+    typedef typename Frag<T>::operand operand_t;
     constexpr uint32_t kOwn = 32 * WAVES;
     typedef Tile<T, D, WAVES, D == 128 ? 32 : Frag<T>::kTile> RowTile;  // (64 rows of 128 columns on their way leave too few registers)
     constexpr bool kHalf = !Frag<T>::kFloat;
@@ -337,7 +339,7 @@ __global__ __launch_bounds__(WAVES *kWave, Frag<T>::kFloat || WAVES == 1 ? 1 : 2
     const T *qbase = static_cast<const T *>(a.q.at) + (packed ? 0 : b * a.q.batch) + (size_t)q0 * a.q.row + head * a.s.group * a.q.head;
     const T *gbase = static_cast<const T *>(a.dout.at) + (packed ? 0 : b * a.dout.batch) + (size_t)q0 * a.dout.row + head * a.s.group * a.dout.head;
     const size_t place0 = ((size_t)(packed ? 0 : b) * lq + q0) * a.s.heads + head * a.s.group;
-    frag k[KD], v[kVInLds ? 1 : KD];
+    operand_t k[KD], v[kVInLds ? 1 : KD];
     load_frags<T, D>(live ? kbase : nullptr, a.s.dim, a.vec, k);
     if constexpr (kVInLds) {
         typedef typename KeptValues<T, D, WAVES, true>::type Values;
@@ -354,7 +356,7 @@ __global__ __launch_bounds__(WAVES *kWave, Frag<T>::kFloat || WAVES == 1 ? 1 : 2
     } else {
         load_frags<T, D>(live ? vbase : nullptr, a.s.dim, a.vec, v);
     }
-    auto value = [&](int c) -> frag {
+    auto value = [&](int c) -> operand_t {
         if constexpr (kVInLds)
             return values.rows(lanes, wave * 32, c);
         else
@@ -478,7 +480,7 @@ __global__ __launch_bounds__(WAVES *kWave, Frag<T>::kFloat || WAVES == 1 ? 1 : 2
                         for (int r = 0; r < 16; r++)
                             if (first + 32 * n + 8 * (r / 4) + 4 * h + r % 4 < from) s[r] = dp[r] = 0.0f;
                     }
-                    frag p[2], ds[2];
+                    operand_t p[2], ds[2];
 #pragma unroll
                     for (int u = 0; u < 2; u++) {
                         to_frag(s, u, p[u]);

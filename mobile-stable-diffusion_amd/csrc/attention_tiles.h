@@ -4,8 +4,11 @@
 // Products are formed transposed, so that what one leaves in registers is what the next one takes.  With A's rows and B's
 // columns both indexed by lane & 31, the accumulator's lane has column lane & 31 and, in register 4 i + j, row 8 i + 4 h + j
 // with h = lane / 32.  Registers 8 t ... 8 t + 7 are then, rounded to the storage type, the B operand of the product over
-// rows 16 t ... 16 t + 15, if its A operand takes the same rows in the same order.  float32 goes through the same fragments,
-// eight values a lane, as eight products of 32 x 32 x 2.
+// rows 16 t ... 16 t + 15, if its A operand takes the same rows in the same order.
+//
+// float32 goes through the same fragments, eight values a lane.  Each value is cut into three bfloat16 (8 bits each, together
+// all 24, and the exponents of float32), and six products of those stand for the one of float32: the three left out are below
+// 2^-23 of it.  Six products of 32 x 32 x 16 take 192 cycles, the eight of 32 x 32 x 2 in float32 512.
 #pragma once
 
 #include <initializer_list>
@@ -24,17 +27,26 @@ constexpr uint32_t kAttnThreads = 256, kAttnWaves = kAttnThreads / kWave;
 // A workgroup has 1 or 4 wavefronts, each with 32 rows of its own; the tiles that pass by are everyone's.
 constexpr uint32_t attn_rows(bool few) { return few ? 32 : 32 * kAttnWaves; }
 
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+struct Thirds {  // eight float32 as sums of three bfloat16 each
+    bf16x8 part[3];
+};
+
+// type: a fragment as it is read; operand: as a product's B operand takes it.
 template <typename T>
 struct Frag;
 template <>
 struct Frag<__half> {
     typedef half8 type;
+    typedef half8 operand;
     static constexpr int kTile = 64;  // rows of a tile in LDS
     static constexpr bool kFloat = false;
 };
 template <>
 struct Frag<float> {
     typedef f32x8 type;
+    typedef Thirds operand;
     static constexpr int kTile = 32;
     static constexpr bool kFloat = true;
 };
@@ -42,9 +54,32 @@ struct Frag<float> {
 __device__ __forceinline__ f32x16 mma(const half8 &a, const half8 &b, const f32x16 &c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
-__device__ __forceinline__ f32x16 mma(const f32x8 &a, const f32x8 &b, f32x16 c) {
+__device__ __forceinline__ half8 operand(const half8 &f) { return f; }
+__device__ __forceinline__ Thirds operand(const f32x8 &f) {
+    Thirds t;
+    uint32_t w[8];
+    __builtin_memcpy(w, &f, sizeof(w));
 #pragma unroll
-    for (int j = 0; j < 8; j++) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+    for (int n = 0; n < 3; n++) {
+        u32x4 packed;
+#pragma unroll
+        for (int j = 0; j < 4; j++) packed[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x07060302u);  // (the upper halves)
+        t.part[n] = __builtin_bit_cast(bf16x8, packed);
+        if (n == 2) break;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const float left = __uint_as_float(w[j]) - __uint_as_float(w[j] & 0xFFFF0000u);
+            w[j] = __float_as_uint(n == 0 && left != left ? 0.0f : left);  // (nothing is left of an infinity)
+        }
+    }
+    return t;
+}
+__device__ __forceinline__ f32x16 mma(const f32x8 &a, const Thirds &b, f32x16 c) {
+    const Thirds t = operand(a);
+    constexpr int kPairs[6][2] = {{0, 2}, {2, 0}, {1, 1}, {0, 1}, {1, 0}, {0, 0}};  // (the small ones first)
+#pragma unroll
+    for (int n = 0; n < 6; n++)
+        c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(t.part[kPairs[n][0]], b.part[kPairs[n][1]], c, 0, 0, 0);
     return c;
 }
 
@@ -66,9 +101,11 @@ __device__ __forceinline__ void to_frag(const f32x16 &c, int t, half8 &b) {
         b[2 * j + 1] = v[1];
     }
 }
-__device__ __forceinline__ void to_frag(const f32x16 &c, int t, f32x8 &b) {
+__device__ __forceinline__ void to_frag(const f32x16 &c, int t, Thirds &b) {
+    f32x8 f;
 #pragma unroll
-    for (int j = 0; j < 8; j++) b[j] = c[8 * t + j];
+    for (int j = 0; j < 8; j++) f[j] = c[8 * t + j];
+    b = operand(f);
 }
 
 __device__ __forceinline__ f32x16 zero16() {
@@ -85,7 +122,7 @@ __device__ __forceinline__ void keep_here(half8 &f) {
     f = __builtin_bit_cast(half8, v);
 }
 
-__device__ __forceinline__ void keep_here(f32x8 &) {}
+__device__ __forceinline__ void keep_here(Thirds &) {}
 
 // A masked pair's weight is zero, but zero times an infinity or NaN is not.  Where a tile has masked pairs, what its A operands
 // hold of those is left out of the product, and `add_odd` puts it back for the pairs that are visible.
@@ -123,9 +160,10 @@ __device__ __forceinline__ void add_odd(const Tile &tile, const TileLanes<T, D> 
     const uint32_t h = threadIdx.x % kWave / 32;
 #pragma unroll 1
     for (int r0 = 0; r0 < ROWS; r0 += 16) {
-        frag seen;
+        frag ones;
 #pragma unroll
-        for (int j = 0; j < 8; j++) seen[j] = visible(r0 + 8 * (j / 4) + 4 * h + j % 4) ? 1 : 0;
+        for (int j = 0; j < 8; j++) ones[j] = visible(r0 + 8 * (j / 4) + 4 * h + j % 4) ? 1 : 0;
+        const typename Frag<T>::operand seen = operand(ones);
 #pragma unroll
         for (int d = 0; d < D / 32; d++) {
             const frag one[1] = {tile.columns(lanes, r0, d)}, &a = one[0];
@@ -160,7 +198,7 @@ __device__ __forceinline__ u32x4 load_chunk(const T *row, uint32_t d, uint32_t d
 
 // Operands that a wavefront keeps: 32 rows (its lane's row, or null) as KD fragments.
 template <typename T, int D>
-__device__ __forceinline__ void load_frags(const T *row, uint32_t dim, bool vec, typename Frag<T>::type (&f)[D / 16]) {
+__device__ __forceinline__ void load_frags(const T *row, uint32_t dim, bool vec, typename Frag<T>::operand (&f)[D / 16]) {
     const uint32_t h = threadIdx.x % kWave / 32;
 #pragma unroll
     for (int k = 0; k < D / 16; k++) {
@@ -168,7 +206,9 @@ __device__ __forceinline__ void load_frags(const T *row, uint32_t dim, bool vec,
 #pragma unroll
         for (uint32_t i = 0; i < sizeof(T) / 2; i++)
             v[i] = row != nullptr ? load_chunk<T>(row, 16 * k + 8 * h + i * (16 / sizeof(T)), dim, vec) : u32x4{0, 0, 0, 0};
-        __builtin_memcpy(&f[k], v, sizeof(f[k]));
+        typename Frag<T>::type one;
+        __builtin_memcpy(&one, v, sizeof(one));
+        f[k] = operand(one);
     }
 }
 
