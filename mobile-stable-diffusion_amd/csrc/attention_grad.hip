@@ -24,7 +24,7 @@ struct Backward {
     const void *rest;  // [rows][heads][dim] what rounding took from out, or null
     float *delta, *norm, *v_norm;  // [rows][heads] D and |do|, [keys][kv_heads] |v|; the norms null for float32
     float *part;  // parts > 1: [parts][keys][kv_heads][dk, dv][dim]
-    uint32_t total_rows, total_keys, parts;
+    uint32_t total_rows, total_keys, parts, kv_blocks;
     FastDiv by_group;
     bool vec;
 };
@@ -150,19 +150,23 @@ __device__ __forceinline__ void store_rows(T *to, const f32x16 (&acc)[D / 32], f
 
 // dq: the forward kernel's tiles of rows over tiles of keys.
 template <typename T, int D, int WAVES>
-__global__ __launch_bounds__(WAVES *kWave, Frag<T>::kFloat || WAVES == 1 ? 1 : 2) void attn_grad_q_kernel(const Backward a) {
+struct ForQ {
+    Tile<T, D, WAVES> tiles[2][2];  // [buffer][K, V]
+};
+template <typename T, int D, int WAVES>
+__device__ __forceinline__ void attn_grad_q(const Backward &a, const uint32_t block, ForQ<T, D, WAVES> &lds) {
     typedef typename Frag<T>::type frag;
     typedef typename Frag<T>::operand operand_t;
     typedef Tile<T, D, WAVES> KvTile;
     constexpr uint32_t kOwn = 32 * WAVES;
     constexpr bool kHalf = !Frag<T>::kFloat;
     constexpr int R = KvTile::kRows, KD = D / 16, DB = D / 32;
-    __shared__ KvTile tiles[2][2];
+    KvTile(&tiles)[2][2] = lds.tiles;
     const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, h = lane / 32;
     const TileLanes<T, D> lanes;
-    const uint32_t head = blockIdx.x % a.s.kv_heads;
+    const uint32_t head = block % a.s.kv_heads;
     uint32_t b, tile, q0, lq, k0, lk;
-    if (!find_tile(a.s.q_offsets, a.s.batch, a.s.q_rows, a.s.group, kOwn, blockIdx.x / a.s.kv_heads, a.s.q_by_tile, b, tile)) return;
+    if (!find_tile(a.s.q_offsets, a.s.batch, a.s.q_rows, a.s.group, kOwn, block / a.s.kv_heads, a.s.q_by_tile, b, tile)) return;
     span(a.s.q_offsets, b, a.s.q_rows, q0, lq);
     span(a.s.k_offsets, b, a.s.k_rows, k0, lk);
     const uint32_t rows = lq * a.s.group;
@@ -290,8 +294,12 @@ __global__ __launch_bounds__(WAVES *kWave, Frag<T>::kFloat || WAVES == 1 ? 1 : 2
                 work(std::false_type{});
         }
     }
-    if (!live) return;
-    T *const to = static_cast<T *>(const_cast<void *>(a.dq.at)) + (packed ? 0 : b * a.dq.batch) + (size_t)(q0 + i) * a.dq.row + qh * a.dq.head;
+    uint32_t thread = threadIdx.x;  // (the row's number is formed again: over the loop there is no register for it)
+    asm volatile("" : "+v"(thread));
+    const uint32_t own_row = tile * kOwn + thread / kWave * 32 + thread % 32, own_i = own_row / a.s.group;
+    if (own_row >= rows) return;
+    T *const to = static_cast<T *>(const_cast<void *>(a.dq.at)) + (packed ? 0 : b * a.dq.batch) + (size_t)(q0 + own_i) * a.dq.row +
+                  (head * a.s.group + own_row - own_i * a.s.group) * a.dq.head;
     const float natural = a.s.scale2 * (1.0f / kLog2e);
     store_rows<T, D>(to, dq, kHalf ? ldexpf(natural, -scale.power) : natural, a.s.dim, a.vec);
 }
@@ -307,25 +315,33 @@ struct KeptValues<T, D, WAVES, false> {
 
 // dk and dv: a wavefront owns 32 keys as the columns of S = Q K^T; the rows that see them pass by.
 template <typename T, int D, int WAVES>
-__global__ __launch_bounds__(WAVES *kWave, Frag<T>::kFloat || WAVES == 1 ? 1 : 2) void attn_grad_kv_kernel(const Backward a) {
+struct ForKv {
+    static constexpr bool kVInLds = !Frag<T>::kFloat && D == 128;
+    static constexpr int kRows = D == 128 ? 32 : Frag<T>::kTile;  // (64 rows of 128 columns on their way leave too few registers)
+    Tile<T, D, WAVES, kRows> tiles[2][2];  // [buffer][Q, dO]
+    float stats[2][3][kRows];              // [buffer][- log2 sum, D, |do|]
+    typename KeptValues<T, D, WAVES, kVInLds>::type values;
+};
+template <typename T, int D, int WAVES>
+__device__ __forceinline__ void attn_grad_kv(const Backward &a, const uint32_t block, ForKv<T, D, WAVES> &lds) {
     typedef typename Frag<T>::type frag;
     typedef typename Frag<T>::operand operand_t;
     constexpr uint32_t kOwn = 32 * WAVES;
-    typedef Tile<T, D, WAVES, D == 128 ? 32 : Frag<T>::kTile> RowTile;  // (64 rows of 128 columns on their way leave too few registers)
+    typedef Tile<T, D, WAVES, ForKv<T, D, WAVES>::kRows> RowTile;
     constexpr bool kHalf = !Frag<T>::kFloat;
     constexpr int R = RowTile::kRows, KD = D / 16, DB = D / 32;
-    __shared__ RowTile tiles[2][2];                // [buffer][Q, dO]
-    constexpr bool kVInLds = kHalf && D == 128;
-    __shared__ typename KeptValues<T, D, WAVES, kVInLds>::type values;
-    __shared__ __align__(16) float stats[2][3][R]; // [buffer][- log2 sum, D, |do|]
+    constexpr bool kVInLds = ForKv<T, D, WAVES>::kVInLds;
+    RowTile(&tiles)[2][2] = lds.tiles;
+    float(&stats)[2][3][R] = lds.stats;
+    auto &values = lds.values;
     const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, h = lane / 32;
     const TileLanes<T, D> lanes;
-    const uint32_t head = blockIdx.x % a.s.kv_heads;
+    const uint32_t head = block % a.s.kv_heads;
     uint32_t b, tile, q0, lq, k0, lk;
-    if (!find_tile(a.s.k_offsets, a.s.batch, a.s.k_rows, 1, kOwn, blockIdx.x / a.s.kv_heads / a.parts, a.s.k_by_tile, b, tile)) return;
-    const uint32_t part = blockIdx.x / a.s.kv_heads % a.parts;
-    span(a.s.q_offsets, b, a.s.q_rows, q0, lq);
-    span(a.s.k_offsets, b, a.s.k_rows, k0, lk);
+    if (!find_tile(a.s.k_offsets, a.s.batch, a.s.k_rows, 1, kOwn, block / a.s.kv_heads / a.parts, a.s.k_by_tile, b, tile)) return;
+    const uint32_t part = block / a.s.kv_heads % a.parts;
+    span_of_all(a.s.q_offsets, b, a.s.q_rows, q0, lq);
+    span_of_all(a.s.k_offsets, b, a.s.k_rows, k0, lk);
     const bool packed = a.s.q_offsets != nullptr;
     const uint32_t rows = lq * a.s.group, key = tile * kOwn + wave * 32 + lane % 32;
     const bool live = key < lk;
@@ -536,13 +552,14 @@ __global__ __launch_bounds__(WAVES *kWave, Frag<T>::kFloat || WAVES == 1 ? 1 : 2
     asm volatile("" : "+v"(thread));
     const uint32_t own_key = tile * kOwn + thread / kWave * 32 + thread % 32;
     if (own_key >= lk) return;
+    const uint32_t own_b = packed ? 0 : __builtin_amdgcn_readfirstlane(b), first_key = __builtin_amdgcn_readfirstlane(k0);
     auto out = [&](const AttnView &to) {
-        return static_cast<T *>(const_cast<void *>(to.at)) + (packed ? 0 : b * to.batch) + (size_t)(k0 + own_key) * to.row + head * to.head;
+        return static_cast<T *>(const_cast<void *>(to.at)) + own_b * to.batch + (size_t)(first_key + own_key) * to.row + head * to.head;
     };
     const float natural = a.s.scale2 * (1.0f / kLog2e);
     const float by_k = kHalf ? ldexpf(natural, -scale.power) : natural, by_v = ldexpf(1.0f, -kPShift<T>);
     if (a.parts > 1) {
-        const size_t place = ((size_t)(packed ? 0 : b) * lk + k0 + own_key) * a.s.kv_heads + head;
+        const size_t place = ((size_t)own_b * lk + first_key + own_key) * a.s.kv_heads + head;
         float *const to = a.part + (part * (size_t)a.total_keys * a.s.kv_heads + place) * 2 * a.s.dim;
         const bool whole = a.s.dim % 4 == 0;
         store_rows<float, D>(to, dk, by_k, a.s.dim, whole);
@@ -551,6 +568,18 @@ __global__ __launch_bounds__(WAVES *kWave, Frag<T>::kFloat || WAVES == 1 ? 1 : 2
     }
     store_rows<T, D>(out(a.dk), dk, by_k, a.s.dim, a.vec);
     store_rows<T, D>(out(a.dv), dv, by_v, a.s.dim, a.vec);
+}
+
+// The workgroups of dk and dv, then those of dq, which fill up what the former leave; or one kind alone (float16 with 128 columns:
+// together they have a few registers too few).
+template <typename T, int D, int WAVES, bool KV, bool Q>
+__global__ __launch_bounds__(WAVES *kWave, Frag<T>::kFloat || WAVES == 1 ? 1 : 2) void attn_grad_kernel(const Backward a) {
+    constexpr size_t kBytes = std::max(KV ? sizeof(ForKv<T, D, WAVES>) : 0, Q ? sizeof(ForQ<T, D, WAVES>) : 0);
+    __shared__ __align__(16) char lds[kBytes];
+    if constexpr (KV) {
+        if (!Q || blockIdx.x < a.kv_blocks) return attn_grad_kv<T, D, WAVES>(a, blockIdx.x, *reinterpret_cast<ForKv<T, D, WAVES> *>(lds));
+    }
+    if constexpr (Q) attn_grad_q<T, D, WAVES>(a, blockIdx.x - (KV ? a.kv_blocks : 0), *reinterpret_cast<ForQ<T, D, WAVES> *>(lds));
 }
 
 // dk and dv from the parts, in their order, for a few keys of a head.
@@ -586,9 +615,8 @@ size_t tiles_of(const int32_t *offsets, size_t batch, size_t rows, size_t times,
     if (offsets == nullptr) return batch * ((rows * times + own - 1) / own);
     return rows * times / own + batch;
 }
-size_t tiles_of_keys(const AttnProblem &p) {
-    return tiles_of(p.k_offsets, p.batch, p.k_rows, 1, attn_rows(attn_few(p, p.k_rows, 1)));
-}
+bool few_rows_and_keys(const AttnProblem &p) { return attn_few(p, p.q_rows, p.heads / p.kv_heads) && attn_few(p, p.k_rows, 1); }
+size_t tiles_of_keys(const AttnProblem &p) { return tiles_of(p.k_offsets, p.batch, p.k_rows, 1, attn_rows(few_rows_and_keys(p))); }
 
 // Parts of the rows for dk and dv.  Under a causal mask tiles of keys differ in the rows that see them: cut in two they fill up
 // a launch of few rounds.  Few keys and many rows (a prompt's keys, an image's rows) are cut until the chip is full, with
@@ -623,29 +651,26 @@ int attn_grad_dispatch(const AttnProblem &p, const AttnGradViews &g, const float
     const uint32_t parts = (uint32_t)std::max<size_t>(1, std::min<size_t>(row_parts(p), (workspace_bytes - vectors) / part_bytes));
     const Backward a{attn_shape(p), g.q, g.k, g.v, g.out, g.dout, g.dq, g.dk, g.dv, lse, rest, delta,
                      kHalf ? delta + rows * p.heads : nullptr, kHalf ? delta + 2 * rows * p.heads : nullptr, part, (uint32_t)rows, (uint32_t)keys, parts,
+                     (uint32_t)(tiles_of_keys(p) * p.kv_heads * parts),
                      make_fast_div((uint32_t)(p.heads / p.kv_heads)), attn_vectors(sizeof(T), p, {g.q, g.k, g.v, g.out, g.dout, g.dq, g.dk, g.dv, AttnView{rest, 0, 0, 0}})};
     const size_t items = rows * p.heads + (kHalf ? keys * p.kv_heads : 0);
     if (items != 0)
         launch((attn_grad_rows_kernel<T>), dim3((uint32_t)((items + 15) / 16)), dim3(kAttnThreads), 0, stream, a);
-    const size_t group = p.heads / p.kv_heads;
-    const bool few_rows = attn_few(p, p.q_rows, group), few_keys = attn_few(p, p.k_rows, 1);
-    const dim3 of_rows((uint32_t)(tiles_of(p.q_offsets, p.batch, p.q_rows, group, attn_rows(few_rows)) * p.kv_heads));
-    const dim3 of_keys((uint32_t)(tiles_of_keys(p) * p.kv_heads * parts));
-    if (of_keys.x != 0) {
-        if (few_keys)
-            launch((attn_grad_kv_kernel<T, 64, 1>), of_keys, dim3(kWave), 0, stream, a);
-        else if (p.dim <= 64)
-            launch((attn_grad_kv_kernel<T, 64, kAttnWaves>), of_keys, dim3(kAttnThreads), 0, stream, a);
-        else
-            launch((attn_grad_kv_kernel<T, 128, kAttnWaves>), of_keys, dim3(kAttnThreads), 0, stream, a);
-    }
-    if (of_rows.x != 0) {
-        if (few_rows)
-            launch((attn_grad_q_kernel<T, 64, 1>), of_rows, dim3(kWave), 0, stream, a);
-        else if (p.dim <= 64)
-            launch((attn_grad_q_kernel<T, 64, kAttnWaves>), of_rows, dim3(kAttnThreads), 0, stream, a);
-        else
-            launch((attn_grad_q_kernel<T, 128, kAttnWaves>), of_rows, dim3(kAttnThreads), 0, stream, a);
+    const bool few = few_rows_and_keys(p);
+    const size_t row_blocks = tiles_of(p.q_offsets, p.batch, p.q_rows, p.heads / p.kv_heads, attn_rows(few)) * p.kv_heads;
+    const dim3 grid((uint32_t)(a.kv_blocks + row_blocks));
+    if (grid.x != 0) {
+        if (few) {
+            launch((attn_grad_kernel<T, 64, 1, true, true>), grid, dim3(kWave), 0, stream, a);
+        } else if (p.dim <= 64) {
+            launch((attn_grad_kernel<T, 64, kAttnWaves, true, true>), grid, dim3(kAttnThreads), 0, stream, a);
+        } else if constexpr (!kHalf) {
+            launch((attn_grad_kernel<T, 128, kAttnWaves, true, true>), grid, dim3(kAttnThreads), 0, stream, a);
+        } else {
+            if (a.kv_blocks != 0) launch((attn_grad_kernel<T, 128, kAttnWaves, true, false>), dim3(a.kv_blocks), dim3(kAttnThreads), 0, stream, a);
+            if (row_blocks != 0)
+                launch((attn_grad_kernel<T, 128, kAttnWaves, false, true>), dim3((uint32_t)row_blocks), dim3(kAttnThreads), 0, stream, a);
+        }
     }
     if (parts > 1) {
         const size_t joins = tiles_of(p.k_offsets, p.batch, p.k_rows, 1, kJoinKeys) * p.kv_heads;

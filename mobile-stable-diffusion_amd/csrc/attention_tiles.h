@@ -360,6 +360,12 @@ __device__ __forceinline__ void span(const int32_t *offsets, uint32_t b, uint32_
     first = (uint32_t)from;
     count = (uint32_t)(to - from);
 }
+// The same for a sequence that is the whole wavefront's, in scalar registers.
+__device__ __forceinline__ void span_of_all(const int32_t *offsets, uint32_t b, uint32_t rows, uint32_t &first, uint32_t &count) {
+    span(offsets, b, rows, first, count);
+    first = __builtin_amdgcn_readfirstlane(first);
+    count = __builtin_amdgcn_readfirstlane(count);
+}
 
 // Tile number `index` of all sequences' tiles, `per` rows each: a sequence has `times` rows for each of its offsets' rows.
 // `by_tile`: see AttnShape.  False where there are fewer tiles.  Whole wavefronts look, 64 sequences at a time.
