@@ -23,8 +23,8 @@ struct Backward {
     const float *lse;
     const void *rest;  // [rows][heads][dim] what rounding took from out, or null
     float *delta, *norm, *v_norm;  // [rows][heads] D and |do|, [keys][kv_heads] |v|; the norms null for float32
-    float *part;  // parts > 1: [parts][keys][kv_heads][dk, dv][dim]
-    uint32_t total_rows, total_keys, parts, kv_blocks;
+    float *part, *q_part;  // parts > 1: [parts][keys][kv_heads][dk, dv][dim]; q_parts > 1: [q_parts][rows][heads][dim]
+    uint32_t total_rows, total_keys, parts, q_parts, kv_blocks;
     FastDiv by_group;
     bool vec;
 };
@@ -166,7 +166,8 @@ __device__ __forceinline__ void attn_grad_q(const Backward &a, const uint32_t bl
     const TileLanes<T, D> lanes;
     const uint32_t head = block % a.s.kv_heads;
     uint32_t b, tile, q0, lq, k0, lk;
-    if (!find_tile(a.s.q_offsets, a.s.batch, a.s.q_rows, a.s.group, kOwn, block / a.s.kv_heads, a.s.q_by_tile, b, tile)) return;
+    if (!find_tile(a.s.q_offsets, a.s.batch, a.s.q_rows, a.s.group, kOwn, block / a.s.kv_heads / a.q_parts, a.s.q_by_tile, b, tile)) return;
+    const uint32_t part = block / a.s.kv_heads % a.q_parts;
     span(a.s.q_offsets, b, a.s.q_rows, q0, lq);
     span(a.s.k_offsets, b, a.s.k_rows, k0, lk);
     const uint32_t rows = lq * a.s.group;
@@ -194,7 +195,8 @@ __device__ __forceinline__ void attn_grad_q(const Backward &a, const uint32_t bl
     const float *const v_norm = kHalf ? a.v_norm + ((size_t)(packed ? 0 : b) * lk + k0) * a.s.kv_heads + head : nullptr;
 
     const uint32_t last_row = min(rows, (tile + 1) * kOwn) - 1;
-    const uint32_t t1 = (seen_by(last_row / a.s.group) + R - 1) / R;
+    const uint32_t all = (seen_by(last_row / a.s.group) + R - 1) / R, each = (all + a.q_parts - 1) / a.q_parts;
+    const uint32_t t0 = min(all, part * each), t1 = min(all, t0 + each);
     const uint32_t wave_row = tile * kOwn + wave * 32;
     const uint32_t wave_limit = wave_row < rows ? seen_by(min(rows - 1, wave_row + 31) / a.s.group) : 0;
     const uint32_t wave_full = wave_row < rows ? seen_by(wave_row / a.s.group) : 0;
@@ -223,13 +225,13 @@ __device__ __forceinline__ void attn_grad_q(const Backward &a, const uint32_t bl
 #pragma unroll
     for (int d = 0; d < DB; d++) dq[d] = zero16();
     DsScale scale;
-    if (t1 != 0) fetch(0, 0);
-    for (uint32_t t = 0; t < t1; t++) {
+    if (t0 < t1) fetch(t0, 0);
+    for (uint32_t t = t0; t < t1; t++) {
         const float v_norms = next_norm;  // (of the tile's keys, one to a lane)
         wait_tiles();
         __syncthreads();
-        if (t + 1 < t1) fetch(t + 1, (t + 1) & 1);
-        const KvTile &kt = tiles[t & 1][0], &vt = tiles[t & 1][1];
+        if (t + 1 < t1) fetch(t + 1, (t + 1 - t0) & 1);
+        const KvTile &kt = tiles[(t - t0) & 1][0], &vt = tiles[(t - t0) & 1][1];
         const uint32_t first = t * R;
         if (first < wave_limit) {
             auto work = [&](auto with_masked) {  // (apart for tiles with masked pairs, as in the forward call)
@@ -300,8 +302,13 @@ __device__ __forceinline__ void attn_grad_q(const Backward &a, const uint32_t bl
     if (own_row >= rows) return;
     T *const to = static_cast<T *>(const_cast<void *>(a.dq.at)) + (packed ? 0 : b * a.dq.batch) + (size_t)(q0 + own_i) * a.dq.row +
                   (head * a.s.group + own_row - own_i * a.s.group) * a.dq.head;
-    const float natural = a.s.scale2 * (1.0f / kLog2e);
-    store_rows<T, D>(to, dq, kHalf ? ldexpf(natural, -scale.power) : natural, a.s.dim, a.vec);
+    const float natural = a.s.scale2 * (1.0f / kLog2e), by_q = kHalf ? ldexpf(natural, -scale.power) : natural;
+    if (a.q_parts > 1) {
+        const size_t own = ((size_t)(packed ? 0 : b) * lq + q0 + own_i) * a.s.heads + head * a.s.group + own_row - own_i * a.s.group;
+        store_rows<float, D>(a.q_part + (part * (size_t)a.total_rows * a.s.heads + own) * a.s.dim, dq, by_q, a.s.dim, a.s.dim % 4 == 0);
+        return;
+    }
+    store_rows<T, D>(to, dq, by_q, a.s.dim, a.vec);
 }
 
 template <typename T, int D, int WAVES, bool IN_LDS>
@@ -582,32 +589,34 @@ __global__ __launch_bounds__(WAVES *kWave, Frag<T>::kFloat || WAVES == 1 ? 1 : 2
     if constexpr (Q) attn_grad_q<T, D, WAVES>(a, blockIdx.x - (KV ? a.kv_blocks : 0), *reinterpret_cast<ForQ<T, D, WAVES> *>(lds));
 }
 
-// dk and dv from the parts, in their order, for a few keys of a head.
-constexpr uint32_t kJoinKeys = 8;
-template <typename T>
+// Gradients from their parts, in the parts' order, for a few rows of a head: of dk and dv, or of dq.
+constexpr uint32_t kJoinRows = 8;
+template <typename T, bool OF_KEYS>
 __global__ __launch_bounds__(kAttnThreads) void attn_grad_join_kernel(const Backward a) {
-    const uint32_t head = blockIdx.x % a.s.kv_heads;
-    uint32_t b, tile, k0, lk;
-    if (!find_tile(a.s.k_offsets, a.s.batch, a.s.k_rows, 1, kJoinKeys, blockIdx.x / a.s.kv_heads, false, b, tile)) return;
-    span(a.s.k_offsets, b, a.s.k_rows, k0, lk);
-    const bool packed = a.s.k_offsets != nullptr;
-    const uint32_t n = min(kJoinKeys, lk - tile * kJoinKeys), row = 2 * a.s.dim;
-    const size_t step = (size_t)a.total_keys * a.s.kv_heads * row;
+    const uint32_t heads = OF_KEYS ? a.s.kv_heads : a.s.heads, parts = OF_KEYS ? a.parts : a.q_parts, head = blockIdx.x % heads;
+    const int32_t *const offsets = OF_KEYS ? a.s.k_offsets : a.s.q_offsets;
+    const uint32_t rows = OF_KEYS ? a.s.k_rows : a.s.q_rows;
+    uint32_t b, tile, first, count;
+    if (!find_tile(offsets, a.s.batch, rows, 1, kJoinRows, blockIdx.x / heads, false, b, tile)) return;
+    span(offsets, b, rows, first, count);
+    const uint32_t n = min(kJoinRows, count - tile * kJoinRows), row = (OF_KEYS ? 2 : 1) * a.s.dim;
+    const size_t step = (size_t)(OF_KEYS ? a.total_keys : a.total_rows) * heads * row;
     for (uint32_t at = threadIdx.x; at < n * row; at += kAttnThreads) {
-        const uint32_t r = at / row, c = at - r * row, key = tile * kJoinKeys + r;
-        const float *from = a.part + (((size_t)(packed ? 0 : b) * lk + k0 + key) * a.s.kv_heads + head) * row + c;
+        const uint32_t r = at / row, c = at - r * row;
+        const size_t own = first + tile * kJoinRows + r;
+        const float *from = (OF_KEYS ? a.part : a.q_part) + (((size_t)(offsets != nullptr ? 0 : b) * count + own) * heads + head) * row + c;
         float sum = 0.0f;
-        for (uint32_t p0 = 0; p0 < a.parts; p0 += 8) {
+        for (uint32_t p0 = 0; p0 < parts; p0 += 8) {
             float f[8];
 #pragma unroll
-            for (uint32_t u = 0; u < 8; u++) f[u] = p0 + u < a.parts ? from[(p0 + u) * step] : 0.0f;
+            for (uint32_t u = 0; u < 8; u++) f[u] = p0 + u < parts ? from[(p0 + u) * step] : 0.0f;
 #pragma unroll
             for (uint32_t u = 0; u < 8; u++) sum += f[u];
         }
-        const bool of_k = c < a.s.dim;
-        const AttnView &to = of_k ? a.dk : a.dv;
-        Store<T>::store1(static_cast<T *>(const_cast<void *>(to.at)) + (packed ? 0 : b * to.batch) + (size_t)(k0 + key) * to.row +
-                             head * to.head + (of_k ? c : c - a.s.dim), sum);
+        const bool first_half = c < a.s.dim;
+        const AttnView &to = !OF_KEYS ? a.dq : first_half ? a.dk : a.dv;
+        Store<T>::store1(static_cast<T *>(const_cast<void *>(to.at)) + (offsets != nullptr ? 0 : b * to.batch) + own * to.row + head * to.head +
+                             (first_half ? c : c - a.s.dim), sum);
     }
 }
 
@@ -629,15 +638,39 @@ uint32_t row_parts(const AttnProblem &p) {
     return (uint32_t)std::max<size_t>(1, std::min<size_t>(parts, rows / 256));
 }
 
+// Parts of the keys for dq, where rows are too few to fill the chip, as in the forward call.
+uint32_t dq_parts(const AttnProblem &p) {
+    const size_t own = attn_rows(few_rows_and_keys(p)), cus = chip_info().cus;
+    const size_t blocks = std::max<size_t>(1, tiles_of(p.q_offsets, p.batch, p.q_rows, p.heads / p.kv_heads, own) * p.kv_heads);
+    const size_t keys = p.k_offsets != nullptr ? p.k_rows / std::max<size_t>(1, p.batch) : p.k_rows;
+    if (blocks > cus) return 1;
+    return (uint32_t)std::max<size_t>(1, std::min<size_t>((p.k_offsets != nullptr ? 8 : 2) * cus / blocks, keys / 256));
+}
+
+// Floats of the workspace: vectors over rows and keys, parts of dk and dv, parts of dq.
+struct Room {
+    size_t vectors, part, q_part;  // (of one part)
+};
+Room room_of(const AttnProblem &p) {
+    const size_t rows = p.q_offsets == nullptr ? p.batch * p.q_rows : p.q_rows, keys = p.k_offsets == nullptr ? p.batch * p.k_rows : p.k_rows;
+    return Room{(2 * rows * p.heads + keys * p.kv_heads + 3) / 4 * 4, (keys * p.kv_heads * 2 * p.dim + 3) / 4 * 4, (rows * p.heads * p.dim + 3) / 4 * 4};
+}
+
 }  // namespace
 
 size_t attn_grad_workspace_bytes(const AttnProblem &p) {
-    const size_t rows = p.q_offsets == nullptr ? p.batch * p.q_rows : p.q_rows, keys = p.k_offsets == nullptr ? p.batch * p.k_rows : p.k_rows;
     AttnProblem masked = p, open = p;  // (the bytes go by the sizes alone, the parts by the mask too)
     masked.causal = true;
     open.causal = false;
-    const size_t parts = std::max(row_parts(masked), row_parts(open)), vectors = (2 * rows * p.heads + keys * p.kv_heads + 3) / 4 * 4;
-    return (vectors + (parts > 1 ? parts * keys * p.kv_heads * 2 * p.dim : 0)) * sizeof(float);
+    const size_t parts = std::max(row_parts(masked), row_parts(open)), q_parts = dq_parts(p);
+    const Room r = room_of(p);
+    return (r.vectors + (parts > 1 ? parts * r.part : 0) + (q_parts > 1 ? q_parts * r.q_part : 0)) * sizeof(float);
+}
+
+template <typename T, int D>
+static void launch_apart(const Backward &a, uint32_t row_blocks, hipStream_t stream) {
+    if (a.kv_blocks != 0) launch((attn_grad_kernel<T, D, kAttnWaves, true, false>), dim3(a.kv_blocks), dim3(kAttnThreads), 0, stream, a);
+    if (row_blocks != 0) launch((attn_grad_kernel<T, D, kAttnWaves, false, true>), dim3(row_blocks), dim3(kAttnThreads), 0, stream, a);
 }
 
 template <typename T>
@@ -646,36 +679,46 @@ int attn_grad_dispatch(const AttnProblem &p, const AttnGradViews &g, const float
     const size_t rows = p.q_offsets == nullptr ? p.batch * p.q_rows : p.q_rows, keys = p.k_offsets == nullptr ? p.batch * p.k_rows : p.k_rows;
     float *const delta = static_cast<float *>(workspace);
     constexpr bool kHalf = !Frag<T>::kFloat;
-    float *const part = delta + (2 * rows * p.heads + keys * p.kv_heads + 3) / 4 * 4;
-    const size_t vectors = (size_t)(part - delta) * sizeof(float), part_bytes = std::max<size_t>(1, keys * p.kv_heads * 2 * p.dim * sizeof(float));
-    const uint32_t parts = (uint32_t)std::max<size_t>(1, std::min<size_t>(row_parts(p), (workspace_bytes - vectors) / part_bytes));
+    // no more parts than the workspace holds, those of dk and dv first
+    const Room r = room_of(p);
+    size_t left = workspace_bytes / sizeof(float) - r.vectors;
+    const uint32_t parts = (uint32_t)std::max<size_t>(1, std::min<size_t>(row_parts(p), left / std::max<size_t>(1, r.part)));
+    if (parts > 1) left -= parts * r.part;
+    const uint32_t q_parts = (uint32_t)std::max<size_t>(1, std::min<size_t>(dq_parts(p), left / std::max<size_t>(1, r.q_part)));
+    float *const part = delta + r.vectors, *const q_part = part + (parts > 1 ? parts * r.part : 0);
     const Backward a{attn_shape(p), g.q, g.k, g.v, g.out, g.dout, g.dq, g.dk, g.dv, lse, rest, delta,
-                     kHalf ? delta + rows * p.heads : nullptr, kHalf ? delta + 2 * rows * p.heads : nullptr, part, (uint32_t)rows, (uint32_t)keys, parts,
+                     kHalf ? delta + rows * p.heads : nullptr, kHalf ? delta + 2 * rows * p.heads : nullptr, part, q_part, (uint32_t)rows, (uint32_t)keys, parts, q_parts,
                      (uint32_t)(tiles_of_keys(p) * p.kv_heads * parts),
                      make_fast_div((uint32_t)(p.heads / p.kv_heads)), attn_vectors(sizeof(T), p, {g.q, g.k, g.v, g.out, g.dout, g.dq, g.dk, g.dv, AttnView{rest, 0, 0, 0}})};
     const size_t items = rows * p.heads + (kHalf ? keys * p.kv_heads : 0);
     if (items != 0)
         launch((attn_grad_rows_kernel<T>), dim3((uint32_t)((items + 15) / 16)), dim3(kAttnThreads), 0, stream, a);
     const bool few = few_rows_and_keys(p);
-    const size_t row_blocks = tiles_of(p.q_offsets, p.batch, p.q_rows, p.heads / p.kv_heads, attn_rows(few)) * p.kv_heads;
+    const size_t row_blocks = tiles_of(p.q_offsets, p.batch, p.q_rows, p.heads / p.kv_heads, attn_rows(few)) * p.kv_heads * q_parts;
     const dim3 grid((uint32_t)(a.kv_blocks + row_blocks));
     if (grid.x != 0) {
         if (few) {
             launch((attn_grad_kernel<T, 64, 1, true, true>), grid, dim3(kWave), 0, stream, a);
         } else if (p.dim <= 64) {
-            launch((attn_grad_kernel<T, 64, kAttnWaves, true, true>), grid, dim3(kAttnThreads), 0, stream, a);
+            // (apart, dq has three wavefronts per SIMD in float16: 5 % faster where there are rounds enough)
+            bool apart = false;
+            if constexpr (kHalf) {
+                apart = grid.x > 8 * chip_info().cus;
+                if (apart) launch_apart<T, 64>(a, (uint32_t)row_blocks, stream);
+            }
+            if (!apart) launch((attn_grad_kernel<T, 64, kAttnWaves, true, true>), grid, dim3(kAttnThreads), 0, stream, a);
         } else if constexpr (!kHalf) {
             launch((attn_grad_kernel<T, 128, kAttnWaves, true, true>), grid, dim3(kAttnThreads), 0, stream, a);
         } else {
-            if (a.kv_blocks != 0) launch((attn_grad_kernel<T, 128, kAttnWaves, true, false>), dim3(a.kv_blocks), dim3(kAttnThreads), 0, stream, a);
-            if (row_blocks != 0)
-                launch((attn_grad_kernel<T, 128, kAttnWaves, false, true>), dim3((uint32_t)row_blocks), dim3(kAttnThreads), 0, stream, a);
+            launch_apart<T, 128>(a, (uint32_t)row_blocks, stream);
         }
     }
-    if (parts > 1) {
-        const size_t joins = tiles_of(p.k_offsets, p.batch, p.k_rows, 1, kJoinKeys) * p.kv_heads;
-        launch((attn_grad_join_kernel<T>), dim3((uint32_t)joins), dim3(kAttnThreads), 0, stream, a);
-    }
+    if (parts > 1)
+        launch((attn_grad_join_kernel<T, true>), dim3((uint32_t)(tiles_of(p.k_offsets, p.batch, p.k_rows, 1, kJoinRows) * p.kv_heads)),
+               dim3(kAttnThreads), 0, stream, a);
+    if (q_parts > 1)
+        launch((attn_grad_join_kernel<T, false>), dim3((uint32_t)(tiles_of(p.q_offsets, p.batch, p.q_rows, 1, kJoinRows) * p.heads)),
+               dim3(kAttnThreads), 0, stream, a);
     return launch_status();
 }
 

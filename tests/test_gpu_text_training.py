@@ -252,9 +252,10 @@ def test_float16_gradients_keep_their_digits_at_any_size(msd, cuda, size):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
-@pytest.mark.parametrize("causal,lengths", [(False, [(2100, 77)]), (True, [(900, 900)]), (False, [(1500, 20), (0, 5), (3, 0), (700, 130)])])
-def test_gradients_of_keys_that_many_rows_see(msd, cuda, dtype, causal, lengths):
-    """Few keys, many rows: the rows are cut into parts that are added afterwards."""
+@pytest.mark.parametrize("causal,lengths", [(False, [(2100, 77)]), (True, [(900, 900)]), (False, [(1500, 20), (0, 5), (3, 0), (700, 130)]),
+                                            (False, [(3, 2500)]), (True, [(2, 1500), (0, 4), (9, 700), (5, 0)])])
+def test_gradients_of_few_keys_and_of_few_rows(msd, cuda, dtype, causal, lengths):
+    """Few keys and many rows, few rows and many keys: the many are cut into parts that are added afterwards."""
     q, k, v, dout = _pack(lengths, 4, 2, 48, DTYPES[dtype])
     want = plain.attention(q, k, v, causal, 0.2, dout, lengths)
     offsets, offsets_k = _offsets([a for a, _ in lengths], cuda), _offsets([b for _, b in lengths], cuda)
