@@ -466,7 +466,7 @@ int msd_softmax(const void *x, void *y, size_t rows, size_t cols, int stable, in
  * workspace: 16-byte aligned device memory of at least the bytes that msd_attention_workspace reports (host only; dtype as for
  * the call; backward = 0), apart from all else; its contents need not be set, are left undefined, and belong to this call until it (or every
  * replay of it) is done.  The call allocates nothing and gives the same bits every time, in a capture too.
- * At most 2^27 rows times heads of queries and of keys, and 2^22 sequences times kv_heads.
+ * At most 2^27 rows times heads of queries and of keys, 2^20 heads, and 2^22 sequences times kv_heads.
  */
 int msd_attention_workspace(size_t batch, size_t q_rows, size_t k_rows, size_t heads, size_t kv_heads, size_t dim, int packed,
                             int backward, int dtype, size_t *bytes);

@@ -859,7 +859,7 @@ static int attention_checks(size_t batch, size_t q_rows, size_t k_rows, size_t h
     constexpr size_t kMost = size_t(1) << 27;
     if (dtype != MSD_DTYPE_F32 && dtype != MSD_DTYPE_F16) return MSD_ERR_INVALID_VALUE;
     if (heads == 0 || kv_heads == 0 || heads % kv_heads != 0 || dim == 0 || dim > 128) return MSD_ERR_INVALID_VALUE;
-    if (batch > kMost || q_rows > kMost || k_rows > kMost || heads > kMost || batch * kv_heads > (size_t(1) << 22))
+    if (batch > kMost || q_rows > kMost || k_rows > kMost || heads > (size_t(1) << 20) || batch * kv_heads > (size_t(1) << 22))
         return MSD_ERR_INVALID_VALUE;
     *all_q = packed ? (batch != 0 ? q_rows : 0) : batch * q_rows;
     *all_k = packed ? (batch != 0 ? k_rows : 0) : batch * k_rows;

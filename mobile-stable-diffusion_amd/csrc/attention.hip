@@ -39,10 +39,10 @@ __global__ __launch_bounds__(WAVES *kWave, Frag<T>::kFloat || WAVES == 1 ? 1 : 2
     __shared__ KvTile tiles[2][2];  // [buffer][K, V]
     const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, h = lane / 32;
     const TileLanes<T, D> lanes;
-    const uint32_t head = blockIdx.x % a.s.kv_heads, rest = blockIdx.x / a.s.kv_heads;
-    const uint32_t part = rest % a.parts;
+    const uint32_t rest = fast_div(blockIdx.x, a.s.by_kv_heads), head = blockIdx.x - rest * a.s.kv_heads;
+    const uint32_t tiles_at = a.parts == 1 ? rest : rest / a.parts, part = rest - tiles_at * a.parts;
     uint32_t b, tile, q0, lq, k0, lk;
-    if (!find_tile(a.s.q_offsets, a.s.batch, a.s.q_rows, a.s.group, kOwn, rest / a.parts, a.s.q_by_tile, b, tile)) return;
+    if (!find_tile(a.s.q_offsets, a.s.batch, a.s.q_rows, a.s.group, kOwn, tiles_at, a.s.q_by_tile, b, tile)) return;
     span(a.s.q_offsets, b, a.s.q_rows, q0, lq);
     span(a.s.k_offsets, b, a.s.k_rows, k0, lk);
     const uint32_t rows = lq * a.s.group;
@@ -51,7 +51,7 @@ __global__ __launch_bounds__(WAVES *kWave, Frag<T>::kFloat || WAVES == 1 ? 1 : 2
     const bool packed_q = a.s.q_offsets != nullptr, packed_k = a.s.k_offsets != nullptr;
     // the lane's row: query i of head `qh`; it sees the keys [0, limit)
     const uint32_t row = tile * kOwn + wave * 32 + lane % 32;
-    const uint32_t i = row / a.s.group, qh = head * a.s.group + row % a.s.group;
+    const uint32_t i = fast_div(row, a.s.by_group), qh = head * a.s.group + row - i * a.s.group;
     const bool live = row < rows;
     auto seen_by = [&](uint32_t query) -> uint32_t {
         return a.s.causal ? (uint32_t)max((int64_t)0, min((int64_t)lk, (int64_t)query + 1 + lk - lq)) : lk;
@@ -65,11 +65,11 @@ __global__ __launch_bounds__(WAVES *kWave, Frag<T>::kFloat || WAVES == 1 ? 1 : 2
 
     // tiles of keys: what the workgroup's last row sees, this part's share of it
     const uint32_t last_row = min(rows, (tile + 1) * kOwn) - 1;
-    const uint32_t all = (seen_by(last_row / a.s.group) + R - 1) / R, each = (all + a.parts - 1) / a.parts;
+    const uint32_t all = (seen_by(fast_div(last_row, a.s.by_group)) + R - 1) / R, each = (all + a.parts - 1) / a.parts;
     const uint32_t t0 = min(all, part * each), t1 = min(all, t0 + each);
     const uint32_t wave_row = tile * kOwn + wave * 32;
-    const uint32_t wave_limit = wave_row < rows ? seen_by(min(rows - 1, wave_row + 31) / a.s.group) : 0;  // the most any row sees
-    const uint32_t wave_full = wave_row < rows ? seen_by(wave_row / a.s.group) : 0;                       // what every row sees
+    const uint32_t wave_limit = wave_row < rows ? seen_by(fast_div(min(rows - 1, wave_row + 31), a.s.by_group)) : 0;  // the most any row sees
+    const uint32_t wave_full = wave_row < rows ? seen_by(fast_div(wave_row, a.s.by_group)) : 0;                       // what every row sees
 
     uint32_t k_base[KvTile::kTurn], v_base[KvTile::kTurn];
     const uint32_t k_row = (uint32_t)a.k.row, v_row = (uint32_t)a.v.row;
@@ -170,56 +170,13 @@ __global__ __launch_bounds__(WAVES *kWave, Frag<T>::kFloat || WAVES == 1 ? 1 : 2
     const float lse = sum == 0.0f ? -__builtin_inff() : top - kShift<T> + __builtin_amdgcn_logf(sum);
     const size_t place = ((size_t)(packed_q ? 0 : b) * lq + q0 + i) * a.s.heads + qh;
     if (a.parts > 1) {
-        float *const to = a.part + (part * (size_t)a.total_rows * a.s.heads + place) * a.s.dim;
-#pragma unroll
-        for (int d = 0; d < DB; d++)
-#pragma unroll
-            for (int r = 0; r < 16; r++) {
-                const uint32_t col = 32 * d + 8 * (r / 4) + 4 * h + r % 4;
-                if (col < a.s.dim) to[col] = o[d][r] * inv;
-            }
+        store_rows<float, D>(a.part + (part * (size_t)a.total_rows * a.s.heads + place) * a.s.dim, o, inv, a.s.dim, a.s.dim % 4 == 0);
         if (h == 0) a.part_lse[part * (size_t)a.total_rows * a.s.heads + place] = lse;
         return;
     }
     T *const to = static_cast<T *>(const_cast<void *>(a.out.at)) + (packed_q ? 0 : b * a.out.batch) + (size_t)(q0 + i) * a.out.row + qh * a.out.head;
-#pragma unroll
-    for (int d = 0; d < DB; d++)
-#pragma unroll
-        for (int g = 0; g < 4; g++) {
-            const uint32_t col = 32 * d + 8 * g + 4 * h;
-            T v[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) Store<T>::store1(v + j, o[d][4 * g + j] * inv);
-            if (a.vec) {
-                if (col < a.s.dim) __builtin_memcpy(__builtin_assume_aligned(to + col, 4 * sizeof(T)), v, sizeof(v));
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    if (col + j < a.s.dim) to[col + j] = v[j];
-            }
-        }
-    if (!Frag<T>::kFloat && a.rest != nullptr) {
-        T *const left = static_cast<T *>(a.rest) + place * a.s.dim;
-#pragma unroll
-        for (int d = 0; d < DB; d++)
-#pragma unroll
-            for (int g = 0; g < 4; g++) {
-                const uint32_t col = 32 * d + 8 * g + 4 * h;
-                T v[4];
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const float value = o[d][4 * g + j] * inv;
-                    Store<T>::store1(v + j, value - round_to_storage<T>(value));
-                }
-                if (a.vec) {
-                    if (col < a.s.dim) __builtin_memcpy(__builtin_assume_aligned(left + col, 4 * sizeof(T)), v, sizeof(v));
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        if (col + j < a.s.dim) left[col + j] = v[j];
-                }
-            }
-    }
+    T *const rest_to = !Frag<T>::kFloat && a.rest != nullptr ? static_cast<T *>(a.rest) + place * a.s.dim : nullptr;
+    store_rows<T, D>(to, o, inv, a.s.dim, a.vec, rest_to);
     if (a.lse != nullptr && h == 0) a.lse[place] = lse;
 }
 
@@ -315,7 +272,8 @@ AttnShape attn_shape(const AttnProblem &p) {
     const size_t few = 8 * (size_t)chip_info().cus;
     const size_t own = attn_rows(attn_few(p, p.k_rows, 1)), k_blocks = p.batch * ((p.k_rows + own - 1) / own) * p.kv_heads;
     return AttnShape{p.q_offsets, p.k_offsets, (uint32_t)p.batch, (uint32_t)p.q_rows, (uint32_t)p.k_rows, (uint32_t)p.heads,
-                     (uint32_t)p.kv_heads, (uint32_t)(p.heads / p.kv_heads), (uint32_t)p.dim, p.scale * kLog2e, p.causal,
+                     (uint32_t)p.kv_heads, (uint32_t)(p.heads / p.kv_heads), (uint32_t)p.dim,
+                     make_fast_div((uint32_t)(p.heads / p.kv_heads)), make_fast_div((uint32_t)p.kv_heads), p.scale * kLog2e, p.causal,
                      p.causal && row_tiles(p) * p.kv_heads <= few, p.causal && k_blocks <= few};
 }
 

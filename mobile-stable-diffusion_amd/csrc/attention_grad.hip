@@ -22,12 +22,17 @@ struct Backward {
     AttnView q, k, v, out, dout, dq, dk, dv;
     const float *lse;
     const void *rest;  // [rows][heads][dim] what rounding took from out, or null
-    float *delta, *norm, *v_norm;  // [rows][heads] D and |do|, [keys][kv_heads] |v|; the norms null for float32
+    // [rows][heads] what the weights' exponents take (kPShift less the log2 sum), D and |do|, [keys][kv_heads] |v|; the norms null
+    // for float32
+    float *base, *delta, *norm, *v_norm;
     float *part, *q_part;  // parts > 1: [parts][keys][kv_heads][dk, dv][dim]; q_parts > 1: [q_parts][rows][heads][dim]
     uint32_t total_rows, total_keys, parts, q_parts, kv_blocks;
-    FastDiv by_group;
     bool vec;
 };
+
+// kPShift: float16 weights are kept that many powers of two larger where they are an operand themselves (they are at most 1).
+template <typename T>
+constexpr int kPShift = Frag<T>::kFloat ? 0 : 15;
 
 // 16 lanes to a row of a head.
 template <typename T>
@@ -55,15 +60,15 @@ __global__ __launch_bounds__(kAttnThreads) void attn_grad_rows_kernel(const Back
     float dot = 0.0f, square = 0.0f;
     for (uint32_t d = threadIdx.x % kTeam * E; d < a.s.dim; d += kTeam * E) {
         float x[E], y[E];
-        Store<T>::unpack(load_chunk<T>(first, d, a.s.dim, a.vec), x);
-        Store<T>::unpack(load_chunk<T>(second, d, a.s.dim, a.vec), y);
+        Store<T>::unpack(a.vec ? *reinterpret_cast<const u32x4 *>(first + d) : load_chunk<T>(first, d, a.s.dim), x);
+        Store<T>::unpack(a.vec ? *reinterpret_cast<const u32x4 *>(second + d) : load_chunk<T>(second, d, a.s.dim), y);
 #pragma unroll
         for (uint32_t e = 0; e < E; e++) {
             dot = fmaf(x[e], y[e], dot);
             square = fmaf(x[e], x[e], square);
         }
         if (rest != nullptr) {
-            Store<T>::unpack(load_chunk<T>(rest, d, a.s.dim, a.vec), y);
+            Store<T>::unpack(a.vec ? *reinterpret_cast<const u32x4 *>(rest + d) : load_chunk<T>(rest, d, a.s.dim), y);
 #pragma unroll
             for (uint32_t e = 0; e < E; e++) dot = fmaf(x[e], y[e], dot);
         }
@@ -74,26 +79,22 @@ __global__ __launch_bounds__(kAttnThreads) void attn_grad_rows_kernel(const Back
     if (of_keys) {
         a.v_norm[item] = sqrtf(square);
     } else {
+        const float lse = a.lse[item];
+        a.base[item] = lse == -__builtin_inff() ? lse : (float)kPShift<T> - lse;  // (a row that sees nothing: weights of zero)
         a.delta[item] = dot;
         if (a.norm != nullptr) a.norm[item] = sqrtf(square);
     }
 }
 
-// Largest value of the lanes up to this one, and from this one on.
+// Largest of the (not negative) values of the lanes up to this one.
 __device__ __forceinline__ float max_up_to(float v) {
-#pragma unroll
-    for (uint32_t d = 1; d < kWave; d *= 2) {
-        const float o = __shfl_up(v, d, kWave);
-        if (threadIdx.x % kWave >= d) v = fmaxf(v, o);
-    }
-    return v;
-}
-__device__ __forceinline__ float max_from(float v) {
-#pragma unroll
-    for (uint32_t d = 1; d < kWave; d *= 2) {
-        const float o = __shfl_down(v, d, kWave);
-        if (threadIdx.x % kWave + d < kWave) v = fmaxf(v, o);
-    }
+    v = fmaxf(v, dpp_move<0x111>(v));  // from 1, 2, 4 and 8 lanes below, within 16
+    v = fmaxf(v, dpp_move<0x112>(v));
+    v = fmaxf(v, dpp_move<0x114>(v));
+    v = fmaxf(v, dpp_move<0x118>(v));
+    // the last lane of the 16 below, for the odd ones of four; the last of the lower 32, for the upper ones
+    v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x142, 0xA, 0xF, true)));
+    v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x143, 0xC, 0xF, true)));
     return v;
 }
 
@@ -109,10 +110,6 @@ struct DsScale {
     }
 };
 
-// kPShift: float16 weights are kept that many powers of two larger where they are an operand themselves (they are at most 1).
-template <typename T>
-constexpr int kPShift = Frag<T>::kFloat ? 0 : 15;
-
 // Whether a sequence's float16 score gradients go into their products in two parts, the rounded value and what it left.  The
 // roundings of one part are as large as that of the result itself, 1.41 times it together, where many terms make a sum;
 // of few terms, or of few columns (dS sums to zero over the keys, and what is left of such sums is smaller), they come to 1.7 times
@@ -125,28 +122,6 @@ __device__ __forceinline__ void left_by(const half8 &f, int u, f32x16 &c) {
     for (int j = 0; j < 8; j++) c[8 * u + j] -= (float)f[j];
 }
 [[maybe_unused]] __device__ __forceinline__ void left_by(const Thirds &, int, f32x16 &) {}
-
-// Stores an accumulator's columns: row `to` gets the lane's column times `by`.
-template <typename T, int D>
-__device__ __forceinline__ void store_rows(T *to, const f32x16 (&acc)[D / 32], float by, uint32_t dim, bool vec) {
-    const uint32_t h = threadIdx.x % kWave / 32;
-#pragma unroll
-    for (int d = 0; d < D / 32; d++)
-#pragma unroll
-        for (int g = 0; g < 4; g++) {
-            const uint32_t col = 32 * d + 8 * g + 4 * h;
-            T v[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) Store<T>::store1(v + j, acc[d][4 * g + j] * by);
-            if (vec) {
-                if (col < dim) __builtin_memcpy(__builtin_assume_aligned(to + col, 4 * sizeof(T)), v, sizeof(v));
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    if (col + j < dim) to[col + j] = v[j];
-            }
-        }
-}
 
 // dq: the forward kernel's tiles of rows over tiles of keys.
 template <typename T, int D, int WAVES>
@@ -164,17 +139,17 @@ __device__ __forceinline__ void attn_grad_q(const Backward &a, const uint32_t bl
     KvTile(&tiles)[2][2] = lds.tiles;
     const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, h = lane / 32;
     const TileLanes<T, D> lanes;
-    const uint32_t head = block % a.s.kv_heads;
+    const uint32_t rest = fast_div(block, a.s.by_kv_heads), head = block - rest * a.s.kv_heads;
+    const uint32_t tiles_at = a.q_parts == 1 ? rest : rest / a.q_parts, part = rest - tiles_at * a.q_parts;
     uint32_t b, tile, q0, lq, k0, lk;
-    if (!find_tile(a.s.q_offsets, a.s.batch, a.s.q_rows, a.s.group, kOwn, block / a.s.kv_heads / a.q_parts, a.s.q_by_tile, b, tile)) return;
-    const uint32_t part = block / a.s.kv_heads % a.q_parts;
+    if (!find_tile(a.s.q_offsets, a.s.batch, a.s.q_rows, a.s.group, kOwn, tiles_at, a.s.q_by_tile, b, tile)) return;
     span(a.s.q_offsets, b, a.s.q_rows, q0, lq);
     span(a.s.k_offsets, b, a.s.k_rows, k0, lk);
     const uint32_t rows = lq * a.s.group;
     if (a.s.causal) tile = (rows + kOwn - 1) / kOwn - 1 - tile;
     const bool packed = a.s.q_offsets != nullptr;
     const uint32_t row = tile * kOwn + wave * 32 + lane % 32;
-    const uint32_t i = row / a.s.group, qh = head * a.s.group + row % a.s.group;
+    const uint32_t i = fast_div(row, a.s.by_group), qh = head * a.s.group + row - i * a.s.group;
     const bool live = row < rows;
     auto seen_by = [&](uint32_t query) -> uint32_t {
         return a.s.causal ? (uint32_t)max((int64_t)0, min((int64_t)lk, (int64_t)query + 1 + lk - lq)) : lk;
@@ -189,17 +164,16 @@ __device__ __forceinline__ void attn_grad_q(const Backward &a, const uint32_t bl
     load_frags<T, D>(live ? at_row(a.q) : nullptr, a.s.dim, a.vec, q);
     load_frags<T, D>(live ? at_row(a.dout) : nullptr, a.s.dim, a.vec, g);
     const size_t place = ((size_t)(packed ? 0 : b) * lq + q0 + i) * a.s.heads + qh;
-    const float lse = live ? a.lse[place] : 0.0f, delta = live ? a.delta[place] : 0.0f;
-    const float base = lse == -__builtin_inff() ? lse : -lse;  // (a row that sees nothing: weights of zero)
+    const float base = live ? a.base[place] - (float)kPShift<T> : 0.0f, delta = live ? a.delta[place] : 0.0f;
     const float norm = kHalf && live ? a.norm[place] : 0.0f;
     const float *const v_norm = kHalf ? a.v_norm + ((size_t)(packed ? 0 : b) * lk + k0) * a.s.kv_heads + head : nullptr;
 
     const uint32_t last_row = min(rows, (tile + 1) * kOwn) - 1;
-    const uint32_t all = (seen_by(last_row / a.s.group) + R - 1) / R, each = (all + a.q_parts - 1) / a.q_parts;
+    const uint32_t all = (seen_by(fast_div(last_row, a.s.by_group)) + R - 1) / R, each = (all + a.q_parts - 1) / a.q_parts;
     const uint32_t t0 = min(all, part * each), t1 = min(all, t0 + each);
     const uint32_t wave_row = tile * kOwn + wave * 32;
-    const uint32_t wave_limit = wave_row < rows ? seen_by(min(rows - 1, wave_row + 31) / a.s.group) : 0;
-    const uint32_t wave_full = wave_row < rows ? seen_by(wave_row / a.s.group) : 0;
+    const uint32_t wave_limit = wave_row < rows ? seen_by(fast_div(min(rows - 1, wave_row + 31), a.s.by_group)) : 0;
+    const uint32_t wave_full = wave_row < rows ? seen_by(fast_div(wave_row, a.s.by_group)) : 0;
 
     uint32_t k_base[KvTile::kTurn], v_base[KvTile::kTurn];
     const uint32_t k_row = (uint32_t)a.k.row, v_row = (uint32_t)a.v.row;
@@ -298,7 +272,7 @@ __device__ __forceinline__ void attn_grad_q(const Backward &a, const uint32_t bl
     }
     uint32_t thread = threadIdx.x;  // (the row's number is formed again: over the loop there is no register for it)
     asm volatile("" : "+v"(thread));
-    const uint32_t own_row = tile * kOwn + thread / kWave * 32 + thread % 32, own_i = own_row / a.s.group;
+    const uint32_t own_row = tile * kOwn + thread / kWave * 32 + thread % 32, own_i = fast_div(own_row, a.s.by_group);
     if (own_row >= rows) return;
     T *const to = static_cast<T *>(const_cast<void *>(a.dq.at)) + (packed ? 0 : b * a.dq.batch) + (size_t)(q0 + own_i) * a.dq.row +
                   (head * a.s.group + own_row - own_i * a.s.group) * a.dq.head;
@@ -326,7 +300,7 @@ struct ForKv {
     static constexpr bool kVInLds = !Frag<T>::kFloat && D == 128;
     static constexpr int kRows = D == 128 ? 32 : Frag<T>::kTile;  // (64 rows of 128 columns on their way leave too few registers)
     Tile<T, D, WAVES, kRows> tiles[2][2];  // [buffer][Q, dO]
-    float stats[2][3][kRows];              // [buffer][- log2 sum, D, |do|]
+    float stats[2][3][kRows];              // [buffer][base, D, |do|]
     typename KeptValues<T, D, WAVES, kVInLds>::type values;
 };
 template <typename T, int D, int WAVES>
@@ -338,15 +312,16 @@ __device__ __forceinline__ void attn_grad_kv(const Backward &a, const uint32_t b
     constexpr bool kHalf = !Frag<T>::kFloat;
     constexpr int R = RowTile::kRows, KD = D / 16, DB = D / 32;
     constexpr bool kVInLds = ForKv<T, D, WAVES>::kVInLds;
+    constexpr int kAtOnce = D == 64 ? DB : 1;  // column blocks whose operands are read, and looked through, at once
     RowTile(&tiles)[2][2] = lds.tiles;
     float(&stats)[2][3][R] = lds.stats;
     auto &values = lds.values;
     const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, h = lane / 32;
     const TileLanes<T, D> lanes;
-    const uint32_t head = block % a.s.kv_heads;
+    const uint32_t rest = fast_div(block, a.s.by_kv_heads), head = block - rest * a.s.kv_heads;
+    const uint32_t tiles_at = a.parts == 1 ? rest : rest / a.parts, part = rest - tiles_at * a.parts;
     uint32_t b, tile, q0, lq, k0, lk;
-    if (!find_tile(a.s.k_offsets, a.s.batch, a.s.k_rows, 1, kOwn, block / a.s.kv_heads / a.parts, a.s.k_by_tile, b, tile)) return;
-    const uint32_t part = block / a.s.kv_heads % a.parts;
+    if (!find_tile(a.s.k_offsets, a.s.batch, a.s.k_rows, 1, kOwn, tiles_at, a.s.k_by_tile, b, tile)) return;
     span_of_all(a.s.q_offsets, b, a.s.q_rows, q0, lq);
     span_of_all(a.s.k_offsets, b, a.s.k_rows, k0, lk);
     const bool packed = a.s.q_offsets != nullptr;
@@ -394,16 +369,15 @@ __device__ __forceinline__ void attn_grad_kv(const Backward &a, const uint32_t b
     const uint32_t from_tile = min(first_row(tile * kOwn), rows) / R, all = (rows + R - 1) / R - from_tile;
     const uint32_t each = (all + a.parts - 1) / a.parts, t0 = from_tile + min(all, part * each), t1 = min(from_tile + all, t0 + each);
 
-    float next_stat[3] = {0.0f, 0.0f, 0.0f};
     auto fetch = [&](uint32_t t, uint32_t buffer) {
-        const uint32_t i0 = t * R / a.s.group;  // the query of the tile's first row
+        const uint32_t i0 = fast_div(t * R, a.s.by_group);  // the query of the tile's first row
         const T *const q = qbase + (size_t)i0 * a.q.row, *const g = gbase + (size_t)i0 * a.dout.row;
-        const uint32_t last = min(rows, (t + 1) * R) - 1, n = last / a.s.group - i0;
+        const uint32_t last = min(rows, (t + 1) * R) - 1, n = fast_div(last, a.s.by_group) - i0;
         if (a.vec) {
             uint32_t q_offset[RowTile::kPerThread], g_offset[RowTile::kPerThread];
 #pragma unroll
             for (int p = 0; p < RowTile::kPerThread; p++) {
-                const uint32_t r = t * R + RowTile::row_of(p), d = RowTile::column_of(p), i = fast_div(r, a.by_group), gh = r - i * a.s.group;
+                const uint32_t r = t * R + RowTile::row_of(p), d = RowTile::column_of(p), i = fast_div(r, a.s.by_group), gh = r - i * a.s.group;
                 const bool in = r < rows && d < a.s.dim;
                 q_offset[p] = in ? (uint32_t)(((i - i0) * a.q.row + gh * a.q.head + d) * sizeof(T)) : kNowhere;
                 g_offset[p] = in ? (uint32_t)(((i - i0) * a.dout.row + gh * a.dout.head + d) * sizeof(T)) : kNowhere;
@@ -414,27 +388,20 @@ __device__ __forceinline__ void attn_grad_kv(const Backward &a, const uint32_t b
         } else {
             auto from = [&](const T *base, const AttnView &v) {
                 return [=](uint32_t r) -> const T * {
-                    const uint32_t i = (t * R + r) / a.s.group, gh = t * R + r - i * a.s.group;
+                    const uint32_t i = fast_div(t * R + r, a.s.by_group), gh = t * R + r - i * a.s.group;
                     return t * R + r < rows ? base + (i - i0) * v.row + gh * v.head : nullptr;
                 };
             };
             tiles[buffer][0].copy(from(q, a.q), a.s.dim);
             tiles[buffer][1].copy(from(g, a.dout), a.s.dim);
         }
-        if (threadIdx.x < R) {
-            const uint32_t r = t * R + threadIdx.x, i = fast_div(r, a.by_group);
-            const bool in = r < rows;
-            const size_t at = place0 + (size_t)i * a.s.heads + (r - i * a.s.group);
-            const float lse = in ? a.lse[at] : -__builtin_inff();
-            next_stat[0] = lse == -__builtin_inff() ? lse : (float)kPShift<T> - lse;  // (rows that see nothing: weights of zero)
-            next_stat[1] = in ? a.delta[at] : 0.0f;
-            if (kHalf) next_stat[2] = in ? a.norm[at] : 0.0f;
-        }
-    };
-    auto put = [&](uint32_t buffer) {  // (what the next tile's rows have beside their values)
-        if (threadIdx.x < R) {
-#pragma unroll
-            for (int i = 0; i < 3; i++) stats[buffer][i][threadIdx.x] = next_stat[i];
+        if (threadIdx.x < R) {  // (rows behind the last have zeros, as in the tiles: nothing comes of them)
+            const uint32_t r = t * R + threadIdx.x, i = fast_div(r, a.s.by_group), at = (i - i0) * a.s.heads + r - i * a.s.group;
+            const size_t from = place0 + (size_t)i0 * a.s.heads;
+            const uint32_t bytes = (n * a.s.heads + a.s.group) * (uint32_t)sizeof(float), offset = r < rows ? at * (uint32_t)sizeof(float) : kNowhere;
+            request_floats(stats[buffer][0], a.base + from, bytes, offset);
+            request_floats(stats[buffer][1], a.delta + from, bytes, offset);
+            if (kHalf) request_floats(stats[buffer][2], a.norm + from, bytes, offset);
         }
     };
     const bool few = kHalf && few_terms(lq, lk, a.s.dim);
@@ -442,10 +409,7 @@ __device__ __forceinline__ void attn_grad_kv(const Backward &a, const uint32_t b
 #pragma unroll
     for (int d = 0; d < DB; d++) dk[d] = dv[d] = zero16();
     DsScale scale;
-    if (t0 < t1) {
-        fetch(t0, 0);
-        put(0);
-    }
+    if (t0 < t1) fetch(t0, 0);
     for (uint32_t t = t0; t < t1; t++) {
         wait_tiles();
         __syncthreads();
@@ -458,14 +422,15 @@ __device__ __forceinline__ void attn_grad_kv(const Backward &a, const uint32_t b
                 float by = 1.0f;
                 bool odd = false;
                 if (kHalf) {
-                    float down, norms = stats[buffer][2][lane % R], deltas = fabsf(stats[buffer][1][lane % R]);
+                    // (the tile's rows from the last to the first, one to a lane)
+                    float down, norms = stats[buffer][2][R - 1 - lane % R], deltas = fabsf(stats[buffer][1][R - 1 - lane % R]);
                     if constexpr (MASKED) {
-                        norms = max_from(lane < R ? norms : 0.0f);
-                        deltas = max_from(lane < R ? deltas : 0.0f);
-                        const uint32_t behind = from > first ? min(from - first, (uint32_t)R) : 0;  // the tile's rows that do not see the key
-                        norms = __shfl(norms, (int)min(behind, (uint32_t)R - 1), kWave);
-                        deltas = __shfl(deltas, (int)min(behind, (uint32_t)R - 1), kWave);
-                        if (behind == R) norms = deltas = 0.0f;
+                        norms = max_up_to(norms);
+                        deltas = max_up_to(deltas);
+                        const uint32_t seeing = from > first ? R - min(from - first, (uint32_t)R) : R;  // rows that see the key
+                        norms = __shfl(norms, (int)max(seeing, 1u) - 1, kWave);
+                        deltas = __shfl(deltas, (int)max(seeing, 1u) - 1, kWave);
+                        if (seeing == 0) norms = deltas = 0.0f;
                     } else {
                         norms = team_max<64>(norms);
                         deltas = team_max<64>(deltas);
@@ -517,14 +482,19 @@ __device__ __forceinline__ void attn_grad_kv(const Backward &a, const uint32_t b
 #pragma unroll
                     for (int u = 0; u < 2; u++) {
 #pragma unroll
-                        for (int d = 0; d < DB; d++) {
-                            frag gc[1] = {gt.columns(lanes, 32 * n + 16 * u, d)}, qc[1] = {qt.columns(lanes, 32 * n + 16 * u, d)};
-                            if constexpr (MASKED) {
-                                leave_out_odd<1>(gc, odd);
-                                leave_out_odd<1>(qc, odd);
+                        for (int d0 = 0; d0 < DB; d0 += kAtOnce) {
+                            frag c[2 * kAtOnce];
+#pragma unroll
+                            for (int d = 0; d < kAtOnce; d++) {
+                                c[2 * d] = gt.columns(lanes, 32 * n + 16 * u, d0 + d);
+                                c[2 * d + 1] = qt.columns(lanes, 32 * n + 16 * u, d0 + d);
                             }
-                            dv[d] = mma(gc[0], p[u], dv[d]);
-                            dk[d] = mma(qc[0], ds[u], dk[d]);
+                            if constexpr (MASKED) leave_out_odd<2 * kAtOnce>(c, odd);
+#pragma unroll
+                            for (int d = 0; d < kAtOnce; d++) {
+                                dv[d0 + d] = mma(c[2 * d], p[u], dv[d0 + d]);
+                                dk[d0 + d] = mma(c[2 * d + 1], ds[u], dk[d0 + d]);
+                            }
                             step_end<Frag<T>::kFloat || D == 128>();
                         }
                     }
@@ -533,10 +503,13 @@ __device__ __forceinline__ void attn_grad_kv(const Backward &a, const uint32_t b
                         for (int u = 0; u < 2; u++) {
                             to_frag(dp, u, ds[u]);
 #pragma unroll
-                            for (int d = 0; d < DB; d++) {
-                                frag qc[1] = {qt.columns(lanes, 32 * n + 16 * u, d)};
-                                leave_out_odd<1>(qc, odd);
-                                dk[d] = mma(qc[0], ds[u], dk[d]);
+                            for (int d0 = 0; d0 < DB; d0 += kAtOnce) {
+                                frag c[kAtOnce];
+#pragma unroll
+                                for (int d = 0; d < kAtOnce; d++) c[d] = qt.columns(lanes, 32 * n + 16 * u, d0 + d);
+                                leave_out_odd<kAtOnce>(c, odd);
+#pragma unroll
+                                for (int d = 0; d < kAtOnce; d++) dk[d0 + d] = mma(c[d], ds[u], dk[d0 + d]);
                                 step_end<D == 128>();
                             }
                         }
@@ -553,7 +526,6 @@ __device__ __forceinline__ void attn_grad_kv(const Backward &a, const uint32_t b
             else
                 work(std::false_type{});
         }
-        if (t + 1 < t1) put((t + 1 - t0) & 1);
     }
     uint32_t thread = threadIdx.x;  // (the key's number is formed again: over the loop there is no register for it)
     asm volatile("" : "+v"(thread));
@@ -653,7 +625,7 @@ struct Room {
 };
 Room room_of(const AttnProblem &p) {
     const size_t rows = p.q_offsets == nullptr ? p.batch * p.q_rows : p.q_rows, keys = p.k_offsets == nullptr ? p.batch * p.k_rows : p.k_rows;
-    return Room{(2 * rows * p.heads + keys * p.kv_heads + 3) / 4 * 4, (keys * p.kv_heads * 2 * p.dim + 3) / 4 * 4, (rows * p.heads * p.dim + 3) / 4 * 4};
+    return Room{(3 * rows * p.heads + keys * p.kv_heads + 3) / 4 * 4, (keys * p.kv_heads * 2 * p.dim + 3) / 4 * 4, (rows * p.heads * p.dim + 3) / 4 * 4};
 }
 
 }  // namespace
@@ -677,7 +649,7 @@ template <typename T>
 int attn_grad_dispatch(const AttnProblem &p, const AttnGradViews &g, const float *lse, const void *rest, void *workspace, size_t workspace_bytes,
                        hipStream_t stream) {
     const size_t rows = p.q_offsets == nullptr ? p.batch * p.q_rows : p.q_rows, keys = p.k_offsets == nullptr ? p.batch * p.k_rows : p.k_rows;
-    float *const delta = static_cast<float *>(workspace);
+    float *const base = static_cast<float *>(workspace), *const delta = base + rows * p.heads;
     constexpr bool kHalf = !Frag<T>::kFloat;
     // no more parts than the workspace holds, those of dk and dv first
     const Room r = room_of(p);
@@ -685,11 +657,11 @@ int attn_grad_dispatch(const AttnProblem &p, const AttnGradViews &g, const float
     const uint32_t parts = (uint32_t)std::max<size_t>(1, std::min<size_t>(row_parts(p), left / std::max<size_t>(1, r.part)));
     if (parts > 1) left -= parts * r.part;
     const uint32_t q_parts = (uint32_t)std::max<size_t>(1, std::min<size_t>(dq_parts(p), left / std::max<size_t>(1, r.q_part)));
-    float *const part = delta + r.vectors, *const q_part = part + (parts > 1 ? parts * r.part : 0);
-    const Backward a{attn_shape(p), g.q, g.k, g.v, g.out, g.dout, g.dq, g.dk, g.dv, lse, rest, delta,
+    float *const part = base + r.vectors, *const q_part = part + (parts > 1 ? parts * r.part : 0);
+    const Backward a{attn_shape(p), g.q, g.k, g.v, g.out, g.dout, g.dq, g.dk, g.dv, lse, rest, base, delta,
                      kHalf ? delta + rows * p.heads : nullptr, kHalf ? delta + 2 * rows * p.heads : nullptr, part, q_part, (uint32_t)rows, (uint32_t)keys, parts, q_parts,
                      (uint32_t)(tiles_of_keys(p) * p.kv_heads * parts),
-                     make_fast_div((uint32_t)(p.heads / p.kv_heads)), attn_vectors(sizeof(T), p, {g.q, g.k, g.v, g.out, g.dout, g.dq, g.dk, g.dv, AttnView{rest, 0, 0, 0}})};
+                     attn_vectors(sizeof(T), p, {g.q, g.k, g.v, g.out, g.dout, g.dq, g.dk, g.dv, AttnView{rest, 0, 0, 0}})};
     const size_t items = rows * p.heads + (kHalf ? keys * p.kv_heads : 0);
     if (items != 0)
         launch((attn_grad_rows_kernel<T>), dim3((uint32_t)((items + 15) / 16)), dim3(kAttnThreads), 0, stream, a);

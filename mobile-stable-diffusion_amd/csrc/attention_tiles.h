@@ -183,11 +183,10 @@ __device__ __forceinline__ void add_odd(const Tile &tile, const TileLanes<T, D> 
     }
 }
 
-// 16 bytes of a row from column d on, zeros behind its end.  vec: rows are whole aligned 16-byte vectors.
+// 16 bytes of a row from column d on, zeros behind its end, for rows that are no whole aligned vectors.
 template <typename T>
-__device__ __forceinline__ u32x4 load_chunk(const T *row, uint32_t d, uint32_t dim, bool vec) {
+__device__ __forceinline__ u32x4 load_chunk(const T *row, uint32_t d, uint32_t dim) {
     constexpr int E = 16 / sizeof(T);
-    if (vec) return d < dim ? *reinterpret_cast<const u32x4 *>(row + d) : u32x4{0, 0, 0, 0};
     T v[E];
 #pragma unroll
     for (int e = 0; e < E; e++) v[e] = d + e < dim ? row[d + e] : T(0.0f);
@@ -200,14 +199,23 @@ __device__ __forceinline__ u32x4 load_chunk(const T *row, uint32_t d, uint32_t d
 template <typename T, int D>
 __device__ __forceinline__ void load_frags(const T *row, uint32_t dim, bool vec, typename Frag<T>::operand (&f)[D / 16]) {
     const uint32_t h = threadIdx.x % kWave / 32;
+    constexpr uint32_t kPer = sizeof(T) / 2, E = 16 / sizeof(T);  // chunks of a fragment, elements of a chunk
+    u32x4 v[D / 16 * kPer];
+    if (vec) {
+#pragma unroll
+        for (uint32_t c = 0; c < D / 16 * kPer; c++) {
+            const uint32_t d = 16 * (c / kPer) + 8 * h + c % kPer * E;
+            v[c] = row != nullptr && d < dim ? *reinterpret_cast<const u32x4 *>(row + d) : u32x4{0, 0, 0, 0};
+        }
+    } else {
+#pragma unroll
+        for (uint32_t c = 0; c < D / 16 * kPer; c++)
+            v[c] = row != nullptr ? load_chunk<T>(row, 16 * (c / kPer) + 8 * h + c % kPer * E, dim) : u32x4{0, 0, 0, 0};
+    }
 #pragma unroll
     for (int k = 0; k < D / 16; k++) {
-        u32x4 v[sizeof(T) / 2];
-#pragma unroll
-        for (uint32_t i = 0; i < sizeof(T) / 2; i++)
-            v[i] = row != nullptr ? load_chunk<T>(row, 16 * k + 8 * h + i * (16 / sizeof(T)), dim, vec) : u32x4{0, 0, 0, 0};
         typename Frag<T>::type one;
-        __builtin_memcpy(&one, v, sizeof(one));
+        __builtin_memcpy(&one, v + k * kPer, sizeof(one));
         f[k] = operand(one);
     }
 }
@@ -216,6 +224,22 @@ constexpr uint32_t kNowhere = 0x80000000u;  // an offset behind the end of any r
 
 // Until what Tile::request asked for is in LDS (this wavefront's part; a barrier makes it everyone's).
 __device__ __forceinline__ void wait_tiles() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+__device__ __forceinline__ u32x4 buffer_resource(const void *from, uint32_t bytes) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(from);
+    return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)at), (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(at >> 32)),
+                 (uint32_t)__builtin_amdgcn_readfirstlane(bytes), 0x00020000u};
+}
+// A float of each lane straight from memory, `offset` bytes behind `from`, to one place after the other of LDS; as Tile::request.
+__device__ __forceinline__ void request_floats(float *lds, const void *from, uint32_t bytes, uint32_t offset) {
+    const u32x4 resource = buffer_resource(from, bytes);
+    const uint32_t to = __builtin_amdgcn_readfirstlane((uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char *)lds));
+    uint32_t m0;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dword %2, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
+                 : "=&s"(m0)
+                 : "s"(to), "v"(offset), "s"(resource)
+                 : "memory");
+}
 
 // Where a lane reads in a tile (below), in bytes from its beginning.  The places differ by more than a constant only in the three
 // bits of the chunk's number that the row's number goes into: a few registers, and the rest is in the instructions.
@@ -267,9 +291,7 @@ struct Tile {
     // the compiler, which knows no more than that these write LDS, would wait for them in front of every read by columns.
     template <typename Offset>
     __device__ __forceinline__ void request(const void *from, uint32_t bytes, Offset offset) {
-        const uintptr_t at = reinterpret_cast<uintptr_t>(from);
-        const u32x4 resource = {(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)at), (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(at >> 32)),
-                                (uint32_t)__builtin_amdgcn_readfirstlane(bytes), 0x00020000u};
+        const u32x4 resource = buffer_resource(from, bytes);
         const uint32_t first = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) * kWave;
         const uint32_t lds = __builtin_amdgcn_readfirstlane(
             (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char *)data) + first * 16);
@@ -288,7 +310,7 @@ struct Tile {
 #pragma unroll 1
         for (int p = 0; p < kPerThread; p++) {
             const T *const from = row(row_of(p));
-            data[p * kThreads + threadIdx.x] = from != nullptr ? load_chunk<T>(from, column_of(p), dim, false) : u32x4{0, 0, 0, 0};
+            data[p * kThreads + threadIdx.x] = from != nullptr ? load_chunk<T>(from, column_of(p), dim) : u32x4{0, 0, 0, 0};
         }
     }
 
@@ -330,6 +352,49 @@ struct Tile {
     }
 };
 
+// a b in float32.  (Left to itself the compiler joins some of these with the rounding to float16 that follows, and other alignments
+// have other bits.)
+__device__ __forceinline__ float rounded_product(float a, float b) {
+    float v = a * b;
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
+// Stores an accumulator's columns: row `to` gets the lane's column times `by`; `left`, if not null, what rounding took from it.
+template <typename T, int D>
+__device__ __forceinline__ void store_rows(T *to, const f32x16 (&acc)[D / 32], float by, uint32_t dim, bool vec, T *left = nullptr) {
+    const uint32_t h = threadIdx.x % kWave / 32;
+    if (vec) {
+#pragma unroll
+        for (int d = 0; d < D / 32; d++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const uint32_t col = 32 * d + 8 * g + 4 * h;
+                T v[4], l[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const float value = rounded_product(acc[d][4 * g + j], by);
+                    Store<T>::store1(v + j, value);
+                    Store<T>::store1(l + j, value - Store<T>::load1(v + j));
+                }
+                if (col >= dim) continue;
+                __builtin_memcpy(__builtin_assume_aligned(to + col, 4 * sizeof(T)), v, sizeof(v));
+                if (left != nullptr) __builtin_memcpy(__builtin_assume_aligned(left + col, 4 * sizeof(T)), l, sizeof(l));
+            }
+        return;
+    }
+#pragma unroll
+    for (int d = 0; d < D / 32; d++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+            const uint32_t col = 32 * d + 8 * (r / 4) + 4 * h + r % 4;
+            if (col >= dim) continue;
+            const float value = rounded_product(acc[d][r], by);
+            Store<T>::store1(to + col, value);
+            if (left != nullptr) Store<T>::store1(left + col, value - round_to_storage<T>(value));
+        }
+}
+
 // Maximum with the lane of the other half.
 __device__ __forceinline__ float halves_max(float v) { return fmaxf(v, half_swap(v)); }
 
@@ -337,6 +402,7 @@ struct AttnShape {
     const int32_t *q_offsets, *k_offsets;  // [batch + 1] or null: sequences of equal length
     uint32_t batch, q_rows, k_rows;        // rows of all sequences (of one, without offsets)
     uint32_t heads, kv_heads, group, dim;
+    FastDiv by_group, by_kv_heads;
     float scale2;  // scale * log2(e)
     bool causal;
     // Order of equal sequences' tiles.  Tile by tile (of all sequences, the longest first) where the work of tiles differs and a
