@@ -449,8 +449,8 @@ int msd_softmax(const void *x, void *y, size_t rows, size_t cols, int stable, in
  *   q, out [batch][q_rows][heads][dim], k, v [batch][k_rows][kv_heads][dim] in the storage type, dim from 1 to 128, heads a
  *   multiple of kv_heads: heads / kv_heads neighbouring query heads share a key head.
  *   strides: host array of (batch, row, head) strides in elements for q, k, v, out in turn (the values of a head lie together),
- *   or NULL: as listed, without gaps.  Views of one projection are fine, also for outputs: one is apart from an input or from another
- *   output too where both have the same batch and row strides and their heads lie beside each other in a row.
+ *   or NULL: as listed, without gaps.  Views of one projection are fine, also for outputs: one is apart from an input or
+ *   from another output too where, modulo one of their strides, they reach over different bytes.
  *   Packed sequences: q_offsets and k_offsets, device arrays of batch + 1 ascending int32 (both or neither): sequence b has
  *   the rows offsets[b] ... offsets[b + 1] - 1; q_rows and k_rows are then all rows, batch strides do not count, and rows
  *   of no sequence stay as they were.  Lengths may be zero and differ between queries and keys.  Offsets are read on the device:

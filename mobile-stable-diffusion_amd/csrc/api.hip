@@ -872,11 +872,10 @@ static AttnProblem attention_problem(const int32_t *q_offsets, const int32_t *k_
     return AttnProblem{q_offsets, k_offsets, batch, q_rows, k_rows, heads, kv_heads, dim, scale, causal != 0};
 }
 
-// A strided tensor of an attention call: its view, and from where to where it reaches.
+// A strided tensor of an attention call: its view, its strides, how far each axis reaches, a head's values and the whole in bytes.
 struct Strided {
     AttnView view;
-    size_t heads_bytes, row_bytes, bytes;  // heads of a row from the first value to the last; stride of rows; the whole tensor
-    size_t batch_bytes;
+    size_t stride[3], reach[3], head_bytes, bytes;
 };
 
 static bool make_strided(const void *at, size_t batch, size_t rows, size_t heads, size_t dim, size_t elt, bool packed, const size_t *strides,
@@ -888,7 +887,7 @@ static bool make_strided(const void *at, size_t batch, size_t rows, size_t heads
     const size_t counts[3] = {batch, rows, heads};
     for (int i = 0; i < 3; i++)
         if (counts[i] <= 1) s[i] = 0;  // (the stride of a single one is never taken)
-    *to = Strided{AttnView{at, s[0], s[1], s[2]}, 0, s[1] * elt, 0, s[0] * elt};
+    *to = Strided{AttnView{at, s[0], s[1], s[2]}, {}, {}, dim * elt, 0};
     if (batch == 0 || rows == 0 || heads == 0) return true;
     if (at == nullptr) return false;
     size_t reach[3], end = dim;
@@ -896,8 +895,9 @@ static bool make_strided(const void *at, size_t batch, size_t rows, size_t heads
         if (s[i] > (SIZE_MAX >> 4) || __builtin_mul_overflow(s[i], counts[i] - 1, &reach[i]) || reach[i] > (SIZE_MAX >> 4) ||
             __builtin_add_overflow(end, reach[i], &end) || end > (SIZE_MAX >> 4))
             return false;
+        to->stride[i] = s[i] * elt;
+        to->reach[i] = reach[i] * elt;
     }
-    to->heads_bytes = (reach[2] + dim) * elt;
     to->bytes = end * elt;
     if (!output) return true;
     // an output's values are all different ones: taken by size, each stride passes what the smaller ones reach
@@ -911,15 +911,23 @@ static bool make_strided(const void *at, size_t batch, size_t rows, size_t heads
     return true;
 }
 
+// Whether two tensors share no value: their ranges are apart, or the ranges modulo one of their strides are (views of one
+// projection, whose rows or sequences lie between each other's).
 static bool strided_apart(const Strided &a, const Strided &b) {
     if (a.bytes == 0 || b.bytes == 0 || !ranges_overlap(a.view.at, a.bytes, b.view.at, b.bytes)) return true;
-    if (a.row_bytes != b.row_bytes || a.row_bytes == 0) return false;
-    if (a.batch_bytes != b.batch_bytes && a.batch_bytes != 0 && b.batch_bytes != 0) return false;
-    // every row of one lies in the gaps between the rows of the other
     const Strided &low = a.view.at < b.view.at ? a : b, &high = a.view.at < b.view.at ? b : a;
-    const size_t step = (const char *)high.view.at - (const char *)low.view.at;
-    return low.heads_bytes <= step && step + high.heads_bytes <= low.row_bytes &&
-           (low.batch_bytes == 0 || low.batch_bytes % low.row_bytes == 0) && (high.batch_bytes == 0 || high.batch_bytes % high.row_bytes == 0);
+    const size_t apart = (const char *)high.view.at - (const char *)low.view.at;
+    for (int i = 0; i < 6; i++) {
+        const size_t step = i < 3 ? a.stride[i] : b.stride[i - 3];
+        if (step == 0) continue;
+        size_t low_bytes = low.head_bytes, high_bytes = high.head_bytes;
+        for (int j = 0; j < 3; j++) {
+            low_bytes += low.stride[j] % step != 0 ? low.reach[j] : 0;
+            high_bytes += high.stride[j] % step != 0 ? high.reach[j] : 0;
+        }
+        if (low_bytes <= apart % step && high_bytes <= step - apart % step) return true;
+    }
+    return false;
 }
 
 int msd_attention_workspace(size_t batch, size_t q_rows, size_t k_rows, size_t heads, size_t kv_heads, size_t dim, int packed, int backward,
