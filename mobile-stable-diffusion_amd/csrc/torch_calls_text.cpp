@@ -119,6 +119,7 @@ PyObject *token_embedding_backward(PyObject *, Args a, Py_ssize_t n) {  // dy, i
         if (!c.ok || !here(*dy) || dy->dim() != ids->dim() + 1 || dy->sizes().slice(0, ids->dim()) != ids->sizes() || vocab < 0 || positions < 0)
             return nullptr;
         const int64_t dim = dy->size(-1), tokens = ids->numel(), length = ids->size(-1);
+        if (positions != 0 && positions < length) return nullptr;
         size_t bytes = 0;
         if (abi.msd_token_embedding_backward_workspace(tokens, length, vocab, positions, dim, code, &bytes) != 0) return nullptr;
         const at::Tensor workspace = new_tensor({(int64_t)bytes}, at::kByte, *dy);
