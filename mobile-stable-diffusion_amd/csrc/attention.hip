@@ -142,20 +142,26 @@ __global__ __launch_bounds__(WAVES *kWave, Frag<T>::kFloat || WAVES == 1 ? 1 : 2
                         s[n][r] = __builtin_amdgcn_exp2f(fmaf(s[n][r], a.s.scale2, base));
                         sum += s[n][r];
                     }
+                if constexpr (Frag<T>::kFloat) {
+                    operand_t p[2];
+                    to_frag(s[0], 0, p[0]);
+                    to_frag(s[0], 1, p[1]);
+                    add_products<MASKED, true, T, D>(vt, lanes, p, o, odd);
+                } else {
 #pragma unroll
-                for (int n = 0; n < R / 32; n++)
+                    for (int n = 0; n < R / 32; n++)
 #pragma unroll
-                    for (int u = 0; u < 2; u++) {
-                        operand_t p;
-                        to_frag(s[n], u, p);
-                        frag v[DB];
+                        for (int u = 0; u < 2; u++) {
+                            operand_t p;
+                            to_frag(s[n], u, p);
+                            frag v[DB];
 #pragma unroll
-                        for (int d = 0; d < DB; d++) v[d] = vt.columns(lanes, 32 * n + 16 * u, d);
-                        if constexpr (MASKED) leave_out_odd<DB>(v, odd);
+                            for (int d = 0; d < DB; d++) v[d] = vt.columns(lanes, 32 * n + 16 * u, d);
+                            if constexpr (MASKED) leave_out_odd<DB>(v, odd);
 #pragma unroll
-                        for (int d = 0; d < DB; d++) o[d] = mma(v[d], p, o[d]);
-                        step_end<Frag<T>::kFloat>();
-                    }
+                            for (int d = 0; d < DB; d++) o[d] = mma(v[d], p, o[d]);
+                        }
+                }
                 if (MASKED && odd) add_odd<T, D, R>(vt, lanes, o, [&](uint32_t r) { return first + r < limit; });
             };
             if (first + R > wave_full)

@@ -246,20 +246,30 @@ __device__ __forceinline__ void attn_grad_q(const Backward &a, const uint32_t bl
                         for (int r = 0; r < 16; r++)
                             if (first + 32 * n + 8 * (r / 4) + 4 * h + r % 4 >= limit) s[r] = 0.0f;
                     }
+                    if constexpr (Frag<T>::kFloat) {
+                        operand_t ds[2];
+                        to_frag(s, 0, ds[0]);
+                        to_frag(s, 1, ds[1]);
+                        add_products<MASKED, true, T, D>(kt, lanes, ds, dq, odd);
+                        continue;
+                    }
 #pragma unroll
-                    for (int u = 0; u < (MASKED && kHalf ? 4 : 2); u++) {
-                        operand_t ds;
-                        to_frag(s, u % 2, ds);
-                        if constexpr (MASKED && kHalf) {  // (a second time with what the rounding took away)
-                            if (u < 2) left_by(ds, u, s);
+                    for (int u = 0; u < 2; u++) {
+                        operand_t ds[MASKED ? 2 : 1];
+                        to_frag(s, u, ds[0]);
+                        if constexpr (MASKED) {  // (and what the rounding took away)
+                            left_by(ds[0], u, s);
+                            to_frag(s, u, ds[1]);
                         }
                         frag k[DB];
 #pragma unroll
-                        for (int d = 0; d < DB; d++) k[d] = kt.columns(lanes, 32 * n + 16 * (u % 2), d);
+                        for (int d = 0; d < DB; d++) k[d] = kt.columns(lanes, 32 * n + 16 * u, d);
                         if constexpr (MASKED) leave_out_odd<DB>(k, odd);
 #pragma unroll
-                        for (int d = 0; d < DB; d++) dq[d] = mma(k[d], ds, dq[d]);
-                        step_end<Frag<T>::kFloat || D == 128>();
+                        for (const operand_t &w : ds)
+#pragma unroll
+                            for (int d = 0; d < DB; d++) dq[d] = mma(k[d], w, dq[d]);
+                        step_end<D == 128>();
                     }
                 }
                 if (MASKED && odd) add_odd<T, D, R>(kt, lanes, dq, [&](uint32_t r) { return first + r < limit; });
@@ -322,6 +332,8 @@ __device__ __forceinline__ void attn_grad_kv(const Backward &a, const uint32_t b
     const uint32_t tiles_at = a.parts == 1 ? rest : rest / a.parts, part = rest - tiles_at * a.parts;
     uint32_t b, tile, q0, lq, k0, lk;
     if (!find_tile(a.s.k_offsets, a.s.batch, a.s.k_rows, 1, kOwn, tiles_at, a.s.k_by_tile, b, tile)) return;
+    b = __builtin_amdgcn_readfirstlane(b);
+    tile = __builtin_amdgcn_readfirstlane(tile);
     span_of_all(a.s.q_offsets, b, a.s.q_rows, q0, lq);
     span_of_all(a.s.k_offsets, b, a.s.k_rows, k0, lk);
     const bool packed = a.s.q_offsets != nullptr;
@@ -468,50 +480,52 @@ __device__ __forceinline__ void attn_grad_kv(const Backward &a, const uint32_t b
                         for (int r = 0; r < 16; r++)
                             if (first + 32 * n + 8 * (r / 4) + 4 * h + r % 4 < from) s[r] = dp[r] = 0.0f;
                     }
-                    operand_t p[2], ds[2];
+                    if constexpr (Frag<T>::kFloat) {
+                        operand_t w[2];
+                        to_frag(s, 0, w[0]);
+                        to_frag(s, 1, w[1]);
+                        add_products<MASKED, D == 64, T, D>(gt, lanes, w, dv, odd);
+                        to_frag(dp, 0, w[0]);
+                        to_frag(dp, 1, w[1]);
+                        add_products<MASKED, D == 64, T, D>(qt, lanes, w, dk, odd);
+                        continue;
+                    }
+                    constexpr int kTimes = MASKED ? 4 : 2;  // (two more are what the rounding took away)
+                    operand_t p[kTimes], ds[kTimes];
 #pragma unroll
-                    for (int u = 0; u < 2; u++) {
-                        to_frag(s, u, p[u]);
-                        to_frag(dp, u, ds[u]);
+                    for (int u = 0; u < kTimes; u++) {
+                        to_frag(s, u % 2, p[u]);
+                        to_frag(dp, u % 2, ds[u]);
                         if constexpr (MASKED) {
                             keep_here(p[u]);
                             keep_here(ds[u]);
-                            if constexpr (kHalf) left_by(ds[u], u, dp);
+                            if (u < 2) {
+                                left_by(p[u], u, s);
+                                left_by(ds[u], u, dp);
+                            }
                         }
                     }
 #pragma unroll
                     for (int u = 0; u < 2; u++) {
 #pragma unroll
                         for (int d0 = 0; d0 < DB; d0 += kAtOnce) {
-                            frag c[2 * kAtOnce];
+                            frag c[kAtOnce];
 #pragma unroll
-                            for (int d = 0; d < kAtOnce; d++) {
-                                c[2 * d] = gt.columns(lanes, 32 * n + 16 * u, d0 + d);
-                                c[2 * d + 1] = qt.columns(lanes, 32 * n + 16 * u, d0 + d);
-                            }
-                            if constexpr (MASKED) leave_out_odd<2 * kAtOnce>(c, odd);
+                            for (int d = 0; d < kAtOnce; d++) c[d] = gt.columns(lanes, 32 * n + 16 * u, d0 + d);
+                            if constexpr (MASKED) leave_out_odd<kAtOnce>(c, odd);
 #pragma unroll
-                            for (int d = 0; d < kAtOnce; d++) {
-                                dv[d0 + d] = mma(c[2 * d], p[u], dv[d0 + d]);
-                                dk[d0 + d] = mma(c[2 * d + 1], ds[u], dk[d0 + d]);
-                            }
-                            step_end<Frag<T>::kFloat || D == 128>();
-                        }
-                    }
-                    if constexpr (MASKED && kHalf) {  // (a second time with what the rounding took away)
+                            for (int w = u; w < kTimes; w += 2)
 #pragma unroll
-                        for (int u = 0; u < 2; u++) {
-                            to_frag(dp, u, ds[u]);
+                                for (int d = 0; d < kAtOnce; d++) dv[d0 + d] = mma(c[d], p[w], dv[d0 + d]);
+                            step_end<D == 128>();
 #pragma unroll
-                            for (int d0 = 0; d0 < DB; d0 += kAtOnce) {
-                                frag c[kAtOnce];
+                            for (int d = 0; d < kAtOnce; d++) c[d] = qt.columns(lanes, 32 * n + 16 * u, d0 + d);
+                            if constexpr (MASKED) leave_out_odd<kAtOnce>(c, odd);
 #pragma unroll
-                                for (int d = 0; d < kAtOnce; d++) c[d] = qt.columns(lanes, 32 * n + 16 * u, d0 + d);
-                                leave_out_odd<kAtOnce>(c, odd);
+                            for (int w = u; w < kTimes; w += 2)
 #pragma unroll
-                                for (int d = 0; d < kAtOnce; d++) dk[d0 + d] = mma(c[d], ds[u], dk[d0 + d]);
-                                step_end<D == 128>();
-                            }
+                                for (int d = 0; d < kAtOnce; d++) dk[d0 + d] = mma(c[d], ds[w], dk[d0 + d]);
+                            step_end<D == 128>();
                         }
                     }
                 }
@@ -527,11 +541,14 @@ __device__ __forceinline__ void attn_grad_kv(const Backward &a, const uint32_t b
                 work(std::false_type{});
         }
     }
-    uint32_t thread = threadIdx.x;  // (the key's number is formed again: over the loop there is no register for it)
+    uint32_t thread = threadIdx.x;  // (the key's number is formed again, and the keys' count is a scalar: over the loop there is no
+                                    // vector register for them)
     asm volatile("" : "+v"(thread));
+    asm volatile("" : "+s"(lk));
     const uint32_t own_key = tile * kOwn + thread / kWave * 32 + thread % 32;
     if (own_key >= lk) return;
-    const uint32_t own_b = packed ? 0 : __builtin_amdgcn_readfirstlane(b), first_key = __builtin_amdgcn_readfirstlane(k0);
+    const uint32_t own_b = packed ? 0 : __builtin_amdgcn_readfirstlane(b);
+    const uint32_t first_key = __builtin_amdgcn_readfirstlane(k0);
     auto out = [&](const AttnView &to) {
         return static_cast<T *>(const_cast<void *>(to.at)) + own_b * to.batch + (size_t)(first_key + own_key) * to.row + head * to.head;
     };
