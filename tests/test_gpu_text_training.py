@@ -20,7 +20,8 @@ def _normal(seed, *shape):
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
 @pytest.mark.parametrize("batch,length,vocab,dim,places,scale", [
     (2, 77, 1000, 768, 77, 1.0), (1, 1, 1, 1, 0, 3.0), (3, 5, 7, 33, 9, 0.5), (40, 61, 513, 40, 61, 25.5), (70, 77, 300, 24, 80, 1.0),
-    (1, 64, 2, 8, 0, 1.0), (1, 65, 2, 8, 64 + 1, -2.0), (100, 90, 70000, 8, 90, 1.0), (5, 0, 10, 16, 3, 1.0), (0, 4, 10, 16, 5, 1.0),
+    (1, 64, 2, 8, 0, 1.0), (1, 65, 2, 8, 64 + 1, -2.0), (16, 64, 5000, 650, 64, 1.0), (25, 41, 5000, 650, 41, 1.0), (64, 16, 300, 12, 20, 1.0), (65, 15, 300, 12, 20, 1.0),
+    (1, 1024, 100, 1025, 0, 1.0), (1, 1024, 5, 1024, 0, 1.0), (3, 100, 2049, 4, 100, 1.0), (1, 700, 1, 20000, 0, 1.0), (100, 90, 70000, 8, 90, 1.0), (5, 0, 10, 16, 3, 1.0), (0, 4, 10, 16, 5, 1.0),
 ])
 def test_token_embedding_and_its_gradient(msd, cuda, dtype, batch, length, vocab, dim, places, scale):
     t = DTYPES[dtype]
