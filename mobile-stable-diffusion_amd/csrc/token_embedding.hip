@@ -498,7 +498,7 @@ __global__ __launch_bounds__(kSortThreads) void embed_grad_join_kernel(const Ent
 }
 
 // ---- few tokens ------------------------------------------------------------------
-constexpr uint32_t kFewTokens = 1024, kFewBatch = 64, kFewWaves = kThreads / kWave, kFewEach = kFewTokens / kFewWaves;
+constexpr uint32_t kFewTokens = 1024, kFewBatch = 64, kFewThreads = 512, kFewWaves = kFewThreads / kWave, kFewEach = kFewTokens / kFewWaves;
 constexpr uint32_t kZeroRows = 2048, kFewAtOnce = 8;
 
 struct Few {
@@ -509,23 +509,23 @@ struct Few {
 };
 
 // Everything in one launch, without a sort: a workgroup for a token and 64 pieces of its row looks at all ids, leaves if the token's
-// id occurs before it, and otherwise adds the rows of dy that have the id, a wavefront those of a quarter of the tokens in ascending
+// id occurs before it, and otherwise adds the rows of dy that have the id, a wavefront those of its share of the tokens in ascending
 // order.  Other workgroups write the zeros of a range of table rows, but for those that some token names; others again dpositions.
 template <typename T, int N>
-__global__ __launch_bounds__(kThreads) void embed_grad_few_kernel(const int64_t *ids, const T *dy, T *dtable, T *dpositions, const Few f) {
+__global__ __launch_bounds__(kFewThreads) void embed_grad_few_kernel(const int64_t *ids, const T *dy, T *dtable, T *dpositions, const Few f) {
     __shared__ uint32_t keys[kFewTokens];
     __shared__ float sums[kFewWaves][kWave * N];
     const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     const size_t dim = (size_t)f.pieces * N;
     uint32_t block = blockIdx.x;
     if (block < f.sum_blocks + f.zero_blocks) {
-        for (uint32_t i = threadIdx.x; i < kFewTokens; i += kThreads) keys[i] = i < f.tokens ? key_of(ids, i, f.vocab) : f.vocab;
+        for (uint32_t i = threadIdx.x; i < kFewTokens; i += kFewThreads) keys[i] = i < f.tokens ? key_of(ids, i, f.vocab) : f.vocab;
         __syncthreads();
     }
     if (block < f.sum_blocks) {
         const uint32_t token = block / f.chunks, piece = (block - token * f.chunks) * kWave + lane, key = keys[token];
         bool before = false;
-        for (uint32_t i = threadIdx.x; i < token; i += kThreads) before |= keys[i] == key;
+        for (uint32_t i = threadIdx.x; i < token; i += kFewThreads) before |= keys[i] == key;
         if (__syncthreads_or(before) != 0 || key == f.vocab) return;
         float sum[N];
 #pragma unroll
@@ -574,19 +574,19 @@ __global__ __launch_bounds__(kThreads) void embed_grad_few_kernel(const int64_t 
         const uint32_t first = block * f.zero_rows, rows = min(f.zero_rows, f.vocab - first);
         if (threadIdx.x < kZeroRows / 32) named[threadIdx.x] = 0;
         __syncthreads();
-        for (uint32_t i = threadIdx.x; i < f.tokens; i += kThreads) {
+        for (uint32_t i = threadIdx.x; i < f.tokens; i += kFewThreads) {
             const uint32_t r = keys[i] - first;
             if (keys[i] < f.vocab && r < rows) atomicOr(&named[r / 32], 1u << r % 32);  // (any order gives the same)
         }
         __syncthreads();
-        for (uint32_t i = threadIdx.x; i < rows * f.pieces; i += kThreads) {
+        for (uint32_t i = threadIdx.x; i < rows * f.pieces; i += kFewThreads) {
             const uint32_t r = fast_div(i, f.by_pieces);
             if ((named[r / 32] >> r % 32 & 1) == 0) store_piece<T, N>(dtable + (size_t)first * dim + (size_t)i * N, zero);
         }
         return;
     }
     block -= f.zero_blocks;
-    const uint32_t i = block * kThreads + threadIdx.x;
+    const uint32_t i = block * kFewThreads + threadIdx.x;
     if (i >= f.positions * f.pieces) return;
     const uint32_t step = f.length * f.pieces, batch = i < step ? f.tokens / max(1u, f.length) : 0;
     for (uint32_t b = 0; b < batch; b += 8) {
@@ -601,9 +601,9 @@ __global__ __launch_bounds__(kThreads) void embed_grad_few_kernel(const int64_t 
     store_piece<T, N>(dpositions + (size_t)i * N, zero);
 }
 
-// Whether that launch does.  13 sequences of 77, 1000 rows of 768, float16: 7.2 us, by the sort 18.1; where a third of the text is one
-// token 16.6 and 19.8; 549 tokens, 8191 rows of 650, float32: 9.4 and 17.7.  1024 tokens of 4096 columns, 32000 rows: 64 and 50 (each
-// workgroup goes through all ids for 64 pieces of one token).
+// Whether that launch does.  13 sequences of 77, 1000 rows of 768, float16: 9.0 us, by the sort 18.1; where two thirds of the text are
+// one token 12.4 and 19.8; 9 of 61, 8191 rows of 650, float32: 12.2 and 11.4, by the sort 17.7 and 18.9 (with workgroups of 256 threads
+// 9.5 and 15.8).  1024 tokens of 4096 columns, 32000 rows: 64 and 50 (each workgroup goes through all ids for 64 pieces of one token).
 bool few_tokens(size_t tokens, size_t length, size_t vocab, size_t positions, size_t dim) {
     return tokens <= kFewTokens && tokens * dim <= (size_t(1) << 20) && (positions == 0 || tokens <= kFewBatch * length) &&
            vocab * dim <= (size_t(1) << 35);  // (a launch holds the workgroups of the zeros)
@@ -748,8 +748,8 @@ static int embed_grad_few(const EmbedGrad &g, size_t tokens, size_t length, size
     f.zero_blocks = (uint32_t)((vocab + f.zero_rows - 1) / f.zero_rows);
     f.by_pieces = make_fast_div(f.pieces);
     f.scale = scale;
-    const size_t blocks = (size_t)f.sum_blocks + f.zero_blocks + ((size_t)f.positions * pieces + kThreads - 1) / kThreads;
-    launch((embed_grad_few_kernel<T, N>), dim3((uint32_t)blocks), dim3(kThreads), 0, stream, g.ids, static_cast<const T *>(g.dy),
+    const size_t blocks = (size_t)f.sum_blocks + f.zero_blocks + ((size_t)f.positions * pieces + kFewThreads - 1) / kFewThreads;
+    launch((embed_grad_few_kernel<T, N>), dim3((uint32_t)blocks), dim3(kFewThreads), 0, stream, g.ids, static_cast<const T *>(g.dy),
            static_cast<T *>(g.dtable), static_cast<T *>(g.dpositions), f);
     return launch_status();
 }
