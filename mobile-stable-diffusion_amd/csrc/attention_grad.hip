@@ -578,34 +578,42 @@ __global__ __launch_bounds__(WAVES *kWave, Frag<T>::kFloat || WAVES == 1 ? 1 : 2
     if constexpr (Q) attn_grad_q<T, D, WAVES>(a, blockIdx.x - (KV ? a.kv_blocks : 0), *reinterpret_cast<ForQ<T, D, WAVES> *>(lds));
 }
 
-// Gradients from their parts, in the parts' order, for a few rows of a head: of dk and dv, or of dq.
+// Gradients from their parts, in the parts' order, for a few rows of a head: of dk and dv, or of dq.  V values a lane: 4 where rows
+// are whole vectors of the parts and of the gradients, or 1.
 constexpr uint32_t kJoinRows = 8;
-template <typename T, bool OF_KEYS>
+template <typename T, bool OF_KEYS, int V>
 __global__ __launch_bounds__(kAttnThreads) void attn_grad_join_kernel(const Backward a) {
-    const uint32_t heads = OF_KEYS ? a.s.kv_heads : a.s.heads, parts = OF_KEYS ? a.parts : a.q_parts, head = blockIdx.x % heads;
+    typedef float floats __attribute__((ext_vector_type(V)));
+    const uint32_t heads = OF_KEYS ? a.s.kv_heads : a.s.heads, parts = OF_KEYS ? a.parts : a.q_parts;
+    const uint32_t all = blockIdx.x / heads, head = blockIdx.x - all * heads;
     const int32_t *const offsets = OF_KEYS ? a.s.k_offsets : a.s.q_offsets;
     const uint32_t rows = OF_KEYS ? a.s.k_rows : a.s.q_rows;
     uint32_t b, tile, first, count;
-    if (!find_tile(offsets, a.s.batch, rows, 1, kJoinRows, blockIdx.x / heads, false, b, tile)) return;
+    if (!find_tile(offsets, a.s.batch, rows, 1, kJoinRows, all, false, b, tile)) return;
     span(offsets, b, rows, first, count);
-    const uint32_t n = min(kJoinRows, count - tile * kJoinRows), row = (OF_KEYS ? 2 : 1) * a.s.dim;
+    const uint32_t n = min(kJoinRows, count - tile * kJoinRows), row = (OF_KEYS ? 2 : 1) * a.s.dim / V;
     const size_t step = (size_t)(OF_KEYS ? a.total_keys : a.total_rows) * heads * row;
     for (uint32_t at = threadIdx.x; at < n * row; at += kAttnThreads) {
         const uint32_t r = at / row, c = at - r * row;
         const size_t own = first + tile * kJoinRows + r;
-        const float *from = (OF_KEYS ? a.part : a.q_part) + (((size_t)(offsets != nullptr ? 0 : b) * count + own) * heads + head) * row + c;
-        float sum = 0.0f;
+        const floats *from = reinterpret_cast<const floats *>(OF_KEYS ? a.part : a.q_part) +
+                             (((size_t)(offsets != nullptr ? 0 : b) * count + own) * heads + head) * row + c;
+        floats sum = floats(0.0f);
         for (uint32_t p0 = 0; p0 < parts; p0 += 8) {
-            float f[8];
+            floats f[8];
 #pragma unroll
-            for (uint32_t u = 0; u < 8; u++) f[u] = p0 + u < parts ? from[(p0 + u) * step] : 0.0f;
+            for (uint32_t u = 0; u < 8; u++) f[u] = p0 + u < parts ? from[(p0 + u) * step] : floats(0.0f);
 #pragma unroll
             for (uint32_t u = 0; u < 8; u++) sum += f[u];
         }
-        const bool first_half = c < a.s.dim;
+        const bool first_half = c * V < a.s.dim;
         const AttnView &to = !OF_KEYS ? a.dq : first_half ? a.dk : a.dv;
-        Store<T>::store1(static_cast<T *>(const_cast<void *>(to.at)) + (offsets != nullptr ? 0 : b * to.batch) + own * to.row + head * to.head +
-                             (first_half ? c : c - a.s.dim), sum);
+        T v[V];
+#pragma unroll
+        for (int e = 0; e < V; e++) Store<T>::store1(v + e, sum[e]);
+        T *const out = static_cast<T *>(const_cast<void *>(to.at)) + (offsets != nullptr ? 0 : b * to.batch) + own * to.row + head * to.head +
+                       (first_half ? c * V : c * V - a.s.dim);
+        __builtin_memcpy(__builtin_assume_aligned(out, sizeof(v)), v, sizeof(v));
     }
 }
 
@@ -662,6 +670,16 @@ static void launch_apart(const Backward &a, uint32_t row_blocks, hipStream_t str
     if (row_blocks != 0) launch((attn_grad_kernel<T, D, kAttnWaves, false, true>), dim3(row_blocks), dim3(kAttnThreads), 0, stream, a);
 }
 
+template <typename T, int V>
+static void launch_joins(const AttnProblem &p, const Backward &a, hipStream_t stream) {
+    if (a.parts > 1)
+        launch((attn_grad_join_kernel<T, true, V>), dim3((uint32_t)(tiles_of(p.k_offsets, p.batch, p.k_rows, 1, kJoinRows) * p.kv_heads)),
+               dim3(kAttnThreads), 0, stream, a);
+    if (a.q_parts > 1)
+        launch((attn_grad_join_kernel<T, false, V>), dim3((uint32_t)(tiles_of(p.q_offsets, p.batch, p.q_rows, 1, kJoinRows) * p.heads)),
+               dim3(kAttnThreads), 0, stream, a);
+}
+
 template <typename T>
 int attn_grad_dispatch(const AttnProblem &p, const AttnGradViews &g, const float *lse, const void *rest, void *workspace, size_t workspace_bytes,
                        hipStream_t stream) {
@@ -702,12 +720,10 @@ int attn_grad_dispatch(const AttnProblem &p, const AttnGradViews &g, const float
             launch_apart<T, 128>(a, (uint32_t)row_blocks, stream);
         }
     }
-    if (parts > 1)
-        launch((attn_grad_join_kernel<T, true>), dim3((uint32_t)(tiles_of(p.k_offsets, p.batch, p.k_rows, 1, kJoinRows) * p.kv_heads)),
-               dim3(kAttnThreads), 0, stream, a);
-    if (q_parts > 1)
-        launch((attn_grad_join_kernel<T, false>), dim3((uint32_t)(tiles_of(p.q_offsets, p.batch, p.q_rows, 1, kJoinRows) * p.heads)),
-               dim3(kAttnThreads), 0, stream, a);
+    if (a.vec)
+        launch_joins<T, 4>(p, a, stream);
+    else
+        launch_joins<T, 1>(p, a, stream);
     return launch_status();
 }
 
