@@ -375,7 +375,7 @@ __device__ __forceinline__ void attn_grad_kv(const Backward &a, const uint32_t b
     const float v_norm = kHalf && live ? a.v_norm[(((size_t)(packed ? 0 : b) * lk + k0) + key) * a.s.kv_heads + head] : 0.0f;
 
     const uint32_t wave_key = tile * kOwn + wave * 32;
-    const uint32_t from = live ? first_row(key) : rows;                                  // the lane's rows: [from, rows)
+    const uint32_t own_from = live ? first_row(key) : rows;                              // the lane's rows: [own_from, rows)
     const uint32_t wave_from = wave_key < lk ? first_row(wave_key) : rows;               // the first any key is seen by
     const uint32_t wave_full = wave_key < lk ? first_row(min(lk - 1, wave_key + 31)) : rows; // from here on all are
     const uint32_t from_tile = min(first_row(tile * kOwn), rows) / R, all = (rows + R - 1) / R - from_tile;
@@ -433,6 +433,13 @@ __device__ __forceinline__ void attn_grad_kv(const Backward &a, const uint32_t b
                 constexpr bool MASKED = decltype(with_masked)::value;
                 float by = 1.0f;
                 bool odd = false;
+                uint32_t from = own_from;
+                if constexpr (MASKED && kVInLds) {  // (formed again: over the loop there is no register for it)
+                    uint32_t thread = threadIdx.x;
+                    asm volatile("" : "+v"(thread));
+                    const uint32_t own = tile * kOwn + thread / kWave * 32 + thread % 32;
+                    from = own < lk ? first_row(own) : rows;
+                }
                 if (kHalf) {
                     // (the tile's rows from the last to the first, one to a lane)
                     float down, norms = stats[buffer][2][R - 1 - lane % R], deltas = fabsf(stats[buffer][1][R - 1 - lane % R]);
@@ -505,6 +512,24 @@ __device__ __forceinline__ void attn_grad_kv(const Backward &a, const uint32_t b
                             }
                         }
                     }
+                    if constexpr (D == 128 && !MASKED) {
+                        // (each operand is read one product ahead: there are registers for that, not for the compiler's choice)
+                        auto read = [&](int step) { return (step % 2 == 0 ? gt : qt).columns(lanes, 32 * n + step / (2 * DB) * 16, step / 2 % DB); };
+                        frag c = read(0);
+#pragma unroll
+                        for (int step = 0; step < 4 * DB; step++) {
+                            const int u = step / (2 * DB), d = step / 2 % DB;
+                            frag next = c;
+                            if (step + 1 < 4 * DB) next = read(step + 1);
+                            if (step % 2 == 0)
+                                dv[d] = mma(c, p[u], dv[d]);
+                            else
+                                dk[d] = mma(c, ds[u], dk[d]);
+                            c = next;
+                            step_end<true>();
+                        }
+                        continue;
+                    }
 #pragma unroll
                     for (int u = 0; u < 2; u++) {
 #pragma unroll
@@ -571,7 +596,7 @@ __device__ __forceinline__ void attn_grad_kv(const Backward &a, const uint32_t b
 template <typename T, int D, int WAVES, bool KV, bool Q>
 __global__ __launch_bounds__(WAVES *kWave, Frag<T>::kFloat || WAVES == 1 ? 1 : 2) void attn_grad_kernel(const Backward a) {
     constexpr size_t kBytes = std::max(KV ? sizeof(ForKv<T, D, WAVES>) : 0, Q ? sizeof(ForQ<T, D, WAVES>) : 0);
-    __shared__ __align__(16) char lds[kBytes];
+    __shared__ __align__(256) char lds[kBytes];
     if constexpr (KV) {
         if (!Q || blockIdx.x < a.kv_blocks) return attn_grad_kv<T, D, WAVES>(a, blockIdx.x, *reinterpret_cast<ForKv<T, D, WAVES> *>(lds));
     }

@@ -261,28 +261,47 @@ __device__ __forceinline__ void request_floats(float *lds, const void *from, uin
                  : "memory");
 }
 
+// Rows of 128 float16 are 256 bytes, as many as the banks of LDS are together: see place_of.
+template <typename T, int D>
+constexpr bool kWideRows = !Frag<T>::kFloat && D == 128;
+
+// What the number of a chunk is crossed with in row r of a tile, so that lanes that read one chunk of neighbouring rows, or
+// neighbouring chunks of four rows, meet different banks.  Rows of 256 bytes: four bits, of which four neighbouring rows differ in the
+// upper two (reads by columns: four chunks of four rows at a time) and sixteen in all.  With the three bits of the others
+// conflicts were two fifths of the time of the kernel for dk and dv.
+template <typename T, int D>
+__device__ __forceinline__ uint32_t place_of(uint32_t r) {
+    return kWideRows<T, D> ? (r & 3) << 2 | (r >> 2 & 3) : r & 7;
+}
+
 // Where a lane reads in a tile (below), in bytes from its beginning.  The places differ by more than a constant only in the three
-// bits of the chunk's number that the row's number goes into: a few registers, and the rest is in the instructions.
+// bits of the chunk's number that the row's number goes into: a few registers, and the rest is in the instructions.  Wide rows: one
+// register each, crossed with a constant (a tile begins at a multiple of 256).
 template <typename T, int D>
 struct TileLanes {
     static constexpr uint32_t kRowBytes = D * sizeof(T);
-    uint32_t row[4], column[Frag<T>::kFloat ? 4 : 2];
+    uint32_t row[kWideRows<T, D> ? 1 : 4], column[kWideRows<T, D> ? 1 : Frag<T>::kFloat ? 4 : 2];
     __device__ __forceinline__ TileLanes() {
         const uint32_t lane = threadIdx.x % kWave, h = lane / 32, i = lane % 16;
-        for (uint32_t j = 0; j < 4; j++)
-            row[j] = lane % 32 * kRowBytes + (((Frag<T>::kFloat ? 4 * (j / 2) + 2 * h + j % 2 : 2 * j + h) ^ lane % 8) * 16);
+        if constexpr (kWideRows<T, D>) {
+            row[0] = lane % 32 * kRowBytes + (h ^ place_of<T, D>(lane)) * 16;
+            column[0] = (4 * h + i / 4) * kRowBytes + ((2 * (lane / 16 % 2) + i % 4 / 2) ^ place_of<T, D>(4 * h + i / 4)) * 16 + i % 2 * 8;
+            return;
+        } else {
+            for (uint32_t j = 0; j < 4; j++)
+                row[j] = lane % 32 * kRowBytes + (((Frag<T>::kFloat ? 4 * (j / 2) + 2 * h + j % 2 : 2 * j + h) ^ lane % 8) * 16);
+        }
         if constexpr (Frag<T>::kFloat) {
             for (uint32_t j = 0; j < 4; j++)
                 column[j] = (4 * h + j) * kRowBytes + (lane % 32 / 4 ^ (4 * h + j)) * 16 + lane % 4 * 4;
-        } else {
+        } else if constexpr (!kWideRows<T, D>) {
             for (uint32_t j = 0; j < 2; j++)
                 column[j] = (4 * h + i / 4) * kRowBytes + ((4 * j + 2 * (lane / 16 % 2) + i % 4 / 2) ^ (4 * h + i / 4)) * 16 + i % 2 * 8;
         }
     }
 };
 
-// A tile in LDS: ROWS rows of D values as 16-byte chunks, chunk c of row r at place c ^ (r & 7), so that lanes that read one
-// chunk of neighbouring rows, or neighbouring chunks of four rows, meet different banks.
+// A tile in LDS: ROWS rows of D values as 16-byte chunks, chunk c of row r at place c ^ place_of(r).
 template <typename T, int D, int WAVES, int ROWS = Frag<T>::kTile>
 struct Tile {
     static constexpr int kThreads = WAVES * kWave, kRows = ROWS, kChunks = D * (int)sizeof(T) / 16;
@@ -290,12 +309,12 @@ struct Tile {
     // places of a thread that lie kTurn apart are kTurn * kStep rows apart, in the same column
     static constexpr int kStep = kThreads / kChunks, kTurn = kStep >= 8 ? 1 : 8 / kStep;
     typedef typename Frag<T>::type frag;
-    u32x4 data[kRows * kChunks];
+    alignas(kWideRows<T, D> ? 256 : 16) u32x4 data[kRows * kChunks];
 
     // Row and column of the chunk that belongs at this thread's place number p.
     static __device__ __forceinline__ uint32_t row_of(int p) { return (p * kThreads + threadIdx.x) / kChunks; }
     static __device__ __forceinline__ uint32_t column_of(int p) {
-        return ((p * kThreads + threadIdx.x) % kChunks ^ (row_of(p) & 7)) * (16 / (uint32_t)sizeof(T));
+        return ((p * kThreads + threadIdx.x) % kChunks ^ place_of<T, D>(row_of(p))) * (16 / (uint32_t)sizeof(T));
     }
     // Bytes from a tile's first row to this thread's first kTurn chunks, for rows of `row` elements; chunk p is at
     // `offset_of(base, row, p)`.
@@ -335,12 +354,18 @@ struct Tile {
     }
 
     typedef __attribute__((address_space(3))) const char *lds_t;
+    // (wide rows) A lane's place, crossed with a constant below 256.
+    __device__ __forceinline__ lds_t crossed(uint32_t lane, uint32_t with) const {
+        return (lds_t)(((uint32_t)(uintptr_t)(lds_t)data + lane) ^ with);
+    }
     // A operand by rows: row r0 + (lane & 31), columns 16 k + 8 h ...
     __device__ __forceinline__ frag rows(const TileLanes<T, D> &l, int r0, int k) const {
         const lds_t at = (lds_t)data;
         frag f;
         u32x4 v[sizeof(T) / 2];
-        if constexpr (!Frag<T>::kFloat) {
+        if constexpr (kWideRows<T, D>) {
+            v[0] = *(__attribute__((address_space(3))) const u32x4 *)(crossed(l.row[0], 32 * k) + r0 * kChunks * 16);
+        } else if constexpr (!Frag<T>::kFloat) {
             v[0] = *(__attribute__((address_space(3))) const u32x4 *)(at + l.row[k % 4] + (r0 * kChunks * 16 + k / 4 * 128));
         } else {
 #pragma unroll
@@ -358,8 +383,13 @@ struct Tile {
             // 16 lanes read 4 rows of 16 columns, 8 bytes a lane, and each gets a column of 4
 #pragma unroll
             for (int u = 0; u < 2; u++) {
-                const fp16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4f16(
-                    (fp16x4 __attribute__((address_space(3))) *)(at + l.column[db % 2] + ((r0 + 8 * u) * kChunks * 16 + db / 2 * 128)));
+                typedef fp16x4 __attribute__((address_space(3))) *four_t;
+                four_t from;
+                if constexpr (kWideRows<T, D>)
+                    from = (four_t)(crossed(l.column[0], 64 * db ^ 32 * u) + (r0 + 8 * u) * kChunks * 16);
+                else
+                    from = (four_t)(at + l.column[db % 2] + ((r0 + 8 * u) * kChunks * 16 + db / 2 * 128));
+                const fp16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4f16(from);
 #pragma unroll
                 for (int j = 0; j < 4; j++) f[4 * u + j] = (_Float16)v[j];
             }
