@@ -378,8 +378,11 @@ __device__ __forceinline__ void attn_grad_kv(const Backward &a, const uint32_t b
     const uint32_t own_from = live ? first_row(key) : rows;                              // the lane's rows: [own_from, rows)
     const uint32_t wave_from = wave_key < lk ? first_row(wave_key) : rows;               // the first any key is seen by
     const uint32_t wave_full = wave_key < lk ? first_row(min(lk - 1, wave_key + 31)) : rows; // from here on all are
+    // Tiles of rows from the last one back, every parts-th of them: under a mask, too, all workgroups are then at the same rows at a
+    // time, and read them from L2 (from the first row on: of the requests of 4 sequences of 4000 26 % were served there, now 69 %).
     const uint32_t from_tile = min(first_row(tile * kOwn), rows) / R, all = (rows + R - 1) / R - from_tile;
-    const uint32_t each = (all + a.parts - 1) / a.parts, t0 = from_tile + min(all, part * each), t1 = min(from_tile + all, t0 + each);
+    const uint32_t count = all > part ? (all - part + a.parts - 1) / a.parts : 0;
+    auto tile_of = [&](uint32_t n) { return from_tile + all - 1 - part - n * a.parts; };
 
     auto fetch = [&](uint32_t t, uint32_t buffer) {
         const uint32_t i0 = fast_div(t * R, a.s.by_group);  // the query of the tile's first row
@@ -421,12 +424,12 @@ __device__ __forceinline__ void attn_grad_kv(const Backward &a, const uint32_t b
 #pragma unroll
     for (int d = 0; d < DB; d++) dk[d] = dv[d] = zero16();
     DsScale scale;
-    if (t0 < t1) fetch(t0, 0);
-    for (uint32_t t = t0; t < t1; t++) {
+    if (count != 0) fetch(tile_of(0), 0);
+    for (uint32_t at = 0; at < count; at++) {
         wait_tiles();
         __syncthreads();
-        if (t + 1 < t1) fetch(t + 1, (t + 1 - t0) & 1);
-        const uint32_t buffer = (t - t0) & 1, first = t * R;
+        if (at + 1 < count) fetch(tile_of(at + 1), (at + 1) & 1);
+        const uint32_t buffer = at & 1, first = tile_of(at) * R;
         const RowTile &qt = tiles[buffer][0], &gt = tiles[buffer][1];
         if (first + R > wave_from && wave_from < rows) {
             auto work = [&](auto with_masked) {
