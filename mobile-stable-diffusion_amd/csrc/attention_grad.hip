@@ -468,11 +468,34 @@ __device__ __forceinline__ void attn_grad_kv(const Backward &a, const uint32_t b
 #pragma unroll
                 for (int n = 0; n < R / 32; n++) {
                     f32x16 s = zero16(), dp = zero16();
+                    if constexpr (kVInLds) {  // (operands are read a step ahead: there are registers for that, not for the compiler's choice)
+                        frag qc = qt.rows(lanes, 32 * n, 0), gc = gt.rows(lanes, 32 * n, 0);
+                        operand_t vc = value(0);
 #pragma unroll
-                    for (int c = 0; c < KD; c++) {
-                        s = mma(qt.rows(lanes, 32 * n, c), k[c], s);
-                        dp = mma(gt.rows(lanes, 32 * n, c), value(c), dp);
-                        step_end<Frag<T>::kFloat>();
+                        for (int c = 0; c < KD; c++) {
+                            const int next = c + 1 < KD ? c + 1 : c;
+                            frag qn = qc, gn = gc;
+                            operand_t vn = vc;
+                            if (next != c) {
+                                qn = qt.rows(lanes, 32 * n, next);
+                                gn = gt.rows(lanes, 32 * n, next);
+                                vn = value(next);
+                            }
+                            step_end<true>();
+                            s = mma(qc, k[c], s);
+                            dp = mma(gc, vc, dp);
+                            step_end<true>();
+                            qc = qn;
+                            gc = gn;
+                            vc = vn;
+                        }
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < KD; c++) {
+                            s = mma(qt.rows(lanes, 32 * n, c), k[c], s);
+                            dp = mma(gt.rows(lanes, 32 * n, c), value(c), dp);
+                            step_end<Frag<T>::kFloat>();
+                        }
                     }
 #pragma unroll
                     for (int g = 0; g < 4; g++) {
@@ -524,6 +547,7 @@ __device__ __forceinline__ void attn_grad_kv(const Backward &a, const uint32_t b
                             const int u = step / (2 * DB), d = step / 2 % DB;
                             frag next = c;
                             if (step + 1 < 4 * DB) next = read(step + 1);
+                            step_end<true>();
                             if (step % 2 == 0)
                                 dv[d] = mma(c, p[u], dv[d]);
                             else
