@@ -1,9 +1,17 @@
 // Gradient of attention for gfx950.  With p as in the forward call (formed again from its log2 sums) and D_i = do_i . out_i,
 //     dS_ij = p_ij (do_i . v_j - D_i),   dq_i = scale sum_j dS_ij k_j,   dk_j = scale sum_i dS_ij q_i,   dv_j = sum_i p_ij do_i.
-// Three launches: D (and row norms); dq with a workgroup for rows, over the keys, as the forward call; dk and dv with a
-// workgroup for keys, over the rows.  Each gradient is owned by one workgroup, so nothing is added by atomics, at the price of
-// forming S and dO V^T twice (7 products for 5).  The heads of a key head are rows of the same tiles, so their gradients
-// add up in the accumulators.
+// A launch for D (and row norms); dq with a workgroup for rows, over the keys, as the forward call; dk and dv with a workgroup for
+// keys, over the rows: one launch or one for each.  Each gradient is owned by one workgroup, so nothing is added by atomics, at the
+// price of forming S and dO V^T twice (7 products for 5).  The heads of a key head are rows of the same tiles, so their gradients
+// add up in the accumulators.  Where either kind of workgroup is few, its rows or keys are cut into parts, joined by another launch.
+//
+// Measured (10 d operations for each visible pair):
+//   float16, 4 x 4000 causal, 16 heads of 128 on 4: D 41 us (at the rate of a large copy), dk and dv 670 and their join 34, dq 420:
+//     595 TFLOP/s.  4 x 4096, 32 heads on 8: 4.08 ms, 674.  dk and dv hold 254 of 256 registers: waits for operands and tiles are
+//     36 % of a wavefront's cycles, matrix instructions 42 % of the SIMD's.
+//   float16, 8 x 4096, 16 heads of 64: 2.4 ms, 575 TFLOP/s.
+//   float32, 32 sequences of up to 77, 12 heads of 64: 4 and 23 us; a launch's fixed 6, the wavefronts' own first rows, then 5 a tile.
+//   float32, 2 x 2048 causal, 8 heads: 68 TFLOP/s with 64 columns, 80 with 128.
 //
 // float16: dS is rounded to float16 for its product, after a power of two that brings the largest it can be,
 // |do_i| max |v_j| + |D_i|, next to 2^14: it keeps 11 bits down to 2^-28 of that, whatever the gradients' size.  Each row of dq
@@ -135,6 +143,9 @@ __device__ __forceinline__ void attn_grad_q(const Backward &a, const uint32_t bl
     typedef Tile<T, D, WAVES> KvTile;
     constexpr uint32_t kOwn = 32 * WAVES;
     constexpr bool kHalf = !Frag<T>::kFloat;
+    // Operands from LDS are read a step ahead, in this order: there are registers for that, not for the compiler's choice, which
+    // waits for most reads right behind them.
+    constexpr bool kAhead = kHalf && D == 128;
     constexpr int R = KvTile::kRows, KD = D / 16, DB = D / 32;
     KvTile(&tiles)[2][2] = lds.tiles;
     const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, h = lane / 32;
@@ -232,11 +243,29 @@ __device__ __forceinline__ void attn_grad_q(const Backward &a, const uint32_t bl
 #pragma unroll
                 for (int n = 0; n < R / 32; n++) {
                     f32x16 s = zero16(), dp = zero16();
+                    if constexpr (kAhead) {
+                        frag kc = kt.rows(lanes, 32 * n, 0), vc = vt.rows(lanes, 32 * n, 0);
 #pragma unroll
-                    for (int k = 0; k < KD; k++) {
-                        s = mma(kt.rows(lanes, 32 * n, k), q[k], s);
-                        dp = mma(vt.rows(lanes, 32 * n, k), g[k], dp);
-                        step_end<Frag<T>::kFloat>();
+                        for (int k = 0; k < KD; k++) {
+                            frag kn = kc, vn = vc;
+                            if (k + 1 < KD) {
+                                kn = kt.rows(lanes, 32 * n, k + 1);
+                                vn = vt.rows(lanes, 32 * n, k + 1);
+                            }
+                            step_end<true>();
+                            s = mma(kc, q[k], s);
+                            dp = mma(vc, g[k], dp);
+                            step_end<true>();
+                            kc = kn;
+                            vc = vn;
+                        }
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < KD; k++) {
+                            s = mma(kt.rows(lanes, 32 * n, k), q[k], s);
+                            dp = mma(vt.rows(lanes, 32 * n, k), g[k], dp);
+                            step_end<Frag<T>::kFloat>();
+                        }
                     }
 #pragma unroll
                     for (int r = 0; r < 16; r++)
@@ -251,6 +280,22 @@ __device__ __forceinline__ void attn_grad_q(const Backward &a, const uint32_t bl
                         to_frag(s, 0, ds[0]);
                         to_frag(s, 1, ds[1]);
                         add_products<MASKED, true, T, D>(kt, lanes, ds, dq, odd);
+                        continue;
+                    }
+                    if constexpr (kAhead && !MASKED) {
+                        operand_t ds[2];
+                        to_frag(s, 0, ds[0]);
+                        to_frag(s, 1, ds[1]);
+                        frag c = kt.columns(lanes, 32 * n, 0);
+#pragma unroll
+                        for (int step = 0; step < 2 * DB; step++) {
+                            frag next = c;
+                            if (step + 1 < 2 * DB) next = kt.columns(lanes, 32 * n + (step + 1) / DB * 16, (step + 1) % DB);
+                            step_end<true>();
+                            dq[step % DB] = mma(c, ds[step / DB], dq[step % DB]);
+                            step_end<true>();
+                            c = next;
+                        }
                         continue;
                     }
 #pragma unroll

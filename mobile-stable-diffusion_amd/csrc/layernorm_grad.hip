@@ -5,6 +5,9 @@
 // reductions more per row, where keeping them would change the forward call and add a read.  A lane owns the same columns in
 // every row that it handles, so dgamma and dbeta gather in its registers over the rows; a workgroup adds its teams through LDS
 // and writes one row of partial sums, and a second launch adds those in order: no atomics, the same bits every time.
+//
+// Measured: 65536 x 320 float16 with dsum 34 us (168 MB, 4.9 TB/s, the rate of a large copy) and 4.8 for the sums of the partial rows;
+// 2049 x 777 float32 with dsum 10.5 us (rows of no whole vectors: single values) and 4.4; 154 x 768 float32 4.3 and 2.3, latency.
 #include <algorithm>
 
 #include "msd_device.h"

