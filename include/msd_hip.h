@@ -456,9 +456,10 @@ int msd_softmax(const void *x, void *y, size_t rows, size_t cols, int stable, in
  *   of no sequence stay as they were.  Lengths may be zero and differ between queries and keys.  Offsets are read on the device:
  *   what lies outside the tensors is cut off, sequences that overlap give undefined values.
  *   causal != 0: the last query sees every key, the one before all but the last, ...: i sees j <= i + (keys - queries).
- *   scale: positive and finite.
+ *   scale: positive, below 10^30.
  * A row that sees no key, or whose scores are all -infinity, gives zeros.  What a row does not see has no part in it, infinities
- * and NaN included.  Scores, maxima and sums are float32; float16 weights are rounded to float16 for the product with v.
+ * and NaN included.  Scores, maxima and sums are float32; float16 weights are rounded to float16 for the product with v; float32
+ * values enter the products as three bfloat16 each, which leaves out at most 2^-23 of a product (and what is below 2^-126).
  *   lse    NULL, or float32 [rows of q][heads]: log2 of the sum of exp(scale q . k) (-infinity for a row that sees nothing),
  *          kept for msd_attention_backward.
  *   rest   NULL, or with float16 [rows of q][heads][dim] float16 without gaps: what the rounding of out took away, kept for
@@ -466,7 +467,7 @@ int msd_softmax(const void *x, void *y, size_t rows, size_t cols, int stable, in
  * workspace: 16-byte aligned device memory of at least the bytes that msd_attention_workspace reports (host only; dtype as for
  * the call; backward = 0), apart from all else; its contents need not be set, are left undefined, and belong to this call until it (or every
  * replay of it) is done.  The call allocates nothing and gives the same bits every time, in a capture too.
- * At most 2^27 rows times heads of queries and of keys, 2^20 heads, and 2^22 sequences times kv_heads.
+ * At most 2^26 rows times heads of queries and of keys, 2^20 heads, 2^22 sequences times kv_heads, and 2^16 packed sequences.
  */
 int msd_attention_workspace(size_t batch, size_t q_rows, size_t k_rows, size_t heads, size_t kv_heads, size_t dim, int packed,
                             int backward, int dtype, size_t *bytes);

@@ -856,10 +856,11 @@ int msd_softmax(const void *x, void *y, size_t rows, size_t cols, int stable, in
 
 static int attention_checks(size_t batch, size_t q_rows, size_t k_rows, size_t heads, size_t kv_heads, size_t dim, bool packed, int dtype,
                             size_t *all_q, size_t *all_k) {
-    constexpr size_t kMost = size_t(1) << 27;
+    constexpr size_t kMost = size_t(1) << 26, kPacked = size_t(1) << 16;
     if (dtype != MSD_DTYPE_F32 && dtype != MSD_DTYPE_F16) return MSD_ERR_INVALID_VALUE;
     if (heads == 0 || kv_heads == 0 || heads % kv_heads != 0 || dim == 0 || dim > 128) return MSD_ERR_INVALID_VALUE;
-    if (batch > kMost || q_rows > kMost || k_rows > kMost || heads > (size_t(1) << 20) || batch * kv_heads > (size_t(1) << 22))
+    if (batch > kMost || q_rows > kMost || k_rows > kMost || heads > (size_t(1) << 20) || batch * kv_heads > (size_t(1) << 22) ||
+        (packed && batch > kPacked))  // (each workgroup looks for its sequence among all)
         return MSD_ERR_INVALID_VALUE;
     *all_q = packed ? (batch != 0 ? q_rows : 0) : batch * q_rows;
     *all_k = packed ? (batch != 0 ? k_rows : 0) : batch * k_rows;
@@ -948,7 +949,7 @@ int msd_attention(const void *q, const void *k, const void *v, void *out, float 
                   int causal, int dtype, void *workspace, size_t workspace_bytes, void *stream) {
     size_t all_q, all_k, need;
     const bool packed = q_offsets != nullptr;
-    if (packed != (k_offsets != nullptr) || !(scale > 0.0f) || !std::isfinite(scale)) return MSD_ERR_INVALID_VALUE;
+    if (packed != (k_offsets != nullptr) || !(scale > 0.0f) || !(scale < 1e30f)) return MSD_ERR_INVALID_VALUE;
     int rc = attention_checks(batch, q_rows, k_rows, heads, kv_heads, dim, packed, dtype, &all_q, &all_k);
     if (rc == MSD_OK) rc = msd_attention_workspace(batch, q_rows, k_rows, heads, kv_heads, dim, packed, 0, dtype, &need);
     if (rc != MSD_OK) return rc;
@@ -986,7 +987,7 @@ int msd_attention_backward(const void *dout, const void *q, const void *k, const
                            int dtype, void *workspace, size_t workspace_bytes, void *stream) {
     size_t all_q, all_k, need;
     const bool packed = q_offsets != nullptr;
-    if (packed != (k_offsets != nullptr) || !(scale > 0.0f) || !std::isfinite(scale)) return MSD_ERR_INVALID_VALUE;
+    if (packed != (k_offsets != nullptr) || !(scale > 0.0f) || !(scale < 1e30f)) return MSD_ERR_INVALID_VALUE;
     int rc = attention_checks(batch, q_rows, k_rows, heads, kv_heads, dim, packed, dtype, &all_q, &all_k);
     if (rc == MSD_OK) rc = msd_attention_workspace(batch, q_rows, k_rows, heads, kv_heads, dim, packed, 1, dtype, &need);
     if (rc != MSD_OK) return rc;

@@ -558,6 +558,11 @@ __device__ __forceinline__ void attn_grad_kv(const Backward &a, const uint32_t b
                         for (int r = 0; r < 16; r++)
                             if (first + 32 * n + 8 * (r / 4) + 4 * h + r % 4 < from) s[r] = dp[r] = 0.0f;
                     }
+                    if (first + 32 * n + 32 > rows) {  // (zeros behind the last row times an infinite key are NaN)
+#pragma unroll
+                        for (int r = 0; r < 16; r++)
+                            if (first + 32 * n + 8 * (r / 4) + 4 * h + r % 4 >= rows) s[r] = dp[r] = 0.0f;
+                    }
                     if constexpr (Frag<T>::kFloat) {
                         operand_t w[2];
                         to_frag(s, 0, w[0]);

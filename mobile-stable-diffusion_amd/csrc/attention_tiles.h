@@ -55,22 +55,28 @@ __device__ __forceinline__ f32x16 mma(const half8 &a, const half8 &b, const f32x
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 __device__ __forceinline__ half8 operand(const half8 &f) { return f; }
+template <bool ODD = true>
 __device__ __forceinline__ Thirds operand(const f32x8 &f) {
+    // ODD: an infinity is the largest finite values and an infinity in the third part, which meets the other operand's first alone:
+    // times a zero second or third part of a finite value it would be NaN.  A NaN is in the third part, too.  (Weights and score
+    // gradients are not infinite but where the gradient is NaN.)
+    constexpr float kMost = 0x1.fffffep127f;
     Thirds t;
-    uint32_t w[8];
-    __builtin_memcpy(w, &f, sizeof(w));
+    float left[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) left[j] = f[j];
 #pragma unroll
     for (int n = 0; n < 3; n++) {
+        uint32_t w[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            w[j] = __float_as_uint(ODD && n < 2 ? __builtin_amdgcn_fmed3f(left[j], -kMost, kMost) : left[j]);
+            left[j] -= __uint_as_float(w[j] & 0xFFFF0000u);
+        }
         u32x4 packed;
 #pragma unroll
         for (int j = 0; j < 4; j++) packed[j] = __builtin_amdgcn_perm(w[2 * j + 1], w[2 * j], 0x07060302u);  // (the upper halves)
         t.part[n] = __builtin_bit_cast(bf16x8, packed);
-        if (n == 2) break;
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const float left = __uint_as_float(w[j]) - __uint_as_float(w[j] & 0xFFFF0000u);
-            w[j] = __float_as_uint(n == 0 && left != left ? 0.0f : left);  // (nothing is left of an infinity)
-        }
     }
     return t;
 }
@@ -105,7 +111,7 @@ __device__ __forceinline__ void to_frag(const f32x16 &c, int t, Thirds &b) {
     f32x8 f;
 #pragma unroll
     for (int j = 0; j < 8; j++) f[j] = c[8 * t + j];
-    b = operand(f);
+    b = operand<false>(f);
 }
 
 __device__ __forceinline__ f32x16 zero16() {

@@ -96,6 +96,10 @@ def attention_head(q, k, v, causal, scale, dout=None):
     weight_off = 2 * score_off + (lk / 32 + 40) * EPS
     out, out_size = p @ v, p @ v.abs()
     off = (weight_half + weight_off + (lk / 16 + 16) * EPS) * out_size + 2.0 ** -31 * v.abs().sum(0)
+    # float32: a value's three bfloat16 have float32's exponents, and those below 2^-126 count as zero in a product: of a weight or
+    # score gradient each is lost with at most 2^-126 of it, a term's loss is up to three of those times the other operand, and
+    # weights below 2^-126, zero, take as much of dS as (dp - D) is large
+    lost = 2.0 ** -124
     if dout is None:
         return (out, off),
     g = dout.double()
@@ -108,10 +112,12 @@ def attention_head(q, k, v, causal, scale, dout=None):
     # (float16: what is far below the largest it can be keeps no digits)
     if weight_half:
         ds_off = ds_off + torch.where(seen, 2.0 ** -37 * ((g.norm(dim=1, keepdim=True) * v.norm(dim=1).amax() if lk else 0.0) + delta.abs().amax()), 0.0)
+    if not weight_half:
+        ds_off = ds_off + torch.where(seen, lost * (1 + dp.abs() + delta.abs()), 0.0)
     n = (max(lq, lk) / 16 + 40) * EPS
     dq, dq_off = scale * (ds @ k), scale * (ds_off + n * ds.abs()) @ k.abs()
     dk, dk_off = scale * (ds.t() @ q), scale * (ds_off + n * ds.abs()).t() @ q.abs()
-    p_off = (weight_half + n) * p + weight_off * p + (2.0 ** -40 if weight_half else 0.0)
+    p_off = (weight_half + n) * p + weight_off * p + (2.0 ** -40 if weight_half else lost)
     dv, dv_off = p.t() @ g, torch.where(seen, p_off, 0.0).t() @ g.abs()
     return (out, off), (dq, dq_off), (dk, dk_off), (dv, dv_off)
 

@@ -318,6 +318,104 @@ def test_gradients_as_views_of_one_projection_by_sequence(msd, cuda, dtype):
     assert all(torch.equal(a, c) for a, c in zip(got, want)) and got[1].data_ptr() == grads[:, 1].data_ptr()
 
 
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_broadcast_operands(msd, cuda, dtype):
+    """One key sequence for a batch, one head for all: views with strides of zero.  Their gradients come back for every copy."""
+    t = DTYPES[dtype]
+    q, k = _normal(1, 1, 40, 1, 64).to(t).to(cuda), _normal(2, 1, 90, 2, 64).to(t).to(cuda)
+    wide = [q.expand(3, 40, 4, 64), k.expand(3, 90, 2, 64), k.expand(3, 90, 2, 64)]
+    out, kept = msd.attention_kept(*wide, True)
+    dense, dense_kept = msd.attention_kept(*(x.contiguous() for x in wide), True)
+    dout = _normal(3, 3, 40, 4, 64).to(t).to(cuda)
+    assert torch.equal(out, dense)
+    grads = msd.attention_backward(dout, kept)
+    assert all(torch.equal(a, b) and a.is_contiguous() for a, b in zip(grads, msd.attention_backward(dout, dense_kept)))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_rows_whose_scores_are_all_minus_infinity_give_zeros(msd, cuda, dtype):
+    t = DTYPES[dtype]
+    q, k, v = (_normal(i, 1, 70, 2, 64).to(t).to(cuda) for i in range(3))
+    q[..., 0] = q[..., 0].abs() + 0.5
+    k[:, :30, :, 0] = -math.inf  # (causal: rows 0 to 29 see no other keys)
+    out, kept = msd.attention_kept(q, k, v, True)
+    assert not out[:, :30].any() and bool((kept.lse[:, :30] == -math.inf).all())
+    want = plain.attention(q[0, 30:].cpu(), k[0, 30:].cpu(), v[0, 30:].cpu(), True, 64 ** -0.5, None, [(40, 40)])
+    plain.check(out[0, 30:], want[0])
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("causal,dim", [(False, 64), (True, 64), (False, 128), (True, 128), (False, 40)])
+def test_visible_infinities_are_those_of_the_formula(msd, cuda, dtype, causal, dim):
+    """Keys of minus infinity have no weight, values of infinity reach all rows that see them; operands of few digits, whose products
+    with infinities must not become NaN."""
+    t, n = DTYPES[dtype], 150
+    q, k, v, dout = _pack([(n, n)], 2, 2, dim, t, 3)
+    q[..., 0], q[..., 1] = 1.0, 0.5
+    k[20, 0, 0] = k[100, 0, 1] = -math.inf
+    v[140, 1, 7], v[9, 1, 5] = math.inf, -math.inf
+    d = [x[None].to(cuda) for x in (q, k, v)]
+    out, kept = msd.attention_kept(*d, causal, 0.1)
+    gone = k.clone()
+    gone[[20, 100], 0] = 0
+    rest = torch.arange(n) != 20
+    rest &= torch.arange(n) != 100
+    sees = plain.visible(n, n, causal) & rest
+    score = torch.where(sees, 0.1 * q[:, 0].double() @ gone[:, 0].double().t(), -math.inf)
+    want = torch.softmax(score, 1) @ v[:, 0].double()
+    size = torch.softmax(score, 1) @ v[:, 0].double().abs()
+    assert bool(((out[0, :, 0].cpu().double() - want).abs() <= 4 * plain.HALF[t] * size + 2000 * plain.EPS * size + 2.0 ** -24).all())
+    row = torch.arange(n)
+    up, down = out[0, :, 1, 7].cpu(), out[0, :, 1, 5].cpu()
+    assert bool((up == math.inf)[(row >= 140) | torch.tensor(not causal)].all()) and bool((down == -math.inf)[(row >= 9) | torch.tensor(not causal)].all())
+    if causal:
+        assert torch.isfinite(up[:140]).all() and torch.isfinite(down[:9]).all()
+    others = [c for c in range(dim) if c not in (5, 7)]
+    assert torch.isfinite(out[0, :, 1][:, others]).all()
+    # what the keys without weight give back is nothing, and the others' gradients are finite
+    clean = d[2].clone()
+    clean[0, 140, 1, 7] = clean[0, 9, 1, 5] = 0
+    out, kept = msd.attention_kept(d[0], d[1], clean, causal, 0.1)
+    dq, dk, dv = msd.attention_backward(dout[None].to(cuda), kept)
+    assert not dv[0, [20, 100], 0].any() and not dk[0, [20, 100], 0].any()
+    assert torch.isfinite(dk).all() and torch.isfinite(dv).all()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("size", [30.0, 1e-3])
+def test_scores_of_any_size(msd, cuda, dtype, size):
+    """Weights of one key alone, and all alike."""
+    t, lengths = DTYPES[dtype], [(150, 150)]
+    q, k, v, dout = _pack(lengths, 2, 1, 64, t, 9)
+    q = (q * size).to(t)
+    want = plain.attention(q, k, v, True, 0.5, dout, lengths)
+    out, kept = msd.attention_kept(*(x[None].to(cuda) for x in (q, k, v)), True, 0.5)
+    plain.check(out[0], want[0], "out")
+    for g, w, what in zip(msd.attention_backward(dout[None].to(cuda), kept), want[1:], ("dq", "dk", "dv")):
+        plain.check(g[0], w, what)
+
+
+@pytest.mark.parametrize("count", [63, 64, 65, 1000])
+def test_many_packed_sequences(msd, cuda, count):
+    gen = torch.Generator().manual_seed(count)
+    lengths = [(int(a), int(b)) for a, b in torch.randint(0, 9, (count, 2), generator=gen)]
+    q, k, v, dout = _pack(lengths, 2, 1, 16, torch.float32, count)
+    want = plain.attention(q, k, v, True, 0.25, dout, lengths)
+    o, ok = _offsets([a for a, _ in lengths], cuda), _offsets([b for _, b in lengths], cuda)
+    out, kept = msd.attention_kept(q.to(cuda), k.to(cuda), v.to(cuda), True, 0.25, o, ok)
+    plain.check(out, want[0], "out")
+    for g, w, what in zip(msd.attention_backward(dout.to(cuda), kept), want[1:], ("dq", "dk", "dv")):
+        plain.check(g, w, what)
+
+
+@pytest.mark.parametrize("dim", [20000, 100001])
+def test_layernorm_gradient_of_long_rows(msd, cuda, dim):
+    dy, x, gamma, dsum = _normal(1, 3, dim), _normal(2, 3, dim) + 1, 1 + 0.1 * _normal(3, dim), _normal(4, 3, dim)
+    want = plain.layernorm_backward(dy, x, gamma, 1e-5, dsum)
+    for g, w in zip(msd.layernorm_backward(dy.to(cuda), x.to(cuda), gamma.to(cuda), 1e-5, dsum.to(cuda)), want):
+        plain.check(g, w)
+
+
 # ---- native calls ---------------------------------------------------------------------------------------
 def _cases(msd, cuda, half):
     gen = torch.Generator(device=cuda).manual_seed(6)

@@ -103,7 +103,8 @@ def test_attention_refusals(msd):
                    dict(FEW, workspace=D), dict(FEW, workspace=E), dict(FEW, workspace=G), dict(qo=D, ko=I), dict(qo=I, ko=E),
                    strided(s9=0), strided(s10=255), strided(s10=0), strided(s11=63), strided(s9=50 * 256 - 1), strided(s0=1 << 62), strided(s10=1 << 62),
                    dict(batch=1 << 28), dict(rows=1 << 28), dict(keys=1 << 28), dict(heads=1 << 21, kv_heads=1), dict(rows=1 << 26, batch=1),
-                   dict(batch=1 << 22, rows=1, keys=1, kv_heads=4)):
+                   dict(batch=1 << 22, rows=1, keys=1, kv_heads=4), dict(scale=1e30), dict(qo=I, ko=J, batch=(1 << 16) + 1, rows=1 << 17, keys=1 << 17),
+                   dict(rows=1 << 24, keys=1, heads=8, kv_heads=1)):
         assert _attention(lib, **change) == 1, change
     assert _attention(lib, batch=0, q=None, k=None, v=None, out=None, lse=None, rest=None, workspace=None) == 0
     assert _attention(lib, rows=0, q=None, out=None, lse=None, rest=None, workspace=None) == 0
