@@ -58,6 +58,7 @@ def test_token_embedding_takes_unaligned_tables(msd, cuda):
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
 @pytest.mark.parametrize("rows,dim", [
     (154, 768), (1, 1), (3, 5), (7, 64), (33, 320), (1000, 40), (17, 1280), (9, 2048), (5, 4096), (300, 777), (2, 4099), (3, 9000), (2, 8192), (5000, 8), (129, 256),
+    (70, 384), (70, 392), (70, 512), (70, 776), (40, 1024), (40, 1536), (40, 1544), (9, 6152), (40, 1100), (9, 2049),
 ])
 @pytest.mark.parametrize("add", [False, True])
 def test_layernorm_gradient(msd, cuda, dtype, rows, dim, add):
