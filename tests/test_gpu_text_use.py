@@ -148,6 +148,34 @@ def test_calls_use_the_current_stream(msd, cuda):
             assert bool((out - k).abs().max() <= 1e-5) and bool((dv - k).abs().max() <= 1e-5) and bool((dbeta == 10.0 * k).all())
 
 
+def test_two_threads_at_once(msd, cuda):
+    """Each with operands and a stream of its own: the results of the calls one after another."""
+    import threading
+    texts = [_text(torch.float16, 2 + i, 40 + 30 * i, 100, cuda)[1] for i in range(2)]
+    want = [{k: v.clone() for k, v in _step(msd, d).items()} for d in texts]
+    torch.cuda.synchronize()
+    wrong, begin = [], threading.Barrier(2, timeout=60)
+
+    def work(i):
+        try:
+            stream = torch.cuda.Stream()
+            begin.wait()
+            with torch.cuda.stream(stream):
+                got = [_step(msd, texts[i]) for _ in range(20)]
+            stream.synchronize()
+            wrong.extend((i, k) for r in got for k in r if not torch.equal(r[k], want[i][k]))
+        except Exception as e:  # (to the test's own thread)
+            wrong.append(repr(e))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    torch.cuda.synchronize()
+    assert not wrong and not any(t.is_alive() for t in threads)
+
+
 # ---- memory beyond 2^31 values ---------------------------------------------------------------------
 @pytest.mark.parametrize("shift", [0, 1], ids=["aligned", "unaligned"])
 def test_attention_over_a_cache_beyond_32_bits(msd, cuda, shift):
