@@ -737,7 +737,7 @@ uint32_t row_parts(const AttnProblem &p) {
     return (uint32_t)std::max<size_t>(1, std::min<size_t>(parts, rows / 256));
 }
 
-// Parts of the keys for dq, where rows are too few to fill the chip, as in the forward call.
+// Parts of the keys for dq, where rows are too few to fill the chip, of at least 256 keys on average.
 uint32_t dq_parts(const AttnProblem &p) {
     const size_t own = attn_rows(few_rows_and_keys(p)), cus = chip_info().cus;
     const size_t blocks = std::max<size_t>(1, tiles_of(p.q_offsets, p.batch, p.q_rows, p.heads / p.kv_heads, own) * p.kv_heads);
@@ -752,7 +752,8 @@ struct Room {
 };
 Room room_of(const AttnProblem &p) {
     const size_t rows = p.q_offsets == nullptr ? p.batch * p.q_rows : p.q_rows, keys = p.k_offsets == nullptr ? p.batch * p.k_rows : p.k_rows;
-    return Room{(3 * rows * p.heads + keys * p.kv_heads + 3) / 4 * 4, (keys * p.kv_heads * 2 * p.dim + 3) / 4 * 4, (rows * p.heads * p.dim + 3) / 4 * 4};
+    return Room{(3 * rows * p.heads + keys * p.kv_heads + 3) / 4 * 4, (keys * p.kv_heads * 2 * p.dim + 3) / 4 * 4,
+                (rows * p.heads * p.dim + 3) / 4 * 4};
 }
 
 }  // namespace
@@ -796,7 +797,8 @@ int attn_grad_dispatch(const AttnProblem &p, const AttnGradViews &g, const float
     const uint32_t q_parts = (uint32_t)std::max<size_t>(1, std::min<size_t>(dq_parts(p), left / std::max<size_t>(1, r.q_part)));
     float *const part = base + r.vectors, *const q_part = part + (parts > 1 ? parts * r.part : 0);
     const Backward a{attn_shape(p), g.q, g.k, g.v, g.out, g.dout, g.dq, g.dk, g.dv, lse, rest, base, delta,
-                     kHalf ? delta + rows * p.heads : nullptr, kHalf ? delta + 2 * rows * p.heads : nullptr, part, q_part, (uint32_t)rows, (uint32_t)keys, parts, q_parts,
+                     kHalf ? delta + rows * p.heads : nullptr, kHalf ? delta + 2 * rows * p.heads : nullptr, part, q_part, (uint32_t)rows,
+                     (uint32_t)keys, parts, q_parts,
                      (uint32_t)(tiles_of_keys(p) * p.kv_heads * parts),
                      attn_vectors(sizeof(T), p, {g.q, g.k, g.v, g.out, g.dout, g.dq, g.dk, g.dv, AttnView{rest, 0, 0, 0}})};
     const size_t items = rows * p.heads + (kHalf ? keys * p.kv_heads : 0);
