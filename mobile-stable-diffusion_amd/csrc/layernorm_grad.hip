@@ -163,7 +163,8 @@ __global__ __launch_bounds__(kThreads) void ln_grad_kernel(const T *dy, const T 
             }
         // (three sums side by side: a row waits for two rounds of reductions in all)
         row_sums<TL>(q, m1, m2, slots + kWaves);
-        const float rstd = __builtin_amdgcn_rsqf(q * inv_dim + eps);
+        // (the zeros of a team past the last row: 1 / sqrt(eps) times them is NaN for eps = 0, and the sums over rows take in every team)
+        const float rstd = row < rows ? __builtin_amdgcn_rsqf(q * inv_dim + eps) : 0.0f;
         m1 *= inv_dim;
         m2 *= rstd * inv_dim;
 #pragma unroll
