@@ -154,15 +154,12 @@ struct Heads {
         strides[3 * i + 2] = t->stride(d - 2);
         return t;
     }
-    const int32_t *offsets(Call &c, PyObject *o) {
+    // int32 [sequences + 1], of as many as `other` where that is not null
+    const at::Tensor *offsets(Call &c, PyObject *o, const at::Tensor *other) {
         const at::Tensor *t = c.tensor(o);
         if (t == nullptr) return nullptr;
-        if (t->scalar_type() != at::kInt || t->dim() != 1 || t->numel() == 0 || !here(*t) || (batch != 0 && (size_t)t->numel() != batch + 1)) {
-            c.ok = false;
-            return nullptr;
-        }
-        batch = (size_t)t->numel() - 1;
-        return static_cast<const int32_t *>(t->data_ptr());
+        if (t->scalar_type() != at::kInt || t->dim() != 1 || t->numel() == 0 || !here(*t)) return c.fail();
+        return other == nullptr || t->numel() == other->numel() ? t : c.fail();
     }
     Heads(Call &c, PyObject *qo, PyObject *ko, PyObject *vo, PyObject *offsets_q, PyObject *offsets_k) {
         q = view(c, qo, 0);
@@ -184,9 +181,12 @@ struct Heads {
             batch = q->size(0);
         } else if (c.ok) {
             if (offsets_k == Py_None && k_rows != q_rows) c.ok = false;
-            if (c.ok) q_offsets = offsets(c, offsets_q);
-            if (c.ok) k_offsets = offsets_k == Py_None ? q_offsets : offsets(c, offsets_k);
-            if (q_offsets == nullptr || k_offsets == nullptr) c.ok = false;
+            const at::Tensor *of_q = c.ok ? offsets(c, offsets_q, nullptr) : nullptr;
+            const at::Tensor *of_k = !c.ok || offsets_k == Py_None ? of_q : offsets(c, offsets_k, of_q);
+            if (!c.ok) return;
+            batch = (size_t)of_q->numel() - 1;
+            q_offsets = static_cast<const int32_t *>(of_q->data_ptr());
+            k_offsets = static_cast<const int32_t *>(of_k->data_ptr());
         }
         if (heads == 0 || kv_heads == 0 || heads % kv_heads != 0 || dim == 0) c.ok = false;
     }

@@ -1,8 +1,10 @@
 """LayerNorm's gradient, attention and its gradient at the ends of what their calls allow."""
 import pytest
+import torch
 
 import plain_text as plain
-from test_gpu_text_training import DTYPES, _normal
+from test_gpu_text_training import DTYPES, _normal, _offsets
+from test_gpu_torch_calls import _General
 
 pytestmark = pytest.mark.gpu
 
@@ -19,3 +21,27 @@ def test_layernorm_gradient_without_eps(msd, cuda, dtype, rows, dim, add):
     got = msd.layernorm_backward(dy.to(cuda), x.to(cuda), gamma.to(cuda), 0.0, None if dsum is None else dsum.to(cuda))
     for g, w, what in zip(got, plain.layernorm_backward(dy, x, gamma, 0.0, dsum), ("dx", "dgamma", "dbeta")):
         plain.check(g, w, what)
+
+
+# ---- packed sequences ----------------------------------------------------------------------------
+@pytest.mark.parametrize("counts,counts_k", [([], [6]), ([], [2, 3, 1]), ([6], []), ([3, 3], [6]), ([6], [3, 3])])
+def test_offsets_of_different_lengths_are_refused(msd, cuda, monkeypatch, counts, counts_k):
+    """Also where one of them has no sequence at all."""
+    q, k = torch.ones(6, 4, 16, device=cuda), torch.ones(6, 2, 16, device=cuda)
+    o, ok = _offsets(counts, cuda), _offsets(counts_k, cuda)
+    kept = msd.attention_kept(q, k, k, offsets=_offsets([6], cuda))[1]._replace(offsets=o, offsets_k=ok)
+    for native in (msd._bind_native_text(), _General()):
+        monkeypatch.setattr(msd, "_native_text", native)
+        for call in (lambda: msd.attention(q, k, k, offsets=o, offsets_k=ok), lambda: msd.attention_kept(q, k, k, offsets=o, offsets_k=ok),
+                     lambda: msd.attention_backward(q, kept)):
+            with pytest.raises(msd.MsdError):
+                call()
+
+
+def test_offsets_of_one_element(msd, cuda):
+    """No sequence: every row stays as it was."""
+    q, k = torch.ones(6, 4, 16, device=cuda), torch.ones(5, 2, 16, device=cuda)
+    none = _offsets([], cuda)
+    out, kept = msd.attention_kept(q, k, k, offsets=none, offsets_k=none, out=torch.full_like(q, 3.0))
+    grads = msd.attention_backward(q, kept, tuple(torch.full_like(t, 3.0) for t in (q, k, k)))
+    assert all(bool((t == 3).all()) for t in (out,) + grads)
