@@ -789,12 +789,12 @@ int attn_grad_dispatch(const AttnProblem &p, const AttnGradViews &g, const float
     const size_t rows = p.q_offsets == nullptr ? p.batch * p.q_rows : p.q_rows, keys = p.k_offsets == nullptr ? p.batch * p.k_rows : p.k_rows;
     float *const base = static_cast<float *>(workspace), *const delta = base + rows * p.heads;
     constexpr bool kHalf = !Frag<T>::kFloat;
-    // no more parts than the workspace holds, those of dk and dv first
+    // no more parts than the workspace holds, those of dk and dv first; none of a side without rows, which has no workgroups to join them
     const Room r = room_of(p);
     size_t left = workspace_bytes / sizeof(float) - r.vectors;
-    const uint32_t parts = (uint32_t)std::max<size_t>(1, std::min<size_t>(row_parts(p), left / std::max<size_t>(1, r.part)));
+    const uint32_t parts = r.part == 0 ? 1 : (uint32_t)std::max<size_t>(1, std::min<size_t>(row_parts(p), left / r.part));
     if (parts > 1) left -= parts * r.part;
-    const uint32_t q_parts = (uint32_t)std::max<size_t>(1, std::min<size_t>(dq_parts(p), left / std::max<size_t>(1, r.q_part)));
+    const uint32_t q_parts = r.q_part == 0 ? 1 : (uint32_t)std::max<size_t>(1, std::min<size_t>(dq_parts(p), left / r.q_part));
     float *const part = base + r.vectors, *const q_part = part + (parts > 1 ? parts * r.part : 0);
     const Backward a{attn_shape(p), g.q, g.k, g.v, g.out, g.dout, g.dq, g.dk, g.dv, lse, rest, base, delta,
                      kHalf ? delta + rows * p.heads : nullptr, kHalf ? delta + 2 * rows * p.heads : nullptr, part, q_part, (uint32_t)rows,

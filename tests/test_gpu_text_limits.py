@@ -1,4 +1,6 @@
 """LayerNorm's gradient, attention and its gradient at the ends of what their calls allow."""
+import ctypes
+
 import pytest
 import torch
 
@@ -45,3 +47,36 @@ def test_offsets_of_one_element(msd, cuda):
     out, kept = msd.attention_kept(q, k, k, offsets=none, offsets_k=none, out=torch.full_like(q, 3.0))
     grads = msd.attention_backward(q, kept, tuple(torch.full_like(t, 3.0) for t in (q, k, k)))
     assert all(bool((t == 3).all()) for t in (out,) + grads)
+
+
+# ---- workspaces ------------------------------------------------------------------------------------
+def _backward(msd, dout, kept, more, causal):
+    """msd_attention_backward of dense tensors with `more` bytes of workspace than it asks for."""
+    lib, (q, k, v) = msd.load_library(), (kept.q, kept.k, kept.v)
+    code = {torch.float32: msd.DTYPE_F32, torch.float16: msd.DTYPE_F16}[q.dtype]
+    sizes = (q.shape[0], q.shape[1], k.shape[1], q.shape[2], k.shape[2], q.shape[3])
+    need = ctypes.c_size_t(0)
+    assert lib.msd_attention_workspace(*sizes, 0, 1, code, ctypes.byref(need)) == 0
+    workspace = torch.empty(need.value + more, dtype=torch.uint8, device=q.device)
+    grads = [torch.full_like(t, 9.0) for t in (q, k, v)]
+    rc = lib.msd_attention_backward(*[t.data_ptr() if t is not None else None for t in (dout, q, k, v, kept.out, kept.lse, kept.rest, *grads)], None, None,
+                                    *sizes, None, kept.scale, int(causal), code, workspace.data_ptr(), workspace.numel(),
+                                    torch.cuda.current_stream().cuda_stream)
+    return rc, grads
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("rows,keys", [(1024, 0), (0, 1024), (600, 600), (2000, 40), (3, 2500)])
+@pytest.mark.parametrize("more", [8, 1 << 24])
+def test_more_workspace_than_needed(msd, cuda, dtype, causal, rows, keys, more):
+    """Also where one side has no rows: the other's gradients are zeros."""
+    t = DTYPES[dtype]
+    q, k, v, dout = (_normal(i, 1, n, h, 40).to(t).to(cuda) for i, (n, h) in enumerate([(rows, 4), (keys, 2), (keys, 2), (rows, 4)]))
+    kept = msd.attention_kept(q, k, v, causal)[1]
+    rc, grads = _backward(msd, dout, kept, more, causal)
+    assert rc == 0
+    want = msd.attention_backward(dout, kept)
+    assert all(torch.equal(a, b) for a, b in zip(grads, want))
+    if rows == 0 or keys == 0:
+        assert not any(bool(g.any()) for g in grads)
