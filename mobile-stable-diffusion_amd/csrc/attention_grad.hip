@@ -106,11 +106,12 @@ __device__ __forceinline__ float max_up_to(float v) {
     return v;
 }
 
-// A lane's power of two for dS of up to `bound`; where that lowers any lane's, its sums are to be scaled by `down`.
+// A lane's power of two for dS of up to `bound`; where that lowers any lane's, its sums are to be scaled by `down`.  (A bound of 0, of
+// rows that the loss leaves out, says nothing of the size of others.)
 struct DsScale {
     int power = 100;
     __device__ __forceinline__ bool lower(float bound, float &down) {
-        const int p = min(power, max(-100, min(100, 14 - __builtin_amdgcn_frexp_expf(bound))));
+        const int p = bound > 0.0f ? min(power, max(-100, min(100, 14 - __builtin_amdgcn_frexp_expf(bound)))) : power;
         if (__builtin_amdgcn_ballot_w64(p < power) == 0) return false;
         down = ldexpf(1.0f, max(-126, p - power));
         power = p;

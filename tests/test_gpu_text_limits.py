@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import plain_text as plain
-from test_gpu_text_training import DTYPES, _normal, _offsets
+from test_gpu_text_training import DTYPES, _normal, _offsets, _pack
 from test_gpu_torch_calls import _General
 
 pytestmark = pytest.mark.gpu
@@ -80,3 +80,21 @@ def test_more_workspace_than_needed(msd, cuda, dtype, causal, rows, keys, more):
     assert all(torch.equal(a, b) for a, b in zip(grads, want))
     if rows == 0 or keys == 0:
         assert not any(bool(g.any()) for g in grads)
+
+
+# ---- gradients that are zero in whole tiles ----------------------------------------------------------
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("rows,keys", [(264, 1000), (700, 1000)])
+def test_rows_without_a_gradient_take_no_digits_from_the_others(msd, cuda, causal, dim, rows, keys):
+    """The last 64 rows are left out of the loss.  Score gradients are near 10^-11 (float16's least step is 6 10^-8), large queries bring
+    those of the keys back to 10^-3."""
+    q, k, v, dout = _pack([(rows, keys)], 2, 1, dim, torch.float16)
+    q, k, v = (q * 600).half(), (k * 2.0 ** -24).half(), (v * 0.01).half()
+    dout = (dout * 1e-7).half()
+    dout[-64:] = 0
+    want = plain.attention(q, k, v, causal, 2000.0, dout, [(rows, keys)])
+    d = [x[None].to(cuda) for x in (q, k, v, dout)]
+    kept = msd.attention_kept(d[0], d[1], d[2], causal, 2000.0)[1]
+    for g, w, what in zip(msd.attention_backward(d[3], kept), want[1:], ("dq", "dk", "dv")):
+        plain.check(g[0], w, what)
