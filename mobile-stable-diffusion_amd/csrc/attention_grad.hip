@@ -470,7 +470,10 @@ __device__ __forceinline__ void attn_grad_kv(const Backward &a, const uint32_t b
 #pragma unroll
     for (int d = 0; d < DB; d++) dk[d] = dv[d] = zero16();
     DsScale scale;
-    if (count != 0) fetch(tile_of(0), 0);
+    if (count != 0)
+        fetch(tile_of(0), 0);
+    else
+        wait_tiles();  // (keys that no row sees: their values are on the way to LDS, which is not given back before they are there)
     for (uint32_t at = 0; at < count; at++) {
         wait_tiles();
         __syncthreads();

@@ -98,3 +98,21 @@ def test_rows_without_a_gradient_take_no_digits_from_the_others(msd, cuda, causa
     kept = msd.attention_kept(d[0], d[1], d[2], causal, 2000.0)[1]
     for g, w, what in zip(msd.attention_backward(d[3], kept), want[1:], ("dq", "dk", "dv")):
         plain.check(g[0], w, what)
+
+
+# ---- keys that no row sees -----------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_keys_of_sequences_without_rows(msd, cuda, dtype, causal, dim):
+    """Their gradients are zeros, and the sequences between them (whose workgroups run where theirs have been) have theirs."""
+    lengths = [(0, 500), (130, 130)] * 8 + [(0, 1000)]
+    q, k, v, dout = _pack(lengths, 4, 2, dim, DTYPES[dtype])
+    want = plain.attention(q, k, v, causal, 0.1, dout, lengths)
+    o, ok = _offsets([a for a, _ in lengths], cuda), _offsets([b for _, b in lengths], cuda)
+    out, kept = msd.attention_kept(q.to(cuda), k.to(cuda), v.to(cuda), causal, 0.1, o, ok)
+    grads = msd.attention_backward(dout.to(cuda), kept)
+    for g, w, what in zip((out,) + grads, want, ("out", "dq", "dk", "dv")):
+        plain.check(g, w, what)
+    for g in grads[1:]:
+        assert not g[:500].any() and not g[-1000:].any()
