@@ -985,9 +985,10 @@ def attention_backward(dout, kept, out=None):
     lib = _lib or load_library()
     q, k, v = kept.q, kept.k, kept.v
     sizes, qo, ko = _attention_sizes(q, k, v, kept.offsets, kept.offsets_k)
-    if out is None:
-        out = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
-    tensors = (q, k, v, kept.out, dout) + tuple(out)
+    out = (q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)) if out is None else tuple(out)
+    if len(out) != 3:
+        raise MsdError("out must be three tensors (got %d)" % len(out))
+    tensors = (q, k, v, kept.out, dout) + out
     strides = ()
     for t, like, what in zip(tensors, (q, k, k, q, q, q, k, k), ("q", "k", "v", "out", "dout", "dq", "dk", "dv")):
         if t.shape != like.shape:
@@ -1000,7 +1001,7 @@ def attention_backward(dout, kept, out=None):
     check(lib.msd_attention_backward(dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), kept.out.data_ptr(), lp, rp,
                                      *[t.data_ptr() for t in out], qo, ko, *sizes, (ctypes.c_size_t * 24)(*strides), kept.scale,
                                      int(kept.causal), code, wp, size, _stream()))
-    return tuple(out)
+    return out
 
 
 def alphas_cumprod():

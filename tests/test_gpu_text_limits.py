@@ -116,3 +116,13 @@ def test_keys_of_sequences_without_rows(msd, cuda, dtype, causal, dim):
         plain.check(g, w, what)
     for g in grads[1:]:
         assert not g[:500].any() and not g[-1000:].any()
+
+
+@pytest.mark.parametrize("count", [0, 1, 2, 4, 5])
+def test_gradients_into_another_number_of_tensors_are_refused(msd, cuda, count):
+    q, k = torch.ones(1, 6, 4, 16, device=cuda), torch.ones(1, 6, 4, 16, device=cuda)
+    kept = msd.attention_kept(q, k, k)[1]
+    packed = msd.attention_kept(q[0], k[0], k[0], offsets=_offsets([6], cuda))[1]
+    for case, like in ((kept, q), (packed, q[0])):
+        with pytest.raises(msd.MsdError):
+            msd.attention_backward(like, case, tuple(torch.empty_like(like) for _ in range(count)))
