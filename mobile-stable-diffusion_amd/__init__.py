@@ -997,7 +997,7 @@ def attention_backward(dout, kept, out=None):
     code = _dtype_code(q)
     lp = _affine(kept.lse, q.numel() // sizes[5] if sizes[5] else 0, q, "lse")
     rp = _same(kept.rest, q, q.numel(), "rest") if kept.rest is not None else None
-    workspace, wp, size = _workspace(q, "msd_attention_workspace", *sizes, int(qo is not None), 1, code)
+    workspace, wp, size = _workspace(q, "msd_attention_workspace", *sizes, int(qo is not None), 1 if kept.causal else 2, code)
     check(lib.msd_attention_backward(dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), kept.out.data_ptr(), lp, rp,
                                      *[t.data_ptr() for t in out], qo, ko, *sizes, (ctypes.c_size_t * 24)(*strides), kept.scale,
                                      int(kept.causal), code, wp, size, _stream()))

@@ -940,7 +940,7 @@ int msd_attention_workspace(size_t batch, size_t q_rows, size_t k_rows, size_t h
     static const int32_t any = 0;  // (only whether there are offsets counts)
     const int32_t *offsets = packed ? &any : nullptr;
     const AttnProblem p = attention_problem(offsets, offsets, batch, q_rows, k_rows, heads, kv_heads, dim, 1.0f, 0);
-    *bytes = all_q == 0 && (backward == 0 || all_k == 0) ? 0 : backward ? attn_grad_workspace_bytes(p) : attn_workspace_bytes(p);
+    *bytes = all_q == 0 && (backward == 0 || all_k == 0) ? 0 : backward ? attn_grad_workspace_bytes(p, backward != 2) : attn_workspace_bytes(p);
     return MSD_OK;
 }
 
@@ -989,7 +989,7 @@ int msd_attention_backward(const void *dout, const void *q, const void *k, const
     const bool packed = q_offsets != nullptr;
     if (packed != (k_offsets != nullptr) || !(scale > 0.0f) || !(scale < 1e30f)) return MSD_ERR_INVALID_VALUE;
     int rc = attention_checks(batch, q_rows, k_rows, heads, kv_heads, dim, packed, dtype, &all_q, &all_k);
-    if (rc == MSD_OK) rc = msd_attention_workspace(batch, q_rows, k_rows, heads, kv_heads, dim, packed, 1, dtype, &need);
+    if (rc == MSD_OK) rc = msd_attention_workspace(batch, q_rows, k_rows, heads, kv_heads, dim, packed, causal ? 1 : 2, dtype, &need);
     if (rc != MSD_OK) return rc;
     if (all_q == 0 && all_k == 0) return MSD_OK;
     if (need != 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return MSD_ERR_INVALID_VALUE;

@@ -762,11 +762,10 @@ Room room_of(const AttnProblem &p) {
 
 }  // namespace
 
-size_t attn_grad_workspace_bytes(const AttnProblem &p) {
-    AttnProblem masked = p, open = p;  // (the bytes go by the sizes alone, the parts by the mask too)
-    masked.causal = true;
-    open.causal = false;
-    const size_t parts = std::max(row_parts(masked), row_parts(open)), q_parts = dq_parts(p);
+size_t attn_grad_workspace_bytes(const AttnProblem &p, bool any_mask) {
+    AttnProblem other = p;  // (the bytes go by the sizes, the parts by the mask too)
+    other.causal = !p.causal;
+    const size_t parts = any_mask ? std::max(row_parts(p), row_parts(other)) : row_parts(p), q_parts = dq_parts(p);
     const Room r = room_of(p);
     return (r.vectors + (parts > 1 ? parts * r.part : 0) + (q_parts > 1 ? q_parts * r.q_part : 0)) * sizeof(float);
 }

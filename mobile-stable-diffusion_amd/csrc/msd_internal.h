@@ -219,7 +219,7 @@ int attn_dispatch(const AttnProblem &p, const AttnView &q, const AttnView &k, co
 struct AttnGradViews {
     AttnView q, k, v, out, dout, dq, dk, dv;
 };
-size_t attn_grad_workspace_bytes(const AttnProblem &p);
+size_t attn_grad_workspace_bytes(const AttnProblem &p, bool any_mask);  // any_mask: for either, not p's alone
 template <typename T>
 int attn_grad_dispatch(const AttnProblem &p, const AttnGradViews &g, const float *lse, const void *rest, void *workspace, size_t workspace_bytes,
                        hipStream_t stream);

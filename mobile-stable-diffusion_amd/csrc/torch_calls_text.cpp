@@ -250,7 +250,7 @@ PyObject *attention_backward(PyObject *, Args a, Py_ssize_t n) {
         const at::Tensor *out = h.view(c, kept[3], 3), *dout = h.view(c, a[0], 4);
         const int causal = c.truth(kept[6]);
         const double scale = c.number(kept[7]);
-        const at::Tensor workspace = h.workspace(c, 1);
+        const at::Tensor workspace = h.workspace(c, causal ? 1 : 2);
         if (!c.ok || out->sizes() != h.q->sizes() || dout->sizes() != h.q->sizes()) return nullptr;
         const int64_t rows = h.q->numel() / (int64_t)h.dim;
         const float *lse = c.affine(kept[4], rows, *h.q);

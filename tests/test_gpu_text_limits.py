@@ -82,6 +82,28 @@ def test_more_workspace_than_needed(msd, cuda, dtype, causal, rows, keys, more):
         assert not any(bool(g.any()) for g in grads)
 
 
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("native", [False, True])
+def test_a_gradient_without_the_mask_takes_its_own_bytes(msd, cuda, monkeypatch, dtype, native):
+    t = DTYPES[dtype]
+    q, k, v, dout = (_normal(i, 8, 1500, h, 64).to(t).to(cuda) for i, h in enumerate((8, 4, 4, 8)))
+    monkeypatch.setattr(msd, "_native_text", msd._bind_native_text() if native else _General())
+    peak = {}
+    for causal in (True, False):
+        kept = msd.attention_kept(q, k, v, causal)[1]
+        rc, want = _backward(msd, dout, kept, 0, causal)
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        grads = msd.attention_backward(dout, kept)
+        peak[causal] = torch.cuda.max_memory_allocated() - before - sum(g.numel() * g.element_size() for g in grads)
+        assert rc == 0 and all(torch.equal(a, b) for a, b in zip(grads, want))
+        del kept, grads, want
+    parts = 2 * 2 * 4 * k.numel()  # two parts of dk and dv in float32, under the mask alone
+    assert peak[True] >= parts and peak[False] <= parts / 2
+
+
 # ---- gradients that are zero in whole tiles ----------------------------------------------------------
 @pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("dim", [64, 128])
