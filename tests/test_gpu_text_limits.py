@@ -148,3 +148,18 @@ def test_gradients_into_another_number_of_tensors_are_refused(msd, cuda, count):
     for case, like in ((kept, q), (packed, q[0])):
         with pytest.raises(msd.MsdError):
             msd.attention_backward(like, case, tuple(torch.empty_like(like) for _ in range(count)))
+
+
+# ---- parts of rows that are no whole vectors ---------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dim", [33, 127])
+@pytest.mark.parametrize("lengths", [[(3, 2500)], [(2, 1500), (0, 4), (9, 700), (5, 0)], [(1500, 20)]], ids=lambda l: "-".join("%dx%d" % p for p in l))
+def test_parts_of_an_odd_number_of_columns(msd, cuda, dtype, causal, dim, lengths):
+    """Keys in parts for dq (and out), rows in parts for dk and dv."""
+    q, k, v, dout = _pack(lengths, 4, 2, dim, DTYPES[dtype])
+    want = plain.attention(q, k, v, causal, 0.2, dout, lengths)
+    o, ok = _offsets([a for a, _ in lengths], cuda), _offsets([b for _, b in lengths], cuda)
+    out, kept = msd.attention_kept(q.to(cuda), k.to(cuda), v.to(cuda), causal, 0.2, o, ok)
+    for g, w, what in zip((out,) + msd.attention_backward(dout.to(cuda), kept), want, ("out", "dq", "dk", "dv")):
+        plain.check(g, w, what)
