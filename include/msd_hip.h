@@ -460,6 +460,8 @@ int msd_softmax(const void *x, void *y, size_t rows, size_t cols, int stable, in
  * A row that sees no key, or whose scores are all -infinity, gives zeros.  What a row does not see has no part in it, infinities
  * and NaN included.  Scores, maxima and sums are float32; float16 weights are rounded to float16 for the product with v; float32
  * values enter the products as three bfloat16 each, which leaves out at most 2^-23 of a product (and what is below 2^-126).
+ * Scores (scale q . k) are taken up to 2^21 in size; beyond, a weight may overflow and give NaN.  lse, which joins the parts of many keys
+ * and gives the gradient its weights, has float32's digits: these weights are off by up to 2^-23 of themselves times the score.
  *   lse    NULL, or float32 [rows of q][heads]: log2 of the sum of exp(scale q . k) (-infinity for a row that sees nothing),
  *          kept for msd_attention_backward.
  *   rest   NULL, or with float16 [rows of q][heads][dim] float16 without gaps: what the rounding of out took away, kept for

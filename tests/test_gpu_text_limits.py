@@ -163,3 +163,28 @@ def test_parts_of_an_odd_number_of_columns(msd, cuda, dtype, causal, dim, length
     out, kept = msd.attention_kept(q.to(cuda), k.to(cuda), v.to(cuda), causal, 0.2, o, ok)
     for g, w, what in zip((out,) + msd.attention_backward(dout.to(cuda), kept), want, ("out", "dq", "dk", "dv")):
         plain.check(g, w, what)
+
+
+# ---- the largest scores ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("rows,keys", [(70, 200), (2, 2000), (600, 600)])
+def test_scores_of_the_largest_size(msd, cuda, dtype, dim, rows, keys):
+    """Scores up to 2^21, 1024 apart: each row has one key.  Out is its values, off by the weight's rounding (float16) and the result's; the
+    gradient's weights are off by 2^-23 times the score, 1/4 of themselves."""
+    t, gen = DTYPES[dtype], torch.Generator().manual_seed(rows)
+    q, k, v, dout = _pack([(rows, keys)], 1, 1, dim, t, 5)
+    q, k = torch.zeros_like(q), torch.zeros_like(k)
+    q[:, 0, 1] = torch.where(torch.rand(rows, generator=gen) < 0.5, -1024.0, 1024.0).to(t)
+    k[:, 0, 1] = (torch.randperm(2 * keys, generator=gen)[:keys] - keys).clamp(-2047, 2047).to(t)
+    k[3, 0, 1], k[keys - 2, 0, 1] = 2048.0, -2048.0
+    d = [x[None].to(cuda) for x in (q, k, v, dout)]
+    out, kept = msd.attention_kept(d[0], d[1], d[2], False, 1.0)
+    best = torch.where(q[:, 0, 1] > 0, 3, keys - 2)
+    off = 2 * plain.HALF[t] + 2.0 ** -20
+    assert bool(((out[0, :, 0].cpu().double() - v[best, 0].double()).abs() <= off * v[best, 0].double().abs() + plain.TINY[t]).all())
+    dq, dk, dv = msd.attention_backward(d[3], kept)
+    want = torch.zeros(keys, dim, dtype=torch.float64).index_add_(0, best, dout[:, 0].double())
+    size = torch.zeros(keys, dim, dtype=torch.float64).index_add_(0, best, dout[:, 0].double().abs())
+    assert bool(((dv[0, :, 0].cpu().double() - want).abs() <= 0.26 * size + plain.TINY[t]).all())
+    assert bool(torch.isfinite(dq).all()) and bool(torch.isfinite(dk).all())
