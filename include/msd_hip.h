@@ -458,7 +458,8 @@ int msd_softmax(const void *x, void *y, size_t rows, size_t cols, int stable, in
  *   causal != 0: the last query sees every key, the one before all but the last, ...: i sees j <= i + (keys - queries).
  *   scale: positive, below 10^30.
  * A row that sees no key, or whose scores are all -infinity, gives zeros.  What a row does not see has no part in it, infinities
- * and NaN included.  Scores, maxima and sums are float32; float16 weights are rounded to float16 for the product with v; float32
+ * and NaN included.  What it sees of those in v makes its column of the row infinite or NaN; which of the two is not defined where
+ * the weight has underflowed to zero (it differs between tiles of keys that a mask cuts and others).  Scores, maxima and sums are float32; float16 weights are rounded to float16 for the product with v; float32
  * values enter the products as three bfloat16 each, which leaves out at most 2^-23 of a product (and what is below 2^-126).
  * Scores (scale q . k) are taken up to 2^21 in size; beyond, a weight may overflow and give NaN.  lse, which joins the parts of many keys
  * and gives the gradient its weights, has float32's digits: these weights are off by up to 2^-23 of themselves times the score.

@@ -1,5 +1,6 @@
 """LayerNorm's gradient, attention and its gradient at the ends of what their calls allow."""
 import ctypes
+import math
 
 import pytest
 import torch
@@ -188,3 +189,20 @@ def test_scores_of_the_largest_size(msd, cuda, dtype, dim, rows, keys):
     size = torch.zeros(keys, dim, dtype=torch.float64).index_add_(0, best, dout[:, 0].double().abs())
     assert bool(((dv[0, :, 0].cpu().double() - want).abs() <= 0.26 * size + plain.TINY[t]).all())
     assert bool(torch.isfinite(dq).all()) and bool(torch.isfinite(dk).all())
+
+
+# ---- infinities that rows see -----------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("at", [5, 70, 149])
+def test_infinities_without_weight_leave_nothing_finite(msd, cuda, dtype, causal, at):
+    """A key far below the others: its infinite value times a weight of zero is an infinity or NaN in that column, and nowhere else."""
+    t, n = DTYPES[dtype], 150
+    q, k, v, _ = _pack([(n, n)], 1, 1, 64, t, 11)
+    q[..., 0], k[..., 0] = 4.0, 0.0
+    k[at, 0, 0] = -1000.0
+    v[at, 0, 9] = math.inf
+    out = msd.attention(*(x[None].to(cuda) for x in (q, k, v)), causal)[0, :, 0].cpu()
+    sees = torch.arange(n) >= at if causal else torch.ones(n, dtype=torch.bool)
+    assert not torch.isfinite(out[sees, 9]).any() and torch.isfinite(out[~sees, 9]).all()
+    assert torch.isfinite(out[:, [c for c in range(64) if c != 9]]).all()
