@@ -283,6 +283,7 @@ int msd_layernorm_backward(const void *dy, const void *x, const void *dsum, cons
  *           nothing to dtable.  Sums are float32, a token's rows added in a fixed order, and rounded once to the storage type: the
  *           same bits every time.  workspace as for msd_layernorm_backward.
  * At most 2^25 tokens, 2^28 rows, 2^20 columns, 2^35 values of dy, and fewer than 2^31 values in `length` (and in `positions`) rows.
+ * (Beyond some 2^22 tokens the gradient's time grows faster than they do: 2^25 tokens of 8 float16 columns take 17.6 ms, 2^22 0.64.)
  */
 int msd_token_embedding(const int64_t *ids, const void *table, const void *positions, void *y, size_t tokens, size_t length,
                         size_t vocab, size_t dim, float scale, int dtype, void *stream);
@@ -459,8 +460,9 @@ int msd_softmax(const void *x, void *y, size_t rows, size_t cols, int stable, in
  *   scale: positive, below 10^30.
  * A row that sees no key, or whose scores are all -infinity, gives zeros.  What a row does not see has no part in it, infinities
  * and NaN included.  What it sees of those in v makes its column of the row infinite or NaN; which of the two is not defined where
- * the weight has underflowed to zero (it differs between tiles of keys that a mask cuts and others).  Scores, maxima and sums are float32; float16 weights are rounded to float16 for the product with v; float32
- * values enter the products as three bfloat16 each, which leaves out at most 2^-23 of a product (and what is below 2^-126).
+ * the weight has underflowed to zero (it differs between tiles of keys that a mask cuts and others).
+ * Scores, maxima and sums are float32; float16 weights are rounded to float16 for the product with v; float32 values enter the
+ * products as three bfloat16 each, which leaves out at most 2^-23 of a product (and what is below 2^-126).
  * Scores (scale q . k) are taken up to 2^21 in size; beyond, a weight may overflow and give NaN.  lse, which joins the parts of many keys
  * and gives the gradient its weights, has float32's digits: these weights are off by up to 2^-23 of themselves times the score.
  *   lse    NULL, or float32 [rows of q][heads]: log2 of the sum of exp(scale q . k) (-infinity for a row that sees nothing),

@@ -6,13 +6,15 @@
 // chip, the keys are cut into parts, each with a workgroup of its own, and a second launch joins them.
 //
 // Measured (4 d operations for each visible pair; a library product of 8192 x 8192 reaches 1100 TFLOP/s in float16, 154 in float32):
-//   float16, 4 x 4096, 32 heads of 128 on 8: 1.13 ms, 970 TFLOP/s; 8 x 4096, 16 heads of 64: 0.69 ms, 797.  The two wavefronts of a
+//   float16, 4 x 4096, 32 heads of 128 on 8: 1.14 ms, 960 TFLOP/s; 8 x 4096, 16 heads of 64: 0.66 ms, 838.  The two wavefronts of a
 //     SIMD wait for each other's matrix and exp2 instructions (38 % of their cycles) and for tiles (22 %).
-//   float16, 2 x 4096, 5 heads of 64: 85 us, 500 TFLOP/s: 320 workgroups on 256 CUs.  In three parts of the keys, joined, 96 for 97.
+//   float16, 2 x 4096, 5 heads of 64: 85 us, 500 TFLOP/s: 320 workgroups on 256 CUs (see key_parts).
 //   float16, one query of 16 sequences of up to 16385 keys, 32 heads on 8: 104 us and 7 for the join, 4.3 TB/s.
 //   float16, 2 x 77, 12 heads of 64: 7.8 us, of which 6.5 are there for one key too: launch, arguments, two reads of memory in a row
 //     (queries and the first tile), instructions from no cache; a tile of 64 keys is 0.8.
-//   float32, 2 x 2048, 8 heads: 85 TFLOP/s with 64 columns, 96 with 128 (six products for one: 183 at the library's float16 rate).
+//   float32, 2 x 2048, 8 heads: 110 TFLOP/s with 64 columns, 106 with 128, causal 77 and 87 (six products for one: 183 at the library's
+//     float16 rate; cutting the values of each fragment in three takes more cycles than they do).  One query of 16 sequences of 16384
+//     keys, 32 heads of 128 on 8: 1.05 ms, 2.0 TB/s: 32 columns of each product for 4 rows.
 #include <algorithm>
 #include <type_traits>
 
@@ -266,8 +268,14 @@ size_t row_tiles(const AttnProblem &p) {
 
 // Parts of the keys: workgroups for eight rounds of the chip where the sequences' lengths may differ, for two otherwise, with at
 // least 256 keys in a part on average, or 128 as long as all are at work at once; one wavefront joins at most kWave of them.  (Four
-// workgroups of one wavefront count as one.  one query of 32 sequences of 4096 keys, 12 heads of 64, float16: 115 us in one part, 79 in five; one of
-// 1000 keys, 32 heads of 128 on 8: 15.8 us in parts of 256 keys, 12.1 of 128.)
+// workgroups of one wavefront count as one.)  One query of 32 sequences of 4096 keys, 12 heads of 64, float16: 115 us in one part, 79
+// in five; one of 1000 keys, 32 heads of 128 on 8: 15.8 us in parts of 256 keys, 12.1 of 128.  Many rows, float16, heads of 64, calls
+// without a profiler (the join, a row to a wavefront, takes 4-byte loads):
+//   workgroups                               one part   two parts   three   four
+//   320  2 x 4096, 5 heads                      85.2        85.5     91.0   82.0 us  (one is taken)
+//   160  1 x 4096, 5 heads                      87.2       106.7     81.8   86.1     (three)
+//   160  2 x 1024, 10 heads                     24.3        42.0     37.7   40.7     (three, though the join costs more than they give:
+//                                                                                     the rule does not count it)
 uint32_t key_parts(const AttnProblem &p) {
     const bool packed = p.k_offsets != nullptr;
     const size_t keys = packed ? p.k_rows / std::max<size_t>(1, p.batch) : p.k_rows;

@@ -9,9 +9,9 @@
 //   float16, 4 x 4000 causal, 16 heads of 128 on 4: D 41 us (at the rate of a large copy), dk and dv 670 and their join 34, dq 420:
 //     595 TFLOP/s.  4 x 4096, 32 heads on 8: 4.08 ms, 674.  dk and dv hold 254 of 256 registers: waits for operands and tiles are
 //     36 % of a wavefront's cycles, matrix instructions 42 % of the SIMD's.
-//   float16, 8 x 4096, 16 heads of 64: 2.4 ms, 575 TFLOP/s.
+//   float16, 8 x 4096, 16 heads of 64: 2.36 ms, 582 TFLOP/s; 2 x 4096 rows over 77 keys, 5 heads of 64: 36 us.
 //   float32, 32 sequences of up to 77, 12 heads of 64: 4 and 23 us; a launch's fixed 6, the wavefronts' own first rows, then 5 a tile.
-//   float32, 2 x 2048 causal, 8 heads: 68 TFLOP/s with 64 columns, 80 with 128.
+//   float32, 2 x 2048 causal, 8 heads: 67 TFLOP/s with 64 columns, 78 with 128.
 //
 // float16: dS is rounded to float16 for its product, after a power of two that brings the largest it can be,
 // |do_i| max |v_j| + |D_i|, next to 2^14: it keeps 11 bits down to 2^-28 of that, whatever the gradients' size.  Each row of dq

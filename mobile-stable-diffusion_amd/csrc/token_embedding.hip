@@ -280,7 +280,9 @@ __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(const int64_t 
     if (threadIdx.x < kBins) table[(size_t)blockIdx.x * kBins + threadIdx.x] = bins[threadIdx.x];
 }
 
-// Every block adds the table's columns for itself: what lies before it in its bins, and the bins' totals.
+// Every block adds the table's columns for itself: what lies before it in its bins, and the bins' totals.  That saves a launch, and
+// grows with the square of the tokens: a pass over 2^20 takes 21 us, over 2^22 0.16 ms (as long as the sums of 8 columns), over 2^25,
+// the most there are, 7.5 ms of a call's 17.6.
 template <typename T, uint32_t ROUNDS>
 __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(const int64_t *ids, const Entry *from, const uint32_t *table, Entry *to,
                                                                   uint32_t tokens, uint32_t vocab, uint32_t shift, uint32_t blocks,
