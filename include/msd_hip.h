@@ -483,7 +483,8 @@ int msd_attention(const void *q, const void *k, const void *v, void *out, float 
 /*
  * Gradient of msd_attention: from dout (as out), the forward call's q, k, v, out, lse and rest (or NULL): dq (as q), dk and dv (as k), the
  * gradients of shared key heads summed over their query heads.  strides: as above for q, k, v, out, dout, dq, dk, dv in turn.
- * Rows that see nothing give zeros and add nothing, rows of no sequence stay as they were.  Sums are float32 in a fixed order
+ * Rows that see nothing give zeros and add nothing, rows of no sequence stay as they were.  Infinities and NaN of rows and keys that see
+ * each other come out as one or the other, as in the forward call.  Sums are float32 in a fixed order
  * without atomics, the same bits every time; float16 weights and score gradients are rounded to float16 for their products,
  * the latter scaled by a power of two that keeps small gradients' digits.  workspace as above: msd_attention_workspace with backward = 1
  * for either mask, or 2 for causal = 0 alone, which needs less where a causal call's rows are in two parts: each part has dk and dv in
